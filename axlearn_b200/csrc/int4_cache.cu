@@ -1,0 +1,634 @@
+// A paged KV cache held in 4 bits (`int4.cuh`): new tokens are quantised into it, and one new token a sequence attends to it.
+//
+// Pools: codes [pages, Nkv, page_size, H / 2], pairs (s, m) [pages, Nkv, page_size, H / 32, 2] in bf16, for K and for V, so
+// that a head's rows of a page are one run of memory; page table [B, max_pages], H 64 or 128.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <float.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "chain.cuh"
+#include "cluster.cuh"
+#include "int4.cuh"
+#include "mma_sync.cuh"
+
+namespace axb {
+
+struct Int4Pool {
+  uint8_t* codes;
+  uint32_t* pairs;
+};
+
+// Rows of heads in: element strides of (sequence, token, head); dims are neighbours.
+struct HeadRows {
+  const __nv_bfloat16* x;
+  int64_t b, t, h;
+};
+
+struct Int4AppendParams {
+  HeadRows q, k, v;
+  __nv_bfloat16 *q_out, *k_out, *v_out;  // where the rotated q and the values of k and v go, or null
+  int64_t qo_b, qo_t, qo_h, ko_b, ko_t, ko_h, vo_b, vo_t, vo_h;
+  Int4Pool k_pool, v_pool;
+  const int* page_table;
+  const int* start;     // null: 0
+  const int* live;      // null: all tokens
+  const float2* angle;  // (sin, cos) of [position][H / 2], null: nothing is rotated
+  int* status;
+  int start_offset, angle_rows;
+  int B, T, num_q_heads, num_kv_heads, page_size, max_pages, num_pages;
+};
+
+// The eight dims 8 l .. 8 l + 7 of a lane, groups of 32 dims are four neighbouring lanes: codes (dim i in bits 4 i) and pair.
+__device__ __forceinline__ uint32_t quantize8(const uint4& x, uint32_t& pair) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&x);
+  __nv_bfloat162 lo2 = __hmin2_nan(__hmin2_nan(h[0], h[1]), __hmin2_nan(h[2], h[3]));
+  __nv_bfloat162 hi2 = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+#pragma unroll
+  for (int off = 1; off <= 2; off <<= 1) {
+    lo2 = __hmin2_nan(lo2, __shfl_xor_sync(0xffffffffu, lo2, off));
+    hi2 = __hmax2_nan(hi2, __shfl_xor_sync(0xffffffffu, hi2, off));
+  }
+  const float lo = __bfloat162float(__hmin_nan(lo2.x, lo2.y)), hi = __bfloat162float(__hmax_nan(hi2.x, hi2.y));
+  const float range = hi - lo;
+  const bool good = range <= FLT_MAX;  // neither NaN nor an infinity nor an overflow
+  float s = __bfloat162float(__float2bfloat16(range * (1.f / 15.f)));
+  if (!good || s < FLT_MIN) s = 0.f;
+  const uint32_t m_bits = good ? __float_as_uint(lo) : 0x7fff0000u;
+  pair = (__float_as_uint(s) >> 16) | m_bits;
+  if (s == 0.f) return 0;
+  uint32_t codes = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __bfloat1622float2(h[i]);
+    const float a = rintf(__fdiv_rn(f.x - lo, s)), b = rintf(__fdiv_rn(f.y - lo, s));
+    codes |= static_cast<uint32_t>(fminf(fmaxf(a, 0.f), 15.f)) << (8 * i);
+    codes |= static_cast<uint32_t>(fminf(fmaxf(b, 0.f), 15.f)) << (8 * i + 4);
+  }
+  return codes;
+}
+
+__device__ __forceinline__ uint4 values8(uint32_t codes, uint32_t pair) {
+  const float s = pair_s(pair), m = pair_m(pair);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = pack2(fmaf(s, static_cast<float>((codes >> (8 * i)) & 15u), m),
+                 fmaf(s, static_cast<float>((codes >> (8 * i + 4)) & 15u), m));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The four bytes that a lane stores of a row, and where: lanes of neighbouring groups swap halves, so that each has the
+// same chunk of two groups.  `lane`: within the row (H / 8 lanes).
+template <int H>
+__device__ __forceinline__ uint32_t row_word(uint32_t codes, int lane, int& byte) {
+  constexpr int G = H / kInt4Group;
+  const int g = lane >> 2, sub = lane & 3;
+  const uint32_t other = __shfl_xor_sync(0xffffffffu, codes, 4);
+  byte = (2 * sub + (g & 1)) * (2 * G) + (g >> 1) * 4;
+  return g & 1 ? __byte_perm(other, codes, 0x7632) : __byte_perm(codes, other, 0x5410);
+}
+
+__device__ __forceinline__ uint4 rotate8(uint4 x, const float2* at) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpack2(w[i]), a = at[i];
+    w[i] = pack2(f.x * a.y - f.y * a.x, f.y * a.y + f.x * a.x);
+  }
+  return x;
+}
+
+constexpr int kAppendThreads = 256;
+
+// A row of H values (one head of one token) is H / 8 lanes of 16 bytes; rows run over heads (q, k, v), tokens, sequences.
+template <int H>
+__global__ void __launch_bounds__(kAppendThreads)
+int4_append_kernel(Int4AppendParams p) {
+  chain_link();
+  constexpr int kLanes = H / 8, kRows = kAppendThreads / kLanes;
+  const int lane = threadIdx.x % kLanes;
+  const int heads = p.num_q_heads + 2 * p.num_kv_heads;
+  const int64_t rows = static_cast<int64_t>(p.B) * p.T * heads;
+  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRows; row0 < rows; row0 += static_cast<int64_t>(gridDim.x) * kRows) {
+    const int64_t row = row0 + threadIdx.x / kLanes;  // (shuffles: all lanes stay)
+    const bool inside = row < rows;
+    const int64_t token = inside ? row / heads : 0;
+    const int head = inside ? static_cast<int>(row - token * heads) : 0;
+    const int b = static_cast<int>(token / p.T), t = static_cast<int>(token - static_cast<int64_t>(b) * p.T);
+    const int pos = (p.start == nullptr ? 0 : p.start[b]) + p.start_offset + t;
+    const bool live = inside && (p.live == nullptr || t < p.live[b]);
+    const bool is_q = head < p.num_q_heads, is_v = head >= p.num_q_heads + p.num_kv_heads;
+    const int kvh = is_v ? head - p.num_q_heads - p.num_kv_heads : head - p.num_q_heads;
+    const HeadRows& src = is_q ? p.q : is_v ? p.v : p.k;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (live) x = *reinterpret_cast<const uint4*>(src.x + b * src.b + t * src.t + (is_q ? head : kvh) * src.h + lane * 8);
+    if (live && !is_v && p.angle != nullptr) {
+      if (pos >= 0 && pos < p.angle_rows)
+        x = rotate8(x, p.angle + static_cast<int64_t>(pos) * (H / 2) + lane * 4);
+      else
+        int4_report(p.status);
+    }
+    uint32_t pair;
+    const uint32_t codes = quantize8(x, pair);
+    int byte;
+    const uint32_t word = row_word<H>(codes, lane, byte);
+    if (!inside) continue;
+    if (is_q) {
+      if (live) *reinterpret_cast<uint4*>(p.q_out + b * p.qo_b + t * p.qo_t + head * p.qo_h + lane * 8) = x;
+      continue;
+    }
+    __nv_bfloat16* out = is_v ? p.v_out : p.k_out;
+    if (out != nullptr) {
+      const int64_t at = is_v ? b * p.vo_b + t * p.vo_t + kvh * p.vo_h : b * p.ko_b + t * p.ko_t + kvh * p.ko_h;
+      *reinterpret_cast<uint4*>(out + at + lane * 8) = live ? values8(codes, pair) : make_uint4(0, 0, 0, 0);
+    }
+    if (!live) continue;
+    const int col = pos / p.page_size;
+    if (pos < 0 || col >= p.max_pages) {
+      int4_report(p.status);
+      continue;
+    }
+    const int page = p.page_table[static_cast<int64_t>(b) * p.max_pages + col];
+    if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_pages)) {
+      int4_report(p.status);
+      continue;
+    }
+    const int64_t slot = (static_cast<int64_t>(page) * p.num_kv_heads + kvh) * p.page_size + (pos - col * p.page_size);
+    const Int4Pool& pool = is_v ? p.v_pool : p.k_pool;
+    *reinterpret_cast<uint32_t*>(pool.codes + slot * (H / 2) + byte) = word;
+    if ((lane & 3) == 0) pool.pairs[slot * (H / kInt4Group) + (lane >> 2)] = pair;
+  }
+}
+
+struct Int4AttnParams {
+  const __nv_bfloat16* q;  // [B, Nq, H]
+  Int4Pool k_pool, v_pool;
+  const int* page_table;
+  const int* lengths;
+  float* part_out;         // [B, Nq, splits, H]
+  float* part_ml;          // [B, Nq, splits, 2]
+  __nv_bfloat16* out;
+  int* status;
+  int num_q_heads, num_kv_heads, page_size, max_pages, num_pages, splits;
+  float scale_log2;
+};
+
+constexpr int kAttnThreads = 128, kAttnWarps = kAttnThreads / 32;
+constexpr int kAttnRows = 8;   // query heads of a CTA: the columns of the second product
+constexpr int kAttnKeys = 32;  // keys of a tile
+constexpr int kAttnStages = 2;
+constexpr int kAttnCluster = 8;
+
+template <int H>
+struct Int4Tile {
+  static constexpr int kGroups = H / kInt4Group;
+  static constexpr int kRow = H / 2, kPairs = kGroups * 4;        // bytes of a key's codes and pairs
+  static constexpr int kK = 0, kV = kAttnKeys * kRow, kKPairs = 2 * kV, kVPairs = kKPairs + kAttnKeys * kPairs;
+  static constexpr int kBytes = kVPairs + kAttnKeys * kPairs;
+  static constexpr int kSmem(int rows) {
+    const int merge = (kAttnWarps + 1) * rows * (H + 2) * 4, tiles = kAttnWarps * kAttnStages * kBytes;
+    return merge > tiles ? merge : tiles;
+  }
+  // 16-byte unit u of V's row `key`: units are swapped so that eight lanes of four keys, every second one, hit all banks.
+  __device__ static int v_unit(int key, int u) {
+    if constexpr (H == 128) return (key >> 1) * 128 + ((((key & 1) * 4 + u) ^ (((key >> 1) & 3) << 1)) << 4);
+    return (key >> 2) * 128 + ((((key & 3) * 2 + u) ^ (((key >> 2) & 1) << 1)) << 4);
+  }
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(ok ? 8 : 0) : "memory");
+}
+
+// S = Q K^T: rows 0-7 of the m16n8k16 tile are the query heads, K is the B operand; a lane takes dims 8c .. 8c + 7 of each
+// group of a key and the sums of a group are multiplied by its s: q.k = sum_g s_g (sum q c) + m_g sum q.  The products
+// start at -128 sum q.
+// O^T = V^T P^T: 16 dims of one group are the rows, the heads the columns; s of a key's group is multiplied into P, which is
+// rounded to bf16 (2^-9 of a probability, the sums of p m stay in 32 bits).  The products start at -128 sum P, by an MMA.
+template <int H, bool kCluster>
+__global__ void __launch_bounds__(kAttnThreads)
+int4_attn_kernel(Int4AttnParams p) {
+  chain_link();
+  using Tile = Int4Tile<H>;
+  constexpr int G = Tile::kGroups;
+  extern __shared__ __align__(128) uint8_t s_ring[];
+  const int split = blockIdx.x;
+  const int group = p.num_q_heads / p.num_kv_heads;
+  const int parts = (group + kAttnRows - 1) / kAttnRows;
+  const int kvh = blockIdx.y / parts;
+  const int first = blockIdx.y % parts * kAttnRows;
+  const int rows = min(kAttnRows, group - first);
+  const int qh0 = kvh * group + first;
+  const int b = blockIdx.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = lane >> 2, c = lane & 3;
+  int len = p.lengths[b];
+  if (len > p.max_pages * static_cast<int64_t>(p.page_size)) {
+    if (threadIdx.x == 0) int4_report(p.status);
+    len = p.max_pages * p.page_size;
+  }
+  const int tiles = (max(len, 0) + kAttnKeys - 1) / kAttnKeys;
+  const int per_split = (tiles + p.splits - 1) / p.splits;
+  const int hi = min(tiles, (split + 1) * per_split);
+  const int* table = p.page_table + static_cast<int64_t>(b) * p.max_pages;
+
+  // Row of the pools of key `lane` of a tile, -1 beyond the sequence.
+  auto slot_of = [&](int tile) -> int64_t {
+    const int t = tile * kAttnKeys + lane;
+    if (tile >= hi || t >= len) return -1;
+    const int col = t / p.page_size, page = table[col];
+    if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_pages)) {
+      int4_report(p.status);
+      return -1;
+    }
+    return (static_cast<int64_t>(page) * p.num_kv_heads + kvh) * p.page_size + (t - col * p.page_size);
+  };
+  uint8_t* ring = s_ring + warp * kAttnStages * Tile::kBytes;
+  auto load_tile = [&](int stage, int64_t slot) {
+    const uint32_t dst = sptr(ring) + stage * Tile::kBytes;
+    constexpr int kUnits = Tile::kRow / 16, kKeys = 32 / kUnits;  // keys an instruction
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      const int key = i * kKeys + lane / kUnits, u = lane % kUnits;
+      const int64_t at = __shfl_sync(0xffffffffu, slot, key);
+      const int64_t off = (at < 0 ? 0 : at) * Tile::kRow + u * 16;
+      cp_async16(dst + Tile::kK + key * Tile::kRow + u * 16, p.k_pool.codes + off, at >= 0);
+      cp_async16(dst + Tile::kV + Tile::v_unit(key, u), p.v_pool.codes + off, at >= 0);
+    }
+    const int64_t off = (slot < 0 ? 0 : slot) * G;
+    const uint32_t kd = dst + Tile::kKPairs + lane * Tile::kPairs, vd = dst + Tile::kVPairs + lane * Tile::kPairs;
+    if constexpr (G == 4) {
+      cp_async16(kd, p.k_pool.pairs + off, slot >= 0);
+      cp_async16(vd, p.v_pool.pairs + off, slot >= 0);
+    } else {
+      cp_async8(kd, p.k_pool.pairs + off, slot >= 0);
+      cp_async8(vd, p.v_pool.pairs + off, slot >= 0);
+    }
+  };
+  int tile = split * per_split + warp;
+#pragma unroll
+  for (int i = 0; i < kAttnStages; ++i) {
+    const int64_t slot = slot_of(tile + i * kAttnWarps);
+    if (tile + i * kAttnWarps < hi) load_tile(i, slot);
+    cp_commit();
+  }
+  int64_t slot = slot_of(tile + kAttnStages * kAttnWarps);
+
+  // Q in the order of K's codes: MMA i of group g takes dims 8c + 2i, 8c + 2i + 4 and the two behind them.
+  uint32_t qa[2 * G][2];
+  float qs[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (r < rows)
+      x = *reinterpret_cast<const uint4*>(p.q + (static_cast<int64_t>(b) * p.num_q_heads + qh0 + r) * H + g * 32 + c * 8);
+    qa[2 * g][0] = __byte_perm(x.x, x.z, 0x5410);
+    qa[2 * g][1] = __byte_perm(x.x, x.z, 0x7632);
+    qa[2 * g + 1][0] = __byte_perm(x.y, x.w, 0x5410);
+    qa[2 * g + 1][1] = __byte_perm(x.y, x.w, 0x7632);
+    const float2 f0 = unpack2(x.x), f1 = unpack2(x.y), f2 = unpack2(x.z), f3 = unpack2(x.w);
+    float sum = ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    qs[g] = sum;
+  }
+
+  float m = -INFINITY, l = 0.f;
+  float acc[2 * G][4];  // [group, half][dim 32 g + 4 r + 2 half (+ 1: entries 2, 3)][columns 2c, 2c + 1]
+  float acc_m[G];       // sums of p m of head r, this lane's keys
+#pragma unroll
+  for (int i = 0; i < 2 * G; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+#pragma unroll
+  for (int g = 0; g < G; ++g) acc_m[g] = 0.f;
+
+  int stage = 0;
+  for (; tile < hi; tile += kAttnWarps) {
+    cp_wait_group<kAttnStages - 1>();
+    __syncwarp();
+    const uint8_t* st = ring + stage * Tile::kBytes;
+    float s[8];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      uint32_t w[G], pairs[2][G];
+      const uint8_t* kr = st + Tile::kK + (n * 8 + r) * Tile::kRow + c * (Tile::kRow / 4);
+      const uint8_t* pr = st + Tile::kKPairs + (n * 8 + 2 * c) * Tile::kPairs;
+      if constexpr (G == 4) {
+        *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(kr);
+        *reinterpret_cast<uint4*>(pairs[0]) = *reinterpret_cast<const uint4*>(pr);
+        *reinterpret_cast<uint4*>(pairs[1]) = *reinterpret_cast<const uint4*>(pr + 16);
+      } else {
+        *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(kr);
+        *reinterpret_cast<uint2*>(pairs[0]) = *reinterpret_cast<const uint2*>(pr);
+        *reinterpret_cast<uint2*>(pairs[1]) = *reinterpret_cast<const uint2*>(pr + 8);
+      }
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const uint32_t x = __byte_perm(w[g >> 1], w[G / 2 + (g >> 1)], g & 1 ? 0x7632 : 0x5410);
+        float part[4] = {-128.f * qs[g], -128.f * qs[g], 0.f, 0.f};
+        const uint32_t a0[4] = {qa[2 * g][0], 0u, qa[2 * g][1], 0u}, a1[4] = {qa[2 * g + 1][0], 0u, qa[2 * g + 1][1], 0u};
+        mma(part, a0, int4_pair(x, 0), int4_pair(x, 1));
+        mma(part, a1, int4_pair(x, 2), int4_pair(x, 3));
+        s0 += pair_s(pairs[0][g]) * part[0] + pair_m(pairs[0][g]) * qs[g];
+        s1 += pair_s(pairs[1][g]) * part[1] + pair_m(pairs[1][g]) * qs[g];
+      }
+      s[2 * n] = s0 * p.scale_log2;
+      s[2 * n + 1] = s1 * p.scale_log2;
+    }
+    if ((tile + 1) * kAttnKeys > len) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (tile * kAttnKeys + (i >> 1) * 8 + 2 * c + (i & 1) >= len) s[i] = -INFINITY;
+    }
+    float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const float m_new = fmaxf(m, top);
+    if (__any_sync(0xffffffffu, m_new != m)) {
+      const float corr = m_new == -INFINITY ? 1.f : exp2f(m - m_new);
+      l *= corr;
+#pragma unroll
+      for (int g = 0; g < G; ++g) acc_m[g] *= corr;
+      const float c0 = __shfl_sync(0xffffffffu, corr, 8 * c), c1 = __shfl_sync(0xffffffffu, corr, 8 * c + 4);
+#pragma unroll
+      for (int i = 0; i < 2 * G; ++i) {
+        acc[i][0] *= c0;
+        acc[i][1] *= c1;
+        acc[i][2] *= c0;
+        acc[i][3] *= c1;
+      }
+      m = m_new;
+    }
+    // A row of -inf alone keeps zeros; NaN stays.
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      s[i] = exp2f(s[i] - base);
+      l += s[i];
+    }
+    // Keys 16 j + 2c, + 1, + 8, + 9 are the columns of P that this lane holds: s[4 j .. 4 j + 3].
+    uint32_t w[8][G / 2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int key = (i >> 1) * 8 + 2 * c + (i & 1);
+      if constexpr (G == 4) {
+        *reinterpret_cast<uint2*>(w[i]) =
+            *reinterpret_cast<const uint2*>(st + Tile::kV + Tile::v_unit(key, r >> 1) + (r & 1) * 8);
+      } else {
+        w[i][0] = *reinterpret_cast<const uint32_t*>(st + Tile::kV + Tile::v_unit(key, r >> 2) + (r & 3) * 4);
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      uint32_t pb[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* pr = st + Tile::kVPairs + (i * 8 + 2 * c) * Tile::kPairs + g * 4;
+        const uint32_t u0 = *reinterpret_cast<const uint32_t*>(pr), u1 = *reinterpret_cast<const uint32_t*>(pr + Tile::kPairs);
+        pb[i] = pack2(s[2 * i] * pair_s(u0), s[2 * i + 1] * pair_s(u1));
+        acc_m[g] += s[2 * i] * pair_m(u0) + s[2 * i + 1] * pair_m(u1);
+      }
+      const uint32_t less[4] = {0xc300c300u, 0xc300c300u, 0xc300c300u, 0xc300c300u};  // -128
+      float off[4] = {0.f, 0.f, 0.f, 0.f};
+      mma(off, less, pb[0], pb[1]);
+      mma(off, less, pb[2], pb[3]);
+      uint32_t x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = __byte_perm(w[2 * i][g >> 1], w[2 * i + 1][g >> 1], g & 1 ? 0x7632 : 0x5410);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float o[4] = {off[0], off[1], off[2], off[3]};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t a[4] = {int4_pair(x[2 * j], 2 * h), int4_pair(x[2 * j], 2 * h + 1), int4_pair(x[2 * j + 1], 2 * h),
+                                 int4_pair(x[2 * j + 1], 2 * h + 1)};
+          mma(o, a, pb[2 * j], pb[2 * j + 1]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[2 * g + h][i] += o[i];
+      }
+    }
+    __syncwarp();  // the stage has been read
+    if (tile + kAttnStages * kAttnWarps < hi) load_tile(stage, slot);
+    cp_commit();
+    slot = slot_of(tile + (kAttnStages + 1) * kAttnWarps);
+    if (++stage == kAttnStages) stage = 0;
+  }
+  cp_wait_all();
+  __syncthreads();  // the merge buffers overlay the tiles
+  l += __shfl_xor_sync(0xffffffffu, l, 1);
+  l += __shfl_xor_sync(0xffffffffu, l, 2);
+  float* s_part = reinterpret_cast<float*>(s_ring);  // 4 warps and the CTA: [rows][H] sums, then maxima, then weights
+  const int per_warp = rows * H;
+  float* s_m = s_part + (kAttnWarps + 1) * per_warp;
+  float* s_l = s_m + (kAttnWarps + 1) * rows;
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    acc_m[g] += __shfl_xor_sync(0xffffffffu, acc_m[g], 1);
+    acc_m[g] += __shfl_xor_sync(0xffffffffu, acc_m[g], 2);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const float add = __shfl_sync(0xffffffffu, acc_m[g], 8 * c + 4 * n);
+      if (2 * c + n < rows) {
+        float* dst = s_part + warp * per_warp + (2 * c + n) * H + g * 32 + r * 4;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          *reinterpret_cast<float2*>(dst + 2 * h) = make_float2(acc[2 * g + h][n] + add, acc[2 * g + h][2 + n] + add);
+      }
+    }
+  }
+  if (r < rows && c == 0) {
+    s_m[warp * rows + r] = m;
+    s_l[warp * rows + r] = l;
+  }
+  __syncthreads();
+  // Thread (g, d) of H threads a head owns output dim d.
+  constexpr int kSets = kAttnThreads / H;
+  const int d = threadIdx.x % H;
+  for (int g = threadIdx.x / H; g < rows; g += kSets) {
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kAttnWarps; ++w) mm = fmaxf(mm, s_m[w * rows + g]);
+    float ll = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < kAttnWarps; ++w) {
+      const float f = mm == -INFINITY ? 1.f : exp2f(s_m[w * rows + g] - mm);
+      ll += s_l[w * rows + g] * f;
+      o += s_part[w * per_warp + g * H + d] * f;
+    }
+    const int64_t row = static_cast<int64_t>(b) * p.num_q_heads + qh0 + g;
+    if (p.splits == 1) {
+      p.out[row * H + d] = __float2bfloat16(ll == 0.f ? 0.f : o / ll);
+    } else if (kCluster) {
+      s_part[kAttnWarps * per_warp + g * H + d] = o;
+      if (d == 0) {
+        s_m[kAttnWarps * rows + g] = mm;
+        s_l[kAttnWarps * rows + g] = ll;
+      }
+    } else {
+      p.part_out[(row * p.splits + split) * H + d] = o;
+      if (d == 0) {
+        p.part_ml[(row * p.splits + split) * 2] = mm;
+        p.part_ml[(row * p.splits + split) * 2 + 1] = ll;
+      }
+    }
+  }
+  if constexpr (kCluster) {
+    cluster_sync_all();
+    for (int g = split * kSets + threadIdx.x / H; g < rows; g += p.splits * kSets) {
+      float mv[kAttnCluster], lv[kAttnCluster], ov[kAttnCluster];
+#pragma unroll
+      for (int s = 0; s < kAttnCluster; ++s) {
+        const bool have = s < p.splits;
+        mv[s] = have ? ld_cluster_f32(sptr(s_m + kAttnWarps * rows + g), s) : -INFINITY;
+        lv[s] = have ? ld_cluster_f32(sptr(s_l + kAttnWarps * rows + g), s) : 0.f;
+        ov[s] = have ? ld_cluster_f32(sptr(s_part + kAttnWarps * per_warp + g * H + d), s) : 0.f;
+      }
+      float mm = -INFINITY;
+#pragma unroll
+      for (int s = 0; s < kAttnCluster; ++s) mm = fmaxf(mm, mv[s]);
+      float ll = 0.f, o = 0.f;
+#pragma unroll
+      for (int s = 0; s < kAttnCluster; ++s) {
+        const float f = mm == -INFINITY ? 1.f : exp2f(mv[s] - mm);
+        ll += lv[s] * f;
+        o += ov[s] * f;
+      }
+      p.out[(static_cast<int64_t>(b) * p.num_q_heads + qh0 + g) * H + d] = __float2bfloat16(ll == 0.f ? 0.f : o / ll);
+    }
+    cluster_sync_all();  // a CTA's shared memory outlives its readers
+  }
+}
+
+template <int H>
+__global__ void __launch_bounds__(H)
+int4_combine_kernel(const float* part_out, const float* part_ml, __nv_bfloat16* out, int splits) {
+  chain_link();
+  const int64_t row = blockIdx.x;
+  const int d = threadIdx.x;
+  float mm = -INFINITY;
+  for (int s = 0; s < splits; ++s) mm = fmaxf(mm, part_ml[(row * splits + s) * 2]);
+  float ll = 0.f, o = 0.f;
+  for (int s = 0; s < splits; ++s) {
+    const float f = mm == -INFINITY ? 1.f : exp2f(part_ml[(row * splits + s) * 2] - mm);
+    ll += part_ml[(row * splits + s) * 2 + 1] * f;
+    o += part_out[(row * splits + s) * H + d] * f;
+  }
+  out[row * H + d] = __float2bfloat16(ll == 0.f ? 0.f : o / ll);
+}
+
+template <int H, bool kCluster>
+static int launch_int4_attn(const Int4AttnParams& p, dim3 grid, int rows, cudaStream_t stream) {
+  constexpr auto kernel = int4_attn_kernel<H, kCluster>;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {grid.x, 1, 1};
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kAttnThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(Int4Tile<H>::kSmem(rows));
+  static_assert(Int4Tile<H>::kSmem(kAttnRows) <= 48 * 1024, "no opt-in");
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = static_cast<unsigned>(chain_attribute(attr, kCluster ? 1 : 0));
+  return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? 0 : -4;
+}
+
+template <int H>
+static int int4_attn(const Int4AttnParams& p, int B, cudaStream_t stream) {
+  const int g = p.num_q_heads / p.num_kv_heads;
+  const bool cluster = p.splits > 1 && p.splits <= kAttnCluster;
+  const dim3 grid(p.splits, p.num_kv_heads * ((g + kAttnRows - 1) / kAttnRows), B);
+  const int rows = g < kAttnRows ? g : kAttnRows;
+  const int rc = cluster ? launch_int4_attn<H, true>(p, grid, rows, stream) : launch_int4_attn<H, false>(p, grid, rows, stream);
+  if (rc != 0) return rc;
+  if (p.splits > kAttnCluster)
+    launch_chained(int4_combine_kernel<H>, B * p.num_q_heads, H, 0, stream, p.part_out, p.part_ml, p.out, p.splits);
+  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+}
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace axb
+
+// `rows`: pointers q, k, v, q_out, k_out, v_out (null: not there), each with element strides of (sequence, token, head) in
+// `strides`.  -10: not supported.
+extern "C" int axb_int4_append(void* const* rows, const int64_t* strides, void* k_codes, void* k_pairs, void* v_codes,
+                               void* v_pairs, const int* page_table, const int* start, int start_offset, const int* live,
+                               const float* angle, int angle_rows, int B, int T, int num_q_heads, int num_kv_heads,
+                               int head_dim, int page_size, int max_pages, int num_pages, int* status,
+                               cudaStream_t stream) {
+  using namespace axb;
+  if ((head_dim != 64 && head_dim != 128) || page_size < 1 || num_kv_heads < 1 || num_q_heads < 0 || B < 0 || T < 0) return -10;
+  for (int i = 0; i < 6; ++i)
+    if (!aligned16(rows[i]) || (strides[3 * i] | strides[3 * i + 1] | strides[3 * i + 2]) % 8) return -10;
+  if (!aligned16(k_codes) || !aligned16(k_pairs) || !aligned16(v_codes) || !aligned16(v_pairs) || !aligned16(angle)) return -10;
+  if (B == 0 || T == 0) return 0;
+  Int4AppendParams p;
+  HeadRows* in[3] = {&p.q, &p.k, &p.v};
+  for (int i = 0; i < 3; ++i)
+    *in[i] = {static_cast<const __nv_bfloat16*>(rows[i]), strides[3 * i], strides[3 * i + 1], strides[3 * i + 2]};
+  p.q_out = static_cast<__nv_bfloat16*>(rows[3]);
+  p.k_out = static_cast<__nv_bfloat16*>(rows[4]);
+  p.v_out = static_cast<__nv_bfloat16*>(rows[5]);
+  p.qo_b = strides[9], p.qo_t = strides[10], p.qo_h = strides[11];
+  p.ko_b = strides[12], p.ko_t = strides[13], p.ko_h = strides[14];
+  p.vo_b = strides[15], p.vo_t = strides[16], p.vo_h = strides[17];
+  p.k_pool = {static_cast<uint8_t*>(k_codes), static_cast<uint32_t*>(k_pairs)};
+  p.v_pool = {static_cast<uint8_t*>(v_codes), static_cast<uint32_t*>(v_pairs)};
+  p.page_table = page_table;
+  p.start = start;
+  p.live = live;
+  p.angle = reinterpret_cast<const float2*>(angle);
+  p.status = status;
+  p.start_offset = start_offset;
+  p.angle_rows = angle_rows;
+  p.B = B, p.T = T, p.num_q_heads = num_q_heads, p.num_kv_heads = num_kv_heads;
+  p.page_size = page_size, p.max_pages = max_pages, p.num_pages = num_pages;
+  const int64_t per_cta = kAppendThreads / (head_dim / 8);
+  int64_t ctas = (static_cast<int64_t>(B) * T * (num_q_heads + 2 * num_kv_heads) + per_cta - 1) / per_cta;
+  if (ctas > 148 * 32) ctas = 148 * 32;
+  if (head_dim == 128)
+    launch_chained(int4_append_kernel<128>, static_cast<unsigned>(ctas), kAppendThreads, 0, stream, p);
+  else
+    launch_chained(int4_append_kernel<64>, static_cast<unsigned>(ctas), kAppendThreads, 0, stream, p);
+  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+}
+
+// Scratch of axb_int4_decode_attn in floats: up to a cluster's splits meet without any.
+extern "C" int64_t axb_int4_attn_scratch_floats(int B, int num_q_heads, int head_dim, int splits) {
+  if (splits <= axb::kAttnCluster) return 0;
+  return static_cast<int64_t>(B) * num_q_heads * splits * (head_dim + 2);
+}
+
+extern "C" int axb_int4_decode_attn(const void* q, void* k_codes, void* k_pairs, void* v_codes, void* v_pairs,
+                                    const int* page_table, const int* lengths, void* out, float* scratch, int B,
+                                    int num_q_heads, int num_kv_heads, int head_dim, int page_size, int max_pages,
+                                    int num_pages, int splits, float softmax_scale, int* status, cudaStream_t stream) {
+  using namespace axb;
+  if ((head_dim != 64 && head_dim != 128) || page_size < 1 || num_kv_heads < 1 || num_q_heads < 1 ||
+      num_q_heads % num_kv_heads || splits < 1 || B < 0 || B > 65535)
+    return -10;
+  if (!aligned16(q) || !aligned16(k_codes) || !aligned16(k_pairs) || !aligned16(v_codes) || !aligned16(v_pairs)) return -10;
+  if (splits > kAttnCluster && scratch == nullptr) return -10;
+  if (B == 0) return 0;
+  Int4AttnParams p;
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.k_pool = {static_cast<uint8_t*>(k_codes), static_cast<uint32_t*>(k_pairs)};
+  p.v_pool = {static_cast<uint8_t*>(v_codes), static_cast<uint32_t*>(v_pairs)};
+  p.page_table = page_table;
+  p.lengths = lengths;
+  p.part_out = scratch;
+  p.part_ml = scratch == nullptr ? nullptr : scratch + static_cast<int64_t>(B) * num_q_heads * splits * head_dim;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.status = status;
+  p.num_q_heads = num_q_heads, p.num_kv_heads = num_kv_heads, p.page_size = page_size;
+  p.max_pages = max_pages, p.num_pages = num_pages, p.splits = splits;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  return head_dim == 128 ? int4_attn<128>(p, B, stream) : int4_attn<64>(p, B, stream);
+}

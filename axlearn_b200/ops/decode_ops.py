@@ -222,6 +222,23 @@ def prompt_attention(qkv: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tens
     return out
 
 
+def packed_prompt_attention(qkv: torch.Tensor, *, num_q_heads: int, num_kv_heads: int, softmax_scale: float) -> torch.Tensor:
+    """Causal attention of whole prompts over a packed projection ``[B, T, (Nq + 2 Nkv) * H]`` as it lies (queries and keys are
+    rotated already).  Returns ``[B, T, Nq * H]``."""
+    b, t, width = qkv.shape
+    h = width // (num_q_heads + 2 * num_kv_heads)
+    q, k, v = qkv.view(b, t, -1, h).split((num_q_heads, num_kv_heads, num_kv_heads), 2)
+    if flash_sm100.FORWARD_VARIANT != "v3":
+        out, _ = flash_sm100.forward(q.contiguous(), k.contiguous(), v.contiguous(), causal=True, scale=softmax_scale)
+        return out.reshape(b, t, num_q_heads * h)
+    out = torch.empty((b, t, num_q_heads * h), dtype=qkv.dtype, device=qkv.device)
+    rc = _lib().axb_flash_fwd_strided(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), b, t, num_q_heads,
+                                      num_kv_heads, h, width, t * width, width, t * width, softmax_scale,
+                                      cuda_ops.status_word(qkv.device).data_ptr(), cuda_ops._stream())  # pylint: disable=protected-access
+    cuda_ops._check(rc, "axb_flash_fwd_strided")  # pylint: disable=protected-access
+    return out
+
+
 def swiglu_packed(gu: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     rows, two_f = gu.shape
     f = two_f // 2

@@ -1,0 +1,469 @@
+"""Serving in 4 bits: products with 4-bit weights and a paged 4-bit KV cache (``csrc/int4_linear.cu``,
+``csrc/int4_cache.cu``).
+
+A group of neighbouring values shares two bf16 numbers, its smallest value ``m`` and a step ``s``, a fifteenth of its range;
+a value is held as the code ``c = round((x - m) / s)`` of 0 to 15 (ties to the even code) and stands for ``m + s * c``.  A step
+below the smallest normal fp32 number counts as 0.  A group with a NaN or an infinity in it, or whose range
+overflows, stands for NaN.
+
+* ``quantize_weight`` / ``int4_linear``: ``x [..., K] @ w [K, N]``, groups of 64 or 128 rows of a column.
+* ``append_int4``: keys and values of new tokens into the cache (prompts, chunks, single tokens), groups of 32 dims of a head.
+* ``paged_decode_attention_int4``: one query token per sequence over the cache.
+* ``prompt_attention_int4``, ``rope_decode_attention_int4``: what a prompt and a decoding step run, with the rotation of
+  queries and keys and the append.
+
+Attention sees what the cache stands for, in prompts as in steps.  CUDA tensors in bf16 go to the kernels, everything
+else runs the plain statements, which are also the oracle in tests.  Places on the GPU that a page table or a length gets
+wrong (a page that the pool does not have, a position behind the table) are not touched; they set the device's status
+word, which ``cuda_ops.check_status`` raises.  The bf16 forms of these operations are ``cuda_ops.gemm`` and
+``decode_ops``; the reference has no 4-bit form (its quantised layers: axlearn/common/quantized_dot_general/layers.py).
+"""
+
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import dataclasses
+import math
+from typing import NamedTuple, Optional, Union
+
+import torch
+
+from axlearn_b200.ops import cuda_ops, dispatch
+
+c_void_p, c_int, c_int64, c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+Tensor = torch.Tensor
+
+CACHE_GROUP = 32
+# Rows of x up to which weights are expanded in registers; beyond, W is expanded to bf16 once and multiplied by the GEMM.
+MAX_STREAMED_ROWS = 64
+_configured = False
+
+
+def _lib():
+    global _configured
+    h = cuda_ops.lib()
+    if not _configured:
+        h.axb_int4_append.argtypes = [c_void_p] * 8 + [c_int, c_void_p, c_void_p] + [c_int] * 9 + [c_void_p] * 2
+        h.axb_int4_decode_attn.argtypes = [c_void_p] * 9 + [c_int] * 8 + [c_float, c_void_p, c_void_p]
+        h.axb_int4_attn_scratch_floats.argtypes = [c_int] * 4
+        h.axb_int4_attn_scratch_floats.restype = c_int64
+        h.axb_int4_linear.argtypes = [c_void_p] * 4 + [c_int] * 4 + [c_int64, c_int64, c_int, c_void_p]
+        h.axb_int4_expand.argtypes = [c_void_p] * 3 + [c_int] * 3 + [c_void_p]
+        for f in (h.axb_int4_append, h.axb_int4_decode_attn, h.axb_int4_linear, h.axb_int4_expand):
+            f.restype = c_int
+        _configured = True
+    return h
+
+
+def _on_kernel(x: Tensor) -> bool:
+    return x.is_cuda and x.dtype == torch.bfloat16 and not dispatch._flags.force_reference  # pylint: disable=protected-access
+
+
+def _device_of(x: Tensor):
+    """Launches go to the device of the operands."""
+    return contextlib.nullcontext() if x.device.index == torch.cuda.current_device() else torch.cuda.device(x.device)
+
+
+# ------------------------------------------------------------------------------------------
+# Groups.
+# ------------------------------------------------------------------------------------------
+
+
+def quantize_groups(x: Tensor, group: int) -> tuple[Tensor, Tensor]:
+    """Groups along the last dim: codes ``[..., H]`` (uint8) and ``[..., H / group, 2]`` bf16 pairs (step, smallest)."""
+    g = x.float().unflatten(-1, (-1, group))
+    m = g.amin(-1).bfloat16()
+    spread = g.amax(-1) - m.float()
+    good = torch.isfinite(spread)
+    s = (spread * (1.0 / 15.0)).bfloat16()
+    s = torch.where(good & (s.float() >= torch.finfo(torch.float32).tiny), s, 0)
+    m = torch.where(good, m, torch.nan)
+    level = (g - m.float()[..., None]) / torch.where(s > 0, s.float(), torch.inf)[..., None]
+    codes = level.round().clamp(0, 15).nan_to_num(0.0).to(torch.uint8)
+    return codes.flatten(-2), torch.stack((s, m), -1)
+
+
+def group_values(codes: Tensor, scales: Tensor) -> Tensor:
+    """fp32 values ``[..., H]`` of codes ``[..., H]`` and pairs ``[..., groups, 2]``."""
+    c = codes.float().unflatten(-1, (scales.shape[-2], -1))
+    s, m = scales.float().unbind(-1)
+    return (m[..., None] + s[..., None] * c).flatten(-2)
+
+
+# ------------------------------------------------------------------------------------------
+# Weights.
+# ------------------------------------------------------------------------------------------
+
+
+@dataclasses.dataclass(frozen=True)
+class Int4Weight:
+    """A matrix ``[k, n]`` in 4 bits.  ``codes [ceil(n / 16), ceil(k / 128) * 2, 512]`` (uint8) are blocks of 16 columns and 64
+    rows in the order of the kernel's operands (``csrc/int4_linear.cu``), ``scales [ceil(n / 16), groups, 8, 2, 2]`` (bf16)
+    run over column mod 8, column / 8 and (step, smallest)."""
+
+    codes: Tensor
+    scales: Tensor
+    k: int
+    n: int
+    group: int
+
+    def __post_init__(self):
+        codes, scales, tiles, blocks = self.codes, self.scales, -(-self.n // 16), -(-self.k // 128) * 2
+        if self.k % 8 or self.n % 8 or self.k < 8 or self.n < 8 or self.group not in (64, 128):
+            raise ValueError(f"a 4-bit weight has dims that are multiples of 8 and groups of 64 or 128: {self.k, self.n, self.group}")
+        if (codes.shape != (tiles, blocks, 512) or codes.dtype != torch.uint8 or scales.dtype != torch.bfloat16
+                or scales.shape != (tiles, blocks * 64 // self.group, 8, 2, 2) or codes.device != scales.device
+                or not codes.is_contiguous() or not scales.is_contiguous()):
+            raise ValueError(f"codes {tuple(codes.shape)} {codes.dtype} and scales {tuple(scales.shape)} {scales.dtype} are not "
+                             f"those of a [{self.k}, {self.n}] weight with groups of {self.group}")
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return self.k, self.n
+
+
+def _pack_blocks(codes: Tensor) -> Tensor:
+    """``[N, K]`` (multiples of 16 and 64) -> ``[N / 16, K / 64, 512]``."""
+    n, k = codes.shape
+    x = codes.reshape(n // 16, 2, 8, k // 64, 4, 4, 2, 2)    # half, column, block, lane, MMA, pair, odd
+    x = x.permute(0, 3, 2, 4, 5, 7, 6, 1)
+    return (x[..., 0] | (x[..., 1] << 4)).reshape(n // 16, k // 64, 512)
+
+
+def _unpack_blocks(blocks: Tensor) -> Tensor:
+    tiles, k64, _ = blocks.shape
+    x = torch.stack((blocks & 15, blocks >> 4), -1).reshape(tiles, k64, 8, 4, 4, 2, 2, 2)
+    return x.permute(0, 7, 2, 1, 3, 4, 6, 5).reshape(tiles * 16, k64 * 64)
+
+
+def quantize_weight(w: Tensor, *, group: int = 128) -> Int4Weight:
+    """``w [K, N]`` (K and N multiples of 8) with groups of ``group`` rows of a column; the rows behind K that fill its last
+    group are zeros."""
+    if w.dim() != 2:
+        raise ValueError(f"a weight is a matrix: {tuple(w.shape)}")
+    k, n = w.shape
+    kp, np_ = -(-k // 128) * 128, -(-n // 16) * 16
+    padded = torch.nn.functional.pad(w.detach().float().t(), (0, kp - k, 0, np_ - n))
+    codes, scales = quantize_groups(padded, group)
+    scales = scales.reshape(np_ // 16, 2, 8, kp // group, 2).permute(0, 3, 2, 1, 4).contiguous()
+    return Int4Weight(_pack_blocks(codes), scales, k=k, n=n, group=group)
+
+
+def dequantize_weight(w: Int4Weight, dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """``[K, N]``, rounded to ``dtype``; on the GPU in bf16 a transposed view of a ``[N, K]`` buffer, for the GEMM."""
+    if w.codes.is_cuda and dtype == torch.bfloat16 and not dispatch._flags.force_reference:  # pylint: disable=protected-access
+        with _device_of(w.codes):
+            out = torch.empty((w.codes.shape[0] * 16, w.codes.shape[1] * 64), dtype=dtype, device=w.codes.device)
+            rc = _lib().axb_int4_expand(w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), w.n, w.k, w.group,
+                                        cuda_ops._stream())  # pylint: disable=protected-access
+            cuda_ops._check(rc, "axb_int4_expand")  # pylint: disable=protected-access
+        return out[:w.n, :w.k].t()
+    tiles, groups = w.scales.shape[:2]
+    scales = w.scales.permute(0, 3, 2, 1, 4).reshape(tiles * 16, groups, 2)
+    return group_values(_unpack_blocks(w.codes), scales).t()[:w.k, :w.n].to(dtype)
+
+
+def int4_linear(x: Tensor, w: Int4Weight, *, out: Optional[Tensor] = None, accumulate: bool = False) -> Tensor:
+    """``x [..., K] @ w`` with fp32 accumulation, rounded to ``x.dtype``; into ``out [..., N]``, or with ``accumulate`` added to
+    it.  Up to 64 rows read the 4-bit weights as they are; more rows multiply with their values rounded to bf16.  Serving
+    only: there is no gradient.  (Sums that overflow fp32 on the way, as with an infinity in x, are NaN.)"""
+    if x.shape[-1] != w.k or x.device != w.codes.device:
+        raise ValueError(f"x {tuple(x.shape)} on {x.device} and a {w.shape} weight on {w.codes.device}")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise ValueError("int4_linear has no gradient")
+    shape = x.shape[:-1] + (w.n,)
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate needs out")
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    elif out.shape != shape or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous():
+        raise ValueError(f"out {tuple(out.shape)} {out.dtype}: contiguous {tuple(shape)} {x.dtype} is wanted")
+    rows = out.numel() // w.n
+    if not _on_kernel(x):
+        y = x.float() @ dequantize_weight(w, torch.float32)
+        return out.copy_(out.float() + y if accumulate else y)
+    if rows == 0:
+        return out
+    if x.dim() != 2 or x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < w.k or x.data_ptr() % 16:
+        x = x.reshape(rows, w.k).contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+    if rows <= MAX_STREAMED_ROWS:
+        with _device_of(x):
+            rc = _lib().axb_int4_linear(x.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, w.n, w.k,
+                                        w.group, x.stride(0), w.n, 1 if accumulate else 0,
+                                        cuda_ops._stream())  # pylint: disable=protected-access
+            cuda_ops._check(rc, "axb_int4_linear")  # pylint: disable=protected-access
+        return out
+    with _device_of(x):
+        cuda_ops.gemm(x, dequantize_weight(w), out=out.view(rows, w.n), accumulate=accumulate)
+    return out
+
+
+# ------------------------------------------------------------------------------------------
+# Cache.
+# ------------------------------------------------------------------------------------------
+
+
+class Int4Pages(NamedTuple):
+    """A page pool of keys or values: ``codes [pages, Nkv, page_size, H / 2]`` (uint8), ``scales [pages, Nkv, page_size, H / 32,
+    2]`` (bf16; step and smallest value of every 32 dims).  A row's codes are 8 chunks; chunk r holds dims 4r .. 4r + 3 of
+    every group, group by group, the lower dim in the lower half of a byte."""
+
+    codes: Tensor
+    scales: Tensor
+
+
+def int4_pages(num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, device=None) -> Int4Pages:
+    """A pool of zeros."""
+    if head_dim not in (64, 128):
+        raise ValueError(f"the 4-bit cache holds heads of 64 or 128, not {head_dim}")
+    shape = (num_pages, num_kv_heads, page_size)
+    return Int4Pages(torch.zeros(shape + (head_dim // 2,), dtype=torch.uint8, device=device),
+                     torch.zeros(shape + (head_dim // CACHE_GROUP, 2), dtype=torch.bfloat16, device=device))
+
+
+def _pack_rows(codes: Tensor) -> Tensor:
+    h = codes.shape[-1]
+    x = codes.unflatten(-1, (h // 32, 8, 2, 2)).transpose(-4, -3)
+    return (x[..., 0] | (x[..., 1] << 4)).flatten(-3)
+
+
+def _unpack_rows(rows: Tensor) -> Tensor:
+    groups = rows.shape[-1] // 16
+    x = torch.stack((rows & 15, rows >> 4), -1).flatten(-2).unflatten(-1, (8, groups, 4))
+    return x.transpose(-3, -2).flatten(-3)
+
+
+def page_values(pages: Int4Pages, dtype: torch.dtype = torch.float32) -> Tensor:
+    """What a pool (or rows of it) stands for: ``[pages, Nkv, page_size, H]``."""
+    return group_values(_unpack_rows(pages.codes), pages.scales).to(dtype)
+
+
+def _check_pages(k_pages: Int4Pages, v_pages: Int4Pages, page_table: Tensor, heads: int, head_dim: int, device) -> tuple:
+    """``(pages, Nkv, page size)`` of a cache that fits."""
+    codes, scales = k_pages
+    shape = codes.shape
+    if (len(shape) != 4 or head_dim not in (64, 128) or shape[3] * 2 != head_dim or v_pages.codes.shape != shape or not shape[1]
+            or heads % shape[1] or scales.shape != shape[:3] + (head_dim // CACHE_GROUP, 2)
+            or v_pages.scales.shape != scales.shape or not shape[2]):
+        raise ValueError(f"4-bit pages {tuple(shape)}, {tuple(scales.shape)} for {heads} heads of {head_dim} (64 or 128)")
+    for codes, scales in (k_pages, v_pages):
+        if (codes.dtype != torch.uint8 or scales.dtype != torch.bfloat16 or not codes.is_contiguous()
+                or not scales.is_contiguous() or codes.device != device or scales.device != device):
+            raise ValueError(f"4-bit pages are contiguous uint8 and bf16 tensors on {device}")
+    if (page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous()
+            or page_table.device != device):
+        raise ValueError(f"a page table is a contiguous int32 matrix on {device}")
+    return shape[0], shape[1], shape[2]
+
+
+def _check_counts(counts: Tensor, batch: int, name: str, device) -> Tensor:
+    if counts.dtype != torch.int32 or counts.shape != (batch,) or not counts.is_contiguous() or counts.device != device:
+        raise ValueError(f"{name} is [{batch}] int32 on {device}: {tuple(counts.shape)} {counts.dtype}")
+    return counts
+
+
+def _rotate(x: Tensor, table: Tensor, pos: Tensor) -> Tensor:
+    """``x [B, T, N, H]`` with interleaved pairs turned by ``table [positions, H / 2, 2]`` (sin, cos) at ``pos [B, T]``."""
+    sn, cs = table[pos.clamp(0, table.shape[0] - 1)].unbind(-1)
+    sn, cs = sn[:, :, None], cs[:, :, None]
+    x0, x1 = x.float().unflatten(-1, (-1, 2)).unbind(-1)
+    return torch.stack((x0 * cs - x1 * sn, x1 * cs + x0 * sn), -1).flatten(-2).to(x.dtype)
+
+
+def _append_plain(k, v, k_pages, v_pages, page_table, start, live):
+    b, t = k.shape[:2]
+    page_size = k_pages.codes.shape[2]
+    at = torch.arange(t, device=k.device)
+    pos = start[:, None].long() + at
+    keep = (at < live[:, None]) if live is not None else torch.ones((b, t), dtype=torch.bool, device=k.device)
+    inside = keep & (pos >= 0) & (pos < page_table.shape[1] * page_size)
+    page = page_table.long().gather(1, (pos // page_size).clamp(0, page_table.shape[1] - 1))
+    inside &= (page >= 0) & (page < k_pages.codes.shape[0])
+    if not k.is_cuda and bool((keep & ~inside).any()):
+        raise IndexError("a token's place is outside the page table, or its page outside the pool")
+    row, values = pos % page_size, []
+    for x, pages in ((k, k_pages), (v, v_pages)):
+        codes, scales = quantize_groups(x, CACHE_GROUP)
+        pages.codes[page[inside], :, row[inside]] = _pack_rows(codes)[inside]
+        pages.scales[page[inside], :, row[inside]] = scales[inside]
+        values.append(torch.where(keep[..., None, None], group_values(codes, scales).to(x.dtype), 0))
+    return values
+
+
+def _launch_append(rows, k_pages, v_pages, page_table, start, start_offset, live, table, b, t, nq, nkv, h):
+    """``rows``: q, k, v, where q goes, where the values of k and v go (None: not there), ``[B, T, heads, H]`` each."""
+    ptrs = (c_void_p * 6)(*[None if x is None else x.data_ptr() for x in rows])
+    strides = (c_int64 * 18)(*[s for x in rows for s in ((0, 0, 0) if x is None else x.stride()[:3])])
+    rc = _lib().axb_int4_append(
+        ptrs, strides, k_pages.codes.data_ptr(), k_pages.scales.data_ptr(), v_pages.codes.data_ptr(),
+        v_pages.scales.data_ptr(), page_table.data_ptr(), None if start is None else start.data_ptr(), start_offset,
+        None if live is None else live.data_ptr(), None if table is None else table.data_ptr(),
+        0 if table is None else table.shape[0], b, t, nq, nkv, h, k_pages.codes.shape[2], page_table.shape[1],
+        k_pages.codes.shape[0], cuda_ops.status_word(k_pages.codes.device).data_ptr(),
+        cuda_ops._stream())  # pylint: disable=protected-access
+    cuda_ops._check(rc, "axb_int4_append")  # pylint: disable=protected-access
+
+
+def append_int4(k: Tensor, v: Tensor, k_pages: Int4Pages, v_pages: Int4Pages, page_table: Tensor, start: Tensor, *,
+                live: Optional[Tensor] = None, values: bool = False) -> Optional[tuple[Tensor, Tensor]]:
+    """Quantises ``k`` and ``v [B, T, Nkv, H]`` (strided views may be given) into the pages of positions ``start[b] ..`` of
+    ``page_table [B, max_pages]``; ``start [B]`` and ``live [B]`` (how many of the T tokens are there; None: all) are int32.
+    Nothing else in the pages changes.  ``values``: also returns what the cache stands for at these tokens, ``(k, v)`` of
+    the inputs' shape and type, zeros behind ``live``.  No two sequences may own a page that is written."""
+    b, t, nkv, h = k.shape
+    if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
+        raise ValueError(f"k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} differ")
+    if _check_pages(k_pages, v_pages, page_table, nkv, h, k.device)[1] != nkv or page_table.shape[0] != b:
+        raise ValueError(f"pages of {k_pages.codes.shape[1]} heads and a table of {page_table.shape[0]} rows for {nkv} heads of {b} "
+                         "sequences")
+    _check_counts(start, b, "start", k.device)
+    if live is not None:
+        _check_counts(live, b, "live", k.device)
+    if not _on_kernel(k):
+        out = _append_plain(k, v, k_pages, v_pages, page_table, start, live)
+        return tuple(out) if values else None
+    k, v = (x if x.stride(3) == 1 and not (x.stride(0) | x.stride(1) | x.stride(2)) % 8 and x.data_ptr() % 16 == 0
+            else x.clone(memory_format=torch.contiguous_format) for x in (k, v))
+    out = tuple(torch.empty((b, t, nkv, h), dtype=k.dtype, device=k.device) for _ in range(2)) if values else (None, None)
+    with _device_of(k):
+        _launch_append((None, k, v, None) + out, k_pages, v_pages, page_table, start, 0, live, None, b, t, 0, nkv, h)
+    return out if values else None
+
+
+def attention_splits(batch: int, num_kv_heads: int, group: int, max_len: int, sms: int = 148) -> int:
+    """KV splits of attention over the 4-bit cache: one wave of CTAs (two fit an SM; one takes a split, a KV head and eight
+    query heads), at least half a 32-token tile for each of a CTA's four warps."""
+    ctas = batch * num_kv_heads * ((group + 7) // 8)
+    splits = max(1, min(max_len // 64, 2 * sms // max(1, ctas)))
+    return min(splits, 8 if 16 * ctas > sms else 32)
+
+
+def _attention_plain(q, k_pages, v_pages, page_table, lengths, scale):
+    b, nq, h = q.shape
+    pages = page_table.long()
+    if not q.is_cuda and b:
+        used = torch.arange(pages.shape[1])[None] * k_pages.codes.shape[2] < lengths[:, None]
+        if bool((used & ((pages < 0) | (pages >= k_pages.codes.shape[0]))).any()) or (
+                int(lengths.max()) > pages.shape[1] * k_pages.codes.shape[2]):
+            raise IndexError("a length behind the page table, or a page outside the pool")
+        pages = torch.where(used, pages, 0)
+    k, v = (page_values(Int4Pages(x.codes[pages], x.scales[pages])).transpose(1, 2).flatten(2, 3) for x in (k_pages, v_pages))
+    seen = (torch.arange(k.shape[2], device=q.device) < lengths[:, None])[:, None, :, None]
+    k, v = torch.where(seen, k, 0), torch.where(seen, v, 0)
+    scores = q.float().unflatten(1, (k.shape[1], -1)) @ k.transpose(2, 3) * scale
+    p = torch.softmax(scores.masked_fill(~seen.transpose(2, 3), -torch.inf), -1)
+    out = torch.where((lengths > 0)[:, None, None, None], p @ v, 0)
+    return out.reshape(b, nq, h).to(q.dtype)
+
+
+def paged_decode_attention_int4(q: Tensor, k_pages: Int4Pages, v_pages: Int4Pages, page_table: Tensor, lengths: Tensor, *,
+                                softmax_scale: Optional[float] = None, splits: Optional[int] = None,
+                                out: Optional[Tensor] = None, scratch: Optional[Tensor] = None) -> Tensor:
+    """q ``[B, Nq, H]``; page_table ``[B, max_pages]``, lengths ``[B]`` int32 (valid tokens per sequence; 0: zeros).  Query heads
+    are grouped by KV head.  ``scratch``: ``attention_scratch_floats`` fp32 values, for more than eight splits.  Returns
+    ``[B, Nq, H]``."""
+    b, nq, h = q.shape
+    device = q.device
+    num_pages, nkv, page_size = _check_pages(k_pages, v_pages, page_table, nq, h, device)
+    _check_counts(lengths, b, "lengths", device)
+    if page_table.shape[0] != b:
+        raise ValueError(f"a page table of {page_table.shape[0]} rows for {b} sequences")
+    scale = 1.0 / math.sqrt(h) if softmax_scale is None else softmax_scale
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != device or not out.is_contiguous()):
+        raise ValueError(f"out {tuple(out.shape)} {out.dtype}: contiguous {tuple(q.shape)} {q.dtype} is wanted")
+    if not _on_kernel(q):
+        y = _attention_plain(q, k_pages, v_pages, page_table, lengths, scale)
+        return y if out is None else out.copy_(y)
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    max_pages = page_table.shape[1]
+    if splits is None:
+        splits = attention_splits(b, nkv, nq // nkv, max_pages * page_size)
+    if out is None:
+        out = torch.empty_like(q)
+    with _device_of(q):
+        if splits > 8:
+            floats = attention_scratch_floats(b, nq, h, splits)
+            if scratch is None:
+                scratch = torch.empty(floats, dtype=torch.float32, device=device)
+            elif scratch.numel() < floats or scratch.dtype != torch.float32 or scratch.device != device or not scratch.is_contiguous():
+                raise ValueError(f"scratch is {floats} contiguous fp32 values on {device}")
+        rc = _lib().axb_int4_decode_attn(
+            q.data_ptr(), k_pages.codes.data_ptr(), k_pages.scales.data_ptr(), v_pages.codes.data_ptr(),
+            v_pages.scales.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(),
+            None if scratch is None else scratch.data_ptr(), b, nq, nkv, h, page_size, max_pages, num_pages, splits, scale,
+            cuda_ops.status_word(device).data_ptr(), cuda_ops._stream())  # pylint: disable=protected-access
+        cuda_ops._check(rc, "axb_int4_decode_attn")  # pylint: disable=protected-access
+    return out
+
+
+def attention_scratch_floats(batch: int, num_q_heads: int, head_dim: int, splits: int) -> int:
+    return _lib().axb_int4_attn_scratch_floats(batch, num_q_heads, head_dim, splits)
+
+
+def _split_qkv(qkv: Tensor, nq: int, nkv: int) -> tuple[Tensor, Tensor, Tensor]:
+    """``[..., (Nq + 2 Nkv) * H]`` as views ``[..., heads, H]`` of q, k and v."""
+    return qkv.unflatten(-1, (nq + 2 * nkv, -1)).split((nq, nkv, nkv), -2)
+
+
+def _check_packed(qkv: Tensor, k_pages: Int4Pages, table: Tensor, nq: int) -> tuple[int, int]:
+    nkv, h = k_pages.codes.shape[1], k_pages.codes.shape[3] * 2
+    if qkv.shape[-1] != (nq + 2 * nkv) * h or not qkv.is_contiguous() or qkv.data_ptr() % 16:
+        raise ValueError(f"a packed projection of {nq} + 2 x {nkv} heads of {h} is contiguous and 16-byte aligned: {tuple(qkv.shape)}")
+    if (table.dtype != torch.float32 or table.shape[1:] != (h // 2, 2) or not table.is_contiguous() or table.device != qkv.device
+            or table.data_ptr() % 16):
+        raise ValueError(f"a rotation table is [positions, {h // 2}, 2] fp32 on {qkv.device}: {tuple(table.shape)} {table.dtype}")
+    return nkv, h
+
+
+def rope_decode_attention_int4(qkv: Tensor, k_pages: Int4Pages, v_pages: Int4Pages, page_table: Tensor, lengths: Tensor,
+                               table: Tensor, *, num_q_heads: int, softmax_scale: float, splits: Optional[int] = None,
+                               scratch: Optional[Tensor] = None) -> Tensor:
+    """``qkv [B, (Nq + 2 Nkv) * H]`` of the token at position ``lengths - 1``: rotates its query and key by ``table [positions,
+    H / 2, 2]`` (``decode_ops.rope_table``), appends key and value to the cache and attends to it.  Rows of length 0 append
+    nothing and get zeros.  Returns ``[B, Nq, H]``."""
+    nkv, h = _check_packed(qkv, k_pages, table, num_q_heads)
+    b = qkv.shape[0]
+    _check_pages(k_pages, v_pages, page_table, num_q_heads, h, qkv.device)
+    _check_counts(lengths, b, "lengths", qkv.device)
+    q, k, v = (x[:, None] for x in _split_qkv(qkv, num_q_heads, nkv))
+    live = (lengths > 0).to(torch.int32)
+    if not _on_kernel(qkv):
+        pos = lengths[:, None].long() - 1
+        q, k = _rotate(q, table, pos), _rotate(k, table, pos)
+        _append_plain(k, v, k_pages, v_pages, page_table, lengths - 1, live)
+        return paged_decode_attention_int4(q[:, 0], k_pages, v_pages, page_table, lengths, softmax_scale=softmax_scale)
+    q_out = torch.empty((b, 1, num_q_heads, h), dtype=qkv.dtype, device=qkv.device)
+    with _device_of(qkv):
+        _launch_append((q, k, v, q_out, None, None), k_pages, v_pages, page_table, lengths, -1, live, table, b, 1, num_q_heads, nkv, h)
+    return paged_decode_attention_int4(q_out[:, 0], k_pages, v_pages, page_table, lengths, softmax_scale=softmax_scale,
+                                       splits=splits, scratch=scratch)
+
+
+def prompt_attention_int4(qkv: Tensor, k_pages: Int4Pages, v_pages: Int4Pages, page_table: Tensor, table: Tensor, *,
+                          num_q_heads: int, softmax_scale: float) -> Tensor:
+    """Whole prompts from position 0: ``qkv [B, T, (Nq + 2 Nkv) * H]`` of one projection.  Rotates queries and keys by ``table``,
+    appends keys and values to the cache and runs causal attention over what the cache then stands for: in ``qkv`` queries
+    are replaced by rotated ones, keys and values by the cache's.  Returns ``[B, T, Nq * H]``."""
+    nkv, h = _check_packed(qkv, k_pages, table, num_q_heads)
+    b, t, width = qkv.shape
+    _check_pages(k_pages, v_pages, page_table, num_q_heads, h, qkv.device)
+    if table.shape[0] < t or page_table.shape[0] != b or page_table.shape[1] * k_pages.codes.shape[2] < t:
+        raise ValueError(f"{b} x {t} tokens, a rotation table of {table.shape[0]} positions, a page table {tuple(page_table.shape)}")
+    q, k, v = _split_qkv(qkv, num_q_heads, nkv)
+    if not _on_kernel(qkv):
+        pos = torch.arange(t, device=qkv.device).expand(b, t)
+        q.copy_(_rotate(q, table, pos))
+        start = torch.zeros(b, dtype=torch.int32, device=qkv.device)
+        for x, y in zip((k, v), _append_plain(_rotate(k, table, pos), v, k_pages, v_pages, page_table, start, None)):
+            x.copy_(y)
+        out = dispatch.reference.attention(q, k, v, causal=True, softmax_scale=softmax_scale)
+        return out.reshape(b, t, num_q_heads * h)
+    from axlearn_b200.ops import decode_ops
+
+    with _device_of(qkv):
+        _launch_append((q, k, v, q, k, v), k_pages, v_pages, page_table, None, 0, None, table, b, t, num_q_heads, nkv, h)
+        return decode_ops.packed_prompt_attention(qkv, num_q_heads=num_q_heads, num_kv_heads=nkv, softmax_scale=softmax_scale)

@@ -1,0 +1,350 @@
+"""Kernels of the 4-bit weights and cache against plain statements in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _normal(gen, *shape):
+    return torch.randn(*shape, device="cuda", generator=gen)
+
+
+def _plain(fn, *args, **kwargs):
+    from axlearn_b200.ops.dispatch import use_reference_ops
+
+    with use_reference_ops():
+        return fn(*args, **kwargs)
+
+
+def _cache(b, max_pages, page_size, kv, dim, seed=0, spare=3):
+    """Pools of quantised normal values with larger and shifted channels, and a scrambled table."""
+    from axlearn_b200.ops import int4_ops
+
+    gen, pools = _gen(seed), []
+    for _ in range(2):
+        gain, mean = torch.exp(0.5 * _normal(gen, kv, 1, dim)), 0.5 * _normal(gen, kv, 1, dim)
+        x = (_normal(gen, b * max_pages + spare, kv, page_size, dim) * gain + mean).bfloat16()
+        codes, scales = int4_ops.quantize_groups(x, 32)
+        pools.append(int4_ops.Int4Pages(int4_ops._pack_rows(codes), scales))  # pylint: disable=protected-access
+    table = torch.randperm(b * max_pages + spare, device="cuda", generator=gen)[:b * max_pages]
+    return pools[0], pools[1], table.to(torch.int32).reshape(b, max_pages).contiguous()
+
+
+def _attention64(q, k_pages, v_pages, table, lengths, scale):
+    """``(out, bound)``: attention in 64 bits, and what rounding may add to it."""
+    from axlearn_b200.ops import int4_ops
+
+    b, nq, h = q.shape
+    kv = k_pages.codes.shape[1]
+    out, bound = torch.zeros(b, nq, h, dtype=torch.float64, device="cuda"), torch.zeros(b, nq, h, dtype=torch.float64, device="cuda")
+    for i, n in enumerate(lengths.tolist()):
+        if not n:
+            continue
+        pages = table[i, :-(-n // k_pages.codes.shape[2])].long()
+        (k, ks), (v, vs) = ((int4_ops.page_values(int4_ops.Int4Pages(x.codes[pages], x.scales[pages]), torch.float64),
+                             x.scales[pages].double()) for x in (k_pages, v_pages))
+        k, ks, v, vs = (x.transpose(0, 1).flatten(1, 2)[:, :n] for x in (k, ks, v, vs))
+        qg = q[i].double().view(kv, -1, h)
+        p = torch.softmax(qg @ k.transpose(1, 2) * scale, -1)
+        out[i] = (p @ v).flatten(0, 1)
+        # A score is a sum of products with 128 + c (tensor cores cut sums off at 2^-23 of their largest term): some 12 steps.
+        size = ks.abs() @ torch.tensor([143.0, 1.0], device="cuda", dtype=torch.float64)
+        moved = 12 * 2.0 ** -23 * scale * (qg.abs().unflatten(-1, (-1, 32)).sum(-1) @ size.transpose(1, 2)).amax(-1, keepdim=True)
+        # A probability's factor s is rounded to bf16 (2^-8); sums with 128 + c of it; the output's rounding.
+        low = vs[..., 1].repeat_interleave(32, -1)
+        step = vs[..., 0].repeat_interleave(32, -1)
+        bound[i] = (2.0 ** -8 * (p @ (v - low)) + 8 * 2.0 ** -23 * 143 * (p @ step) + torch.expm1(2 * moved) * (p @ v.abs())
+                    + 2.0 ** -20 * (p @ v.abs())).flatten(0, 1)
+        bound[i] = 1.01 * bound[i] + 2.0 ** -8 * (out[i].abs() + bound[i])
+    return out, bound
+
+
+@pytest.mark.parametrize("nq,kv,dim", [(4, 4, 128), (8, 4, 64), (3, 1, 128), (8, 2, 128), (16, 2, 64), (12, 1, 128), (40, 2, 128)])
+@pytest.mark.parametrize("page_size,splits", [(1, 1), (12, 2), (16, 3), (64, 8), (20, 9), (16, 17)])
+def test_attention_at_tile_split_and_page_edges(nq, kv, dim, page_size, splits):
+    from axlearn_b200.ops import cuda_ops, int4_ops
+
+    lens = [0, 1, 31, 32, 33, 127, 128, 129, 255, 320]
+    k_pages, v_pages, table = _cache(len(lens), -(-320 // page_size), page_size, kv, dim, seed=splits)
+    lengths = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q = (2 * _normal(_gen(1), len(lens), nq, dim)).bfloat16()
+    out = int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, lengths, splits=splits)
+    want, bound = _attention64(q, k_pages, v_pages, table, lengths, dim ** -0.5)
+    cuda_ops.check_status()
+    assert not out[0].any() and ((out.double() - want).abs() <= bound).all()
+    again = int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, lengths, splits=splits)
+    assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("b,nq,kv,dim,tokens", [(1, 16, 16, 128, 300), (1, 8, 2, 128, 40000), (33, 32, 8, 64, 700), (7, 32, 8, 128, 1)])
+def test_attention_with_splits_of_its_own(b, nq, kv, dim, tokens):
+    from axlearn_b200.ops import int4_ops
+
+    k_pages, v_pages, table = _cache(b, -(-tokens // 16), 16, kv, dim, seed=b)
+    lengths = torch.randint(0, tokens + 1, (b,), dtype=torch.int32, device="cuda", generator=_gen(2))
+    lengths[0] = tokens
+    q = _normal(_gen(3), b, 2 * nq, dim).bfloat16()[:, ::2]  # not contiguous
+    out = torch.full((b, nq, dim), 7.0, device="cuda", dtype=torch.bfloat16)
+    assert int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, lengths, softmax_scale=0.2, out=out) is out
+    want, bound = _attention64(q, k_pages, v_pages, table, lengths, 0.2)
+    assert ((out.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_rows_behind_a_sequence_and_other_pages_are_not_read(dim):
+    from axlearn_b200.ops import int4_ops
+
+    k_pages, v_pages, table = _cache(3, 4, 16, 2, dim, seed=5)
+    lengths = torch.tensor([5, 33, 47], dtype=torch.int32, device="cuda")
+    q = _normal(_gen(4), 3, 4, dim).bfloat16()
+    before = int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, lengths, splits=2)
+    for pages in (k_pages, v_pages):
+        used = torch.zeros(pages.codes.shape[0], 16, dtype=torch.bool, device="cuda")
+        for i, n in enumerate(lengths.tolist()):
+            for pos in range(n):
+                used[table[i, pos // 16].long(), pos % 16] = True
+        pages.scales.transpose(1, 2)[~used] = torch.nan
+        pages.codes.transpose(1, 2)[~used] = 255
+    table[0, 1:], table[1, 3:] = 10 ** 9, -7  # behind the sequences' last pages
+    after = int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, lengths, splits=2)
+    assert torch.equal(before, after)
+
+
+def test_values_that_are_not_numbers_stay_where_they_belong():
+    from axlearn_b200.ops import int4_ops
+
+    k_pages, v_pages, table = _cache(3, 4, 16, 2, 128, seed=6)
+    lengths = torch.tensor([60, 60, 1], dtype=torch.int32, device="cuda")
+    v_pages.scales[table[0, 1].long(), 1, 3, 2] = torch.tensor([0.0, torch.nan])
+    k_pages.scales[table[1, 0].long(), 0, 5, 0] = torch.tensor([0.0, torch.nan])
+    k_pages.scales[table[2, 0].long(), 1, 0, 1] = torch.tensor([0.0, torch.nan])   # the sequence's only key
+    q = _normal(_gen(5), 3, 4, 128).bfloat16()
+    for splits in (1, 2, 9):
+        bad = int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, lengths, splits=splits).isnan()
+        want = torch.zeros_like(bad)
+        want[0, 2:, 64:96] = want[1, :2] = want[2, 2:] = True
+        assert torch.equal(bad, want)
+
+
+def test_bad_places_are_reported_and_not_touched():
+    from axlearn_b200.ops import cuda_ops, int4_ops
+
+    k_pages, v_pages, table = _cache(2, 4, 16, 2, 128, seed=7)
+    q = _normal(_gen(6), 2, 4, 128).bfloat16()
+    k = _normal(_gen(7), 2, 3, 2, 128).bfloat16()
+    good = torch.tensor([64, 20], dtype=torch.int32, device="cuda")
+    want = int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, good)
+    cuda_ops.check_status()
+    out = int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, torch.tensor([65, 20], dtype=torch.int32, device="cuda"))
+    with pytest.raises(RuntimeError, match="status 5"):
+        cuda_ops.check_status()
+    assert torch.equal(out, want)
+    before = [x.clone() for x in (*k_pages, *v_pages)]
+    for page, start in ((11, 0), (-1, 0), (0, 62), (0, -1)):
+        bad = table.clone()
+        if page:
+            bad[0, 0] = page
+        at = torch.tensor([start, 61], dtype=torch.int32, device="cuda")
+        live = torch.tensor([3, 0], dtype=torch.int32, device="cuda")
+        int4_ops.append_int4(k, k, k_pages, v_pages, bad, at, live=live)
+        with pytest.raises(RuntimeError, match="status 5"):
+            cuda_ops.check_status()
+        if page:
+            assert all(torch.equal(x, y) for x, y in zip(before, (*k_pages, *v_pages)))
+            int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, bad, good)
+            with pytest.raises(RuntimeError, match="status 5"):
+                cuda_ops.check_status()
+
+
+@pytest.mark.parametrize("b,t,kv,dim,page_size,packed", [(1, 1, 1, 128, 16, False), (3, 37, 2, 64, 12, True), (5, 9, 3, 128, 1, True),
+                                                       (64, 1, 32, 128, 16, True), (2, 700, 8, 128, 64, True)])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_append_has_the_bits_of_the_plain_statement(b, t, kv, dim, page_size, packed, ragged):
+    from axlearn_b200.ops import cuda_ops, int4_ops
+
+    gen, pages = _gen(b), -(-(t + 40) // page_size)
+    k_pages, v_pages, table = _cache(b, pages, page_size, kv, dim, seed=t)
+    other = [int4_ops.Int4Pages(*(x.clone() for x in p)) for p in (k_pages, v_pages)]
+    x = (_normal(gen, b, t, 2 * kv + 1, dim) * torch.exp(3 * _normal(gen, b, t, 2 * kv + 1, 1))).bfloat16()
+    x[0, 0, 1] = 2.5                      # no range
+    x[0, -1, 1, 3], x[0, -1, -1, -1] = torch.nan, torch.inf
+    x[-1, 0, 2, :32], x[-1, 0, 2, 32:64] = 0.0, x[-1, 0, 2, 32:64] * 2.0 ** -126
+    k, v = x[:, :, 1:kv + 1], x[:, :, kv + 1:]
+    if not packed:
+        k, v = k.contiguous(), v.contiguous()
+    start = torch.randint(0, 41, (b,), dtype=torch.int32, device="cuda", generator=gen)
+    live = torch.randint(0, t + 1, (b,), dtype=torch.int32, device="cuda", generator=gen) if ragged else None
+    got = int4_ops.append_int4(k, v, k_pages, v_pages, table, start, live=live, values=True)
+    want = _plain(int4_ops.append_int4, k, v, *other, table, start, live=live, values=True)
+    cuda_ops.check_status()
+    for x, y in zip((*k_pages, *v_pages, *got), (*other[0], *other[1], *want)):
+        assert x.dtype == y.dtype and torch.equal(x.nan_to_num(nan=12345.0) if x.is_floating_point() else x,
+                                                  y.nan_to_num(nan=12345.0) if y.is_floating_point() else y)
+
+
+def _linear64(x, w):
+    """``(y, bound)`` in 64 bits."""
+    from axlearn_b200.ops import int4_ops
+
+    values = _plain(int4_ops.dequantize_weight, w, torch.float32).double()
+    y = x.double() @ values
+    terms = x.double().abs() @ values.abs()
+    if x.shape[0] > int4_ops.MAX_STREAMED_ROWS:
+        bound = 2.0 ** -8 * terms + 2.0 ** -23 * w.k * terms  # weights rounded to bf16; sums of k terms in any order
+    else:
+        # Products with 128 + c of up to 128 values (tensor cores cut sums off at 2^-23 of their largest term), 8 steps a group
+        # and a few in 32 bits for every group and warp.
+        tiles, groups = w.scales.shape[:2]
+        pairs = w.scales.double().abs().permute(0, 3, 2, 1, 4).reshape(tiles * 16, groups, 2)[:w.n]
+        size = (pairs @ torch.tensor([271.0, 2.0], device="cuda", dtype=torch.float64)).t()
+        xs = torch.nn.functional.pad(x.double().abs(), (0, groups * w.group - w.k)).unflatten(-1, (groups, w.group)).sum(-1)
+        bound = (10 + groups / 8 + 8) * 2.0 ** -23 * (xs @ size)
+    return y, 1.01 * bound + 2.0 ** -8 * (y.abs() + bound)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 7, 8, 9, 16, 17, 31, 33, 64, 65, 200])
+@pytest.mark.parametrize("k,n,group", [(8, 8, 64), (72, 24, 128), (200, 40, 64), (1096, 328, 128), (2048, 96, 64)])
+def test_linear_of_few_and_many_rows(rows, k, n, group):
+    from axlearn_b200.ops import cuda_ops, int4_ops
+
+    gen = _gen(rows + k)
+    w = int4_ops.quantize_weight(_normal(gen, k, n) * k ** -0.5 + 0.01, group=group)
+    x = (_normal(gen, rows, k) * torch.exp(_normal(gen, k))).bfloat16()
+    y, bound = _linear64(x, w)
+    got = int4_ops.int4_linear(x, w)
+    assert got.dtype == torch.bfloat16 and ((got.double() - y).abs() <= bound).all()
+    out = _normal(gen, rows, n).bfloat16()
+    want = out.double() + y
+    assert int4_ops.int4_linear(x, w, out=out, accumulate=True) is out
+    cuda_ops.check_status()
+    # The sum is rounded again; behind the GEMM it may be added to an unrounded or a rounded product.
+    assert ((out.double() - want).abs() <= bound + 2.0 ** -8 * (want.abs() + y.abs() + bound)).all()
+
+
+@pytest.mark.parametrize("rows", [3, 40, 90])
+def test_linear_takes_strided_rows_and_keeps_rows_apart(rows):
+    from axlearn_b200.ops import int4_ops
+
+    gen = _gen(11)
+    w = int4_ops.quantize_weight(_normal(gen, 256, 48))
+    wide = _normal(gen, 2, rows, 300).bfloat16()
+    for x in (wide[0, :, 16:272], wide[0, :, 1:257], wide[:, :, :256], wide[0, :, 44:], wide[0, :256 // rows * 0 + rows, 8:264]):
+        assert torch.equal(int4_ops.int4_linear(x, w), int4_ops.int4_linear(x.clone(memory_format=torch.contiguous_format), w))
+    x = wide[0, :, :256].clone()
+    before = int4_ops.int4_linear(x, w)
+    x[rows // 2, 5], x[0, 0] = torch.nan, torch.inf
+    after = int4_ops.int4_linear(x, w)
+    hit = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    hit[0] = hit[rows // 2] = True
+    assert torch.equal(before[~hit], after[~hit]) and not after[hit].isfinite().any()
+    assert int4_ops.int4_linear(x[:0], w).shape == (0, 48)
+
+
+@pytest.mark.parametrize("k,n,group", [(8, 8, 128), (200, 40, 64), (1096, 328, 128)])
+def test_expanded_weights_have_the_bits_of_the_plain_statement(k, n, group):
+    from axlearn_b200.ops import int4_ops
+
+    w = int4_ops.quantize_weight(_normal(_gen(k), k, n), group=group)
+    assert torch.equal(int4_ops.dequantize_weight(w), _plain(int4_ops.dequantize_weight, w))
+
+
+@pytest.mark.parametrize("nq,kv,dim,splits", [(4, 4, 128, 1), (8, 2, 64, 3), (20, 2, 128, 9), (32, 8, 128, None)])
+def test_a_step_is_rotation_append_and_attention(nq, kv, dim, splits):
+    from axlearn_b200.ops import cuda_ops, decode_ops, int4_ops
+
+    lens = [0, 1, 16, 17, 32, 33, 95, 96]
+    b, page_size = len(lens), 16
+    k_pages, v_pages, table = _cache(b, 6, page_size, kv, dim, seed=8)
+    other = [int4_ops.Int4Pages(*(x.clone() for x in p)) for p in (k_pages, v_pages)]
+    rope = decode_ops.rope_table(96, dim, 1e4, "cuda")
+    lengths = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    qkv = _normal(_gen(9), b, (nq + 2 * kv) * dim).bfloat16()
+    given = qkv.clone()
+    out = int4_ops.rope_decode_attention_int4(qkv, k_pages, v_pages, table, lengths, rope, num_q_heads=nq, softmax_scale=dim ** -0.5,
+                                              splits=splits)
+    _plain(int4_ops.rope_decode_attention_int4, qkv, *other, table, lengths, rope, num_q_heads=nq, softmax_scale=dim ** -0.5)
+    cuda_ops.check_status()
+    assert torch.equal(qkv, given)
+    q = qkv.view(b, -1, dim)[:, :nq]
+    q = int4_ops._rotate(q[:, None], rope, lengths[:, None].long() - 1)[:, 0]  # pylint: disable=protected-access
+    want, bound = _attention64(q, k_pages, v_pages, table, lengths, dim ** -0.5)
+    # The rotated query may round the other way where products are fused: 2^-8 of it, as a score's move.
+    scale = 2.0 ** -8 * dim ** -0.5 * dim * q.abs().max() * int4_ops.page_values(k_pages).abs().max()
+    slack = torch.expm1(2 * scale * 2.0 ** -8) * int4_ops.page_values(v_pages).abs().max()
+    assert ((out.double() - want).abs() <= bound + slack).all() and not out[0].any()
+    # The new rows: a rotated key may round the other way, which moves a level by one step at most.
+    for mine, plain in zip((k_pages, v_pages), other):
+        a, c = int4_ops.page_values(mine), int4_ops.page_values(plain)
+        step = plain.scales[..., 0].float().repeat_interleave(32, -1)
+        assert ((a - c).abs() <= 1.1 * step + 2.0 ** -6 * c.abs()).all()
+        assert (a != c).float().mean() < 1e-3
+    assert torch.equal(v_pages.codes, other[1].codes) and torch.equal(v_pages.scales, other[1].scales)
+
+
+@pytest.mark.parametrize("b,t,nq,kv,dim", [(2, 300, 8, 2, 128), (1, 1, 4, 4, 64), (3, 130, 12, 4, 64)])
+def test_prompts_attend_to_what_the_cache_stands_for(b, t, nq, kv, dim):
+    from axlearn_b200.ops import cuda_ops, decode_ops, int4_ops
+
+    k_pages, v_pages, table = _cache(b, -(-t // 16), 16, kv, dim, seed=10)
+    rope = decode_ops.rope_table(t, dim, 1e4, "cuda")
+    qkv = _normal(_gen(12), b, t, (nq + 2 * kv) * dim).bfloat16()
+    given = qkv.clone()
+    out = int4_ops.prompt_attention_int4(qkv, k_pages, v_pages, table, rope, num_q_heads=nq, softmax_scale=dim ** -0.5)
+    cuda_ops.check_status()
+    q, k, v = qkv.view(b, t, -1, dim).split((nq, kv, kv), 2)
+    pos = torch.arange(t, device="cuda")
+    for x, pages in ((k, k_pages), (v, v_pages)):  # what attention read is what the cache holds
+        held = int4_ops.page_values(pages, torch.bfloat16)[table.long()].transpose(2, 3).flatten(1, 2)[:, :t]
+        assert torch.equal(x, held)
+    g = given.view(b, t, -1, dim)
+    turned = int4_ops._rotate(g, rope, pos.expand(b, t))  # pylint: disable=protected-access
+    assert ((q.float() - turned[:, :, :nq].float()).abs() <= 2.0 ** -7 * turned[:, :, :nq].float().abs() + 2.0 ** -20).all()
+    qq, kk, vv = (x.double().transpose(1, 2) for x in (q, k.repeat_interleave(nq // kv, 2), v.repeat_interleave(nq // kv, 2)))
+    seen = pos[:, None] >= pos
+    p = torch.softmax((qq @ kk.transpose(2, 3) * dim ** -0.5).masked_fill(~seen, -torch.inf), -1)
+    want, size = ((p @ x).transpose(1, 2).flatten(2) for x in (vv, vv.abs()))
+    # Probabilities in bf16 and the output's rounding; scores and sums in 32 bits.
+    assert ((out.double() - want).abs() <= 2.0 ** -8 * (want.abs() + 1.02 * size) + 2.0 ** -12 * size).all()
+
+
+def test_calls_replay_in_a_graph_and_on_another_stream():
+    """Captured append, step and product: replays see new inputs, and have the bits of separate calls."""
+    from axlearn_b200.ops import cuda_ops, decode_ops, int4_ops
+
+    b, nq, kv, dim = 2, 8, 2, 128
+    k_pages, v_pages, table = _cache(b, 80, 16, kv, dim, seed=13)
+    rope = decode_ops.rope_table(1280, dim, 1e4, "cuda")
+    lengths = torch.tensor([700, 9], dtype=torch.int32, device="cuda")
+    w = int4_ops.quantize_weight(_normal(_gen(14), 512, (nq + 2 * kv) * dim))
+    x = _normal(_gen(15), b, 512).bfloat16()
+
+    def step(cache):
+        qkv = int4_ops.int4_linear(x, w)
+        return int4_ops.rope_decode_attention_int4(qkv, *cache, table, lengths, rope, num_q_heads=nq, softmax_scale=0.05, splits=9)
+
+    mine = [int4_ops.Int4Pages(*(t.clone() for t in p)) for p in (k_pages, v_pages)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        warm = step(mine)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(warm, step((k_pages, v_pages)))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph), cuda_ops.chained_launches():
+        out = step(mine)
+    for seed in (16, 17, 18):
+        lengths.add_(1)
+        x.copy_(_normal(_gen(seed), b, 512))
+        graph.replay()
+        assert torch.equal(out, step((k_pages, v_pages)))
+    for p, o in zip(mine, (k_pages, v_pages)):
+        row = (table.long().gather(1, (lengths[:, None].long() - 1) // 16)[:, 0], (lengths.long() - 1) % 16)
+        assert torch.equal(p.codes[row[0], :, row[1]], o.codes[row[0], :, row[1]])
+    cuda_ops.check_status()

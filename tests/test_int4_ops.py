@@ -1,0 +1,280 @@
+"""4-bit weights and cache: the format, the plain statements and the refusals (no GPU)."""
+
+import math
+
+import pytest
+import torch
+
+from axlearn_b200.ops import int4_ops
+
+
+def _values(*shape, seed=0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed))
+
+
+def _level(x: float, low: float, step: float) -> int:
+    """The code of one value, by Python's own rounding (ties to even)."""
+    return min(15, max(0, round((x - low) / step))) if step else 0
+
+
+@pytest.mark.parametrize("group", [32, 64])
+def test_groups_hold_the_nearest_level(group):
+    x = torch.cat([_values(5, 3 * group) * s + o for s, o in ((1, 0), (1e-3, 7), (300, -900))]).bfloat16()
+    codes, scales = int4_ops.quantize_groups(x, group)
+    assert codes.shape == x.shape and scales.shape == (15, 3, 2) and scales.dtype == torch.bfloat16
+    for row in range(15):
+        for g in range(3):
+            part = x[row, g * group:(g + 1) * group].double().tolist()
+            step, low = scales[row, g].double().tolist()
+            assert low == min(part)
+            # A fifteenth of the range: to half a unit of bf16, and the range and its product with 1 / 15 in 32 bits.
+            assert abs(step - (max(part) - low) / 15) <= (2.0 ** -8 + 2.0 ** -20) * (max(part) - low) / 15
+            for value, code in zip(part, codes[row, g * group:(g + 1) * group].tolist()):
+                assert code == _level(value, low, step)
+    # Half a step, and what the rounding of the step leaves behind level 15: 15 * 2^-8 of a step; sums in 32 bits.
+    step = scales[..., :1].double()
+    error = (int4_ops.group_values(codes, scales).double() - x.double()).abs().unflatten(-1, (-1, group))
+    assert (error <= step * (0.5 + 15 * 2.0 ** -8) + 2.0 ** -22 * x.double().abs().amax()).all()
+
+
+def test_groups_without_a_range_and_groups_that_are_not_finite():
+    x = torch.zeros(8, 32).bfloat16()
+    x[1] = 3.25
+    x[2, 4], x[3, 5], x[4, 6] = float("nan"), float("inf"), -float("inf")
+    x[5, 0], x[5, 1] = 3e38, -3e38                    # the range overflows
+    x[6] = torch.linspace(0, 1, 32).bfloat16() * 2.0 ** -126   # a step below the smallest normal number
+    x[7, 31] = 15.0
+    codes, scales = int4_ops.quantize_groups(x, 32)
+    values = int4_ops.group_values(codes, scales)
+    assert torch.equal(values[:2], x[:2].float()) and not codes[:6].any()
+    assert values[2:6].isnan().all()
+    assert (values[6] == 0).all() and not scales[6].any()
+    assert torch.equal(values[7], x[7].float()) and codes[7, 31] == 15
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_rows_of_the_cache_are_in_the_documented_order(dim):
+    codes = torch.randint(0, 16, (3, 5, dim), dtype=torch.uint8, generator=torch.Generator().manual_seed(1))
+    rows = int4_ops._pack_rows(codes)  # pylint: disable=protected-access
+    assert rows.shape == (3, 5, dim // 2) and torch.equal(int4_ops._unpack_rows(rows), codes)  # pylint: disable=protected-access
+    groups = dim // 32
+    for d in range(dim):
+        g, chunk, rest = d // 32, d % 32 // 4, d % 4
+        byte = rows[..., chunk * 2 * groups + 2 * g + rest // 2]
+        assert torch.equal(byte >> 4 if rest % 2 else byte & 15, codes[..., d])
+
+
+@pytest.mark.parametrize("k,n,group", [(8, 8, 64), (72, 24, 64), (128, 16, 128), (200, 40, 128), (384, 56, 64)])
+def test_weights_hold_their_groups_and_keep_their_order(k, n, group):
+    w = _values(k, n, seed=k) * 0.1
+    q = int4_ops.quantize_weight(w, group=group)
+    assert q.shape == (k, n) and q.codes.shape == (-(-n // 16), -(-k // 128) * 2, 512)
+    got = int4_ops.dequantize_weight(q, torch.float32)
+    assert got.shape == (k, n)
+    for lo in range(0, k, group):
+        part = torch.zeros(group, n)
+        part[:min(group, k - lo)] = w[lo:lo + group]
+        codes, scales = int4_ops.quantize_groups(part.t(), group)
+        want = int4_ops.group_values(codes, scales).t()[:min(group, k - lo)]
+        assert torch.equal(got[lo:lo + group], want)
+    # One column and one row of a block by the documented places.
+    column, row = n - 1, min(k - 1, 63)
+    block = q.codes[column // 16, 0].view(8, 4, 4, 2, 2)[column % 8, row // 16, row % 16 // 4, row % 2, row % 4 // 2]
+    code = int(block) >> 4 if column % 16 >= 8 else int(block) & 15
+    step, low = q.scales[column // 16, 0, column % 8, column % 16 // 8].float().tolist()
+    assert got[row, column].item() == pytest.approx(low + step * code, rel=1e-6)
+
+
+def test_linear_matches_its_formula_and_adds_to_out():
+    w = int4_ops.quantize_weight(_values(72, 24, seed=2), group=64)
+    x = _values(2, 3, 72, seed=3)
+    want = x.double() @ int4_ops.dequantize_weight(w, torch.float32).double()
+    # 72 products and sums in 32 bits.
+    bound = 74 * 2.0 ** -24 * (x.double().abs() @ int4_ops.dequantize_weight(w, torch.float32).double().abs())
+    got = int4_ops.int4_linear(x, w)
+    assert got.shape == (2, 3, 24) and ((got - want).abs() <= bound).all()
+    out = torch.ones(2, 3, 24)
+    assert int4_ops.int4_linear(x, w, out=out, accumulate=True) is out
+    assert ((out - 1 - want).abs() <= bound + 2.0 ** -23 * (1 + want.abs())).all()
+    assert int4_ops.int4_linear(x[:0], w).shape == (0, 3, 24)
+
+
+def _cache(b, max_pages, page_size, kv, dim, seed=0, spare=2):
+    gen = torch.Generator().manual_seed(seed)
+    pools = [int4_ops.int4_pages(b * max_pages + spare, page_size, kv, dim) for _ in range(2)]
+    table = torch.randperm(b * max_pages + spare, generator=gen)[:b * max_pages].to(torch.int32).reshape(b, max_pages)
+    return pools[0], pools[1], table
+
+
+@pytest.mark.parametrize("dim,page_size", [(64, 5), (128, 16)])
+def test_append_writes_live_tokens_and_nothing_else(dim, page_size):
+    b, t, kv = 3, 7, 2
+    k_pages, v_pages, table = _cache(b, 4, page_size, kv, dim)
+    for pages in (k_pages, v_pages):
+        pages.codes.random_(0, 255)
+        pages.scales.normal_()
+    before = [x.clone() for x in (*k_pages, *v_pages)]
+    start, live = torch.tensor([0, 3, 9], dtype=torch.int32), torch.tensor([7, 0, 4], dtype=torch.int32)
+    k, v = (_values(b, t, kv, dim, seed=s).bfloat16() for s in (5, 6))
+    kv_values = int4_ops.append_int4(k, v, k_pages, v_pages, table, start, live=live, values=True)
+    touched = torch.zeros(k_pages.codes.shape[0], page_size, dtype=torch.bool)
+    for x, pages, got in zip((k, v), (k_pages, v_pages), kv_values):
+        held = int4_ops.page_values(pages)
+        for i in range(b):
+            for j in range(t):
+                if j >= live[i]:
+                    assert not got[i, j].any()
+                    continue
+                pos = int(start[i]) + j
+                page, row = int(table[i, pos // page_size]), pos % page_size
+                touched[page, row] = True
+                codes, scales = int4_ops.quantize_groups(x[i, j], 32)
+                assert torch.equal(held[page, :, row], int4_ops.group_values(codes, scales))
+                assert torch.equal(got[i, j], held[page, :, row].bfloat16())
+    for old, new in zip(before, (*k_pages, *v_pages)):
+        assert torch.equal(old.transpose(1, 2)[~touched], new.transpose(1, 2)[~touched])
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(4, 4, 64), (6, 2, 128)])
+def test_attention_over_the_cache_matches_a_loop(heads, kv, dim):
+    b, page_size, lengths = 4, 6, [0, 1, 13, 18]
+    k_pages, v_pages, table = _cache(b, 3, page_size, kv, dim, seed=7)
+    k, v = (_values(b, 18, kv, dim, seed=s).bfloat16() for s in (8, 9))
+    lens = torch.tensor(lengths, dtype=torch.int32)
+    int4_ops.append_int4(k, v, k_pages, v_pages, table, torch.zeros(b, dtype=torch.int32), live=lens)
+    k_pages.scales[table[2, 2].long(), :, 2:] = torch.nan  # behind the third sequence's last token
+    q = _values(b, heads, dim, seed=10).bfloat16()
+    out = int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, lens)
+    assert not out[0].any()
+    kk, vv = int4_ops.page_values(k_pages, torch.float64), int4_ops.page_values(v_pages, torch.float64)
+    for i in range(1, b):
+        for h in range(heads):
+            at = [(int(table[i, p // page_size]), h // (heads // kv), p % page_size) for p in range(lengths[i])]
+            keys, vals = (torch.stack([x[j] for j in at]) for x in (kk, vv))
+            p = torch.softmax(keys @ q[i, h].double() / math.sqrt(dim), 0)
+            # The output's rounding, and a few hundred operations in 32 bits.
+            assert ((out[i, h].double() - p @ vals).abs() <= 2.0 ** -8 * (p @ vals).abs() + 2.0 ** -14 * vals.abs().max()).all()
+
+
+def test_a_decoding_step_is_rotation_append_and_attention():
+    b, heads, kv, dim, page_size = 3, 4, 2, 64, 4
+    k_pages, v_pages, table = _cache(b, 3, page_size, kv, dim, seed=11)
+    past = [_values(b, 12, kv, dim, seed=s).bfloat16() for s in (12, 13)]
+    lens = torch.tensor([0, 5, 12], dtype=torch.int32)
+    int4_ops.append_int4(*past, k_pages, v_pages, table, torch.zeros(b, dtype=torch.int32), live=(lens - 1).clamp(min=0))
+    angle = torch.arange(12)[:, None] * 0.3 ** torch.arange(dim // 2)
+    rope = torch.stack((angle.sin(), angle.cos()), -1)
+    qkv = _values(b, (heads + 2 * kv) * dim, seed=14).bfloat16()
+    out = int4_ops.rope_decode_attention_int4(qkv, k_pages, v_pages, table, lens, rope, num_q_heads=heads, softmax_scale=0.1)
+    q, k, v = qkv.view(b, -1, dim).split((heads, kv, kv), 1)
+
+    def turned(x, pos):
+        z = torch.view_as_complex(x.float().unflatten(-1, (-1, 2)).contiguous()) * torch.polar(torch.ones(dim // 2), angle[pos])
+        return torch.view_as_real(z).flatten(-2).bfloat16()
+
+    for i, n in ((1, 5), (2, 12)):
+        page, row = int(table[i, (n - 1) // page_size]), (n - 1) % page_size
+        for x, pages in ((turned(k[i], n - 1), k_pages), (v[i], v_pages)):
+            codes, scales = int4_ops.quantize_groups(x, 32)
+            assert torch.equal(int4_ops.page_values(pages)[page, :, row], int4_ops.group_values(codes, scales))
+        want = int4_ops.paged_decode_attention_int4(turned(q[i], n - 1)[None], k_pages, v_pages, table[i:i + 1], lens[i:i + 1],
+                                                    softmax_scale=0.1)
+        assert torch.equal(out[i], want[0])
+    assert not out[0].any()
+
+
+def test_prompts_attend_to_what_the_cache_stands_for():
+    b, t, heads, kv, dim = 2, 9, 4, 2, 64
+    k_pages, v_pages, table = _cache(b, 3, 4, kv, dim, seed=15)
+    angle = torch.arange(t)[:, None] * 0.5 ** torch.arange(dim // 2)
+    rope = torch.stack((angle.sin(), angle.cos()), -1)
+    qkv = _values(b, t, (heads + 2 * kv) * dim, seed=16).bfloat16()
+    given = qkv.clone()
+    out = int4_ops.prompt_attention_int4(qkv, k_pages, v_pages, table, rope, num_q_heads=heads, softmax_scale=0.2)
+    step_pages = _cache(b, 3, 4, kv, dim, seed=15)
+    for i in range(t):
+        lens = torch.full((b,), i + 1, dtype=torch.int32)
+        one = int4_ops.rope_decode_attention_int4(given[:, i].contiguous(), step_pages[0], step_pages[1], table, lens, rope,
+                                                  num_q_heads=heads, softmax_scale=0.2)
+        # The prompt reads values rounded to bf16: a score moves by up to 2^-8 of its terms, a probability by e^(2 move), a
+        # value by 2^-8; then both outputs are rounded.
+        terms = 0.2 * dim * qkv[:, i, :heads * dim].abs().max() * int4_ops.page_values(k_pages).abs().max()
+        bound = (torch.expm1(2 * 2.0 ** -8 * terms) + 3 * 2.0 ** -8) * int4_ops.page_values(v_pages).abs().max()
+        assert (one.flatten(1).float() - out[:, i].float()).abs().max() <= bound
+    for x, y in zip((*k_pages, *v_pages), (*step_pages[0], *step_pages[1])):
+        assert torch.equal(x, y)
+
+
+def _attend_args(**change):
+    k_pages, v_pages, table = _cache(2, 3, 4, 2, 64)
+    args = dict(q=_values(2, 4, 64).bfloat16(), k_pages=k_pages, v_pages=v_pages, page_table=table,
+                lengths=torch.tensor([3, 12], dtype=torch.int32))
+    args.update(change)
+    return args
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(q=torch.zeros(2, 3, 64).bfloat16()), ValueError),                          # heads are no multiple of the cache's
+    (dict(q=torch.zeros(2, 4, 128).bfloat16()), ValueError),                         # another head size
+    (dict(q=torch.zeros(1, 4, 64).bfloat16()), ValueError),                          # another batch
+    (dict(lengths=torch.tensor([3, 12])), ValueError),                               # int64
+    (dict(lengths=torch.tensor([3, 13], dtype=torch.int32)), IndexError),            # behind the table
+    (dict(page_table=torch.zeros(2, 3, dtype=torch.int64)), ValueError),
+    (dict(page_table=torch.zeros(3, 2, dtype=torch.int32).t()), ValueError),         # not contiguous
+    (dict(page_table=torch.full((2, 3), 8, dtype=torch.int32)), IndexError),         # pages that the pool does not have
+    (dict(page_table=torch.full((2, 3), -1, dtype=torch.int32)), IndexError),
+    (dict(out=torch.zeros(2, 4, 64)), ValueError),                                   # out of another type
+    (dict(k_pages=int4_ops.int4_pages(8, 4, 2, 128)), ValueError),
+    (dict(v_pages=int4_ops.int4_pages(7, 4, 2, 64)), ValueError),                    # pools of two sizes
+])
+def test_attention_refuses(change, error):
+    int4_ops.paged_decode_attention_int4(**_attend_args())
+    with pytest.raises(error):
+        int4_ops.paged_decode_attention_int4(**_attend_args(**change))
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(v=torch.zeros(2, 5, 2, 64)), ValueError),                                  # another type than k
+    (dict(k=torch.zeros(2, 5, 4, 64).bfloat16(), v=torch.zeros(2, 5, 4, 64).bfloat16()), ValueError),
+    (dict(start=torch.tensor([0, 0])), ValueError),
+    (dict(start=torch.tensor([0], dtype=torch.int32)), ValueError),
+    (dict(live=torch.tensor([5.0, 5.0])), ValueError),
+    (dict(start=torch.tensor([0, 8], dtype=torch.int32)), IndexError),               # position 12 of 12
+    (dict(start=torch.tensor([-1, 0], dtype=torch.int32)), IndexError),
+    (dict(page_table=torch.full((2, 3), 8, dtype=torch.int32)), IndexError),
+])
+def test_append_refuses(change, error):
+    k_pages, v_pages, table = _cache(2, 3, 4, 2, 64)
+    args = dict(k=_values(2, 5, 2, 64).bfloat16(), v=_values(2, 5, 2, 64).bfloat16(), k_pages=k_pages, v_pages=v_pages,
+                page_table=table, start=torch.zeros(2, dtype=torch.int32))
+    int4_ops.append_int4(**args)
+    with pytest.raises(error):
+        int4_ops.append_int4(**{**args, **change})
+
+
+def test_weights_and_products_refuse():
+    w = int4_ops.quantize_weight(_values(64, 16))
+    for shape, group in (((60, 16), 128), ((64, 12), 128), ((64, 16), 32)):
+        with pytest.raises(ValueError):
+            int4_ops.quantize_weight(_values(*shape), group=group)
+    with pytest.raises(ValueError):
+        int4_ops.quantize_weight(_values(2, 64, 16))
+    with pytest.raises(ValueError):
+        int4_ops.Int4Weight(w.codes, w.scales, k=64, n=16, group=64)
+    with pytest.raises(ValueError):
+        int4_ops.int4_linear(_values(3, 72), w)
+    with pytest.raises(ValueError):
+        int4_ops.int4_linear(_values(3, 64).requires_grad_(), w)
+    with pytest.raises(ValueError):
+        int4_ops.int4_linear(_values(3, 64), w, accumulate=True)
+    with pytest.raises(ValueError):
+        int4_ops.int4_linear(_values(3, 64), w, out=torch.zeros(3, 24))
+    with pytest.raises(ValueError):
+        int4_ops.int4_pages(2, 16, 2, 96)
+
+
+@pytest.mark.parametrize("batch,kv,group,tokens", [(1, 16, 1, 300), (16, 8, 4, 2048), (64, 32, 1, 2000), (1, 8, 4, 130048),
+                                                   (1, 1, 1, 1), (0, 4, 1, 64), (300, 32, 16, 4096)])
+def test_splits_of_attention(batch, kv, group, tokens):
+    splits = int4_ops.attention_splits(batch, kv, group, tokens)
+    assert 1 <= splits <= 64 and (splits == 1 or tokens >= 32 * splits)
