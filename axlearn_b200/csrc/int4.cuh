@@ -13,13 +13,16 @@ namespace axb {
 
 constexpr int kInt4Group = 32;
 
-// Bits [4i, 4i + 4) and [16 + 4i, 20 + 4i) of x as two bf16 numbers 128 + code: the codes are the last bits of a mantissa
-// of 128 = 2^7, so a shift and one logic operation convert two of them.  The 128 is taken off the sums.
-__device__ __forceinline__ uint32_t int4_pair(uint32_t x, int i) {
-  uint32_t y;
-  asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xEA;" : "=r"(y) : "r"(x >> (4 * i)));
-  return y;
-}
+// Codes as operands of a product: the bf16 number with the bits v < 256 is v 2^-133 (below 2^-126 a denormal, which MMAs take
+// as it is, then the first binade of the same spacing).  So the low nibble of each half is a code times 2^-133 as it lies,
+// the next one 16 times that: one logic operation for two codes, and no offset.  The other operand carries 2^kInt4Shift, so
+// that products stay far above the denormal numbers of fp32: results are 2^(kInt4Shift - 133) of the sums of codes.
+constexpr int kInt4Shift = 32;
+constexpr float kInt4Scale = 4294967296.f;                         // 2^kInt4Shift
+constexpr float kInt4Back = 2535301200456458802993406410752.f;    // 2^(133 - kInt4Shift)
+
+__device__ __forceinline__ uint32_t int4_low(uint32_t x) { return x & 0x000f000fu; }
+__device__ __forceinline__ uint32_t int4_high(uint32_t x) { return x & 0x00f000f0u; }  // 16 codes
 
 // The two bf16 of a pair (s, m) as they lie.
 __device__ __forceinline__ float pair_s(uint32_t u) { return __uint_as_float(u << 16); }

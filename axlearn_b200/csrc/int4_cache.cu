@@ -171,8 +171,8 @@ struct Int4AttnParams {
   float* part_ml;          // [B, Nq, splits, 2]
   __nv_bfloat16* out;
   int* status;
-  int num_q_heads, num_kv_heads, page_size, max_pages, num_pages, splits;
-  float scale_log2;
+  int num_q_heads, num_kv_heads, page_size, page_shift, max_pages, num_pages, splits;  // page_shift: -1 where no power of two
+  float scale_log2;      // softmax scale * log2(e) * kInt4Back, > 0
 };
 
 constexpr int kAttnThreads = 128, kAttnWarps = kAttnThreads / 32;
@@ -198,6 +198,32 @@ struct Int4Tile {
   }
 };
 
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* src) {
+  static_assert(N == 2 || N == 4, "8 or 16 bytes");
+  if constexpr (N == 4) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(src);
+  else *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(src);
+}
+
+// d = a b + c.
+__device__ __forceinline__ void mma_add(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+
+__device__ __forceinline__ uint32_t times(uint32_t x, __nv_bfloat162 f) {
+  const __nv_bfloat162 y = __hmul2(reinterpret_cast<__nv_bfloat162&>(x), f);
+  return reinterpret_cast<const uint32_t&>(y);
+}
+
+// An 8 x 8 tile of bf16 pairs, lane (r, c) with entries (r, 2c), (r, 2c + 1): its transpose in the same layout.
+__device__ __forceinline__ uint32_t turned_round(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
@@ -205,13 +231,17 @@ __device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, bool ok
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(ok ? 8 : 0) : "memory");
 }
 
-// S = Q K^T: rows 0-7 of the m16n8k16 tile are the query heads, K is the B operand; a lane takes dims 8c .. 8c + 7 of each
-// group of a key and the sums of a group are multiplied by its s: q.k = sum_g s_g (sum q c) + m_g sum q.  The products
-// start at -128 sum q.
+// S^T = K Q^T: 16 keys are the rows of the m16n8k16 tile, the query heads its columns; a lane takes dims 8c .. 8c + 7 of each
+// group of a key, and the sums of a group are multiplied by its s: k.q = sum_g s_g (sum c q) + m_g sum q.
 // O^T = V^T P^T: 16 dims of one group are the rows, the heads the columns; s of a key's group is multiplied into P, which is
-// rounded to bf16 (2^-9 of a probability, the sums of p m stay in 32 bits).  The products start at -128 sum P, by an MMA.
+// rounded to bf16 (2^-9 of a probability, the sums of p m stay in 32 bits) and turned round by `movmatrix`.
+// Codes enter as denormal bf16 numbers (`int4.cuh`): scores carry 1 / kInt4Back until the exponential, probabilities and the
+// sums of them alone kInt4Scale, and the sums of p c 1 / kInt4Back.
+// The maximum that probabilities are relative to moves only when a score passes it by kSlack (a factor of 2^kSlack).
+constexpr float kSlack = 8.f;
+
 template <int H, bool kCluster>
-__global__ void __launch_bounds__(kAttnThreads)
+__global__ void __launch_bounds__(kAttnThreads, 4)
 int4_attn_kernel(Int4AttnParams p) {
   chain_link();
   using Tile = Int4Tile<H>;
@@ -237,178 +267,199 @@ int4_attn_kernel(Int4AttnParams p) {
   const int hi = min(tiles, (split + 1) * per_split);
   const int* table = p.page_table + static_cast<int64_t>(b) * p.max_pages;
 
-  // Row of the pools of key `lane` of a tile, -1 beyond the sequence.
-  auto slot_of = [&](int tile) -> int64_t {
+  // Row of the pools of key `lane` of a tile, kNone beyond the sequence (the launcher keeps rows below it).
+  constexpr uint32_t kNone = 0xffffffffu;
+  auto slot_of = [&](int tile) -> uint32_t {
     const int t = tile * kAttnKeys + lane;
-    if (tile >= hi || t >= len) return -1;
-    const int col = t / p.page_size, page = table[col];
-    if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_pages)) {
+    if (tile >= hi || t >= len) return kNone;
+    const int col = p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size;
+    const uint32_t page = static_cast<uint32_t>(table[col]);
+    if (page >= static_cast<uint32_t>(p.num_pages)) {
       int4_report(p.status);
-      return -1;
+      return kNone;
     }
-    return (static_cast<int64_t>(page) * p.num_kv_heads + kvh) * p.page_size + (t - col * p.page_size);
+    return (page * p.num_kv_heads + kvh) * p.page_size + (t - col * p.page_size);
   };
   uint8_t* ring = s_ring + warp * kAttnStages * Tile::kBytes;
-  auto load_tile = [&](int stage, int64_t slot) {
-    const uint32_t dst = sptr(ring) + stage * Tile::kBytes;
-    constexpr int kUnits = Tile::kRow / 16, kKeys = 32 / kUnits;  // keys an instruction
+  constexpr int kUnits = Tile::kRow / 16, kKeys = 32 / kUnits;  // 16-byte units of a row, keys an instruction
+  const uint32_t k_dst = sptr(ring) + Tile::kK + lane * 16;
+  const uint32_t v_dst = sptr(ring) + Tile::kV + Tile::v_unit(lane / kUnits, lane % kUnits);
+  const uint32_t pair_dst = sptr(ring) + Tile::kKPairs + lane * Tile::kPairs;
+  const uint8_t* k_src = p.k_pool.codes + lane % kUnits * 16;
+  const uint8_t* v_src = p.v_pool.codes + lane % kUnits * 16;
+  auto load_tile = [&](int stage, uint32_t slot) {
+    const uint32_t at_stage = stage * Tile::kBytes;
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
-      const int key = i * kKeys + lane / kUnits, u = lane % kUnits;
-      const int64_t at = __shfl_sync(0xffffffffu, slot, key);
-      const int64_t off = (at < 0 ? 0 : at) * Tile::kRow + u * 16;
-      cp_async16(dst + Tile::kK + key * Tile::kRow + u * 16, p.k_pool.codes + off, at >= 0);
-      cp_async16(dst + Tile::kV + Tile::v_unit(key, u), p.v_pool.codes + off, at >= 0);
+      const uint32_t at = __shfl_sync(0xffffffffu, slot, i * kKeys + lane / kUnits);
+      const bool ok = at != kNone;
+      const uint64_t off = ok ? static_cast<uint64_t>(at) * Tile::kRow : 0;
+      cp_async16(k_dst + at_stage + i * 512, k_src + off, ok);
+      cp_async16(v_dst + at_stage + i * 512, v_src + off, ok);
     }
-    const int64_t off = (slot < 0 ? 0 : slot) * G;
-    const uint32_t kd = dst + Tile::kKPairs + lane * Tile::kPairs, vd = dst + Tile::kVPairs + lane * Tile::kPairs;
+    const bool ok = slot != kNone;
+    const uint64_t off = ok ? static_cast<uint64_t>(slot) * G : 0;
     if constexpr (G == 4) {
-      cp_async16(kd, p.k_pool.pairs + off, slot >= 0);
-      cp_async16(vd, p.v_pool.pairs + off, slot >= 0);
+      cp_async16(pair_dst + at_stage, p.k_pool.pairs + off, ok);
+      cp_async16(pair_dst + at_stage + kAttnKeys * Tile::kPairs, p.v_pool.pairs + off, ok);
     } else {
-      cp_async8(kd, p.k_pool.pairs + off, slot >= 0);
-      cp_async8(vd, p.v_pool.pairs + off, slot >= 0);
+      cp_async8(pair_dst + at_stage, p.k_pool.pairs + off, ok);
+      cp_async8(pair_dst + at_stage + kAttnKeys * Tile::kPairs, p.v_pool.pairs + off, ok);
     }
   };
   int tile = split * per_split + warp;
 #pragma unroll
   for (int i = 0; i < kAttnStages; ++i) {
-    const int64_t slot = slot_of(tile + i * kAttnWarps);
+    const uint32_t slot = slot_of(tile + i * kAttnWarps);
     if (tile + i * kAttnWarps < hi) load_tile(i, slot);
     cp_commit();
   }
-  int64_t slot = slot_of(tile + kAttnStages * kAttnWarps);
+  uint32_t slot = slot_of(tile + kAttnStages * kAttnWarps);
 
-  // Q in the order of K's codes: MMA i of group g takes dims 8c + 2i, 8c + 2i + 4 and the two behind them.
-  uint32_t qa[2 * G][2];
-  float qs[G];
+  // Q of head r in the order of K's codes: MMA i of group g takes dims 8c + 2i, 8c + 2i + 4 and the two behind them, whose
+  // codes are 16 times as large.
+  uint32_t qb[2 * G][2];
+  float qs[G][2];  // sums of heads 2c, 2c + 1
+  const __nv_bfloat162 even = __float2bfloat162_rn(kInt4Scale), odd = __float2bfloat162_rn(kInt4Scale / 16.f);
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     uint4 x = make_uint4(0, 0, 0, 0);
     if (r < rows)
       x = *reinterpret_cast<const uint4*>(p.q + (static_cast<int64_t>(b) * p.num_q_heads + qh0 + r) * H + g * 32 + c * 8);
-    qa[2 * g][0] = __byte_perm(x.x, x.z, 0x5410);
-    qa[2 * g][1] = __byte_perm(x.x, x.z, 0x7632);
-    qa[2 * g + 1][0] = __byte_perm(x.y, x.w, 0x5410);
-    qa[2 * g + 1][1] = __byte_perm(x.y, x.w, 0x7632);
     const float2 f0 = unpack2(x.x), f1 = unpack2(x.y), f2 = unpack2(x.z), f3 = unpack2(x.w);
     float sum = ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    qs[g] = sum;
+    qs[g][0] = __shfl_sync(0xffffffffu, sum, 8 * c) * (1.f / kInt4Back);
+    qs[g][1] = __shfl_sync(0xffffffffu, sum, 8 * c + 4) * (1.f / kInt4Back);
+    qb[2 * g][0] = times(__byte_perm(x.x, x.z, 0x5410), even);
+    qb[2 * g][1] = times(__byte_perm(x.x, x.z, 0x7632), odd);
+    qb[2 * g + 1][0] = times(__byte_perm(x.y, x.w, 0x5410), even);
+    qb[2 * g + 1][1] = times(__byte_perm(x.y, x.w, 0x7632), odd);
   }
 
-  float m = -INFINITY, l = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // heads 2c, 2c + 1; l: this lane's keys
+  const float slack = kSlack / p.scale_log2;
   float acc[2 * G][4];  // [group, half][dim 32 g + 4 r + 2 half (+ 1: entries 2, 3)][columns 2c, 2c + 1]
-  float acc_m[G];       // sums of p m of head r, this lane's keys
+  float acc_m[G][2];    // sums of p m of this lane's keys
 #pragma unroll
   for (int i = 0; i < 2 * G; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
 #pragma unroll
-  for (int g = 0; g < G; ++g) acc_m[g] = 0.f;
+  for (int g = 0; g < G; ++g) acc_m[g][0] = acc_m[g][1] = 0.f;
+  const float zero[4] = {0.f, 0.f, 0.f, 0.f};
 
   int stage = 0;
   for (; tile < hi; tile += kAttnWarps) {
     cp_wait_group<kAttnStages - 1>();
     __syncwarp();
     const uint8_t* st = ring + stage * Tile::kBytes;
-    float s[8];
+    float s[4][2];  // keys 8 i + r, heads 2c, 2c + 1
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      uint32_t w[G], pairs[2][G];
-      const uint8_t* kr = st + Tile::kK + (n * 8 + r) * Tile::kRow + c * (Tile::kRow / 4);
-      const uint8_t* pr = st + Tile::kKPairs + (n * 8 + 2 * c) * Tile::kPairs;
-      if constexpr (G == 4) {
-        *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(kr);
-        *reinterpret_cast<uint4*>(pairs[0]) = *reinterpret_cast<const uint4*>(pr);
-        *reinterpret_cast<uint4*>(pairs[1]) = *reinterpret_cast<const uint4*>(pr + 16);
-      } else {
-        *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(kr);
-        *reinterpret_cast<uint2*>(pairs[0]) = *reinterpret_cast<const uint2*>(pr);
-        *reinterpret_cast<uint2*>(pairs[1]) = *reinterpret_cast<const uint2*>(pr + 8);
+    for (int n = 0; n < 2; ++n) {
+      uint32_t w[2][G], pairs[2][G];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int key = (2 * n + i) * 8 + r;
+        load_words<G>(w[i], st + Tile::kK + key * Tile::kRow + c * (Tile::kRow / 4));
+        load_words<G>(pairs[i], st + Tile::kKPairs + key * Tile::kPairs);
+        s[2 * n + i][0] = s[2 * n + i][1] = 0.f;
       }
-      float s0 = 0.f, s1 = 0.f;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        const uint32_t x = __byte_perm(w[g >> 1], w[G / 2 + (g >> 1)], g & 1 ? 0x7632 : 0x5410);
-        float part[4] = {-128.f * qs[g], -128.f * qs[g], 0.f, 0.f};
-        const uint32_t a0[4] = {qa[2 * g][0], 0u, qa[2 * g][1], 0u}, a1[4] = {qa[2 * g + 1][0], 0u, qa[2 * g + 1][1], 0u};
-        mma(part, a0, int4_pair(x, 0), int4_pair(x, 1));
-        mma(part, a1, int4_pair(x, 2), int4_pair(x, 3));
-        s0 += pair_s(pairs[0][g]) * part[0] + pair_m(pairs[0][g]) * qs[g];
-        s1 += pair_s(pairs[1][g]) * part[1] + pair_m(pairs[1][g]) * qs[g];
+        uint32_t x[2], y[2];  // dims 8c, + 1, + 4, + 5 and the two behind each pair
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          x[i] = __byte_perm(w[i][g >> 1], w[i][G / 2 + (g >> 1)], g & 1 ? 0x7632 : 0x5410);
+          y[i] = __byte_perm(w[i][g >> 1], w[i][G / 2 + (g >> 1)], g & 1 ? 0x7733 : 0x5511);
+        }
+        float d[4];
+        const uint32_t a0[4] = {int4_low(x[0]), int4_low(x[1]), int4_high(x[0]), int4_high(x[1])};
+        const uint32_t a1[4] = {int4_low(y[0]), int4_low(y[1]), int4_high(y[0]), int4_high(y[1])};
+        mma_add(d, a0, qb[2 * g][0], qb[2 * g][1], zero);
+        mma_add(d, a1, qb[2 * g + 1][0], qb[2 * g + 1][1], d);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float ps = pair_s(pairs[i][g]), pm = pair_m(pairs[i][g]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) s[2 * n + i][h] = fmaf(ps, d[2 * i + h], fmaf(pm, qs[g][h], s[2 * n + i][h]));
+        }
       }
-      s[2 * n] = s0 * p.scale_log2;
-      s[2 * n + 1] = s1 * p.scale_log2;
     }
     if ((tile + 1) * kAttnKeys > len) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (tile * kAttnKeys + (i >> 1) * 8 + 2 * c + (i & 1) >= len) s[i] = -INFINITY;
+      for (int i = 0; i < 4; ++i)
+        if (tile * kAttnKeys + i * 8 + r >= len) s[i][0] = s[i][1] = -INFINITY;
     }
-    float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const float m_new = fmaxf(m, top);
-    if (__any_sync(0xffffffffu, m_new != m)) {
-      const float corr = m_new == -INFINITY ? 1.f : exp2f(m - m_new);
-      l *= corr;
+    float top[2];
 #pragma unroll
-      for (int g = 0; g < G; ++g) acc_m[g] *= corr;
-      const float c0 = __shfl_sync(0xffffffffu, corr, 8 * c), c1 = __shfl_sync(0xffffffffu, corr, 8 * c + 4);
+    for (int h = 0; h < 2; ++h) top[h] = fmaxf(fmaxf(s[0][h], s[1][h]), fmaxf(s[2][h], s[3][h]));
+    if (__any_sync(0xffffffffu, top[0] > m[0] + slack || top[1] > m[1] + slack)) {
+      float corr[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int off = 4; off <= 16; off <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], off));
+        const float m_new = fmaxf(m[h], top[h]);
+        corr[h] = m[h] == -INFINITY ? 0.f : ex2((m[h] - m_new) * p.scale_log2);  // (nothing is there yet)
+        m[h] = m_new;
+        l[h] *= corr[h];
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) acc_m[g][0] *= corr[0], acc_m[g][1] *= corr[1];
 #pragma unroll
       for (int i = 0; i < 2 * G; ++i) {
-        acc[i][0] *= c0;
-        acc[i][1] *= c1;
-        acc[i][2] *= c0;
-        acc[i][3] *= c1;
+        acc[i][0] *= corr[0];
+        acc[i][1] *= corr[1];
+        acc[i][2] *= corr[0];
+        acc[i][3] *= corr[1];
       }
-      m = m_new;
     }
-    // A row of -inf alone keeps zeros; NaN stays.
-    const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      s[i] = exp2f(s[i] - base);
-      l += s[i];
+    for (int h = 0; h < 2; ++h) {
+      // (a row of -inf alone keeps zeros; NaN stays)
+      const float base = m[h] == -INFINITY ? 0.f : fmaf(-m[h], p.scale_log2, kInt4Shift);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[i][h] = ex2(fmaf(s[i][h], p.scale_log2, base));
+        l[h] += s[i][h];
+      }
     }
-    // Keys 16 j + 2c, + 1, + 8, + 9 are the columns of P that this lane holds: s[4 j .. 4 j + 3].
-    uint32_t w[8][G / 2];
+    uint32_t pairs[4][G];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) load_words<G>(pairs[i], st + Tile::kVPairs + (i * 8 + r) * Tile::kPairs);
+    uint32_t w[8][G / 2];  // keys 8 i + 2c, + 1
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int key = (i >> 1) * 8 + 2 * c + (i & 1);
-      if constexpr (G == 4) {
-        *reinterpret_cast<uint2*>(w[i]) =
-            *reinterpret_cast<const uint2*>(st + Tile::kV + Tile::v_unit(key, r >> 1) + (r & 1) * 8);
-      } else {
+      if constexpr (G == 4)
+        load_words<2>(w[i], st + Tile::kV + Tile::v_unit(key, r >> 1) + (r & 1) * 8);
+      else
         w[i][0] = *reinterpret_cast<const uint32_t*>(st + Tile::kV + Tile::v_unit(key, r >> 2) + (r & 3) * 4);
-      }
     }
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       uint32_t pb[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint8_t* pr = st + Tile::kVPairs + (i * 8 + 2 * c) * Tile::kPairs + g * 4;
-        const uint32_t u0 = *reinterpret_cast<const uint32_t*>(pr), u1 = *reinterpret_cast<const uint32_t*>(pr + Tile::kPairs);
-        pb[i] = pack2(s[2 * i] * pair_s(u0), s[2 * i + 1] * pair_s(u1));
-        acc_m[g] += s[2 * i] * pair_m(u0) + s[2 * i + 1] * pair_m(u1);
+        const float ps = pair_s(pairs[i][g]), pm = pair_m(pairs[i][g]);
+        pb[i] = turned_round(pack2(s[i][0] * ps, s[i][1] * ps));
+        acc_m[g][0] = fmaf(s[i][0], pm, acc_m[g][0]);
+        acc_m[g][1] = fmaf(s[i][1], pm, acc_m[g][1]);
       }
-      const uint32_t less[4] = {0xc300c300u, 0xc300c300u, 0xc300c300u, 0xc300c300u};  // -128
-      float off[4] = {0.f, 0.f, 0.f, 0.f};
-      mma(off, less, pb[0], pb[1]);
-      mma(off, less, pb[2], pb[3]);
-      uint32_t x[4];
+      uint32_t x[4], y[4];  // dims 4r, 4r + 1 and the two behind them of keys 8 i + 2c, + 1
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = __byte_perm(w[2 * i][g >> 1], w[2 * i + 1][g >> 1], g & 1 ? 0x7632 : 0x5410);
+      for (int i = 0; i < 4; ++i) {
+        x[i] = __byte_perm(w[2 * i][g >> 1], w[2 * i + 1][g >> 1], g & 1 ? 0x7632 : 0x5410);
+        y[i] = __byte_perm(w[2 * i][g >> 1], w[2 * i + 1][g >> 1], g & 1 ? 0x7733 : 0x5511);
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float o[4] = {off[0], off[1], off[2], off[3]};
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t a[4] = {int4_pair(x[2 * j], 2 * h), int4_pair(x[2 * j], 2 * h + 1), int4_pair(x[2 * j + 1], 2 * h),
-                                 int4_pair(x[2 * j + 1], 2 * h + 1)};
-          mma(o, a, pb[2 * j], pb[2 * j + 1]);
-        }
+        float o[4];
+        const uint32_t(&u)[4] = h ? y : x;
+        const uint32_t a0[4] = {int4_low(u[0]), int4_high(u[0]), int4_low(u[1]), int4_high(u[1])};
+        const uint32_t a1[4] = {int4_low(u[2]), int4_high(u[2]), int4_low(u[3]), int4_high(u[3])};
+        mma_add(o, a0, pb[0], pb[1], zero);
+        mma_add(o, a1, pb[2], pb[3], o);
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[2 * g + h][i] += o[i];
       }
@@ -421,30 +472,33 @@ int4_attn_kernel(Int4AttnParams p) {
   }
   cp_wait_all();
   __syncthreads();  // the merge buffers overlay the tiles
-  l += __shfl_xor_sync(0xffffffffu, l, 1);
-  l += __shfl_xor_sync(0xffffffffu, l, 2);
+#pragma unroll
+  for (int off = 4; off <= 16; off <<= 1) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], off);
+#pragma unroll
+      for (int g = 0; g < G; ++g) acc_m[g][h] += __shfl_xor_sync(0xffffffffu, acc_m[g][h], off);
+    }
+  }
   float* s_part = reinterpret_cast<float*>(s_ring);  // 4 warps and the CTA: [rows][H] sums, then maxima, then weights
   const int per_warp = rows * H;
   float* s_m = s_part + (kAttnWarps + 1) * per_warp;
   float* s_l = s_m + (kAttnWarps + 1) * rows;
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    acc_m[g] += __shfl_xor_sync(0xffffffffu, acc_m[g], 1);
-    acc_m[g] += __shfl_xor_sync(0xffffffffu, acc_m[g], 2);
+  for (int n = 0; n < 2; ++n) {
+    if (2 * c + n >= rows) break;
+    float* dst = s_part + warp * per_warp + (2 * c + n) * H + r * 4;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const float add = __shfl_sync(0xffffffffu, acc_m[g], 8 * c + 4 * n);
-      if (2 * c + n < rows) {
-        float* dst = s_part + warp * per_warp + (2 * c + n) * H + g * 32 + r * 4;
+    for (int g = 0; g < G; ++g)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          *reinterpret_cast<float2*>(dst + 2 * h) = make_float2(acc[2 * g + h][n] + add, acc[2 * g + h][2 + n] + add);
-      }
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<float2*>(dst + g * 32 + 2 * h) =
+            make_float2(fmaf(acc[2 * g + h][n], kInt4Back, acc_m[g][n] * (1.f / kInt4Scale)), fmaf(acc[2 * g + h][2 + n], kInt4Back / 16.f, acc_m[g][n] * (1.f / kInt4Scale)));
+    if (r == 0) {
+      s_m[warp * rows + 2 * c + n] = m[n] * p.scale_log2;
+      s_l[warp * rows + 2 * c + n] = l[n] * (1.f / kInt4Scale);
     }
-  }
-  if (r < rows && c == 0) {
-    s_m[warp * rows + r] = m;
-    s_l[warp * rows + r] = l;
   }
   __syncthreads();
   // Thread (g, d) of H threads a head owns output dim d.
@@ -612,7 +666,8 @@ extern "C" int axb_int4_decode_attn(const void* q, void* k_codes, void* k_pairs,
                                     int num_pages, int splits, float softmax_scale, int* status, cudaStream_t stream) {
   using namespace axb;
   if ((head_dim != 64 && head_dim != 128) || page_size < 1 || num_kv_heads < 1 || num_q_heads < 1 ||
-      num_q_heads % num_kv_heads || splits < 1 || B < 0 || B > 65535)
+      num_q_heads % num_kv_heads || splits < 1 || B < 0 || B > 65535 || !(softmax_scale > 0.f && softmax_scale < 1048576.f) ||
+      static_cast<int64_t>(num_pages) * num_kv_heads * page_size >= 0xffffffffll)
     return -10;
   if (!aligned16(q) || !aligned16(k_codes) || !aligned16(k_pairs) || !aligned16(v_codes) || !aligned16(v_pairs)) return -10;
   if (splits > kAttnCluster && scratch == nullptr) return -10;
@@ -629,6 +684,9 @@ extern "C" int axb_int4_decode_attn(const void* q, void* k_codes, void* k_pairs,
   p.status = status;
   p.num_q_heads = num_q_heads, p.num_kv_heads = num_kv_heads, p.page_size = page_size;
   p.max_pages = max_pages, p.num_pages = num_pages, p.splits = splits;
-  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (page_size == 1 << i) p.page_shift = i;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f * kInt4Back;
   return head_dim == 128 ? int4_attn<128>(p, B, stream) : int4_attn<64>(p, B, stream);
 }

@@ -22,6 +22,12 @@
 
 namespace axb {
 
+__device__ __forceinline__ uint32_t int4_pair(uint32_t x, int i) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xEA;" : "=r"(y) : "r"(x >> (4 * i)));
+  return y;
+}
+
 struct Int4LinearParams {
   const __nv_bfloat16* x;  // [M, ldx]
   const uint4* codes;

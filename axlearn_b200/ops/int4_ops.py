@@ -372,6 +372,8 @@ def paged_decode_attention_int4(q: Tensor, k_pages: Int4Pages, v_pages: Int4Page
     if page_table.shape[0] != b:
         raise ValueError(f"a page table of {page_table.shape[0]} rows for {b} sequences")
     scale = 1.0 / math.sqrt(h) if softmax_scale is None else softmax_scale
+    if not 0 < scale < 2 ** 20:
+        raise ValueError(f"softmax_scale {scale} is not in (0, 2^20)")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != device or not out.is_contiguous()):
         raise ValueError(f"out {tuple(out.shape)} {out.dtype}: contiguous {tuple(q.shape)} {q.dtype} is wanted")
     if not _on_kernel(q):
