@@ -184,7 +184,7 @@ constexpr int kAttnCluster = 8;
 template <int H>
 struct Int4Tile {
   static constexpr int kGroups = H / kInt4Group;
-  static constexpr int kRow = H / 2, kPairs = kGroups * 4;        // bytes of a key's codes and pairs
+  static constexpr int kRow = H / 2, kPairs = 16;                 // bytes of a key's codes and pairs (8 of 16 where H is 64)
   static constexpr int kK = 0, kV = kAttnKeys * kRow, kKPairs = 2 * kV, kVPairs = kKPairs + kAttnKeys * kPairs;
   static constexpr int kBytes = kVPairs + kAttnKeys * kPairs;
   static constexpr int kSmem(int rows) {
@@ -217,6 +217,17 @@ __device__ __forceinline__ uint32_t times(uint32_t x, __nv_bfloat162 f) {
   return reinterpret_cast<const uint32_t&>(y);
 }
 
+// Three bf16 terms each that add up to (x, y): 24 bits of mantissa, cut off from the top.
+__device__ __forceinline__ void split_terms(float x, float y, uint32_t (&t)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    const uint32_t ux = __float_as_uint(x), uy = __float_as_uint(y);
+    t[i] = __byte_perm(ux, uy, 0x7632);
+    x -= __uint_as_float(ux & 0xffff0000u);
+    y -= __uint_as_float(uy & 0xffff0000u);
+  }
+}
+
 // An 8 x 8 tile of bf16 pairs, lane (r, c) with entries (r, 2c), (r, 2c + 1): its transpose in the same layout.
 __device__ __forceinline__ uint32_t turned_round(uint32_t x) {
   uint32_t y;
@@ -233,8 +244,11 @@ __device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, bool ok
 
 // S^T = K Q^T: 16 keys are the rows of the m16n8k16 tile, the query heads its columns; a lane takes dims 8c .. 8c + 7 of each
 // group of a key, and the sums of a group are multiplied by its s: k.q = sum_g s_g (sum c q) + m_g sum q.
-// O^T = V^T P^T: 16 dims of one group are the rows, the heads the columns; s of a key's group is multiplied into P, which is
-// rounded to bf16 (2^-9 of a probability, the sums of p m stay in 32 bits) and turned round by `movmatrix`.
+// sum_g m_g sum q is one product of its own: the sums of q are three bf16 terms that add up to their 32 bits.
+// O^T = V^T P^T: 16 dims of one group are the rows, the heads the columns.  P is rounded to bf16 as the operand of all
+// products, as in the prompts' kernels, turned round by `movmatrix`, and multiplied by s of a key's group, which rounds again;
+// sum p m is one product of its own with the pairs' transpose.  Two roundings of half a step, 2^-8 of a probability each;
+// against 64 bits an output is off by 0.0019 of itself (2-norm), 0.0017 of it the output's own rounding.
 // Codes enter as denormal bf16 numbers (`int4.cuh`): scores carry 1 / kInt4Back until the exponential, probabilities and the
 // sums of them alone kInt4Scale, and the sums of p c 1 / kInt4Back.
 // The maximum that probabilities are relative to moves only when a score passes it by kSlack (a factor of 2^kSlack).
@@ -267,18 +281,22 @@ int4_attn_kernel(Int4AttnParams p) {
   const int hi = min(tiles, (split + 1) * per_split);
   const int* table = p.page_table + static_cast<int64_t>(b) * p.max_pages;
 
-  // Row of the pools of key `lane` of a tile, kNone beyond the sequence (the launcher keeps rows below it).
+  // Key `lane` of a tile: its page, asked for long before `row_of` makes it the row of the pools; kNone beyond the sequence
+  // (the launcher keeps rows below it).
   constexpr uint32_t kNone = 0xffffffffu;
-  auto slot_of = [&](int tile) -> uint32_t {
+  auto col_of = [&](int t) { return p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size; };
+  auto page_of = [&](int tile) -> uint32_t {
+    const int t = tile * kAttnKeys + lane;
+    return tile < hi && t < len ? static_cast<uint32_t>(table[col_of(t)]) : 0u;
+  };
+  auto row_of = [&](int tile, uint32_t page) -> uint32_t {
     const int t = tile * kAttnKeys + lane;
     if (tile >= hi || t >= len) return kNone;
-    const int col = p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size;
-    const uint32_t page = static_cast<uint32_t>(table[col]);
     if (page >= static_cast<uint32_t>(p.num_pages)) {
       int4_report(p.status);
       return kNone;
     }
-    return (page * p.num_kv_heads + kvh) * p.page_size + (t - col * p.page_size);
+    return (page * p.num_kv_heads + kvh) * p.page_size + (t - col_of(t) * p.page_size);
   };
   uint8_t* ring = s_ring + warp * kAttnStages * Tile::kBytes;
   constexpr int kUnits = Tile::kRow / 16, kKeys = 32 / kUnits;  // 16-byte units of a row, keys an instruction
@@ -308,18 +326,20 @@ int4_attn_kernel(Int4AttnParams p) {
     }
   };
   int tile = split * per_split + warp;
+  uint32_t pages[kAttnStages + 1];
+#pragma unroll
+  for (int i = 0; i <= kAttnStages; ++i) pages[i] = page_of(tile + i * kAttnWarps);
 #pragma unroll
   for (int i = 0; i < kAttnStages; ++i) {
-    const uint32_t slot = slot_of(tile + i * kAttnWarps);
-    if (tile + i * kAttnWarps < hi) load_tile(i, slot);
+    if (tile + i * kAttnWarps < hi) load_tile(i, row_of(tile + i * kAttnWarps, pages[i]));
     cp_commit();
   }
-  uint32_t slot = slot_of(tile + kAttnStages * kAttnWarps);
+  uint32_t page = pages[kAttnStages];
 
   // Q of head r in the order of K's codes: MMA i of group g takes dims 8c + 2i, 8c + 2i + 4 and the two behind them, whose
   // codes are 16 times as large.
   uint32_t qb[2 * G][2];
-  float qs[G][2];  // sums of heads 2c, 2c + 1
+  float sums[G];
   const __nv_bfloat162 even = __float2bfloat162_rn(kInt4Scale), odd = __float2bfloat162_rn(kInt4Scale / 16.f);
 #pragma unroll
   for (int g = 0; g < G; ++g) {
@@ -330,22 +350,39 @@ int4_attn_kernel(Int4AttnParams p) {
     float sum = ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    qs[g][0] = __shfl_sync(0xffffffffu, sum, 8 * c) * (1.f / kInt4Back);
-    qs[g][1] = __shfl_sync(0xffffffffu, sum, 8 * c + 4) * (1.f / kInt4Back);
+    sums[g] = sum * (1.f / kInt4Back);
     qb[2 * g][0] = times(__byte_perm(x.x, x.z, 0x5410), even);
     qb[2 * g][1] = times(__byte_perm(x.x, x.z, 0x7632), odd);
     qb[2 * g + 1][0] = times(__byte_perm(x.y, x.w, 0x5410), even);
     qb[2 * g + 1][1] = times(__byte_perm(x.y, x.w, 0x7632), odd);
   }
 
+  // Column k of that product is term k / G of the sum of group k % G, for two neighbours k = 2c and two k = 8 + 2c.
+  uint32_t qm[2];
+  {
+    uint32_t terms[3][G / 2];
+#pragma unroll
+    for (int g = 0; g < G; g += 2) {
+      uint32_t t[3];
+      split_terms(sums[g], sums[g + 1], t);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) terms[i][g / 2] = t[i];
+    }
+    if constexpr (G == 4) {
+      qm[0] = c == 0 ? terms[0][0] : c == 1 ? terms[0][1] : c == 2 ? terms[1][0] : terms[1][1];
+      qm[1] = c == 0 ? terms[2][0] : c == 1 ? terms[2][1] : 0u;
+    } else {
+      qm[0] = c == 0 ? terms[0][0] : c == 1 ? terms[1][0] : c == 2 ? terms[2][0] : 0u;
+      qm[1] = 0u;
+    }
+  }
+
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // heads 2c, 2c + 1; l: this lane's keys
   const float slack = kSlack / p.scale_log2;
   float acc[2 * G][4];  // [group, half][dim 32 g + 4 r + 2 half (+ 1: entries 2, 3)][columns 2c, 2c + 1]
-  float acc_m[G][2];    // sums of p m of this lane's keys
+  float acc_m[4] = {};  // row 2 g + 1: sums of p m of group g
 #pragma unroll
   for (int i = 0; i < 2 * G; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-#pragma unroll
-  for (int g = 0; g < G; ++g) acc_m[g][0] = acc_m[g][1] = 0.f;
   const float zero[4] = {0.f, 0.f, 0.f, 0.f};
 
   int stage = 0;
@@ -356,14 +393,21 @@ int4_attn_kernel(Int4AttnParams p) {
     float s[4][2];  // keys 8 i + r, heads 2c, 2c + 1
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      uint32_t w[2][G], pairs[2][G];
+      uint32_t w[2][G], pairs[2][G], low[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int key = (2 * n + i) * 8 + r;
         load_words<G>(w[i], st + Tile::kK + key * Tile::kRow + c * (Tile::kRow / 4));
         load_words<G>(pairs[i], st + Tile::kKPairs + key * Tile::kPairs);
-        s[2 * n + i][0] = s[2 * n + i][1] = 0.f;
+        uint32_t two[2];  // of groups 2 (c % 2) and the next
+        load_words<2>(two, st + Tile::kKPairs + key * Tile::kPairs + (G == 4 ? (c & 1) * 8 : 0));
+        low[i] = __byte_perm(two[0], two[1], 0x7632);
       }
+      float dm[4];
+      const uint32_t am[4] = {low[0], low[1], low[0], low[1]};
+      mma_add(dm, am, qm[0], qm[1], zero);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[2 * n + (i >> 1)][i & 1] = dm[i];
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         uint32_t x[2], y[2];  // dims 8c, + 1, + 4, + 5 and the two behind each pair
@@ -379,9 +423,9 @@ int4_attn_kernel(Int4AttnParams p) {
         mma_add(d, a1, qb[2 * g + 1][0], qb[2 * g + 1][1], d);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float ps = pair_s(pairs[i][g]), pm = pair_m(pairs[i][g]);
+          const float ps = pair_s(pairs[i][g]);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) s[2 * n + i][h] = fmaf(ps, d[2 * i + h], fmaf(pm, qs[g][h], s[2 * n + i][h]));
+          for (int h = 0; h < 2; ++h) s[2 * n + i][h] = fmaf(ps, d[2 * i + h], s[2 * n + i][h]);
         }
       }
     }
@@ -404,8 +448,7 @@ int4_attn_kernel(Int4AttnParams p) {
         m[h] = m_new;
         l[h] *= corr[h];
       }
-#pragma unroll
-      for (int g = 0; g < G; ++g) acc_m[g][0] *= corr[0], acc_m[g][1] *= corr[1];
+      acc_m[0] *= corr[0], acc_m[1] *= corr[1];
 #pragma unroll
       for (int i = 0; i < 2 * G; ++i) {
         acc[i][0] *= corr[0];
@@ -424,9 +467,15 @@ int4_attn_kernel(Int4AttnParams p) {
         l[h] += s[i][h];
       }
     }
-    uint32_t pairs[4][G];
+    uint32_t pt[4], vt[4];  // rows: heads / entries of pairs; columns: keys 8 i + 2c, + 1
+    ldsm4t(vt, st + Tile::kVPairs + lane * Tile::kPairs);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load_words<G>(pairs[i], st + Tile::kVPairs + (i * 8 + r) * Tile::kPairs);
+    for (int i = 0; i < 4; ++i) pt[i] = turned_round(pack2(s[i][0], s[i][1]));
+    {
+      const uint32_t a0[4] = {vt[0], 0u, vt[1], 0u}, a1[4] = {vt[2], 0u, vt[3], 0u};
+      mma(acc_m, a0, pt[0], pt[1]);
+      mma(acc_m, a1, pt[2], pt[3]);
+    }
     uint32_t w[8][G / 2];  // keys 8 i + 2c, + 1
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -441,10 +490,8 @@ int4_attn_kernel(Int4AttnParams p) {
       uint32_t pb[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float ps = pair_s(pairs[i][g]), pm = pair_m(pairs[i][g]);
-        pb[i] = turned_round(pack2(s[i][0] * ps, s[i][1] * ps));
-        acc_m[g][0] = fmaf(s[i][0], pm, acc_m[g][0]);
-        acc_m[g][1] = fmaf(s[i][1], pm, acc_m[g][1]);
+        const uint32_t ps = __shfl_sync(0xffffffffu, vt[i], 8 * g + c);  // row 2 g
+        pb[i] = times(pt[i], reinterpret_cast<const __nv_bfloat162&>(ps));
       }
       uint32_t x[4], y[4];  // dims 4r, 4r + 1 and the two behind them of keys 8 i + 2c, + 1
 #pragma unroll
@@ -454,20 +501,17 @@ int4_attn_kernel(Int4AttnParams p) {
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float o[4];
         const uint32_t(&u)[4] = h ? y : x;
         const uint32_t a0[4] = {int4_low(u[0]), int4_high(u[0]), int4_low(u[1]), int4_high(u[1])};
         const uint32_t a1[4] = {int4_low(u[2]), int4_high(u[2]), int4_low(u[3]), int4_high(u[3])};
-        mma_add(o, a0, pb[0], pb[1], zero);
-        mma_add(o, a1, pb[2], pb[3], o);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[2 * g + h][i] += o[i];
+        mma(acc[2 * g + h], a0, pb[0], pb[1]);
+        mma(acc[2 * g + h], a1, pb[2], pb[3]);
       }
     }
     __syncwarp();  // the stage has been read
-    if (tile + kAttnStages * kAttnWarps < hi) load_tile(stage, slot);
+    if (tile + kAttnStages * kAttnWarps < hi) load_tile(stage, row_of(tile + kAttnStages * kAttnWarps, page));
     cp_commit();
-    slot = slot_of(tile + (kAttnStages + 1) * kAttnWarps);
+    page = page_of(tile + (kAttnStages + 1) * kAttnWarps);
     if (++stage == kAttnStages) stage = 0;
   }
   cp_wait_all();
@@ -475,11 +519,7 @@ int4_attn_kernel(Int4AttnParams p) {
 #pragma unroll
   for (int off = 4; off <= 16; off <<= 1) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], off);
-#pragma unroll
-      for (int g = 0; g < G; ++g) acc_m[g][h] += __shfl_xor_sync(0xffffffffu, acc_m[g][h], off);
-    }
+    for (int h = 0; h < 2; ++h) l[h] += __shfl_xor_sync(0xffffffffu, l[h], off);
   }
   float* s_part = reinterpret_cast<float*>(s_ring);  // 4 warps and the CTA: [rows][H] sums, then maxima, then weights
   const int per_warp = rows * H;
@@ -487,15 +527,17 @@ int4_attn_kernel(Int4AttnParams p) {
   float* s_l = s_m + (kAttnWarps + 1) * rows;
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
-    if (2 * c + n >= rows) break;
     float* dst = s_part + warp * per_warp + (2 * c + n) * H + r * 4;
 #pragma unroll
-    for (int g = 0; g < G; ++g)
+    for (int g = 0; g < G; ++g) {
+      const float low = __shfl_sync(0xffffffffu, acc_m[n], 8 * g + 4 + c) * (1.f / kInt4Scale);
+      if (2 * c + n >= rows) continue;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        *reinterpret_cast<float2*>(dst + g * 32 + 2 * h) =
-            make_float2(fmaf(acc[2 * g + h][n], kInt4Back, acc_m[g][n] * (1.f / kInt4Scale)), fmaf(acc[2 * g + h][2 + n], kInt4Back / 16.f, acc_m[g][n] * (1.f / kInt4Scale)));
-    if (r == 0) {
+        *reinterpret_cast<float2*>(dst + g * 32 + 2 * h) = make_float2(fmaf(acc[2 * g + h][n], kInt4Back, low),
+                                                                      fmaf(acc[2 * g + h][2 + n], kInt4Back / 16.f, low));
+    }
+    if (r == 0 && 2 * c + n < rows) {
       s_m[warp * rows + 2 * c + n] = m[n] * p.scale_log2;
       s_l[warp * rows + 2 * c + n] = l[n] * (1.f / kInt4Scale);
     }

@@ -334,11 +334,12 @@ def append_int4(k: Tensor, v: Tensor, k_pages: Int4Pages, v_pages: Int4Pages, pa
 
 
 def attention_splits(batch: int, num_kv_heads: int, group: int, max_len: int, sms: int = 148) -> int:
-    """KV splits of attention over the 4-bit cache: one wave of CTAs (two fit an SM; one takes a split, a KV head and eight
-    query heads), at least half a 32-token tile for each of a CTA's four warps."""
+    """KV splits of attention over the 4-bit cache: one wave of CTAs (four fit an SM; one takes a split, a KV head and eight
+    query heads), 64 tokens or more for each."""
     ctas = batch * num_kv_heads * ((group + 7) // 8)
-    splits = max(1, min(max_len // 64, 2 * sms // max(1, ctas)))
-    return min(splits, 8 if 16 * ctas > sms else 32)
+    splits = max(1, min(max_len // 64, 4 * sms // max(1, ctas)))
+    many = math.isqrt(max_len) // 4
+    return min(splits, many if many >= 16 else 8)
 
 
 def _attention_plain(q, k_pages, v_pages, page_table, lengths, scale):

@@ -57,10 +57,11 @@ def _attention64(q, k_pages, v_pages, table, lengths, scale):
         # A score is a sum of products with 128 + c (tensor cores cut sums off at 2^-23 of their largest term): some 12 steps.
         size = ks.abs() @ torch.tensor([143.0, 1.0], device="cuda", dtype=torch.float64)
         moved = 12 * 2.0 ** -23 * scale * (qg.abs().unflatten(-1, (-1, 32)).sum(-1) @ size.transpose(1, 2)).amax(-1, keepdim=True)
-        # A probability's factor s is rounded to bf16 (2^-8); sums with 128 + c of it; the output's rounding.
+        # A probability is rounded to bf16, its product with s again: p (m + s c) becomes p (1 + a) (m + s c (1 + b)) with a
+        # and b up to 2^-8, off by 2^-8 p |v| and (1 + 2^-8) 2^-8 p s c.  Sums in 32 bits; the output's rounding.
         low = vs[..., 1].repeat_interleave(32, -1)
         step = vs[..., 0].repeat_interleave(32, -1)
-        bound[i] = (2.0 ** -8 * (p @ (v - low)) + 8 * 2.0 ** -23 * 143 * (p @ step) + torch.expm1(2 * moved) * (p @ v.abs())
+        bound[i] = (2.0 ** -8 * (p @ v.abs() + 1.004 * (p @ (v - low))) + 8 * 2.0 ** -23 * 143 * (p @ step) + torch.expm1(2 * moved) * (p @ v.abs())
                     + 2.0 ** -20 * (p @ v.abs())).flatten(0, 1)
         bound[i] = 1.01 * bound[i] + 2.0 ** -8 * (out[i].abs() + bound[i])
     return out, bound
