@@ -17,9 +17,10 @@ constexpr int kInt4Group = 32;
 // as it is, then the first binade of the same spacing).  So the low nibble of each half is a code times 2^-133 as it lies,
 // the next one 16 times that: one logic operation for two codes, and no offset.  The other operand carries 2^kInt4Shift, so
 // that products stay far above the denormal numbers of fp32: results are 2^(kInt4Shift - 133) of the sums of codes.
-constexpr int kInt4Shift = 32;
-constexpr float kInt4Scale = 4294967296.f;                         // 2^kInt4Shift
-constexpr float kInt4Back = 2535301200456458802993406410752.f;    // 2^(133 - kInt4Shift)
+// 64 keeps both sides of fp32's range: x and p up to 2^63, and s and m times them up to 2^55, are no overflow.
+constexpr int kInt4Shift = 64;
+constexpr float kInt4Scale = 18446744073709551616.f;   // 2^kInt4Shift
+constexpr float kInt4Back = 590295810358705651712.f;   // 2^(133 - kInt4Shift)
 
 __device__ __forceinline__ uint32_t int4_low(uint32_t x) { return x & 0x000f000fu; }
 __device__ __forceinline__ uint32_t int4_high(uint32_t x) { return x & 0x00f000f0u; }  // 16 codes

@@ -28,15 +28,15 @@ struct HeadRows {
 
 struct Int4AppendParams {
   HeadRows q, k, v;
-  __nv_bfloat16 *q_out, *k_out, *v_out;  // where the rotated q and the values of k and v go, or null
-  int64_t qo_b, qo_t, qo_h, ko_b, ko_t, ko_h, vo_b, vo_t, vo_h;
+  __nv_bfloat16 *q_out, *k_out, *v_out;  // where the rotated q and the values of k and v go; null: not wanted
+  int64_t out_b, out_t, out_h;
   Int4Pool k_pool, v_pool;
   const int* page_table;
   const int* start;     // null: 0
   const int* live;      // null: all tokens
   const float2* angle;  // (sin, cos) of [position][H / 2], null: nothing is rotated
   int* status;
-  int start_offset, angle_rows;
+  int angle_rows;
   int B, T, num_q_heads, num_kv_heads, page_size, max_pages, num_pages;
 };
 
@@ -100,6 +100,8 @@ __device__ __forceinline__ uint4 rotate8(uint4 x, const float2* at) {
   return x;
 }
 
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
 constexpr int kAppendThreads = 256;
 
 // A row of H values (one head of one token) is H / 8 lanes of 16 bytes; rows run over heads (q, k, v), tokens, sequences.
@@ -117,7 +119,7 @@ int4_append_kernel(Int4AppendParams p) {
     const int64_t token = inside ? row / heads : 0;
     const int head = inside ? static_cast<int>(row - token * heads) : 0;
     const int b = static_cast<int>(token / p.T), t = static_cast<int>(token - static_cast<int64_t>(b) * p.T);
-    const int pos = (p.start == nullptr ? 0 : p.start[b]) + p.start_offset + t;
+    const int pos = (p.start == nullptr ? 0 : p.start[b]) + t;
     const bool live = inside && (p.live == nullptr || t < p.live[b]);
     const bool is_q = head < p.num_q_heads, is_v = head >= p.num_q_heads + p.num_kv_heads;
     const int kvh = is_v ? head - p.num_q_heads - p.num_kv_heads : head - p.num_q_heads;
@@ -136,14 +138,13 @@ int4_append_kernel(Int4AppendParams p) {
     const uint32_t word = row_word<H>(codes, lane, byte);
     if (!inside) continue;
     if (is_q) {
-      if (live) *reinterpret_cast<uint4*>(p.q_out + b * p.qo_b + t * p.qo_t + head * p.qo_h + lane * 8) = x;
+      if (live) *reinterpret_cast<uint4*>(p.q_out + b * p.out_b + t * p.out_t + head * p.out_h + lane * 8) = x;
       continue;
     }
     __nv_bfloat16* out = is_v ? p.v_out : p.k_out;
-    if (out != nullptr) {
-      const int64_t at = is_v ? b * p.vo_b + t * p.vo_t + kvh * p.vo_h : b * p.ko_b + t * p.ko_t + kvh * p.ko_h;
-      *reinterpret_cast<uint4*>(out + at + lane * 8) = live ? values8(codes, pair) : make_uint4(0, 0, 0, 0);
-    }
+    if (out != nullptr)
+      *reinterpret_cast<uint4*>(out + b * p.out_b + t * p.out_t + kvh * p.out_h + lane * 8) =
+          live ? values8(codes, pair) : make_uint4(0, 0, 0, 0);
     if (!live) continue;
     const int col = pos / p.page_size;
     if (pos < 0 || col >= p.max_pages) {
@@ -163,7 +164,8 @@ int4_append_kernel(Int4AppendParams p) {
 }
 
 struct Int4AttnParams {
-  const __nv_bfloat16* q;  // [B, Nq, H]
+  const __nv_bfloat16* q;  // [B, Nq, H]; kAppend: the packed projection [B, Nq + 2 Nkv, H] of the new token, not rotated
+  const float2* angle;     // kAppend: (sin, cos) of [position][H / 2]
   Int4Pool k_pool, v_pool;
   const int* page_table;
   const int* lengths;
@@ -172,6 +174,7 @@ struct Int4AttnParams {
   __nv_bfloat16* out;
   int* status;
   int num_q_heads, num_kv_heads, page_size, page_shift, max_pages, num_pages, splits;  // page_shift: -1 where no power of two
+  int angle_rows;
   float scale_log2;      // softmax scale * log2(e) * kInt4Back, > 0
 };
 
@@ -254,7 +257,11 @@ __device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, bool ok
 // The maximum that probabilities are relative to moves only when a score passes it by kSlack (a factor of 2^kSlack).
 constexpr float kSlack = 8.f;
 
-template <int H, bool kCluster>
+//
+// kAppend: a decoding step in one launch.  A warp turns its query heads in registers; the warp whose tile holds the new token
+// turns its key, quantises key and value, stores them in their page slot and puts them into the tile itself, so nobody reads
+// the slot.
+template <int H, bool kCluster, bool kAppend>
 __global__ void __launch_bounds__(kAttnThreads, 4)
 int4_attn_kernel(Int4AttnParams p) {
   chain_link();
@@ -274,7 +281,7 @@ int4_attn_kernel(Int4AttnParams p) {
   int len = p.lengths[b];
   if (len > p.max_pages * static_cast<int64_t>(p.page_size)) {
     if (threadIdx.x == 0) int4_report(p.status);
-    len = p.max_pages * p.page_size;
+    len = kAppend ? 0 : p.max_pages * p.page_size;  // a new token without a place: nothing is appended
   }
   const int tiles = (max(len, 0) + kAttnKeys - 1) / kAttnKeys;
   const int per_split = (tiles + p.splits - 1) / p.splits;
@@ -284,14 +291,15 @@ int4_attn_kernel(Int4AttnParams p) {
   // Key `lane` of a tile: its page, asked for long before `row_of` makes it the row of the pools; kNone beyond the sequence
   // (the launcher keeps rows below it).
   constexpr uint32_t kNone = 0xffffffffu;
+  const int cached = kAppend ? len - 1 : len;
   auto col_of = [&](int t) { return p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size; };
   auto page_of = [&](int tile) -> uint32_t {
     const int t = tile * kAttnKeys + lane;
-    return tile < hi && t < len ? static_cast<uint32_t>(table[col_of(t)]) : 0u;
+    return tile < hi && t < cached ? static_cast<uint32_t>(table[col_of(t)]) : 0u;
   };
   auto row_of = [&](int tile, uint32_t page) -> uint32_t {
     const int t = tile * kAttnKeys + lane;
-    if (tile >= hi || t >= len) return kNone;
+    if (tile >= hi || t >= cached) return kNone;
     if (page >= static_cast<uint32_t>(p.num_pages)) {
       int4_report(p.status);
       return kNone;
@@ -335,6 +343,37 @@ int4_attn_kernel(Int4AttnParams p) {
     cp_commit();
   }
   uint32_t page = pages[kAttnStages];
+  const int q_heads = kAppend ? p.num_q_heads + 2 * p.num_kv_heads : p.num_q_heads;  // of a row of q
+  const int pos = len - 1;
+  // The new token: lane l of the first H / 8 has dims 8 l .. 8 l + 7 of its key, the next H / 8 lanes its value.
+  const int new_tile = pos / kAttnKeys;
+  const bool appends = kAppend && len > 0 && new_tile >= split * per_split && new_tile < hi &&
+                       (new_tile - split * per_split) % kAttnWarps == warp;
+  const float2* angle = nullptr;
+  uint32_t new_word = 0, new_pair = 0;
+  int new_byte = 0;
+  constexpr int kRowLanes = H / 8;
+  if constexpr (kAppend) {
+    if (pos >= p.angle_rows && threadIdx.x == 0) int4_report(p.status);
+    angle = p.angle + static_cast<int64_t>(max(0, min(pos, p.angle_rows - 1))) * (H / 2);
+    if (appends) {
+      const int is_v = lane / kRowLanes & 1, l8 = lane % kRowLanes;
+      uint4 x = *reinterpret_cast<const uint4*>(
+          p.q + (static_cast<int64_t>(b) * q_heads + p.num_q_heads + is_v * p.num_kv_heads + kvh) * H + l8 * 8);
+      if (!is_v) x = rotate8(x, angle + l8 * 4);
+      new_word = row_word<H>(quantize8(x, new_pair), l8, new_byte);
+      const uint32_t to = static_cast<uint32_t>(table[col_of(pos)]);
+      if (to >= static_cast<uint32_t>(p.num_pages)) {
+        int4_report(p.status);
+      } else if (first == 0 && lane < 2 * kRowLanes) {  // (the other parts of a large group have the same)
+        const int64_t slot =
+            (static_cast<int64_t>(to) * p.num_kv_heads + kvh) * p.page_size + (pos - col_of(pos) * p.page_size);
+        const Int4Pool& pool = is_v ? p.v_pool : p.k_pool;
+        *reinterpret_cast<uint32_t*>(pool.codes + slot * (H / 2) + new_byte) = new_word;
+        if ((l8 & 3) == 0) pool.pairs[slot * G + (l8 >> 2)] = new_pair;
+      }
+    }
+  }
 
   // Q of head r in the order of K's codes: MMA i of group g takes dims 8c + 2i, 8c + 2i + 4 and the two behind them, whose
   // codes are 16 times as large.
@@ -345,7 +384,8 @@ int4_attn_kernel(Int4AttnParams p) {
   for (int g = 0; g < G; ++g) {
     uint4 x = make_uint4(0, 0, 0, 0);
     if (r < rows)
-      x = *reinterpret_cast<const uint4*>(p.q + (static_cast<int64_t>(b) * p.num_q_heads + qh0 + r) * H + g * 32 + c * 8);
+      x = *reinterpret_cast<const uint4*>(p.q + (static_cast<int64_t>(b) * q_heads + qh0 + r) * H + g * 32 + c * 8);
+    if constexpr (kAppend) x = rotate8(x, angle + g * 16 + c * 4);
     const float2 f0 = unpack2(x.x), f1 = unpack2(x.y), f2 = unpack2(x.z), f3 = unpack2(x.w);
     float sum = ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
@@ -389,7 +429,17 @@ int4_attn_kernel(Int4AttnParams p) {
   for (; tile < hi; tile += kAttnWarps) {
     cp_wait_group<kAttnStages - 1>();
     __syncwarp();
-    const uint8_t* st = ring + stage * Tile::kBytes;
+    uint8_t* st = ring + stage * Tile::kBytes;
+    if (appends && tile == new_tile) {
+      const int row = pos % kAttnKeys, is_v = lane / kRowLanes & 1, l8 = lane % kRowLanes;
+      if (lane < 2 * kRowLanes) {
+        const int at = is_v ? Tile::kV + Tile::v_unit(row, new_byte >> 4) + (new_byte & 15) : Tile::kK + row * Tile::kRow + new_byte;
+        *reinterpret_cast<uint32_t*>(st + at) = new_word;
+        if ((l8 & 3) == 0)
+          *reinterpret_cast<uint32_t*>(st + (is_v ? Tile::kVPairs : Tile::kKPairs) + row * Tile::kPairs + (l8 >> 2) * 4) = new_pair;
+      }
+      __syncwarp();
+    }
     float s[4][2];  // keys 8 i + r, heads 2c, 2c + 1
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
@@ -618,9 +668,9 @@ int4_combine_kernel(const float* part_out, const float* part_ml, __nv_bfloat16* 
   out[row * H + d] = __float2bfloat16(ll == 0.f ? 0.f : o / ll);
 }
 
-template <int H, bool kCluster>
+template <int H, bool kCluster, bool kAppend>
 static int launch_int4_attn(const Int4AttnParams& p, dim3 grid, int rows, cudaStream_t stream) {
-  constexpr auto kernel = int4_attn_kernel<H, kCluster>;
+  constexpr auto kernel = int4_attn_kernel<H, kCluster, kAppend>;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {grid.x, 1, 1};
@@ -635,59 +685,27 @@ static int launch_int4_attn(const Int4AttnParams& p, dim3 grid, int rows, cudaSt
   return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? 0 : -4;
 }
 
-template <int H>
+template <int H, bool kAppend>
 static int int4_attn(const Int4AttnParams& p, int B, cudaStream_t stream) {
   const int g = p.num_q_heads / p.num_kv_heads;
   const bool cluster = p.splits > 1 && p.splits <= kAttnCluster;
   const dim3 grid(p.splits, p.num_kv_heads * ((g + kAttnRows - 1) / kAttnRows), B);
   const int rows = g < kAttnRows ? g : kAttnRows;
-  const int rc = cluster ? launch_int4_attn<H, true>(p, grid, rows, stream) : launch_int4_attn<H, false>(p, grid, rows, stream);
+  const int rc = cluster ? launch_int4_attn<H, true, kAppend>(p, grid, rows, stream)
+                         : launch_int4_attn<H, false, kAppend>(p, grid, rows, stream);
   if (rc != 0) return rc;
   if (p.splits > kAttnCluster)
     launch_chained(int4_combine_kernel<H>, B * p.num_q_heads, H, 0, stream, p.part_out, p.part_ml, p.out, p.splits);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
-static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
 }  // namespace axb
 
-// `rows`: pointers q, k, v, q_out, k_out, v_out (null: not there), each with element strides of (sequence, token, head) in
-// `strides`.  -10: not supported.
-extern "C" int axb_int4_append(void* const* rows, const int64_t* strides, void* k_codes, void* k_pairs, void* v_codes,
-                               void* v_pairs, const int* page_table, const int* start, int start_offset, const int* live,
-                               const float* angle, int angle_rows, int B, int T, int num_q_heads, int num_kv_heads,
-                               int head_dim, int page_size, int max_pages, int num_pages, int* status,
-                               cudaStream_t stream) {
-  using namespace axb;
-  if ((head_dim != 64 && head_dim != 128) || page_size < 1 || num_kv_heads < 1 || num_q_heads < 0 || B < 0 || T < 0) return -10;
-  for (int i = 0; i < 6; ++i)
-    if (!aligned16(rows[i]) || (strides[3 * i] | strides[3 * i + 1] | strides[3 * i + 2]) % 8) return -10;
-  if (!aligned16(k_codes) || !aligned16(k_pairs) || !aligned16(v_codes) || !aligned16(v_pairs) || !aligned16(angle)) return -10;
-  if (B == 0 || T == 0) return 0;
-  Int4AppendParams p;
-  HeadRows* in[3] = {&p.q, &p.k, &p.v};
-  for (int i = 0; i < 3; ++i)
-    *in[i] = {static_cast<const __nv_bfloat16*>(rows[i]), strides[3 * i], strides[3 * i + 1], strides[3 * i + 2]};
-  p.q_out = static_cast<__nv_bfloat16*>(rows[3]);
-  p.k_out = static_cast<__nv_bfloat16*>(rows[4]);
-  p.v_out = static_cast<__nv_bfloat16*>(rows[5]);
-  p.qo_b = strides[9], p.qo_t = strides[10], p.qo_h = strides[11];
-  p.ko_b = strides[12], p.ko_t = strides[13], p.ko_h = strides[14];
-  p.vo_b = strides[15], p.vo_t = strides[16], p.vo_h = strides[17];
-  p.k_pool = {static_cast<uint8_t*>(k_codes), static_cast<uint32_t*>(k_pairs)};
-  p.v_pool = {static_cast<uint8_t*>(v_codes), static_cast<uint32_t*>(v_pairs)};
-  p.page_table = page_table;
-  p.start = start;
-  p.live = live;
-  p.angle = reinterpret_cast<const float2*>(angle);
-  p.status = status;
-  p.start_offset = start_offset;
-  p.angle_rows = angle_rows;
-  p.B = B, p.T = T, p.num_q_heads = num_q_heads, p.num_kv_heads = num_kv_heads;
-  p.page_size = page_size, p.max_pages = max_pages, p.num_pages = num_pages;
+namespace axb {
+
+static int int4_append(const Int4AppendParams& p, int head_dim, cudaStream_t stream) {
   const int64_t per_cta = kAppendThreads / (head_dim / 8);
-  int64_t ctas = (static_cast<int64_t>(B) * T * (num_q_heads + 2 * num_kv_heads) + per_cta - 1) / per_cta;
+  int64_t ctas = (static_cast<int64_t>(p.B) * p.T * (p.num_q_heads + 2 * p.num_kv_heads) + per_cta - 1) / per_cta;
   if (ctas > 148 * 32) ctas = 148 * 32;
   if (head_dim == 128)
     launch_chained(int4_append_kernel<128>, static_cast<unsigned>(ctas), kAppendThreads, 0, stream, p);
@@ -696,39 +714,110 @@ extern "C" int axb_int4_append(void* const* rows, const int64_t* strides, void* 
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
+}  // namespace axb
+
+// k and v [B, T, Nkv, H] with element strides of (sequence, token, head); k_out and v_out (null: not wanted) are contiguous.
+// -10: not supported.
+extern "C" int axb_int4_append(const void* k, const void* v, int64_t k_b, int64_t k_t, int64_t k_h, int64_t v_b, int64_t v_t,
+                               int64_t v_h, void* k_out, void* v_out, void* k_codes, void* k_pairs, void* v_codes,
+                               void* v_pairs, const int* page_table, const int* start, const int* live, int B, int T,
+                               int num_kv_heads, int head_dim, int page_size, int max_pages, int num_pages, int* status,
+                               cudaStream_t stream) {
+  using namespace axb;
+  if ((head_dim != 64 && head_dim != 128) || page_size < 1 || num_kv_heads < 1 || B < 0 || T < 0 ||
+      (k_b | k_t | k_h | v_b | v_t | v_h) % 8)
+    return -10;
+  for (const void* x : {k, v, static_cast<const void*>(k_out), static_cast<const void*>(v_out), static_cast<const void*>(k_codes),
+                        static_cast<const void*>(k_pairs), static_cast<const void*>(v_codes), static_cast<const void*>(v_pairs)})
+    if (!aligned16(x)) return -10;
+  if (B == 0 || T == 0) return 0;
+  Int4AppendParams p = {};
+  p.k = {static_cast<const __nv_bfloat16*>(k), k_b, k_t, k_h};
+  p.v = {static_cast<const __nv_bfloat16*>(v), v_b, v_t, v_h};
+  p.k_out = static_cast<__nv_bfloat16*>(k_out);
+  p.v_out = static_cast<__nv_bfloat16*>(v_out);
+  p.out_h = head_dim, p.out_t = static_cast<int64_t>(num_kv_heads) * head_dim, p.out_b = T * p.out_t;
+  p.k_pool = {static_cast<uint8_t*>(k_codes), static_cast<uint32_t*>(k_pairs)};
+  p.v_pool = {static_cast<uint8_t*>(v_codes), static_cast<uint32_t*>(v_pairs)};
+  p.page_table = page_table, p.start = start, p.live = live, p.status = status;
+  p.B = B, p.T = T, p.num_kv_heads = num_kv_heads;
+  p.page_size = page_size, p.max_pages = max_pages, p.num_pages = num_pages;
+  return int4_append(p, head_dim, stream);
+}
+
+// Whole prompts from position 0: qkv [B, T, (Nq + 2 Nkv) * H] of one projection.  Queries and keys are rotated by `angle`
+// ([position][H / 2] of (sin, cos), T positions or more), keys and values go to the cache, and what it then stands for
+// replaces them in qkv.
+extern "C" int axb_int4_append_prompt(void* qkv, void* k_codes, void* k_pairs, void* v_codes, void* v_pairs,
+                                      const int* page_table, const float* angle, int angle_rows, int B, int T,
+                                      int num_q_heads, int num_kv_heads, int head_dim, int page_size, int max_pages,
+                                      int num_pages, int* status, cudaStream_t stream) {
+  using namespace axb;
+  if ((head_dim != 64 && head_dim != 128) || page_size < 1 || num_kv_heads < 1 || num_q_heads < 1 || B < 0 || T < 0) return -10;
+  for (const void* x : {static_cast<const void*>(qkv), static_cast<const void*>(angle), static_cast<const void*>(k_codes),
+                        static_cast<const void*>(k_pairs), static_cast<const void*>(v_codes), static_cast<const void*>(v_pairs)})
+    if (!aligned16(x)) return -10;
+  if (B == 0 || T == 0) return 0;
+  Int4AppendParams p = {};
+  __nv_bfloat16* q = static_cast<__nv_bfloat16*>(qkv);
+  const int64_t t = static_cast<int64_t>(num_q_heads + 2 * num_kv_heads) * head_dim;
+  p.out_h = head_dim, p.out_t = t, p.out_b = T * t;
+  p.q_out = q;
+  p.k_out = q + num_q_heads * head_dim;
+  p.v_out = p.k_out + num_kv_heads * head_dim;
+  p.q = {p.q_out, p.out_b, t, head_dim};
+  p.k = {p.k_out, p.out_b, t, head_dim};
+  p.v = {p.v_out, p.out_b, t, head_dim};
+  p.k_pool = {static_cast<uint8_t*>(k_codes), static_cast<uint32_t*>(k_pairs)};
+  p.v_pool = {static_cast<uint8_t*>(v_codes), static_cast<uint32_t*>(v_pairs)};
+  p.page_table = page_table, p.status = status;
+  p.angle = reinterpret_cast<const float2*>(angle);
+  p.angle_rows = angle_rows;
+  p.B = B, p.T = T, p.num_q_heads = num_q_heads, p.num_kv_heads = num_kv_heads;
+  p.page_size = page_size, p.max_pages = max_pages, p.num_pages = num_pages;
+  return int4_append(p, head_dim, stream);
+}
+
 // Scratch of axb_int4_decode_attn in floats: up to a cluster's splits meet without any.
 extern "C" int64_t axb_int4_attn_scratch_floats(int B, int num_q_heads, int head_dim, int splits) {
   if (splits <= axb::kAttnCluster) return 0;
   return static_cast<int64_t>(B) * num_q_heads * splits * (head_dim + 2);
 }
 
+// One new token a sequence: q [B, Nq, H] over the cache; with `angle` ([position][H / 2] of (sin, cos)) q is the packed
+// projection [B, (Nq + 2 Nkv) * H] of the token at position lengths - 1, which is rotated and appended first.
 extern "C" int axb_int4_decode_attn(const void* q, void* k_codes, void* k_pairs, void* v_codes, void* v_pairs,
-                                    const int* page_table, const int* lengths, void* out, float* scratch, int B,
-                                    int num_q_heads, int num_kv_heads, int head_dim, int page_size, int max_pages,
-                                    int num_pages, int splits, float softmax_scale, int* status, cudaStream_t stream) {
+                                    const int* page_table, const int* lengths, const float* angle, void* out, float* scratch,
+                                    int angle_rows, int B, int num_q_heads, int num_kv_heads, int head_dim, int page_size,
+                                    int max_pages, int num_pages, int splits, float softmax_scale, int* status,
+                                    cudaStream_t stream) {
   using namespace axb;
   if ((head_dim != 64 && head_dim != 128) || page_size < 1 || num_kv_heads < 1 || num_q_heads < 1 ||
       num_q_heads % num_kv_heads || splits < 1 || B < 0 || B > 65535 || !(softmax_scale > 0.f && softmax_scale < 1048576.f) ||
-      static_cast<int64_t>(num_pages) * num_kv_heads * page_size >= 0xffffffffll)
+      static_cast<int64_t>(num_pages) * num_kv_heads * page_size >= 0xffffffffll || (angle != nullptr && angle_rows < 1))
     return -10;
-  if (!aligned16(q) || !aligned16(k_codes) || !aligned16(k_pairs) || !aligned16(v_codes) || !aligned16(v_pairs)) return -10;
+  for (const void* x : {q, static_cast<const void*>(angle), static_cast<const void*>(k_codes), static_cast<const void*>(k_pairs),
+                        static_cast<const void*>(v_codes), static_cast<const void*>(v_pairs)})
+    if (!aligned16(x)) return -10;
   if (splits > kAttnCluster && scratch == nullptr) return -10;
   if (B == 0) return 0;
-  Int4AttnParams p;
+  Int4AttnParams p = {};
   p.q = static_cast<const __nv_bfloat16*>(q);
+  p.angle = reinterpret_cast<const float2*>(angle);
   p.k_pool = {static_cast<uint8_t*>(k_codes), static_cast<uint32_t*>(k_pairs)};
   p.v_pool = {static_cast<uint8_t*>(v_codes), static_cast<uint32_t*>(v_pairs)};
-  p.page_table = page_table;
-  p.lengths = lengths;
+  p.page_table = page_table, p.lengths = lengths;
   p.part_out = scratch;
   p.part_ml = scratch == nullptr ? nullptr : scratch + static_cast<int64_t>(B) * num_q_heads * splits * head_dim;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.status = status;
   p.num_q_heads = num_q_heads, p.num_kv_heads = num_kv_heads, p.page_size = page_size;
   p.max_pages = max_pages, p.num_pages = num_pages, p.splits = splits;
+  p.angle_rows = angle_rows;
   p.page_shift = -1;
   for (int i = 0; i < 31; ++i)
     if (page_size == 1 << i) p.page_shift = i;
   p.scale_log2 = softmax_scale * 1.4426950408889634f * kInt4Back;
-  return head_dim == 128 ? int4_attn<128>(p, B, stream) : int4_attn<64>(p, B, stream);
+  if (angle == nullptr) return head_dim == 128 ? int4_attn<128, false>(p, B, stream) : int4_attn<64, false>(p, B, stream);
+  return head_dim == 128 ? int4_attn<128, true>(p, B, stream) : int4_attn<64, true>(p, B, stream);
 }

@@ -21,11 +21,10 @@ word, which ``cuda_ops.check_status`` raises.  The bf16 forms of these operation
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import dataclasses
 import math
-from typing import NamedTuple, Optional, Union
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -44,13 +43,14 @@ def _lib():
     global _configured
     h = cuda_ops.lib()
     if not _configured:
-        h.axb_int4_append.argtypes = [c_void_p] * 8 + [c_int, c_void_p, c_void_p] + [c_int] * 9 + [c_void_p] * 2
-        h.axb_int4_decode_attn.argtypes = [c_void_p] * 9 + [c_int] * 8 + [c_float, c_void_p, c_void_p]
+        h.axb_int4_append.argtypes = [c_void_p] * 2 + [c_int64] * 6 + [c_void_p] * 9 + [c_int] * 7 + [c_void_p] * 2
+        h.axb_int4_append_prompt.argtypes = [c_void_p] * 7 + [c_int] * 9 + [c_void_p] * 2
+        h.axb_int4_decode_attn.argtypes = [c_void_p] * 10 + [c_int] * 9 + [c_float, c_void_p, c_void_p]
         h.axb_int4_attn_scratch_floats.argtypes = [c_int] * 4
         h.axb_int4_attn_scratch_floats.restype = c_int64
-        h.axb_int4_linear.argtypes = [c_void_p] * 4 + [c_int] * 4 + [c_int64, c_int64, c_int, c_void_p]
+        h.axb_int4_linear.argtypes = [c_void_p] * 4 + [c_int] * 4 + [c_int64, c_int64, c_int, c_int, c_void_p]
         h.axb_int4_expand.argtypes = [c_void_p] * 3 + [c_int] * 3 + [c_void_p]
-        for f in (h.axb_int4_append, h.axb_int4_decode_attn, h.axb_int4_linear, h.axb_int4_expand):
+        for f in (h.axb_int4_append, h.axb_int4_append_prompt, h.axb_int4_decode_attn, h.axb_int4_linear, h.axb_int4_expand):
             f.restype = c_int
         _configured = True
     return h
@@ -60,9 +60,13 @@ def _on_kernel(x: Tensor) -> bool:
     return x.is_cuda and x.dtype == torch.bfloat16 and not dispatch._flags.force_reference  # pylint: disable=protected-access
 
 
-def _device_of(x: Tensor):
-    """Launches go to the device of the operands."""
-    return contextlib.nullcontext() if x.device.index == torch.cuda.current_device() else torch.cuda.device(x.device)
+def _call(device: torch.device, name: str, *args) -> None:
+    """Launches on the device of the operands, on its current stream."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _call(device, name, *args)
+    rc = getattr(_lib(), name)(*args, cuda_ops._stream())  # pylint: disable=protected-access
+    return cuda_ops._check(rc, name)  # pylint: disable=protected-access
 
 
 # ------------------------------------------------------------------------------------------
@@ -153,51 +157,55 @@ def quantize_weight(w: Tensor, *, group: int = 128) -> Int4Weight:
 def dequantize_weight(w: Int4Weight, dtype: torch.dtype = torch.bfloat16) -> Tensor:
     """``[K, N]``, rounded to ``dtype``; on the GPU in bf16 a transposed view of a ``[N, K]`` buffer, for the GEMM."""
     if w.codes.is_cuda and dtype == torch.bfloat16 and not dispatch._flags.force_reference:  # pylint: disable=protected-access
-        with _device_of(w.codes):
-            out = torch.empty((w.codes.shape[0] * 16, w.codes.shape[1] * 64), dtype=dtype, device=w.codes.device)
-            rc = _lib().axb_int4_expand(w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), w.n, w.k, w.group,
-                                        cuda_ops._stream())  # pylint: disable=protected-access
-            cuda_ops._check(rc, "axb_int4_expand")  # pylint: disable=protected-access
+        out = torch.empty((w.codes.shape[0] * 16, w.codes.shape[1] * 64), dtype=dtype, device=w.codes.device)
+        _call(out.device, "axb_int4_expand", w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), w.n, w.k, w.group)
         return out[:w.n, :w.k].t()
     tiles, groups = w.scales.shape[:2]
     scales = w.scales.permute(0, 3, 2, 1, 4).reshape(tiles * 16, groups, 2)
     return group_values(_unpack_blocks(w.codes), scales).t()[:w.k, :w.n].to(dtype)
 
 
+def linear_splits(rows: int, k: int, n: int, sms: int = 148) -> int:
+    """Slices of K of a product of few rows: one wave of CTAs (four fit an SM; a CTA takes 64 columns, 32 or 16 of more than 16
+    or 32 rows), 512 rows of the weight or more for each.  More than four slices pay where columns are few and K is long."""
+    ctas = -(-n // (64 if rows <= 16 else 32 if rows <= 32 else 16))
+    return max(1, min(8 if ctas <= 32 and k >= 8192 else 4, k // 512, 4 * sms // ctas))
+
+
 def int4_linear(x: Tensor, w: Int4Weight, *, out: Optional[Tensor] = None, accumulate: bool = False) -> Tensor:
     """``x [..., K] @ w`` with fp32 accumulation, rounded to ``x.dtype``; into ``out [..., N]``, or with ``accumulate`` added to
     it.  Up to 64 rows read the 4-bit weights as they are; more rows multiply with their values rounded to bf16.  Serving
     only: there is no gradient.  (Sums that overflow fp32 on the way, as with an infinity in x, are NaN.)"""
-    if x.shape[-1] != w.k or x.device != w.codes.device:
-        raise ValueError(f"x {tuple(x.shape)} on {x.device} and a {w.shape} weight on {w.codes.device}")
-    if torch.is_grad_enabled() and x.requires_grad:
+    k, n, codes = w.k, w.n, w.codes
+    device = x.device
+    if x.shape[-1] != k or device != codes.device:
+        raise ValueError(f"x {tuple(x.shape)} on {device} and a {w.shape} weight on {codes.device}")
+    if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("int4_linear has no gradient")
-    shape = x.shape[:-1] + (w.n,)
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
-    elif out.shape != shape or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous():
-        raise ValueError(f"out {tuple(out.shape)} {out.dtype}: contiguous {tuple(shape)} {x.dtype} is wanted")
-    rows = out.numel() // w.n
+        out = x.new_empty(x.shape[:-1] + (n,))
+    elif out.shape != x.shape[:-1] + (n,) or out.dtype != x.dtype or out.device != device or not out.is_contiguous():
+        raise ValueError(f"out {tuple(out.shape)} {out.dtype}: contiguous {tuple(x.shape[:-1]) + (n,)} {x.dtype} is wanted")
     if not _on_kernel(x):
         y = x.float() @ dequantize_weight(w, torch.float32)
         return out.copy_(out.float() + y if accumulate else y)
+    rows = x.shape[0] if x.dim() == 2 else out.numel() // n
     if rows == 0:
         return out
-    if x.dim() != 2 or x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < w.k or x.data_ptr() % 16:
-        x = x.reshape(rows, w.k).contiguous()
+    ldx = x.stride(0) if x.dim() == 2 and x.stride(1) == 1 else 0
+    if ldx < k or ldx % 8 or x.data_ptr() % 16:
+        x, ldx = x.reshape(rows, k).contiguous(), k
         if x.data_ptr() % 16:
             x = x.clone()
     if rows <= MAX_STREAMED_ROWS:
-        with _device_of(x):
-            rc = _lib().axb_int4_linear(x.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, w.n, w.k,
-                                        w.group, x.stride(0), w.n, 1 if accumulate else 0,
-                                        cuda_ops._stream())  # pylint: disable=protected-access
-            cuda_ops._check(rc, "axb_int4_linear")  # pylint: disable=protected-access
+        _call(device, "axb_int4_linear", x.data_ptr(), codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, n, k, w.group,
+              ldx, n, 1 if accumulate else 0, linear_splits(rows, k, n))
         return out
-    with _device_of(x):
-        cuda_ops.gemm(x, dequantize_weight(w), out=out.view(rows, w.n), accumulate=accumulate)
+    expanded = dequantize_weight(w)
+    with torch.cuda.device(device):
+        cuda_ops.gemm(x, expanded, out=out.view(rows, n), accumulate=accumulate)
     return out
 
 
@@ -241,22 +249,25 @@ def page_values(pages: Int4Pages, dtype: torch.dtype = torch.float32) -> Tensor:
     return group_values(_unpack_rows(pages.codes), pages.scales).to(dtype)
 
 
-def _check_pages(k_pages: Int4Pages, v_pages: Int4Pages, page_table: Tensor, heads: int, head_dim: int, device) -> tuple:
+def _check_pages(k_pages: Int4Pages, v_pages: Int4Pages, page_table: Tensor, batch: int, heads: int, head_dim: int,
+                 device: torch.device) -> tuple:
     """``(pages, Nkv, page size)`` of a cache that fits."""
-    codes, scales = k_pages
-    shape = codes.shape
-    if (len(shape) != 4 or head_dim not in (64, 128) or shape[3] * 2 != head_dim or v_pages.codes.shape != shape or not shape[1]
-            or heads % shape[1] or scales.shape != shape[:3] + (head_dim // CACHE_GROUP, 2)
-            or v_pages.scales.shape != scales.shape or not shape[2]):
-        raise ValueError(f"4-bit pages {tuple(shape)}, {tuple(scales.shape)} for {heads} heads of {head_dim} (64 or 128)")
+    (kc, ks), (vc, vs) = k_pages, v_pages
+    shape = kc.shape
+    num_pages, nkv, page_size, half = shape if len(shape) == 4 else (0, 0, 0, 0)
+    if (half * 2 != head_dim or head_dim not in (64, 128) or not nkv or heads % nkv or not page_size or vc.shape != shape
+            or ks.shape != (num_pages, nkv, page_size, half // 16, 2) or vs.shape != ks.shape):
+        raise ValueError(f"4-bit pages {tuple(shape)} with {tuple(ks.shape)}, {tuple(vc.shape)} with {tuple(vs.shape)} for {heads} "
+                         f"heads of {head_dim} (64 or 128)")
     for codes, scales in (k_pages, v_pages):
-        if (codes.dtype != torch.uint8 or scales.dtype != torch.bfloat16 or not codes.is_contiguous()
-                or not scales.is_contiguous() or codes.device != device or scales.device != device):
+        if (codes.dtype is not torch.uint8 or scales.dtype is not torch.bfloat16 or codes.device != device
+                or scales.device != device or not codes.is_contiguous() or not scales.is_contiguous()):
             raise ValueError(f"4-bit pages are contiguous uint8 and bf16 tensors on {device}")
-    if (page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous()
-            or page_table.device != device):
-        raise ValueError(f"a page table is a contiguous int32 matrix on {device}")
-    return shape[0], shape[1], shape[2]
+    if (page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch
+            or page_table.device != device or not page_table.is_contiguous()):
+        raise ValueError(f"a page table is a contiguous int32 matrix of {batch} rows on {device}: {tuple(page_table.shape)} "
+                         f"{page_table.dtype}")
+    return num_pages, nkv, page_size
 
 
 def _check_counts(counts: Tensor, batch: int, name: str, device) -> Tensor:
@@ -293,20 +304,6 @@ def _append_plain(k, v, k_pages, v_pages, page_table, start, live):
     return values
 
 
-def _launch_append(rows, k_pages, v_pages, page_table, start, start_offset, live, table, b, t, nq, nkv, h):
-    """``rows``: q, k, v, where q goes, where the values of k and v go (None: not there), ``[B, T, heads, H]`` each."""
-    ptrs = (c_void_p * 6)(*[None if x is None else x.data_ptr() for x in rows])
-    strides = (c_int64 * 18)(*[s for x in rows for s in ((0, 0, 0) if x is None else x.stride()[:3])])
-    rc = _lib().axb_int4_append(
-        ptrs, strides, k_pages.codes.data_ptr(), k_pages.scales.data_ptr(), v_pages.codes.data_ptr(),
-        v_pages.scales.data_ptr(), page_table.data_ptr(), None if start is None else start.data_ptr(), start_offset,
-        None if live is None else live.data_ptr(), None if table is None else table.data_ptr(),
-        0 if table is None else table.shape[0], b, t, nq, nkv, h, k_pages.codes.shape[2], page_table.shape[1],
-        k_pages.codes.shape[0], cuda_ops.status_word(k_pages.codes.device).data_ptr(),
-        cuda_ops._stream())  # pylint: disable=protected-access
-    cuda_ops._check(rc, "axb_int4_append")  # pylint: disable=protected-access
-
-
 def append_int4(k: Tensor, v: Tensor, k_pages: Int4Pages, v_pages: Int4Pages, page_table: Tensor, start: Tensor, *,
                 live: Optional[Tensor] = None, values: bool = False) -> Optional[tuple[Tensor, Tensor]]:
     """Quantises ``k`` and ``v [B, T, Nkv, H]`` (strided views may be given) into the pages of positions ``start[b] ..`` of
@@ -316,21 +313,32 @@ def append_int4(k: Tensor, v: Tensor, k_pages: Int4Pages, v_pages: Int4Pages, pa
     b, t, nkv, h = k.shape
     if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
         raise ValueError(f"k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} differ")
-    if _check_pages(k_pages, v_pages, page_table, nkv, h, k.device)[1] != nkv or page_table.shape[0] != b:
-        raise ValueError(f"pages of {k_pages.codes.shape[1]} heads and a table of {page_table.shape[0]} rows for {nkv} heads of {b} "
-                         "sequences")
-    _check_counts(start, b, "start", k.device)
+    device = k.device
+    num_pages, held, page_size = _check_pages(k_pages, v_pages, page_table, b, nkv, h, device)
+    if held != nkv:
+        raise ValueError(f"pages of {held} heads for {nkv}")
+    _check_counts(start, b, "start", device)
     if live is not None:
-        _check_counts(live, b, "live", k.device)
+        _check_counts(live, b, "live", device)
     if not _on_kernel(k):
         out = _append_plain(k, v, k_pages, v_pages, page_table, start, live)
         return tuple(out) if values else None
-    k, v = (x if x.stride(3) == 1 and not (x.stride(0) | x.stride(1) | x.stride(2)) % 8 and x.data_ptr() % 16 == 0
-            else x.clone(memory_format=torch.contiguous_format) for x in (k, v))
-    out = tuple(torch.empty((b, t, nkv, h), dtype=k.dtype, device=k.device) for _ in range(2)) if values else (None, None)
-    with _device_of(k):
-        _launch_append((None, k, v, None) + out, k_pages, v_pages, page_table, start, 0, live, None, b, t, 0, nkv, h)
-    return out if values else None
+    k, v = _aligned_rows(k), _aligned_rows(v)
+    out = (k.new_empty((b, t, nkv, h)), k.new_empty((b, t, nkv, h))) if values else None
+    _call(device, "axb_int4_append", k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3],
+          out[0].data_ptr() if values else None, out[1].data_ptr() if values else None, k_pages.codes.data_ptr(),
+          k_pages.scales.data_ptr(), v_pages.codes.data_ptr(), v_pages.scales.data_ptr(), page_table.data_ptr(), start.data_ptr(),
+          None if live is None else live.data_ptr(), b, t, nkv, h, page_size, page_table.shape[1], num_pages,
+          cuda_ops.status_word(device).data_ptr())
+    return out
+
+
+def _aligned_rows(x: Tensor) -> Tensor:
+    """``x [B, T, N, H]`` with 16-byte aligned rows of neighbouring dims."""
+    b, t, n, h = x.stride()
+    if h == 1 and not (b | t | n) % 8 and not x.data_ptr() % 16:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 def attention_splits(batch: int, num_kv_heads: int, group: int, max_len: int, sms: int = 148) -> int:
@@ -368,10 +376,8 @@ def paged_decode_attention_int4(q: Tensor, k_pages: Int4Pages, v_pages: Int4Page
     ``[B, Nq, H]``."""
     b, nq, h = q.shape
     device = q.device
-    num_pages, nkv, page_size = _check_pages(k_pages, v_pages, page_table, nq, h, device)
+    num_pages, nkv, page_size = _check_pages(k_pages, v_pages, page_table, b, nq, h, device)
     _check_counts(lengths, b, "lengths", device)
-    if page_table.shape[0] != b:
-        raise ValueError(f"a page table of {page_table.shape[0]} rows for {b} sequences")
     scale = 1.0 / math.sqrt(h) if softmax_scale is None else softmax_scale
     if not 0 < scale < 2 ** 20:
         raise ValueError(f"softmax_scale {scale} is not in (0, 2^20)")
@@ -382,28 +388,30 @@ def paged_decode_attention_int4(q: Tensor, k_pages: Int4Pages, v_pages: Int4Page
         return y if out is None else out.copy_(y)
     if not q.is_contiguous() or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
-    max_pages = page_table.shape[1]
-    if splits is None:
-        splits = attention_splits(b, nkv, nq // nkv, max_pages * page_size)
     if out is None:
         out = torch.empty_like(q)
-    with _device_of(q):
-        if splits > 8:
-            floats = attention_scratch_floats(b, nq, h, splits)
-            if scratch is None:
-                scratch = torch.empty(floats, dtype=torch.float32, device=device)
-            elif scratch.numel() < floats or scratch.dtype != torch.float32 or scratch.device != device or not scratch.is_contiguous():
-                raise ValueError(f"scratch is {floats} contiguous fp32 values on {device}")
-        rc = _lib().axb_int4_decode_attn(
-            q.data_ptr(), k_pages.codes.data_ptr(), k_pages.scales.data_ptr(), v_pages.codes.data_ptr(),
-            v_pages.scales.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(),
-            None if scratch is None else scratch.data_ptr(), b, nq, nkv, h, page_size, max_pages, num_pages, splits, scale,
-            cuda_ops.status_word(device).data_ptr(), cuda_ops._stream())  # pylint: disable=protected-access
-        cuda_ops._check(rc, "axb_int4_decode_attn")  # pylint: disable=protected-access
+    _launch_attention(q, k_pages, v_pages, page_table, lengths, None, out, scratch, b, nq, nkv, h, page_size, num_pages, splits, scale)
     return out
 
 
+def _launch_attention(q, k_pages, v_pages, page_table, lengths, table, out, scratch, b, nq, nkv, h, page_size, num_pages, splits, scale):
+    max_pages, device = page_table.shape[1], q.device
+    if splits is None:
+        splits = attention_splits(b, nkv, nq // nkv, max_pages * page_size)
+    if splits > 8:
+        floats = attention_scratch_floats(b, nq, h, splits)
+        if scratch is None:
+            scratch = torch.empty(floats, dtype=torch.float32, device=device)
+        elif scratch.numel() < floats or scratch.dtype != torch.float32 or scratch.device != device or not scratch.is_contiguous():
+            raise ValueError(f"scratch is {floats} contiguous fp32 values on {device}")
+    _call(device, "axb_int4_decode_attn", q.data_ptr(), k_pages.codes.data_ptr(), k_pages.scales.data_ptr(), v_pages.codes.data_ptr(),
+          v_pages.scales.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), None if table is None else table.data_ptr(),
+          out.data_ptr(), None if scratch is None else scratch.data_ptr(), 0 if table is None else table.shape[0], b, nq, nkv, h,
+          page_size, max_pages, num_pages, splits, scale, cuda_ops.status_word(device).data_ptr())
+
+
 def attention_scratch_floats(batch: int, num_q_heads: int, head_dim: int, splits: int) -> int:
+    """fp32 values that the parts of more than eight splits take."""
     return _lib().axb_int4_attn_scratch_floats(batch, num_q_heads, head_dim, splits)
 
 
@@ -413,6 +421,7 @@ def _split_qkv(qkv: Tensor, nq: int, nkv: int) -> tuple[Tensor, Tensor, Tensor]:
 
 
 def _check_packed(qkv: Tensor, k_pages: Int4Pages, table: Tensor, nq: int) -> tuple[int, int]:
+    """``(Nkv, H)`` of a packed projection that fits the cache and the rotation table."""
     nkv, h = k_pages.codes.shape[1], k_pages.codes.shape[3] * 2
     if qkv.shape[-1] != (nq + 2 * nkv) * h or not qkv.is_contiguous() or qkv.data_ptr() % 16:
         raise ValueError(f"a packed projection of {nq} + 2 x {nkv} heads of {h} is contiguous and 16-byte aligned: {tuple(qkv.shape)}")
@@ -429,21 +438,21 @@ def rope_decode_attention_int4(qkv: Tensor, k_pages: Int4Pages, v_pages: Int4Pag
     H / 2, 2]`` (``decode_ops.rope_table``), appends key and value to the cache and attends to it.  Rows of length 0 append
     nothing and get zeros.  Returns ``[B, Nq, H]``."""
     nkv, h = _check_packed(qkv, k_pages, table, num_q_heads)
-    b = qkv.shape[0]
-    _check_pages(k_pages, v_pages, page_table, num_q_heads, h, qkv.device)
-    _check_counts(lengths, b, "lengths", qkv.device)
-    q, k, v = (x[:, None] for x in _split_qkv(qkv, num_q_heads, nkv))
-    live = (lengths > 0).to(torch.int32)
+    b, device = qkv.shape[0], qkv.device
+    num_pages, _, page_size = _check_pages(k_pages, v_pages, page_table, b, num_q_heads, h, device)
+    _check_counts(lengths, b, "lengths", device)
+    if not 0 < softmax_scale < 2 ** 20:
+        raise ValueError(f"softmax_scale {softmax_scale} is not in (0, 2^20)")
     if not _on_kernel(qkv):
+        q, k, v = (x[:, None] for x in _split_qkv(qkv, num_q_heads, nkv))
         pos = lengths[:, None].long() - 1
         q, k = _rotate(q, table, pos), _rotate(k, table, pos)
-        _append_plain(k, v, k_pages, v_pages, page_table, lengths - 1, live)
+        _append_plain(k, v, k_pages, v_pages, page_table, lengths - 1, (lengths > 0).to(torch.int32))
         return paged_decode_attention_int4(q[:, 0], k_pages, v_pages, page_table, lengths, softmax_scale=softmax_scale)
-    q_out = torch.empty((b, 1, num_q_heads, h), dtype=qkv.dtype, device=qkv.device)
-    with _device_of(qkv):
-        _launch_append((q, k, v, q_out, None, None), k_pages, v_pages, page_table, lengths, -1, live, table, b, 1, num_q_heads, nkv, h)
-    return paged_decode_attention_int4(q_out[:, 0], k_pages, v_pages, page_table, lengths, softmax_scale=softmax_scale,
-                                       splits=splits, scratch=scratch)
+    out = torch.empty((b, num_q_heads, h), dtype=qkv.dtype, device=device)
+    _launch_attention(qkv, k_pages, v_pages, page_table, lengths, table, out, scratch, b, num_q_heads, nkv, h, page_size, num_pages,
+                      splits, softmax_scale)
+    return out
 
 
 def prompt_attention_int4(qkv: Tensor, k_pages: Int4Pages, v_pages: Int4Pages, page_table: Tensor, table: Tensor, *,
@@ -453,8 +462,9 @@ def prompt_attention_int4(qkv: Tensor, k_pages: Int4Pages, v_pages: Int4Pages, p
     are replaced by rotated ones, keys and values by the cache's.  Returns ``[B, T, Nq * H]``."""
     nkv, h = _check_packed(qkv, k_pages, table, num_q_heads)
     b, t, width = qkv.shape
-    _check_pages(k_pages, v_pages, page_table, num_q_heads, h, qkv.device)
-    if table.shape[0] < t or page_table.shape[0] != b or page_table.shape[1] * k_pages.codes.shape[2] < t:
+    device = qkv.device
+    num_pages, _, page_size = _check_pages(k_pages, v_pages, page_table, b, num_q_heads, h, device)
+    if table.shape[0] < t or page_table.shape[1] * k_pages.codes.shape[2] < t:
         raise ValueError(f"{b} x {t} tokens, a rotation table of {table.shape[0]} positions, a page table {tuple(page_table.shape)}")
     q, k, v = _split_qkv(qkv, num_q_heads, nkv)
     if not _on_kernel(qkv):
@@ -467,6 +477,8 @@ def prompt_attention_int4(qkv: Tensor, k_pages: Int4Pages, v_pages: Int4Pages, p
         return out.reshape(b, t, num_q_heads * h)
     from axlearn_b200.ops import decode_ops
 
-    with _device_of(qkv):
-        _launch_append((q, k, v, q, k, v), k_pages, v_pages, page_table, None, 0, None, table, b, t, num_q_heads, nkv, h)
+    _call(device, "axb_int4_append_prompt", qkv.data_ptr(), k_pages.codes.data_ptr(), k_pages.scales.data_ptr(),
+          v_pages.codes.data_ptr(), v_pages.scales.data_ptr(), page_table.data_ptr(), table.data_ptr(), table.shape[0], b, t,
+          num_q_heads, nkv, h, page_size, page_table.shape[1], num_pages, cuda_ops.status_word(device).data_ptr())
+    with torch.cuda.device(device):
         return decode_ops.packed_prompt_attention(qkv, num_q_heads=num_q_heads, num_kv_heads=nkv, softmax_scale=softmax_scale)

@@ -289,6 +289,27 @@ def test_a_step_is_rotation_append_and_attention(nq, kv, dim, splits):
     assert torch.equal(v_pages.codes, other[1].codes) and torch.equal(v_pages.scales, other[1].scales)
 
 
+def test_a_step_without_a_place_appends_nothing():
+    from axlearn_b200.ops import cuda_ops, decode_ops, int4_ops
+
+    k_pages, v_pages, table = _cache(3, 2, 16, 2, 128, seed=20)
+    rope = decode_ops.rope_table(40, 128, 1e4, "cuda")
+    qkv = _normal(_gen(21), 3, 8 * 128).bfloat16()
+    before = [x.clone() for x in (*k_pages, *v_pages)]
+    lengths = torch.tensor([33, 0, 20], dtype=torch.int32, device="cuda")
+    table[2, 1] = 99                                            # the third sequence's new page is none of the pool's
+    out = int4_ops.rope_decode_attention_int4(qkv, k_pages, v_pages, table, lengths, rope, num_q_heads=4, softmax_scale=0.1)
+    with pytest.raises(RuntimeError, match="status 5"):
+        cuda_ops.check_status()
+    assert not out[:2].any() and all(torch.equal(x, y) for x, y in zip(before, (*k_pages, *v_pages)))
+    # A position that the rotation table does not have is reported, too.
+    table[2, 1] = table[1, 1]
+    int4_ops.rope_decode_attention_int4(qkv, k_pages, v_pages, table, torch.tensor([0, 0, 20], dtype=torch.int32, device="cuda"),
+                                        rope[:19].contiguous(), num_q_heads=4, softmax_scale=0.1)
+    with pytest.raises(RuntimeError, match="status 5"):
+        cuda_ops.check_status()
+
+
 @pytest.mark.parametrize("b,t,nq,kv,dim", [(2, 300, 8, 2, 128), (1, 1, 4, 4, 64), (3, 130, 12, 4, 64)])
 def test_prompts_attend_to_what_the_cache_stands_for(b, t, nq, kv, dim):
     from axlearn_b200.ops import cuda_ops, decode_ops, int4_ops
