@@ -47,6 +47,8 @@ KNOBS: dict[str, tuple[str, str]] = {
     "AXB200_TP_PEER_MAX_BYTES": (str(2 << 30), "Largest staging buffer of the one-shot peer all-reduce; larger messages go to NCCL."),
     "AXB200_NVLS": ("0", "1: bind symmetric buffers to an NVLink multicast object and reduce with multimem instructions."),
     "AXB200_DECODE_ENGINE": ("1", "0: sample_decode stays on the eager extend_step path instead of the CUDA-graph engine."),
+    "AXB200_DECODE_WEIGHT_BITS": ("16", "4: the engine of sample_decode holds a Fuji decoder's matrices in 4 bits (groups of 128)."),
+    "AXB200_DECODE_CACHE_BITS": ("16", "4: the engine of sample_decode holds a Fuji decoder's keys and values in 4 bits (groups of 32)."),
     "AXB_DECODE_FUSED_PUSH": ("", "1 / 0 forces the fused-epilogue push of the decode all-reduce on or off (empty: by rank count)."),
     "AXB200_STACK_SUMMARY": ("1", "0: exceptions keep their full tracebacks instead of the summary that drops framework-internal frames."),
 }

@@ -4,7 +4,8 @@
         -m axlearn_b200.inference.bench_decode --model 7B --batch 64 --prompt-len 2048 --new-tokens 256
 
 Tensor parallel over all ranks (``model`` = world size), random-init bf16 weights, uniform-random
-prompt tokens from seed 0, greedy decoding, paged bf16 KV cache with 16-token pages.  Times are
+prompt tokens from seed 0, greedy decoding, paged KV cache with 16-token pages; ``--weight-bits 4`` and ``--cache-bits
+4`` hold the layers' matrices and the cache in 4 bits (one GPU).  Times are
 CUDA-event times on each rank, reported as the max over ranks.  Prints one JSON line on rank 0.
 """
 
@@ -17,7 +18,7 @@ import os
 import torch
 import torch.distributed as dist
 
-from axlearn_b200.inference.decode_engine import DecodeEngine, FujiDims, LayerWeights
+from axlearn_b200.inference.decode_engine import DecodeEngine, FujiDims, LayerWeights, quantize_weights
 
 MODELS = {
     "7B": FujiDims(num_layers=32, hidden_dim=4096, num_heads=32, num_kv_heads=32, head_dim=128, ffn_dim=11008,
@@ -64,6 +65,8 @@ def main():
     ap.add_argument("--prompt-len", type=int, default=2048)
     ap.add_argument("--new-tokens", type=int, default=256)
     ap.add_argument("--page-size", type=int, default=16)
+    ap.add_argument("--weight-bits", type=int, default=16, choices=(4, 16))
+    ap.add_argument("--cache-bits", type=int, default=16, choices=(4, 16))
     ap.add_argument("--no-graph", action="store_true")
     args = ap.parse_args()
 
@@ -78,8 +81,11 @@ def main():
         group = dist.group.WORLD
     dims = MODELS[args.model]
     weights = random_weights(dims, rank=rank, world=world, device=device)
+    if args.weight_bits == 4:
+        weights = quantize_weights(weights)
     engine = DecodeEngine(weights, dims, batch=args.batch, max_len=args.prompt_len + args.new_tokens + 16,
-                          page_size=args.page_size, group=group, device=device, use_graph=not args.no_graph)
+                          page_size=args.page_size, group=group, device=device, use_graph=not args.no_graph,
+                          cache_bits=args.cache_bits)
     g = torch.Generator().manual_seed(0)
     prompts = torch.randint(0, dims.vocab_size, (args.batch, args.prompt_len), generator=g).to(device)
 
@@ -123,7 +129,8 @@ def main():
             "ttft_ms": ttft_ms, "prefill_tokens_per_s": args.batch * args.prompt_len / (ttft_ms / 1e3),
             "decode_ms_per_token": decode_ms / steps, "decode_tokens_per_s": args.batch * steps / (decode_ms / 1e3),
             "kv_splits": engine.splits, "kernel_launches_per_step": engine.launches_per_step,
-            "cuda_graph": not args.no_graph, "ranks_agree": same, "dtype": "bf16", "data": "synthetic",
+            "cuda_graph": not args.no_graph, "ranks_agree": same, "dtype": "bf16",
+            "weight_bits": args.weight_bits, "cache_bits": args.cache_bits, "data": "synthetic",
         }))
     if world > 1:
         dist.destroy_process_group()

@@ -21,6 +21,9 @@ persistent buffers, so the engine:
 * captures one decode step (all layers, head, greedy pick, length bump) in a CUDA graph and
   replays it per token.
 
+With ``cache_bits=4`` the pools hold keys and values in 4 bits, and weights may be in 4 bits too (``quantize_weights``):
+``ops/int4_ops.py``, on one GPU.
+
 Prefill runs the same weights over whole prompts with the flash-attention forward kernel and
 writes K/V into the pages.  Sequences own a contiguous run of pages (sequence ``b`` owns pages
 ``[b * max_pages, (b + 1) * max_pages)``), which keeps the page table trivial without making
@@ -34,14 +37,15 @@ import dataclasses
 import gc
 import math
 import os
-from typing import Any, Optional
+from typing import Any, Optional, Union
 
 import torch
 
 from axlearn_b200.common.utils import flatten_items
-from axlearn_b200.ops import cuda_ops, decode_ops, packed_ops, step_ops
+from axlearn_b200.ops import cuda_ops, decode_ops, int4_ops, packed_ops, step_ops
 
 Tensor = torch.Tensor
+Matrix = Union[Tensor, int4_ops.Int4Weight]
 
 
 @dataclasses.dataclass
@@ -60,11 +64,21 @@ class FujiDims:
 @dataclasses.dataclass
 class LayerWeights:
     attn_norm: Tensor   # [D]
-    wqkv: Tensor        # [D, (Nq_l + 2 Nkv_l) * H]
-    wo: Tensor          # [Nq_l * H, D]
+    wqkv: Matrix        # [D, (Nq_l + 2 Nkv_l) * H]
+    wo: Matrix          # [Nq_l * H, D]
     ffn_norm: Tensor    # [D]
-    wgu: Tensor         # [D, 2 F_l]  (gate | up)
-    wdown: Tensor       # [F_l, D]
+    wgu: Matrix         # [D, 2 F_l]  (gate | up)
+    wdown: Matrix       # [F_l, D]
+
+
+def quantize_weights(weights: dict, *, group: int = 128) -> dict:
+    """The weights of an engine with the layers' matrices in 4 bits (``int4_ops.quantize_weight``); norms, embedding and
+    output head stay as they are."""
+    def layer(lw: LayerWeights) -> LayerWeights:
+        return dataclasses.replace(lw, **{name: int4_ops.quantize_weight(getattr(lw, name), group=group)
+                                          for name in ("wqkv", "wo", "wgu", "wdown")})
+
+    return {**weights, "layers": [layer(lw) for lw in weights["layers"]]}
 
 
 def _get(tree: dict, path: str):
@@ -248,10 +262,11 @@ class BaseDecodeEngine:
 
 class DecodeEngine(BaseDecodeEngine):
     """Greedy generation for ``batch`` sequences of up to ``max_len`` tokens on one GPU of a
-    tensor-parallel group (``group=None``: single GPU)."""
+    tensor-parallel group (``group=None``: single GPU).  ``cache_bits``: 16 or 4, on one GPU also with the weights of
+    ``quantize_weights``."""
 
     def __init__(self, weights: dict, dims: FujiDims, *, batch: int, max_len: int, page_size: int = 16,
-                 group=None, device=None, use_graph: bool = True, prefill_chunk_tokens: int = 16384):
+                 group=None, device=None, use_graph: bool = True, prefill_chunk_tokens: int = 16384, cache_bits: int = 16):
         super().__init__(batch=batch, vocab_size=dims.vocab_size, use_graph=use_graph,
                          device=device if device is not None else weights["emb"].device)
         self.w, self.dims, self.page_size = weights, dims, page_size
@@ -267,15 +282,23 @@ class DecodeEngine(BaseDecodeEngine):
         self.nq_l, self.nkv_l = d.num_heads // self.world, d.num_kv_heads // self.world
         self.max_pages = (max_len + page_size - 1) // page_size
         self.max_len = self.max_pages * page_size
-        pool = (batch * self.max_pages, page_size, self.nkv_l, d.head_dim)
-        self.k_pools = [torch.zeros(pool, dtype=torch.bfloat16, device=self.device) for _ in range(d.num_layers)]
-        self.v_pools = [torch.zeros(pool, dtype=torch.bfloat16, device=self.device) for _ in range(d.num_layers)]
+        if cache_bits not in (4, 16):
+            raise ValueError(f"a cache of {cache_bits} bits: 4 or 16 are there")
+        self.cache_bits = cache_bits
+        if self.world > 1 and (cache_bits == 4 or any(
+                isinstance(w, int4_ops.Int4Weight) for lw in weights["layers"] for w in (lw.wqkv, lw.wo, lw.wgu, lw.wdown))):
+            raise NotImplementedError("4-bit weights and caches run on one GPU")
+        self.k_pools, self.v_pools = ([self._pool(batch * self.max_pages) for _ in range(d.num_layers)] for _ in range(2))
         self.page_table = torch.arange(batch * self.max_pages, dtype=torch.int32, device=self.device).reshape(
             batch, self.max_pages)
-        self.splits = decode_ops.tile_splits(batch, self.nkv_l, self.nq_l // self.nkv_l, self.max_len)
-        self._scratch = torch.empty(
-            max(1, decode_ops._lib().axb_decode_attn_scratch_floats(batch, self.nq_l, self.splits)),  # pylint: disable=protected-access
-            dtype=torch.float32, device=self.device)
+        if cache_bits == 4:
+            self.splits = int4_ops.attention_splits(batch, self.nkv_l, self.nq_l // self.nkv_l, self.max_len)
+            floats = int4_ops.attention_scratch_floats(batch, self.nq_l, d.head_dim, self.splits)
+            self._rope_table = decode_ops.rope_table(self.max_len, d.head_dim, d.rope_theta, self.device)
+        else:
+            self.splits = decode_ops.tile_splits(batch, self.nkv_l, self.nq_l // self.nkv_l, self.max_len)
+            floats = decode_ops._lib().axb_decode_attn_scratch_floats(batch, self.nq_l, self.splits)  # pylint: disable=protected-access
+        self._scratch = torch.empty(max(1, floats), dtype=torch.float32, device=self.device)
         self._softmax_scale = 1.0 / math.sqrt(d.head_dim)
         self._allreduce: Optional[decode_ops.OneShotAllReduce] = None
         if self.world > 1:
@@ -284,6 +307,11 @@ class DecodeEngine(BaseDecodeEngine):
         self._prefill_chunk_tokens = prefill_chunk_tokens
 
     # ------------------------------------------------------------------ shared pieces
+    def _pool(self, pages: int) -> Union[Tensor, int4_ops.Int4Pages]:
+        if self.cache_bits == 4:
+            return int4_ops.int4_pages(pages, self.page_size, self.nkv_l, self.dims.head_dim, device=self.device)
+        return torch.zeros((pages, self.page_size, self.nkv_l, self.dims.head_dim), dtype=torch.bfloat16, device=self.device)
+
     def _id_range(self) -> Optional[tuple]:
         rows = self.w["emb"].shape[0]
         return -rows, rows  # negative ids count from the end
@@ -315,8 +343,10 @@ class DecodeEngine(BaseDecodeEngine):
         return total, y
 
     @staticmethod
-    def _product(x: Tensor, w: Tensor) -> Tensor:
+    def _product(x: Tensor, w: Matrix) -> Tensor:
         """``x [rows, K] @ w``: the kernel without an autograd node around it where it takes the sizes."""
+        if isinstance(w, int4_ops.Int4Weight):
+            return int4_ops.int4_linear(x, w)
         return cuda_ops.linear(x, w) if x.shape[1] % 8 or w.shape[1] % 8 else cuda_ops.gemm(x, w)
 
     def _sum_ranks(self, x: Tensor) -> Tensor:
@@ -337,7 +367,7 @@ class DecodeEngine(BaseDecodeEngine):
         assert b == self.batch and t <= self.max_len
         h = d.head_dim
         per_chunk = max(1, self._prefill_chunk_tokens // t)
-        table = decode_ops.rope_table(t, h, d.rope_theta, self.device)
+        table = self._rope_table if self.cache_bits == 4 else decode_ops.rope_table(t, h, d.rope_theta, self.device)
         last_hidden = torch.empty((b, d.hidden_dim), dtype=torch.bfloat16, device=self.device)
         for b0 in range(0, b, per_chunk):
             b1 = min(b, b0 + per_chunk)
@@ -347,13 +377,18 @@ class DecodeEngine(BaseDecodeEngine):
             for li, lw in enumerate(self.w["layers"]):
                 x, hn = self._add_norm(x, branch, lw.attn_norm)
                 qkv = self._product(hn, lw.wqkv).reshape(b1 - b0, t, -1)
-                attn = decode_ops.prompt_attention(
-                    qkv, self.k_pools[li].view(b, self.max_len, self.nkv_l, h)[b0:b1],
-                    self.v_pools[li].view(b, self.max_len, self.nkv_l, h)[b0:b1], table, num_q_heads=self.nq_l,
-                    softmax_scale=self._softmax_scale)
+                if self.cache_bits == 4:
+                    attn = int4_ops.prompt_attention_int4(
+                        qkv, self.k_pools[li], self.v_pools[li], self.page_table[b0:b1], table, num_q_heads=self.nq_l,
+                        softmax_scale=self._softmax_scale)
+                else:
+                    attn = decode_ops.prompt_attention(
+                        qkv, self.k_pools[li].view(b, self.max_len, self.nkv_l, h)[b0:b1],
+                        self.v_pools[li].view(b, self.max_len, self.nkv_l, h)[b0:b1], table, num_q_heads=self.nq_l,
+                        softmax_scale=self._softmax_scale)
                 branch = self._sum_ranks(self._product(attn.reshape(rows, self.nq_l * h), lw.wo))
                 x, hn = self._add_norm(x, branch, lw.ffn_norm)
-                act = cuda_ops.gemm_swiglu(hn, lw.wgu)
+                act = None if isinstance(lw.wgu, int4_ops.Int4Weight) else cuda_ops.gemm_swiglu(hn, lw.wgu)
                 if act is None:
                     act = decode_ops.swiglu_packed(self._product(hn, lw.wgu))
                 branch = self._sum_ranks(self._product(act, lw.wdown))
@@ -378,6 +413,24 @@ class DecodeEngine(BaseDecodeEngine):
         cuda_ops.gemm(hn, self.w["head"].t(), out=self.logits, resident=True)
 
     # ------------------------------------------------------------------ decode
+    @staticmethod
+    def _step_product(x: Tensor, w: Matrix, residual: Optional[Tensor] = None) -> Tensor:
+        """``x @ w``, into ``residual`` where there is one."""
+        if isinstance(w, int4_ops.Int4Weight):
+            return int4_ops.int4_linear(x, w, out=residual, accumulate=residual is not None)
+        return cuda_ops.gemm(x, w, out=residual, accumulate=residual is not None, resident=True)
+
+    def _attend(self, layer: int, qkv: Tensor) -> Tensor:
+        """Attention of the new token, appended to the layer's cache."""
+        cache = (self.k_pools[layer], self.v_pools[layer], self.page_table, self.lengths)
+        if self.cache_bits == 4:
+            return int4_ops.rope_decode_attention_int4(
+                qkv, *cache, self._rope_table, num_q_heads=self.nq_l, softmax_scale=self._softmax_scale, splits=self.splits,
+                scratch=self._scratch)
+        return decode_ops.rope_decode_attention(
+            qkv, *cache, num_q_heads=self.nq_l, theta=self.dims.rope_theta, softmax_scale=self._softmax_scale,
+            splits=self.splits, scratch=self._scratch)
+
     def _step(self) -> None:
         """One token for every sequence: consumes ``self.tokens`` (the latest token), appends
         its K/V, and leaves the next token in ``self.tokens``."""
@@ -393,21 +446,18 @@ class DecodeEngine(BaseDecodeEngine):
             x = self.w["emb"][self.tokens]                                    # [B, D]
         for li, lw in enumerate(self.w["layers"]):
             hn = cuda_ops.rms_norm(x, lw.attn_norm, d.norm_eps)
-            qkv = cuda_ops.gemm(hn, lw.wqkv, resident=True)
-            attn = decode_ops.rope_decode_attention(
-                qkv, self.k_pools[li], self.v_pools[li], self.page_table, self.lengths, num_q_heads=self.nq_l,
-                theta=d.rope_theta, softmax_scale=self._softmax_scale, splits=self.splits, scratch=self._scratch)
+            attn = self._attend(li, self._step_product(hn, lw.wqkv))
             attn2 = attn.reshape(self.batch, self.nq_l * d.head_dim)
             if self.world > 1:
                 x = self._gemm_reduce(attn2, lw.wo, x, 2 * li)
             else:
-                cuda_ops.gemm(attn2, lw.wo, out=x, accumulate=True, resident=True)  # x += attn @ Wo
+                self._step_product(attn2, lw.wo, residual=x)
             hn = cuda_ops.rms_norm(x, lw.ffn_norm, d.norm_eps)
-            act = decode_ops.swiglu_packed(cuda_ops.gemm(hn, lw.wgu, resident=True))
+            act = decode_ops.swiglu_packed(self._step_product(hn, lw.wgu))
             if self.world > 1:
                 x = self._gemm_reduce(act, lw.wdown, x, 2 * li + 1)
             else:
-                cuda_ops.gemm(act, lw.wdown, out=x, accumulate=True, resident=True)
+                self._step_product(act, lw.wdown, residual=x)
         self._logits(x)
         step_ops.step_end(self.logits, self.tokens)
         self.launches_per_step = cuda_ops.launch_count - before
@@ -564,6 +614,13 @@ def dims_from_decoder(decoder) -> Optional[FujiDims]:
         return None
 
 
+def _bits(name: str) -> int:
+    value = os.environ.get("AXB200_DECODE_WEIGHT_BITS", "16") if name == "WEIGHT" else os.environ.get("AXB200_DECODE_CACHE_BITS", "16")
+    if value not in ("4", "16"):
+        raise ValueError(f"AXB200_DECODE_{name}_BITS is 4 or 16, not {value!r}")
+    return int(value)
+
+
 def engine_for_decoder(decoder, *, batch: int, max_len: int) -> Optional[BaseDecodeEngine]:
     """A (cached) engine over the decoder's current parameters, or None when the decoder, its
     placement or its shapes are outside what the engine implements."""
@@ -591,11 +648,14 @@ def engine_for_decoder(decoder, *, batch: int, max_len: int) -> Optional[BaseDec
     emb = _get(state, "emb/token_emb/weight")
     if not emb.is_cuda or emb.dtype != torch.bfloat16:
         return None
-    key = (id(decoder), batch, max_len, emb.data_ptr())
+    weight_bits, cache_bits = (_bits(name) for name in ("WEIGHT", "CACHE"))
+    key = (id(decoder), batch, max_len, emb.data_ptr(), weight_bits, cache_bits)
     engine = _ENGINES.get(key)
     if engine is None:
         _ENGINES.clear()          # one resident engine: its caches and weight copies are large
         weights = weights_from_fuji_state({"decoder": state}, dims, device=emb.device)
-        engine = DecodeEngine(weights, dims, batch=batch, max_len=max_len, device=emb.device)
+        if weight_bits == 4:
+            weights = quantize_weights(weights)
+        engine = DecodeEngine(weights, dims, batch=batch, max_len=max_len, device=emb.device, cache_bits=cache_bits)
         _ENGINES[key] = engine
     return engine

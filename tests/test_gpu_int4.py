@@ -370,3 +370,107 @@ def test_calls_replay_in_a_graph_and_on_another_stream():
         row = (table.long().gather(1, (lengths[:, None].long() - 1) // 16)[:, 0], (lengths.long() - 1) % 16)
         assert torch.equal(p.codes[row[0], :, row[1]], o.codes[row[0], :, row[1]])
     cuda_ops.check_status()
+
+
+def _engine_weights(d, f, vocab, nq, nkv, layers, seed=0):
+    from axlearn_b200.inference.decode_engine import FujiDims, LayerWeights
+
+    g = _gen(seed)
+
+    def w(*shape):
+        return (_normal(g, *shape) * shape[0] ** -0.5).bfloat16()
+
+    weights = {"layers": [LayerWeights(attn_norm=1 + 0.1 * w(d), wqkv=w(d, (nq + 2 * nkv) * 128), wo=w(nq * 128, d),
+                                       ffn_norm=1 + 0.1 * w(d), wgu=w(d, 2 * f), wdown=w(f, d)) for _ in range(layers)],
+               "emb": w(vocab, d) * 16, "head": w(vocab, d), "final_norm": 1 + 0.1 * w(d)}
+    return weights, FujiDims(num_layers=layers, hidden_dim=d, num_heads=nq, num_kv_heads=nkv, head_dim=128, ffn_dim=f,
+                             vocab_size=vocab)
+
+
+@pytest.mark.parametrize("weight_bits,cache_bits", [(4, 4), (4, 16), (16, 4)])
+@pytest.mark.parametrize("b,nq,nkv", [(1, 4, 4), (5, 8, 2)])
+def test_engine_in_4_bits_matches_its_plain_statements(weight_bits, cache_bits, b, nq, nkv):
+    """Prompts and steps with the kernels against the same engine on the plain 4-bit statements, the captured step against
+    separate launches."""
+    from axlearn_b200.inference import decode_engine
+    from axlearn_b200.ops import int4_ops
+
+    weights, dims = _engine_weights(256, 520, 1000, nq, nkv, 2, seed=b)
+    if weight_bits == 4:
+        weights = decode_engine.quantize_weights(weights, group=64)
+        assert all(isinstance(lw.wgu, int4_ops.Int4Weight) for lw in weights["layers"])
+    ids = torch.randint(0, 1000, (b, 90), device="cuda", generator=_gen(1))
+    lengths = torch.randint(1, 71, (b,), device="cuda", generator=_gen(2))
+    lengths[0] = 70
+
+    def engine(use_graph):
+        return decode_engine.DecodeEngine(weights, dims, batch=b, max_len=96, use_graph=use_graph, cache_bits=cache_bits)
+
+    chained, separate, plain = engine(True), engine(False), engine(False)
+
+    def close():
+        # Two layers of some five operations, each of which may round its output the other way (2^-8 of it); norms and
+        # residuals pass that on with a gain of about one.  A key or value x that does moves to the next level of its group in
+        # 2^-8 |x| / s of the cases, by s: with |x| about 0.8 sigma and s a fifteenth of 4.2 sigma that is sqrt(2 * 2^-8 * 0.8
+        # * 0.28) = 0.042 sigma (rms; both sides may move) of keys and values alike, in each layer's attention.
+        off = (separate.logits - plain.logits).norm() / plain.logits.norm()
+        assert off < 10 * 2.0 ** -8 + (2 * 0.042 if cache_bits == 4 else 0), off
+
+    firsts = [e.prefill(ids[:, :70], lengths=lengths) for e in (chained, separate)]
+    assert torch.equal(firsts[0], firsts[1])
+    _plain(plain.prefill, ids[:, :70], lengths=lengths)
+    close()
+    for i in range(70, 90):
+        x, y = chained.step_logits(ids[:, i]).clone(), separate.step_logits(ids[:, i])
+        assert torch.equal(x, y)
+        _plain(plain.step_logits, ids[:, i])
+        close()
+    tokens = chained.generate(ids[:, :33], 5)
+    assert tokens.shape == (b, 5) and torch.equal(tokens, separate.generate(ids[:, :33], 5))
+
+
+@pytest.mark.parametrize("batch", [1, 16])
+def test_engine_steps_in_4_bits_at_serving_widths(batch):
+    """Kernels that overlap for long: replays of the chained step against separate launches, bit for bit."""
+    from axlearn_b200.inference import decode_engine
+
+    weights, dims = _engine_weights(4096, 14336, 8192, 32, 8, 2, seed=3)
+    weights = decode_engine.quantize_weights(weights)
+    engines = [decode_engine.DecodeEngine(weights, dims, batch=batch, max_len=2048, use_graph=use, cache_bits=4) for use in (True, False)]
+    ids = torch.randint(0, 8192, (batch, 1500), device="cuda", generator=_gen(4))
+    lengths = torch.randint(1, 1501, (batch,), device="cuda", generator=_gen(5))
+    for e in engines:
+        e.prefill(ids, lengths=lengths)
+    for i in range(12):
+        x, y = (e.step_logits(ids[:, i]).clone() for e in engines)
+        assert torch.equal(x, y), i
+
+
+def test_sample_decode_takes_the_bits_of_the_environment(monkeypatch):
+    from axlearn_b200.common import decoding, logit_modifiers, prng
+    from axlearn_b200.common.module import functional
+    from axlearn_b200.common.utils import tree_map
+    from axlearn_b200.inference import decode_engine
+    from axlearn_b200.ops import int4_ops
+    from tests.test_gpu_decode import _tiny_model
+
+    model, params = _tiny_model(1)
+    params = tree_map(lambda t: t.cuda().bfloat16() if t.is_floating_point() else t.cuda(), params)
+    prefix = torch.randint(2, 512, (2, 24), device="cuda", generator=_gen(6))
+    prefix[1, 9:] = 0
+    kwargs = dict(input_batch={"prefix": prefix}, num_decodes=2, max_sequence_length=40, logits_modifier=logit_modifiers.top_k_logits(1),
+                  stop_decoding_condition=decoding.StopOnSubsequence([[511]]))
+    seen = []
+    real = decode_engine.DecodeEngine.step_logits
+    monkeypatch.setattr(decode_engine.DecodeEngine, "step_logits", lambda self, tokens: (seen.append(self), real(self, tokens))[1])
+    monkeypatch.setenv("AXB200_DECODE_WEIGHT_BITS", "4")
+    monkeypatch.setenv("AXB200_DECODE_CACHE_BITS", "4")
+    out, _ = functional(model, prng.PRNGKey(5), params, kwargs, is_training=False, method="sample_decode")
+    assert out.sequences.shape == (2, 2, 39) and seen[-1].cache_bits == 4
+    assert isinstance(seen[-1].w["layers"][0].wo, int4_ops.Int4Weight)
+    monkeypatch.delenv("AXB200_DECODE_WEIGHT_BITS")
+    functional(model, prng.PRNGKey(5), params, kwargs, is_training=False, method="sample_decode")
+    assert seen[-1].cache_bits == 4 and isinstance(seen[-1].w["layers"][0].wo, torch.Tensor)
+    monkeypatch.setenv("AXB200_DECODE_CACHE_BITS", "8")
+    with pytest.raises(ValueError, match="4 or 16"):
+        functional(model, prng.PRNGKey(5), params, kwargs, is_training=False, method="sample_decode")
