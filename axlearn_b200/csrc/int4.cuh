@@ -4,7 +4,10 @@
 // chunk is what a row of an MMA tile needs of V, two neighbouring chunks are what a lane needs of K.
 #pragma once
 
+#include <atomic>
+
 #include <cuda_bf16.h>
+#include <cuda_runtime.h>
 #include <stdint.h>
 
 #include "mma_sync.cuh"
@@ -31,5 +34,21 @@ __device__ __forceinline__ float pair_m(uint32_t u) { return __uint_as_float(u &
 
 // A bad index that the device found: code 5 of the status word.
 __device__ __forceinline__ void int4_report(int* status) { *reinterpret_cast<volatile int*>(status) = 5; }
+
+// A kernel's shared memory above 48 KB, asked for once on each device.
+struct OptIn {
+  std::atomic<uint64_t> devices{0};
+
+  template <typename Kernel>
+  bool done(Kernel kernel, int bytes) {
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device > 63) return false;
+    const uint64_t bit = uint64_t{1} << device;
+    if (devices.load(std::memory_order_acquire) & bit) return true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+    devices.fetch_or(bit, std::memory_order_release);
+    return true;
+  }
+};
 
 }  // namespace axb

@@ -262,8 +262,8 @@ template <int kBlocks, int kTiles, int kGroup>
 static int launch_int4_linear(Int4LinearParams p, int splits, cudaStream_t stream) {
   using L = Int4Lin<kBlocks, kTiles, kGroup>;
   constexpr auto kernel = int4_linear_kernel<kBlocks, kTiles, kGroup>;
-  static const cudaError_t configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
-  if (configured != cudaSuccess) return -3;
+  static OptIn opt_in;
+  if (!opt_in.done(kernel, L::kSmem)) return -3;
   p.splits = splits;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;

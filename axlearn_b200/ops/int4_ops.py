@@ -34,8 +34,9 @@ c_void_p, c_int, c_int64, c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_int6
 Tensor = torch.Tensor
 
 CACHE_GROUP = 32
-# Rows of x up to which weights are expanded in registers; beyond, W is expanded to bf16 once and multiplied by the GEMM.
-MAX_STREAMED_ROWS = 64
+# Rows of x up to which codes are operands as they are, and up to which weights are expanded inside the product; beyond, W is
+# expanded to bf16 once and multiplied by the GEMM.
+MAX_STREAMED_ROWS, MAX_FUSED_ROWS = 16, 128
 _configured = False
 
 
@@ -49,8 +50,10 @@ def _lib():
         h.axb_int4_attn_scratch_floats.argtypes = [c_int] * 4
         h.axb_int4_attn_scratch_floats.restype = c_int64
         h.axb_int4_linear.argtypes = [c_void_p] * 4 + [c_int] * 4 + [c_int64, c_int64, c_int, c_int, c_void_p]
+        h.axb_int4_gemm.argtypes = [c_void_p] * 4 + [c_int] * 4 + [c_int64, c_int64, c_int, c_int, c_void_p, c_void_p]
         h.axb_int4_expand.argtypes = [c_void_p] * 3 + [c_int] * 3 + [c_void_p]
-        for f in (h.axb_int4_append, h.axb_int4_append_prompt, h.axb_int4_decode_attn, h.axb_int4_linear, h.axb_int4_expand):
+        for f in (h.axb_int4_append, h.axb_int4_append_prompt, h.axb_int4_decode_attn, h.axb_int4_linear, h.axb_int4_gemm,
+                  h.axb_int4_expand):
             f.restype = c_int
         _configured = True
     return h
@@ -172,9 +175,14 @@ def linear_splits(rows: int, k: int, n: int, sms: int = 148) -> int:
     return max(1, min(8 if ctas <= 32 and k >= 8192 else 4, k // 512, 4 * sms // ctas))
 
 
+def fused_splits(k: int, n: int, sms: int = 148) -> int:
+    """Slices of K of a product of 17 to 128 rows: about one CTA of 128 columns an SM, 512 rows of the weight or more for each."""
+    return max(1, min(8, k // 512, sms // -(-n // 128)))
+
+
 def int4_linear(x: Tensor, w: Int4Weight, *, out: Optional[Tensor] = None, accumulate: bool = False) -> Tensor:
     """``x [..., K] @ w`` with fp32 accumulation, rounded to ``x.dtype``; into ``out [..., N]``, or with ``accumulate`` added to
-    it.  Up to 64 rows read the 4-bit weights as they are; more rows multiply with their values rounded to bf16.  Serving
+    it.  Up to 16 rows multiply with the 4-bit weights as they are, more rows with their values rounded to bf16.  Serving
     only: there is no gradient.  (Sums that overflow fp32 on the way, as with an infinity in x, are NaN.)"""
     k, n, codes = w.k, w.n, w.codes
     device = x.device
@@ -202,6 +210,10 @@ def int4_linear(x: Tensor, w: Int4Weight, *, out: Optional[Tensor] = None, accum
     if rows <= MAX_STREAMED_ROWS:
         _call(device, "axb_int4_linear", x.data_ptr(), codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, n, k, w.group,
               ldx, n, 1 if accumulate else 0, linear_splits(rows, k, n))
+        return out
+    if rows <= MAX_FUSED_ROWS:
+        _call(device, "axb_int4_gemm", x.data_ptr(), codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, n, k, w.group,
+              ldx, n, 1 if accumulate else 0, fused_splits(k, n), cuda_ops.status_word(device).data_ptr())
         return out
     expanded = dequantize_weight(w)
     with torch.cuda.device(device):
