@@ -1,10 +1,10 @@
 // y[M, N] = x[M, K] W (+ y) for up to 128 rows with weights held in 4 bits (layout: int4_linear.cu), on the fifth-generation
 // tensor cores: 128 features are the M side of the MMA, the rows of x its N side.
 //
-// Eight warps feed: each owns 16 features and turns their codes of 64 rows of W into bf16 values m + s c (one rounding, 2^-9 of
+// Eight warps feed: each owns 16 features and turns their codes of 128 rows of W into bf16 values m + s c (one rounding, 2^-9 of
 // a weight, as in the expansion for the GEMM of more rows), which `tcgen05.st` puts into tensor memory -- a lane's words are
 // the fragment of the 16x256b shape as they lie --, so that weights never pass through shared memory once they are 16 bits
-// wide: writing and reading them there would cost eight times the bytes of the codes.  They also bring x, 64 columns of it at
+// wide: writing and reading them there would cost eight times the bytes of the codes.  They also bring x, 128 columns of it at
 // a time, to shared memory in the order in which the codes run over K.  A ninth warp issues the MMAs.
 // K slices are the CTAs of a cluster; partial sums meet in distributed shared memory in a fixed order.
 //
@@ -27,32 +27,31 @@ struct Int4GemmParams {
   const uint8_t* pairs;    // [n16, groups, 64]
   __nv_bfloat16* y;        // [M, ldy]
   int64_t ldx, ldy;
-  int M, N, K, group_shift;  // rows of W a group, as a power of two of 64
+  int M, N, K, pair_bytes;   // pairs of 16 features and 128 rows of W
   int accumulate, splits;
   int* status;
 };
 
 constexpr int kIgWarps = 8, kIgThreads = 32 * (kIgWarps + 1), kIgFeatures = 16 * kIgWarps;
 constexpr int kIgMaxSplits = 8;
-constexpr int kIgAStages = 4;  // of 64 rows of W in tensor memory: 32 columns
+constexpr int kIgLag = 2;  // stages that the products may be behind
 
+// A stage is 128 rows of W: 64 columns of tensor memory, two 64-column tiles of x, eight warps' codes and pairs.
 template <int BN>
 struct Int4GemmCfg {
-  static constexpr int kRing = BN <= 32 ? 10 : BN <= 64 ? 8 : 9;  // stages in shared memory
-  static constexpr int kLag = 3;                                  // stages that the products may be behind
-  static constexpr int kAhead = kRing - kLag;                     // stages on their way
-  static constexpr int kX = BN * 128, kCodes = 576;               // bytes of a stage; of a warp's codes and pairs in it
-  static constexpr int kStage = kX + kIgWarps * kCodes;
-  static constexpr int kXRing = kRing * kX;
-  static constexpr int kRingBytes = kRing * kStage;
-  static constexpr int kSums = BN * kIgFeatures * 4;              // partial sums overlay the ring
+  static constexpr int kRing = BN <= 16 ? 7 : BN <= 32 ? 6 : BN <= 64 ? 4 : 5;
+  static constexpr int kAhead = kRing - kIgLag;              // stages on their way
+  static constexpr int kX = BN * 128, kCodes = 1024 + 128;   // bytes of a tile of x; of a warp's codes and pairs
+  static constexpr int kXRing = kRing * 2 * kX;
+  static constexpr int kRingBytes = kXRing + kRing * kIgWarps * kCodes;
+  static constexpr int kSums = BN * kIgFeatures * 4;         // partial sums overlay the ring
   static constexpr int kBody = kRingBytes > kSums ? kRingBytes : kSums;
-  static constexpr int kSmem = kBody + 256 + 1024;                // barriers, alignment slack
+  static constexpr int kSmem = kBody + 256 + 1024;           // barriers, alignment slack
   static constexpr int kResident = BN <= 64 ? 2 : 1;
-  static constexpr int kACol = BN <= 64 ? 64 : 128;
-  static constexpr int kTmemCols = 256;
-  static_assert(kACol + kIgAStages * 32 <= kTmemCols && kIgAStages > kLag, "tensor memory");
-  static_assert(kResident * (kSmem + 1024) <= 228 * 1024, "resident CTAs");
+  static constexpr int kACol = BN <= 64 ? 64 : 128, kAStages = BN <= 64 ? 3 : 4;
+  static constexpr int kTmemCols = BN <= 64 ? 256 : 512;
+  static_assert(kACol + kAStages * 64 <= kTmemCols && kAStages > kIgLag, "tensor memory");
+  static_assert(kResident * (kSmem + 1024) <= 228 * 1024 && kResident * kTmemCols <= 512, "resident CTAs");
 };
 
 __device__ __forceinline__ void ig_copy(uint32_t dst, const void* src, bool ok) {
@@ -72,14 +71,20 @@ __device__ __forceinline__ void tmem_st_16x256(uint32_t taddr, const uint32_t (&
       : "memory");
 }
 
-// The codes in bits [4i, 4i + 4) and [16 + 4i, 20 + 4i) as values m + s c: 128 + c by one logic operation, c and the value
-// by one packed operation each.
-__device__ __forceinline__ uint32_t ig_values(uint32_t word, int i, __nv_bfloat162 s, __nv_bfloat162 m) {
-  uint32_t u;
-  asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xEA;" : "=r"(u) : "r"(word >> (4 * i)));
-  const __nv_bfloat162 c = __hsub2(reinterpret_cast<__nv_bfloat162&>(u), __float2bfloat162_rn(128.f));
-  const __nv_bfloat162 v = __hfma2(c, s, m);
-  return reinterpret_cast<const uint32_t&>(v);
+// The four registers of a word's k16 step: codes as denormal bf16 numbers (`int4.cuh`), multiplied by 2^127 (the high nibbles
+// by 2^123) to c / 64, and turned into m + s c by one operation; s0 and s1 carry 64.
+__device__ __forceinline__ void ig_values(uint32_t word, __nv_bfloat162 s0, __nv_bfloat162 m0, __nv_bfloat162 s1,
+                                          __nv_bfloat162 m1, uint32_t* v) {
+  const uint32_t next = word >> 8;
+  const __nv_bfloat162 low = __float2bfloat162_rn(1.7014118346046923e38f), high = __float2bfloat162_rn(1.0633823966279327e37f);
+  auto value = [](uint32_t u, __nv_bfloat162 f, __nv_bfloat162 s, __nv_bfloat162 m) {
+    const __nv_bfloat162 x = __hfma2(__hmul2(reinterpret_cast<__nv_bfloat162&>(u), f), s, m);
+    return reinterpret_cast<const uint32_t&>(x);
+  };
+  v[0] = value(int4_low(word), low, s0, m0);
+  v[1] = value(int4_low(next), low, s0, m0);
+  v[2] = value(int4_high(word), high, s1, m1);
+  v[3] = value(int4_high(next), high, s1, m1);
 }
 
 template <int BN>
@@ -97,8 +102,8 @@ int4_gemm_kernel(Int4GemmParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = static_cast<int>(blockIdx.x) % p.splits;
   const int n0 = static_cast<int>(blockIdx.x) / p.splits * kIgFeatures;
-  const int k64 = (p.K + 127) / 128 * 2, num_kb = (p.K + 63) / 64;
-  const int kb_lo = split * num_kb / p.splits, count = (split + 1) * num_kb / p.splits - kb_lo;
+  const int k128 = (p.K + 127) / 128;
+  const int kb_lo = split * k128 / p.splits, count = (split + 1) * k128 / p.splits - kb_lo;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kRing; ++i) {
@@ -124,97 +129,109 @@ int4_gemm_kernel(Int4GemmParams p) {
     const int tile = n0 / 16 + sub;
     const bool have = tile < (p.N + 15) / 16;
     const uint32_t a_addr = tmem + (static_cast<uint32_t>(sub * 16) << 16) + S::kACol;
-    const uint8_t* codes = p.codes + (static_cast<int64_t>(have ? tile : 0) * k64 + kb_lo) * 512 + lane * 16;
-    const int groups = k64 >> p.group_shift;
-    const uint8_t* pairs = p.pairs + static_cast<int64_t>(have ? tile : 0) * groups * 64 + lane * 16;
+    const int64_t block = static_cast<int64_t>(have ? tile : 0) * k128 + kb_lo;
+    const uint8_t* codes = p.codes + block * 1024 + lane * 16;
+    const int pair_bytes = p.pair_bytes;  // of a stage: 64 or 128
+    const uint8_t* pairs = p.pairs + block * pair_bytes + lane * 16;
+    const bool pair_lane = lane * 16 < pair_bytes;
     const uint32_t own = smem_u32(smem) + S::kXRing + warp * S::kCodes;  // + stage * kIgWarps * kCodes
-    // x: 16-byte pieces (row, i) of a stage, i of 8: columns 16 c + 8 q + 0 .. 7 with c = i / 2, q = i % 2.  Their halves go
-    // to places 4c .. 4c + 3 of the k16 steps 2q and 2q + 1, where the codes of these columns are.
-    constexpr int kPieces = BN * 8, kMine = (kPieces + 255) / 256;
-    const __nv_bfloat16* x_src[kMine];
-    uint32_t x_dst[kMine];
-    int x_left[kMine];  // columns from this piece on, in the whole slice and behind it
-#pragma unroll
-    for (int j = 0; j < kMine; ++j) {
-      const int piece = j * 256 + static_cast<int>(threadIdx.x);
-      const int row = piece >> 3, i = piece & 7, c = i >> 1, q = i & 1;
-      const int unit = 4 * q + (c >> 1);  // of 16 bytes; the second half's is two further
-      x_src[j] = p.x + (row < p.M ? row : 0) * p.ldx + kb_lo * 64 + c * 16 + q * 8;
-      x_dst[j] = smem_u32(smem) + row * 128 + ((unit ^ (row & 7)) << 4) + (c & 1) * 8;
-      x_left[j] = row < p.M && piece < kPieces ? p.K - kb_lo * 64 - c * 16 - q * 8 : 0;
-    }
-    auto load = [&](int it) {
-      const int slot = it % S::kRing;
-      const uint32_t dst = own + slot * (kIgWarps * S::kCodes) + lane * 16;
-      ig_copy(dst, codes + static_cast<int64_t>(it) * 512, have);
-      if (lane < 4) ig_copy(dst + 512, pairs + static_cast<int64_t>((kb_lo + it) >> p.group_shift) * 64, have);
+    // x: 16-byte pieces (row, h, i), tile h of 2 and i of 8: columns 64 h + 16 c + 8 q + 0 .. 7 with c = i / 2, q = i % 2.
+    // Their halves go to places 4c .. 4c + 3 of the k16 steps 2q and 2q + 1, where the codes of these columns are.
+    constexpr int kPieces = BN * 16, kMine = kPieces / 256;
+    const int i8 = threadIdx.x & 7, h = threadIdx.x >> 3 & 1, row0 = threadIdx.x >> 4;  // 16 rows are 256 pieces
+    const int c = i8 >> 1, q = i8 & 1, unit = 4 * q + (c >> 1);  // unit of 16 bytes; the second half's is two further
+    const __nv_bfloat16* x_src = p.x + row0 * p.ldx + static_cast<int64_t>(kb_lo) * 128 + h * 64 + c * 16 + q * 8;
+    int x_left = p.K - kb_lo * 128 - h * 64 - c * 16 - q * 8;    // columns from this piece on
+    const uint32_t x_dst = smem_u32(smem) + h * S::kX + row0 * 128 + ((unit ^ (row0 & 7)) << 4) + (c & 1) * 8;
+    int load_slot = 0;
+    auto load = [&] {  // the next stage
+      const uint32_t dst = own + load_slot * (kIgWarps * S::kCodes) + lane * 16;
+      ig_copy(dst, codes, have);
+      ig_copy(dst + 512, codes + 512, have);
+      if (pair_lane) ig_copy(dst + 1024, pairs, have);
+      codes += 1024;
+      pairs += pair_bytes;
+      const uint32_t at = x_dst + load_slot * (2 * S::kX);
+      const __nv_bfloat16* src = x_src;
 #pragma unroll
       for (int j = 0; j < kMine; ++j) {
-        if (kPieces < 256 && static_cast<int>(threadIdx.x) >= kPieces) break;
-        const bool there = it * 64 < x_left[j];
-        const __nv_bfloat16* src = there ? x_src[j] + it * 64 : p.x;
-        const uint32_t at = x_dst[j] + slot * S::kX;
-        ig_copy8(at, src, there);
-        ig_copy8(at ^ 32, src + 4, there);  // two units further: bit 1 of the unit is 0, swapped or not
+        const bool there = x_left > 0 && row0 + j * 16 < p.M;
+        const __nv_bfloat16* from = there ? src : p.x;
+        ig_copy8(at + j * 2048, from, there);
+        ig_copy8((at ^ 32) + j * 2048, from + 4, there);  // two units further: bit 1 of the unit is 0, swapped or not
+        src += 16 * p.ldx;
       }
+      x_src += 128;
+      x_left -= 128;
+      if (++load_slot == S::kRing) load_slot = 0;
     };
 #pragma unroll 1
     for (int it = 0; it < S::kAhead; ++it) {
-      if (it < count) load(it);
+      if (it < count) load();
       cp_commit();
     }
+    int slot = 0, a_stage = 0, freed = 0;
+    uint32_t freed_phase = 0;
 #pragma unroll 1
     for (int it = 0; it < count; ++it) {
-      // Products up to it - kLag are done: their places in the ring and in tensor memory are free.
-      if (it >= S::kLag) {
-        const int j = it - S::kLag;
-        ok = mbar_wait_warp(&empty_bar[j % S::kRing], (j / S::kRing) & 1, p.status, kStatusWaitTimeoutProducer);
+      // Products up to it - kIgLag are done: their places in the ring and in tensor memory are free.
+      if (it >= kIgLag) {
+        ok = mbar_wait_warp(&empty_bar[freed], freed_phase, p.status, kStatusWaitTimeoutProducer);
         if (!ok) break;
         tc_fence_after_sync();
+        if (++freed == S::kRing) freed = 0, freed_phase ^= 1;
       }
-      if (it + S::kAhead < count) load(it + S::kAhead);
+      if (it + S::kAhead < count) load();
       cp_commit();
       cp_wait_group<S::kAhead>();
       __syncwarp();
-      const uint8_t* unit = smem + S::kXRing + (it % S::kRing) * (kIgWarps * S::kCodes) + warp * S::kCodes;
-      const uint4 w = *reinterpret_cast<const uint4*>(unit + lane * 16);
-      const uint2 u = *reinterpret_cast<const uint2*>(unit + 512 + (lane >> 2) * 8);
-      const __nv_bfloat162 pa = reinterpret_cast<const __nv_bfloat162&>(u.x), pb = reinterpret_cast<const __nv_bfloat162&>(u.y);
-      const __nv_bfloat162 s0 = __low2bfloat162(pa), m0 = __high2bfloat162(pa), s1 = __low2bfloat162(pb), m1 = __high2bfloat162(pb);
-      const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-      uint32_t v[16];
+      const uint8_t* mine = smem + S::kXRing + slot * (kIgWarps * S::kCodes) + warp * S::kCodes;
+      const uint32_t a_stage_addr = a_addr + a_stage * 64;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[4 * j] = ig_values(words[j], 0, s0, m0);
-        v[4 * j + 1] = ig_values(words[j], 2, s0, m0);
-        v[4 * j + 2] = ig_values(words[j], 1, s1, m1);
-        v[4 * j + 3] = ig_values(words[j], 3, s1, m1);
+      for (int half = 0; half < 2; ++half) {
+        const uint4 w = *reinterpret_cast<const uint4*>(mine + half * 512 + lane * 16);
+        const uint2 u = *reinterpret_cast<const uint2*>(mine + 1024 + (pair_bytes == 128 ? half * 64 : 0) + (lane >> 2) * 8);
+        const __nv_bfloat162 pa = reinterpret_cast<const __nv_bfloat162&>(u.x), pb = reinterpret_cast<const __nv_bfloat162&>(u.y);
+        const __nv_bfloat162 up = __float2bfloat162_rn(64.f);
+        const __nv_bfloat162 s0 = __hmul2(__low2bfloat162(pa), up), m0 = __high2bfloat162(pa);
+        const __nv_bfloat162 s1 = __hmul2(__low2bfloat162(pb), up), m1 = __high2bfloat162(pb);
+        uint32_t v[16];
+        ig_values(w.x, s0, m0, s1, m1, v);
+        ig_values(w.y, s0, m0, s1, m1, v + 4);
+        ig_values(w.z, s0, m0, s1, m1, v + 8);
+        ig_values(w.w, s0, m0, s1, m1, v + 12);
+        tmem_st_16x256(a_stage_addr + half * 32, v);
       }
-      tmem_st_16x256(a_addr + it % kIgAStages * 32, v);
       tmem_st_wait();
       fence_proxy_async();  // x
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&full_bar[it % S::kRing]);
+      if (lane == 0) mbar_arrive(&full_bar[slot]);
+      if (++slot == S::kRing) slot = 0;
+      if (++a_stage == S::kAStages) a_stage = 0;
     }
     cp_wait_all();
     if (ok) ok = mbar_wait_warp(done_bar, 0, p.status, kStatusWaitTimeoutEpilogue);
   } else if (elect_one()) {
     constexpr uint32_t idesc = umma_idesc_f16(kIgFeatures, BN, 1, 1, 0, 0);
     bool fed = true;
+    int slot = 0, a_stage = 0;
+    uint32_t phase = 0;
 #pragma unroll 1
     for (int it = 0; it < count; ++it) {
-      if (!mbar_wait(&full_bar[it % S::kRing], (it / S::kRing) & 1, p.status, kStatusWaitTimeoutMma)) {
+      if (!mbar_wait(&full_bar[slot], phase, p.status, kStatusWaitTimeoutMma)) {
         fed = false;
         break;
       }
       tc_fence_after_sync();
-      const uint32_t sx = smem_u32(smem) + it % S::kRing * S::kX;
+      const uint32_t sx = smem_u32(smem) + slot * (2 * S::kX), a = tmem + S::kACol + a_stage * 64;
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        tc_mma_f16_ts(tmem, tmem + S::kACol + it % kIgAStages * 32 + k * 8, umma_smem_desc(sx + k * 32, 16, 1024), idesc,
+      for (int k = 0; k < 8; ++k)
+        tc_mma_f16_ts(tmem, a + k * 8, umma_smem_desc(sx + (k >> 2) * S::kX + (k & 3) * 32, 16, 1024), idesc,
                       it > 0 || k > 0 ? 1u : 0u);
-      tc_commit(&empty_bar[it % S::kRing]);
+      tc_commit(&empty_bar[slot]);
+      if (++slot == S::kRing) slot = 0, phase ^= 1;
+      if (++a_stage == S::kAStages) a_stage = 0;
     }
     if (fed) tc_commit(done_bar);
   }
@@ -303,18 +320,18 @@ static int launch_int4_gemm(const Int4GemmParams& p, cudaStream_t stream) {
 }  // namespace axb
 
 // x [M, K] bf16 with rows of ldx (K, ldx multiples of 8, 16-byte aligned), y [M, N] with rows of ldy; M <= 128.  `splits`:
-// slices of K, up to 8 and one for every 64 rows of W at most.
+// slices of K, up to 8 and one for every 128 rows of W at most.
 extern "C" int axb_int4_gemm(const void* x, const void* codes, const void* pairs, void* y, int M, int N, int K, int group,
                              int64_t ldx, int64_t ldy, int accumulate, int splits, int* status, cudaStream_t stream) {
   using namespace axb;
   const uintptr_t align = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(pairs);
   if (M < 0 || M > 128 || N < 1 || K < 1 || K % 8 || ldx % 8 || (align & 15) || (group != 64 && group != 128) || splits < 1 ||
-      splits > kIgMaxSplits || splits > (K + 63) / 64)
+      splits > kIgMaxSplits || splits > (K + 127) / 128)
     return -10;
   if (M == 0) return 0;
   const Int4GemmParams p{static_cast<const __nv_bfloat16*>(x), static_cast<const uint8_t*>(codes),
                          static_cast<const uint8_t*>(pairs), static_cast<__nv_bfloat16*>(y), ldx, ldy, M, N, K,
-                         group == 64 ? 0 : 1, accumulate, splits, status};
+                         group == 64 ? 128 : 64, accumulate, splits, status};
   if (M <= 16) return launch_int4_gemm<16>(p, stream);
   if (M <= 32) return launch_int4_gemm<32>(p, stream);
   if (M <= 64) return launch_int4_gemm<64>(p, stream);
