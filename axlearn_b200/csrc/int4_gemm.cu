@@ -1,11 +1,11 @@
 // y[M, N] = x[M, K] W (+ y) for up to 128 rows with weights held in 4 bits (layout: int4_linear.cu), on the fifth-generation
 // tensor cores: 128 features are the M side of the MMA, the rows of x its N side.
 //
-// Eight warps feed: each owns 16 features and turns their codes of 128 rows of W into bf16 values m + s c (one rounding, 2^-9 of
-// a weight, as in the expansion for the GEMM of more rows), which `tcgen05.st` puts into tensor memory -- a lane's words are
-// the fragment of the 16x256b shape as they lie --, so that weights never pass through shared memory once they are 16 bits
-// wide: writing and reading them there would cost eight times the bytes of the codes.  They also bring x, 128 columns of it at
-// a time, to shared memory in the order in which the codes run over K.  A ninth warp issues the MMAs.
+// Eight warps feed: each owns 16 features and turns their codes of 128 rows of W into bf16 values m + s c (one rounding, 2^-9
+// of a weight, as in the expansion for the GEMM of more rows), which `tcgen05.st` puts into tensor memory -- a lane's words
+// are the fragment of the 16x256b shape as they lie --, so that weights never pass through shared memory once they are 16
+// bits wide: writing and reading them there would cost eight times the bytes of the codes.  Other warps bring x, 128 columns
+// of it at a time, to shared memory in the order in which the codes run over K, and one issues the MMAs.
 // K slices are the CTAs of a cluster; partial sums meet in distributed shared memory in a fixed order.
 //
 // Launched in the ordinary way in a captured step, too: a successor that started early could hold the tensor memory that a
@@ -27,31 +27,42 @@ struct Int4GemmParams {
   const uint8_t* pairs;    // [n16, groups, 64]
   __nv_bfloat16* y;        // [M, ldy]
   int64_t ldx, ldy;
-  int M, N, K, pair_bytes;   // pairs of 16 features and 128 rows of W
+  int M, N, K;
   int accumulate, splits;
   int* status;
 };
 
-constexpr int kIgWarps = 8, kIgThreads = 32 * (kIgWarps + 1), kIgFeatures = 16 * kIgWarps;
+constexpr int kIgWarps = 8, kIgFeatures = 16 * kIgWarps;
 constexpr int kIgMaxSplits = 8;
-constexpr int kIgLag = 2;  // stages that the products may be behind
 
-// A stage is 128 rows of W: 64 columns of tensor memory, two 64-column tiles of x, eight warps' codes and pairs.
+// A stage is 128 rows of W: 64 columns of tensor memory, two 64-column tiles of x, eight warps' codes and pairs.  Codes, on
+// their way from memory, have the deepest ring; x comes from the L2.
 template <int BN>
 struct Int4GemmCfg {
-  static constexpr int kRing = BN <= 16 ? 7 : BN <= 32 ? 6 : BN <= 64 ? 4 : 5;
-  static constexpr int kAhead = kRing - kIgLag;              // stages on their way
+  static constexpr int kXRing = BN == 64 ? 3 : 4;            // each place has a warp of its own
+  static constexpr int kThreads = 32 * (kIgWarps + kXRing + 1);
+  static constexpr int kCodeRing = BN <= 16 ? 9 : BN <= 32 ? 7 : BN <= 64 ? 6 : 8;
   static constexpr int kX = BN * 128, kCodes = 1024 + 128;   // bytes of a tile of x; of a warp's codes and pairs
-  static constexpr int kXRing = kRing * 2 * kX;
-  static constexpr int kRingBytes = kXRing + kRing * kIgWarps * kCodes;
-  static constexpr int kSums = BN * kIgFeatures * 4;         // partial sums overlay the ring
+  static constexpr int kXBytes = kXRing * 2 * kX;
+  static constexpr int kRingBytes = kXBytes + kCodeRing * kIgWarps * kCodes;
+  static constexpr int kSums = BN * kIgFeatures * 4;         // partial sums overlay the rings
   static constexpr int kBody = kRingBytes > kSums ? kRingBytes : kSums;
   static constexpr int kSmem = kBody + 256 + 1024;           // barriers, alignment slack
   static constexpr int kResident = BN <= 64 ? 2 : 1;
-  static constexpr int kACol = BN <= 64 ? 64 : 128, kAStages = BN <= 64 ? 3 : 4;
+  static constexpr int kACol = BN <= 64 ? 64 : 128, kARing = BN <= 64 ? 3 : 4;
   static constexpr int kTmemCols = BN <= 64 ? 256 : 512;
-  static_assert(kACol + kAStages * 64 <= kTmemCols && kAStages > kIgLag, "tensor memory");
+  static_assert(kACol + kARing * 64 <= kTmemCols, "tensor memory");
   static_assert(kResident * (kSmem + 1024) <= 228 * 1024 && kResident * kTmemCols <= 512, "resident CTAs");
+};
+
+// Slot and phase of a ring.
+template <int N>
+struct IgPlace {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == N) slot = 0, phase ^= 1;
+  }
 };
 
 __device__ __forceinline__ void ig_copy(uint32_t dst, const void* src, bool ok) {
@@ -71,32 +82,38 @@ __device__ __forceinline__ void tmem_st_16x256(uint32_t taddr, const uint32_t (&
       : "memory");
 }
 
-// The four registers of a word's k16 step: codes as denormal bf16 numbers (`int4.cuh`), multiplied by 2^127 (the high nibbles
-// by 2^123) to c / 64, and turned into m + s c by one operation; s0 and s1 carry 64.
+// The four registers of a word's k16 step: codes as denormal bf16 numbers (`int4.cuh`; the high nibbles are 16 times theirs),
+// turned into 2^-kIgDown (m + s c) by one operation.  s0 (s1) carries 2^(133 - kIgDown) (a sixteenth of it), m0 and m1
+// 2^-kIgDown, so that neither steps up to 2^31 nor values down to 2^-89 leave the range of bf16.
+constexpr int kIgDown = 37;
+constexpr float kIgStep = 79228162514264337593543950336.f, kIgLow = 1.f / 137438953472.f;  // 2^(133 - kIgDown), 2^-kIgDown
+
 __device__ __forceinline__ void ig_values(uint32_t word, __nv_bfloat162 s0, __nv_bfloat162 m0, __nv_bfloat162 s1,
                                           __nv_bfloat162 m1, uint32_t* v) {
   const uint32_t next = word >> 8;
-  const __nv_bfloat162 low = __float2bfloat162_rn(1.7014118346046923e38f), high = __float2bfloat162_rn(1.0633823966279327e37f);
-  auto value = [](uint32_t u, __nv_bfloat162 f, __nv_bfloat162 s, __nv_bfloat162 m) {
-    const __nv_bfloat162 x = __hfma2(__hmul2(reinterpret_cast<__nv_bfloat162&>(u), f), s, m);
+  auto value = [](uint32_t u, __nv_bfloat162 s, __nv_bfloat162 m) {
+    const __nv_bfloat162 x = __hfma2(reinterpret_cast<__nv_bfloat162&>(u), s, m);
     return reinterpret_cast<const uint32_t&>(x);
   };
-  v[0] = value(int4_low(word), low, s0, m0);
-  v[1] = value(int4_low(next), low, s0, m0);
-  v[2] = value(int4_high(word), high, s1, m1);
-  v[3] = value(int4_high(next), high, s1, m1);
+  v[0] = value(int4_low(word), s0, m0);
+  v[1] = value(int4_low(next), s0, m0);
+  v[2] = value(int4_high(word), s1, m1);
+  v[3] = value(int4_high(next), s1, m1);
 }
 
-template <int BN>
-__global__ void __launch_bounds__(kIgThreads, Int4GemmCfg<BN>::kResident)
+// kGroup: 64 or 128.
+template <int BN, int kGroup>
+__global__ void __launch_bounds__(Int4GemmCfg<BN>::kThreads, Int4GemmCfg<BN>::kResident)
 int4_gemm_kernel(Int4GemmParams p) {
   using S = Int4GemmCfg<BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem =
       reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S::kBody);
-  uint64_t* empty_bar = full_bar + S::kRing;
-  uint64_t* done_bar = empty_bar + S::kRing;
+  uint64_t* x_full = reinterpret_cast<uint64_t*>(smem + S::kBody);
+  uint64_t* x_empty = x_full + S::kXRing;
+  uint64_t* a_full = x_empty + S::kXRing;
+  uint64_t* a_empty = a_full + S::kARing;
+  uint64_t* done_bar = a_empty + S::kARing;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -106,14 +123,19 @@ int4_gemm_kernel(Int4GemmParams p) {
   const int kb_lo = split * k128 / p.splits, count = (split + 1) * k128 / p.splits - kb_lo;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < S::kRing; ++i) {
-      mbar_init(&full_bar[i], kIgWarps);
-      mbar_init(&empty_bar[i], 1);
+    for (int i = 0; i < S::kXRing; ++i) {
+      mbar_init(&x_full[i], 1);
+      mbar_init(&x_empty[i], 1);
+    }
+    for (int i = 0; i < S::kARing; ++i) {
+      mbar_init(&a_full[i], kIgWarps);
+      mbar_init(&a_empty[i], 1);
     }
     mbar_init(done_bar, 1);
     fence_barrier_init();
   }
-  if (warp == kIgWarps) {
+  constexpr int kMmaWarp = kIgWarps + S::kXRing;
+  if (warp == kMmaWarp) {
     tmem_alloc(tmem_slot, S::kTmemCols);
     tmem_relinquish();
   }
@@ -131,70 +153,50 @@ int4_gemm_kernel(Int4GemmParams p) {
     const uint32_t a_addr = tmem + (static_cast<uint32_t>(sub * 16) << 16) + S::kACol;
     const int64_t block = static_cast<int64_t>(have ? tile : 0) * k128 + kb_lo;
     const uint8_t* codes = p.codes + block * 1024 + lane * 16;
-    const int pair_bytes = p.pair_bytes;  // of a stage: 64 or 128
-    const uint8_t* pairs = p.pairs + block * pair_bytes + lane * 16;
-    const bool pair_lane = lane * 16 < pair_bytes;
-    const uint32_t own = smem_u32(smem) + S::kXRing + warp * S::kCodes;  // + stage * kIgWarps * kCodes
-    // x: 16-byte pieces (row, h, i), tile h of 2 and i of 8: columns 64 h + 16 c + 8 q + 0 .. 7 with c = i / 2, q = i % 2.
-    // Their halves go to places 4c .. 4c + 3 of the k16 steps 2q and 2q + 1, where the codes of these columns are.
-    constexpr int kPieces = BN * 16, kMine = kPieces / 256;
-    const int i8 = threadIdx.x & 7, h = threadIdx.x >> 3 & 1, row0 = threadIdx.x >> 4;  // 16 rows are 256 pieces
-    const int c = i8 >> 1, q = i8 & 1, unit = 4 * q + (c >> 1);  // unit of 16 bytes; the second half's is two further
-    const __nv_bfloat16* x_src = p.x + row0 * p.ldx + static_cast<int64_t>(kb_lo) * 128 + h * 64 + c * 16 + q * 8;
-    int x_left = p.K - kb_lo * 128 - h * 64 - c * 16 - q * 8;    // columns from this piece on
-    const uint32_t x_dst = smem_u32(smem) + h * S::kX + row0 * 128 + ((unit ^ (row0 & 7)) << 4) + (c & 1) * 8;
-    int load_slot = 0;
+    constexpr int kPairBytes = kGroup == 64 ? 128 : 64;  // of a stage
+    const uint8_t* pairs = p.pairs + block * kPairBytes + lane * 16;
+    constexpr int kStride = kIgWarps * S::kCodes;        // of a stage in the ring
+    const uint8_t* own = smem + S::kXBytes + warp * S::kCodes;
+    const uint32_t dst0 = smem_u32(own) + lane * 16;
+    uint32_t dst = dst0;
     auto load = [&] {  // the next stage
-      const uint32_t dst = own + load_slot * (kIgWarps * S::kCodes) + lane * 16;
       ig_copy(dst, codes, have);
       ig_copy(dst + 512, codes + 512, have);
-      if (pair_lane) ig_copy(dst + 1024, pairs, have);
+      if (lane * 16 < kPairBytes) ig_copy(dst + 1024, pairs, have);
       codes += 1024;
-      pairs += pair_bytes;
-      const uint32_t at = x_dst + load_slot * (2 * S::kX);
-      const __nv_bfloat16* src = x_src;
-#pragma unroll
-      for (int j = 0; j < kMine; ++j) {
-        const bool there = x_left > 0 && row0 + j * 16 < p.M;
-        const __nv_bfloat16* from = there ? src : p.x;
-        ig_copy8(at + j * 2048, from, there);
-        ig_copy8((at ^ 32) + j * 2048, from + 4, there);  // two units further: bit 1 of the unit is 0, swapped or not
-        src += 16 * p.ldx;
-      }
-      x_src += 128;
-      x_left -= 128;
-      if (++load_slot == S::kRing) load_slot = 0;
+      pairs += kPairBytes;
+      dst += kStride;
+      if (dst == dst0 + S::kCodeRing * kStride) dst = dst0;
     };
 #pragma unroll 1
-    for (int it = 0; it < S::kAhead; ++it) {
+    for (int it = 0; it < S::kCodeRing; ++it) {
       if (it < count) load();
       cp_commit();
     }
-    int slot = 0, a_stage = 0, freed = 0;
-    uint32_t freed_phase = 0;
+    IgPlace<S::kCodeRing> code;
+    IgPlace<S::kARing> a;
 #pragma unroll 1
     for (int it = 0; it < count; ++it) {
-      // Products up to it - kIgLag are done: their places in the ring and in tensor memory are free.
-      if (it >= kIgLag) {
-        ok = mbar_wait_warp(&empty_bar[freed], freed_phase, p.status, kStatusWaitTimeoutProducer);
+      if (it >= S::kARing) {
+        ok = mbar_wait_warp(&a_empty[a.slot], a.phase ^ 1, p.status, kStatusWaitTimeoutProducer);
         if (!ok) break;
         tc_fence_after_sync();
-        if (++freed == S::kRing) freed = 0, freed_phase ^= 1;
       }
-      if (it + S::kAhead < count) load();
-      cp_commit();
-      cp_wait_group<S::kAhead>();
+      cp_wait_group<S::kCodeRing - 1>();
       __syncwarp();
-      const uint8_t* mine = smem + S::kXRing + slot * (kIgWarps * S::kCodes) + warp * S::kCodes;
-      const uint32_t a_stage_addr = a_addr + a_stage * 64;
+      const uint8_t* mine = own + code.slot * kStride;
+      const uint32_t a_stage_addr = a_addr + a.slot * 64;
+      __nv_bfloat162 s0, m0, s1, m1;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const uint4 w = *reinterpret_cast<const uint4*>(mine + half * 512 + lane * 16);
-        const uint2 u = *reinterpret_cast<const uint2*>(mine + 1024 + (pair_bytes == 128 ? half * 64 : 0) + (lane >> 2) * 8);
-        const __nv_bfloat162 pa = reinterpret_cast<const __nv_bfloat162&>(u.x), pb = reinterpret_cast<const __nv_bfloat162&>(u.y);
-        const __nv_bfloat162 up = __float2bfloat162_rn(64.f);
-        const __nv_bfloat162 s0 = __hmul2(__low2bfloat162(pa), up), m0 = __high2bfloat162(pa);
-        const __nv_bfloat162 s1 = __hmul2(__low2bfloat162(pb), up), m1 = __high2bfloat162(pb);
+        if (half == 0 || kGroup == 64) {
+          const uint2 u = *reinterpret_cast<const uint2*>(mine + 1024 + half * 64 + (lane >> 2) * 8);
+          const __nv_bfloat162 pa = reinterpret_cast<const __nv_bfloat162&>(u.x), pb = reinterpret_cast<const __nv_bfloat162&>(u.y);
+          const __nv_bfloat162 low = __float2bfloat162_rn(kIgLow);
+          s0 = __hmul2(__low2bfloat162(pa), __float2bfloat162_rn(kIgStep)), m0 = __hmul2(__high2bfloat162(pa), low);
+          s1 = __hmul2(__low2bfloat162(pb), __float2bfloat162_rn(kIgStep / 16.f)), m1 = __hmul2(__high2bfloat162(pb), low);
+        }
         uint32_t v[16];
         ig_values(w.x, s0, m0, s1, m1, v);
         ig_values(w.y, s0, m0, s1, m1, v + 4);
@@ -203,35 +205,77 @@ int4_gemm_kernel(Int4GemmParams p) {
         tmem_st_16x256(a_stage_addr + half * 32, v);
       }
       tmem_st_wait();
-      fence_proxy_async();  // x
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&full_bar[slot]);
-      if (++slot == S::kRing) slot = 0;
-      if (++a_stage == S::kAStages) a_stage = 0;
+      if (lane == 0) mbar_arrive(&a_full[a.slot]);
+      if (it + S::kCodeRing < count) load();  // into the place that has been read
+      cp_commit();
+      code.next();
+      a.next();
     }
     cp_wait_all();
     if (ok) ok = mbar_wait_warp(done_bar, 0, p.status, kStatusWaitTimeoutEpilogue);
+  } else if (warp < kMmaWarp) {
+    // x: 16-byte pieces (row, h, i), tile h of 2 and i of 8: columns 64 h + 16 c + 8 q + 0 .. 7 with c = i / 2, q = i % 2.
+    // Their halves go to places 4c .. 4c + 3 of the k16 steps 2q and 2q + 1, where the codes of these columns are.  A warp fills
+    // one place of the ring, a lane the pieces (h, i) of every second row.
+    constexpr int kMine = BN / 2;
+    const int place = warp - kIgWarps;
+    const int i = lane & 7, h = lane >> 3 & 1, row0 = lane >> 4;
+    const int c = i >> 1, q = i & 1, unit = 4 * q + (c >> 1);  // of 16 bytes; the second half's is two further
+    const int column = (kb_lo + place) * 128 + h * 64 + c * 16 + q * 8;
+    const __nv_bfloat16* src = p.x + row0 * p.ldx + column;
+    int left = p.K - column;                                   // columns from this piece on
+    const int rows = min(kMine, (p.M - row0 + 1) / 2);         // of this lane
+    const uint32_t at = smem_u32(smem) + place * (2 * S::kX) + h * S::kX + row0 * 128 + (c & 1) * 8;
+    uint32_t phase = 1;
+#pragma unroll 1
+    for (int it = place; it < count; it += S::kXRing) {
+      if (it >= S::kXRing) {
+        ok = mbar_wait_warp(&x_empty[place], phase, p.status, kStatusWaitTimeoutProducer);
+        if (!ok) break;
+      }
+      phase ^= 1;
+      const int there = left > 0 ? rows : 0;
+      const __nv_bfloat16* from = src;
+#pragma unroll 8
+      for (int j = 0; j < kMine; ++j) {
+        // Rows of the lane are two apart: the swizzle takes the row mod 8.
+        const uint32_t to = at + j * 256 + ((unit ^ ((row0 + 2 * j) & 7)) << 4);
+        const __nv_bfloat16* piece = j < there ? from : p.x;
+        ig_copy8(to, piece, j < there);
+        ig_copy8(to ^ 32, piece + 4, j < there);  // two units further: bit 1 of the unit is 0, swapped or not
+        from += 2 * p.ldx;
+      }
+      src += S::kXRing * 128;
+      left -= S::kXRing * 128;
+      cp_wait_all();
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&x_full[place]);
+    }
   } else if (elect_one()) {
     constexpr uint32_t idesc = umma_idesc_f16(kIgFeatures, BN, 1, 1, 0, 0);
     bool fed = true;
-    int slot = 0, a_stage = 0;
-    uint32_t phase = 0;
+    IgPlace<S::kXRing> x;
+    IgPlace<S::kARing> a;
 #pragma unroll 1
     for (int it = 0; it < count; ++it) {
-      if (!mbar_wait(&full_bar[slot], phase, p.status, kStatusWaitTimeoutMma)) {
+      if (!mbar_wait(&x_full[x.slot], x.phase, p.status, kStatusWaitTimeoutMma) ||
+          !mbar_wait(&a_full[a.slot], a.phase, p.status, kStatusWaitTimeoutMma)) {
         fed = false;
         break;
       }
       tc_fence_after_sync();
-      const uint32_t sx = smem_u32(smem) + slot * (2 * S::kX), a = tmem + S::kACol + a_stage * 64;
+      const uint32_t sx = smem_u32(smem) + x.slot * (2 * S::kX), sa = tmem + S::kACol + a.slot * 64;
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        tc_mma_f16_ts(tmem, a + k * 8, umma_smem_desc(sx + (k >> 2) * S::kX + (k & 3) * 32, 16, 1024), idesc,
+        tc_mma_f16_ts(tmem, sa + k * 8, umma_smem_desc(sx + (k >> 2) * S::kX + (k & 3) * 32, 16, 1024), idesc,
                       it > 0 || k > 0 ? 1u : 0u);
-      tc_commit(&empty_bar[slot]);
-      if (++slot == S::kRing) slot = 0, phase ^= 1;
-      if (++a_stage == S::kAStages) a_stage = 0;
+      tc_commit(&x_empty[x.slot]);
+      tc_commit(&a_empty[a.slot]);
+      x.next();
+      a.next();
     }
     if (fed) tc_commit(done_bar);
   }
@@ -257,7 +301,7 @@ int4_gemm_kernel(Int4GemmParams p) {
         if (kStep == 8 && (j >> 3) != (c0 >> 3 & 1)) continue;
         const int row = (kStep == 16 ? c0 : (c0 & ~15)) + j;
         if (row >= p.M) continue;
-        float v = __uint_as_float(r[j]);
+        float v = __uint_as_float(r[j]) * (1.f / kIgLow);
         if (p.splits > 1) {
           part[row * kIgFeatures + feature] = v;
         } else if (n < p.N) {
@@ -288,7 +332,7 @@ int4_gemm_kernel(Int4GemmParams p) {
   }
   tc_fence_before_sync();
   const int gave_up = __syncthreads_or(!ok);
-  if (warp == kIgWarps) {
+  if (warp == kMmaWarp) {
     if (gave_up) {
       // A wait gave up: let what may still be in flight land before the CTA exits.
       for (int i = 0; i < 2000; ++i) __nanosleep(1000);
@@ -298,10 +342,10 @@ int4_gemm_kernel(Int4GemmParams p) {
   }
 }
 
-template <int BN>
+template <int BN, int kGroup>
 static int launch_int4_gemm(const Int4GemmParams& p, cudaStream_t stream) {
   using S = Int4GemmCfg<BN>;
-  constexpr auto kernel = int4_gemm_kernel<BN>;
+  constexpr auto kernel = int4_gemm_kernel<BN, kGroup>;
   static OptIn opt_in;
   if (!opt_in.done(kernel, S::kSmem)) return -3;
   cudaLaunchAttribute attr[1];
@@ -309,12 +353,20 @@ static int launch_int4_gemm(const Int4GemmParams& p, cudaStream_t stream) {
   attr[0].val.clusterDim = {static_cast<unsigned>(p.splits), 1, 1};
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((p.N + kIgFeatures - 1) / kIgFeatures * p.splits));
-  cfg.blockDim = dim3(kIgThreads);
+  cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? 0 : -4;
+}
+
+template <int kGroup>
+static int int4_gemm(const Int4GemmParams& p, cudaStream_t stream) {
+  if (p.M <= 16) return launch_int4_gemm<16, kGroup>(p, stream);
+  if (p.M <= 32) return launch_int4_gemm<32, kGroup>(p, stream);
+  if (p.M <= 64) return launch_int4_gemm<64, kGroup>(p, stream);
+  return launch_int4_gemm<128, kGroup>(p, stream);
 }
 
 }  // namespace axb
@@ -331,9 +383,6 @@ extern "C" int axb_int4_gemm(const void* x, const void* codes, const void* pairs
   if (M == 0) return 0;
   const Int4GemmParams p{static_cast<const __nv_bfloat16*>(x), static_cast<const uint8_t*>(codes),
                          static_cast<const uint8_t*>(pairs), static_cast<__nv_bfloat16*>(y), ldx, ldy, M, N, K,
-                         group == 64 ? 128 : 64, accumulate, splits, status};
-  if (M <= 16) return launch_int4_gemm<16>(p, stream);
-  if (M <= 32) return launch_int4_gemm<32>(p, stream);
-  if (M <= 64) return launch_int4_gemm<64>(p, stream);
-  return launch_int4_gemm<128>(p, stream);
+                         accumulate, splits, status};
+  return group == 64 ? int4_gemm<64>(p, stream) : int4_gemm<128>(p, stream);
 }
