@@ -20,6 +20,19 @@ struct Int4Pool {
   uint32_t* pairs;
 };
 
+// n / d for n below 2^31.
+struct FastDiv {
+  uint32_t d, mul, shift;
+  FastDiv() = default;
+  explicit FastDiv(int by) : d(static_cast<uint32_t>(by)), shift(31) {
+    while ((uint64_t{1} << (shift - 31)) < d) ++shift;
+    mul = static_cast<uint32_t>(((uint64_t{1} << shift) + d - 1) / d);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const {
+    return static_cast<uint32_t>((static_cast<uint64_t>(n) * mul) >> shift);
+  }
+};
+
 // Rows of heads in: element strides of (sequence, token, head); dims are neighbours.
 struct HeadRows {
   const __nv_bfloat16* x;
@@ -36,12 +49,19 @@ struct Int4AppendParams {
   const int* live;      // null: all tokens
   const float2* angle;  // (sin, cos) of [position][H / 2], null: nothing is rotated
   int* status;
-  int angle_rows;
-  int B, T, num_q_heads, num_kv_heads, page_size, max_pages, num_pages;
+  FastDiv heads, tokens, page;  // units of a token, tokens of a sequence, positions of a page
+  uint32_t units;
+  int angle_rows, num_q_heads, num_kv_heads, max_pages, num_pages;
 };
 
-// The eight dims 8 l .. 8 l + 7 of a lane, groups of 32 dims are four neighbouring lanes: codes (dim i in bits 4 i) and pair.
-__device__ __forceinline__ uint32_t quantize8(const uint4& x, uint32_t& pair) {
+// The eight dims 8 l .. 8 l + 7 of a lane, groups of 32 dims are four neighbouring lanes: codes (dim i in bits 4 i), pair and the
+// codes as floats.
+//
+// Level d / s to the nearest, ties to even.  A product with the reciprocal is within 2^-22 of the quotient, so its rounding is
+// right unless it ends next to a half; there (one warp in forty on normal values) d - c s, which is exact (c s has 12 bits),
+// tells whether a neighbour is nearer.  That is the rounding of the 32-bit quotient, too: a d that is not (k + 1/2) s is off
+// it by more than half a unit of the quotient.  No level passes 15: s is at least 1 - 2^-8 of a fifteenth of the range.
+__device__ __forceinline__ uint32_t quantize8(const uint4& x, uint32_t& pair, float (&level)[8]) {
   const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&x);
   __nv_bfloat162 lo2 = __hmin2_nan(__hmin2_nan(h[0], h[1]), __hmin2_nan(h[2], h[3]));
   __nv_bfloat162 hi2 = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
@@ -55,27 +75,42 @@ __device__ __forceinline__ uint32_t quantize8(const uint4& x, uint32_t& pair) {
   const bool good = range <= FLT_MAX;  // neither NaN nor an infinity nor an overflow
   float s = __bfloat162float(__float2bfloat16(range * (1.f / 15.f)));
   if (!good || s < FLT_MIN) s = 0.f;
-  const uint32_t m_bits = good ? __float_as_uint(lo) : 0x7fff0000u;
-  pair = (__float_as_uint(s) >> 16) | m_bits;
-  if (s == 0.f) return 0;
-  uint32_t codes = 0;
+  pair = (__float_as_uint(s) >> 16) | (good ? __float_as_uint(lo) : 0x7fff0000u);
+  const float inverse = s == 0.f ? 0.f : __frcp_rn(s);
+  constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: whole numbers are the last bits
+  float off_by = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __bfloat1622float2(h[i]);
-    const float a = rintf(__fdiv_rn(f.x - lo, s)), b = rintf(__fdiv_rn(f.y - lo, s));
-    codes |= static_cast<uint32_t>(fminf(fmaxf(a, 0.f), 15.f)) << (8 * i);
-    codes |= static_cast<uint32_t>(fminf(fmaxf(b, 0.f), 15.f)) << (8 * i + 4);
+  for (int i = 0; i < 8; ++i) {
+    const float2 f = __bfloat1622float2(h[i >> 1]);
+    const float t = ((i & 1 ? f.y : f.x) - lo) * inverse;
+    level[i] = (t + kWhole) - kWhole;
+    off_by = fmaxf(off_by, fabsf(t - level[i]));
   }
-  return codes;
+  if (__any_sync(0xffffffffu, off_by > 0.5f - 0x1p-16f)) {
+    const float half = 0.5f * s;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 f = __bfloat1622float2(h[i >> 1]);
+      const float rest = fmaf(-level[i], s, (i & 1 ? f.y : f.x) - lo);
+      const bool odd = static_cast<int>(level[i]) & 1;
+      if (rest > half || (rest == half && odd)) level[i] += 1.f;
+      if (rest < -half || (rest == -half && odd)) level[i] -= 1.f;
+    }
+  }
+  if (s == 0.f) {  // (a NaN among the values is one among the levels)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) level[i] = 0.f;
+  }
+  const float a = fmaf(level[3], 4096.f, fmaf(level[2], 256.f, fmaf(level[1], 16.f, level[0])));
+  const float b = fmaf(level[7], 4096.f, fmaf(level[6], 256.f, fmaf(level[5], 16.f, level[4])));
+  return __byte_perm(__float_as_uint(a + kWhole), __float_as_uint(b + kWhole), 0x5410);
 }
 
-__device__ __forceinline__ uint4 values8(uint32_t codes, uint32_t pair) {
+__device__ __forceinline__ uint4 values8(const float (&level)[8], uint32_t pair) {
   const float s = pair_s(pair), m = pair_m(pair);
   uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w[i] = pack2(fmaf(s, static_cast<float>((codes >> (8 * i)) & 15u), m),
-                 fmaf(s, static_cast<float>((codes >> (8 * i + 4)) & 15u), m));
+  for (int i = 0; i < 4; ++i) w[i] = pack2(fmaf(s, level[2 * i], m), fmaf(s, level[2 * i + 1], m));
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
@@ -104,49 +139,69 @@ static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 constexpr int kAppendThreads = 256;
 
-// A row of H values (one head of one token) is H / 8 lanes of 16 bytes; rows run over heads (q, k, v), tokens, sequences.
+// A unit is the key and the value of a KV head of one token, or two of its query heads to be rotated: H / 8 lanes with 16 bytes
+// of either row.  Units run over heads (KV, then pairs of q), tokens, sequences.  The pass is bound by its instructions: where
+// a row goes is found once for both, and nothing is quantised behind `live`.
 template <int H>
 __global__ void __launch_bounds__(kAppendThreads)
 int4_append_kernel(Int4AppendParams p) {
   chain_link();
-  constexpr int kLanes = H / 8, kRows = kAppendThreads / kLanes;
+  constexpr int kLanes = H / 8, kUnits = kAppendThreads / kLanes;
   const int lane = threadIdx.x % kLanes;
-  const int heads = p.num_q_heads + 2 * p.num_kv_heads;
-  const int64_t rows = static_cast<int64_t>(p.B) * p.T * heads;
-  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRows; row0 < rows; row0 += static_cast<int64_t>(gridDim.x) * kRows) {
-    const int64_t row = row0 + threadIdx.x / kLanes;  // (shuffles: all lanes stay)
-    const bool inside = row < rows;
-    const int64_t token = inside ? row / heads : 0;
-    const int head = inside ? static_cast<int>(row - token * heads) : 0;
-    const int b = static_cast<int>(token / p.T), t = static_cast<int>(token - static_cast<int64_t>(b) * p.T);
-    const int pos = (p.start == nullptr ? 0 : p.start[b]) + t;
+  const uint4 zeros = make_uint4(0, 0, 0, 0);
+  for (uint32_t unit0 = blockIdx.x * kUnits; unit0 < p.units; unit0 += gridDim.x * kUnits) {
+    const uint32_t unit = unit0 + threadIdx.x / kLanes;  // (shuffles: all lanes stay)
+    const bool inside = unit < p.units;
+    const uint32_t token = inside ? p.heads.div(unit) : 0;
+    int head = inside ? static_cast<int>(unit - token * p.heads.d) : 0;
+    const int b = static_cast<int>(p.tokens.div(token)), t = static_cast<int>(token - b * p.tokens.d);
     const bool live = inside && (p.live == nullptr || t < p.live[b]);
-    const bool is_q = head < p.num_q_heads, is_v = head >= p.num_q_heads + p.num_kv_heads;
-    const int kvh = is_v ? head - p.num_q_heads - p.num_kv_heads : head - p.num_q_heads;
-    const HeadRows& src = is_q ? p.q : is_v ? p.v : p.k;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (live) x = *reinterpret_cast<const uint4*>(src.x + b * src.b + t * src.t + (is_q ? head : kvh) * src.h + lane * 8);
-    if (live && !is_v && p.angle != nullptr) {
-      if (pos >= 0 && pos < p.angle_rows)
-        x = rotate8(x, p.angle + static_cast<int64_t>(pos) * (H / 2) + lane * 4);
-      else
-        int4_report(p.status);
-    }
-    uint32_t pair;
-    const uint32_t codes = quantize8(x, pair);
-    int byte;
-    const uint32_t word = row_word<H>(codes, lane, byte);
-    if (!inside) continue;
-    if (is_q) {
-      if (live) *reinterpret_cast<uint4*>(p.q_out + b * p.out_b + t * p.out_t + head * p.out_h + lane * 8) = x;
+    const bool is_q = head >= p.num_kv_heads;
+    const int64_t out_at = b * p.out_b + t * p.out_t + lane * 8;
+    if (!__any_sync(0xffffffffu, live)) {
+      if (inside && !is_q && p.k_out != nullptr) {
+        *reinterpret_cast<uint4*>(p.k_out + out_at + head * p.out_h) = zeros;
+        *reinterpret_cast<uint4*>(p.v_out + out_at + head * p.out_h) = zeros;
+      }
       continue;
     }
-    __nv_bfloat16* out = is_v ? p.v_out : p.k_out;
-    if (out != nullptr)
-      *reinterpret_cast<uint4*>(out + b * p.out_b + t * p.out_t + kvh * p.out_h + lane * 8) =
-          live ? values8(codes, pair) : make_uint4(0, 0, 0, 0);
-    if (!live) continue;
-    const int col = pos / p.page_size;
+    uint4 x0 = zeros, x1 = zeros;
+    if (is_q) head = 2 * (head - p.num_kv_heads);
+    const bool pair_of_q = is_q && head + 1 < p.num_q_heads;
+    if (live) {
+      const HeadRows& first = is_q ? p.q : p.k;
+      x0 = *reinterpret_cast<const uint4*>(first.x + b * first.b + t * first.t + head * first.h + lane * 8);
+      const HeadRows& second = is_q ? p.q : p.v;
+      if (!is_q || pair_of_q)
+        x1 = *reinterpret_cast<const uint4*>(second.x + b * second.b + t * second.t + (head + is_q) * second.h + lane * 8);
+    }
+    const int pos = (p.start == nullptr ? 0 : p.start[b]) + t;
+    if (live && p.angle != nullptr) {
+      if (pos >= 0 && pos < p.angle_rows) {
+        const float2* angle = p.angle + static_cast<int64_t>(pos) * (H / 2) + lane * 4;
+        x0 = rotate8(x0, angle);
+        if (is_q) x1 = rotate8(x1, angle);
+      } else {
+        int4_report(p.status);
+      }
+    }
+    if (is_q && live) {
+      *reinterpret_cast<uint4*>(p.q_out + out_at + head * p.out_h) = x0;
+      if (pair_of_q) *reinterpret_cast<uint4*>(p.q_out + out_at + (head + 1) * p.out_h) = x1;
+    }
+    const bool quantised = live && !is_q;
+    if (!__any_sync(0xffffffffu, quantised)) continue;
+    uint32_t k_pair, v_pair;
+    float k_level[8], v_level[8];
+    int byte;
+    const uint32_t k_word = row_word<H>(quantize8(x0, k_pair, k_level), lane, byte);
+    const uint32_t v_word = row_word<H>(quantize8(x1, v_pair, v_level), lane, byte);
+    if (inside && !is_q && p.k_out != nullptr) {
+      *reinterpret_cast<uint4*>(p.k_out + out_at + head * p.out_h) = live ? values8(k_level, k_pair) : zeros;
+      *reinterpret_cast<uint4*>(p.v_out + out_at + head * p.out_h) = live ? values8(v_level, v_pair) : zeros;
+    }
+    if (!quantised) continue;
+    const int col = static_cast<int>(p.page.div(static_cast<uint32_t>(max(pos, 0))));
     if (pos < 0 || col >= p.max_pages) {
       int4_report(p.status);
       continue;
@@ -156,10 +211,14 @@ int4_append_kernel(Int4AppendParams p) {
       int4_report(p.status);
       continue;
     }
-    const int64_t slot = (static_cast<int64_t>(page) * p.num_kv_heads + kvh) * p.page_size + (pos - col * p.page_size);
-    const Int4Pool& pool = is_v ? p.v_pool : p.k_pool;
-    *reinterpret_cast<uint32_t*>(pool.codes + slot * (H / 2) + byte) = word;
-    if ((lane & 3) == 0) pool.pairs[slot * (H / kInt4Group) + (lane >> 2)] = pair;
+    const int page_size = static_cast<int>(p.page.d);
+    const int64_t slot = (static_cast<int64_t>(page) * p.num_kv_heads + head) * page_size + (pos - col * page_size);
+    *reinterpret_cast<uint32_t*>(p.k_pool.codes + slot * (H / 2) + byte) = k_word;
+    *reinterpret_cast<uint32_t*>(p.v_pool.codes + slot * (H / 2) + byte) = v_word;
+    if ((lane & 3) == 0) {
+      p.k_pool.pairs[slot * (H / kInt4Group) + (lane >> 2)] = k_pair;
+      p.v_pool.pairs[slot * (H / kInt4Group) + (lane >> 2)] = v_pair;
+    }
   }
 }
 
@@ -361,7 +420,8 @@ int4_attn_kernel(Int4AttnParams p) {
       uint4 x = *reinterpret_cast<const uint4*>(
           p.q + (static_cast<int64_t>(b) * q_heads + p.num_q_heads + is_v * p.num_kv_heads + kvh) * H + l8 * 8);
       if (!is_v) x = rotate8(x, angle + l8 * 4);
-      new_word = row_word<H>(quantize8(x, new_pair), l8, new_byte);
+      float level[8];
+      new_word = row_word<H>(quantize8(x, new_pair, level), l8, new_byte);
       const uint32_t to = static_cast<uint32_t>(table[col_of(pos)]);
       if (to >= static_cast<uint32_t>(p.num_pages)) {
         int4_report(p.status);
@@ -703,9 +763,14 @@ static int int4_attn(const Int4AttnParams& p, int B, cudaStream_t stream) {
 
 namespace axb {
 
-static int int4_append(const Int4AppendParams& p, int head_dim, cudaStream_t stream) {
+static int int4_append(Int4AppendParams& p, int B, int T, int page_size, int head_dim, cudaStream_t stream) {
+  const int heads = p.num_kv_heads + (p.num_q_heads + 1) / 2;
+  const int64_t units = static_cast<int64_t>(B) * T * heads;
+  if (units >= (int64_t{1} << 30)) return -10;
+  p.heads = FastDiv(heads), p.tokens = FastDiv(T), p.page = FastDiv(page_size);
+  p.units = static_cast<uint32_t>(units);
   const int64_t per_cta = kAppendThreads / (head_dim / 8);
-  int64_t ctas = (static_cast<int64_t>(p.B) * p.T * (p.num_q_heads + 2 * p.num_kv_heads) + per_cta - 1) / per_cta;
+  int64_t ctas = (units + per_cta - 1) / per_cta;
   if (ctas > 148 * 32) ctas = 148 * 32;
   if (head_dim == 128)
     launch_chained(int4_append_kernel<128>, static_cast<unsigned>(ctas), kAppendThreads, 0, stream, p);
@@ -740,9 +805,8 @@ extern "C" int axb_int4_append(const void* k, const void* v, int64_t k_b, int64_
   p.k_pool = {static_cast<uint8_t*>(k_codes), static_cast<uint32_t*>(k_pairs)};
   p.v_pool = {static_cast<uint8_t*>(v_codes), static_cast<uint32_t*>(v_pairs)};
   p.page_table = page_table, p.start = start, p.live = live, p.status = status;
-  p.B = B, p.T = T, p.num_kv_heads = num_kv_heads;
-  p.page_size = page_size, p.max_pages = max_pages, p.num_pages = num_pages;
-  return int4_append(p, head_dim, stream);
+  p.num_kv_heads = num_kv_heads, p.max_pages = max_pages, p.num_pages = num_pages;
+  return int4_append(p, B, T, page_size, head_dim, stream);
 }
 
 // Whole prompts from position 0: qkv [B, T, (Nq + 2 Nkv) * H] of one projection.  Queries and keys are rotated by `angle`
@@ -773,9 +837,8 @@ extern "C" int axb_int4_append_prompt(void* qkv, void* k_codes, void* k_pairs, v
   p.page_table = page_table, p.status = status;
   p.angle = reinterpret_cast<const float2*>(angle);
   p.angle_rows = angle_rows;
-  p.B = B, p.T = T, p.num_q_heads = num_q_heads, p.num_kv_heads = num_kv_heads;
-  p.page_size = page_size, p.max_pages = max_pages, p.num_pages = num_pages;
-  return int4_append(p, head_dim, stream);
+  p.num_q_heads = num_q_heads, p.num_kv_heads = num_kv_heads, p.max_pages = max_pages, p.num_pages = num_pages;
+  return int4_append(p, B, T, page_size, head_dim, stream);
 }
 
 // Scratch of axb_int4_decode_attn in floats: up to a cluster's splits meet without any.
