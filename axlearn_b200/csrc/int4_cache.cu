@@ -228,8 +228,8 @@ struct Int4AttnParams {
   Int4Pool k_pool, v_pool;
   const int* page_table;
   const int* lengths;
-  float* part_out;         // [B, Nq, splits, H]
-  float* part_ml;          // [B, Nq, splits, 2]
+  float* part_out;         // [B, Nq, splits / 8, H]: of each cluster, where there are several
+  float* part_ml;          // [B, Nq, splits / 8, 2]
   __nv_bfloat16* out;
   int* status;
   int num_q_heads, num_kv_heads, page_size, page_shift, max_pages, num_pages, splits;  // page_shift: -1 where no power of two
@@ -338,13 +338,14 @@ int4_attn_kernel(Int4AttnParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, c = lane & 3;
   int len = p.lengths[b];
+  // Tiles go to the warps of all splits in turn, so which pages a warp needs does not depend on the length.
+  const int step = kAttnWarps * p.splits;
+  int tile = split * kAttnWarps + warp;
   if (len > p.max_pages * static_cast<int64_t>(p.page_size)) {
     if (threadIdx.x == 0) int4_report(p.status);
     len = kAppend ? 0 : p.max_pages * p.page_size;  // a new token without a place: nothing is appended
   }
-  const int tiles = (max(len, 0) + kAttnKeys - 1) / kAttnKeys;
-  const int per_split = (tiles + p.splits - 1) / p.splits;
-  const int hi = min(tiles, (split + 1) * per_split);
+  const int hi = (max(len, 0) + kAttnKeys - 1) / kAttnKeys;
   const int* table = p.page_table + static_cast<int64_t>(b) * p.max_pages;
 
   // Key `lane` of a tile: its page, asked for long before `row_of` makes it the row of the pools; kNone beyond the sequence
@@ -353,8 +354,8 @@ int4_attn_kernel(Int4AttnParams p) {
   const int cached = kAppend ? len - 1 : len;
   auto col_of = [&](int t) { return p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size; };
   auto page_of = [&](int tile) -> uint32_t {
-    const int t = tile * kAttnKeys + lane;
-    return tile < hi && t < cached ? static_cast<uint32_t>(table[col_of(t)]) : 0u;
+    const int col = col_of(tile * kAttnKeys + lane);
+    return col < p.max_pages ? static_cast<uint32_t>(table[col]) : 0u;
   };
   auto row_of = [&](int tile, uint32_t page) -> uint32_t {
     const int t = tile * kAttnKeys + lane;
@@ -392,13 +393,12 @@ int4_attn_kernel(Int4AttnParams p) {
       cp_async8(pair_dst + at_stage + kAttnKeys * Tile::kPairs, p.v_pool.pairs + off, ok);
     }
   };
-  int tile = split * per_split + warp;
   uint32_t pages[kAttnStages + 1];
 #pragma unroll
-  for (int i = 0; i <= kAttnStages; ++i) pages[i] = page_of(tile + i * kAttnWarps);
+  for (int i = 0; i <= kAttnStages; ++i) pages[i] = page_of(tile + i * step);
 #pragma unroll
   for (int i = 0; i < kAttnStages; ++i) {
-    if (tile + i * kAttnWarps < hi) load_tile(i, row_of(tile + i * kAttnWarps, pages[i]));
+    if (tile + i * step < hi) load_tile(i, row_of(tile + i * step, pages[i]));
     cp_commit();
   }
   uint32_t page = pages[kAttnStages];
@@ -406,8 +406,7 @@ int4_attn_kernel(Int4AttnParams p) {
   const int pos = len - 1;
   // The new token: lane l of the first H / 8 has dims 8 l .. 8 l + 7 of its key, the next H / 8 lanes its value.
   const int new_tile = pos / kAttnKeys;
-  const bool appends = kAppend && len > 0 && new_tile >= split * per_split && new_tile < hi &&
-                       (new_tile - split * per_split) % kAttnWarps == warp;
+  const bool appends = kAppend && len > 0 && new_tile % step == tile;
   const float2* angle = nullptr;
   uint32_t new_word = 0, new_pair = 0;
   int new_byte = 0;
@@ -486,7 +485,7 @@ int4_attn_kernel(Int4AttnParams p) {
   const float zero[4] = {0.f, 0.f, 0.f, 0.f};
 
   int stage = 0;
-  for (; tile < hi; tile += kAttnWarps) {
+  for (; tile < hi; tile += step) {
     cp_wait_group<kAttnStages - 1>();
     __syncwarp();
     uint8_t* st = ring + stage * Tile::kBytes;
@@ -619,9 +618,9 @@ int4_attn_kernel(Int4AttnParams p) {
       }
     }
     __syncwarp();  // the stage has been read
-    if (tile + kAttnStages * kAttnWarps < hi) load_tile(stage, row_of(tile + kAttnStages * kAttnWarps, page));
+    if (tile + kAttnStages * step < hi) load_tile(stage, row_of(tile + kAttnStages * step, page));
     cp_commit();
-    page = page_of(tile + (kAttnStages + 1) * kAttnWarps);
+    page = page_of(tile + (kAttnStages + 1) * step);
     if (++stage == kAttnStages) stage = 0;
   }
   cp_wait_all();
@@ -670,27 +669,22 @@ int4_attn_kernel(Int4AttnParams p) {
     const int64_t row = static_cast<int64_t>(b) * p.num_q_heads + qh0 + g;
     if (p.splits == 1) {
       p.out[row * H + d] = __float2bfloat16(ll == 0.f ? 0.f : o / ll);
-    } else if (kCluster) {
+    } else {
       s_part[kAttnWarps * per_warp + g * H + d] = o;
       if (d == 0) {
         s_m[kAttnWarps * rows + g] = mm;
         s_l[kAttnWarps * rows + g] = ll;
       }
-    } else {
-      p.part_out[(row * p.splits + split) * H + d] = o;
-      if (d == 0) {
-        p.part_ml[(row * p.splits + split) * 2] = mm;
-        p.part_ml[(row * p.splits + split) * 2 + 1] = ll;
-      }
     }
   }
   if constexpr (kCluster) {
+    const int cluster = min(p.splits, kAttnCluster), rank = split % cluster, parts = p.splits / cluster;
     cluster_sync_all();
-    for (int g = split * kSets + threadIdx.x / H; g < rows; g += p.splits * kSets) {
+    for (int g = rank * kSets + threadIdx.x / H; g < rows; g += cluster * kSets) {
       float mv[kAttnCluster], lv[kAttnCluster], ov[kAttnCluster];
 #pragma unroll
       for (int s = 0; s < kAttnCluster; ++s) {
-        const bool have = s < p.splits;
+        const bool have = s < cluster;
         mv[s] = have ? ld_cluster_f32(sptr(s_m + kAttnWarps * rows + g), s) : -INFINITY;
         lv[s] = have ? ld_cluster_f32(sptr(s_l + kAttnWarps * rows + g), s) : 0.f;
         ov[s] = have ? ld_cluster_f32(sptr(s_part + kAttnWarps * per_warp + g * H + d), s) : 0.f;
@@ -705,25 +699,50 @@ int4_attn_kernel(Int4AttnParams p) {
         ll += lv[s] * f;
         o += ov[s] * f;
       }
-      p.out[(static_cast<int64_t>(b) * p.num_q_heads + qh0 + g) * H + d] = __float2bfloat16(ll == 0.f ? 0.f : o / ll);
+      const int64_t row = static_cast<int64_t>(b) * p.num_q_heads + qh0 + g;
+      if (parts == 1) {
+        p.out[row * H + d] = __float2bfloat16(ll == 0.f ? 0.f : o / ll);
+      } else {
+        const int64_t part = row * parts + split / cluster;
+        p.part_out[part * H + d] = o;
+        if (d == 0) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(mm, ll);
+      }
     }
     cluster_sync_all();  // a CTA's shared memory outlives its readers
   }
 }
 
+// The clusters' parts of a row, eight at a time on their way.
 template <int H>
 __global__ void __launch_bounds__(H)
-int4_combine_kernel(const float* part_out, const float* part_ml, __nv_bfloat16* out, int splits) {
+int4_combine_kernel(const float* part_out, const float* part_ml, __nv_bfloat16* out, int parts) {
   chain_link();
+  constexpr int kAtOnce = 8;
   const int64_t row = blockIdx.x;
   const int d = threadIdx.x;
-  float mm = -INFINITY;
-  for (int s = 0; s < splits; ++s) mm = fmaxf(mm, part_ml[(row * splits + s) * 2]);
-  float ll = 0.f, o = 0.f;
-  for (int s = 0; s < splits; ++s) {
-    const float f = mm == -INFINITY ? 1.f : exp2f(part_ml[(row * splits + s) * 2] - mm);
-    ll += part_ml[(row * splits + s) * 2 + 1] * f;
-    o += part_out[(row * splits + s) * H + d] * f;
+  float mm = -INFINITY, ll = 0.f, o = 0.f;
+  for (int s0 = 0; s0 < parts; s0 += kAtOnce) {
+    float2 ml[kAtOnce];
+    float ov[kAtOnce];
+#pragma unroll
+    for (int s = 0; s < kAtOnce; ++s) {
+      const bool have = s0 + s < parts;
+      ml[s] = have ? *reinterpret_cast<const float2*>(part_ml + (row * parts + s0 + s) * 2) : make_float2(-INFINITY, 0.f);
+      ov[s] = have ? part_out[(row * parts + s0 + s) * H + d] : 0.f;
+    }
+    float top = mm;
+#pragma unroll
+    for (int s = 0; s < kAtOnce; ++s) top = fmaxf(top, ml[s].x);
+    const float old = top == -INFINITY ? 1.f : exp2f(mm - top);
+    ll *= old;
+    o *= old;
+#pragma unroll
+    for (int s = 0; s < kAtOnce; ++s) {
+      const float f = top == -INFINITY ? 1.f : exp2f(ml[s].x - top);
+      ll += ml[s].y * f;
+      o += ov[s] * f;
+    }
+    mm = top;
   }
   out[row * H + d] = __float2bfloat16(ll == 0.f ? 0.f : o / ll);
 }
@@ -733,7 +752,7 @@ static int launch_int4_attn(const Int4AttnParams& p, dim3 grid, int rows, cudaSt
   constexpr auto kernel = int4_attn_kernel<H, kCluster, kAppend>;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {grid.x, 1, 1};
+  attr[0].val.clusterDim = {static_cast<unsigned>(p.splits < kAttnCluster ? p.splits : kAttnCluster), 1, 1};
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(kAttnThreads);
@@ -748,14 +767,15 @@ static int launch_int4_attn(const Int4AttnParams& p, dim3 grid, int rows, cudaSt
 template <int H, bool kAppend>
 static int int4_attn(const Int4AttnParams& p, int B, cudaStream_t stream) {
   const int g = p.num_q_heads / p.num_kv_heads;
-  const bool cluster = p.splits > 1 && p.splits <= kAttnCluster;
+  const bool cluster = p.splits > 1;
   const dim3 grid(p.splits, p.num_kv_heads * ((g + kAttnRows - 1) / kAttnRows), B);
   const int rows = g < kAttnRows ? g : kAttnRows;
   const int rc = cluster ? launch_int4_attn<H, true, kAppend>(p, grid, rows, stream)
                          : launch_int4_attn<H, false, kAppend>(p, grid, rows, stream);
   if (rc != 0) return rc;
   if (p.splits > kAttnCluster)
-    launch_chained(int4_combine_kernel<H>, B * p.num_q_heads, H, 0, stream, p.part_out, p.part_ml, p.out, p.splits);
+    launch_chained(int4_combine_kernel<H>, B * p.num_q_heads, H, 0, stream, p.part_out, p.part_ml, p.out,
+                   p.splits / kAttnCluster);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
@@ -841,10 +861,10 @@ extern "C" int axb_int4_append_prompt(void* qkv, void* k_codes, void* k_pairs, v
   return int4_append(p, B, T, page_size, head_dim, stream);
 }
 
-// Scratch of axb_int4_decode_attn in floats: up to a cluster's splits meet without any.
+// Scratch of axb_int4_decode_attn in floats: up to a cluster's splits meet without any.  More are a multiple of a cluster's.
 extern "C" int64_t axb_int4_attn_scratch_floats(int B, int num_q_heads, int head_dim, int splits) {
   if (splits <= axb::kAttnCluster) return 0;
-  return static_cast<int64_t>(B) * num_q_heads * splits * (head_dim + 2);
+  return static_cast<int64_t>(B) * num_q_heads * (splits / axb::kAttnCluster) * (head_dim + 2);
 }
 
 // One new token a sequence: q [B, Nq, H] over the cache; with `angle` ([position][H / 2] of (sin, cos)) q is the packed
@@ -862,7 +882,7 @@ extern "C" int axb_int4_decode_attn(const void* q, void* k_codes, void* k_pairs,
   for (const void* x : {q, static_cast<const void*>(angle), static_cast<const void*>(k_codes), static_cast<const void*>(k_pairs),
                         static_cast<const void*>(v_codes), static_cast<const void*>(v_pairs)})
     if (!aligned16(x)) return -10;
-  if (splits > kAttnCluster && scratch == nullptr) return -10;
+  if (splits > kAttnCluster && (scratch == nullptr || splits % kAttnCluster)) return -10;
   if (B == 0) return 0;
   Int4AttnParams p = {};
   p.q = static_cast<const __nv_bfloat16*>(q);
@@ -871,7 +891,7 @@ extern "C" int axb_int4_decode_attn(const void* q, void* k_codes, void* k_pairs,
   p.v_pool = {static_cast<uint8_t*>(v_codes), static_cast<uint32_t*>(v_pairs)};
   p.page_table = page_table, p.lengths = lengths;
   p.part_out = scratch;
-  p.part_ml = scratch == nullptr ? nullptr : scratch + static_cast<int64_t>(B) * num_q_heads * splits * head_dim;
+  p.part_ml = scratch == nullptr ? nullptr : scratch + static_cast<int64_t>(B) * num_q_heads * (splits / kAttnCluster) * head_dim;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.status = status;
   p.num_q_heads = num_q_heads, p.num_kv_heads = num_kv_heads, p.page_size = page_size;

@@ -355,11 +355,15 @@ def _aligned_rows(x: Tensor) -> Tensor:
 
 def attention_splits(batch: int, num_kv_heads: int, group: int, max_len: int, sms: int = 148) -> int:
     """KV splits of attention over the 4-bit cache: one wave of CTAs (four fit an SM; one takes a split, a KV head and eight
-    query heads), 64 tokens or more for each."""
+    query heads), 64 tokens or more for each.  Beyond 8, which meet in a cluster, the clusters' parts are merged by a second
+    launch: for long sequences, growing with the root of their length (8 heads, us with 8 / 16 / 32 / 64 splits: 4000 tokens 8.3
+    9.5 8.6 10.9, 16000 tokens 24 19 14.6 16.0, 130001 tokens 151 91 52 47), and as many as clusters of 8 fit the GPU."""
     ctas = batch * num_kv_heads * ((group + 7) // 8)
     splits = max(1, min(max_len // 64, 4 * sms // max(1, ctas)))
-    many = math.isqrt(max_len) // 4
-    return min(splits, many if many >= 16 else 8)
+    if splits <= 8:
+        return splits
+    many = min((math.isqrt(max_len) // 4 + 4) // 8, 512 // ctas // 8) * 8
+    return many if many >= 24 else 8
 
 
 def _attention_plain(q, k_pages, v_pages, page_table, lengths, scale):
@@ -384,7 +388,8 @@ def paged_decode_attention_int4(q: Tensor, k_pages: Int4Pages, v_pages: Int4Page
                                 softmax_scale: Optional[float] = None, splits: Optional[int] = None,
                                 out: Optional[Tensor] = None, scratch: Optional[Tensor] = None) -> Tensor:
     """q ``[B, Nq, H]``; page_table ``[B, max_pages]``, lengths ``[B]`` int32 (valid tokens per sequence; 0: zeros).  Query heads
-    are grouped by KV head.  ``scratch``: ``attention_scratch_floats`` fp32 values, for more than eight splits.  Returns
+    are grouped by KV head.  ``scratch``: ``attention_scratch_floats`` fp32 values, for more than eight splits (made a
+    multiple of eight).  Returns
     ``[B, Nq, H]``."""
     b, nq, h = q.shape
     device = q.device
@@ -411,6 +416,7 @@ def _launch_attention(q, k_pages, v_pages, page_table, lengths, table, out, scra
     if splits is None:
         splits = attention_splits(b, nkv, nq // nkv, max_pages * page_size)
     if splits > 8:
+        splits = -(-splits // 8) * 8
         floats = attention_scratch_floats(b, nq, h, splits)
         if scratch is None:
             scratch = torch.empty(floats, dtype=torch.float32, device=device)
@@ -423,7 +429,8 @@ def _launch_attention(q, k_pages, v_pages, page_table, lengths, table, out, scra
 
 
 def attention_scratch_floats(batch: int, num_q_heads: int, head_dim: int, splits: int) -> int:
-    """fp32 values that the parts of more than eight splits take."""
+    """fp32 values that the parts of more than eight splits take (a multiple of eight)."""
+    splits = -(-splits // 8) * 8 if splits > 8 else splits
     return _lib().axb_int4_attn_scratch_floats(batch, num_q_heads, head_dim, splits)
 
 
