@@ -2,10 +2,17 @@
 // tensor cores: 128 features are the M side of the MMA, the rows of x its N side.
 //
 // Eight warps feed: each owns 16 features and turns their codes of 128 rows of W into bf16 values m + s c (one rounding, 2^-9
-// of a weight, as in the expansion for the GEMM of more rows), which `tcgen05.st` puts into tensor memory -- a lane's words
-// are the fragment of the 16x256b shape as they lie --, so that weights never pass through shared memory once they are 16
-// bits wide: writing and reading them there would cost eight times the bytes of the codes.  Other warps bring x, 128 columns
-// of it at a time, to shared memory in the order in which the codes run over K, and one issues the MMAs.
+// of a weight, as in the expansion for the GEMM of more rows), which `tcgen05.st` puts into tensor memory, so that weights
+// never pass through shared memory once they are 16 bits wide: writing and reading them there would cost eight times the
+// bytes of the codes.  A 16x256b store takes from lane (r, c) the columns 2c, 2c + 1 of every k16 step, 4 rows of W: the word c of
+// piece (r, s) of a block for step s.  `ldmatrix` hands out words that way, pieces being rows of its matrices, and x keeps its
+// own order over K.  Codes (64-byte swizzle: no bank conflicts), pairs and x come by TMA: with 16-byte `cp.async` by the
+// feeding warps the copies alone, about 32 cycles of the load unit for each of a warp, took 80% of the product's time.
+// A feeding warp has the next stage's codes in registers before it waits for a place.
+//
+// Measured (us; the codes at the copy rate): 64 x 4096 x 22016 24.2 (8.3), 64 x 14336 x 4096 16.5 (5.1), 128 x 4096 x 28672 39
+// (10.8).  A stage of one CTA an SM takes 0.35 us, of two 0.27; ALU instructions of the conversion are the largest part.
+//
 // K slices are the CTAs of a cluster; partial sums meet in distributed shared memory in a fixed order.
 //
 // Launched in the ordinary way in a captured step, too: a successor that started early could hold the tensor memory that a
@@ -15,6 +22,7 @@
 #include <stdint.h>
 
 #include "cluster.cuh"
+#include "host_utils.cuh"
 #include "int4.cuh"
 #include "mma_sync.cuh"
 #include "sm100.cuh"
@@ -22,36 +30,32 @@
 namespace axb {
 
 struct Int4GemmParams {
-  const __nv_bfloat16* x;  // [M, ldx]
-  const uint8_t* codes;    // [n16, k64, 512]
-  const uint8_t* pairs;    // [n16, groups, 64]
   __nv_bfloat16* y;        // [M, ldy]
-  int64_t ldx, ldy;
+  int64_t ldy;
   int M, N, K;
   int accumulate, splits;
   int* status;
 };
 
-constexpr int kIgWarps = 8, kIgFeatures = 16 * kIgWarps;
+constexpr int kIgWarps = 8, kIgThreads = 32 * (kIgWarps + 3), kIgFeatures = 16 * kIgWarps;
 constexpr int kIgMaxSplits = 8;
 
 // A stage is 128 rows of W: 64 columns of tensor memory, two 64-column tiles of x, eight warps' codes and pairs.  Codes, on
 // their way from memory, have the deepest ring; x comes from the L2.
 template <int BN>
 struct Int4GemmCfg {
-  static constexpr int kXRing = BN == 64 ? 3 : 4;            // each place has a warp of its own
-  static constexpr int kThreads = 32 * (kIgWarps + kXRing + 1);
+  static constexpr int kRing = BN <= 64 ? 3 : 4;             // places for x and for operands in tensor memory
   static constexpr int kCodeRing = BN <= 16 ? 9 : BN <= 32 ? 7 : BN <= 64 ? 6 : 8;
-  static constexpr int kX = BN * 128, kCodes = 1024 + 128;   // bytes of a tile of x; of a warp's codes and pairs
-  static constexpr int kXBytes = kXRing * 2 * kX;
-  static constexpr int kRingBytes = kXBytes + kCodeRing * kIgWarps * kCodes;
+  static constexpr int kX = BN * 128, kCodes = kIgWarps * 1024, kPairs = kIgWarps * 128;  // bytes: a tile of x, codes, pairs
+  static constexpr int kXBytes = kRing * 2 * kX, kCodeBytes = kCodeRing * kCodes;
+  static constexpr int kRingBytes = kXBytes + kCodeBytes + kCodeRing * kPairs;
   static constexpr int kSums = BN * kIgFeatures * 4;         // partial sums overlay the rings
   static constexpr int kBody = kRingBytes > kSums ? kRingBytes : kSums;
   static constexpr int kSmem = kBody + 256 + 1024;           // barriers, alignment slack
   static constexpr int kResident = BN <= 64 ? 2 : 1;
-  static constexpr int kACol = BN <= 64 ? 64 : 128, kARing = BN <= 64 ? 3 : 4;
+  static constexpr int kACol = BN <= 64 ? 64 : 128;
   static constexpr int kTmemCols = BN <= 64 ? 256 : 512;
-  static_assert(kACol + kARing * 64 <= kTmemCols, "tensor memory");
+  static_assert(kACol + kRing * 64 <= kTmemCols, "tensor memory");
   static_assert(kResident * (kSmem + 1024) <= 228 * 1024 && kResident * kTmemCols <= 512, "resident CTAs");
 };
 
@@ -65,13 +69,6 @@ struct IgPlace {
   }
 };
 
-__device__ __forceinline__ void ig_copy(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void ig_copy8(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(ok ? 8 : 0) : "memory");
-}
-
 // 16 lanes x 32 columns: thread (r, c) has columns 8 n + 2c, + 1 of lanes r (entries 4 n, 4 n + 1) and r + 8.
 __device__ __forceinline__ void tmem_st_16x256(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -83,10 +80,9 @@ __device__ __forceinline__ void tmem_st_16x256(uint32_t taddr, const uint32_t (&
 }
 
 // The four registers of a word's k16 step: codes as denormal bf16 numbers (`int4.cuh`; the high nibbles are 16 times theirs),
-// turned into 2^-kIgDown (m + s c) by one operation.  s0 (s1) carries 2^(133 - kIgDown) (a sixteenth of it), m0 and m1
-// 2^-kIgDown, so that neither steps up to 2^31 nor values down to 2^-89 leave the range of bf16.
-constexpr int kIgDown = 37;
-constexpr float kIgStep = 79228162514264337593543950336.f, kIgLow = 1.f / 137438953472.f;  // 2^(133 - kIgDown), 2^-kIgDown
+// turned into 2^-37 (m + s c) by one operation.  s0 (s1) carries 2^(133 - 37) (a sixteenth of it), m0 and m1
+// 2^-37, so that neither steps up to 2^31 nor values down to 2^-89 leave the range of bf16.
+constexpr float kIgStep = 79228162514264337593543950336.f, kIgLow = 1.f / 137438953472.f;  // 2^(133 - 37), 2^-37
 
 __device__ __forceinline__ void ig_values(uint32_t word, __nv_bfloat162 s0, __nv_bfloat162 m0, __nv_bfloat162 s1,
                                           __nv_bfloat162 m1, uint32_t* v) {
@@ -103,17 +99,18 @@ __device__ __forceinline__ void ig_values(uint32_t word, __nv_bfloat162 s0, __nv
 
 // kGroup: 64 or 128.
 template <int BN, int kGroup>
-__global__ void __launch_bounds__(Int4GemmCfg<BN>::kThreads, Int4GemmCfg<BN>::kResident)
-int4_gemm_kernel(Int4GemmParams p) {
+__global__ void __launch_bounds__(kIgThreads, Int4GemmCfg<BN>::kResident)
+int4_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_codes,
+                 const __grid_constant__ CUtensorMap map_pairs, Int4GemmParams p) {
   using S = Int4GemmCfg<BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem =
       reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint64_t* x_full = reinterpret_cast<uint64_t*>(smem + S::kBody);
-  uint64_t* x_empty = x_full + S::kXRing;
-  uint64_t* a_full = x_empty + S::kXRing;
-  uint64_t* a_empty = a_full + S::kARing;
-  uint64_t* done_bar = a_empty + S::kARing;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S::kBody);
+  uint64_t* empty_bar = full_bar + S::kRing;
+  uint64_t* code_full = empty_bar + S::kRing;
+  uint64_t* code_empty = code_full + S::kCodeRing;
+  uint64_t* done_bar = code_empty + S::kCodeRing;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -123,18 +120,18 @@ int4_gemm_kernel(Int4GemmParams p) {
   const int kb_lo = split * k128 / p.splits, count = (split + 1) * k128 / p.splits - kb_lo;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < S::kXRing; ++i) {
-      mbar_init(&x_full[i], 1);
-      mbar_init(&x_empty[i], 1);
+    for (int i = 0; i < S::kRing; ++i) {
+      mbar_init(&full_bar[i], kIgWarps + 1);
+      mbar_init(&empty_bar[i], 1);
     }
-    for (int i = 0; i < S::kARing; ++i) {
-      mbar_init(&a_full[i], kIgWarps);
-      mbar_init(&a_empty[i], 1);
+    for (int i = 0; i < S::kCodeRing; ++i) {
+      mbar_init(&code_full[i], 1);
+      mbar_init(&code_empty[i], kIgWarps);
     }
     mbar_init(done_bar, 1);
     fence_barrier_init();
   }
-  constexpr int kMmaWarp = kIgWarps + S::kXRing;
+  constexpr int kXWarp = kIgWarps, kCodeWarp = kIgWarps + 1, kMmaWarp = kIgWarps + 2;
   if (warp == kMmaWarp) {
     tmem_alloc(tmem_slot, S::kTmemCols);
     tmem_relinquish();
@@ -144,138 +141,112 @@ int4_gemm_kernel(Int4GemmParams p) {
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
 
+  constexpr int kPairBytes = kGroup == 64 ? 128 : 64;  // of a stage and 16 features
   bool ok = true;
   if (warp < kIgWarps) {
     // Tensor-memory lanes [32 (warp % 4) + 16 (warp / 4), + 16): features of this warp, in their order.
     const int sub = 2 * (warp & 3) + (warp >> 2);
-    const int tile = n0 / 16 + sub;
-    const bool have = tile < (p.N + 15) / 16;
     const uint32_t a_addr = tmem + (static_cast<uint32_t>(sub * 16) << 16) + S::kACol;
-    const int64_t block = static_cast<int64_t>(have ? tile : 0) * k128 + kb_lo;
-    const uint8_t* codes = p.codes + block * 1024 + lane * 16;
-    constexpr int kPairBytes = kGroup == 64 ? 128 : 64;  // of a stage
-    const uint8_t* pairs = p.pairs + block * kPairBytes + lane * 16;
-    constexpr int kStride = kIgWarps * S::kCodes;        // of a stage in the ring
-    const uint8_t* own = smem + S::kXBytes + warp * S::kCodes;
-    const uint32_t dst0 = smem_u32(own) + lane * 16;
-    uint32_t dst = dst0;
-    auto load = [&] {  // the next stage
-      ig_copy(dst, codes, have);
-      ig_copy(dst + 512, codes + 512, have);
-      if (lane * 16 < kPairBytes) ig_copy(dst + 1024, pairs, have);
-      codes += 1024;
-      pairs += kPairBytes;
-      dst += kStride;
-      if (dst == dst0 + S::kCodeRing * kStride) dst = dst0;
-    };
-#pragma unroll 1
-    for (int it = 0; it < S::kCodeRing; ++it) {
-      if (it < count) load();
-      cp_commit();
-    }
+    const int r = lane >> 2;
+    // Row lane % 8 of matrix lane / 8: the copy swaps 16-byte units as the 64-byte swizzle does.
+    const uint8_t* mine = smem + S::kXBytes + sub * 1024 + (lane & 7) * 64 + (((lane >> 3) ^ (lane >> 1 & 3)) << 4);
+    const uint8_t* mine_pairs = smem + S::kXBytes + S::kCodeBytes + sub * kPairBytes + r * 8;
+    uint32_t w[2][4];
+    uint2 u[128 / kGroup];
     IgPlace<S::kCodeRing> code;
-    IgPlace<S::kARing> a;
+    auto take = [&] {  // the next stage's codes and pairs, into registers
+      if (!mbar_wait_warp(&code_full[code.slot], code.phase, p.status, kStatusWaitTimeoutProducer)) return false;
+      ldsm4(w[0], mine + code.slot * S::kCodes);
+      ldsm4(w[1], mine + code.slot * S::kCodes + 512);
+#pragma unroll
+      for (int g = 0; g < 128 / kGroup; ++g)
+        u[g] = *reinterpret_cast<const uint2*>(mine_pairs + code.slot * S::kPairs + g * 64);
+      return true;
+    };
+    ok = take();
+    IgPlace<S::kRing> a;
 #pragma unroll 1
-    for (int it = 0; it < count; ++it) {
-      if (it >= S::kARing) {
-        ok = mbar_wait_warp(&a_empty[a.slot], a.phase ^ 1, p.status, kStatusWaitTimeoutProducer);
-        if (!ok) break;
-        tc_fence_after_sync();
-      }
-      cp_wait_group<S::kCodeRing - 1>();
-      __syncwarp();
-      const uint8_t* mine = own + code.slot * kStride;
-      const uint32_t a_stage_addr = a_addr + a.slot * 64;
+    for (int it = 0; ok && it < count; ++it) {
+      uint32_t v[2][16];
       __nv_bfloat162 s0, m0, s1, m1;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const uint4 w = *reinterpret_cast<const uint4*>(mine + half * 512 + lane * 16);
         if (half == 0 || kGroup == 64) {
-          const uint2 u = *reinterpret_cast<const uint2*>(mine + 1024 + half * 64 + (lane >> 2) * 8);
-          const __nv_bfloat162 pa = reinterpret_cast<const __nv_bfloat162&>(u.x), pb = reinterpret_cast<const __nv_bfloat162&>(u.y);
-          const __nv_bfloat162 low = __float2bfloat162_rn(kIgLow);
+          const uint2 pair = u[kGroup == 64 ? half : 0];
+          const __nv_bfloat162 pa = reinterpret_cast<const __nv_bfloat162&>(pair.x),
+                               pb = reinterpret_cast<const __nv_bfloat162&>(pair.y), low = __float2bfloat162_rn(kIgLow);
           s0 = __hmul2(__low2bfloat162(pa), __float2bfloat162_rn(kIgStep)), m0 = __hmul2(__high2bfloat162(pa), low);
           s1 = __hmul2(__low2bfloat162(pb), __float2bfloat162_rn(kIgStep / 16.f)), m1 = __hmul2(__high2bfloat162(pb), low);
         }
-        uint32_t v[16];
-        ig_values(w.x, s0, m0, s1, m1, v);
-        ig_values(w.y, s0, m0, s1, m1, v + 4);
-        ig_values(w.z, s0, m0, s1, m1, v + 8);
-        ig_values(w.w, s0, m0, s1, m1, v + 12);
-        tmem_st_16x256(a_stage_addr + half * 32, v);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) ig_values(w[half][q], s0, m0, s1, m1, v[half] + 4 * q);
       }
+      // The next stage's codes, while this stage's values wait for their place.
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&code_empty[code.slot]);
+      code.next();
+      if (it + 1 < count && !take()) {
+        ok = false;
+        break;
+      }
+      if (it >= S::kRing) {
+        ok = mbar_wait_warp(&empty_bar[a.slot], a.phase ^ 1, p.status, kStatusWaitTimeoutProducer);
+        if (!ok) break;
+        tc_fence_after_sync();
+      }
+      tmem_st_16x256(a_addr + a.slot * 64, v[0]);
+      tmem_st_16x256(a_addr + a.slot * 64 + 32, v[1]);
       tmem_st_wait();
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&a_full[a.slot]);
-      if (it + S::kCodeRing < count) load();  // into the place that has been read
-      cp_commit();
-      code.next();
+      if (lane == 0) mbar_arrive(&full_bar[a.slot]);
       a.next();
     }
-    cp_wait_all();
     if (ok) ok = mbar_wait_warp(done_bar, 0, p.status, kStatusWaitTimeoutEpilogue);
-  } else if (warp < kMmaWarp) {
-    // x: 16-byte pieces (row, h, i), tile h of 2 and i of 8: columns 64 h + 16 c + 8 q + 0 .. 7 with c = i / 2, q = i % 2.
-    // Their halves go to places 4c .. 4c + 3 of the k16 steps 2q and 2q + 1, where the codes of these columns are.  A warp fills
-    // one place of the ring, a lane the pieces (h, i) of every second row.
-    constexpr int kMine = BN / 2;
-    const int place = warp - kIgWarps;
-    const int i = lane & 7, h = lane >> 3 & 1, row0 = lane >> 4;
-    const int c = i >> 1, q = i & 1, unit = 4 * q + (c >> 1);  // of 16 bytes; the second half's is two further
-    const int column = (kb_lo + place) * 128 + h * 64 + c * 16 + q * 8;
-    const __nv_bfloat16* src = p.x + row0 * p.ldx + column;
-    int left = p.K - column;                                   // columns from this piece on
-    const int rows = min(kMine, (p.M - row0 + 1) / 2);         // of this lane
-    const uint32_t at = smem_u32(smem) + place * (2 * S::kX) + h * S::kX + row0 * 128 + (c & 1) * 8;
-    uint32_t phase = 1;
+  } else if (warp == kXWarp) {
+    if (elect_one()) {
+      IgPlace<S::kRing> x;
 #pragma unroll 1
-    for (int it = place; it < count; it += S::kXRing) {
-      if (it >= S::kXRing) {
-        ok = mbar_wait_warp(&x_empty[place], phase, p.status, kStatusWaitTimeoutProducer);
-        if (!ok) break;
+      for (int it = 0; it < count; ++it) {
+        if (it >= S::kRing && !mbar_wait(&empty_bar[x.slot], x.phase ^ 1, p.status, kStatusWaitTimeoutProducer)) break;
+        uint8_t* tile = smem + x.slot * (2 * S::kX);
+        mbar_arrive_expect_tx(&full_bar[x.slot], 2 * S::kX);
+        tma_load_2d(tile, &map_x, &full_bar[x.slot], (kb_lo + it) * 128, 0);
+        tma_load_2d(tile + S::kX, &map_x, &full_bar[x.slot], (kb_lo + it) * 128 + 64, 0);
+        x.next();
       }
-      phase ^= 1;
-      const int there = left > 0 ? rows : 0;
-      const __nv_bfloat16* from = src;
-#pragma unroll 8
-      for (int j = 0; j < kMine; ++j) {
-        // Rows of the lane are two apart: the swizzle takes the row mod 8.
-        const uint32_t to = at + j * 256 + ((unit ^ ((row0 + 2 * j) & 7)) << 4);
-        const __nv_bfloat16* piece = j < there ? from : p.x;
-        ig_copy8(to, piece, j < there);
-        ig_copy8(to ^ 32, piece + 4, j < there);  // two units further: bit 1 of the unit is 0, swapped or not
-        from += 2 * p.ldx;
+    }
+  } else if (warp == kCodeWarp) {
+    if (elect_one()) {
+      IgPlace<S::kCodeRing> code;
+#pragma unroll 1
+      for (int it = 0; it < count; ++it) {
+        if (it >= S::kCodeRing && !mbar_wait(&code_empty[code.slot], code.phase ^ 1, p.status, kStatusWaitTimeoutProducer)) break;
+        mbar_arrive_expect_tx(&code_full[code.slot], S::kCodes + kIgWarps * kPairBytes);
+        tma_load_3d(smem + S::kXBytes + code.slot * S::kCodes, &map_codes, &code_full[code.slot], 0, (kb_lo + it) * 16, n0 / 16);
+        tma_load_2d(smem + S::kXBytes + S::kCodeBytes + code.slot * S::kPairs, &map_pairs, &code_full[code.slot],
+                    (kb_lo + it) * kPairBytes, n0 / 16);
+        code.next();
       }
-      src += S::kXRing * 128;
-      left -= S::kXRing * 128;
-      cp_wait_all();
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&x_full[place]);
     }
   } else if (elect_one()) {
     constexpr uint32_t idesc = umma_idesc_f16(kIgFeatures, BN, 1, 1, 0, 0);
     bool fed = true;
-    IgPlace<S::kXRing> x;
-    IgPlace<S::kARing> a;
+    IgPlace<S::kRing> at;
 #pragma unroll 1
     for (int it = 0; it < count; ++it) {
-      if (!mbar_wait(&x_full[x.slot], x.phase, p.status, kStatusWaitTimeoutMma) ||
-          !mbar_wait(&a_full[a.slot], a.phase, p.status, kStatusWaitTimeoutMma)) {
+      if (!mbar_wait(&full_bar[at.slot], at.phase, p.status, kStatusWaitTimeoutMma)) {
         fed = false;
         break;
       }
       tc_fence_after_sync();
-      const uint32_t sx = smem_u32(smem) + x.slot * (2 * S::kX), sa = tmem + S::kACol + a.slot * 64;
+      const uint32_t sx = smem_u32(smem) + at.slot * (2 * S::kX), sa = tmem + S::kACol + at.slot * 64;
 #pragma unroll
       for (int k = 0; k < 8; ++k)
         tc_mma_f16_ts(tmem, sa + k * 8, umma_smem_desc(sx + (k >> 2) * S::kX + (k & 3) * 32, 16, 1024), idesc,
                       it > 0 || k > 0 ? 1u : 0u);
-      tc_commit(&x_empty[x.slot]);
-      tc_commit(&a_empty[a.slot]);
-      x.next();
-      a.next();
+      tc_commit(&empty_bar[at.slot]);
+      at.next();
     }
     if (fed) tc_commit(done_bar);
   }
@@ -343,30 +314,45 @@ int4_gemm_kernel(Int4GemmParams p) {
 }
 
 template <int BN, int kGroup>
-static int launch_int4_gemm(const Int4GemmParams& p, cudaStream_t stream) {
+static int launch_int4_gemm(const void* x, int64_t ldx, const void* codes, const void* pairs, const Int4GemmParams& p,
+                            cudaStream_t stream) {
   using S = Int4GemmCfg<BN>;
   constexpr auto kernel = int4_gemm_kernel<BN, kGroup>;
   static OptIn opt_in;
   if (!opt_in.done(kernel, S::kSmem)) return -3;
+  CUtensorMap map_x, map_codes, map_pairs;
+  const uint64_t n16 = (p.N + 15) / 16, k128 = (p.K + 127) / 128, pair_bytes = kGroup == 64 ? 128 : 64;
+  const uint64_t x_dims[2] = {static_cast<uint64_t>(p.K), static_cast<uint64_t>(p.M)}, x_stride[1] = {static_cast<uint64_t>(ldx) * 2};
+  const uint32_t x_box[2] = {64, BN};
+  const uint64_t code_dims[3] = {64, k128 * 16, n16}, code_strides[2] = {64, k128 * 1024};
+  const uint32_t code_box[3] = {64, 16, kIgWarps};
+  const uint64_t pair_dims[2] = {k128 * pair_bytes, n16}, pair_stride[1] = {k128 * pair_bytes};
+  const uint32_t pair_box[2] = {static_cast<uint32_t>(pair_bytes), kIgWarps};
+  if (make_tensor_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, x_dims, x_stride, x_box, CU_TENSOR_MAP_SWIZZLE_128B) != 0 ||
+      make_tensor_map(&map_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, codes, code_dims, code_strides, code_box,
+                      CU_TENSOR_MAP_SWIZZLE_64B) != 0 ||
+      make_tensor_map(&map_pairs, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, pairs, pair_dims, pair_stride, pair_box,
+                      CU_TENSOR_MAP_SWIZZLE_NONE) != 0)
+    return -2;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {static_cast<unsigned>(p.splits), 1, 1};
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((p.N + kIgFeatures - 1) / kIgFeatures * p.splits));
-  cfg.blockDim = dim3(S::kThreads);
+  cfg.blockDim = dim3(kIgThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? 0 : -4;
+  return cudaLaunchKernelEx(&cfg, kernel, map_x, map_codes, map_pairs, p) == cudaSuccess ? 0 : -4;
 }
 
 template <int kGroup>
-static int int4_gemm(const Int4GemmParams& p, cudaStream_t stream) {
-  if (p.M <= 16) return launch_int4_gemm<16, kGroup>(p, stream);
-  if (p.M <= 32) return launch_int4_gemm<32, kGroup>(p, stream);
-  if (p.M <= 64) return launch_int4_gemm<64, kGroup>(p, stream);
-  return launch_int4_gemm<128, kGroup>(p, stream);
+static int int4_gemm(const void* x, int64_t ldx, const void* codes, const void* pairs, const Int4GemmParams& p, cudaStream_t stream) {
+  if (p.M <= 16) return launch_int4_gemm<16, kGroup>(x, ldx, codes, pairs, p, stream);
+  if (p.M <= 32) return launch_int4_gemm<32, kGroup>(x, ldx, codes, pairs, p, stream);
+  if (p.M <= 64) return launch_int4_gemm<64, kGroup>(x, ldx, codes, pairs, p, stream);
+  return launch_int4_gemm<128, kGroup>(x, ldx, codes, pairs, p, stream);
 }
 
 }  // namespace axb
@@ -381,8 +367,6 @@ extern "C" int axb_int4_gemm(const void* x, const void* codes, const void* pairs
       splits > kIgMaxSplits || splits > (K + 127) / 128)
     return -10;
   if (M == 0) return 0;
-  const Int4GemmParams p{static_cast<const __nv_bfloat16*>(x), static_cast<const uint8_t*>(codes),
-                         static_cast<const uint8_t*>(pairs), static_cast<__nv_bfloat16*>(y), ldx, ldy, M, N, K,
-                         accumulate, splits, status};
-  return group == 64 ? int4_gemm<64>(p, stream) : int4_gemm<128>(p, stream);
+  const Int4GemmParams p{static_cast<__nv_bfloat16*>(y), ldy, M, N, K, accumulate, splits, status};
+  return group == 64 ? int4_gemm<64>(x, ldx, codes, pairs, p, stream) : int4_gemm<128>(x, ldx, codes, pairs, p, stream);
 }

@@ -229,6 +229,23 @@ def test_linear_of_few_and_many_rows(rows, k, n, group):
     assert ((out.double() - want).abs() <= bound + 2.0 ** -8 * (want.abs() + y.abs() + bound)).all()
 
 
+@pytest.mark.parametrize("rows", [17, 33, 128])
+@pytest.mark.parametrize("k,n,splits", [(640, 1160, 5), (1096, 264, 8), (200, 904, 2), (2048, 392, 3)])
+def test_linear_with_slices_of_k(rows, k, n, splits, monkeypatch):
+    """Slices of one to a dozen stages, a last tile of few columns and a last stage of few rows."""
+    from axlearn_b200.ops import cuda_ops, int4_ops
+
+    gen = _gen(rows + k)
+    w = int4_ops.quantize_weight(_normal(gen, k, n) * k ** -0.5, group=64)
+    x = _normal(gen, rows, k).bfloat16()
+    y, bound = _linear64(x, w)
+    monkeypatch.setattr(int4_ops, "fused_splits", lambda *_: splits)
+    got = int4_ops.int4_linear(x, w)
+    cuda_ops.check_status()
+    assert ((got.double() - y).abs() <= bound).all()
+    assert torch.equal(got, int4_ops.int4_linear(x, w))
+
+
 @pytest.mark.parametrize("rows", [3, 40, 90])
 def test_linear_takes_strided_rows_and_keeps_rows_apart(rows):
     from axlearn_b200.ops import int4_ops
