@@ -8,11 +8,15 @@
 // [N / 16, K / group, 8, 2, (s, m)] by feature mod 8, feature / 8.  The contraction order is permuted the same way on both
 // sides: a lane reads 16 neighbouring values of a row of x.
 //
-//   int4_linear_kernel   up to 64 rows: features are the M side of the MMA, rows of x its N side.  A CTA takes 64 (32) features
-//                        and a slice of K, its warps every eighth 128 rows of the slice; `cp.async` fills a warp's ring of
+//   int4_linear_kernel   up to 16 rows: features are the M side of the MMA, rows of x its N side.  A CTA takes 64 features and
+//                        a slice of K, its four warps every fourth 128 rows of the slice; `cp.async` fills a warp's ring of
 //                        three units ahead of the arithmetic.  Partial sums meet in shared memory, those of the slices in
 //                        the cluster's.  y = sum_g s_g (sum x c) + m_g sum x, sums of x by an MMA with ones; codes enter as
-//                        denormal bf16 numbers (`int4.cuh`), x is multiplied by 2^kInt4Shift.
+//                        denormal bf16 numbers (`int4.cuh`), x is multiplied by 2^kInt4Shift: no code is ever converted.
+//                        Measured (us; the codes at the copy rate): 1 x 2048 x 2048 3.6 (0.3), 1 x 4096 x 28672 16.9 (9.5: copies
+//                        alone take 11.2, arithmetic alone 15.5), 16 x 14336 x 4096 15.0 (4.9), 1 x 16384 x 18944 33.2 (25.2).
+//                        Masks and shifts of the codes keep the ALU pipe busiest (43%, MMAs 31%); more CTAs an SM with fewer
+//                        features each, or with a shorter ring, were not faster: sums of x and loads of x grow as fast.
 //   int4_expand_kernel   W in bf16 for the tensor-core GEMM of more rows.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -49,28 +53,30 @@ constexpr int kLinWarps = 4, kLinThreads = 32 * kLinWarps;
 constexpr int kLinStages = 3;
 constexpr int kLinMaxSplits = 8;
 
-// kBlocks: 8 rows of x each; kTiles: 16 features each; kGroup: 64 or 128.
-template <int kBlocks, int kTiles, int kGroup>
+constexpr int kLinTiles = 4;  // of 16 features
+
+// kBlocks: 8 rows of x each; kGroup: 64 or 128.
+template <int kBlocks, int kGroup>
 struct Int4Lin {
-  static constexpr int kGroups = 128 / kGroup;                      // of a unit: kTiles x 16 features, 128 rows of W
-  static constexpr int kCodes = kTiles * 1024, kPairs = kTiles * kGroups * 64;
+  static constexpr int kGroups = 128 / kGroup;                      // of a unit: kLinTiles x 16 features, 128 rows of W
+  static constexpr int kCodes = kLinTiles * 1024, kPairs = kLinTiles * kGroups * 64;
   static constexpr int kUnit = kCodes + kPairs;
-  static constexpr int kRows = kBlocks * 8, kFeatures = kTiles * 16;
+  static constexpr int kRows = kBlocks * 8, kFeatures = kLinTiles * 16;
   static constexpr int kPitch = kFeatures + 4;                      // floats of a row of partial sums
   static constexpr int kRing = kLinWarps * kLinStages * kUnit, kSums = (kLinWarps + 1) * kRows * kPitch * 4;
   static constexpr int kSmem = kRing > kSums ? kRing : kSums;
 };
 
-template <int kBlocks, int kTiles, int kGroup>
+template <int kBlocks, int kGroup>
 __global__ void __launch_bounds__(kLinThreads)
 int4_linear_kernel(Int4LinearParams p) {
   chain_link();
-  using L = Int4Lin<kBlocks, kTiles, kGroup>;
+  using L = Int4Lin<kBlocks, kGroup>;
   extern __shared__ __align__(128) uint8_t s_lin[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int n16 = (p.N + 15) / 16, k128 = (p.K + 127) / 128;
   const int split = blockIdx.x % p.splits;
-  const int tile0 = blockIdx.x / p.splits * kTiles;
+  const int tile0 = blockIdx.x / p.splits * kLinTiles;
   const int per_split = (k128 + p.splits - 1) / p.splits;
   const int hi = min(k128, (split + 1) * per_split);
   uint8_t* ring = s_lin + warp * kLinStages * L::kUnit;
@@ -79,7 +85,7 @@ int4_linear_kernel(Int4LinearParams p) {
   auto load = [&](int stage, int kb) {
     const uint32_t dst = sptr(ring) + stage * L::kUnit + lane * 16;
 #pragma unroll
-    for (int i = 0; i < kTiles; ++i) {
+    for (int i = 0; i < kLinTiles; ++i) {
       const bool ok = tile0 + i < n16;
       const int64_t tile = ok ? tile0 + i : 0;
 #pragma unroll
@@ -104,26 +110,24 @@ int4_linear_kernel(Int4LinearParams p) {
     if (kb + i * kLinWarps < hi) load(i, kb + i * kLinWarps);
     cp_commit();
   }
-  float acc[kTiles][kBlocks][4] = {};
+  float acc[kLinTiles][kBlocks][4] = {};
   const __nv_bfloat162 up = __float2bfloat162_rn(kInt4Scale);
-  // 64 rows of W meet 16 neighbouring values of each row of x in a lane: asked for a unit ahead where registers allow.
-  constexpr bool kAhead = kBlocks <= 2;
-  uint4 xv[kAhead ? 2 : 1][kBlocks][2];
+  // 64 rows of W meet 16 neighbouring values of each row of x in a lane: asked for a unit ahead.
+  uint4 xv[2][kBlocks][2];
   auto load_x = [&](int h, int unit) {
 #pragma unroll
     for (int j = 0; j < kBlocks; ++j) {
       const int row = j * 8 + r, k = unit * 128 + h * 64 + c * 16;
       const uint4* src = reinterpret_cast<const uint4*>(p.x + row * p.ldx + k);
       const bool ok = row < p.M && unit < hi;
-      xv[kAhead ? h : 0][j][0] = ok && k < p.K ? src[0] : make_uint4(0, 0, 0, 0);
-      xv[kAhead ? h : 0][j][1] = ok && k + 8 < p.K ? src[1] : make_uint4(0, 0, 0, 0);
+      xv[h][j][0] = ok && k < p.K ? src[0] : make_uint4(0, 0, 0, 0);
+      xv[h][j][1] = ok && k + 8 < p.K ? src[1] : make_uint4(0, 0, 0, 0);
     }
   };
-  if constexpr (kAhead) load_x(0, kb), load_x(1, kb);
+  load_x(0, kb), load_x(1, kb);
   int stage = 0;
   for (; kb < hi; kb += kLinWarps) {
-    float part[kTiles][kBlocks][4], xs[kBlocks][4];
-    if constexpr (!kAhead) load_x(0, kb);
+    float part[kLinTiles][kBlocks][4], xs[kBlocks][4];
     cp_wait_group<kLinStages - 1>();
     __syncwarp();
     const uint8_t* unit = ring + stage * L::kUnit;
@@ -136,29 +140,28 @@ int4_linear_kernel(Int4LinearParams p) {
           for (int e = 0; e < 4; ++e) {
             xs[j][e] = 0.f;
 #pragma unroll
-            for (int i = 0; i < kTiles; ++i) part[i][j][e] = 0.f;
+            for (int i = 0; i < kLinTiles; ++i) part[i][j][e] = 0.f;
           }
         }
       }
-      uint4 w[kTiles];
+      uint4 w[kLinTiles];
 #pragma unroll
-      for (int i = 0; i < kTiles; ++i) w[i] = *reinterpret_cast<const uint4*>(unit + (2 * i + h) * 512 + lane * 16);
+      for (int i = 0; i < kLinTiles; ++i) w[i] = *reinterpret_cast<const uint4*>(unit + (2 * i + h) * 512 + lane * 16);
       uint32_t xb[kBlocks][8];
 #pragma unroll
       for (int j = 0; j < kBlocks; ++j) {
-        const uint32_t* u = reinterpret_cast<const uint32_t*>(xv[kAhead ? h : 0][j]);
+        const uint32_t* u = reinterpret_cast<const uint32_t*>(xv[h][j]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) xb[j][e] = times_bf16x2(u[e], up);
       }
-      if constexpr (kAhead) load_x(h, kb + kLinWarps);
-      else if (h == 0) load_x(1, kb);
+      load_x(h, kb + kLinWarps);
       const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
 #pragma unroll
         for (int j = 0; j < kBlocks; ++j) mma(xs[j], ones, xb[j][2 * q], xb[j][2 * q + 1]);
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
+        for (int i = 0; i < kLinTiles; ++i) {
           const uint32_t word = q == 0 ? w[i].x : q == 1 ? w[i].y : q == 2 ? w[i].z : w[i].w, next = word >> 8;
           const uint32_t a[4] = {int4_low(word), int4_high(word), int4_low(next), int4_high(next)};
 #pragma unroll
@@ -167,7 +170,7 @@ int4_linear_kernel(Int4LinearParams p) {
       }
       if (h == 1 || kGroup == 64) {
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
+        for (int i = 0; i < kLinTiles; ++i) {
           const uint2 u = *reinterpret_cast<const uint2*>(unit + L::kCodes + (i * L::kGroups + (kGroup == 64 ? h : 0)) * 64 + r * 8);
           // x carries kInt4Scale, its products with codes 1 / kInt4Back, those of the features r + 8 sixteen times that.
           const float s0 = pair_s(u.x) * kInt4Back, s1 = pair_s(u.y) * (kInt4Back / 16.f);
@@ -191,7 +194,7 @@ int4_linear_kernel(Int4LinearParams p) {
   __syncthreads();  // the sums overlay the rings
   float* s_sum = reinterpret_cast<float*>(s_lin);
 #pragma unroll
-  for (int i = 0; i < kTiles; ++i)
+  for (int i = 0; i < kLinTiles; ++i)
 #pragma unroll
     for (int j = 0; j < kBlocks; ++j)
 #pragma unroll
@@ -258,10 +261,10 @@ int4_expand_kernel(const uint4* codes, const uint2* pairs, __nv_bfloat16* out, i
   }
 }
 
-template <int kBlocks, int kTiles, int kGroup>
+template <int kBlocks, int kGroup>
 static int launch_int4_linear(Int4LinearParams p, int splits, cudaStream_t stream) {
-  using L = Int4Lin<kBlocks, kTiles, kGroup>;
-  constexpr auto kernel = int4_linear_kernel<kBlocks, kTiles, kGroup>;
+  using L = Int4Lin<kBlocks, kGroup>;
+  constexpr auto kernel = int4_linear_kernel<kBlocks, kGroup>;
   static OptIn opt_in;
   if (!opt_in.done(kernel, L::kSmem)) return -3;
   p.splits = splits;
@@ -280,20 +283,18 @@ static int launch_int4_linear(Int4LinearParams p, int splits, cudaStream_t strea
 
 template <int kGroup>
 static int int4_linear(const Int4LinearParams& p, int splits, cudaStream_t stream) {
-  if (p.M <= 8) return launch_int4_linear<1, 4, kGroup>(p, splits, stream);
-  if (p.M <= 16) return launch_int4_linear<2, 4, kGroup>(p, splits, stream);
-  if (p.M <= 32) return launch_int4_linear<4, 2, kGroup>(p, splits, stream);
-  return launch_int4_linear<8, 1, kGroup>(p, splits, stream);
+  if (p.M <= 8) return launch_int4_linear<1, kGroup>(p, splits, stream);
+  return launch_int4_linear<2, kGroup>(p, splits, stream);
 }
 
 }  // namespace axb
 
-// x [M, K] bf16 with rows of ldx (K, ldx multiples of 8, 16-byte aligned), y [M, N] with rows of ldy; M <= 64.
+// x [M, K] bf16 with rows of ldx (K, ldx multiples of 8, 16-byte aligned), y [M, N] with rows of ldy; M <= 16.
 extern "C" int axb_int4_linear(const void* x, const void* codes, const void* pairs, void* y, int M, int N, int K, int group,
                                int64_t ldx, int64_t ldy, int accumulate, int splits, cudaStream_t stream) {
   using namespace axb;
   const uintptr_t align = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(pairs);
-  if (M < 0 || M > 64 || N < 1 || K < 1 || K % 8 || ldx % 8 || (align & 15) || (group != 64 && group != 128) ||
+  if (M < 0 || M > 16 || N < 1 || K < 1 || K % 8 || ldx % 8 || (align & 15) || (group != 64 && group != 128) ||
       splits < 1 || splits > kLinMaxSplits)
     return -10;
   if (M == 0) return 0;

@@ -34,9 +34,8 @@ c_void_p, c_int, c_int64, c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_int6
 Tensor = torch.Tensor
 
 CACHE_GROUP = 32
-# Rows of x up to which codes are operands as they are, and up to which weights are expanded inside the product; beyond, W is
-# expanded to bf16 once and multiplied by the GEMM.
-MAX_STREAMED_ROWS, MAX_FUSED_ROWS = 16, 128
+# Rows of x up to which weights are expanded inside the product; beyond, W is expanded to bf16 once and multiplied by the GEMM.
+MAX_FUSED_ROWS = 128
 _configured = False
 
 
@@ -168,15 +167,23 @@ def dequantize_weight(w: Int4Weight, dtype: torch.dtype = torch.bfloat16) -> Ten
     return group_values(_unpack_blocks(w.codes), scales).t()[:w.k, :w.n].to(dtype)
 
 
-def linear_splits(rows: int, k: int, n: int, sms: int = 148) -> int:
-    """Slices of K of a product of few rows: one wave of CTAs (four fit an SM; a CTA takes 64 columns, 32 or 16 of more than 16
-    or 32 rows), 512 rows of the weight or more for each.  More than four slices pay where columns are few and K is long."""
-    ctas = -(-n // (64 if rows <= 16 else 32 if rows <= 32 else 16))
+def multiplies_codes(rows: int, n: int) -> bool:
+    """Whether a product multiplies with the codes as they are: up to 8 rows, and up to 16 where columns are few enough for one
+    wave of CTAs (us of 16 rows, so / with weights expanded inside the product, 4096 rows of the weight: 4096 columns 7.8 /
+    8.7, 6144 columns 14.2 / 10.6, 28672 columns 27.0 / 22.8)."""
+    return rows <= 8 or (rows <= 16 and n <= 4096)
+
+
+def linear_splits(k: int, n: int, sms: int = 148) -> int:
+    """Slices of K of a product with the codes: one wave of CTAs (four fit an SM; a CTA takes 64 columns), 512 rows of the weight
+    or more for each.  More than four slices pay where columns are few and K is long (us of one row with 4 / 8: [8192, 2048]
+    7.6 / 6.6, [4096, 2048] 4.8 / 5.0)."""
+    ctas = -(-n // 64)
     return max(1, min(8 if ctas <= 32 and k >= 8192 else 4, k // 512, 4 * sms // ctas))
 
 
 def fused_splits(rows: int, k: int, n: int) -> int:
-    """Slices of K of a product of 17 to 128 rows, the CTAs of a cluster; clusters leave some of the SMs idle, so 128 are counted
+    """Slices of K of a product of up to 128 rows, the CTAs of a cluster; clusters leave some of the SMs idle, so 128 are counted
     on: one CTA of 128 columns on each with 512 rows of the weight or more; of up to 64 rows two with 1024 or more.  (us with
     4 / 8 slices, 64 rows: [14336, 4096] 18.0 / 16.5, [4096, 4096] 10.3 / 10.9.)"""
     tiles = -(-n // 128)
@@ -185,8 +192,8 @@ def fused_splits(rows: int, k: int, n: int) -> int:
 
 def int4_linear(x: Tensor, w: Int4Weight, *, out: Optional[Tensor] = None, accumulate: bool = False) -> Tensor:
     """``x [..., K] @ w`` with fp32 accumulation, rounded to ``x.dtype``; into ``out [..., N]``, or with ``accumulate`` added to
-    it.  Up to 16 rows multiply with the 4-bit weights as they are, more rows with their values rounded to bf16.  Serving
-    only: there is no gradient.  (Sums that overflow fp32 on the way, as with an infinity in x, are NaN.)"""
+    it.  Few rows multiply with the 4-bit weights as they are (``multiplies_codes``), more rows with their values rounded to
+    bf16.  Serving only: there is no gradient.  (Sums that overflow fp32 on the way, as with an infinity in x, are NaN.)"""
     k, n, codes = w.k, w.n, w.codes
     device = x.device
     if x.shape[-1] != k or device != codes.device:
@@ -210,9 +217,9 @@ def int4_linear(x: Tensor, w: Int4Weight, *, out: Optional[Tensor] = None, accum
         x, ldx = x.reshape(rows, k).contiguous(), k
         if x.data_ptr() % 16:
             x = x.clone()
-    if rows <= MAX_STREAMED_ROWS:
+    if multiplies_codes(rows, n):
         _call(device, "axb_int4_linear", x.data_ptr(), codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, n, k, w.group,
-              ldx, n, 1 if accumulate else 0, linear_splits(rows, k, n))
+              ldx, n, 1 if accumulate else 0, linear_splits(k, n))
         return out
     if rows <= MAX_FUSED_ROWS:
         _call(device, "axb_int4_gemm", x.data_ptr(), codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, n, k, w.group,

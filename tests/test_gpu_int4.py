@@ -197,7 +197,7 @@ def _linear64(x, w):
     values = _plain(int4_ops.dequantize_weight, w, torch.float32).double()
     y = x.double() @ values
     terms = x.double().abs() @ values.abs()
-    if x.shape[0] > int4_ops.MAX_STREAMED_ROWS:
+    if not int4_ops.multiplies_codes(x.shape[0], w.n):
         bound = 2.0 ** -8 * terms + 2.0 ** -23 * w.k * terms  # weights rounded to bf16; sums of k terms in any order
     else:
         # Products with 128 + c of up to 128 values (tensor cores cut sums off at 2^-23 of their largest term), 8 steps a group
@@ -244,6 +244,22 @@ def test_linear_with_slices_of_k(rows, k, n, splits, monkeypatch):
     cuda_ops.check_status()
     assert ((got.double() - y).abs() <= bound).all()
     assert torch.equal(got, int4_ops.int4_linear(x, w))
+
+
+@pytest.mark.parametrize("rows", [8, 9, 16, 17])
+@pytest.mark.parametrize("k,n", [(264, 4096), (264, 4104), (8, 4616)])
+def test_linear_where_products_with_codes_end(rows, k, n):
+    from axlearn_b200.ops import cuda_ops, int4_ops
+
+    gen = _gen(rows + n)
+    w = int4_ops.quantize_weight(_normal(gen, k, n) * k ** -0.5, group=64)
+    x = _normal(gen, rows, k).bfloat16()
+    y, bound = _linear64(x, w)
+    got = int4_ops.int4_linear(x, w)
+    cuda_ops.check_status()
+    assert ((got.double() - y).abs() <= bound).all()
+    alone = torch.cat([int4_ops.int4_linear(row, w) for row in x.split(1)])
+    assert ((alone.double() - y).abs() <= bound).all()
 
 
 @pytest.mark.parametrize("rows", [3, 40, 90])
