@@ -297,6 +297,9 @@ __device__ __forceinline__ uint32_t turned_round(uint32_t x) {
   return y;
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
@@ -375,16 +378,16 @@ int4_attn_kernel(Int4AttnParams p) {
   const uint8_t* v_src = p.v_pool.codes + lane % kUnits * 16;
   auto load_tile = [&](int stage, uint32_t slot) {
     const uint32_t at_stage = stage * Tile::kBytes;
+    // Keys that are not there have pairs of zeros; their codes, finite whatever they are, come from the first row.
+    const bool ok = slot != kNone;
+    const uint32_t row = ok ? slot : 0u;
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) {
-      const uint32_t at = __shfl_sync(0xffffffffu, slot, i * kKeys + lane / kUnits);
-      const bool ok = at != kNone;
-      const uint64_t off = ok ? static_cast<uint64_t>(at) * Tile::kRow : 0;
-      cp_async16(k_dst + at_stage + i * 512, k_src + off, ok);
-      cp_async16(v_dst + at_stage + i * 512, v_src + off, ok);
+      const uint64_t off = static_cast<uint64_t>(__shfl_sync(0xffffffffu, row, i * kKeys + lane / kUnits)) * Tile::kRow;
+      cp_async16(k_dst + at_stage + i * 512, k_src + off);
+      cp_async16(v_dst + at_stage + i * 512, v_src + off);
     }
-    const bool ok = slot != kNone;
-    const uint64_t off = ok ? static_cast<uint64_t>(slot) * G : 0;
+    const uint64_t off = static_cast<uint64_t>(row) * G;
     if constexpr (G == 4) {
       cp_async16(pair_dst + at_stage, p.k_pool.pairs + off, ok);
       cp_async16(pair_dst + at_stage + kAttnKeys * Tile::kPairs, p.v_pool.pairs + off, ok);
@@ -876,7 +879,8 @@ extern "C" int axb_int4_decode_attn(const void* q, void* k_codes, void* k_pairs,
                                     cudaStream_t stream) {
   using namespace axb;
   if ((head_dim != 64 && head_dim != 128) || page_size < 1 || num_kv_heads < 1 || num_q_heads < 1 ||
-      num_q_heads % num_kv_heads || splits < 1 || B < 0 || B > 65535 || !(softmax_scale > 0.f && softmax_scale < 1048576.f) ||
+      num_q_heads % num_kv_heads || num_pages < 1 || splits < 1 || B < 0 || B > 65535 ||
+      !(softmax_scale > 0.f && softmax_scale < 1048576.f) ||
       static_cast<int64_t>(num_pages) * num_kv_heads * page_size >= 0xffffffffll || (angle != nullptr && angle_rows < 1))
     return -10;
   for (const void* x : {q, static_cast<const void*>(angle), static_cast<const void*>(k_codes), static_cast<const void*>(k_pairs),

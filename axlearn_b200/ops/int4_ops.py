@@ -277,8 +277,8 @@ def _check_pages(k_pages: Int4Pages, v_pages: Int4Pages, page_table: Tensor, bat
     (kc, ks), (vc, vs) = k_pages, v_pages
     shape = kc.shape
     num_pages, nkv, page_size, half = shape if len(shape) == 4 else (0, 0, 0, 0)
-    if (half * 2 != head_dim or head_dim not in (64, 128) or not nkv or heads % nkv or not page_size or vc.shape != shape
-            or ks.shape != (num_pages, nkv, page_size, half // 16, 2) or vs.shape != ks.shape):
+    if (half * 2 != head_dim or head_dim not in (64, 128) or not nkv or heads % nkv or not num_pages or not page_size
+            or vc.shape != shape or ks.shape != (num_pages, nkv, page_size, half // 16, 2) or vs.shape != ks.shape):
         raise ValueError(f"4-bit pages {tuple(shape)} with {tuple(ks.shape)}, {tuple(vc.shape)} with {tuple(vs.shape)} for {heads} "
                          f"heads of {head_dim} (64 or 128)")
     for codes, scales in (k_pages, v_pages):

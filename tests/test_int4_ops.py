@@ -252,6 +252,16 @@ def test_append_refuses(change, error):
         int4_ops.append_int4(**{**args, **change})
 
 
+def test_a_pool_without_pages_is_refused():
+    empty, table = int4_ops.int4_pages(0, 4, 2, 64), torch.zeros(2, 3, dtype=torch.int32)
+    lengths = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        int4_ops.paged_decode_attention_int4(torch.zeros(2, 4, 64).bfloat16(), empty, empty, table, lengths)
+    rows = torch.zeros(2, 1, 2, 64).bfloat16()
+    with pytest.raises(ValueError):
+        int4_ops.append_int4(rows, rows, empty, empty, table, lengths)
+
+
 def test_weights_and_products_refuse():
     w = int4_ops.quantize_weight(_values(64, 16))
     for shape, group in (((60, 16), 128), ((64, 12), 128), ((64, 16), 32)):
