@@ -1,5 +1,5 @@
-// y[M, N] = x[M, K] W (+ y) for up to 128 rows with weights held in 4 bits (layout: int4_linear.cu), on the fifth-generation
-// tensor cores: 128 features are the M side of the MMA, the rows of x its N side.
+// y[M, N] = x[M, K] W (+ y) for up to 512 rows with weights held in 4 bits (layout: int4_linear.cu), on the fifth-generation
+// tensor cores: 128 features are the M side of the MMA, up to 128 rows of x its N side.
 //
 // Eight warps feed: each owns 16 features and turns their codes of 128 rows of W into bf16 values m + s c (one rounding, 2^-9
 // of a weight, as in the expansion for the GEMM of more rows), which `tcgen05.st` puts into tensor memory, so that weights
@@ -13,6 +13,8 @@
 // Measured (us; the codes at the copy rate): 64 x 4096 x 22016 24.2 (8.3), 64 x 14336 x 4096 16.5 (5.1), 128 x 4096 x 28672 39
 // (10.8).  A stage of one CTA an SM takes 0.35 us, of two 0.27, by what the conversion and the MMAs of 64 columns take.
 // One CTA an SM with sixteen feeding warps and clusters that share runs of tiles evenly was 26.2, 18.4 and 36.8.
+// Blocks of 128 rows against one expansion and the GEMM: 256 x 4096 x 28672 77 / 121, 512 x 4096 x 4096 20.8 / 24.4, 1024 rows of
+// it 40 / 35.
 //
 // K slices are the CTAs of a cluster; partial sums meet in distributed shared memory in a fixed order.
 //
@@ -34,7 +36,7 @@ struct Int4GemmParams {
   __nv_bfloat16* y;        // [M, ldy]
   int64_t ldy;
   int M, N, K;
-  int accumulate, splits;
+  int accumulate, splits, row_blocks;
   int* status;
 };
 
@@ -115,8 +117,10 @@ int4_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = static_cast<int>(blockIdx.x) % p.splits;
-  const int n0 = static_cast<int>(blockIdx.x) / p.splits * kIgFeatures;
+  // Blocks of rows of one tile run side by side: its codes come from memory once.
+  const int split = static_cast<int>(blockIdx.x) % p.splits, block = static_cast<int>(blockIdx.x) / p.splits;
+  const int row0 = block % p.row_blocks * BN, n0 = block / p.row_blocks * kIgFeatures;
+  const int rows = min(p.M - row0, BN);
   const int k128 = (p.K + 127) / 128;
   const int kb_lo = split * k128 / p.splits, count = (split + 1) * k128 / p.splits - kb_lo;
 
@@ -212,8 +216,8 @@ int4_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         if (it >= S::kRing && !mbar_wait(&empty_bar[x.slot], x.phase ^ 1, p.status, kStatusWaitTimeoutProducer)) break;
         uint8_t* tile = smem + x.slot * (2 * S::kX);
         mbar_arrive_expect_tx(&full_bar[x.slot], 2 * S::kX);
-        tma_load_2d(tile, &map_x, &full_bar[x.slot], (kb_lo + it) * 128, 0);
-        tma_load_2d(tile + S::kX, &map_x, &full_bar[x.slot], (kb_lo + it) * 128 + 64, 0);
+        tma_load_2d(tile, &map_x, &full_bar[x.slot], (kb_lo + it) * 128, row0);
+        tma_load_2d(tile + S::kX, &map_x, &full_bar[x.slot], (kb_lo + it) * 128 + 64, row0);
         x.next();
       }
     }
@@ -263,7 +267,7 @@ int4_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     constexpr int kStep = BN >= 32 ? 16 : 8;
 #pragma unroll 1
     for (int c0 = (warp >> 2) * (BN / 2); c0 < ((warp >> 2) + 1) * (BN / 2); c0 += kStep) {
-      if (c0 >= p.M) break;
+      if (c0 >= rows) break;
       uint32_t r[16];
       if constexpr (kStep == 16) tmem_ld_32x16(taddr + c0, r);
       else tmem_ld_32x16(taddr + (c0 & ~15), r);
@@ -272,12 +276,12 @@ int4_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
       for (int j = 0; j < 16; ++j) {
         if (kStep == 8 && (j >> 3) != (c0 >> 3 & 1)) continue;
         const int row = (kStep == 16 ? c0 : (c0 & ~15)) + j;
-        if (row >= p.M) continue;
+        if (row >= rows) continue;
         float v = __uint_as_float(r[j]) * (1.f / kIgLow);
         if (p.splits > 1) {
           part[row * kIgFeatures + feature] = v;
         } else if (n < p.N) {
-          __nv_bfloat16* dst = p.y + row * p.ldy + n;
+          __nv_bfloat16* dst = p.y + (row0 + row) * p.ldy + n;
           if (p.accumulate) v += __bfloat162float(*dst);
           *dst = __float2bfloat16(v);
         }
@@ -287,7 +291,7 @@ int4_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   if (p.splits > 1) {
     cluster_sync_all();
     if (warp < kIgWarps && ok && n < p.N) {
-      for (int row = split + (warp >> 2) * p.splits; row < p.M; row += 2 * p.splits) {
+      for (int row = split + (warp >> 2) * p.splits; row < rows; row += 2 * p.splits) {
         float v[kIgMaxSplits];
 #pragma unroll
         for (int s = 0; s < kIgMaxSplits; ++s)
@@ -295,7 +299,7 @@ int4_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         float sum = v[0];
 #pragma unroll
         for (int s = 1; s < kIgMaxSplits; ++s) sum += v[s];
-        __nv_bfloat16* dst = p.y + row * p.ldy + n;
+        __nv_bfloat16* dst = p.y + (row0 + row) * p.ldy + n;
         if (p.accumulate) sum += __bfloat162float(*dst);
         *dst = __float2bfloat16(sum);
       }
@@ -339,7 +343,7 @@ static int launch_int4_gemm(const void* x, int64_t ldx, const void* codes, const
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {static_cast<unsigned>(p.splits), 1, 1};
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((p.N + kIgFeatures - 1) / kIgFeatures * p.splits));
+  cfg.gridDim = dim3(static_cast<unsigned>((p.N + kIgFeatures - 1) / kIgFeatures * p.row_blocks * p.splits));
   cfg.blockDim = dim3(kIgThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = stream;
@@ -358,16 +362,16 @@ static int int4_gemm(const void* x, int64_t ldx, const void* codes, const void* 
 
 }  // namespace axb
 
-// x [M, K] bf16 with rows of ldx (K, ldx multiples of 8, 16-byte aligned), y [M, N] with rows of ldy; M <= 128.  `splits`:
+// x [M, K] bf16 with rows of ldx (K, ldx multiples of 8, 16-byte aligned), y [M, N] with rows of ldy; M <= 512.  `splits`:
 // slices of K, up to 8 and one for every 128 rows of W at most.
 extern "C" int axb_int4_gemm(const void* x, const void* codes, const void* pairs, void* y, int M, int N, int K, int group,
                              int64_t ldx, int64_t ldy, int accumulate, int splits, int* status, cudaStream_t stream) {
   using namespace axb;
   const uintptr_t align = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(pairs);
-  if (M < 0 || M > 128 || N < 1 || K < 1 || K % 8 || ldx % 8 || (align & 15) || (group != 64 && group != 128) || splits < 1 ||
+  if (M < 0 || M > 512 || N < 1 || K < 1 || K % 8 || ldx % 8 || (align & 15) || (group != 64 && group != 128) || splits < 1 ||
       splits > kIgMaxSplits || splits > (K + 127) / 128)
     return -10;
   if (M == 0) return 0;
-  const Int4GemmParams p{static_cast<__nv_bfloat16*>(y), ldy, M, N, K, accumulate, splits, status};
+  const Int4GemmParams p{static_cast<__nv_bfloat16*>(y), ldy, M, N, K, accumulate, splits, (M + 127) / 128, status};
   return group == 64 ? int4_gemm<64>(x, ldx, codes, pairs, p, stream) : int4_gemm<128>(x, ldx, codes, pairs, p, stream);
 }

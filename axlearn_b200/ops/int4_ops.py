@@ -34,8 +34,9 @@ c_void_p, c_int, c_int64, c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_int6
 Tensor = torch.Tensor
 
 CACHE_GROUP = 32
-# Rows of x up to which weights are expanded inside the product; beyond, W is expanded to bf16 once and multiplied by the GEMM.
-MAX_FUSED_ROWS = 128
+# Rows of x up to which weights are expanded inside the product, for each 128 rows again; beyond, W is expanded to bf16 once and
+# multiplied by the GEMM (us so / with the GEMM: 256 x [4096, 28672] 77 / 121, 512 x [4096, 22016] 97 / 113, 768 rows of it 155 / 138).
+MAX_FUSED_ROWS = 512
 _configured = False
 
 
@@ -183,10 +184,10 @@ def linear_splits(k: int, n: int, sms: int = 148) -> int:
 
 
 def fused_splits(rows: int, k: int, n: int) -> int:
-    """Slices of K of a product of up to 128 rows, the CTAs of a cluster; clusters leave some of the SMs idle, so 128 are counted
-    on: one CTA of 128 columns on each with 512 rows of the weight or more; of up to 64 rows two with 1024 or more.  (us with
-    4 / 8 slices, 64 rows: [14336, 4096] 18.0 / 16.5, [4096, 4096] 10.3 / 10.9.)"""
-    tiles = -(-n // 128)
+    """Slices of K of a product with weights expanded inside, the CTAs of a cluster; clusters leave some of the SMs idle, so 128
+    are counted on: one CTA of 128 columns and up to 128 rows on each with 512 rows of the weight or more; of up to 64 rows two
+    with 1024 or more.  (us with 4 / 8 slices, 64 rows: [14336, 4096] 18.0 / 16.5, [4096, 4096] 10.3 / 10.9.)"""
+    tiles = -(-n // 128) * -(-rows // 128)
     return max(1, min(8, max(min(128 // tiles, k // 512), min(256 // tiles, k // 1024) if rows <= 64 else 0)))
 
 

@@ -262,6 +262,26 @@ def test_linear_where_products_with_codes_end(rows, k, n):
     assert ((alone.double() - y).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("rows", [129, 250, 384, 512, 513])
+@pytest.mark.parametrize("k,n,group", [(1096, 136, 64), (2048, 392, 128), (8, 1160, 64)])
+def test_linear_in_blocks_of_rows(rows, k, n, group):
+    """A last block of one row and of most rows, with and without slices of K; the first rows behind the blocks."""
+    from axlearn_b200.ops import cuda_ops, int4_ops
+
+    gen = _gen(rows + k)
+    w = int4_ops.quantize_weight(_normal(gen, k, n) * k ** -0.5, group=group)
+    x = _normal(gen, rows, k + 8).bfloat16()[:, :k]
+    y, bound = _linear64(x, w)
+    out = _normal(gen, rows + 1, n).bfloat16()
+    before = out.clone()
+    assert ((int4_ops.int4_linear(x, w, out=out[:rows]).double() - y).abs() <= bound).all()
+    assert torch.equal(out[rows], before[rows])
+    want = before[:rows].double() + y
+    got = int4_ops.int4_linear(x, w, out=before[:rows], accumulate=True)
+    cuda_ops.check_status()
+    assert ((got.double() - want).abs() <= bound + 2.0 ** -8 * (want.abs() + y.abs() + bound)).all()
+
+
 @pytest.mark.parametrize("rows", [3, 40, 90])
 def test_linear_takes_strided_rows_and_keeps_rows_apart(rows):
     from axlearn_b200.ops import int4_ops
