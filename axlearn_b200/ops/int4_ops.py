@@ -194,7 +194,8 @@ def fused_splits(rows: int, k: int, n: int) -> int:
 def int4_linear(x: Tensor, w: Int4Weight, *, out: Optional[Tensor] = None, accumulate: bool = False) -> Tensor:
     """``x [..., K] @ w`` with fp32 accumulation, rounded to ``x.dtype``; into ``out [..., N]``, or with ``accumulate`` added to
     it.  Few rows multiply with the 4-bit weights as they are (``multiplies_codes``), more rows with their values rounded to
-    bf16.  Serving only: there is no gradient.  (Sums that overflow fp32 on the way, as with an infinity in x, are NaN.)"""
+    bf16.  Serving only: there is no gradient.  Products keep their digits for x from 2^-57 up to 2^56, weights from 2^-62 and
+    steps below 2^31; sums that overflow fp32 on the way, as with an infinity in x, are NaN."""
     k, n, codes = w.k, w.n, w.codes
     device = x.device
     if x.shape[-1] != k or device != codes.device:
@@ -228,6 +229,10 @@ def int4_linear(x: Tensor, w: Int4Weight, *, out: Optional[Tensor] = None, accum
         return out
     expanded = dequantize_weight(w)
     with torch.cuda.device(device):
+        if out.data_ptr() % 16:  # a view into a larger buffer: the GEMM stores vectors
+            y = out.clone() if accumulate else torch.empty_like(out)
+            cuda_ops.gemm(x, expanded, out=y.view(rows, n), accumulate=accumulate)
+            return out.copy_(y)
         cuda_ops.gemm(x, expanded, out=out.view(rows, n), accumulate=accumulate)
     return out
 
@@ -400,8 +405,7 @@ def paged_decode_attention_int4(q: Tensor, k_pages: Int4Pages, v_pages: Int4Page
                                 out: Optional[Tensor] = None, scratch: Optional[Tensor] = None) -> Tensor:
     """q ``[B, Nq, H]``; page_table ``[B, max_pages]``, lengths ``[B]`` int32 (valid tokens per sequence; 0: zeros).  Query heads
     are grouped by KV head.  ``scratch``: ``attention_scratch_floats`` fp32 values, for more than eight splits (made a
-    multiple of eight).  Returns
-    ``[B, Nq, H]``."""
+    multiple of eight); calls that overlap on the GPU need one each.  Returns ``[B, Nq, H]``."""
     b, nq, h = q.shape
     device = q.device
     num_pages, nkv, page_size = _check_pages(k_pages, v_pages, page_table, b, nq, h, device)
@@ -468,6 +472,8 @@ def rope_decode_attention_int4(qkv: Tensor, k_pages: Int4Pages, v_pages: Int4Pag
     H / 2, 2]`` (``decode_ops.rope_table``), appends key and value to the cache and attends to it.  Rows of length 0 append
     nothing and get zeros.  Returns ``[B, Nq, H]``."""
     nkv, h = _check_packed(qkv, k_pages, table, num_q_heads)
+    if qkv.dim() != 2:
+        raise ValueError(f"a step takes one token a sequence, [B, width]: {tuple(qkv.shape)}")
     b, device = qkv.shape[0], qkv.device
     num_pages, _, page_size = _check_pages(k_pages, v_pages, page_table, b, num_q_heads, h, device)
     _check_counts(lengths, b, "lengths", device)
@@ -476,6 +482,8 @@ def rope_decode_attention_int4(qkv: Tensor, k_pages: Int4Pages, v_pages: Int4Pag
     if not _on_kernel(qkv):
         q, k, v = (x[:, None] for x in _split_qkv(qkv, num_q_heads, nkv))
         pos = lengths[:, None].long() - 1
+        if not qkv.is_cuda and bool((pos >= table.shape[0]).any()):
+            raise IndexError(f"a position behind a rotation table of {table.shape[0]}")
         q, k = _rotate(q, table, pos), _rotate(k, table, pos)
         _append_plain(k, v, k_pages, v_pages, page_table, lengths - 1, (lengths > 0).to(torch.int32))
         return paged_decode_attention_int4(q[:, 0], k_pages, v_pages, page_table, lengths, softmax_scale=softmax_scale)

@@ -282,6 +282,68 @@ def test_linear_in_blocks_of_rows(rows, k, n, group):
     assert ((got.double() - want).abs() <= bound + 2.0 ** -8 * (want.abs() + y.abs() + bound)).all()
 
 
+@pytest.mark.parametrize("rows", [3, 12, 40, 200, 600])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_linear_into_a_place_that_is_not_aligned(rows, accumulate):
+    from axlearn_b200.ops import cuda_ops, int4_ops
+
+    gen = _gen(rows)
+    w = int4_ops.quantize_weight(_normal(gen, 264, 4104) * 264 ** -0.5)
+    x = _normal(gen, rows, 264).bfloat16()
+    flat = torch.ones(rows * 4104 + 2, dtype=torch.bfloat16, device="cuda")
+    out = flat[1:-1].view(rows, 4104)
+    want = int4_ops.int4_linear(x, w, out=torch.ones_like(out), accumulate=accumulate)
+    assert torch.equal(int4_ops.int4_linear(x, w, out=out, accumulate=accumulate), want)
+    cuda_ops.check_status()
+    assert flat[0] == 1 and flat[-1] == 1
+
+
+@pytest.mark.parametrize("rows", [5, 12, 40, 200])
+@pytest.mark.parametrize("x_scale,w_scale", [(2.0 ** 40, 2.0 ** 20), (2.0 ** -40, 2.0 ** -40), (2.0 ** 50, 2.0 ** -50)])
+def test_linear_of_small_and_large_values(rows, x_scale, w_scale):
+    """Powers of two leave every digit as it is."""
+    from axlearn_b200.ops import int4_ops
+
+    gen = _gen(rows)
+    weights, x = _normal(gen, 520, 4104), _normal(gen, rows, 520).bfloat16()
+    plain = int4_ops.int4_linear(x, int4_ops.quantize_weight(weights))
+    scaled = int4_ops.int4_linear(x * x_scale, int4_ops.quantize_weight(weights * w_scale))
+    assert torch.equal(scaled, plain * (x_scale * w_scale))
+
+
+def test_products_of_all_kinds_replay_in_graphs_side_by_side():
+    """Two graphs of the same weights on two streams at once, each with the bits of separate calls."""
+    from axlearn_b200.ops import cuda_ops, int4_ops
+
+    gen = _gen(31)
+    w = int4_ops.quantize_weight(_normal(gen, 1032, 4616) * 1032 ** -0.5)
+    v = int4_ops.quantize_weight(_normal(gen, 4616, 264) * 4616 ** -0.5, group=64)
+    kinds = (1, 12, 40, 128, 300, 600)
+    inputs = [[torch.empty(rows, 1032, dtype=torch.bfloat16, device="cuda") for rows in kinds] for _ in range(2)]
+
+    def run(xs):
+        return [int4_ops.int4_linear(int4_ops.int4_linear(x, w), v) for x in xs]
+
+    streams, graphs, outs = [torch.cuda.Stream() for _ in range(2)], [], []
+    run(inputs[0])
+    for xs in inputs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]), cuda_ops.chained_launches():
+            outs.append(run(xs))
+    for seed in (32, 33, 34):
+        for i, xs in enumerate(inputs):
+            for x in xs:
+                x.copy_(_normal(_gen(2 * seed + i), *x.shape))
+        torch.cuda.synchronize()
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for xs, got in zip(inputs, outs):
+            assert all(torch.equal(a, b) for a, b in zip(got, run(xs)))
+    cuda_ops.check_status()
+
+
 @pytest.mark.parametrize("rows", [3, 40, 90])
 def test_linear_takes_strided_rows_and_keeps_rows_apart(rows):
     from axlearn_b200.ops import int4_ops

@@ -252,6 +252,18 @@ def test_append_refuses(change, error):
         int4_ops.append_int4(**{**args, **change})
 
 
+def test_a_step_refuses_tokens_it_does_not_take():
+    k_pages, v_pages, table = _cache(2, 3, 4, 2, 64)
+    rope, lengths = torch.zeros(8, 32, 2), torch.tensor([8, 0], dtype=torch.int32)
+    args = dict(num_q_heads=4, softmax_scale=0.1)
+    qkv = _values(2, 8 * 64).bfloat16()
+    int4_ops.rope_decode_attention_int4(qkv, k_pages, v_pages, table, lengths, rope, **args)
+    with pytest.raises(ValueError):  # two tokens a sequence
+        int4_ops.rope_decode_attention_int4(_values(2, 2, 8 * 64).bfloat16(), k_pages, v_pages, table, lengths, rope, **args)
+    with pytest.raises(IndexError):  # position 8 of 8
+        int4_ops.rope_decode_attention_int4(qkv, k_pages, v_pages, table, lengths + 1, rope, **args)
+
+
 def test_a_pool_without_pages_is_refused():
     empty, table = int4_ops.int4_pages(0, 4, 2, 64), torch.zeros(2, 3, dtype=torch.int32)
     lengths = torch.zeros(2, dtype=torch.int32)
