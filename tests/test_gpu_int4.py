@@ -118,6 +118,75 @@ def test_rows_behind_a_sequence_and_other_pages_are_not_read(dim):
     assert torch.equal(before, after)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_scale,v_scale", [(2.0 ** 40, 2.0 ** 40), (2.0 ** -40, 2.0 ** -40), (1.0, 2.0 ** -40)])
+def test_attention_over_small_and_large_values(dim, q_scale, v_scale):
+    """Powers of two that leave the scores as they are leave every digit as it is."""
+    from axlearn_b200.ops import int4_ops
+
+    k_pages, v_pages, table = _cache(2, 20, 16, 2, dim, seed=7)
+    lengths = torch.tensor([320, 77], dtype=torch.int32, device="cuda")
+    q = _normal(_gen(8), 2, 8, dim).bfloat16()
+    plain = int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, lengths)
+    k_pages, v_pages = k_pages._replace(scales=k_pages.scales / q_scale), v_pages._replace(scales=v_pages.scales * v_scale)
+    assert torch.equal(int4_ops.paged_decode_attention_int4(q * q_scale, k_pages, v_pages, table, lengths), plain * v_scale)
+
+
+@pytest.mark.parametrize("splits", [1, 8, 16])
+def test_scores_far_apart(splits):
+    """One key that takes all, early or late, and scores that climb by more than the slack from tile to tile."""
+    from axlearn_b200.ops import int4_ops
+
+    k_pages, v_pages, table = _cache(3, 20, 16, 1, 128, seed=9)
+    q = torch.zeros(3, 4, 128, device="cuda").bfloat16()
+    q[:, :, 0] = 100.0
+    k = torch.zeros(3, 320, 1, 128, device="cuda")
+    k[0, 5, 0, 0], k[1, 318, 0, 0], k[2, :, 0, 0] = 30.0, 30.0, torch.arange(320, device="cuda") * 0.25 - 40
+    start = torch.zeros(3, dtype=torch.int32, device="cuda")
+    int4_ops.append_int4(k.bfloat16(), _normal(_gen(10), 3, 320, 1, 128).bfloat16(), k_pages, v_pages, table, start)
+    lengths = torch.tensor([320, 319, 320], dtype=torch.int32, device="cuda")
+    out = int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, lengths, splits=splits)
+    want, bound = _attention64(q, k_pages, v_pages, table, lengths, 128 ** -0.5)
+    assert ((out.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dim,page_size", [(128, 64), (64, 128)])
+def test_pools_beyond_32_bits(dim, page_size):
+    """Pages whose codes lie more than 2^32 bytes into the pool: append, step and attention as over a small pool."""
+    from axlearn_b200.ops import cuda_ops, decode_ops, int4_ops
+
+    kv, b, used = 8, 2, 6
+    pages = 2 ** 32 // (kv * page_size * (dim // 2)) + 40
+    if torch.cuda.mem_get_info()[0] < 30 * 2 ** 30:
+        pytest.skip("a pool of 12 GB")
+    small = _cache(b, used, page_size, kv, dim, seed=11, spare=0)
+    high = [int4_ops.int4_pages(pages, page_size, kv, dim, device="cuda") for _ in range(2)]
+    for pool, low in zip(high, small):
+        pool.codes[-b * used:], pool.scales[-b * used:] = low.codes, low.scales
+    table = small[2] + (pages - b * used)
+    lengths = torch.tensor([used * page_size - 3, 200], dtype=torch.int32, device="cuda")
+    gen = _gen(12)
+    q = _normal(gen, b, 16, dim).bfloat16()
+    qkv = _normal(gen, b, (16 + 2 * kv) * dim).bfloat16()
+    new = [_normal(gen, b, 30, kv, dim).bfloat16() for _ in range(2)]
+    rope = decode_ops.rope_table(used * page_size, dim, 1e4, "cuda")
+
+    def run(k_pages, v_pages, table):
+        outs = []
+        for splits in (1, 4, 16):
+            outs.append(int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, lengths, splits=splits))
+        int4_ops.append_int4(*new, k_pages, v_pages, table, lengths - 40)
+        outs.append(int4_ops.rope_decode_attention_int4(qkv, k_pages, v_pages, table, lengths, rope, num_q_heads=16, softmax_scale=0.1))
+        return outs
+
+    for got, want in zip(run(*high, table), run(*small)):
+        assert torch.equal(got, want)
+    cuda_ops.check_status()
+    for pool, low in zip(high, small):
+        assert torch.equal(pool.codes[-b * used:], low.codes) and torch.equal(pool.scales[-b * used:], low.scales)
+        assert not pool.codes[:64].any() and not pool.codes[-b * used - 64:-b * used].any()
+
+
 def test_values_that_are_not_numbers_stay_where_they_belong():
     from axlearn_b200.ops import int4_ops
 
@@ -342,6 +411,28 @@ def test_products_of_all_kinds_replay_in_graphs_side_by_side():
         for xs, got in zip(inputs, outs):
             assert all(torch.equal(a, b) for a, b in zip(got, run(xs)))
     cuda_ops.check_status()
+
+
+@pytest.mark.parametrize("rows", [1, 12, 40])
+def test_linear_of_codes_beyond_32_bits(rows):
+    from axlearn_b200.ops import cuda_ops, int4_ops
+
+    k, n = 16384, 2 ** 33 // 16384 + 128
+    if torch.cuda.mem_get_info()[0] < 30 * 2 ** 30:
+        pytest.skip("codes of 4.3 GB")
+    part = int4_ops.quantize_weight(_normal(_gen(20), k, 64) * k ** -0.5)
+    codes = torch.zeros(n // 16, k // 64, 512, dtype=torch.uint8, device="cuda")
+    scales = torch.zeros(n // 16, k // 128, 8, 2, 2, dtype=torch.bfloat16, device="cuda")
+    codes[-4:], scales[-4:] = part.codes, part.scales
+    x = _normal(_gen(rows), rows, k).bfloat16()
+    got = int4_ops.int4_linear(x, int4_ops.Int4Weight(codes, scales, k=k, n=n, group=128))
+    cuda_ops.check_status()
+    values = _plain(int4_ops.dequantize_weight, part, torch.float32).double()
+    y, terms = x.double() @ values, x.double().abs() @ values.abs()
+    # Weights may be rounded to bf16, the output is, sums of k terms in any order.
+    bound = 2.0 ** -8 * terms + 2.0 ** -23 * k * terms
+    assert ((got[:, -64:].double() - y).abs() <= bound + 2.0 ** -8 * (y.abs() + bound)).all()
+    assert not got[:, :-64].any()
 
 
 @pytest.mark.parametrize("rows", [3, 40, 90])
