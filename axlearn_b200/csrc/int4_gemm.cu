@@ -1,18 +1,19 @@
 // y[M, N] = x[M, K] W (+ y) for up to 512 rows with weights held in 4 bits (layout: int4_linear.cu), on the fifth-generation
 // tensor cores: 128 features are the M side of the MMA, up to 128 rows of x its N side.
 //
-// Eight warps feed: each owns 16 features and turns their codes of 128 rows of W into bf16 values m + s c (one rounding, 2^-9
+// Up to eight warps feed: each owns 16 features and turns their codes of 128 rows of W into bf16 values m + s c (one rounding, 2^-9
 // of a weight, as in the expansion for the GEMM of more rows), which `tcgen05.st` puts into tensor memory, so that weights
 // never pass through shared memory once they are 16 bits wide: writing and reading them there would cost eight times the
 // bytes of the codes.  A 16x256b store takes from lane (r, c) the columns 2c, 2c + 1 of every k16 step, 4 rows of W: the word c of
 // piece (r, s) of a block for step s.  `ldmatrix` hands out words that way, pieces being rows of its matrices, and x keeps its
 // own order over K.  Codes (64-byte swizzle: no bank conflicts), pairs and x come by TMA: with 16-byte `cp.async` by the
 // feeding warps the copies alone, about 32 cycles of the load unit for each of a warp, took 80% of the product's time.
-// A feeding warp has the next stage's codes in registers before it waits for a place.
 //
-// Measured (us; the codes at the copy rate): 64 x 4096 x 22016 24.2 (8.3), 64 x 14336 x 4096 16.5 (5.1), 128 x 4096 x 28672 39
-// (10.8).  A stage of one CTA an SM takes 0.35 us, of two 0.27, by what the conversion and the MMAs of 64 columns take.
-// One CTA an SM with sixteen feeding warps and clusters that share runs of tiles evenly was 26.2, 18.4 and 36.8.
+// Measured (us; the codes at the copy rate): 64 x 4096 x 22016 22.9 (8.3), 64 x 14336 x 4096 17.1 (5.1), 64 x 4096 x 11008 15.5 (4.0),
+// 128 x 4096 x 28672 40 (10.8).  A stage of one CTA an SM takes 0.35 us, a feeding warp's chain of waits, words, values and
+// store; of two 0.27, by the instructions of both.  So the loop is short: with next codes and values ahead of the waits it
+// was as fast or 4% slower, unrolled round the rings half as fast (the instruction caches).  One CTA an SM with sixteen
+// feeding warps and clusters that share runs of tiles evenly was 26.2, 18.4 and 36.8.
 // Blocks of 128 rows against one expansion and the GEMM: 256 x 4096 x 28672 77 / 121, 512 x 4096 x 4096 20.8 / 24.4, 1024 rows of
 // it 40 / 35.
 //
@@ -37,6 +38,7 @@ struct Int4GemmParams {
   int64_t ldy;
   int M, N, K;
   int accumulate, splits, row_blocks;
+  int warps;               // that feed: a tile is 16 features for each
   int* status;
 };
 
@@ -119,19 +121,19 @@ int4_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // Blocks of rows of one tile run side by side: its codes come from memory once.
   const int split = static_cast<int>(blockIdx.x) % p.splits, block = static_cast<int>(blockIdx.x) / p.splits;
-  const int row0 = block % p.row_blocks * BN, n0 = block / p.row_blocks * kIgFeatures;
+  const int row0 = block % p.row_blocks * BN, n0 = block / p.row_blocks * (16 * p.warps);
   const int rows = min(p.M - row0, BN);
   const int k128 = (p.K + 127) / 128;
   const int kb_lo = split * k128 / p.splits, count = (split + 1) * k128 / p.splits - kb_lo;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kRing; ++i) {
-      mbar_init(&full_bar[i], kIgWarps + 1);
+      mbar_init(&full_bar[i], p.warps + 1);
       mbar_init(&empty_bar[i], 1);
     }
     for (int i = 0; i < S::kCodeRing; ++i) {
       mbar_init(&code_full[i], 1);
-      mbar_init(&code_empty[i], kIgWarps);
+      mbar_init(&code_empty[i], p.warps);
     }
     mbar_init(done_bar, 1);
     fence_barrier_init();
@@ -149,58 +151,43 @@ int4_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   constexpr int kPairBytes = kGroup == 64 ? 128 : 64;  // of a stage and 16 features
   bool ok = true;
   if (warp < kIgWarps) {
-    // Tensor-memory lanes [32 (warp % 4) + 16 (warp / 4), + 16): features of this warp, in their order.
-    const int sub = 2 * (warp & 3) + (warp >> 2);
-    const uint32_t a_addr = tmem + (static_cast<uint32_t>(sub * 16) << 16) + S::kACol;
+    // Features 16 warp .. + 15 of the tile are the tensor-memory lanes from 32 (warp % 4) + 16 (warp / 4) on.
+    const uint32_t a_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32 + (warp >> 2) * 16) << 16) + S::kACol;
     const int r = lane >> 2;
     // Row lane % 8 of matrix lane / 8: the copy swaps 16-byte units as the 64-byte swizzle does.
-    const uint8_t* mine = smem + S::kXBytes + sub * 1024 + (lane & 7) * 64 + (((lane >> 3) ^ (lane >> 1 & 3)) << 4);
-    const uint8_t* mine_pairs = smem + S::kXBytes + S::kCodeBytes + sub * kPairBytes + r * 8;
-    uint32_t w[2][4];
-    uint2 u[128 / kGroup];
+    const uint8_t* mine = smem + S::kXBytes + warp * 1024 + (lane & 7) * 64 + (((lane >> 3) ^ (lane >> 1 & 3)) << 4);
+    const uint8_t* mine_pairs = smem + S::kXBytes + S::kCodeBytes + warp * kPairBytes + r * 8;
     IgPlace<S::kCodeRing> code;
-    auto take = [&] {  // the next stage's codes and pairs, into registers
-      if (!mbar_wait_warp(&code_full[code.slot], code.phase, p.status, kStatusWaitTimeoutProducer)) return false;
-      ldsm4(w[0], mine + code.slot * S::kCodes);
-      ldsm4(w[1], mine + code.slot * S::kCodes + 512);
-#pragma unroll
-      for (int g = 0; g < 128 / kGroup; ++g)
-        u[g] = *reinterpret_cast<const uint2*>(mine_pairs + code.slot * S::kPairs + g * 64);
-      return true;
-    };
-    ok = take();
+    const int mine_count = warp < p.warps ? count : 0;
     IgPlace<S::kRing> a;
 #pragma unroll 1
-    for (int it = 0; ok && it < count; ++it) {
-      uint32_t v[2][16];
-      __nv_bfloat162 s0, m0, s1, m1;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        if (half == 0 || kGroup == 64) {
-          const uint2 pair = u[kGroup == 64 ? half : 0];
-          const __nv_bfloat162 pa = reinterpret_cast<const __nv_bfloat162&>(pair.x),
-                               pb = reinterpret_cast<const __nv_bfloat162&>(pair.y), low = __float2bfloat162_rn(kIgLow);
-          s0 = __hmul2(__low2bfloat162(pa), __float2bfloat162_rn(kIgStep)), m0 = __hmul2(__high2bfloat162(pa), low);
-          s1 = __hmul2(__low2bfloat162(pb), __float2bfloat162_rn(kIgStep / 16.f)), m1 = __hmul2(__high2bfloat162(pb), low);
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) ig_values(w[half][q], s0, m0, s1, m1, v[half] + 4 * q);
-      }
-      // The next stage's codes, while this stage's values wait for their place.
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&code_empty[code.slot]);
-      code.next();
-      if (it + 1 < count && !take()) {
-        ok = false;
-        break;
-      }
+    for (int it = 0; ok && it < mine_count; ++it) {
+      ok = mbar_wait_warp(&code_full[code.slot], code.phase, p.status, kStatusWaitTimeoutProducer);
+      if (!ok) break;
       if (it >= S::kRing) {
         ok = mbar_wait_warp(&empty_bar[a.slot], a.phase ^ 1, p.status, kStatusWaitTimeoutProducer);
         if (!ok) break;
         tc_fence_after_sync();
       }
-      tmem_st_16x256(a_addr + a.slot * 64, v[0]);
-      tmem_st_16x256(a_addr + a.slot * 64 + 32, v[1]);
+      __nv_bfloat162 s0, m0, s1, m1;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (half == 0 || kGroup == 64) {
+          const uint2 pair = *reinterpret_cast<const uint2*>(mine_pairs + code.slot * S::kPairs + half * 64);
+          const __nv_bfloat162 pa = reinterpret_cast<const __nv_bfloat162&>(pair.x),
+                               pb = reinterpret_cast<const __nv_bfloat162&>(pair.y), low = __float2bfloat162_rn(kIgLow);
+          s0 = __hmul2(__low2bfloat162(pa), __float2bfloat162_rn(kIgStep)), m0 = __hmul2(__high2bfloat162(pa), low);
+          s1 = __hmul2(__low2bfloat162(pb), __float2bfloat162_rn(kIgStep / 16.f)), m1 = __hmul2(__high2bfloat162(pb), low);
+        }
+        uint32_t w[4], v[16];
+        ldsm4(w, mine + code.slot * S::kCodes + half * 512);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) ig_values(w[q], s0, m0, s1, m1, v + 4 * q);
+        tmem_st_16x256(a_addr + a.slot * 64 + half * 32, v);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&code_empty[code.slot]);
+      code.next();
       tmem_st_wait();
       tc_fence_before_sync();
       __syncwarp();
@@ -227,7 +214,7 @@ int4_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 #pragma unroll 1
       for (int it = 0; it < count; ++it) {
         if (it >= S::kCodeRing && !mbar_wait(&code_empty[code.slot], code.phase ^ 1, p.status, kStatusWaitTimeoutProducer)) break;
-        mbar_arrive_expect_tx(&code_full[code.slot], S::kCodes + kIgWarps * kPairBytes);
+        mbar_arrive_expect_tx(&code_full[code.slot], p.warps * (1024 + kPairBytes));
         tma_load_3d(smem + S::kXBytes + code.slot * S::kCodes, &map_codes, &code_full[code.slot], 0, (kb_lo + it) * 16, n0 / 16);
         tma_load_2d(smem + S::kXBytes + S::kCodeBytes + code.slot * S::kPairs, &map_pairs, &code_full[code.slot],
                     (kb_lo + it) * kPairBytes, n0 / 16);
@@ -257,9 +244,10 @@ int4_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   }
   __syncwarp();
 
-  // All products have retired.  A thread owns one feature; warps 4 to 7 take the second half of the rows.
-  const int feature = (warp & 3) * 32 + lane, n = n0 + feature;
-  float* part = reinterpret_cast<float*>(smem);  // [row][feature]: the ring is free
+  // All products have retired.  A thread owns one lane of tensor memory; warps 4 to 7 take the second half of the rows.
+  const int feature = (warp & 3) * 32 + lane, n = n0 + 16 * ((warp & 3) + (lane >> 4) * 4) + (lane & 15);
+  const bool there = n < min(p.N, n0 + 16 * p.warps);
+  float* part = reinterpret_cast<float*>(smem);  // [row][lane]: the ring is free
   if (p.splits > 1) __syncthreads();
   if (warp < kIgWarps && ok) {
     tc_fence_after_sync();
@@ -280,7 +268,7 @@ int4_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
         float v = __uint_as_float(r[j]) * (1.f / kIgLow);
         if (p.splits > 1) {
           part[row * kIgFeatures + feature] = v;
-        } else if (n < p.N) {
+        } else if (there) {
           __nv_bfloat16* dst = p.y + (row0 + row) * p.ldy + n;
           if (p.accumulate) v += __bfloat162float(*dst);
           *dst = __float2bfloat16(v);
@@ -290,7 +278,7 @@ int4_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   }
   if (p.splits > 1) {
     cluster_sync_all();
-    if (warp < kIgWarps && ok && n < p.N) {
+    if (warp < kIgWarps && ok && there) {
       for (int row = split + (warp >> 2) * p.splits; row < rows; row += 2 * p.splits) {
         float v[kIgMaxSplits];
 #pragma unroll
@@ -330,9 +318,9 @@ static int launch_int4_gemm(const void* x, int64_t ldx, const void* codes, const
   const uint64_t x_dims[2] = {static_cast<uint64_t>(p.K), static_cast<uint64_t>(p.M)}, x_stride[1] = {static_cast<uint64_t>(ldx) * 2};
   const uint32_t x_box[2] = {64, BN};
   const uint64_t code_dims[3] = {64, k128 * 16, n16}, code_strides[2] = {64, k128 * 1024};
-  const uint32_t code_box[3] = {64, 16, kIgWarps};
+  const uint32_t warps = static_cast<uint32_t>(p.warps), code_box[3] = {64, 16, warps};
   const uint64_t pair_dims[2] = {k128 * pair_bytes, n16}, pair_stride[1] = {k128 * pair_bytes};
-  const uint32_t pair_box[2] = {static_cast<uint32_t>(pair_bytes), kIgWarps};
+  const uint32_t pair_box[2] = {static_cast<uint32_t>(pair_bytes), warps};
   if (make_tensor_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, x_dims, x_stride, x_box, CU_TENSOR_MAP_SWIZZLE_128B) != 0 ||
       make_tensor_map(&map_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, codes, code_dims, code_strides, code_box,
                       CU_TENSOR_MAP_SWIZZLE_64B) != 0 ||
@@ -343,7 +331,7 @@ static int launch_int4_gemm(const void* x, int64_t ldx, const void* codes, const
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {static_cast<unsigned>(p.splits), 1, 1};
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((p.N + kIgFeatures - 1) / kIgFeatures * p.row_blocks * p.splits));
+  cfg.gridDim = dim3(static_cast<unsigned>((p.N + 16 * p.warps - 1) / (16 * p.warps) * p.row_blocks * p.splits));
   cfg.blockDim = dim3(kIgThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = stream;
@@ -365,13 +353,13 @@ static int int4_gemm(const void* x, int64_t ldx, const void* codes, const void* 
 // x [M, K] bf16 with rows of ldx (K, ldx multiples of 8, 16-byte aligned), y [M, N] with rows of ldy; M <= 512.  `splits`:
 // slices of K, up to 8 and one for every 128 rows of W at most.
 extern "C" int axb_int4_gemm(const void* x, const void* codes, const void* pairs, void* y, int M, int N, int K, int group,
-                             int64_t ldx, int64_t ldy, int accumulate, int splits, int* status, cudaStream_t stream) {
+                             int64_t ldx, int64_t ldy, int accumulate, int warps, int splits, int* status, cudaStream_t stream) {
   using namespace axb;
   const uintptr_t align = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(pairs);
-  if (M < 0 || M > 512 || N < 1 || K < 1 || K % 8 || ldx % 8 || (align & 15) || (group != 64 && group != 128) || splits < 1 ||
+  if (M < 0 || M > 512 || N < 1 || K < 1 || K % 8 || ldx % 8 || (align & 15) || (group != 64 && group != 128) || warps < 1 || warps > kIgWarps || splits < 1 ||
       splits > kIgMaxSplits || splits > (K + 127) / 128)
     return -10;
   if (M == 0) return 0;
-  const Int4GemmParams p{static_cast<__nv_bfloat16*>(y), ldy, M, N, K, accumulate, splits, (M + 127) / 128, status};
+  const Int4GemmParams p{static_cast<__nv_bfloat16*>(y), ldy, M, N, K, accumulate, splits, (M + 127) / 128, warps, status};
   return group == 64 ? int4_gemm<64>(x, ldx, codes, pairs, p, stream) : int4_gemm<128>(x, ldx, codes, pairs, p, stream);
 }

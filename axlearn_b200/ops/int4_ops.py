@@ -50,7 +50,7 @@ def _lib():
         h.axb_int4_attn_scratch_floats.argtypes = [c_int] * 4
         h.axb_int4_attn_scratch_floats.restype = c_int64
         h.axb_int4_linear.argtypes = [c_void_p] * 4 + [c_int] * 4 + [c_int64, c_int64, c_int, c_int, c_void_p]
-        h.axb_int4_gemm.argtypes = [c_void_p] * 4 + [c_int] * 4 + [c_int64, c_int64, c_int, c_int, c_void_p, c_void_p]
+        h.axb_int4_gemm.argtypes = [c_void_p] * 4 + [c_int] * 4 + [c_int64] * 2 + [c_int] * 3 + [c_void_p] * 2
         h.axb_int4_expand.argtypes = [c_void_p] * 3 + [c_int] * 3 + [c_void_p]
         for f in (h.axb_int4_append, h.axb_int4_append_prompt, h.axb_int4_decode_attn, h.axb_int4_linear, h.axb_int4_gemm,
                   h.axb_int4_expand):
@@ -183,12 +183,22 @@ def linear_splits(k: int, n: int, sms: int = 148) -> int:
     return max(1, min(8 if ctas <= 32 and k >= 8192 else 4, k // 512, 4 * sms // ctas))
 
 
-def fused_splits(rows: int, k: int, n: int) -> int:
-    """Slices of K of a product with weights expanded inside, the CTAs of a cluster; clusters leave some of the SMs idle, so 128
-    are counted on: one CTA of 128 columns and up to 128 rows on each with 512 rows of the weight or more; of up to 64 rows two
-    with 1024 or more.  (us with 4 / 8 slices, 64 rows: [14336, 4096] 18.0 / 16.5, [4096, 4096] 10.3 / 10.9.)"""
+def fused_plan(rows: int, k: int, n: int) -> tuple[int, int]:
+    """``(warps, splits)`` of a product with weights expanded inside: 16 columns a warp make a tile, slices of K are the CTAs of a
+    cluster.  Of up to 64 rows two CTAs fit an SM.  Tiles of 128 columns in one slice, or in as many as there is a CTA for
+    each SM (clusters leave some idle, so 128 are counted on) with 340 rows of the weight or more; with two CTAs an SM 800 or
+    more, if they fill most of it.  Tiles of 80 columns where those of 128 would be two CTAs on few SMs and one on the others.
+    (us of 64 rows: [14336, 4096] in 4 / 8 slices 18.4 / 17.1, [4096, 4096] 10.2 / 11.1, [4096, 11008] in 2 / 3 19.2 / 15.5,
+    [2048, 2048] in 4 / 6 7.8 / 7.0; [4096, 22016] with 8 / 5 warps 25.1 / 22.9.)"""
     tiles = -(-n // 128) * -(-rows // 128)
-    return max(1, min(8, max(min(128 // tiles, k // 512), min(256 // tiles, k // 1024) if rows <= 64 else 0)))
+    splits = max(1, min(8, 128 // tiles, k // 340))
+    if rows <= 64:
+        if tiles > 148 and n <= 280 * 80:
+            return 5, 1
+        two = min(8, 264 // tiles, k // 800)
+        if two * tiles >= 224:
+            splits = max(splits, two)
+    return 8, splits
 
 
 def int4_linear(x: Tensor, w: Int4Weight, *, out: Optional[Tensor] = None, accumulate: bool = False) -> Tensor:
@@ -225,7 +235,7 @@ def int4_linear(x: Tensor, w: Int4Weight, *, out: Optional[Tensor] = None, accum
         return out
     if rows <= MAX_FUSED_ROWS:
         _call(device, "axb_int4_gemm", x.data_ptr(), codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, n, k, w.group,
-              ldx, n, 1 if accumulate else 0, fused_splits(rows, k, n), cuda_ops.status_word(device).data_ptr())
+              ldx, n, 1 if accumulate else 0, *fused_plan(rows, k, n), cuda_ops.status_word(device).data_ptr())
         return out
     expanded = dequantize_weight(w)
     with torch.cuda.device(device):

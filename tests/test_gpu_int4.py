@@ -299,16 +299,17 @@ def test_linear_of_few_and_many_rows(rows, k, n, group):
 
 
 @pytest.mark.parametrize("rows", [17, 33, 128])
-@pytest.mark.parametrize("k,n,splits", [(640, 1160, 5), (1096, 264, 8), (200, 904, 2), (2048, 392, 3)])
-def test_linear_with_slices_of_k(rows, k, n, splits, monkeypatch):
-    """Slices of one to a dozen stages, a last tile of few columns and a last stage of few rows."""
+@pytest.mark.parametrize("k,n,plan", [(640, 1160, (8, 5)), (1096, 264, (5, 8)), (200, 904, (7, 2)), (2048, 392, (1, 3)),
+                                      (72, 2056, (6, 1)), (640, 24, (3, 4)), (1096, 648, (4, 1))])
+def test_linear_with_slices_of_k_and_narrow_tiles(rows, k, n, plan, monkeypatch):
+    """Slices of one to a dozen stages, tiles of one to eight warps, a last tile of few columns and a last stage of few rows."""
     from axlearn_b200.ops import cuda_ops, int4_ops
 
     gen = _gen(rows + k)
     w = int4_ops.quantize_weight(_normal(gen, k, n) * k ** -0.5, group=64)
     x = _normal(gen, rows, k).bfloat16()
     y, bound = _linear64(x, w)
-    monkeypatch.setattr(int4_ops, "fused_splits", lambda *_: splits)
+    monkeypatch.setattr(int4_ops, "fused_plan", lambda *_: plan)
     got = int4_ops.int4_linear(x, w)
     cuda_ops.check_status()
     assert ((got.double() - y).abs() <= bound).all()

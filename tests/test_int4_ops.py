@@ -295,6 +295,14 @@ def test_weights_and_products_refuse():
         int4_ops.int4_pages(2, 16, 2, 96)
 
 
+@pytest.mark.parametrize("rows", [9, 64, 65, 512])
+@pytest.mark.parametrize("k,n", [(8, 8), (128, 136), (4096, 4096), (4096, 22016), (4096, 28672), (16384, 2048), (2048, 6144), (8, 10 ** 6)])
+def test_plans_of_products(rows, k, n):
+    warps, splits = int4_ops.fused_plan(rows, k, n)
+    assert 1 <= warps <= 8 and 1 <= splits <= min(8, -(-k // 128))
+    assert splits == 1 or -(-n // (16 * warps)) * -(-rows // 128) * splits <= 2 * 148
+
+
 @pytest.mark.parametrize("batch,kv,group,tokens", [(1, 16, 1, 300), (16, 8, 4, 2048), (64, 32, 1, 2000), (1, 8, 4, 130048),
                                                    (1, 1, 1, 1), (0, 4, 1, 64), (300, 32, 16, 4096)])
 def test_splits_of_attention(batch, kv, group, tokens):
