@@ -313,20 +313,23 @@ __device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, bool ok
 // group of a key, and the sums of a group are multiplied by its s: k.q = sum_g s_g (sum c q) + m_g sum q.
 // sum_g m_g sum q is one product of its own: the sums of q are three bf16 terms that add up to their 32 bits.
 // O^T = V^T P^T: 16 dims of one group are the rows, the heads the columns.  P is rounded to bf16 as the operand of all
-// products, as in the prompts' kernels, turned round by `movmatrix`, and multiplied by s of a key's group, which rounds again;
-// sum p m is one product of its own with the pairs' transpose.  Two roundings of half a step, 2^-8 of a probability each;
-// against 64 bits an output is off by 0.0019 of itself (2-norm), 0.0017 of it the output's own rounding.
+// products, as in the prompts' kernels, and normalised by the sum of what it was rounded to; turned round by `movmatrix` and
+// multiplied by s of a key's group, it rounds again.  Values are small sums of large terms p m and p s c, so that this second
+// rounding would count double against codes of 0 to 15: it counts against c - 8, since sums of the rounded and of the exact p s
+// (products with the pairs' transpose and with ones) give back 8 times their difference.  Two roundings of half a step, 2^-8 of
+// a probability each; against 64 bits an output is off by up to 0.0020 of itself (2-norm; 4 to 64 keys, 0.0018 of 2000), 0.0017 of
+// it the output's own rounding; without the shift by 8 up to 0.0029.
 // Codes enter as denormal bf16 numbers (`int4.cuh`): scores carry 1 / kInt4Back until the exponential, probabilities and the
 // sums of them alone kInt4Scale, and the sums of p c 1 / kInt4Back.
 // The maximum that probabilities are relative to moves only when a score passes it by kSlack (a factor of 2^kSlack).
 //
 // A tile is 32 keys, a warp's own from `cp.async` to its sums: no barrier before the end.  Tiles go round the warps of all
 // splits, splits of eight or less are a cluster whose parts meet in distributed shared memory, more are clusters whose
-// parts a second launch joins.  Instructions bind the pass (about 600 a tile and warp; ALU pipe 56%, a third of that unpacking,
-// issue 59%, tensor cores 28%), not the copies: without arithmetic 97 us, without copies 106, together 125 (us; at the copy
-// rate 100.3) for 64 sequences of 2000 tokens and 32 KV heads of 128.  16 x 2048, 8 KV heads for 32: 14.3 (3.3), of which a CTA's
-// start and end are about 4 and the launch 2; 1 x 130001, 8 KV heads for 32: 45.5 (25.4).  With 96 registers and five CTAs an SM
-// 149, with shifts on the FMA pipe 132.
+// parts a second launch joins.  Measured (us; at the copy rate): 64 sequences of 2000 tokens, 32 KV heads of 128, 133 (100.3);
+// 16 x 2048, 8 KV heads for 32, 14.8 (3.3), of which a CTA's start and end are about 4 and the launch 2; 1 x 130001, 8 KV heads
+// for 32, 48.5 (25.4).  Instructions bind the pass (600 a tile and warp, two thirds of the ALU pipe's unpack codes), not the
+// copies; the first case before the shift of the codes by 8, whose products are 8 of it: 125, without arithmetic 97, without
+// copies 106 (issue 59%, ALU 56%, tensor cores 28%), with 96 registers and five CTAs an SM 149, with shifts on the FMA pipe 132.
 //
 // kAppend: a decoding step in one launch.  A warp turns its query heads in registers; the warp whose tile holds the new token
 // turns its key, quantises key and value, stores them in their page slot and puts them into the tile itself, so nobody reads
@@ -489,10 +492,12 @@ int4_attn_kernel(Int4AttnParams p) {
     }
   }
 
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // heads 2c, 2c + 1; l: this lane's keys
+  float m[2] = {-INFINITY, -INFINITY};  // heads 2c, 2c + 1
   const float slack = kSlack / p.scale_log2;
   float acc[2 * G][4];  // [group, half][dim 32 g + 4 r + 2 half (+ 1: entries 2, 3)][columns 2c, 2c + 1]
-  float acc_m[4] = {};  // row 2 g + 1: sums of p m of group g
+  // Rows 2 g, 2 g + 1: sums of p s and p m of group g; 8 + g: sums of the rounded p s; 12: of p.
+  float acc_m[4] = {};
+  const uint32_t one_l = r == 4 ? 0x3f803f80u : 0u;
 #pragma unroll
   for (int i = 0; i < 2 * G; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
   const float zero[4] = {0.f, 0.f, 0.f, 0.f};
@@ -568,9 +573,8 @@ int4_attn_kernel(Int4AttnParams p) {
         const float m_new = fmaxf(m[h], top[h]);
         corr[h] = m[h] == -INFINITY ? 0.f : ex2((m[h] - m_new) * p.scale_log2);  // (nothing is there yet)
         m[h] = m_new;
-        l[h] *= corr[h];
       }
-      acc_m[0] *= corr[0], acc_m[1] *= corr[1];
+      acc_m[0] *= corr[0], acc_m[1] *= corr[1], acc_m[2] *= corr[0], acc_m[3] *= corr[1];
 #pragma unroll
       for (int i = 0; i < 2 * G; ++i) {
         acc[i][0] *= corr[0];
@@ -584,17 +588,14 @@ int4_attn_kernel(Int4AttnParams p) {
       // (a row of -inf alone keeps zeros; NaN stays)
       const float base = m[h] == -INFINITY ? 0.f : fmaf(-m[h], p.scale_log2, kInt4Shift);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[i][h] = ex2(fmaf(s[i][h], p.scale_log2, base));
-        l[h] += s[i][h];
-      }
+      for (int i = 0; i < 4; ++i) s[i][h] = ex2(fmaf(s[i][h], p.scale_log2, base));
     }
     uint32_t pt[4], vt[4];  // rows: heads / entries of pairs; columns: keys 8 i + 2c, + 1
     ldsm4t(vt, st + Tile::kVPairs + lane * Tile::kPairs);
 #pragma unroll
     for (int i = 0; i < 4; ++i) pt[i] = turned_round(pack2(s[i][0], s[i][1]));
     {
-      const uint32_t a0[4] = {vt[0], 0u, vt[1], 0u}, a1[4] = {vt[2], 0u, vt[3], 0u};
+      const uint32_t a0[4] = {vt[0], one_l, vt[1], one_l}, a1[4] = {vt[2], one_l, vt[3], one_l};
       mma(acc_m, a0, pt[0], pt[1]);
       mma(acc_m, a1, pt[2], pt[3]);
     }
@@ -614,6 +615,11 @@ int4_attn_kernel(Int4AttnParams p) {
       for (int i = 0; i < 4; ++i) {
         const uint32_t ps = __shfl_sync(0xffffffffu, vt[i], 8 * g + c);  // row 2 g
         pb[i] = times(pt[i], reinterpret_cast<const __nv_bfloat162&>(ps));
+      }
+      {
+        const uint32_t one_g = r == g ? 0x3f803f80u : 0u, ones[4] = {0u, one_g, 0u, one_g};
+        mma(acc_m, ones, pb[0], pb[1]);
+        mma(acc_m, ones, pb[2], pb[3]);
       }
       uint32_t x[4], y[4];  // dims 4r, 4r + 1 and the two behind them of keys 8 i + 2c, + 1
 #pragma unroll
@@ -638,11 +644,6 @@ int4_attn_kernel(Int4AttnParams p) {
   }
   cp_wait_all();
   __syncthreads();  // the merge buffers overlay the tiles
-#pragma unroll
-  for (int off = 4; off <= 16; off <<= 1) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) l[h] += __shfl_xor_sync(0xffffffffu, l[h], off);
-  }
   float* s_part = reinterpret_cast<float*>(s_ring);  // 4 warps and the CTA: [rows][H] sums, then maxima, then weights
   const int per_warp = rows * H;
   float* s_m = s_part + (kAttnWarps + 1) * per_warp;
@@ -652,16 +653,19 @@ int4_attn_kernel(Int4AttnParams p) {
     float* dst = s_part + warp * per_warp + (2 * c + n) * H + r * 4;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      const float low = __shfl_sync(0xffffffffu, acc_m[n], 8 * g + 4 + c) * (1.f / kInt4Scale);
+      const float exact = __shfl_sync(0xffffffffu, acc_m[n], 8 * g + c), rounded = __shfl_sync(0xffffffffu, acc_m[2 + n], 4 * g + c);
+      const float low =
+          fmaf(-8.f, rounded - exact, __shfl_sync(0xffffffffu, acc_m[n], 8 * g + 4 + c)) * (1.f / kInt4Scale);
       if (2 * c + n >= rows) continue;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         *reinterpret_cast<float2*>(dst + g * 32 + 2 * h) = make_float2(fmaf(acc[2 * g + h][n], kInt4Back, low),
                                                                       fmaf(acc[2 * g + h][2 + n], kInt4Back / 16.f, low));
     }
+    const float l = __shfl_sync(0xffffffffu, acc_m[2 + n], 16 + c);
     if (r == 0 && 2 * c + n < rows) {
       s_m[warp * rows + 2 * c + n] = m[n] * p.scale_log2;
-      s_l[warp * rows + 2 * c + n] = l[n] * (1.f / kInt4Scale);
+      s_l[warp * rows + 2 * c + n] = l * (1.f / kInt4Scale);
     }
   }
   __syncthreads();

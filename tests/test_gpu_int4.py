@@ -132,6 +132,21 @@ def test_attention_over_small_and_large_values(dim, q_scale, v_scale):
     assert torch.equal(int4_ops.paged_decode_attention_int4(q * q_scale, k_pages, v_pages, table, lengths), plain * v_scale)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("tokens", [2, 4, 8, 12, 24, 48, 200])
+def test_short_sequences_keep_their_precision(tokens, dim):
+    """Two roundings of a probability beside the output's own.  The same roundings simulated in 64 bits add up to 1.22 of the
+    output's rounding in the 2-norm; without the shift of the codes by 8 they are 1.4 to 1.8 of it."""
+    from axlearn_b200.ops import int4_ops
+
+    k_pages, v_pages, table = _cache(64, -(-tokens // 16), 16, 4, dim, seed=tokens)
+    lengths = torch.full((64,), tokens, dtype=torch.int32, device="cuda")
+    q = _normal(_gen(4), 64, 8, dim).bfloat16()
+    out = int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, lengths)
+    want, _ = _attention64(q, k_pages, v_pages, table, lengths, dim ** -0.5)
+    assert (out.double() - want).norm() <= 1.35 * (want.float().bfloat16().double() - want).norm()
+
+
 @pytest.mark.parametrize("splits", [1, 8, 16])
 def test_scores_far_apart(splits):
     """One key that takes all, early or late, and scores that climb by more than the slack from tile to tile."""
