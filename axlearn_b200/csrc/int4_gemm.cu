@@ -1,5 +1,5 @@
-// y[M, N] = x[M, K] W (+ y) for up to 512 rows with weights held in 4 bits (layout: int4_linear.cu), on the fifth-generation
-// tensor cores: 128 features are the M side of the MMA, up to 128 rows of x its N side.
+// y[M, N] = x[M, K] W (+ y) with weights held in 4 bits (layout: int4_linear.cu), on the fifth-generation tensor cores: 128
+// features are the M side of the MMA, up to 128 rows of x its N side; more rows are blocks of 128.
 //
 // Up to eight warps feed: each owns 16 features and turns their codes of 128 rows of W into bf16 values m + s c (one rounding, 2^-9
 // of a weight, as in the expansion for the GEMM of more rows), which `tcgen05.st` puts into tensor memory, so that weights
@@ -350,14 +350,14 @@ static int int4_gemm(const void* x, int64_t ldx, const void* codes, const void* 
 
 }  // namespace axb
 
-// x [M, K] bf16 with rows of ldx (K, ldx multiples of 8, 16-byte aligned), y [M, N] with rows of ldy; M <= 512.  `splits`:
+// x [M, K] bf16 with rows of ldx (K, ldx multiples of 8, 16-byte aligned), y [M, N] with rows of ldy; M <= 65536.  `splits`:
 // slices of K, up to 8 and one for every 128 rows of W at most.
 extern "C" int axb_int4_gemm(const void* x, const void* codes, const void* pairs, void* y, int M, int N, int K, int group,
                              int64_t ldx, int64_t ldy, int accumulate, int warps, int splits, int* status, cudaStream_t stream) {
   using namespace axb;
   const uintptr_t align = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(pairs);
-  if (M < 0 || M > 512 || N < 1 || K < 1 || K % 8 || ldx % 8 || (align & 15) || (group != 64 && group != 128) || warps < 1 || warps > kIgWarps || splits < 1 ||
-      splits > kIgMaxSplits || splits > (K + 127) / 128)
+  if (M < 0 || M > 65536 || N < 1 || K < 1 || K % 8 || ldx % 8 || (align & 15) || (group != 64 && group != 128) || warps < 1 ||
+      warps > kIgWarps || splits < 1 || splits > kIgMaxSplits || splits > (K + 127) / 128)
     return -10;
   if (M == 0) return 0;
   const Int4GemmParams p{static_cast<__nv_bfloat16*>(y), ldy, M, N, K, accumulate, splits, (M + 127) / 128, warps, status};

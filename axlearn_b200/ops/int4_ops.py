@@ -21,6 +21,7 @@ word, which ``cuda_ops.check_status`` raises.  The bf16 forms of these operation
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import dataclasses
 import math
@@ -34,9 +35,6 @@ c_void_p, c_int, c_int64, c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_int6
 Tensor = torch.Tensor
 
 CACHE_GROUP = 32
-# Rows of x up to which weights are expanded inside the product, for each 128 rows again; beyond, W is expanded to bf16 once and
-# multiplied by the GEMM (us so / with the GEMM: 256 x [4096, 28672] 77 / 121, 512 x [4096, 22016] 97 / 113, 768 rows of it 155 / 138).
-MAX_FUSED_ROWS = 512
 _configured = False
 
 
@@ -61,6 +59,11 @@ def _lib():
 
 def _on_kernel(x: Tensor) -> bool:
     return x.is_cuda and x.dtype == torch.bfloat16 and not dispatch._flags.force_reference  # pylint: disable=protected-access
+
+
+def _on(device: torch.device):
+    """The device of the operands made the current one, where it is another."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _call(device: torch.device, name: str, *args) -> None:
@@ -162,7 +165,7 @@ def dequantize_weight(w: Int4Weight, dtype: torch.dtype = torch.bfloat16) -> Ten
     if w.codes.is_cuda and dtype == torch.bfloat16 and not dispatch._flags.force_reference:  # pylint: disable=protected-access
         out = torch.empty((w.codes.shape[0] * 16, w.codes.shape[1] * 64), dtype=dtype, device=w.codes.device)
         _call(out.device, "axb_int4_expand", w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), w.n, w.k, w.group)
-        return out[:w.n, :w.k].t()
+        return (out if out.shape == (w.n, w.k) else out[:w.n, :w.k]).t()
     tiles, groups = w.scales.shape[:2]
     scales = w.scales.permute(0, 3, 2, 1, 4).reshape(tiles * 16, groups, 2)
     return group_values(_unpack_blocks(w.codes), scales).t()[:w.k, :w.n].to(dtype)
@@ -173,6 +176,14 @@ def multiplies_codes(rows: int, n: int) -> bool:
     wave of CTAs (us of 16 rows, so / with weights expanded inside the product, 4096 rows of the weight: 4096 columns 7.8 /
     8.7, 6144 columns 14.2 / 10.6, 28672 columns 27.0 / 22.8)."""
     return rows <= 8 or (rows <= 16 and n <= 4096)
+
+
+def expands_inside(rows: int, n: int) -> bool:
+    """Whether a product of more rows expands weights inside, for each 128 rows again; otherwise W is expanded to bf16 once and
+    multiplied by the GEMM: up to 512 rows, and more while tiles of 128 x 128 are one wave.  (us inside / with the GEMM: 256 x
+    [4096, 28672] 77 / 121, 512 x [4096, 22016] 97 / 113, 768 rows of it 155 / 138, 2048 x [14336, 1024] 55 / 66, 1024 x
+    [4096, 4096] 40 / 35; 2048 x [1024, 1024] 11.0 / 10.0, and 12 / 27 as a call.)"""
+    return rows <= 512 or -(-rows // 128) * -(-n // 128) <= 148
 
 
 def linear_splits(k: int, n: int, sms: int = 148) -> int:
@@ -233,12 +244,12 @@ def int4_linear(x: Tensor, w: Int4Weight, *, out: Optional[Tensor] = None, accum
         _call(device, "axb_int4_linear", x.data_ptr(), codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, n, k, w.group,
               ldx, n, 1 if accumulate else 0, linear_splits(k, n))
         return out
-    if rows <= MAX_FUSED_ROWS:
+    if expands_inside(rows, n):
         _call(device, "axb_int4_gemm", x.data_ptr(), codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), rows, n, k, w.group,
               ldx, n, 1 if accumulate else 0, *fused_plan(rows, k, n), cuda_ops.status_word(device).data_ptr())
         return out
     expanded = dequantize_weight(w)
-    with torch.cuda.device(device):
+    with _on(device):
         if out.data_ptr() % 16:  # a view into a larger buffer: the GEMM stores vectors
             y = out.clone() if accumulate else torch.empty_like(out)
             cuda_ops.gemm(x, expanded, out=y.view(rows, n), accumulate=accumulate)
@@ -528,5 +539,5 @@ def prompt_attention_int4(qkv: Tensor, k_pages: Int4Pages, v_pages: Int4Pages, p
     _call(device, "axb_int4_append_prompt", qkv.data_ptr(), k_pages.codes.data_ptr(), k_pages.scales.data_ptr(),
           v_pages.codes.data_ptr(), v_pages.scales.data_ptr(), page_table.data_ptr(), table.data_ptr(), table.shape[0], b, t,
           num_q_heads, nkv, h, page_size, page_table.shape[1], num_pages, cuda_ops.status_word(device).data_ptr())
-    with torch.cuda.device(device):
+    with _on(device):
         return decode_ops.packed_prompt_attention(qkv, num_q_heads=num_q_heads, num_kv_heads=nkv, softmax_scale=softmax_scale)

@@ -348,7 +348,7 @@ def test_linear_where_products_with_codes_end(rows, k, n):
 
 
 @pytest.mark.parametrize("rows", [129, 250, 384, 512, 513])
-@pytest.mark.parametrize("k,n,group", [(1096, 136, 64), (2048, 392, 128), (8, 1160, 64)])
+@pytest.mark.parametrize("k,n,group", [(1096, 136, 64), (2048, 392, 128), (8, 1160, 64), (264, 4616, 128)])
 def test_linear_in_blocks_of_rows(rows, k, n, group):
     """A last block of one row and of most rows, with and without slices of K; the first rows behind the blocks."""
     from axlearn_b200.ops import cuda_ops, int4_ops
