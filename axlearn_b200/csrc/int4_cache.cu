@@ -316,7 +316,8 @@ __device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, bool ok
 // products, as in the prompts' kernels, and normalised by the sum of what it was rounded to; turned round by `movmatrix` and
 // multiplied by s of a key's group, it rounds again.  Values are small sums of large terms p m and p s c, so that this second
 // rounding would count double against codes of 0 to 15: it counts against c - 8, since sums of the rounded and of the exact p s
-// (products with the pairs' transpose and with ones) give back 8 times their difference.  Two roundings of half a step, 2^-8 of
+// give back 8 times their difference.  The sums are products with P as the first operand, in registers as it lies, and pairs or
+// ones as the second: with the roles of the large products they cost 26 register moves a tile (133 us for 127 below).  Two roundings of half a step, 2^-8 of
 // a probability each; against 64 bits an output is off by up to 0.0020 of itself (2-norm; 4 to 64 keys, 0.0018 of 2000), 0.0017 of
 // it the output's own rounding; without the shift by 8 up to 0.0029.
 // Codes enter as denormal bf16 numbers (`int4.cuh`): scores carry 1 / kInt4Back until the exponential, probabilities and the
@@ -325,10 +326,10 @@ __device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, bool ok
 //
 // A tile is 32 keys, a warp's own from `cp.async` to its sums: no barrier before the end.  Tiles go round the warps of all
 // splits, splits of eight or less are a cluster whose parts meet in distributed shared memory, more are clusters whose
-// parts a second launch joins.  Measured (us; at the copy rate): 64 sequences of 2000 tokens, 32 KV heads of 128, 133 (100.3);
-// 16 x 2048, 8 KV heads for 32, 14.8 (3.3), of which a CTA's start and end are about 4 and the launch 2; 1 x 130001, 8 KV heads
-// for 32, 48.5 (25.4).  Instructions bind the pass (600 a tile and warp, two thirds of the ALU pipe's unpack codes), not the
-// copies; the first case before the shift of the codes by 8, whose products are 8 of it: 125, without arithmetic 97, without
+// parts a second launch joins.  Measured (us; at the copy rate): 64 sequences of 2000 tokens, 32 KV heads of 128, 127 (100.3);
+// 16 x 2048, 8 KV heads for 32, 14.5 (3.3), of which a CTA's start and end are about 4 and the launch 2; 1 x 130001, 8 KV heads
+// for 32, 47.4 (25.4).  Instructions bind the pass (600 a tile and warp, two thirds of the ALU pipe's unpack codes), not the
+// copies; the first case without the shift of the codes by 8: 125, without arithmetic 97, without
 // copies 106 (issue 59%, ALU 56%, tensor cores 28%), with 96 registers and five CTAs an SM 149, with shifts on the FMA pipe 132.
 //
 // kAppend: a decoding step in one launch.  A warp turns its query heads in registers; the warp whose tile holds the new token
@@ -495,9 +496,10 @@ int4_attn_kernel(Int4AttnParams p) {
   float m[2] = {-INFINITY, -INFINITY};  // heads 2c, 2c + 1
   const float slack = kSlack / p.scale_log2;
   float acc[2 * G][4];  // [group, half][dim 32 g + 4 r + 2 half (+ 1: entries 2, 3)][columns 2c, 2c + 1]
-  // Rows 2 g, 2 g + 1: sums of p s and p m of group g; 8 + g: sums of the rounded p s; 12: of p.
-  float acc_m[4] = {};
-  const uint32_t one_l = r == 4 ? 0x3f803f80u : 0u;
+  // P as the first operand: its four registers are keys 0 .. 7 and 16 .. 23 in rows 0 to 7, the other keys in rows 8 to 15.
+  float acc_lo[4] = {}, acc_hi[4] = {};  // head r: sums of p s, p m of group c; over the first keys in entries 0, 1 of acc_lo, over
+                                         // the others in entries 2, 3 of acc_hi (what is in the rest is not used)
+  float acc_r[4] = {};                   // both rows together: sums of the rounded p s of groups 2c, 2c + 1; of p where c is 2
 #pragma unroll
   for (int i = 0; i < 2 * G; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
   const float zero[4] = {0.f, 0.f, 0.f, 0.f};
@@ -574,7 +576,11 @@ int4_attn_kernel(Int4AttnParams p) {
         corr[h] = m[h] == -INFINITY ? 0.f : ex2((m[h] - m_new) * p.scale_log2);  // (nothing is there yet)
         m[h] = m_new;
       }
-      acc_m[0] *= corr[0], acc_m[1] *= corr[1], acc_m[2] *= corr[0], acc_m[3] *= corr[1];
+      const float even = __shfl_sync(0xffffffffu, corr[0], r >> 1), odd = __shfl_sync(0xffffffffu, corr[1], r >> 1);
+      const float of_row = r & 1 ? odd : even;
+      acc_lo[0] *= of_row, acc_lo[1] *= of_row, acc_hi[2] *= of_row, acc_hi[3] *= of_row;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc_r[i] *= of_row;
 #pragma unroll
       for (int i = 0; i < 2 * G; ++i) {
         acc[i][0] *= corr[0];
@@ -590,14 +596,15 @@ int4_attn_kernel(Int4AttnParams p) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[i][h] = ex2(fmaf(s[i][h], p.scale_log2, base));
     }
-    uint32_t pt[4], vt[4];  // rows: heads / entries of pairs; columns: keys 8 i + 2c, + 1
-    ldsm4t(vt, st + Tile::kVPairs + lane * Tile::kPairs);
+    uint32_t pt[4], vt[4];  // rows: heads / entries of pairs; columns: keys 8 i + 2c, + 1 (vt: in the order 0, 2, 1, 3)
+    ldsm4t(vt, st + Tile::kVPairs + (((lane & 8) << 1) + (lane >> 4 << 3) + (lane & 7)) * Tile::kPairs);
 #pragma unroll
     for (int i = 0; i < 4; ++i) pt[i] = turned_round(pack2(s[i][0], s[i][1]));
+    mma(acc_lo, pt, vt[0], vt[1]);
+    mma(acc_hi, pt, vt[2], vt[3]);
     {
-      const uint32_t a0[4] = {vt[0], one_l, vt[1], one_l}, a1[4] = {vt[2], one_l, vt[3], one_l};
-      mma(acc_m, a0, pt[0], pt[1]);
-      mma(acc_m, a1, pt[2], pt[3]);
+      const uint32_t one = r == 4 ? 0x3f803f80u : 0u;
+      mma(acc_r, pt, one, one);
     }
     uint32_t w[8][G / 2];  // keys 8 i + 2c, + 1
 #pragma unroll
@@ -613,14 +620,11 @@ int4_attn_kernel(Int4AttnParams p) {
       uint32_t pb[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t ps = __shfl_sync(0xffffffffu, vt[i], 8 * g + c);  // row 2 g
+        const uint32_t ps = __shfl_sync(0xffffffffu, vt[i >> 1 | (i & 1) << 1], 8 * g + c);  // row 2 g
         pb[i] = times(pt[i], reinterpret_cast<const __nv_bfloat162&>(ps));
       }
-      {
-        const uint32_t one_g = r == g ? 0x3f803f80u : 0u, ones[4] = {0u, one_g, 0u, one_g};
-        mma(acc_m, ones, pb[0], pb[1]);
-        mma(acc_m, ones, pb[2], pb[3]);
-      }
+      const uint32_t one = r == g ? 0x3f803f80u : 0u;
+      mma(acc_r, pb, one, one);
       uint32_t x[4], y[4];  // dims 4r, 4r + 1 and the two behind them of keys 8 i + 2c, + 1
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -644,6 +648,7 @@ int4_attn_kernel(Int4AttnParams p) {
   }
   cp_wait_all();
   __syncthreads();  // the merge buffers overlay the tiles
+  acc_lo[0] += acc_hi[2], acc_lo[1] += acc_hi[3], acc_r[0] += acc_r[2], acc_r[1] += acc_r[3];
   float* s_part = reinterpret_cast<float*>(s_ring);  // 4 warps and the CTA: [rows][H] sums, then maxima, then weights
   const int per_warp = rows * H;
   float* s_m = s_part + (kAttnWarps + 1) * per_warp;
@@ -653,16 +658,17 @@ int4_attn_kernel(Int4AttnParams p) {
     float* dst = s_part + warp * per_warp + (2 * c + n) * H + r * 4;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      const float exact = __shfl_sync(0xffffffffu, acc_m[n], 8 * g + c), rounded = __shfl_sync(0xffffffffu, acc_m[2 + n], 4 * g + c);
-      const float low =
-          fmaf(-8.f, rounded - exact, __shfl_sync(0xffffffffu, acc_m[n], 8 * g + 4 + c)) * (1.f / kInt4Scale);
+      const int at = (2 * c + n) * 4;
+      const float exact = __shfl_sync(0xffffffffu, acc_lo[0], at + g);
+      const float rounded = __shfl_sync(0xffffffffu, acc_r[g & 1], at + (g >> 1));
+      const float low = fmaf(-8.f, rounded - exact, __shfl_sync(0xffffffffu, acc_lo[1], at + g)) * (1.f / kInt4Scale);
       if (2 * c + n >= rows) continue;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         *reinterpret_cast<float2*>(dst + g * 32 + 2 * h) = make_float2(fmaf(acc[2 * g + h][n], kInt4Back, low),
                                                                       fmaf(acc[2 * g + h][2 + n], kInt4Back / 16.f, low));
     }
-    const float l = __shfl_sync(0xffffffffu, acc_m[2 + n], 16 + c);
+    const float l = __shfl_sync(0xffffffffu, acc_r[0], (2 * c + n) * 4 + 2);
     if (r == 0 && 2 * c + n < rows) {
       s_m[warp * rows + 2 * c + n] = m[n] * p.scale_log2;
       s_l[warp * rows + 2 * c + n] = l * (1.f / kInt4Scale);
