@@ -456,8 +456,9 @@ def _launch_attention(q, k_pages, v_pages, page_table, lengths, table, out, scra
         floats = attention_scratch_floats(b, nq, h, splits)
         if scratch is None:
             scratch = torch.empty(floats, dtype=torch.float32, device=device)
-        elif scratch.numel() < floats or scratch.dtype != torch.float32 or scratch.device != device or not scratch.is_contiguous():
-            raise ValueError(f"scratch is {floats} contiguous fp32 values on {device}")
+        elif (scratch.numel() < floats or scratch.dtype != torch.float32 or scratch.device != device
+              or not scratch.is_contiguous() or scratch.data_ptr() % 8):
+            raise ValueError(f"scratch is {floats} contiguous fp32 values on {device}, 8-byte aligned")
     _call(device, "axb_int4_decode_attn", q.data_ptr(), k_pages.codes.data_ptr(), k_pages.scales.data_ptr(), v_pages.codes.data_ptr(),
           v_pages.scales.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), None if table is None else table.data_ptr(),
           out.data_ptr(), None if scratch is None else scratch.data_ptr(), 0 if table is None else table.shape[0], b, nq, nkv, h,

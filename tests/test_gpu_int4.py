@@ -347,7 +347,7 @@ def test_linear_where_products_with_codes_end(rows, k, n):
     assert ((alone.double() - y).abs() <= bound).all()
 
 
-@pytest.mark.parametrize("rows", [129, 250, 384, 512, 513])
+@pytest.mark.parametrize("rows", [129, 250, 384, 512, 513, 1500])
 @pytest.mark.parametrize("k,n,group", [(1096, 136, 64), (2048, 392, 128), (8, 1160, 64), (264, 4616, 128)])
 def test_linear_in_blocks_of_rows(rows, k, n, group):
     """A last block of one row and of most rows, with and without slices of K; the first rows behind the blocks."""
@@ -509,6 +509,21 @@ def test_a_step_is_rotation_append_and_attention(nq, kv, dim, splits):
         assert ((a - c).abs() <= 1.1 * step + 2.0 ** -6 * c.abs()).all()
         assert (a != c).float().mean() < 1e-3
     assert torch.equal(v_pages.codes, other[1].codes) and torch.equal(v_pages.scales, other[1].scales)
+
+
+def test_scratch_that_does_not_fit_is_refused():
+    from axlearn_b200.ops import int4_ops
+
+    k_pages, v_pages, table = _cache(2, 20, 16, 2, 128, seed=7)
+    lengths = torch.tensor([320, 77], dtype=torch.int32, device="cuda")
+    q = _normal(_gen(8), 2, 8, 128).bfloat16()
+    floats = int4_ops.attention_scratch_floats(2, 8, 128, 16)
+    whole = torch.empty(floats + 1, device="cuda")
+    for scratch in (whole[:-2], whole[1:], whole[:-1].double(), torch.empty(floats)):
+        with pytest.raises(ValueError):
+            int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, lengths, splits=16, scratch=scratch)
+    out = int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, lengths, splits=16, scratch=whole)
+    assert torch.equal(out, int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, lengths, splits=16))
 
 
 def test_a_step_without_a_place_appends_nothing():
