@@ -51,6 +51,7 @@ struct Int4AppendParams {
   int* status;
   FastDiv heads, tokens, page;  // units of a token, tokens of a sequence, positions of a page
   uint32_t units;
+  int kv_units;                 // of a token
   int angle_rows, num_q_heads, num_kv_heads, max_pages, num_pages;
 };
 
@@ -139,12 +140,13 @@ static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 constexpr int kAppendThreads = 256;
 
-// A unit is the key and the value of a KV head of one token, or two of its query heads to be rotated: H / 8 lanes with 16 bytes
-// of either row.  Units run over heads (KV, then pairs of q), tokens, sequences.  The pass is bound by its instructions: where
-// a row goes is found once for both, and nothing is quantised behind `live`.  Measured with the values written out as well,
-// heads of 128 (us; at the copy rate): 64 x 1 tokens, 32 KV heads, 3.2 (0.4), a launch; 8 x 2048 tokens, 8 KV heads, 30.0 (17.5),
-// and 64 with a row a unit, a 64-bit division for each of its indexes and an IEEE division for each level.
-template <int H>
+// A unit is the key and the value of kHeads KV heads of one token, or twice as many of its query heads to be rotated: H / 8
+// lanes with 16 bytes of each row.  Units run over heads (KV, then q), tokens, sequences.  The pass is bound by its
+// instructions: where rows go is found once for all of a unit, and nothing is quantised behind `live`.  Measured with the values
+// written out as well, heads of 128 (us; at the copy rate): 64 x 1 tokens, 32 KV heads, 3.2 (0.4), a launch; 8 x 2048 tokens,
+// 8 KV heads, 26.2 (17.5); 30.0 with a head a unit, and 64 with a row a unit, a 64-bit division for each of its indexes and an
+// IEEE division for each level.
+template <int H, int kHeads>
 __global__ void __launch_bounds__(kAppendThreads)
 int4_append_kernel(Int4AppendParams p) {
   chain_link();
@@ -155,71 +157,89 @@ int4_append_kernel(Int4AppendParams p) {
     const uint32_t unit = unit0 + threadIdx.x / kLanes;  // (shuffles: all lanes stay)
     const bool inside = unit < p.units;
     const uint32_t token = inside ? p.heads.div(unit) : 0;
-    int head = inside ? static_cast<int>(unit - token * p.heads.d) : 0;
+    const int group = inside ? static_cast<int>(unit - token * p.heads.d) : 0;
     const int b = static_cast<int>(p.tokens.div(token)), t = static_cast<int>(token - b * p.tokens.d);
     const bool live = inside && (p.live == nullptr || t < p.live[b]);
-    const bool is_q = head >= p.num_kv_heads;
-    const int64_t out_at = b * p.out_b + t * p.out_t + lane * 8;
+    const bool is_q = group >= p.kv_units;
+    const int head = is_q ? 2 * kHeads * (group - p.kv_units) : kHeads * group;
+    const int rows = is_q ? p.num_q_heads - head : 2 * (p.num_kv_heads - head);  // (more than a unit's, too)
+    const int64_t out_at = b * p.out_b + t * p.out_t + head * p.out_h + lane * 8;
     if (!__any_sync(0xffffffffu, live)) {
       if (inside && !is_q && p.k_out != nullptr) {
-        *reinterpret_cast<uint4*>(p.k_out + out_at + head * p.out_h) = zeros;
-        *reinterpret_cast<uint4*>(p.v_out + out_at + head * p.out_h) = zeros;
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+          if (2 * i >= rows) break;
+          *reinterpret_cast<uint4*>(p.k_out + out_at + i * p.out_h) = zeros;
+          *reinterpret_cast<uint4*>(p.v_out + out_at + i * p.out_h) = zeros;
+        }
       }
       continue;
     }
-    uint4 x0 = zeros, x1 = zeros;
-    if (is_q) head = 2 * (head - p.num_kv_heads);
-    const bool pair_of_q = is_q && head + 1 < p.num_q_heads;
-    if (live) {
+    uint4 x[kHeads][2];
+    {
       const HeadRows& first = is_q ? p.q : p.k;
-      x0 = *reinterpret_cast<const uint4*>(first.x + b * first.b + t * first.t + head * first.h + lane * 8);
       const HeadRows& second = is_q ? p.q : p.v;
-      if (!is_q || pair_of_q)
-        x1 = *reinterpret_cast<const uint4*>(second.x + b * second.b + t * second.t + (head + is_q) * second.h + lane * 8);
+      const __nv_bfloat16* src = first.x + b * first.b + t * first.t + head * first.h + lane * 8;
+      const __nv_bfloat16* other = second.x + b * second.b + t * second.t + (head + is_q) * second.h + lane * 8;
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i) {
+        x[i][0] = live && 2 * i < rows ? *reinterpret_cast<const uint4*>(src) : zeros;
+        x[i][1] = live && 2 * i + 1 < rows ? *reinterpret_cast<const uint4*>(other) : zeros;
+        src += first.h << is_q;
+        other += second.h << is_q;
+      }
     }
     const int pos = (p.start == nullptr ? 0 : p.start[b]) + t;
     if (live && p.angle != nullptr) {
       if (pos >= 0 && pos < p.angle_rows) {
         const float2* angle = p.angle + static_cast<int64_t>(pos) * (H / 2) + lane * 4;
-        x0 = rotate8(x0, angle);
-        if (is_q) x1 = rotate8(x1, angle);
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+          x[i][0] = rotate8(x[i][0], angle);
+          if (is_q) x[i][1] = rotate8(x[i][1], angle);
+        }
       } else {
         int4_report(p.status);
       }
     }
     if (is_q && live) {
-      *reinterpret_cast<uint4*>(p.q_out + out_at + head * p.out_h) = x0;
-      if (pair_of_q) *reinterpret_cast<uint4*>(p.q_out + out_at + (head + 1) * p.out_h) = x1;
+#pragma unroll
+      for (int i = 0; i < 2 * kHeads; ++i)
+        if (i < rows) *reinterpret_cast<uint4*>(p.q_out + out_at + i * p.out_h) = x[i >> 1][i & 1];
     }
     const bool quantised = live && !is_q;
     if (!__any_sync(0xffffffffu, quantised)) continue;
-    uint32_t k_pair, v_pair;
-    float k_level[8], v_level[8];
-    int byte;
-    const uint32_t k_word = row_word<H>(quantize8(x0, k_pair, k_level), lane, byte);
-    const uint32_t v_word = row_word<H>(quantize8(x1, v_pair, v_level), lane, byte);
-    if (inside && !is_q && p.k_out != nullptr) {
-      *reinterpret_cast<uint4*>(p.k_out + out_at + head * p.out_h) = live ? values8(k_level, k_pair) : zeros;
-      *reinterpret_cast<uint4*>(p.v_out + out_at + head * p.out_h) = live ? values8(v_level, v_pair) : zeros;
+    int64_t slot = -1;  // of the first head; the next one's is a page's rows further
+    if (quantised) {
+      const int col = static_cast<int>(p.page.div(static_cast<uint32_t>(max(pos, 0))));
+      const uint32_t page = pos >= 0 && col < p.max_pages
+                                ? static_cast<uint32_t>(p.page_table[static_cast<int64_t>(b) * p.max_pages + col]) : 0xffffffffu;
+      const int page_size = static_cast<int>(p.page.d);
+      if (page < static_cast<uint32_t>(p.num_pages))
+        slot = (static_cast<int64_t>(page) * p.num_kv_heads + head) * page_size + (pos - col * page_size);
+      else
+        int4_report(p.status);
     }
-    if (!quantised) continue;
-    const int col = static_cast<int>(p.page.div(static_cast<uint32_t>(max(pos, 0))));
-    if (pos < 0 || col >= p.max_pages) {
-      int4_report(p.status);
-      continue;
-    }
-    const int page = p.page_table[static_cast<int64_t>(b) * p.max_pages + col];
-    if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_pages)) {
-      int4_report(p.status);
-      continue;
-    }
-    const int page_size = static_cast<int>(p.page.d);
-    const int64_t slot = (static_cast<int64_t>(page) * p.num_kv_heads + head) * page_size + (pos - col * page_size);
-    *reinterpret_cast<uint32_t*>(p.k_pool.codes + slot * (H / 2) + byte) = k_word;
-    *reinterpret_cast<uint32_t*>(p.v_pool.codes + slot * (H / 2) + byte) = v_word;
-    if ((lane & 3) == 0) {
-      p.k_pool.pairs[slot * (H / kInt4Group) + (lane >> 2)] = k_pair;
-      p.v_pool.pairs[slot * (H / kInt4Group) + (lane >> 2)] = v_pair;
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      uint32_t k_pair, v_pair;
+      float k_level[8], v_level[8];
+      int byte;
+      const uint32_t k_word = row_word<H>(quantize8(x[i][0], k_pair, k_level), lane, byte);
+      const uint32_t v_word = row_word<H>(quantize8(x[i][1], v_pair, v_level), lane, byte);
+      if (2 * i >= rows) continue;
+      if (inside && !is_q && p.k_out != nullptr) {
+        *reinterpret_cast<uint4*>(p.k_out + out_at + i * p.out_h) = live ? values8(k_level, k_pair) : zeros;
+        *reinterpret_cast<uint4*>(p.v_out + out_at + i * p.out_h) = live ? values8(v_level, v_pair) : zeros;
+      }
+      if (slot < 0) continue;
+      const int64_t at = slot + i * static_cast<int64_t>(p.page.d);
+      *reinterpret_cast<uint32_t*>(p.k_pool.codes + at * (H / 2) + byte) = k_word;
+      *reinterpret_cast<uint32_t*>(p.v_pool.codes + at * (H / 2) + byte) = v_word;
+      if ((lane & 3) == 0) {
+        p.k_pool.pairs[at * (H / kInt4Group) + (lane >> 2)] = k_pair;
+        p.v_pool.pairs[at * (H / kInt4Group) + (lane >> 2)] = v_pair;
+      }
     }
   }
 }
@@ -806,20 +826,29 @@ static int int4_attn(const Int4AttnParams& p, int B, cudaStream_t stream) {
 
 namespace axb {
 
-static int int4_append(Int4AppendParams& p, int B, int T, int page_size, int head_dim, cudaStream_t stream) {
-  const int heads = p.num_kv_heads + (p.num_q_heads + 1) / 2;
-  const int64_t units = static_cast<int64_t>(B) * T * heads;
-  if (units >= (int64_t{1} << 30)) return -10;
-  p.heads = FastDiv(heads), p.tokens = FastDiv(T), p.page = FastDiv(page_size);
-  p.units = static_cast<uint32_t>(units);
-  const int64_t per_cta = kAppendThreads / (head_dim / 8);
-  int64_t ctas = (units + per_cta - 1) / per_cta;
+template <int H, int kHeads>
+static int launch_int4_append(Int4AppendParams& p, int64_t tokens, cudaStream_t stream) {
+  p.kv_units = (p.num_kv_heads + kHeads - 1) / kHeads;
+  const int heads = p.kv_units + (p.num_q_heads + 2 * kHeads - 1) / (2 * kHeads);
+  p.heads = FastDiv(heads);
+  p.units = static_cast<uint32_t>(tokens * heads);
+  constexpr int kPerCta = kAppendThreads / (H / 8);
+  int64_t ctas = (tokens * heads + kPerCta - 1) / kPerCta;
   if (ctas > 148 * 32) ctas = 148 * 32;
-  if (head_dim == 128)
-    launch_chained(int4_append_kernel<128>, static_cast<unsigned>(ctas), kAppendThreads, 0, stream, p);
-  else
-    launch_chained(int4_append_kernel<64>, static_cast<unsigned>(ctas), kAppendThreads, 0, stream, p);
+  launch_chained(int4_append_kernel<H, kHeads>, static_cast<unsigned>(ctas), kAppendThreads, 0, stream, p);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
+}
+
+// Two KV heads a unit where units of one would be two waves or more and few units would be half empty (us with one / two: 8 x 2048
+// tokens of 8 heads of 128 43.9 / 38.7, 1 x 2048 7.0 / 7.1, 64 x 1 of 32 2.9 / 3.8).
+static int int4_append(Int4AppendParams& p, int B, int T, int page_size, int head_dim, cudaStream_t stream) {
+  const int64_t tokens = static_cast<int64_t>(B) * T, rows = tokens * (2 * p.num_kv_heads + p.num_q_heads);
+  if (rows >= (int64_t{1} << 31)) return -10;
+  p.tokens = FastDiv(T), p.page = FastDiv(page_size);
+  const bool two = rows / 2 * head_dim >= int64_t{148} * 4 * 2 * kAppendThreads * 8 &&
+                   (p.num_kv_heads % 2 == 0 || p.num_kv_heads > 4);
+  if (head_dim == 128) return two ? launch_int4_append<128, 2>(p, tokens, stream) : launch_int4_append<128, 1>(p, tokens, stream);
+  return two ? launch_int4_append<64, 2>(p, tokens, stream) : launch_int4_append<64, 1>(p, tokens, stream);
 }
 
 }  // namespace axb

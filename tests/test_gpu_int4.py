@@ -249,7 +249,8 @@ def test_bad_places_are_reported_and_not_touched():
 
 
 @pytest.mark.parametrize("b,t,kv,dim,page_size,packed", [(1, 1, 1, 128, 16, False), (3, 37, 2, 64, 12, True), (5, 9, 3, 128, 1, True),
-                                                       (64, 1, 32, 128, 16, True), (2, 700, 8, 128, 64, True)])
+                                                       (64, 1, 32, 128, 16, True), (2, 700, 8, 128, 64, True), (4, 700, 7, 128, 12, True),
+                                                       (6, 900, 8, 64, 16, False)])
 @pytest.mark.parametrize("ragged", [False, True])
 def test_append_has_the_bits_of_the_plain_statement(b, t, kv, dim, page_size, packed, ragged):
     from axlearn_b200.ops import cuda_ops, int4_ops
@@ -547,7 +548,7 @@ def test_a_step_without_a_place_appends_nothing():
         cuda_ops.check_status()
 
 
-@pytest.mark.parametrize("b,t,nq,kv,dim", [(2, 300, 8, 2, 128), (1, 1, 4, 4, 64), (3, 130, 12, 4, 64)])
+@pytest.mark.parametrize("b,t,nq,kv,dim", [(2, 300, 8, 2, 128), (1, 1, 4, 4, 64), (3, 130, 12, 4, 64), (3, 1300, 6, 2, 128)])
 def test_prompts_attend_to_what_the_cache_stands_for(b, t, nq, kv, dim):
     from axlearn_b200.ops import cuda_ops, decode_ops, int4_ops
 
