@@ -403,21 +403,38 @@ def attention_splits(batch: int, num_kv_heads: int, group: int, max_len: int, sm
     return many if many >= 24 else 8
 
 
+def _read_places(page_table: Tensor, lengths: Tensor, page_size: int, num_pages: int) -> tuple[Tensor, Tensor, Tensor]:
+    """Pages to gather ``[B, max_pages]`` (0 where a sequence has none, or one that is not in the pool), which keys are there ``[B,
+    max_pages * page_size]``, and whether a sequence needs a place that is not."""
+    lengths, capacity = lengths.long()[:, None], page_table.shape[1] * page_size
+    at = torch.arange(capacity, device=lengths.device)
+    used = at[::page_size] < lengths
+    inside = (page_table >= 0) & (page_table < num_pages)
+    bad = (used & ~inside).any() | (lengths > capacity).any()
+    there = used & inside
+    return torch.where(there, page_table, 0).long(), there.repeat_interleave(page_size, 1) & (at < lengths), bad
+
+
+def _report_places(bad: Tensor, what: str) -> None:
+    """``bad`` (a truth value): an error on the host, the status word on the GPU."""
+    if bad.is_cuda:
+        word = cuda_ops.status_word(bad.device)
+        word.copy_(torch.where(bad, 5, word))
+    elif bool(bad):
+        raise IndexError(what)
+
+
 def _attention_plain(q, k_pages, v_pages, page_table, lengths, scale):
     b, nq, h = q.shape
-    pages = page_table.long()
-    if not q.is_cuda and b:
-        used = torch.arange(pages.shape[1])[None] * k_pages.codes.shape[2] < lengths[:, None]
-        if bool((used & ((pages < 0) | (pages >= k_pages.codes.shape[0]))).any()) or (
-                int(lengths.max()) > pages.shape[1] * k_pages.codes.shape[2]):
-            raise IndexError("a length behind the page table, or a page outside the pool")
-        pages = torch.where(used, pages, 0)
+    num_pages, _, page_size, _ = k_pages.codes.shape
+    pages, seen, bad = _read_places(page_table, lengths, page_size, num_pages)
+    _report_places(bad, "a length behind the page table, or a page outside the pool")
     k, v = (page_values(Int4Pages(x.codes[pages], x.scales[pages])).transpose(1, 2).flatten(2, 3) for x in (k_pages, v_pages))
-    seen = (torch.arange(k.shape[2], device=q.device) < lengths[:, None])[:, None, :, None]
+    seen = seen[:, None, :, None]
     k, v = torch.where(seen, k, 0), torch.where(seen, v, 0)
     scores = q.float().unflatten(1, (k.shape[1], -1)) @ k.transpose(2, 3) * scale
     p = torch.softmax(scores.masked_fill(~seen.transpose(2, 3), -torch.inf), -1)
-    out = torch.where((lengths > 0)[:, None, None, None], p @ v, 0)
+    out = torch.where(seen.any(2, keepdim=True), p @ v, 0)
     return out.reshape(b, nq, h).to(q.dtype)
 
 

@@ -712,3 +712,25 @@ def test_sample_decode_takes_the_bits_of_the_environment(monkeypatch):
     monkeypatch.setenv("AXB200_DECODE_CACHE_BITS", "8")
     with pytest.raises(ValueError, match="4 or 16"):
         functional(model, prng.PRNGKey(5), params, kwargs, is_training=False, method="sample_decode")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_the_plain_attention_on_the_gpu_reads_the_sequences_pages_alone(dtype):
+    """Types without a kernel, and the plain statement asked for: tables with anything behind a sequence, bad places reported."""
+    from axlearn_b200.ops import cuda_ops, int4_ops
+
+    k_pages, v_pages, table = _cache(3, 4, 16, 2, 64, seed=31)
+    lengths = torch.tensor([5, 33, 0], dtype=torch.int32, device="cuda")
+    q = _normal(_gen(32), 3, 4, 64)
+    want = int4_ops.paged_decode_attention_int4(q.to(dtype), k_pages, v_pages, table, lengths)
+    reference = _plain(int4_ops.paged_decode_attention_int4, q.bfloat16(), k_pages, v_pages, table, lengths)
+    table[0, 1:], table[1, 3:], table[2] = 10 ** 9, -7, 99
+    assert torch.equal(int4_ops.paged_decode_attention_int4(q.to(dtype), k_pages, v_pages, table, lengths), want)
+    assert torch.equal(_plain(int4_ops.paged_decode_attention_int4, q.bfloat16(), k_pages, v_pages, table, lengths), reference)
+    assert not want[2].any()
+    cuda_ops.check_status()
+    table[0, 0] = 99
+    out = int4_ops.paged_decode_attention_int4(q.to(dtype), k_pages, v_pages, table, lengths)
+    with pytest.raises(RuntimeError, match="status 5"):
+        cuda_ops.check_status()
+    assert torch.equal(out[1:], want[1:]) and not out[0].any()

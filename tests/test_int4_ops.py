@@ -156,6 +156,31 @@ def test_attention_over_the_cache_matches_a_loop(heads, kv, dim):
             assert ((out[i, h].double() - p @ vals).abs() <= 2.0 ** -8 * (p @ vals).abs() + 2.0 ** -14 * vals.abs().max()).all()
 
 
+def test_places_read_are_those_of_the_sequences_alone():
+    """What the plain attention gathers on any device: entries behind a sequence may be anything."""
+    table = torch.tensor([[3, 10 ** 9, -7], [0, 6, 2 ** 31 - 1], [-2 ** 31, 7, 7], [1, 2, 3]], dtype=torch.int32)
+    lengths = torch.tensor([4, 5, 0, -3], dtype=torch.int32)
+    pages, seen, bad = int4_ops._read_places(table, lengths, 4, 7)  # pylint: disable=protected-access
+    assert pages.tolist() == [[3, 0, 0], [0, 6, 0], [0, 0, 0], [0, 0, 0]] and not bad
+    assert torch.equal(seen, torch.arange(12) < lengths[:, None])
+    # A page that a sequence needs and the pool does not have, a length behind the table: no key of theirs, nothing outside.
+    for row, page in ((0, 7), (1, -1)):
+        wrong = table.clone()
+        wrong[row, 0] = page
+        pages, seen, bad = int4_ops._read_places(wrong, lengths, 4, 7)  # pylint: disable=protected-access
+        assert bad and pages.min() >= 0 and pages.max() < 7 and not seen[row, :4].any()
+    pages, seen, bad = int4_ops._read_places(table[3:], torch.tensor([13], dtype=torch.int32), 4, 7)  # pylint: disable=protected-access
+    assert bad and pages.tolist() == [[1, 2, 3]] and seen.all()
+    assert int4_ops._read_places(table[:, :0], lengths, 4, 7)[2]  # pylint: disable=protected-access
+
+
+def test_attention_takes_tables_with_anything_behind_a_sequence():
+    args = _attend_args(lengths=torch.tensor([3, 0], dtype=torch.int32))
+    want = int4_ops.paged_decode_attention_int4(**args)
+    args["page_table"][0, 1:], args["page_table"][1] = 10 ** 9, -7
+    assert torch.equal(int4_ops.paged_decode_attention_int4(**args), want)
+
+
 def test_a_decoding_step_is_rotation_append_and_attention():
     b, heads, kv, dim, page_size = 3, 4, 2, 64, 4
     k_pages, v_pages, table = _cache(b, 3, page_size, kv, dim, seed=11)
