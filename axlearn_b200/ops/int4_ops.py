@@ -325,6 +325,15 @@ def _check_counts(counts: Tensor, batch: int, name: str, device) -> Tensor:
     return counts
 
 
+def _report_places(bad: Tensor, what: str) -> None:
+    """``bad`` (a truth value): an error on the host, the status word on the GPU."""
+    if bad.is_cuda:
+        word = cuda_ops.status_word(bad.device)
+        word.copy_(torch.where(bad, 5, word))
+    elif bool(bad):
+        raise IndexError(what)
+
+
 def _rotate(x: Tensor, table: Tensor, pos: Tensor) -> Tensor:
     """``x [B, T, N, H]`` with interleaved pairs turned by ``table [positions, H / 2, 2]`` (sin, cos) at ``pos [B, T]``."""
     sn, cs = table[pos.clamp(0, table.shape[0] - 1)].unbind(-1)
@@ -333,18 +342,25 @@ def _rotate(x: Tensor, table: Tensor, pos: Tensor) -> Tensor:
     return torch.stack((x0 * cs - x1 * sn, x1 * cs + x0 * sn), -1).flatten(-2).to(x.dtype)
 
 
-def _append_plain(k, v, k_pages, v_pages, page_table, start, live):
-    b, t = k.shape[:2]
-    page_size = k_pages.codes.shape[2]
-    at = torch.arange(t, device=k.device)
-    pos = start[:, None].long() + at
-    keep = (at < live[:, None]) if live is not None else torch.ones((b, t), dtype=torch.bool, device=k.device)
+def _write_places(page_table: Tensor, start: Tensor, live: Optional[Tensor], tokens: int, page_size: int, num_pages: int) -> tuple:
+    """``(page, row, keep, inside)`` ``[B, T]`` of new tokens: which are there, and which of them have a place."""
+    pos = start[:, None].long() + torch.arange(tokens, device=start.device)
+    keep = torch.ones_like(pos, dtype=torch.bool)
+    if live is not None:
+        keep = torch.arange(tokens, device=start.device) < live[:, None]
     inside = keep & (pos >= 0) & (pos < page_table.shape[1] * page_size)
-    page = page_table.long().gather(1, (pos // page_size).clamp(0, page_table.shape[1] - 1))
-    inside &= (page >= 0) & (page < k_pages.codes.shape[0])
-    if not k.is_cuda and bool((keep & ~inside).any()):
-        raise IndexError("a token's place is outside the page table, or its page outside the pool")
-    row, values = pos % page_size, []
+    if not page_table.shape[1]:
+        return pos * 0, pos * 0, keep, inside
+    page = page_table.long().gather(1, torch.where(inside, pos // page_size, 0))
+    inside &= (page >= 0) & (page < num_pages)
+    return page, pos % page_size, keep, inside
+
+
+def _append_plain(k, v, k_pages, v_pages, page_table, start, live):
+    num_pages, _, page_size, _ = k_pages.codes.shape
+    page, row, keep, inside = _write_places(page_table, start, live, k.shape[1], page_size, num_pages)
+    _report_places((keep & ~inside).any(), "a token's place is outside the page table, or its page outside the pool")
+    values = []
     for x, pages in ((k, k_pages), (v, v_pages)):
         codes, scales = quantize_groups(x, CACHE_GROUP)
         pages.codes[page[inside], :, row[inside]] = _pack_rows(codes)[inside]
@@ -413,15 +429,6 @@ def _read_places(page_table: Tensor, lengths: Tensor, page_size: int, num_pages:
     bad = (used & ~inside).any() | (lengths > capacity).any()
     there = used & inside
     return torch.where(there, page_table, 0).long(), there.repeat_interleave(page_size, 1) & (at < lengths), bad
-
-
-def _report_places(bad: Tensor, what: str) -> None:
-    """``bad`` (a truth value): an error on the host, the status word on the GPU."""
-    if bad.is_cuda:
-        word = cuda_ops.status_word(bad.device)
-        word.copy_(torch.where(bad, 5, word))
-    elif bool(bad):
-        raise IndexError(what)
 
 
 def _attention_plain(q, k_pages, v_pages, page_table, lengths, scale):

@@ -734,3 +734,25 @@ def test_the_plain_attention_on_the_gpu_reads_the_sequences_pages_alone(dtype):
     with pytest.raises(RuntimeError, match="status 5"):
         cuda_ops.check_status()
     assert torch.equal(out[1:], want[1:]) and not out[0].any()
+
+
+def test_the_plain_append_on_the_gpu_reports_places_that_are_not_there():
+    from axlearn_b200.ops import cuda_ops, int4_ops
+
+    k_pages, v_pages, table = _cache(2, 4, 16, 2, 128, seed=33)
+    k = _normal(_gen(34), 2, 3, 2, 128)
+    before = [x.clone() for x in (*k_pages, *v_pages)]
+    live = torch.tensor([3, 0], dtype=torch.int32, device="cuda")
+    for page, start in ((11, 0), (-1, 0), (0, 64), (0, -3)):
+        bad = table.clone()
+        if page:
+            bad[0, 0] = page
+        int4_ops.append_int4(k, k, k_pages, v_pages, bad, torch.tensor([start, 70], dtype=torch.int32, device="cuda"), live=live)
+        with pytest.raises(RuntimeError, match="status 5"):
+            cuda_ops.check_status()
+        assert all(torch.equal(x, y) for x, y in zip(before, (*k_pages, *v_pages)))
+    int4_ops.append_int4(k, k, k_pages, v_pages, table[:, :0].contiguous(), torch.zeros_like(live), live=live)
+    with pytest.raises(RuntimeError, match="status 5"):
+        cuda_ops.check_status()
+    int4_ops.append_int4(k, k, k_pages, v_pages, table, torch.zeros_like(live), live=live)
+    cuda_ops.check_status()

@@ -135,6 +135,26 @@ def test_append_writes_live_tokens_and_nothing_else(dim, page_size):
         assert torch.equal(old.transpose(1, 2)[~touched], new.transpose(1, 2)[~touched])
 
 
+def test_places_written_are_inside_the_pool():
+    """What the plain append writes to on any device."""
+    table = torch.tensor([[3, 9], [0, 6], [5, -1]], dtype=torch.int32)
+    start, live = torch.tensor([2, 6, -1], dtype=torch.int32), torch.tensor([4, 3, 2], dtype=torch.int32)
+    page, row, keep, inside = int4_ops._write_places(table, start, live, 4, 4, 7)  # pylint: disable=protected-access
+    assert keep.tolist() == [[True] * 4, [True] * 3 + [False], [True] * 2 + [False] * 2]
+    assert inside.tolist() == [[True, True, False, False], [True, True, False, False], [False, True, False, False]]
+    assert page[inside].tolist() == [3, 3, 6, 6, 5] and row[inside].tolist() == [2, 3, 2, 3, 0]
+    _, _, keep, inside = int4_ops._write_places(table[:, :0], start, None, 4, 4, 7)  # pylint: disable=protected-access
+    assert keep.all() and not inside.any()
+
+
+def test_append_refuses_a_table_without_pages():
+    k_pages, v_pages, table = _cache(2, 3, 4, 2, 64)
+    rows, start = _values(2, 1, 2, 64).bfloat16(), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(IndexError, match="page table"):
+        int4_ops.append_int4(rows, rows, k_pages, v_pages, table[:, :0].contiguous(), start)
+    int4_ops.append_int4(rows, rows, k_pages, v_pages, table[:, :0].contiguous(), start, live=start)
+
+
 @pytest.mark.parametrize("heads,kv,dim", [(4, 4, 64), (6, 2, 128)])
 def test_attention_over_the_cache_matches_a_loop(heads, kv, dim):
     b, page_size, lengths = 4, 6, [0, 1, 13, 18]
