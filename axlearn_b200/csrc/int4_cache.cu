@@ -47,12 +47,12 @@ struct Int4AppendParams {
   const int* page_table;
   const int* start;     // null: 0
   const int* live;      // null: all tokens
-  const float2* angle;  // (sin, cos) of [position][H / 2], null: nothing is rotated
+  const float2* angle;  // (sin, cos) of [position][H / 2] for positions 0 to T - 1 (`start` is null); null: nothing is rotated
   int* status;
   FastDiv heads, tokens, page;  // units of a token, tokens of a sequence, positions of a page
   uint32_t units;
   int kv_units;                 // of a token
-  int angle_rows, num_q_heads, num_kv_heads, max_pages, num_pages;
+  int num_q_heads, num_kv_heads, max_pages, num_pages;
 };
 
 // The eight dims 8 l .. 8 l + 7 of a lane, groups of 32 dims are four neighbouring lanes: codes (dim i in bits 4 i), pair and the
@@ -191,15 +191,11 @@ int4_append_kernel(Int4AppendParams p) {
     }
     const int pos = (p.start == nullptr ? 0 : p.start[b]) + t;
     if (live && p.angle != nullptr) {
-      if (pos >= 0 && pos < p.angle_rows) {
-        const float2* angle = p.angle + static_cast<int64_t>(pos) * (H / 2) + lane * 4;
+      const float2* angle = p.angle + static_cast<int64_t>(pos) * (H / 2) + lane * 4;
 #pragma unroll
-        for (int i = 0; i < kHeads; ++i) {
-          x[i][0] = rotate8(x[i][0], angle);
-          if (is_q) x[i][1] = rotate8(x[i][1], angle);
-        }
-      } else {
-        int4_report(p.status);
+      for (int i = 0; i < kHeads; ++i) {
+        x[i][0] = rotate8(x[i][0], angle);
+        if (is_q) x[i][1] = rotate8(x[i][1], angle);
       }
     }
     if (is_q && live) {
@@ -378,9 +374,9 @@ int4_attn_kernel(Int4AttnParams p) {
   // Tiles go to the warps of all splits in turn, so which pages a warp needs does not depend on the length.
   const int step = kAttnWarps * p.splits;
   int tile = split * kAttnWarps + warp;
-  if (len > p.max_pages * static_cast<int64_t>(p.page_size)) {
+  if (len > p.max_pages * static_cast<int64_t>(p.page_size) || (kAppend && len > p.angle_rows)) {
     if (threadIdx.x == 0) int4_report(p.status);
-    len = kAppend ? 0 : p.max_pages * p.page_size;  // a new token without a place: nothing is appended
+    len = kAppend ? 0 : p.max_pages * p.page_size;  // a new token without a place or a rotation: nothing is appended
   }
   const int hi = (max(len, 0) + kAttnKeys - 1) / kAttnKeys;
   const int* table = p.page_table + static_cast<int64_t>(b) * p.max_pages;
@@ -449,8 +445,7 @@ int4_attn_kernel(Int4AttnParams p) {
   int new_byte = 0;
   constexpr int kRowLanes = H / 8;
   if constexpr (kAppend) {
-    if (pos >= p.angle_rows && threadIdx.x == 0) int4_report(p.status);
-    angle = p.angle + static_cast<int64_t>(max(0, min(pos, p.angle_rows - 1))) * (H / 2);
+    angle = p.angle + static_cast<int64_t>(max(0, pos)) * (H / 2);
     if (appends) {
       const int is_v = lane / kRowLanes & 1, l8 = lane % kRowLanes;
       uint4 x = *reinterpret_cast<const uint4*>(
@@ -889,7 +884,8 @@ extern "C" int axb_int4_append_prompt(void* qkv, void* k_codes, void* k_pairs, v
                                       int num_q_heads, int num_kv_heads, int head_dim, int page_size, int max_pages,
                                       int num_pages, int* status, cudaStream_t stream) {
   using namespace axb;
-  if ((head_dim != 64 && head_dim != 128) || page_size < 1 || num_kv_heads < 1 || num_q_heads < 1 || B < 0 || T < 0) return -10;
+  if ((head_dim != 64 && head_dim != 128) || page_size < 1 || num_kv_heads < 1 || num_q_heads < 1 || B < 0 || T < 0 || angle_rows < T)
+    return -10;
   for (const void* x : {static_cast<const void*>(qkv), static_cast<const void*>(angle), static_cast<const void*>(k_codes),
                         static_cast<const void*>(k_pairs), static_cast<const void*>(v_codes), static_cast<const void*>(v_pairs)})
     if (!aligned16(x)) return -10;
@@ -908,7 +904,6 @@ extern "C" int axb_int4_append_prompt(void* qkv, void* k_codes, void* k_pairs, v
   p.v_pool = {static_cast<uint8_t*>(v_codes), static_cast<uint32_t*>(v_pairs)};
   p.page_table = page_table, p.status = status;
   p.angle = reinterpret_cast<const float2*>(angle);
-  p.angle_rows = angle_rows;
   p.num_q_heads = num_q_heads, p.num_kv_heads = num_kv_heads, p.max_pages = max_pages, p.num_pages = num_pages;
   return int4_append(p, B, T, page_size, head_dim, stream);
 }

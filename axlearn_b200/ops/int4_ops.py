@@ -505,7 +505,7 @@ def _check_packed(qkv: Tensor, k_pages: Int4Pages, table: Tensor, nq: int) -> tu
     nkv, h = k_pages.codes.shape[1], k_pages.codes.shape[3] * 2
     if qkv.shape[-1] != (nq + 2 * nkv) * h or not qkv.is_contiguous() or qkv.data_ptr() % 16:
         raise ValueError(f"a packed projection of {nq} + 2 x {nkv} heads of {h} is contiguous and 16-byte aligned: {tuple(qkv.shape)}")
-    if (table.dtype != torch.float32 or table.shape[1:] != (h // 2, 2) or not table.is_contiguous() or table.device != qkv.device
+    if (table.dtype != torch.float32 or table.shape[1:] != (h // 2, 2) or not len(table) or not table.is_contiguous() or table.device != qkv.device
             or table.data_ptr() % 16):
         raise ValueError(f"a rotation table is [positions, {h // 2}, 2] fp32 on {qkv.device}: {tuple(table.shape)} {table.dtype}")
     return nkv, h
@@ -515,8 +515,8 @@ def rope_decode_attention_int4(qkv: Tensor, k_pages: Int4Pages, v_pages: Int4Pag
                                table: Tensor, *, num_q_heads: int, softmax_scale: float, splits: Optional[int] = None,
                                scratch: Optional[Tensor] = None) -> Tensor:
     """``qkv [B, (Nq + 2 Nkv) * H]`` of the token at position ``lengths - 1``: rotates its query and key by ``table [positions,
-    H / 2, 2]`` (``decode_ops.rope_table``), appends key and value to the cache and attends to it.  Rows of length 0 append
-    nothing and get zeros.  Returns ``[B, Nq, H]``."""
+    H / 2, 2]`` (``decode_ops.rope_table``), appends key and value to the cache and attends to it.  Rows of length 0, and those
+    behind the page table or the rotation table, append nothing and get zeros.  Returns ``[B, Nq, H]``."""
     nkv, h = _check_packed(qkv, k_pages, table, num_q_heads)
     if qkv.dim() != 2:
         raise ValueError(f"a step takes one token a sequence, [B, width]: {tuple(qkv.shape)}")
@@ -527,9 +527,10 @@ def rope_decode_attention_int4(qkv: Tensor, k_pages: Int4Pages, v_pages: Int4Pag
         raise ValueError(f"softmax_scale {softmax_scale} is not in (0, 2^20)")
     if not _on_kernel(qkv):
         q, k, v = (x[:, None] for x in _split_qkv(qkv, num_q_heads, nkv))
+        without = lengths > min(table.shape[0], page_table.shape[1] * page_size)  # a place or a rotation
+        _report_places(without.any(), f"a position behind a rotation table of {table.shape[0]} or the page table")
+        lengths = torch.where(without, 0, lengths)
         pos = lengths[:, None].long() - 1
-        if not qkv.is_cuda and bool((pos >= table.shape[0]).any()):
-            raise IndexError(f"a position behind a rotation table of {table.shape[0]}")
         q, k = _rotate(q, table, pos), _rotate(k, table, pos)
         _append_plain(k, v, k_pages, v_pages, page_table, lengths - 1, (lengths > 0).to(torch.int32))
         return paged_decode_attention_int4(q[:, 0], k_pages, v_pages, page_table, lengths, softmax_scale=softmax_scale)

@@ -756,3 +756,28 @@ def test_the_plain_append_on_the_gpu_reports_places_that_are_not_there():
         cuda_ops.check_status()
     int4_ops.append_int4(k, k, k_pages, v_pages, table, torch.zeros_like(live), live=live)
     cuda_ops.check_status()
+
+
+@pytest.mark.parametrize("dim,splits", [(128, 1), (64, 3), (128, 16)])
+@pytest.mark.parametrize("plain", [False, True])
+def test_a_step_behind_the_rotation_table_appends_nothing(dim, splits, plain):
+    from axlearn_b200.ops import cuda_ops, decode_ops, int4_ops
+
+    k_pages, v_pages, table = _cache(3, 8, 16, 2, dim, seed=35)
+    rope = decode_ops.rope_table(128, dim, 1e4, "cuda")
+    qkv = _normal(_gen(36), 3, 8 * dim).bfloat16()
+
+    def step(cache, positions, lengths):
+        call = _plain if plain else (lambda fn, *args, **kwargs: fn(*args, **kwargs))
+        return call(int4_ops.rope_decode_attention_int4, qkv, *cache, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"),
+                    rope[:positions].contiguous(), num_q_heads=4, softmax_scale=0.1, splits=splits)
+
+    caches = [[int4_ops.Int4Pages(*(x.clone() for x in p)) for p in (k_pages, v_pages)] for _ in range(2)]
+    out = step(caches[0], 70, [100, 70, 71])          # the last position of the table is 69
+    with pytest.raises(RuntimeError, match="status 5"):
+        cuda_ops.check_status()
+    want = step(caches[1], 128, [0, 70, 0])
+    cuda_ops.check_status()
+    assert torch.equal(out, want) and not out[0].any() and out[1].any() and not out[2].any()
+    for x, y in zip(caches[0], caches[1]):
+        assert torch.equal(x.codes, y.codes) and torch.equal(x.scales, y.scales)

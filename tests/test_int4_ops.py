@@ -309,6 +309,20 @@ def test_a_step_refuses_tokens_it_does_not_take():
         int4_ops.rope_decode_attention_int4(qkv, k_pages, v_pages, table, lengths + 1, rope, **args)
 
 
+def test_a_step_refused_for_its_position_leaves_the_cache():
+    k_pages, v_pages, table = _cache(2, 3, 4, 2, 64)
+    before = [x.clone() for x in (*k_pages, *v_pages)]
+    qkv = _values(2, 8 * 64).bfloat16()
+    for positions, length in ((8, 9), (20, 13)):     # behind the rotation table, behind the page table
+        with pytest.raises(IndexError):
+            int4_ops.rope_decode_attention_int4(qkv, k_pages, v_pages, table, torch.tensor([3, length], dtype=torch.int32),
+                                                torch.zeros(positions, 32, 2), num_q_heads=4, softmax_scale=0.1)
+        assert all(torch.equal(x, y) for x, y in zip(before, (*k_pages, *v_pages)))
+    with pytest.raises(ValueError):                  # a rotation table without a position
+        int4_ops.rope_decode_attention_int4(qkv, k_pages, v_pages, table, torch.zeros(2, dtype=torch.int32), torch.zeros(0, 32, 2),
+                                            num_q_heads=4, softmax_scale=0.1)
+
+
 def test_a_pool_without_pages_is_refused():
     empty, table = int4_ops.int4_pages(0, 4, 2, 64), torch.zeros(2, 3, dtype=torch.int32)
     lengths = torch.zeros(2, dtype=torch.int32)
