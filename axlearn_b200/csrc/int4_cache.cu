@@ -927,11 +927,11 @@ extern "C" int axb_int4_decode_attn(const void* q, void* k_codes, void* k_pairs,
       !(softmax_scale > 0.f && softmax_scale < 1048576.f) ||
       static_cast<int64_t>(num_pages) * num_kv_heads * page_size >= 0xffffffffll || (angle != nullptr && angle_rows < 1))
     return -10;
+  if (B == 0) return 0;
   for (const void* x : {q, static_cast<const void*>(angle), static_cast<const void*>(k_codes), static_cast<const void*>(k_pairs),
                         static_cast<const void*>(v_codes), static_cast<const void*>(v_pairs)})
     if (!aligned16(x)) return -10;
   if (splits > kAttnCluster && (scratch == nullptr || (reinterpret_cast<uintptr_t>(scratch) & 7) || splits % kAttnCluster)) return -10;
-  if (B == 0) return 0;
   Int4AttnParams p = {};
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.angle = reinterpret_cast<const float2*>(angle);

@@ -411,8 +411,8 @@ def attention_splits(batch: int, num_kv_heads: int, group: int, max_len: int, sm
     query heads), 64 tokens or more for each.  Beyond 8, which meet in a cluster, the clusters' parts are merged by a second
     launch: for long sequences, growing with the root of their length (8 heads, us with 8 / 16 / 32 / 64 splits: 4000 tokens 8.3
     9.5 8.6 10.9, 16000 tokens 24 19 14.6 16.0, 130001 tokens 151 91 52 47), and as many as clusters of 8 fit the GPU."""
-    ctas = batch * num_kv_heads * ((group + 7) // 8)
-    splits = max(1, min(max_len // 64, 4 * sms // max(1, ctas)))
+    ctas = max(1, batch * num_kv_heads * ((group + 7) // 8))
+    splits = max(1, min(max_len // 64, 4 * sms // ctas))
     if splits <= 8:
         return splits
     many = min((math.isqrt(max_len) // 4 + 4) // 8, 512 // ctas // 8) * 8
@@ -551,6 +551,8 @@ def prompt_attention_int4(qkv: Tensor, k_pages: Int4Pages, v_pages: Int4Pages, p
     num_pages, _, page_size = _check_pages(k_pages, v_pages, page_table, b, num_q_heads, h, device)
     if table.shape[0] < t or page_table.shape[1] * k_pages.codes.shape[2] < t:
         raise ValueError(f"{b} x {t} tokens, a rotation table of {table.shape[0]} positions, a page table {tuple(page_table.shape)}")
+    if not qkv.numel():
+        return qkv.new_empty((b, t, num_q_heads * h))
     q, k, v = _split_qkv(qkv, num_q_heads, nkv)
     if not _on_kernel(qkv):
         pos = torch.arange(t, device=qkv.device).expand(b, t)

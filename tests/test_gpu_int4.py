@@ -781,3 +781,25 @@ def test_a_step_behind_the_rotation_table_appends_nothing(dim, splits, plain):
     assert torch.equal(out, want) and not out[0].any() and out[1].any() and not out[2].any()
     for x, y in zip(caches[0], caches[1]):
         assert torch.equal(x.codes, y.codes) and torch.equal(x.scales, y.scales)
+
+
+@pytest.mark.parametrize("splits", [None, 1, 8, 9, 16])
+def test_empty_calls(splits):
+    from axlearn_b200.ops import cuda_ops, decode_ops, int4_ops
+
+    k_pages, v_pages, _ = _cache(2, 3, 16, 2, 128, seed=37)
+    before = [x.clone() for x in (*k_pages, *v_pages)]
+    table, none = (torch.zeros(0, *shape, dtype=torch.int32, device="cuda") for shape in ((200,), ()))
+    rope = decode_ops.rope_table(3200, 128, 1e4, "cuda")
+    q, qkv = (torch.empty(0, *shape, dtype=torch.bfloat16, device="cuda") for shape in ((4, 128), (1024,)))
+    assert int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, none, splits=splits).shape == (0, 4, 128)
+    assert int4_ops.rope_decode_attention_int4(qkv, k_pages, v_pages, table, none, rope, num_q_heads=4, softmax_scale=0.1,
+                                               splits=splits).shape == (0, 4, 128)
+    for b, t in ((0, 5), (2, 0)):
+        table, start = (torch.zeros(b, *shape, dtype=torch.int32, device="cuda") for shape in ((200,), ()))
+        rows = torch.empty(b, t, 2, 128, dtype=torch.bfloat16, device="cuda")
+        assert int4_ops.append_int4(rows, rows, k_pages, v_pages, table, start, values=True)[0].shape == rows.shape
+        prompt = torch.empty(b, t, 1024, dtype=torch.bfloat16, device="cuda")
+        assert int4_ops.prompt_attention_int4(prompt, k_pages, v_pages, table, rope, num_q_heads=4, softmax_scale=0.1).shape == (b, t, 512)
+    cuda_ops.check_status()
+    assert all(torch.equal(x, y) for x, y in zip(before, (*k_pages, *v_pages)))

@@ -362,6 +362,28 @@ def test_plans_of_products(rows, k, n):
     assert splits == 1 or -(-n // (16 * warps)) * -(-rows // 128) * splits <= 2 * 148
 
 
+@pytest.mark.parametrize("tokens", [1, 64, 575, 576, 2048, 130048])
+@pytest.mark.parametrize("kv,group", [(1, 1), (8, 4), (32, 16)])
+def test_splits_of_an_empty_batch(kv, group, tokens):
+    assert int4_ops.attention_splits(0, kv, group, tokens) >= 1
+
+
+def test_empty_calls():
+    k_pages, v_pages, _ = _cache(2, 3, 4, 2, 64)
+    before = [x.clone() for x in (*k_pages, *v_pages)]
+    table, none, rope = torch.zeros(0, 200, dtype=torch.int32), torch.zeros(0, dtype=torch.int32), torch.zeros(8, 32, 2)
+    assert int4_ops.paged_decode_attention_int4(torch.zeros(0, 4, 64).bfloat16(), k_pages, v_pages, table, none).shape == (0, 4, 64)
+    args = dict(num_q_heads=4, softmax_scale=0.1)
+    assert int4_ops.rope_decode_attention_int4(torch.zeros(0, 512).bfloat16(), k_pages, v_pages, table, none, rope, **args).shape == (0, 4, 64)
+    for b, t in ((0, 5), (2, 0)):
+        table, start = torch.zeros(b, 200, dtype=torch.int32), torch.zeros(b, dtype=torch.int32)
+        rows = torch.zeros(b, t, 2, 64).bfloat16()
+        assert int4_ops.append_int4(rows, rows, k_pages, v_pages, table, start, values=True)[0].shape == rows.shape
+        qkv = torch.zeros(b, t, 512).bfloat16()
+        assert int4_ops.prompt_attention_int4(qkv, k_pages, v_pages, table, rope, **args).shape == (b, t, 256)
+    assert all(torch.equal(x, y) for x, y in zip(before, (*k_pages, *v_pages)))
+
+
 @pytest.mark.parametrize("batch,kv,group,tokens", [(1, 16, 1, 300), (16, 8, 4, 2048), (64, 32, 1, 2000), (1, 8, 4, 130048),
                                                    (1, 1, 1, 1), (0, 4, 1, 64), (300, 32, 16, 4096)])
 def test_splits_of_attention(batch, kv, group, tokens):
