@@ -12,7 +12,8 @@ overflows, stands for NaN.
 * ``prompt_attention_int4``, ``rope_decode_attention_int4``: what a prompt and a decoding step run, with the rotation of
   queries and keys and the append.
 
-Attention sees what the cache stands for, in prompts as in steps.  CUDA tensors in bf16 go to the kernels, everything
+Attention sees what the cache stands for, in prompts as in steps.  Serving only: operands that need a gradient, or carry a
+tangent, are refused.  CUDA tensors in bf16 go to the kernels, everything
 else runs the plain statements, which are also the oracle in tests.  Places on the GPU that a page table or a length gets
 wrong (a page that the pool does not have, a position behind the table) are not touched; they set the device's status
 word, which ``cuda_ops.check_status`` raises.  The bf16 forms of these operations are ``cuda_ops.gemm`` and
@@ -59,6 +60,18 @@ def _lib():
 
 def _on_kernel(x: Tensor) -> bool:
     return x.is_cuda and x.dtype == torch.bfloat16 and not dispatch._flags.force_reference  # pylint: disable=protected-access
+
+
+def _no_gradient(name: str, *tensors: Optional[Tensor]) -> None:
+    """Refuses operands that are differentiated, backward or forward, on every device and in every type."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{name} has no gradient")
+    if cuda_ops._transformed():  # pylint: disable=protected-access
+        for t in tensors:
+            if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{name} has no gradient")
 
 
 def _on(device: torch.device):
@@ -221,8 +234,7 @@ def int4_linear(x: Tensor, w: Int4Weight, *, out: Optional[Tensor] = None, accum
     device = x.device
     if x.shape[-1] != k or device != codes.device:
         raise ValueError(f"x {tuple(x.shape)} on {device} and a {w.shape} weight on {codes.device}")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise ValueError("int4_linear has no gradient")
+    _no_gradient("int4_linear", x, w.scales, out)
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
@@ -385,6 +397,7 @@ def append_int4(k: Tensor, v: Tensor, k_pages: Int4Pages, v_pages: Int4Pages, pa
     _check_counts(start, b, "start", device)
     if live is not None:
         _check_counts(live, b, "live", device)
+    _no_gradient("append_int4", k, v, k_pages.scales, v_pages.scales)
     if not _on_kernel(k):
         out = _append_plain(k, v, k_pages, v_pages, page_table, start, live)
         return tuple(out) if values else None
@@ -460,6 +473,7 @@ def paged_decode_attention_int4(q: Tensor, k_pages: Int4Pages, v_pages: Int4Page
         raise ValueError(f"softmax_scale {scale} is not in (0, 2^20)")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != device or not out.is_contiguous()):
         raise ValueError(f"out {tuple(out.shape)} {out.dtype}: contiguous {tuple(q.shape)} {q.dtype} is wanted")
+    _no_gradient("paged_decode_attention_int4", q, k_pages.scales, v_pages.scales, out)
     if not _on_kernel(q):
         y = _attention_plain(q, k_pages, v_pages, page_table, lengths, scale)
         return y if out is None else out.copy_(y)
@@ -525,6 +539,7 @@ def rope_decode_attention_int4(qkv: Tensor, k_pages: Int4Pages, v_pages: Int4Pag
     _check_counts(lengths, b, "lengths", device)
     if not 0 < softmax_scale < 2 ** 20:
         raise ValueError(f"softmax_scale {softmax_scale} is not in (0, 2^20)")
+    _no_gradient("rope_decode_attention_int4", qkv, k_pages.scales, v_pages.scales, table)
     if not _on_kernel(qkv):
         q, k, v = (x[:, None] for x in _split_qkv(qkv, num_q_heads, nkv))
         without = lengths > min(table.shape[0], page_table.shape[1] * page_size)  # a place or a rotation
@@ -551,6 +566,7 @@ def prompt_attention_int4(qkv: Tensor, k_pages: Int4Pages, v_pages: Int4Pages, p
     num_pages, _, page_size = _check_pages(k_pages, v_pages, page_table, b, num_q_heads, h, device)
     if table.shape[0] < t or page_table.shape[1] * k_pages.codes.shape[2] < t:
         raise ValueError(f"{b} x {t} tokens, a rotation table of {table.shape[0]} positions, a page table {tuple(page_table.shape)}")
+    _no_gradient("prompt_attention_int4", qkv, k_pages.scales, v_pages.scales, table)
     if not qkv.numel():
         return qkv.new_empty((b, t, num_q_heads * h))
     q, k, v = _split_qkv(qkv, num_q_heads, nkv)

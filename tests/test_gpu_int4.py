@@ -803,3 +803,22 @@ def test_empty_calls(splits):
         assert int4_ops.prompt_attention_int4(prompt, k_pages, v_pages, table, rope, num_q_heads=4, softmax_scale=0.1).shape == (b, t, 512)
     cuda_ops.check_status()
     assert all(torch.equal(x, y) for x, y in zip(before, (*k_pages, *v_pages)))
+
+
+def test_differentiated_operands_are_refused():
+    from axlearn_b200.ops import int4_ops
+
+    k_pages, v_pages, table = _cache(2, 3, 16, 2, 128, seed=38)
+    lengths = torch.tensor([3, 40], dtype=torch.int32, device="cuda")
+    q, w = _normal(_gen(39), 2, 4, 128).bfloat16(), int4_ops.quantize_weight(_normal(_gen(40), 512, 64))
+    calls = [(q, lambda x: int4_ops.paged_decode_attention_int4(x, k_pages, v_pages, table, lengths)),
+             (q.view(2, 512), lambda x: int4_ops.int4_linear(x, w)),
+             (q.view(2, 2, 2, 128), lambda x: int4_ops.append_int4(x, q.view(2, 2, 2, 128), k_pages, v_pages, table, lengths))]
+    for x, fn in calls:
+        fn(x)
+        with pytest.raises(ValueError, match="no gradient"):
+            fn(x.clone().requires_grad_())
+        with torch.no_grad():
+            fn(x.clone().requires_grad_())
+        with torch.autograd.forward_ad.dual_level(), pytest.raises(ValueError, match="no gradient"):
+            fn(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))

@@ -333,6 +333,44 @@ def test_a_pool_without_pages_is_refused():
         int4_ops.append_int4(rows, rows, empty, empty, table, lengths)
 
 
+def _calls_with_operands():
+    """``(name, call, operands)``: each operand may be differentiated by a caller who does not know better."""
+    k_pages, v_pages, table = _cache(2, 3, 4, 2, 64)
+    lengths, start, rope = torch.tensor([3, 8], dtype=torch.int32), torch.zeros(2, dtype=torch.int32), torch.zeros(8, 32, 2)
+    w = int4_ops.quantize_weight(_values(64, 16))
+    args = dict(num_q_heads=4, softmax_scale=0.1)
+    rows, packed = _values(2, 1, 2, 64).bfloat16(), _values(2, 512).bfloat16()
+    return [
+        ("int4_linear", lambda x, out: int4_ops.int4_linear(x, w, out=out, accumulate=True), (_values(3, 64), torch.zeros(3, 16))),
+        ("append_int4", lambda k, v: int4_ops.append_int4(k, v, k_pages, v_pages, table, start, values=True), (rows, rows.clone())),
+        ("paged_decode_attention_int4", lambda q, out: int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, lengths, out=out),
+         (_values(2, 4, 64).bfloat16(), torch.zeros(2, 4, 64).bfloat16())),
+        ("rope_decode_attention_int4",
+         lambda qkv: int4_ops.rope_decode_attention_int4(qkv, k_pages, v_pages, table, lengths, rope, **args), (packed,)),
+        ("prompt_attention_int4",
+         lambda qkv: int4_ops.prompt_attention_int4(qkv, k_pages, v_pages, table, rope, **args), (packed[:, None].clone(),)),
+    ]
+
+
+@pytest.mark.parametrize("call", range(5))
+def test_differentiated_operands_are_refused(call):
+    name, fn, operands = _calls_with_operands()[call]
+    fn(*operands)
+    for i, x in enumerate(operands):
+        given = [t.clone() for t in operands]
+        given[i].requires_grad_()
+        with pytest.raises(ValueError, match=f"{name} has no gradient"):
+            fn(*given)
+        with torch.no_grad():
+            fn(*given)
+        given = [t.clone() for t in operands]
+        with torch.autograd.forward_ad.dual_level():
+            fn(*given)
+            given[i] = torch.autograd.forward_ad.make_dual(given[i], torch.ones_like(x))
+            with pytest.raises(ValueError, match=f"{name} has no gradient"):
+                fn(*given)
+
+
 def test_weights_and_products_refuse():
     w = int4_ops.quantize_weight(_values(64, 16))
     for shape, group in (((60, 16), 128), ((64, 12), 128), ((64, 16), 32)):
