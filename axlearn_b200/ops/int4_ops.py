@@ -74,6 +74,17 @@ def _no_gradient(name: str, *tensors: Optional[Tensor]) -> None:
                 raise ValueError(f"{name} has no gradient")
 
 
+def _overlap(x: Tensor, y: Tensor) -> bool:
+    """Whether the memory that two tensors span has a part in common."""
+    if not x.numel() or not y.numel():
+        return False
+    spans = []
+    for t in (x, y):
+        elements = 1 + sum((size - 1) * stride for size, stride in zip(t.shape, t.stride()))
+        spans.append((t.data_ptr(), t.data_ptr() + elements * t.element_size()))
+    return spans[0][0] < spans[1][1] and spans[1][0] < spans[0][1]
+
+
 def _on(device: torch.device):
     """The device of the operands made the current one, where it is another."""
     return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
@@ -227,7 +238,7 @@ def fused_plan(rows: int, k: int, n: int) -> tuple[int, int]:
 
 def int4_linear(x: Tensor, w: Int4Weight, *, out: Optional[Tensor] = None, accumulate: bool = False) -> Tensor:
     """``x [..., K] @ w`` with fp32 accumulation, rounded to ``x.dtype``; into ``out [..., N]``, or with ``accumulate`` added to
-    it.  Few rows multiply with the 4-bit weights as they are (``multiplies_codes``), more rows with their values rounded to
+    it; ``out`` may be ``x`` itself, or overlap it.  Few rows multiply with the 4-bit weights as they are (``multiplies_codes``), more rows with their values rounded to
     bf16.  Serving only: there is no gradient.  Products keep their digits for x from 2^-57 up to 2^56, weights from 2^-62 and
     steps below 2^31; sums that overflow fp32 on the way, as with an infinity in x, are NaN."""
     k, n, codes = w.k, w.n, w.codes
@@ -235,7 +246,8 @@ def int4_linear(x: Tensor, w: Int4Weight, *, out: Optional[Tensor] = None, accum
     if x.shape[-1] != k or device != codes.device:
         raise ValueError(f"x {tuple(x.shape)} on {device} and a {w.shape} weight on {codes.device}")
     _no_gradient("int4_linear", x, w.scales, out)
-    if out is None:
+    given = out is not None
+    if not given:
         if accumulate:
             raise ValueError("accumulate needs out")
         out = x.new_empty(x.shape[:-1] + (n,))
@@ -244,6 +256,8 @@ def int4_linear(x: Tensor, w: Int4Weight, *, out: Optional[Tensor] = None, accum
     if not _on_kernel(x):
         y = x.float() @ dequantize_weight(w, torch.float32)
         return out.copy_(out.float() + y if accumulate else y)
+    if given and _overlap(x, out):  # other columns' products still read x
+        x = x.clone()
     rows = x.shape[0] if x.dim() == 2 else out.numel() // n
     if rows == 0:
         return out
@@ -462,7 +476,7 @@ def paged_decode_attention_int4(q: Tensor, k_pages: Int4Pages, v_pages: Int4Page
                                 softmax_scale: Optional[float] = None, splits: Optional[int] = None,
                                 out: Optional[Tensor] = None, scratch: Optional[Tensor] = None) -> Tensor:
     """q ``[B, Nq, H]``; page_table ``[B, max_pages]``, lengths ``[B]`` int32 (valid tokens per sequence; 0: zeros).  Query heads
-    are grouped by KV head.  ``scratch``: ``attention_scratch_floats`` fp32 values, for more than eight splits (made a
+    are grouped by KV head.  ``out`` may be ``q``, or overlap it.  ``scratch``: ``attention_scratch_floats`` fp32 values, for more than eight splits (made a
     multiple of eight); calls that overlap on the GPU need one each.  Returns ``[B, Nq, H]``."""
     b, nq, h = q.shape
     device = q.device
@@ -477,7 +491,8 @@ def paged_decode_attention_int4(q: Tensor, k_pages: Int4Pages, v_pages: Int4Page
     if not _on_kernel(q):
         y = _attention_plain(q, k_pages, v_pages, page_table, lengths, scale)
         return y if out is None else out.copy_(y)
-    if not q.is_contiguous() or q.data_ptr() % 16:
+    # (In place is fine: a CTA, and its cluster, has its heads' queries before it stores their output.)
+    if not q.is_contiguous() or q.data_ptr() % 16 or (out is not None and q.data_ptr() != out.data_ptr() and _overlap(q, out)):
         q = q.clone(memory_format=torch.contiguous_format)
     if out is None:
         out = torch.empty_like(q)

@@ -822,3 +822,35 @@ def test_differentiated_operands_are_refused():
             fn(x.clone().requires_grad_())
         with torch.autograd.forward_ad.dual_level(), pytest.raises(ValueError, match="no gradient"):
             fn(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+@pytest.mark.parametrize("rows", [3, 16, 40, 200, 600])
+@pytest.mark.parametrize("k", [264, 2048, 4104])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_linear_in_place(rows, k, accumulate):
+    """``out`` is x, or begins a row before or behind it."""
+    from axlearn_b200.ops import cuda_ops, int4_ops
+
+    gen = _gen(rows + k)
+    w = int4_ops.quantize_weight(_normal(gen, k, k) * k ** -0.5)
+    flat = _normal(gen, rows + 2, k).bfloat16()
+    for start in (0, 1, 2):
+        buffer = flat.clone()
+        x, out = buffer[1:rows + 1], buffer[start:start + rows]
+        want = int4_ops.int4_linear(x.clone(), w, out=out.clone(), accumulate=accumulate)
+        assert torch.equal(int4_ops.int4_linear(x, w, out=out, accumulate=accumulate), want)
+    cuda_ops.check_status()
+
+
+@pytest.mark.parametrize("nq,kv,dim,splits", [(8, 2, 128, 1), (8, 8, 64, 8), (40, 2, 128, 3), (4, 1, 128, 16)])
+def test_attention_in_place(nq, kv, dim, splits):
+    from axlearn_b200.ops import int4_ops
+
+    k_pages, v_pages, table = _cache(9, 40, 16, kv, dim, seed=41)
+    lengths = torch.arange(0, 9, dtype=torch.int32, device="cuda") * 80
+    flat = _normal(_gen(42), 9 * nq * dim + 64).bfloat16()
+    for start in (0, 16, 64):
+        buffer = flat.clone()
+        q, out = buffer[:-64].view(9, nq, dim), buffer[start:start + 9 * nq * dim].view(9, nq, dim)
+        want = int4_ops.paged_decode_attention_int4(q.clone(), k_pages, v_pages, table, lengths, splits=splits)
+        assert torch.equal(int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, lengths, splits=splits, out=out), want)

@@ -99,6 +99,24 @@ def test_linear_matches_its_formula_and_adds_to_out():
     assert int4_ops.int4_linear(x[:0], w).shape == (0, 3, 24)
 
 
+def test_memory_that_tensors_have_in_common():
+    x = torch.zeros(10, 16)
+    for a, b, want in ((x, x, True), (x[:4], x[4:], False), (x[:4], x[3:], True), (x[:, :8], x[:, 8:], True),  # (spans, not rows)
+                       (x[:0], x, False), (x[2], x.view(-1)[47:48], True), (x[2], x.view(-1)[48:49], False), (x, x.clone(), False)):
+        assert int4_ops._overlap(a, b) == int4_ops._overlap(b, a) == want  # pylint: disable=protected-access
+
+
+def test_products_and_attention_in_place():
+    w, x = int4_ops.quantize_weight(_values(64, 64, seed=4)), _values(3, 64, seed=5)
+    want = int4_ops.int4_linear(x, w)
+    flat = torch.cat([torch.zeros(64), x.flatten()])
+    assert torch.equal(int4_ops.int4_linear(flat[64:].view(3, 64), w, out=flat[:-64].view(3, 64)), want)
+    assert torch.equal(int4_ops.int4_linear(x, w, out=x), want)
+    args = _attend_args()
+    want = int4_ops.paged_decode_attention_int4(**args)
+    assert torch.equal(int4_ops.paged_decode_attention_int4(**args, out=args["q"]), want)
+
+
 def _cache(b, max_pages, page_size, kv, dim, seed=0, spare=2):
     gen = torch.Generator().manual_seed(seed)
     pools = [int4_ops.int4_pages(b * max_pages + spare, page_size, kv, dim) for _ in range(2)]
