@@ -854,3 +854,33 @@ def test_attention_in_place(nq, kv, dim, splits):
         q, out = buffer[:-64].view(9, nq, dim), buffer[start:start + 9 * nq * dim].view(9, nq, dim)
         want = int4_ops.paged_decode_attention_int4(q.clone(), k_pages, v_pages, table, lengths, splits=splits)
         assert torch.equal(int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, lengths, splits=splits, out=out), want)
+
+
+@pytest.mark.parametrize("nq,kv,dim,splits", [(4, 4, 128, 1), (8, 2, 64, 3), (20, 2, 128, 9), (24, 3, 64, 8), (32, 8, 128, None)])
+@pytest.mark.parametrize("page_size", [16, 12])
+def test_a_step_with_exact_rotations(nq, kv, dim, splits, page_size):
+    """Quarter turns: products with 0 and 1 are exact, so what is appended has the plain statement's bits and the output keeps to
+    the bound of attention alone.  The new key is like its first head's query and takes most of that head's weight."""
+    from axlearn_b200.ops import cuda_ops, int4_ops
+
+    lens = [1, 2, 16, 17, 32, 33, 95, 96, 97, 127, 128, 129, 300]
+    b = len(lens)
+    k_pages, v_pages, table = _cache(b, -(-300 // page_size), page_size, kv, dim, seed=43)
+    other = [int4_ops.Int4Pages(*(x.clone() for x in p)) for p in (k_pages, v_pages)]
+    lengths = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    turns = (torch.arange(300, device="cuda")[:, None] + torch.arange(dim // 2, device="cuda")) % 4
+    rope = torch.tensor([[0.0, 1.0], [1.0, 0.0], [0.0, -1.0], [-1.0, 0.0]], device="cuda")[turns].contiguous()
+    qkv = _normal(_gen(44), b, nq + 2 * kv, dim).bfloat16()
+    qkv[:, nq:nq + kv] = 2 * qkv[:, :nq:nq // kv]
+    args = dict(num_q_heads=nq, softmax_scale=dim ** -0.5)
+    out = int4_ops.rope_decode_attention_int4(qkv.flatten(1), k_pages, v_pages, table, lengths, rope, splits=splits, **args)
+    _plain(int4_ops.rope_decode_attention_int4, qkv.flatten(1), *other, table, lengths, rope, **args)
+    cuda_ops.check_status()
+    for mine, plain in zip((k_pages, v_pages), other):
+        assert torch.equal(mine.codes, plain.codes) and torch.equal(mine.scales, plain.scales)
+    q = int4_ops._rotate(qkv[:, None, :nq], rope, lengths[:, None].long() - 1)[:, 0]  # pylint: disable=protected-access
+    want, bound = _attention64(q, k_pages, v_pages, table, lengths, dim ** -0.5)
+    assert ((out.double() - want).abs() <= bound).all()
+    without, _ = _attention64(q, k_pages, v_pages, table, lengths - 1, dim ** -0.5)
+    first = slice(None, None, nq // kv)
+    assert (((want - without).abs() > 8 * bound)[:, first].float().mean((1, 2)) > 0.8).all()

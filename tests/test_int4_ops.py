@@ -268,6 +268,50 @@ def test_prompts_attend_to_what_the_cache_stands_for():
         assert torch.equal(x, y)
 
 
+def _attention64(q, k, v, scale):
+    """One query ``[N, H]`` over ``k, v [S, Nkv, H]`` in 64 bits, and what 32-bit sums and the output's rounding to bf16 may add."""
+    q, k, v = q.double(), k.double().transpose(0, 1), v.double().transpose(0, 1)
+    qg = q.unflatten(0, (k.shape[0], -1))
+    p = torch.softmax(qg @ k.transpose(1, 2) * scale, -1)
+    out, size = p @ v, p @ v.abs()
+    # A score: products of bf16 are exact, H sums and a factor, each 2^-24 of the terms; a probability moves by e^(2 move).  Then exp
+    # and the division, a few 2^-24, and sums of S terms twice.
+    move = (q.shape[1] + 2) * 2.0 ** -24 * scale * (qg.abs() @ k.abs().transpose(1, 2)).amax(-1, keepdim=True)
+    bound = (torch.expm1(2 * move) + (2 * k.shape[1] + 16) * 2.0 ** -24) * size
+    return out.flatten(0, 1), (1.01 * bound + 2.0 ** -8 * (out.abs() + bound)).flatten(0, 1)
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (3, 1, 128)])
+def test_prompts_and_steps_have_the_values_of_their_formula(heads, kv, dim):
+    """Prompts attend to the cache's values rounded to bf16, steps to the values themselves; a token that is missing, or one too
+    many, is far outside the bounds."""
+    b, t, scale = 2, 11, 0.15
+    k_pages, v_pages, table = _cache(b, 3, 4, kv, dim, seed=15)
+    angle = torch.arange(t)[:, None] * 0.5 ** torch.arange(dim // 2)
+    rope = torch.stack((angle.sin(), angle.cos()), -1)
+    qkv = _values(b, t, (heads + 2 * kv) * dim, seed=16).bfloat16()
+    given = qkv.clone()
+    out = int4_ops.prompt_attention_int4(qkv, k_pages, v_pages, table, rope, num_q_heads=heads, softmax_scale=scale).unflatten(-1, (heads, dim))
+    q, k, v = qkv.unflatten(-1, (-1, dim)).split((heads, kv, kv), 2)
+    held = [int4_ops.page_values(p)[table.long()].transpose(2, 3).flatten(1, 2)[:, :t] for p in (k_pages, v_pages)]
+    assert torch.equal(k, held[0].bfloat16()) and torch.equal(v, held[1].bfloat16())
+    step_pages = _cache(b, 3, 4, kv, dim, seed=15)
+    far = 0
+    for i in range(t):
+        lens = torch.full((b,), i + 1, dtype=torch.int32)
+        one = int4_ops.rope_decode_attention_int4(given[:, i].contiguous(), step_pages[0], step_pages[1], table, lens, rope,
+                                                  num_q_heads=heads, softmax_scale=scale)
+        for j in range(b):
+            want, bound = _attention64(q[j, i], k[j, :i + 1], v[j, :i + 1], scale)
+            assert ((out[j, i].double() - want).abs() <= bound).all()
+            want, bound = _attention64(q[j, i], held[0][j, :i + 1], held[1][j, :i + 1], scale)
+            assert ((one[j].double() - want).abs() <= bound).all()
+            for n in {i, i + 2} & set(range(1, t + 1)):
+                other, _ = _attention64(q[j, i], held[0][j, :n], held[1][j, :n], scale)
+                far += ((other - want).abs() > 4 * bound).float().mean() > 0.5
+    assert far >= 0.9 * 2 * b * (t - 1)
+
+
 def _attend_args(**change):
     k_pages, v_pages, table = _cache(2, 3, 4, 2, 64)
     args = dict(q=_values(2, 4, 64).bfloat16(), k_pages=k_pages, v_pages=v_pages, page_table=table,
