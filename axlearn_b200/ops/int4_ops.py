@@ -29,6 +29,7 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from axlearn_b200.ops import cuda_ops, dispatch
 
@@ -68,9 +69,9 @@ def _no_gradient(name: str, *tensors: Optional[Tensor]) -> None:
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise ValueError(f"{name} has no gradient")
-    if cuda_ops._transformed():  # pylint: disable=protected-access
+    if getattr(_forward_ad, "_current_level", 0) >= 0:  # (a name that torch does not promise: without it tangents are looked for)
         for t in tensors:
-            if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
                 raise ValueError(f"{name} has no gradient")
 
 
