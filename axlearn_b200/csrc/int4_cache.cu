@@ -143,9 +143,10 @@ constexpr int kAppendThreads = 256;
 // A unit is the key and the value of kHeads KV heads of one token, or twice as many of its query heads to be rotated: H / 8
 // lanes with 16 bytes of each row.  Units run over heads (KV, then q), tokens, sequences.  The pass is bound by its
 // instructions: where rows go is found once for all of a unit, and nothing is quantised behind `live`.  Measured with the values
-// written out as well, heads of 128 (us; at the copy rate): 64 x 1 tokens, 32 KV heads, 3.2 (0.4), a launch; 8 x 2048 tokens,
-// 8 KV heads, 26.2 (17.5); 30.0 with a head a unit, and 64 with a row a unit, a 64-bit division for each of its indexes and an
-// IEEE division for each level.
+// written out as well, heads of 128 (us; at the copy rate): 64 x 1 tokens, 32 KV heads, 3.2 (0.4), a launch; 8 x up to 2048
+// tokens, 8 KV heads, 26.4 (17.5; issue 71%, ALU 53%); 28.0 with a head a unit, and 64 with a row a unit, a 64-bit division for
+// each of its indexes and an IEEE division for each level.  Prompts with 32 query heads to be rotated beside 8 (32) KV heads, 8 x
+// 2048: 71 (65) and 171 (136).
 template <int H, int kHeads>
 __global__ void __launch_bounds__(kAppendThreads)
 int4_append_kernel(Int4AppendParams p) {
@@ -347,10 +348,11 @@ __device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, bool ok
 // for 32, 47.4 (25.4).  Instructions bind the pass (600 a tile and warp, two thirds of the ALU pipe's unpack codes), not the
 // copies; the first case without the shift of the codes by 8: 125, without arithmetic 97, without
 // copies 106 (issue 59%, ALU 56%, tensor cores 28%), with 96 registers and five CTAs an SM 149, with shifts on the FMA pipe 132.
+// Heads of 128 take all 128 registers that four CTAs an SM leave, and spill 4 to 28 bytes; heads of 64 up to 117.
 //
 // kAppend: a decoding step in one launch.  A warp turns its query heads in registers; the warp whose tile holds the new token
 // turns its key, quantises key and value, stores them in their page slot and puts them into the tile itself, so nobody reads
-// the slot.
+// the slot.  The cases above take 137, 15.6 and 48.4 that way.
 constexpr float kSlack = 8.f;
 
 template <int H, bool kCluster, bool kAppend>
@@ -835,7 +837,7 @@ static int launch_int4_append(Int4AppendParams& p, int64_t tokens, cudaStream_t 
 }
 
 // Two KV heads a unit where units of one would be two waves or more and few units would be half empty (us with one / two: 8 x 2048
-// tokens of 8 heads of 128 43.9 / 38.7, 1 x 2048 7.0 / 7.1, 64 x 1 of 32 2.9 / 3.8).
+// tokens of 8 heads of 128 41.5 / 38.8, 1 x 2048 8.3 / 8.5, 64 x 1 of 32 3.2 / 3.9).
 static int int4_append(Int4AppendParams& p, int B, int T, int page_size, int head_dim, cudaStream_t stream) {
   const int64_t tokens = static_cast<int64_t>(B) * T, rows = tokens * (2 * p.num_kv_heads + p.num_q_heads);
   if (rows >= (int64_t{1} << 31)) return -10;

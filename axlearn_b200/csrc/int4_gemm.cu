@@ -1,8 +1,8 @@
 // y[M, N] = x[M, K] W (+ y) with weights held in 4 bits (layout: int4_linear.cu), on the fifth-generation tensor cores: 128
 // features are the M side of the MMA, up to 128 rows of x its N side; more rows are blocks of 128.
 //
-// Up to eight warps feed: each owns 16 features and turns their codes of 128 rows of W into bf16 values m + s c (one rounding, 2^-9
-// of a weight, as in the expansion for the GEMM of more rows), which `tcgen05.st` puts into tensor memory, so that weights
+// Up to eight warps feed: each owns 16 features and turns their codes of 128 rows of W into bf16 values m + s c (one rounding, up
+// to 2^-8 of a weight, as in the expansion for the GEMM of more rows), which `tcgen05.st` puts into tensor memory, so that weights
 // never pass through shared memory once they are 16 bits wide: writing and reading them there would cost eight times the
 // bytes of the codes.  A 16x256b store takes from lane (r, c) the columns 2c, 2c + 1 of every k16 step, 4 rows of W: the word c of
 // piece (r, s) of a block for step s.  `ldmatrix` hands out words that way, pieces being rows of its matrices, and x keeps its
@@ -19,8 +19,9 @@
 //
 // K slices are the CTAs of a cluster; partial sums meet in distributed shared memory in a fixed order.
 //
-// Launched in the ordinary way in a captured step, too: a successor that started early could hold the tensor memory that a
-// CTA of this kernel has yet to get, and wait for it.
+// Launched in the ordinary way in a captured step, too.  In the chain the wait for the predecessor would have to stand ahead of
+// the allocation of tensor memory and the successor's start behind its release, since kernels that overlap could otherwise hold the
+// tensor memory that each waits for; that has not been built.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

@@ -15,8 +15,10 @@
 //                        denormal bf16 numbers (`int4.cuh`), x is multiplied by 2^kInt4Shift: no code is ever converted.
 //                        Measured (us; the codes at the copy rate): 1 x 2048 x 2048 3.6 (0.3), 1 x 4096 x 28672 16.9 (9.5: copies
 //                        alone take 11.2, arithmetic alone 15.5), 16 x 14336 x 4096 15.0 (4.9), 1 x 16384 x 18944 33.2 (25.2).
-//                        Masks and shifts of the codes keep the ALU pipe busiest (43%, MMAs 31%); more CTAs an SM with fewer
-//                        features each, or with a shorter ring, were not faster: sums of x and loads of x grow as fast.
+//                        No pipe is full (one row: issue 42%, ALU 43%, MMAs 31%; 16 rows, at 182 registers two CTAs an SM: 37%,
+//                        34%, 37%): what bounds it is latency at few warps an SM, and at 28672 columns 448 CTAs on 148 SMs.  More
+//                        CTAs an SM with fewer features each, or with a shorter ring, were not faster: sums of x and loads of x
+//                        grow as fast.
 //   int4_expand_kernel   W in bf16 for the tensor-core GEMM of more rows.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>

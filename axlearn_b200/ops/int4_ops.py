@@ -12,11 +12,11 @@ overflows, stands for NaN.
 * ``prompt_attention_int4``, ``rope_decode_attention_int4``: what a prompt and a decoding step run, with the rotation of
   queries and keys and the append.
 
-Attention sees what the cache stands for, in prompts as in steps.  Serving only: operands that need a gradient, or carry a
-tangent, are refused.  CUDA tensors in bf16 go to the kernels, everything
-else runs the plain statements, which are also the oracle in tests.  Places on the GPU that a page table or a length gets
-wrong (a page that the pool does not have, a position behind the table) are not touched; they set the device's status
-word, which ``cuda_ops.check_status`` raises.  The bf16 forms of these operations are ``cuda_ops.gemm`` and
+Attention sees what the cache stands for: steps ``m + s * c`` itself, prompts that value rounded to bf16 (2^-8 of it at most).
+Serving only: operands that need a gradient, or carry a tangent, are refused.  CUDA tensors in bf16 go to the kernels, everything
+else runs the plain statements, which are also the oracle in tests.  Places that a page table or a length gets wrong (a page that
+the pool does not have, a position behind a table) are not touched: on the GPU they set the device's status word, which
+``cuda_ops.check_status`` raises, on the host they are an ``IndexError``.  The bf16 forms of these operations are ``cuda_ops.gemm`` and
 ``decode_ops``; the reference has no 4-bit form (its quantised layers: axlearn/common/quantized_dot_general/layers.py).
 """
 
@@ -239,8 +239,8 @@ def fused_plan(rows: int, k: int, n: int) -> tuple[int, int]:
 
 def int4_linear(x: Tensor, w: Int4Weight, *, out: Optional[Tensor] = None, accumulate: bool = False) -> Tensor:
     """``x [..., K] @ w`` with fp32 accumulation, rounded to ``x.dtype``; into ``out [..., N]``, or with ``accumulate`` added to
-    it; ``out`` may be ``x`` itself, or overlap it.  Few rows multiply with the 4-bit weights as they are (``multiplies_codes``), more rows with their values rounded to
-    bf16.  Serving only: there is no gradient.  Products keep their digits for x from 2^-57 up to 2^56, weights from 2^-62 and
+    it; ``out`` may be ``x`` itself, or overlap it.  Few rows multiply with the 4-bit weights as they are
+    (``multiplies_codes``), more rows with their values rounded to bf16.  Serving only: there is no gradient.  Products keep their digits for x from 2^-57 up to 2^56, weights from 2^-62 and
     steps below 2^31; sums that overflow fp32 on the way, as with an infinity in x, are NaN."""
     k, n, codes = w.k, w.n, w.codes
     device = x.device
@@ -477,8 +477,9 @@ def paged_decode_attention_int4(q: Tensor, k_pages: Int4Pages, v_pages: Int4Page
                                 softmax_scale: Optional[float] = None, splits: Optional[int] = None,
                                 out: Optional[Tensor] = None, scratch: Optional[Tensor] = None) -> Tensor:
     """q ``[B, Nq, H]``; page_table ``[B, max_pages]``, lengths ``[B]`` int32 (valid tokens per sequence; 0: zeros).  Query heads
-    are grouped by KV head.  ``out`` may be ``q``, or overlap it.  ``scratch``: ``attention_scratch_floats`` fp32 values, for more than eight splits (made a
-    multiple of eight); calls that overlap on the GPU need one each.  Returns ``[B, Nq, H]``."""
+    are grouped by KV head.  ``out`` may be ``q``, or overlap it.  ``scratch``: ``attention_scratch_floats`` fp32 values, for
+    more than eight splits (made a multiple of eight); calls that overlap on the GPU need one each.  Queries from 2^-40 to 2^63 keep their digits, and steps and
+    smallest values in ``v_pages`` up to 2^55 over the number of tokens; sums beyond overflow.  Returns ``[B, Nq, H]``."""
     b, nq, h = q.shape
     device = q.device
     num_pages, nkv, page_size = _check_pages(k_pages, v_pages, page_table, b, nq, h, device)
@@ -535,8 +536,8 @@ def _check_packed(qkv: Tensor, k_pages: Int4Pages, table: Tensor, nq: int) -> tu
     nkv, h = k_pages.codes.shape[1], k_pages.codes.shape[3] * 2
     if qkv.shape[-1] != (nq + 2 * nkv) * h or not qkv.is_contiguous() or qkv.data_ptr() % 16:
         raise ValueError(f"a packed projection of {nq} + 2 x {nkv} heads of {h} is contiguous and 16-byte aligned: {tuple(qkv.shape)}")
-    if (table.dtype != torch.float32 or table.shape[1:] != (h // 2, 2) or not len(table) or not table.is_contiguous() or table.device != qkv.device
-            or table.data_ptr() % 16):
+    if (table.dtype != torch.float32 or table.shape[1:] != (h // 2, 2) or not len(table) or not table.is_contiguous()
+            or table.device != qkv.device or table.data_ptr() % 16):
         raise ValueError(f"a rotation table is [positions, {h // 2}, 2] fp32 on {qkv.device}: {tuple(table.shape)} {table.dtype}")
     return nkv, h
 
@@ -575,7 +576,7 @@ def prompt_attention_int4(qkv: Tensor, k_pages: Int4Pages, v_pages: Int4Pages, p
                           num_q_heads: int, softmax_scale: float) -> Tensor:
     """Whole prompts from position 0: ``qkv [B, T, (Nq + 2 Nkv) * H]`` of one projection.  Rotates queries and keys by ``table``,
     appends keys and values to the cache and runs causal attention over what the cache then stands for: in ``qkv`` queries
-    are replaced by rotated ones, keys and values by the cache's.  Returns ``[B, T, Nq * H]``."""
+    are replaced by rotated ones, keys and values by the cache's, rounded to ``qkv``'s type.  Returns ``[B, T, Nq * H]``."""
     nkv, h = _check_packed(qkv, k_pages, table, num_q_heads)
     b, t, width = qkv.shape
     device = qkv.device

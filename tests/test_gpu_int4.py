@@ -884,3 +884,21 @@ def test_a_step_with_exact_rotations(nq, kv, dim, splits, page_size):
     without, _ = _attention64(q, k_pages, v_pages, table, lengths - 1, dim ** -0.5)
     first = slice(None, None, nq // kv)
     assert (((want - without).abs() > 8 * bound)[:, first].float().mean((1, 2)) > 0.8).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_up_to_the_ranges_of_its_documentation(dim):
+    """Queries up to 2^63, steps and smallest values up to 2^55 over the number of tokens: powers of two leave every digit."""
+    from axlearn_b200.ops import int4_ops
+
+    k_pages, v_pages, table = _cache(2, 20, 16, 2, dim, seed=45)
+    lengths = torch.tensor([320, 77], dtype=torch.int32, device="cuda")
+    q = _normal(_gen(46), 2, 8, dim).bfloat16()
+    q_scale = 2.0 ** (62 - math.ceil(math.log2(q.abs().max().item())))
+    v_scale = 2.0 ** (54 - math.ceil(math.log2(320 * v_pages.scales.abs().max().item())))
+    plain = int4_ops.paged_decode_attention_int4(q, k_pages, v_pages, table, lengths)
+    k_pages, v_pages = k_pages._replace(scales=k_pages.scales / q_scale), v_pages._replace(scales=v_pages.scales * v_scale)
+    for splits in (1, 4, 16):
+        out = int4_ops.paged_decode_attention_int4(q * q_scale, k_pages, v_pages, table, lengths, splits=splits)
+        assert out.isfinite().all()
+    assert torch.equal(int4_ops.paged_decode_attention_int4(q * q_scale, k_pages, v_pages, table, lengths), plain * v_scale)
