@@ -28,6 +28,7 @@ NVCC_FLAGS = [
 # Everything but these is built with --use_fast_math: their fp32 instantiations are held to fp32
 # accuracy (recurrent decays, norms and softmax of the 32-bit inference mode).
 PRECISE_SOURCES = frozenset({"experts.cu", "gated_act.cu", "gla.cu", "hyper.cu", "int4_cache.cu", "int4_gemm.cu", "int4_linear.cu",
+                             "int8_cache.cu", "int8_gemm.cu", "int8_rows.cu",
                              "latent_attn.cu", "skinny_group.cu", "ssd.cu", "window_attn.cu"})
 
 

@@ -35,12 +35,13 @@
 #include "chain.cuh"
 #include "cluster.cuh"
 #include "host_utils.cuh"
+#include "opt_in.cuh"
 #include "sm100.cuh"
 
 namespace axb {
 
 constexpr int kSkTile = 128;  // features of one MMA
-constexpr int kSkK = 64;
+constexpr int kSkRow = 128;  // bytes of a k-block in a row of either operand: 64 bf16 or 128 8-bit values
 constexpr int kSkThreads = 192;
 constexpr int kSkMaxSplit = 8;  // portable cluster size
 
@@ -54,8 +55,8 @@ template <int BN, SkinnyLayout LAYOUT>
 struct SkinnyCfg {
   static constexpr int kTiles = LAYOUT == kWide ? 2 : 1;
   static constexpr int kFeatures = kTiles * kSkTile;
-  static constexpr int kWBytes = kFeatures * kSkK * 2;
-  static constexpr int kXBytes = BN * kSkK * 2;
+  static constexpr int kWBytes = kFeatures * kSkRow;
+  static constexpr int kXBytes = BN * kSkRow;
   static constexpr int kBlockBytes = kWBytes + kXBytes;
   static constexpr int kBlocks = (LAYOUT == kPair ? 110 * 1024 : 200 * 1024) / kBlockBytes;
   // A stage, the unit of waits and commits, is one or two k-blocks.
@@ -82,6 +83,33 @@ struct SkinnyGemmParams {
   int accumulate;
   int split;
   int w_resident;  // in a chained launch: nothing that runs just before this kernel writes W
+  const float *x_scales, *w_scales;  // 8-bit operands: of the rows of X and of the features
+};
+
+// Operands in 8 bits (`int8_t`) are products of whole numbers in 32-bit integers, exact in any order; a sum counts times the
+// scale of its row and of its feature.  Everything up to there moves the same bytes as bf16 operands of half the K.
+template <typename In>
+struct SkinnyIn {
+  static constexpr bool kWhole = sizeof(In) == 1;
+  static constexpr int kK = kSkRow / static_cast<int>(sizeof(In));  // values of a k-block
+  static constexpr CUtensorMapDataType kType = kWhole ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+
+  static __device__ __forceinline__ constexpr uint32_t idesc(int n, int w_mn, int x_mn) {
+    return kWhole ? umma_idesc_i8(kSkTile, n) : umma_idesc_f16(kSkTile, n, 1, 1, w_mn, x_mn);
+  }
+  static __device__ __forceinline__ void mma(uint32_t d, uint64_t w, uint64_t x, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (kWhole) tc_mma_i8(d, w, x, idesc, accumulate);
+    else tc_mma_f16(d, w, x, idesc, accumulate);
+  }
+  // Bits of a partial sum that stand for zero in both forms; the sum of two.
+  static __device__ __forceinline__ float add(float a, float b) {
+    if constexpr (kWhole) return __int_as_float(__float_as_int(a) + __float_as_int(b));
+    else return a + b;
+  }
+  static __device__ __forceinline__ float value(float sum, float x_scale, float w_scale) {
+    if constexpr (kWhole) return __int2float_rn(__float_as_int(sum)) * x_scale * w_scale;
+    else return sum;
+  }
 };
 
 template <typename OutT>
@@ -102,12 +130,14 @@ __device__ __forceinline__ float ld_shared_f32(uint32_t addr) {
   return v;
 }
 
-template <int BN, SkinnyLayout LAYOUT, bool X_MN, bool W_MN, typename OutT>
+template <int BN, SkinnyLayout LAYOUT, bool X_MN, bool W_MN, typename OutT, typename In>
 __global__ void __launch_bounds__(kSkThreads, LAYOUT == kPair ? 2 : 1)
 gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                    SkinnyGemmParams p) {
   using S = SkinnyCfg<BN, LAYOUT>;
-  constexpr int kGroup = S::kGroup;
+  using I = SkinnyIn<In>;
+  static_assert(!I::kWhole || (!X_MN && !W_MN), "8-bit operands are read along K");
+  constexpr int kGroup = S::kGroup, kSkK = I::kK;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem =
       reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -169,7 +199,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
           if constexpr (!W_MN) {
 #pragma unroll
             for (int t = 0; t < S::kTiles; ++t)
-              tma_load_2d(sw + t * (kSkTile * kSkK * 2), &tmap_w, &full_bar[stage], k0, n0 + t * kSkTile);
+              tma_load_2d(sw + t * (kSkTile * kSkRow), &tmap_w, &full_bar[stage], k0, n0 + t * kSkTile);
           } else {
             // (A box that starts beyond the last feature reads the fill value like any other out-of-range column.)
 #pragma unroll
@@ -211,7 +241,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   } else if (warp == 1) {
     if (elect_one()) {
       chain_wait();
-      constexpr uint32_t idesc = umma_idesc_f16(kSkTile, BN, 1, 1, W_MN ? 1 : 0, X_MN ? 1 : 0);
+      constexpr uint32_t idesc = I::idesc(BN, W_MN ? 1 : 0, X_MN ? 1 : 0);
       int stage = 0;
       uint32_t phase = 0;
       bool fed = true;
@@ -227,15 +257,15 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
           const uint32_t sw = smem_u32(smem + (stage * kGroup + j) * S::kBlockBytes);
           const uint32_t sx = sw + S::kWBytes;
 #pragma unroll
-          for (int k = 0; k < kSkK / 16; ++k) {
+          for (int k = 0; k < kSkRow / 32; ++k) {
             const uint64_t dx =
                 X_MN ? umma_smem_desc(sx + k * 2048, 8192, 1024) : umma_smem_desc(sx + k * 32, 16, 1024);
 #pragma unroll
             for (int t = 0; t < S::kTiles; ++t) {
-              const uint32_t st = sw + t * (kSkTile * kSkK * 2);
+              const uint32_t st = sw + t * (kSkTile * kSkRow);
               const uint64_t dw =
                   W_MN ? umma_smem_desc(st + k * 2048, 8192, 1024) : umma_smem_desc(st + k * 32, 16, 1024);
-              tc_mma_f16(tmem + t * BN, dw, dx, idesc, (kb + j > kb_lo || k > 0) ? 1u : 0u);
+              I::mma(tmem + t * BN, dw, dx, idesc, (kb + j > kb_lo || k > 0) ? 1u : 0u);
             }
           }
         }
@@ -270,6 +300,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     for (int t = 0; t < S::kTiles; ++t) {
       const uint32_t taddr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + t * BN;
       const bool stores = n0 + t * kSkTile + feature < p.N;
+      const float w_scale = I::kWhole && stores ? p.w_scales[n0 + t * kSkTile + feature] : 0.f;
 #pragma unroll 1
       for (int c = 0; c < BN; c += 16) {
         if (c >= p.M) break;
@@ -292,7 +323,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             if (c + j >= p.M) break;
-            float v = __uint_as_float(r[j]);
+            float v = I::value(__uint_as_float(r[j]), I::kWhole ? p.x_scales[c + j] : 0.f, w_scale);
             if (p.accumulate) v += kEarlyC > 1 ? before[j] : skinny_read(dst + j * p.ldc);
             skinny_write(dst + j * p.ldc, v);
           }
@@ -303,6 +334,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   if (splits) {
     cluster_sync_all();
     if (warp >= 2 && ok && n0 + feature < p.N) {
+      const float w_scale = I::kWhole ? p.w_scales[n0 + feature] : 0.f;
       auto finish = [&](int i, int row, float old) {
         float v[kSkMaxSplit];
 #pragma unroll
@@ -313,7 +345,8 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
         }
         float sum = v[0];
 #pragma unroll
-        for (int s = 1; s < kSkMaxSplit; ++s) sum += v[s];
+        for (int s = 1; s < kSkMaxSplit; ++s) sum = I::add(sum, v[s]);
+        sum = I::value(sum, I::kWhole ? p.x_scales[row] : 0.f, w_scale);
         skinny_write(out + static_cast<int64_t>(row) * p.ldc, p.accumulate ? sum + old : sum);
       };
       if constexpr (kEarlyC > 1) {
@@ -365,15 +398,14 @@ static int resident_ctas(Kernel kernel, int smem, int split, std::atomic<int>* c
   return clusters * split;
 }
 
-template <int BN, SkinnyLayout LAYOUT, bool X_MN, bool W_MN, typename OutT>
+template <int BN, SkinnyLayout LAYOUT, bool X_MN, bool W_MN, typename OutT, typename In>
 struct SkinnyKernel {
   using S = SkinnyCfg<BN, LAYOUT>;
-  static constexpr auto kernel = gemm_skinny_kernel<BN, LAYOUT, X_MN, W_MN, OutT>;
+  static constexpr auto kernel = gemm_skinny_kernel<BN, LAYOUT, X_MN, W_MN, OutT, In>;
 
   static bool configure() {
-    static const cudaError_t e =
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-    return e == cudaSuccess;
+    static OptIn opt_in;
+    return opt_in.done(kernel, S::kSmem);
   }
 
   // Expected time in us of N features cut into `split` slices of `num_kb` k-blocks: what a k-block takes at the slowest
@@ -420,12 +452,13 @@ struct SkinnyKernel {
 };
 
 // The cheapest layout and split; `forced` split (0 = free).
-template <int BN, bool X_MN, bool W_MN, typename OutT>
+template <int BN, bool X_MN, bool W_MN, typename OutT, typename In = __nv_bfloat16>
 static bool skinny_plan(int N, int K, int forced, int* split, SkinnyLayout* layout) {
-  using Pair = SkinnyKernel<BN, kPair, X_MN, W_MN, OutT>;
-  using Deep = SkinnyKernel<BN, kDeep, X_MN, W_MN, OutT>;
-  using Wide = SkinnyKernel<BN, kWide, X_MN, W_MN, OutT>;
+  using Pair = SkinnyKernel<BN, kPair, X_MN, W_MN, OutT, In>;
+  using Deep = SkinnyKernel<BN, kDeep, X_MN, W_MN, OutT, In>;
+  using Wide = SkinnyKernel<BN, kWide, X_MN, W_MN, OutT, In>;
   if (!Deep::configure() || !Pair::configure() || !Wide::configure()) return false;
+  constexpr int kSkK = SkinnyIn<In>::kK;
   const int num_kb = (K + kSkK - 1) / kSkK;
   float best = 0.f;
   *split = 0;
@@ -444,29 +477,30 @@ static bool skinny_plan(int N, int K, int forced, int* split, SkinnyLayout* layo
   return *split > 0;
 }
 
-template <int BN, bool X_MN, bool W_MN, typename OutT>
+template <int BN, bool X_MN, bool W_MN, typename OutT, typename In = __nv_bfloat16>
 static int launch_skinny(const void* X, const void* W, int64_t ldx, int64_t ldw, SkinnyGemmParams p,
                          cudaStream_t stream) {
   SkinnyLayout layout = kPair;
-  if (!skinny_plan<BN, X_MN, W_MN, OutT>(p.N, p.K, p.split, &p.split, &layout)) return -15;
+  if (!skinny_plan<BN, X_MN, W_MN, OutT, In>(p.N, p.K, p.split, &p.split, &layout)) return -15;
   CUtensorMap tw, tx;
+  constexpr int kSkK = SkinnyIn<In>::kK;
   const uint64_t k = static_cast<uint64_t>(p.K), n = static_cast<uint64_t>(p.N), m = static_cast<uint64_t>(p.M);
   const uint64_t wdims[2] = {W_MN ? n : k, W_MN ? k : n};
-  const uint64_t wstride[1] = {static_cast<uint64_t>(ldw) * 2};
-  const uint32_t wbox[2] = {64, static_cast<uint32_t>(W_MN ? kSkK : kSkTile)};
-  int rc = make_tensor_map(&tw, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, W, wdims, wstride, wbox,
+  const uint64_t wstride[1] = {static_cast<uint64_t>(ldw) * sizeof(In)};
+  const uint32_t wbox[2] = {W_MN ? 64 : kSkK, static_cast<uint32_t>(W_MN ? kSkK : kSkTile)};
+  int rc = make_tensor_map(&tw, SkinnyIn<In>::kType, 2, W, wdims, wstride, wbox,
                            CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc != 0) return rc;
   static_assert(!X_MN || BN >= 64, "an M-major tile of X is at least one 128-byte row wide");
   const uint64_t xdims[2] = {X_MN ? m : k, X_MN ? k : m};
-  const uint64_t xstride[1] = {static_cast<uint64_t>(ldx) * 2};
-  const uint32_t xbox[2] = {64, X_MN ? static_cast<uint32_t>(kSkK) : static_cast<uint32_t>(BN)};
-  rc = make_tensor_map(&tx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, X, xdims, xstride, xbox, CU_TENSOR_MAP_SWIZZLE_128B);
+  const uint64_t xstride[1] = {static_cast<uint64_t>(ldx) * sizeof(In)};
+  const uint32_t xbox[2] = {X_MN ? 64 : kSkK, X_MN ? static_cast<uint32_t>(kSkK) : static_cast<uint32_t>(BN)};
+  rc = make_tensor_map(&tx, SkinnyIn<In>::kType, 2, X, xdims, xstride, xbox, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc != 0) return rc;
   switch (layout) {
-    case kDeep: return SkinnyKernel<BN, kDeep, X_MN, W_MN, OutT>::launch(tw, tx, p, stream);
-    case kWide: return SkinnyKernel<BN, kWide, X_MN, W_MN, OutT>::launch(tw, tx, p, stream);
-    default: return SkinnyKernel<BN, kPair, X_MN, W_MN, OutT>::launch(tw, tx, p, stream);
+    case kDeep: return SkinnyKernel<BN, kDeep, X_MN, W_MN, OutT, In>::launch(tw, tx, p, stream);
+    case kWide: return SkinnyKernel<BN, kWide, X_MN, W_MN, OutT, In>::launch(tw, tx, p, stream);
+    default: return SkinnyKernel<BN, kPair, X_MN, W_MN, OutT, In>::launch(tw, tx, p, stream);
   }
 }
 
@@ -511,8 +545,8 @@ extern "C" int axb_gemm_skinny(const void* X, const void* W, void* C, int M, int
   if ((ldx % 8) || (ldw % 8) || (reinterpret_cast<uintptr_t>(X) & 15) || (reinterpret_cast<uintptr_t>(W) & 15) ||
       (reinterpret_cast<uintptr_t>(C) & 15) || (ldc % (out_fp32 ? 4 : 8)))
     return -10;
-  if (split < 0 || split > kSkMaxSplit || split > (K + kSkK - 1) / kSkK) return -15;
-  const SkinnyGemmParams p{M, N, K, C, ldc, status, accumulate, split, w_resident && chain_launches ? 1 : 0};
+  if (split < 0 || split > kSkMaxSplit || split > (K + SkinnyIn<__nv_bfloat16>::kK - 1) / SkinnyIn<__nv_bfloat16>::kK) return -15;
+  const SkinnyGemmParams p{M, N, K, C, ldc, status, accumulate, split, w_resident && chain_launches ? 1 : 0, nullptr, nullptr};
 #define AXB_SKINNY_BN(BN, XM, WM, T) return launch_skinny<BN, XM, WM, T>(X, W, ldx, ldw, p, stream)
 #define AXB_SKINNY(WM, T)                                  \
   do {                                                     \
@@ -531,4 +565,23 @@ extern "C" int axb_gemm_skinny(const void* X, const void* W, void* C, int M, int
   AXB_SKINNY(false, __nv_bfloat16);
 #undef AXB_SKINNY
 #undef AXB_SKINNY_BN
+}
+
+// C[M, N] (bf16, row pitch ldc) = x_scales[m] w_scales[n] sum_k X[m, k] W[n, k] (+ C when accumulate) of 8-bit whole numbers, X
+// [M, K] and W [N, K] along K with pitches ldx and ldw that are multiples of 16, M <= 128.  `split`, `w_resident` as above.
+extern "C" int axb_gemm_skinny_int8(const void* X, const float* x_scales, const void* W, const float* w_scales, void* C, int M, int N,
+                                    int K, int64_t ldx, int64_t ldw, int64_t ldc, int accumulate, int split, int w_resident,
+                                    int* status, cudaStream_t stream) {
+  using namespace axb;
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (M > 128) return -20;
+  if ((ldx % 16) || (ldw % 16) || (reinterpret_cast<uintptr_t>(X) & 15) || (reinterpret_cast<uintptr_t>(W) & 15) ||
+      (reinterpret_cast<uintptr_t>(C) & 1))
+    return -10;
+  if (split < 0 || split > kSkMaxSplit || split > (K + SkinnyIn<int8_t>::kK - 1) / SkinnyIn<int8_t>::kK) return -15;
+  const SkinnyGemmParams p{M, N, K, C, ldc, status, accumulate, split, w_resident && chain_launches ? 1 : 0, x_scales, w_scales};
+  if (M <= 16) return launch_skinny<16, false, false, __nv_bfloat16, int8_t>(X, W, ldx, ldw, p, stream);
+  if (M <= 32) return launch_skinny<32, false, false, __nv_bfloat16, int8_t>(X, W, ldx, ldw, p, stream);
+  if (M <= 64) return launch_skinny<64, false, false, __nv_bfloat16, int8_t>(X, W, ldx, ldw, p, stream);
+  return launch_skinny<128, false, false, __nv_bfloat16, int8_t>(X, W, ldx, ldw, p, stream);
 }

@@ -1,0 +1,778 @@
+// A paged KV cache held in 8 bits (`int8.cuh`): new tokens are quantised into it, and one new token a sequence attends to it.
+//
+// Pools: codes [pages, Nkv, page_size, H], largest magnitudes [pages, Nkv] in bf16, for K and for V: the tokens of a page of one
+// KV head are a block, and one run of memory; page table [B, max_pages], H 64 or 128, page_size a multiple of 16.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <float.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "cache_rows.cuh"
+#include "chain.cuh"
+#include "cluster.cuh"
+#include "host_utils.cuh"
+#include "int8.cuh"
+#include "mma_sync.cuh"
+#include "opt_in.cuh"
+#include "sm100.cuh"
+
+namespace axb {
+
+struct Int8Pool {
+  uint8_t* codes;
+  __nv_bfloat16* tops;
+};
+
+struct Int8AppendParams {
+  HeadRows q, k, v;
+  __nv_bfloat16 *q_out, *k_out, *v_out;  // where the rotated q and the values of k and v go; null: not wanted
+  int64_t q_out_b, q_out_t, out_b, out_t, out_h;
+  Int8Pool k_pool, v_pool;
+  const int* page_table;
+  const int* start;     // null: 0
+  const int* live;      // null: all tokens
+  const int* lengths;   // a decoding step: its token is at lengths - 1, and not there where that is behind `limit`
+  const float2* angle;  // (sin, cos) of [position][H / 2]; null: nothing is rotated
+  int* status;
+  FastDiv heads, blocks, page, q_units, tokens;  // units of a block, blocks of a sequence, positions of a page, ...
+  uint32_t kv_units, all_units;
+  int T, limit, num_q_heads, num_kv_heads, max_pages, num_pages;
+};
+
+constexpr int kInt8AppendThreads = 256;
+constexpr int kInt8Held = 8;  // rows that a thread keeps
+constexpr int kInt8QRows = 4;
+
+// A unit is what a call brings for one block: up to a page's tokens of the keys, or the values, of a KV head.  Its kWarps warps
+// hold them in registers while the largest magnitude is found (further rows are read again), and turn the codes that are
+// there already, if the magnitude has grown.  Units behind those rotate kInt8QRows times kRows query heads of a token.
+template <int H, int kWarps>
+__global__ void __launch_bounds__(kInt8AppendThreads)
+int8_append_kernel(Int8AppendParams p) {
+  chain_link();
+  constexpr int kLanes = H / 8, kThreads = 32 * kWarps, kRows = kThreads / kLanes, kUnits = kInt8AppendThreads / kThreads;
+  __shared__ uint32_t s_top[kInt8AppendThreads / 32];
+  const int in = threadIdx.x % kThreads, place = threadIdx.x / kThreads;
+  const int l8 = in % kLanes, row_at = in / kLanes;
+  uint32_t unit = blockIdx.x * kUnits + place;
+  if (unit >= p.all_units) return;
+  const uint4 zeros = make_uint4(0, 0, 0, 0);
+  const bool is_q = unit >= p.kv_units;
+  if (is_q) unit -= p.kv_units;
+  const uint32_t outer = is_q ? p.q_units.div(unit) : p.heads.div(unit);
+  const uint32_t inner = unit - outer * (is_q ? p.q_units.d : p.heads.d);
+  const int b = static_cast<int>(is_q ? p.tokens.div(outer) : p.blocks.div(outer));
+  int begin = p.start == nullptr ? 0 : p.start[b];
+  int count = p.live == nullptr ? p.T : min(max(p.live[b], 0), p.T);
+  if (p.lengths != nullptr) {
+    begin = p.lengths[b] - 1;
+    count = begin >= 0 && begin < p.limit ? 1 : 0;
+  }
+  if (is_q) {
+    const int t = static_cast<int>(outer) - b * p.T;
+    if (p.lengths != nullptr && count == 0) return;
+    const float2* angle = p.angle + (static_cast<int64_t>(begin) + t) * (H / 2) + l8 * 4;
+    const int head = static_cast<int>(inner) * kInt8QRows * kRows + row_at;
+    const __nv_bfloat16* src = p.q.x + b * p.q.b + t * p.q.t + head * p.q.h + l8 * 8;
+    __nv_bfloat16* dst = p.q_out + b * p.q_out_b + t * p.q_out_t + head * H + l8 * 8;
+    uint4 x[kInt8QRows];
+#pragma unroll
+    for (int i = 0; i < kInt8QRows; ++i)
+      x[i] = head + i * kRows < p.num_q_heads ? *reinterpret_cast<const uint4*>(src + i * kRows * p.q.h) : zeros;
+#pragma unroll
+    for (int i = 0; i < kInt8QRows; ++i)
+      if (head + i * kRows < p.num_q_heads) *reinterpret_cast<uint4*>(dst + i * kRows * H) = rotate8(x[i], angle);
+    return;
+  }
+  const int j = static_cast<int>(outer) - b * static_cast<int>(p.blocks.d);
+  const bool is_v = inner >= static_cast<uint32_t>(p.num_kv_heads);
+  const int head = static_cast<int>(inner) - (is_v ? p.num_kv_heads : 0);
+  const int page_size = static_cast<int>(p.page.d);
+  const uint32_t at0 = static_cast<uint32_t>(max(begin, 0)), col0 = p.page.div(at0);
+  const int row0 = j == 0 ? static_cast<int>(at0 - col0 * p.page.d) : 0;
+  const int64_t first = j == 0 ? 0 : static_cast<int64_t>(j) * page_size - (at0 - col0 * p.page.d);
+  if (first >= p.T) return;
+  const int t0 = static_cast<int>(first), t1 = min(p.T - t0, page_size - row0) + t0, rows = min(t1, count) - t0;
+  __nv_bfloat16* out = is_v ? p.v_out : p.k_out;
+  if (out != nullptr) {
+    out += b * p.out_b + t0 * p.out_t + head * p.out_h + l8 * 8;
+    for (int r = max(rows, 0) + row_at; r < t1 - t0; r += kRows) *reinterpret_cast<uint4*>(out + r * p.out_t) = zeros;
+  }
+  if (rows <= 0) return;
+  const HeadRows& source = is_v ? p.v : p.k;
+  const __nv_bfloat16* src = source.x + b * source.b + t0 * source.t + head * source.h + l8 * 8;
+  const float2* angle = is_v || p.angle == nullptr
+                            ? nullptr : p.angle + (static_cast<int64_t>(begin) + t0) * (H / 2) + l8 * 4;
+  auto load = [&](int r) {
+    const uint4 x = *reinterpret_cast<const uint4*>(src + r * source.t);
+    return angle == nullptr ? x : rotate8(x, angle + static_cast<int64_t>(r) * (H / 2));
+  };
+  auto largest = [](uint32_t m, const uint4& x) {  // of both halves; NaN is the largest of all
+    m = __vmaxu2(m, __vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu));
+    return __vmaxu2(m, __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
+  };
+  uint4 x[kInt8Held];
+#pragma unroll
+  for (int i = 0; i < kInt8Held; ++i) x[i] = row_at + i * kRows < rows ? load(row_at + i * kRows) : zeros;
+  // The place: a sequence that starts ahead of its first position has none.
+  const Int8Pool& pool = is_v ? p.v_pool : p.k_pool;
+  const int64_t col = static_cast<int64_t>(col0) + j;
+  uint32_t page = 0xffffffffu;
+  if (begin >= 0 && col < p.max_pages) page = static_cast<uint32_t>(p.page_table[static_cast<int64_t>(b) * p.max_pages + col]);
+  const bool placed = page < static_cast<uint32_t>(p.num_pages);
+  if (!placed) int8_report(p.status);
+  const int64_t block = placed ? static_cast<int64_t>(page) * p.num_kv_heads + head : 0;
+  const uint32_t old = placed && row0 > 0
+                           ? static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(pool.tops + block) & 0x7fff) << 16 : 0u;
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < kInt8Held; ++i) m = largest(m, x[i]);
+  for (int r = row_at + kInt8Held * kRows; r < rows; r += kRows) m = largest(m, load(r));
+  m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
+  if constexpr (kWarps > 1) {
+    if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = m;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + place), "r"(kThreads) : "memory");
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) m = max(m, s_top[place * kWarps + w]);
+  }
+  const float top = __uint_as_float(max(m << 16, old));
+  const Int8Scale<> s(top);
+  uint8_t* codes = pool.codes + (block * page_size + row0) * H + l8 * 8;
+  if (placed) {
+    if (in == 0) pool.tops[block] = __float2bfloat16(s.top);
+    if (row0 > 0 && __float_as_uint(s.top) != old && !s.empty()) {
+      const Int8Scale<1> turn(top);
+      const float by = __uint_as_float(old);
+      for (int r = row_at; r < row0; r += kRows) {
+        uint2* at = reinterpret_cast<uint2*>(codes + static_cast<int64_t>(r - row0) * H);
+        const uint2 was = *at;
+        float f[8], level[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          f[i] = by * static_cast<float>(static_cast<int8_t>((i < 4 ? was.x : was.y) >> (8 * (i & 3))));
+        int8_levels(f, turn, level);
+        *at = int8_pack(level);
+      }
+    }
+  }
+  const float back = s.top * (1.f / 127.f);
+  auto hold = [&](int r, const uint4& v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    float f[8], level[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 two = unpack2(w[i]);
+      f[2 * i] = two.x, f[2 * i + 1] = two.y;
+    }
+    int8_levels(f, s, level);
+    if (placed) *reinterpret_cast<uint2*>(codes + static_cast<int64_t>(r) * H) = int8_pack(level);
+    if (out != nullptr)
+      *reinterpret_cast<uint4*>(out + r * p.out_t) =
+          make_uint4(pack2(level[0] * back, level[1] * back), pack2(level[2] * back, level[3] * back),
+                     pack2(level[4] * back, level[5] * back), pack2(level[6] * back, level[7] * back));
+  };
+#pragma unroll
+  for (int i = 0; i < kInt8Held; ++i)
+    if (row_at + i * kRows < rows) hold(row_at + i * kRows, x[i]);
+  for (int r = row_at + kInt8Held * kRows; r < rows; r += kRows) hold(r, load(r));
+}
+
+template <int H, int kWarps>
+static int launch_int8_append(Int8AppendParams& p, int64_t sequences, int q_heads, cudaStream_t stream) {
+  constexpr int kRows = 32 * kWarps / (H / 8), kUnits = kInt8AppendThreads / (32 * kWarps);
+  const int q_units = (q_heads + kRows * kInt8QRows - 1) / (kRows * kInt8QRows);
+  const int64_t kv = sequences * p.blocks.d * 2 * p.num_kv_heads, all = kv + sequences * p.T * q_units;
+  if (all >= (int64_t{1} << 31)) return -10;
+  p.heads = FastDiv(2 * p.num_kv_heads), p.tokens = FastDiv(p.T);
+  p.q_units = FastDiv(q_units > 0 ? q_units : 1);
+  p.kv_units = static_cast<uint32_t>(kv), p.all_units = static_cast<uint32_t>(all);
+  launch_chained(int8_append_kernel<H, kWarps>, static_cast<unsigned>((all + kUnits - 1) / kUnits), kInt8AppendThreads, 0, stream, p);
+  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+}
+
+static int int8_append(Int8AppendParams& p, int B, int page_size, int head_dim, cudaStream_t stream) {
+  p.page = FastDiv(page_size);
+  p.blocks = FastDiv(p.start == nullptr ? (p.T + page_size - 1) / page_size : (p.T - 1 + page_size - 1) / page_size + 1);
+  // Warps of a unit: one as long as they hold its rows.
+  const int rows = p.T < page_size ? p.T : page_size, held = kInt8Held * 32 / (head_dim / 8);
+  const bool four = rows > held;
+  if (head_dim == 128)
+    return four ? launch_int8_append<128, 4>(p, B, p.num_q_heads, stream) : launch_int8_append<128, 1>(p, B, p.num_q_heads, stream);
+  return four ? launch_int8_append<64, 4>(p, B, p.num_q_heads, stream) : launch_int8_append<64, 1>(p, B, p.num_q_heads, stream);
+}
+
+struct Int8AttnParams {
+  const __nv_bfloat16* q;  // [B, Nq, H]
+  const __nv_bfloat16 *k_tops, *v_tops;
+  const int* page_table;
+  const int* lengths;
+  float* part_out;         // [B, Nq, splits / 8, H]: of each cluster, where there are several
+  float* part_ml;          // [B, Nq, splits / 8, 2]
+  __nv_bfloat16* out;
+  int* status;
+  FastDiv page;
+  int num_q_heads, num_kv_heads, max_pages, num_pages, splits;
+  int limit;               // a decoding step: longer sequences than this had no place or rotation and get zeros; else -1
+  float scale_log2;        // softmax scale * log2(e) / 127 * 2^kInt8Back, > 0
+};
+
+constexpr int kI8AttnThreads = 128, kI8AttnWarps = kI8AttnThreads / 32;
+constexpr int kI8AttnRows = 8;   // query heads of a CTA: the columns of both products
+constexpr int kI8Chunk = 16;     // keys of an MMA, of one page
+constexpr int kI8AttnKeys = 2 * kI8Chunk;
+constexpr int kI8AttnStages = 2;
+constexpr int kI8AttnCluster = 8;
+constexpr float kI8Slack = 8.f;
+
+// Codes as operands: c + 128, a byte in the low half of a bf16 lane, is the number (c + 128) 2^-133 as it lies (a denormal, then
+// the first binade of the same spacing).  The other operand carries 2^64, so that products stay in fp32's range.
+constexpr float kInt8Up = 0x1p64f, kInt8Back = 0x1p69f;
+
+__device__ __forceinline__ uint32_t int8_even(uint32_t x) { return (x & 0x00ff00ffu) ^ 0x00800080u; }
+__device__ __forceinline__ uint32_t int8_odd(uint32_t x) { return ((x >> 8) & 0x00ff00ffu) ^ 0x00800080u; }
+
+__device__ __forceinline__ uint32_t int8_turned_round(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <int H>
+struct Int8Tile {
+  static constexpr int kChunk = kI8Chunk * H, kBytes = 4 * kChunk;  // two chunks of K, two of V
+  static constexpr int kSmem(int rows) {
+    const int merge = (kI8AttnWarps + 1) * rows * (H + 2) * 4, tiles = kI8AttnWarps * kI8AttnStages * kBytes;
+    return (merge > tiles ? merge : tiles) + 1024;  // alignment slack
+  }
+  // 16-byte unit u of a chunk's row, as TMA swizzles it: eight lanes of both products hit all banks.
+  __device__ static int unit(int row, int u) {
+    if constexpr (H == 128) return row * 128 + ((u ^ (row & 7)) << 4);
+    return row * 64 + ((u ^ ((row >> 1) & 3)) << 4);
+  }
+};
+
+// S^T = K Q^T: 16 keys are the rows of the m16n8k16 tile, the query heads its columns; a lane takes H / 4 neighbouring dims of a
+// key, so that a word of four codes is two operand registers.  O^T = V^T P^T: 16 dims are the rows, P is turned round by
+// `movmatrix`.  A chunk of 16 keys is of one page, so A / 127 of K multiplies its scores, and that of V its products in fp32;
+// codes enter as c + 128, and 128 times the sums of q and of P leave again.  P is rounded to bf16 once and normalised by the
+// sum of what it was rounded to.  The maximum that P is relative to moves only when a score passes it by kI8Slack.
+//
+// A tile is 32 keys, a warp's own from TMA to its sums: no barrier of the CTA before the end.  Tiles go round the warps of all
+// splits, splits of eight or less are a cluster whose parts meet in distributed shared memory, more are clusters whose parts a
+// second launch joins.
+template <int H, bool kCluster>
+__global__ void __launch_bounds__(kI8AttnThreads, 3)
+int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Int8AttnParams p) {
+  chain_link();
+  using Tile = Int8Tile<H>;
+  constexpr int kSteps = H / 16;  // MMAs of a chunk in either product
+  extern __shared__ uint8_t s_raw[];
+  __shared__ __align__(8) uint64_t s_full[kI8AttnWarps][kI8AttnStages];
+  uint8_t* s_ring = s_raw + (((smem_u32(s_raw) + 1023u) & ~1023u) - smem_u32(s_raw));
+  const int split = blockIdx.x;
+  const int group = p.num_q_heads / p.num_kv_heads;
+  const int parts = (group + kI8AttnRows - 1) / kI8AttnRows;
+  const int kvh = blockIdx.y / parts;
+  const int first = blockIdx.y % parts * kI8AttnRows;
+  const int rows = min(kI8AttnRows, group - first);
+  const int qh0 = kvh * group + first;
+  const int b = blockIdx.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = lane >> 2, c = lane & 3;
+  const int page_size = static_cast<int>(p.page.d);
+  int len = p.lengths[b];
+  const int64_t capacity = p.max_pages * static_cast<int64_t>(page_size);
+  if (len > capacity || (p.limit >= 0 && len > p.limit)) {
+    if (threadIdx.x == 0) int8_report(p.status);
+    len = p.limit >= 0 ? 0 : static_cast<int>(capacity);
+  }
+  len = max(len, 0);
+  const int hi = len / kI8AttnKeys + (len % kI8AttnKeys != 0), step = kI8AttnWarps * p.splits;
+  const int tile0 = split * kI8AttnWarps + warp;
+  const int* table = p.page_table + static_cast<int64_t>(b) * p.max_pages;
+  if (lane == 0) {
+    for (int i = 0; i < kI8AttnStages; ++i) mbar_init(&s_full[warp][i], 1);
+    fence_barrier_init();
+    fence_proxy_async();
+  }
+  __syncwarp();
+
+  // Places of a warp's tiles, sixteen at a time: lane l has chunk l % 2 of tile l / 2 of a batch, its page a batch ahead of the
+  // row of the pools and the magnitudes that follow from it, and those a batch ahead of their use.
+  auto position = [&](int batch) -> int64_t {
+    return (static_cast<int64_t>(tile0) + (static_cast<int64_t>(batch) * 16 + (lane >> 1)) * step) * kI8AttnKeys + (lane & 1) * kI8Chunk;
+  };
+  auto page_of = [&](int batch) -> uint32_t {
+    const int64_t pos = position(batch);
+    return pos < len ? static_cast<uint32_t>(table[p.page.div(static_cast<uint32_t>(pos))]) : 0u;
+  };
+  struct Places {
+    int row;  // of the pools; -1: no keys
+    uint16_t k_top, v_top;
+  };
+  auto places = [&](int batch, uint32_t page) -> Places {
+    const int64_t pos = position(batch);
+    Places at{-1, 0, 0};
+    if (pos >= len) return at;
+    if (page >= static_cast<uint32_t>(p.num_pages)) {
+      int8_report(p.status);
+      return at;
+    }
+    const uint32_t col = p.page.div(static_cast<uint32_t>(pos));
+    const int64_t block = static_cast<int64_t>(page) * p.num_kv_heads + kvh;
+    at.row = static_cast<int>(block * page_size + (pos - static_cast<int64_t>(col) * page_size));
+    at.k_top = *reinterpret_cast<const uint16_t*>(p.k_tops + block);
+    at.v_top = *reinterpret_cast<const uint16_t*>(p.v_tops + block);
+    return at;
+  };
+  uint32_t page = page_of(0), page_next = page_of(1);
+  Places now = places(0, page), next = places(1, page_next);
+  page = page_of(2);
+  uint8_t* ring = s_ring + warp * kI8AttnStages * Tile::kBytes;
+  // Tile `n` of the warp, whose batch is `now` or the next one.
+  auto load_tile = [&](int n, int stage, bool ahead) {
+    const int at = ahead ? next.row : now.row;
+    const int row_a = __shfl_sync(0xffffffffu, at, (n & 15) * 2), row_b = __shfl_sync(0xffffffffu, at, (n & 15) * 2 + 1);
+    if (lane == 0) {
+      uint64_t* bar = &s_full[warp][stage];
+      uint8_t* dst = ring + stage * Tile::kBytes;
+      mbar_arrive_expect_tx(bar, ((row_a >= 0) + (row_b >= 0)) * 2 * Tile::kChunk);
+      if (row_a >= 0) tma_load_2d(dst, &map_k, bar, 0, row_a);
+      if (row_b >= 0) tma_load_2d(dst + Tile::kChunk, &map_k, bar, 0, row_b);
+      if (row_a >= 0) tma_load_2d(dst + 2 * Tile::kChunk, &map_v, bar, 0, row_a);
+      if (row_b >= 0) tma_load_2d(dst + 3 * Tile::kChunk, &map_v, bar, 0, row_b);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kI8AttnStages; ++i)
+    if (tile0 + i * step < hi) load_tile(i, i, false);
+
+  // Q of head r: MMA j takes dims H / 4 * c + 4 j + (0, 2) and (1, 3).
+  uint32_t qb[kSteps][2];
+  float q_sum[2];
+  {
+    float sum = 0.f;
+    const __nv_bfloat162 up = __float2bfloat162_rn(kInt8Up);
+    const __nv_bfloat16* q = p.q + (static_cast<int64_t>(b) * p.num_q_heads + qh0 + r) * H + c * (H / 4);
+#pragma unroll
+    for (int i = 0; i < kSteps / 2; ++i) {
+      const uint4 x = r < rows ? *reinterpret_cast<const uint4*>(q + i * 8) : make_uint4(0, 0, 0, 0);
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = unpack2(w[j]);
+        sum += f.x + f.y;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t e = __byte_perm(w[2 * j], w[2 * j + 1], 0x5410), o = __byte_perm(w[2 * j], w[2 * j + 1], 0x7632);
+        const __nv_bfloat162 be = __hmul2(reinterpret_cast<const __nv_bfloat162&>(e), up);
+        const __nv_bfloat162 bo = __hmul2(reinterpret_cast<const __nv_bfloat162&>(o), up);
+        qb[2 * i + j][0] = reinterpret_cast<const uint32_t&>(be);
+        qb[2 * i + j][1] = reinterpret_cast<const uint32_t&>(bo);
+      }
+    }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    sum *= -128.f / kInt8Back;
+    q_sum[0] = __shfl_sync(0xffffffffu, sum, 8 * c);
+    q_sum[1] = __shfl_sync(0xffffffffu, sum, 8 * c + 4);
+  }
+
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, w_sum[2] = {0.f, 0.f};  // heads 2c, 2c + 1; l and w_sum of this lane's keys
+  float acc[kSteps][4];  // [i][dims H / 8 * r + 2 i, + 1][columns 2c, 2c + 1]
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+
+  int stage = 0, n = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  for (int tile = tile0; tile < hi; tile += step, ++n) {
+    if (n > 0 && (n & 15) == 0) {
+      now = next;
+      const int batch = n >> 4;
+      next = places(batch + 1, page);
+      page = page_of(batch + 2);
+    }
+    if (!mbar_wait_warp(&s_full[warp][stage], phase, p.status, kStatusWaitTimeoutEpilogue)) {
+      ok = false;
+      break;
+    }
+    const uint8_t* st = ring + stage * Tile::kBytes;
+    const int lane_a = (n & 15) * 2;
+    const uint32_t tops = static_cast<uint32_t>(now.k_top) | static_cast<uint32_t>(now.v_top) << 16;
+    float s[2][4], vt[2];
+#pragma unroll
+    for (int ch = 0; ch < 2; ++ch) {
+      const uint32_t pair = __shfl_sync(0xffffffffu, tops, lane_a + ch);
+      const float kt = __uint_as_float(pair << 16) * p.scale_log2;
+      vt[ch] = __uint_as_float(pair & 0xffff0000u) * (1.f / 127.f);
+      uint32_t w[2][kSteps];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int u = 0; u < kSteps / 4; ++u)
+          *reinterpret_cast<uint4*>(&w[i][4 * u]) =
+              *reinterpret_cast<const uint4*>(st + ch * Tile::kChunk + Tile::unit(8 * i + r, kSteps / 4 * c + u));
+      }
+      float d[4] = {q_sum[0], q_sum[1], q_sum[0], q_sum[1]};
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        const uint32_t a[4] = {int8_even(w[0][j]), int8_even(w[1][j]), int8_odd(w[0][j]), int8_odd(w[1][j])};
+        mma(d, a, qb[j][0], qb[j][1]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[ch][i] = d[i] * kt;
+    }
+    if ((tile + 1) * static_cast<int64_t>(kI8AttnKeys) > len) {
+#pragma unroll
+      for (int ch = 0; ch < 2; ++ch) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (tile * kI8AttnKeys + ch * kI8Chunk + i * 8 + r >= len) s[ch][2 * i] = s[ch][2 * i + 1] = -INFINITY;
+      }
+    }
+    // A page that is not in the pool has no keys.
+#pragma unroll
+    for (int ch = 0; ch < 2; ++ch)
+      if (__shfl_sync(0xffffffffu, now.row, lane_a + ch) < 0) s[ch][0] = s[ch][1] = s[ch][2] = s[ch][3] = -INFINITY;
+    float top[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) top[h] = fmaxf(fmaxf(s[0][h], s[0][2 + h]), fmaxf(s[1][h], s[1][2 + h]));
+    if (__any_sync(0xffffffffu, top[0] > m[0] + kI8Slack || top[1] > m[1] + kI8Slack)) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int off = 4; off <= 16; off <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], off));
+        const float m_new = fmaxf(m[h], top[h]);
+        const float by = m[h] == -INFINITY ? 0.f : ex2(m[h] - m_new);  // (nothing is there yet)
+        m[h] = m_new;
+        l[h] *= by;
+        w_sum[h] *= by;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) acc[i][h] *= by, acc[i][2 + h] *= by;
+      }
+    }
+#pragma unroll
+    for (int ch = 0; ch < 2; ++ch) {
+      uint32_t pt[2];
+      float sums[2] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float e[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) e[h] = ex2(s[ch][2 * i + h] + (m[h] == -INFINITY ? 0.f : 64.f - m[h]));  // (NaN stays)
+        const uint32_t two = pack2(e[0], e[1]);
+        sums[0] += __uint_as_float(two << 16);
+        sums[1] += __uint_as_float(two & 0xffff0000u);
+        pt[i] = int8_turned_round(two);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        l[h] += sums[h];
+        w_sum[h] = fmaf(vt[ch], sums[h] * (1.f / kInt8Up), w_sum[h]);
+      }
+      constexpr int kWords = kSteps / 2;  // of a key that a lane takes: dims H / 8 * r ..
+      uint32_t w[4][kWords];              // keys 2c, 2c + 1, 2c + 8, 2c + 9
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = 2 * c + (i & 1) + 8 * (i >> 1);
+        const uint8_t* at = st + (2 + ch) * Tile::kChunk;
+        if constexpr (H == 128) *reinterpret_cast<uint4*>(w[i]) = *reinterpret_cast<const uint4*>(at + Tile::unit(key, r));
+        else *reinterpret_cast<uint2*>(w[i]) = *reinterpret_cast<const uint2*>(at + Tile::unit(key, r >> 1) + (r & 1) * 8);
+      }
+      const float back = vt[ch] * kInt8Back;
+#pragma unroll
+      for (int j = 0; j < kWords; ++j) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t x = __byte_perm(w[0][j], w[1][j], half ? 0x7632 : 0x5410);
+          const uint32_t y = __byte_perm(w[2][j], w[3][j], half ? 0x7632 : 0x5410);
+          const uint32_t a[4] = {int8_even(x), int8_odd(x), int8_even(y), int8_odd(y)};
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+          mma(d, a, pt[0], pt[1]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[2 * j + half][i] = fmaf(back, d[i], acc[2 * j + half][i]);
+        }
+      }
+    }
+    __syncwarp();  // the stage has been read
+    if (tile + kI8AttnStages * static_cast<int64_t>(step) < hi)
+      load_tile(n + kI8AttnStages, stage, (n >> 4) != ((n + kI8AttnStages) >> 4));
+    if (++stage == kI8AttnStages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+  if (!ok)  // let copies that may still be in flight land
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+  __syncthreads();  // the merge buffers overlay the tiles
+  float* s_part = reinterpret_cast<float*>(s_ring);  // 4 warps and the CTA: [rows][H] sums, then maxima, then weights
+  const int per_warp = rows * H;
+  float* s_m = s_part + (kI8AttnWarps + 1) * per_warp;
+  float* s_l = s_m + (kI8AttnWarps + 1) * rows;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int off = 4; off <= 16; off <<= 1) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], off);
+      w_sum[h] += __shfl_xor_sync(0xffffffffu, w_sum[h], off);
+    }
+    if (2 * c + h >= rows) continue;
+    float* dst = s_part + warp * per_warp + (2 * c + h) * H + r * (H / 8);
+    const float low = -128.f * w_sum[h];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+      *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(acc[i][h] + low, acc[i][2 + h] + low);
+    if (r == 0) {
+      s_m[warp * rows + 2 * c + h] = m[h];
+      s_l[warp * rows + 2 * c + h] = l[h] * (1.f / kInt8Up);
+    }
+  }
+  __syncthreads();
+  // Thread (g, d) of H threads a head owns output dim d.
+  constexpr int kSets = kI8AttnThreads / H;
+  const int d = threadIdx.x % H;
+  for (int g = threadIdx.x / H; g < rows; g += kSets) {
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kI8AttnWarps; ++w) mm = fmaxf(mm, s_m[w * rows + g]);
+    float ll = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < kI8AttnWarps; ++w) {
+      const float f = mm == -INFINITY ? 1.f : exp2f(s_m[w * rows + g] - mm);
+      ll += s_l[w * rows + g] * f;
+      o += s_part[w * per_warp + g * H + d] * f;
+    }
+    const int64_t row = static_cast<int64_t>(b) * p.num_q_heads + qh0 + g;
+    if (p.splits == 1) {
+      p.out[row * H + d] = __float2bfloat16(ll == 0.f ? 0.f : o / ll);
+    } else {
+      s_part[kI8AttnWarps * per_warp + g * H + d] = o;
+      if (d == 0) {
+        s_m[kI8AttnWarps * rows + g] = mm;
+        s_l[kI8AttnWarps * rows + g] = ll;
+      }
+    }
+  }
+  if constexpr (kCluster) {
+    const int cluster = min(p.splits, kI8AttnCluster), rank = split % cluster, cluster_parts = p.splits / cluster;
+    cluster_sync_all();
+    for (int g = rank * kSets + threadIdx.x / H; g < rows; g += cluster * kSets) {
+      float mv[kI8AttnCluster], lv[kI8AttnCluster], ov[kI8AttnCluster];
+#pragma unroll
+      for (int s = 0; s < kI8AttnCluster; ++s) {
+        const bool have = s < cluster;
+        mv[s] = have ? ld_cluster_f32(sptr(s_m + kI8AttnWarps * rows + g), s) : -INFINITY;
+        lv[s] = have ? ld_cluster_f32(sptr(s_l + kI8AttnWarps * rows + g), s) : 0.f;
+        ov[s] = have ? ld_cluster_f32(sptr(s_part + kI8AttnWarps * per_warp + g * H + d), s) : 0.f;
+      }
+      float mm = -INFINITY;
+#pragma unroll
+      for (int s = 0; s < kI8AttnCluster; ++s) mm = fmaxf(mm, mv[s]);
+      float ll = 0.f, o = 0.f;
+#pragma unroll
+      for (int s = 0; s < kI8AttnCluster; ++s) {
+        const float f = mm == -INFINITY ? 1.f : exp2f(mv[s] - mm);
+        ll += lv[s] * f;
+        o += ov[s] * f;
+      }
+      const int64_t row = static_cast<int64_t>(b) * p.num_q_heads + qh0 + g;
+      if (cluster_parts == 1) {
+        p.out[row * H + d] = __float2bfloat16(ll == 0.f ? 0.f : o / ll);
+      } else {
+        const int64_t part = row * cluster_parts + split / cluster;
+        p.part_out[part * H + d] = o;
+        if (d == 0) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(mm, ll);
+      }
+    }
+    cluster_sync_all();  // a CTA's shared memory outlives its readers
+  }
+}
+
+// The clusters' parts of a row, eight at a time on their way.
+template <int H>
+__global__ void __launch_bounds__(H)
+int8_combine_kernel(const float* part_out, const float* part_ml, __nv_bfloat16* out, int parts) {
+  chain_link();
+  constexpr int kAtOnce = 8;
+  const int64_t row = blockIdx.x;
+  const int d = threadIdx.x;
+  float mm = -INFINITY, ll = 0.f, o = 0.f;
+  for (int s0 = 0; s0 < parts; s0 += kAtOnce) {
+    float2 ml[kAtOnce];
+    float ov[kAtOnce];
+#pragma unroll
+    for (int s = 0; s < kAtOnce; ++s) {
+      const bool have = s0 + s < parts;
+      ml[s] = have ? *reinterpret_cast<const float2*>(part_ml + (row * parts + s0 + s) * 2) : make_float2(-INFINITY, 0.f);
+      ov[s] = have ? part_out[(row * parts + s0 + s) * H + d] : 0.f;
+    }
+    float top = mm;
+#pragma unroll
+    for (int s = 0; s < kAtOnce; ++s) top = fmaxf(top, ml[s].x);
+    const float old = top == -INFINITY ? 1.f : exp2f(mm - top);
+    ll *= old;
+    o *= old;
+#pragma unroll
+    for (int s = 0; s < kAtOnce; ++s) {
+      const float f = top == -INFINITY ? 1.f : exp2f(ml[s].x - top);
+      ll += ml[s].y * f;
+      o += ov[s] * f;
+    }
+    mm = top;
+  }
+  out[row * H + d] = __float2bfloat16(ll == 0.f ? 0.f : o / ll);
+}
+
+template <int H, bool kCluster>
+static int launch_int8_attn(const CUtensorMap& map_k, const CUtensorMap& map_v, const Int8AttnParams& p, dim3 grid,
+                            cudaStream_t stream) {
+  constexpr auto kernel = int8_attn_kernel<H, kCluster>;
+  static OptIn opt_in;
+  if (!opt_in.done(kernel, Int8Tile<H>::kSmem(kI8AttnRows))) return -3;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {static_cast<unsigned>(p.splits < kI8AttnCluster ? p.splits : kI8AttnCluster), 1, 1};
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kI8AttnThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(Int8Tile<H>::kSmem(kI8AttnRows));
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = static_cast<unsigned>(chain_attribute(attr, kCluster ? 1 : 0));
+  return cudaLaunchKernelEx(&cfg, kernel, map_k, map_v, p) == cudaSuccess ? 0 : -4;
+}
+
+template <int H>
+static int int8_attn(const void* k_codes, const void* v_codes, const Int8AttnParams& p, int B, cudaStream_t stream) {
+  CUtensorMap map[2];
+  const void* codes[2] = {k_codes, v_codes};
+  for (int i = 0; i < 2; ++i) {
+    const uint64_t dims[2] = {H, static_cast<uint64_t>(p.num_pages) * p.num_kv_heads * p.page.d};
+    const uint64_t pitch[1] = {H};
+    const uint32_t box[2] = {H, kI8Chunk};
+    const int rc = make_tensor_map(&map[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes[i], dims, pitch, box,
+                                   H == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+    if (rc != 0) return rc;
+  }
+  const int g = p.num_q_heads / p.num_kv_heads;
+  const dim3 grid(p.splits, p.num_kv_heads * ((g + kI8AttnRows - 1) / kI8AttnRows), B);
+  const int rc = p.splits > 1 ? launch_int8_attn<H, true>(map[0], map[1], p, grid, stream)
+                              : launch_int8_attn<H, false>(map[0], map[1], p, grid, stream);
+  if (rc != 0) return rc;
+  if (p.splits > kI8AttnCluster)
+    launch_chained(int8_combine_kernel<H>, B * p.num_q_heads, H, 0, stream, p.part_out, p.part_ml, p.out,
+                   p.splits / kI8AttnCluster);
+  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+}
+
+// What the entry points below ask of a cache.
+static bool int8_cache_fits(int head_dim, int page_size, int num_kv_heads, int num_pages, const void* k_codes, const void* v_codes) {
+  return (head_dim == 64 || head_dim == 128) && page_size >= 16 && page_size % 16 == 0 && num_kv_heads >= 1 && num_pages >= 1 &&
+         static_cast<int64_t>(num_pages) * num_kv_heads * page_size < 0x7fffffffll && aligned16(k_codes) && aligned16(v_codes);
+}
+
+}  // namespace axb
+
+// k and v [B, T, Nkv, H] with element strides of (sequence, token, head); k_out and v_out (null: not wanted) are contiguous.
+// -10: not supported.
+extern "C" int axb_int8_append(const void* k, const void* v, int64_t k_b, int64_t k_t, int64_t k_h, int64_t v_b, int64_t v_t,
+                               int64_t v_h, void* k_out, void* v_out, void* k_codes, void* k_tops, void* v_codes, void* v_tops,
+                               const int* page_table, const int* start, const int* live, int B, int T, int num_kv_heads,
+                               int head_dim, int page_size, int max_pages, int num_pages, int* status, cudaStream_t stream) {
+  using namespace axb;
+  if (!int8_cache_fits(head_dim, page_size, num_kv_heads, num_pages, k_codes, v_codes) || B < 0 || T < 0 ||
+      (k_b | k_t | k_h | v_b | v_t | v_h) % 8)
+    return -10;
+  for (const void* x : {k, v, static_cast<const void*>(k_out), static_cast<const void*>(v_out)})
+    if (!aligned16(x)) return -10;
+  if (B == 0 || T == 0) return 0;
+  Int8AppendParams p = {};
+  p.k = {static_cast<const __nv_bfloat16*>(k), k_b, k_t, k_h};
+  p.v = {static_cast<const __nv_bfloat16*>(v), v_b, v_t, v_h};
+  p.k_out = static_cast<__nv_bfloat16*>(k_out);
+  p.v_out = static_cast<__nv_bfloat16*>(v_out);
+  p.out_h = head_dim, p.out_t = static_cast<int64_t>(num_kv_heads) * head_dim, p.out_b = T * p.out_t;
+  p.k_pool = {static_cast<uint8_t*>(k_codes), static_cast<__nv_bfloat16*>(k_tops)};
+  p.v_pool = {static_cast<uint8_t*>(v_codes), static_cast<__nv_bfloat16*>(v_tops)};
+  p.page_table = page_table, p.start = start, p.live = live, p.status = status;
+  p.T = T, p.num_kv_heads = num_kv_heads, p.max_pages = max_pages, p.num_pages = num_pages;
+  return int8_append(p, B, page_size, head_dim, stream);
+}
+
+// qkv [B, T, (Nq + 2 Nkv) * H] of one projection, queries and keys to be rotated by `angle` ([position][H / 2] of (sin, cos)).
+// Whole prompts (`lengths` null) start at position 0 and have `live` tokens (null: T): rotated queries and what the cache then
+// stands for replace queries, keys and values (zeros behind `live`).  A decoding step has T = 1 token at position lengths - 1;
+// its rotated queries go to q_out [B, Nq, H], and sequences of length 0 or behind the table or the rotations append nothing.
+extern "C" int axb_int8_rope_append(void* qkv, void* q_out, void* k_codes, void* k_tops, void* v_codes, void* v_tops,
+                                    const int* page_table, const int* lengths, const int* live, const float* angle, int angle_rows,
+                                    int B, int T, int num_q_heads, int num_kv_heads, int head_dim, int page_size, int max_pages,
+                                    int num_pages, int* status, cudaStream_t stream) {
+  using namespace axb;
+  const bool step = lengths != nullptr;
+  if (!int8_cache_fits(head_dim, page_size, num_kv_heads, num_pages, k_codes, v_codes) || num_q_heads < 1 || B < 0 || T < 0 ||
+      (step ? T != 1 || q_out == nullptr || angle_rows < 1 : angle_rows < T))
+    return -10;
+  for (const void* x : {static_cast<const void*>(qkv), static_cast<const void*>(q_out), static_cast<const void*>(angle)})
+    if (!aligned16(x)) return -10;
+  if (B == 0 || T == 0) return 0;
+  Int8AppendParams p = {};
+  __nv_bfloat16* q = static_cast<__nv_bfloat16*>(qkv);
+  const int64_t t = static_cast<int64_t>(num_q_heads + 2 * num_kv_heads) * head_dim;
+  p.q = {q, T * t, t, head_dim};
+  p.k = {q + num_q_heads * head_dim, T * t, t, head_dim};
+  p.v = {p.k.x + num_kv_heads * head_dim, T * t, t, head_dim};
+  if (step) {
+    p.q_out = static_cast<__nv_bfloat16*>(q_out);
+    p.q_out_b = p.q_out_t = static_cast<int64_t>(num_q_heads) * head_dim;
+    const int64_t capacity = static_cast<int64_t>(max_pages) * page_size;
+    p.limit = static_cast<int>(capacity < angle_rows ? capacity : angle_rows);
+  } else {
+    p.q_out = q, p.q_out_b = T * t, p.q_out_t = t;
+    p.k_out = q + num_q_heads * head_dim;
+    p.v_out = p.k_out + num_kv_heads * head_dim;
+    p.out_b = T * t, p.out_t = t, p.out_h = head_dim;
+  }
+  p.k_pool = {static_cast<uint8_t*>(k_codes), static_cast<__nv_bfloat16*>(k_tops)};
+  p.v_pool = {static_cast<uint8_t*>(v_codes), static_cast<__nv_bfloat16*>(v_tops)};
+  p.page_table = page_table, p.lengths = lengths, p.live = live, p.status = status;
+  p.angle = reinterpret_cast<const float2*>(angle);
+  p.T = T, p.num_q_heads = num_q_heads, p.num_kv_heads = num_kv_heads, p.max_pages = max_pages, p.num_pages = num_pages;
+  return int8_append(p, B, page_size, head_dim, stream);
+}
+
+// Scratch of axb_int8_decode_attn in floats: up to a cluster's splits meet without any.  More are a multiple of a cluster's.
+extern "C" int64_t axb_int8_attn_scratch_floats(int B, int num_q_heads, int head_dim, int splits) {
+  if (splits <= axb::kI8AttnCluster) return 0;
+  return static_cast<int64_t>(B) * num_q_heads * (splits / axb::kI8AttnCluster) * (head_dim + 2);
+}
+
+// One new token a sequence: q [B, Nq, H] over the cache, into out [B, Nq, H] (which may be q).  `limit` (-1: none): sequences
+// behind it get zeros.
+extern "C" int axb_int8_decode_attn(const void* q, const void* k_codes, const void* k_tops, const void* v_codes, const void* v_tops,
+                                    const int* page_table, const int* lengths, void* out, float* scratch, int limit, int B,
+                                    int num_q_heads, int num_kv_heads, int head_dim, int page_size, int max_pages, int num_pages,
+                                    int splits, float softmax_scale, int* status, cudaStream_t stream) {
+  using namespace axb;
+  if (!int8_cache_fits(head_dim, page_size, num_kv_heads, num_pages, k_codes, v_codes) || num_q_heads < 1 ||
+      num_q_heads % num_kv_heads || splits < 1 || B < 0 || B > 65535 || !(softmax_scale > 0.f && softmax_scale < 1048576.f) ||
+      !aligned16(q) || num_kv_heads * ((num_q_heads / num_kv_heads + kI8AttnRows - 1) / kI8AttnRows) > 65535)
+    return -10;
+  if (splits > kI8AttnCluster && (scratch == nullptr || (reinterpret_cast<uintptr_t>(scratch) & 7) || splits % kI8AttnCluster)) return -10;
+  if (B == 0) return 0;
+  Int8AttnParams p = {};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.k_tops = static_cast<const __nv_bfloat16*>(k_tops), p.v_tops = static_cast<const __nv_bfloat16*>(v_tops);
+  p.page_table = page_table, p.lengths = lengths;
+  p.part_out = scratch;
+  p.part_ml = scratch == nullptr ? nullptr : scratch + static_cast<int64_t>(B) * num_q_heads * (splits / kI8AttnCluster) * head_dim;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.status = status;
+  p.page = FastDiv(page_size);
+  p.num_q_heads = num_q_heads, p.num_kv_heads = num_kv_heads, p.max_pages = max_pages, p.num_pages = num_pages;
+  p.splits = splits, p.limit = limit;
+  p.scale_log2 = softmax_scale * (1.4426950408889634f / 127.f * kInt8Back);
+  return head_dim == 128 ? int8_attn<128>(k_codes, v_codes, p, B, stream) : int8_attn<64>(k_codes, v_codes, p, B, stream);
+}

@@ -1,0 +1,605 @@
+"""Serving in 8 bits: rows of activations, products with 8-bit weights and a paged 8-bit KV cache (``csrc/int8_rows.cu``,
+``csrc/int8_gemm.cu``, ``csrc/gemm_skinny.cu``, ``csrc/int8_cache.cu``).
+
+A block of values with the largest magnitude ``A`` is held as whole numbers ``c = round(127 x / A)`` (ties to the even one), -127 to
+127, and stands for ``c A / 127``.  A block with a NaN or an infinity in it stands for NaN, one whose ``A`` is below 2^-119 for zeros.
+
+* ``quantize_rows``, ``add_rms_norm_int8``, ``swiglu_int8``: activations, a block a row (a token).
+* ``quantize_weight`` / ``int8_linear``: ``x [..., K] @ w [K, N]``, a block a column of the weight (a channel); sums are integers.
+* ``append_int8``: keys and values of new tokens into the cache (prompts, chunks, single tokens); a block is the tokens of a page of
+  one KV head.  Its ``A`` grows as the page fills, and codes that are there are rounded to the new one, so a token that was
+  followed by larger ones in its page is off by up to half a step for each time ``A`` grew.
+* ``paged_decode_attention_int8``: one query token per sequence over the cache.
+* ``prompt_attention_int8``, ``rope_decode_attention_int8``: what a prompt and a decoding step run, with the rotation of
+  queries and keys and the append.
+
+Attention sees what the cache stands for: steps ``c A / 127`` itself, prompts that value rounded to bf16 (2^-8 of it at most).
+Serving only: operands that need a gradient, or carry a tangent, are refused.  CUDA tensors in bf16 go to the kernels, everything
+else runs the plain statements, which are also the oracle in tests.  Places that a page table or a length gets wrong (a page that
+the pool does not have, a position behind a table) are not touched: on the GPU they set the device's status word, which
+``cuda_ops.check_status`` raises, on the host they are an ``IndexError``.  The 16-bit forms of these operations are
+``cuda_ops.rms_norm``, ``cuda_ops.gemm`` and ``decode_ops``, those of 4 bits ``int4_ops``; the reference quantises inside its layers
+(axlearn/common/quantized_dot_general/layers.py) and has no 8-bit cache.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import dataclasses
+import math
+from typing import NamedTuple, Optional, Union
+
+import torch
+
+from axlearn_b200.ops import cuda_ops, dispatch
+from axlearn_b200.ops.int4_ops import (
+    _aligned_rows,
+    _check_counts,
+    _no_gradient,
+    _on,
+    _on_kernel,
+    _overlap,
+    _read_places,
+    _report_places,
+    _rotate,
+    _split_qkv,
+)
+
+c_void_p, c_int, c_int64, c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+Tensor = torch.Tensor
+
+LEAST = 2.0 ** -119
+MAX_ROW = 65536        # values of a row that the row kernels keep
+MAX_K = 1 << 17        # products of 127 x 127 whose sums fit 32 bits
+PAGE_UNIT = 16         # tokens of a page are a multiple of
+_configured = False
+
+
+def _lib():
+    global _configured
+    h = cuda_ops.lib()
+    if not _configured:
+        h.axb_int8_rows.argtypes = [c_void_p] * 3 + [c_int64, c_int, c_int64, c_int, c_void_p]
+        h.axb_int8_add_rms_norm.argtypes = [c_void_p] * 7 + [c_int64, c_int, c_float, c_void_p]
+        h.axb_gemm_skinny_int8.argtypes = [c_void_p] * 5 + [c_int] * 3 + [c_int64] * 3 + [c_int] * 3 + [c_void_p] * 2
+        h.axb_int8_gemm.argtypes = [c_void_p] * 5 + [c_int] * 3 + [c_int64] * 3 + [c_int] * 2 + [c_void_p] * 2
+        h.axb_int8_append.argtypes = [c_void_p] * 2 + [c_int64] * 6 + [c_void_p] * 9 + [c_int] * 7 + [c_void_p] * 2
+        h.axb_int8_rope_append.argtypes = [c_void_p] * 10 + [c_int] * 9 + [c_void_p] * 2
+        h.axb_int8_decode_attn.argtypes = [c_void_p] * 9 + [c_int] * 9 + [c_float, c_void_p, c_void_p]
+        h.axb_int8_attn_scratch_floats.argtypes = [c_int] * 4
+        h.axb_int8_attn_scratch_floats.restype = c_int64
+        for f in (h.axb_int8_rows, h.axb_int8_add_rms_norm, h.axb_gemm_skinny_int8, h.axb_int8_gemm, h.axb_int8_append,
+                  h.axb_int8_rope_append, h.axb_int8_decode_attn):
+            f.restype = c_int
+        _configured = True
+    return h
+
+
+def _call(device: torch.device, name: str, *args) -> None:
+    """Launches on the device of the operands, on its current stream."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _call(device, name, *args)
+    rc = getattr(_lib(), name)(*args, cuda_ops._stream())  # pylint: disable=protected-access
+    return cuda_ops._check(rc, name)  # pylint: disable=protected-access
+
+
+# ------------------------------------------------------------------------------------------
+# Blocks.
+# ------------------------------------------------------------------------------------------
+
+
+def _tops(top: Tensor) -> Tensor:
+    """Largest magnitudes as blocks have them: NaN where one is not finite, 0 below ``LEAST``."""
+    return torch.where(torch.isfinite(top), torch.where(top < LEAST, 0.0, top), torch.nan)
+
+
+def _codes(x: Tensor, top: Tensor, factor: int = 127) -> Tensor:
+    """``round(factor x / top)`` of values and tops that broadcast, 0 where ``top`` is 0 or NaN (64 bits: no near tie is decided
+    by a rounding ahead of it)."""
+    top = top.double()
+    level = x.double() * factor / torch.where(top > 0, top, 1.0)
+    return torch.where(top > 0, level, 0.0).round().clamp(-127, 127).to(torch.int8)
+
+
+class Int8Rows(NamedTuple):
+    """Rows in 8 bits: ``codes [..., K]`` (int8) times ``scales [...]`` (fp32)."""
+
+    codes: Tensor
+    scales: Tensor
+
+
+def row_values(rows: Int8Rows, dtype: torch.dtype = torch.float32) -> Tensor:
+    """What rows stand for: ``[..., K]``."""
+    return (rows.codes.float() * rows.scales[..., None]).to(dtype)
+
+
+def _plain_rows(x: Tensor) -> Int8Rows:
+    top = _tops(x.abs().amax(-1, keepdim=True).float())
+    return Int8Rows(_codes(x, top), (top.double() / 127.0).float()[..., 0])
+
+
+def _check_row(dim: int) -> None:
+    if dim < 8 or dim % 8 or dim > MAX_ROW:
+        raise ValueError(f"rows in 8 bits have a multiple of 8 values, up to {MAX_ROW}: {dim}")
+
+
+def _row_operand(x: Tensor, dim: int) -> tuple[Tensor, int, int]:
+    """``x [..., dim]`` as ``(tensor, rows, pitch)`` of 16-byte aligned rows; a copy where it does not lie that way."""
+    rows = x.numel() // dim
+    pitch = x.stride(0) if x.dim() == 2 and x.stride(1) == 1 and rows > 1 else dim if x.is_contiguous() else 0
+    if pitch < dim or pitch % 8 or x.data_ptr() % 16:
+        x, pitch = x.clone(memory_format=torch.contiguous_format), dim
+    return x, rows, pitch
+
+
+def quantize_rows(x: Tensor) -> Int8Rows:
+    """``x [..., K]`` (K a multiple of 8) with every row a block."""
+    _check_row(x.shape[-1])
+    _no_gradient("quantize_rows", x)
+    if not _on_kernel(x):
+        return _plain_rows(x)
+    return _launch_rows(x, x.shape[-1], False)
+
+
+def swiglu_int8(gu: Tensor) -> Int8Rows:
+    """``silu(gate) * up`` of ``gu [..., 2 F]`` (gate | up, as of one product) with every row a block of F values."""
+    if gu.shape[-1] % 2:
+        raise ValueError(f"gate and up are halves of a row: {tuple(gu.shape)}")
+    _check_row(gu.shape[-1] // 2)
+    _no_gradient("swiglu_int8", gu)
+    if not _on_kernel(gu):
+        gate, up = gu.float().chunk(2, -1)
+        return _plain_rows(torch.nn.functional.silu(gate) * up)
+    return _launch_rows(gu, gu.shape[-1] // 2, True)
+
+
+def _launch_rows(x: Tensor, dim: int, gated: bool) -> Int8Rows:
+    shape, device = x.shape[:-1], x.device
+    codes = torch.empty(shape + (dim,), dtype=torch.int8, device=device)
+    scales = torch.empty(shape, dtype=torch.float32, device=device)
+    if codes.numel():
+        x, rows, pitch = _row_operand(x, x.shape[-1])
+        _call(device, "axb_int8_rows", x.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, dim, pitch, 1 if gated else 0)
+    return Int8Rows(codes, scales)
+
+
+def add_rms_norm_int8(x: Tensor, residual: Optional[Tensor], scale: Tensor, eps: float, *, values: bool = False) -> tuple:
+    """RMS norm of ``total = x + residual`` (of ``x``, where there is no residual) with weights ``scale [D]`` and every row a
+    block: ``(Int8Rows, total)``, and with ``values`` also what the rows stand for, in ``x``'s type.  ``total`` is rounded to that
+    type ahead of the norm, which is not rounded between its steps; ``scale`` is rounded to it, too."""
+    d = x.shape[-1]
+    _check_row(d)
+    if scale.shape != (d,) or scale.device != x.device:
+        raise ValueError(f"scale {tuple(scale.shape)} on {scale.device} for rows of {d} on {x.device}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+        raise ValueError(f"residual {tuple(residual.shape)} {residual.dtype} for x {tuple(x.shape)} {x.dtype}")
+    _no_gradient("add_rms_norm_int8", x, residual, scale)
+    scale = scale.to(x.dtype)
+    if not _on_kernel(x):
+        total = x if residual is None else x + residual
+        t = total.float()
+        y = t * scale.float()
+        top = _tops(y.abs().amax(-1, keepdim=True))
+        rows = Int8Rows(_codes(y, top), (top / 127.0 * torch.rsqrt(t.square().mean(-1, keepdim=True) + eps))[..., 0])
+        return (rows, total, row_values(rows, x.dtype)) if values else (rows, total)
+    device, shape = x.device, x.shape[:-1]
+    x, n, pitch = _row_operand(x, d)
+    if pitch != d:
+        x = x.contiguous()
+    total = x
+    if residual is not None:
+        residual = residual.contiguous()
+        if residual.data_ptr() % 16:
+            residual = residual.clone()
+        total = torch.empty_like(x)
+    scale = scale.contiguous()
+    if scale.data_ptr() % 16:
+        scale = scale.clone()
+    rows = Int8Rows(torch.empty(x.shape, dtype=torch.int8, device=device), torch.empty(shape, dtype=torch.float32, device=device))
+    held = torch.empty_like(x) if values else None
+    if n:
+        _call(device, "axb_int8_add_rms_norm", x.data_ptr(), None if residual is None else residual.data_ptr(), scale.data_ptr(),
+              None if residual is None else total.data_ptr(), rows.codes.data_ptr(), rows.scales.data_ptr(),
+              None if held is None else held.data_ptr(), n, d, eps)
+    return (rows, total, held) if values else (rows, total)
+
+
+# ------------------------------------------------------------------------------------------
+# Weights.
+# ------------------------------------------------------------------------------------------
+
+
+@dataclasses.dataclass(frozen=True)
+class Int8Weight:
+    """A matrix ``[K, N]`` in 8 bits: ``codes [N, K]`` (int8), a block for each of its columns, and ``scales [N]`` (fp32)."""
+
+    codes: Tensor
+    scales: Tensor
+
+    def __post_init__(self):
+        codes, scales = self.codes, self.scales
+        if (codes.dim() != 2 or codes.dtype != torch.int8 or scales.dtype != torch.float32 or scales.shape != codes.shape[:1]
+                or codes.device != scales.device or not codes.is_contiguous() or not scales.is_contiguous()):
+            raise ValueError(f"codes {tuple(codes.shape)} {codes.dtype} and scales {tuple(scales.shape)} {scales.dtype} are not "
+                             "those of an 8-bit weight: contiguous [N, K] int8 and [N] fp32")
+        n, k = codes.shape
+        if k < 16 or k % 16 or k > MAX_K or n < 8 or n % 8:
+            raise ValueError(f"an 8-bit weight [{k}, {n}] has rows in sixteens up to {MAX_K} and columns in eights")
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return self.codes.shape[1], self.codes.shape[0]
+
+
+def quantize_weight(w: Tensor) -> Int8Weight:
+    """``w [K, N]`` (K a multiple of 16, N of 8) with every column a block."""
+    if w.dim() != 2:
+        raise ValueError(f"a weight is a matrix: {tuple(w.shape)}")
+    rows = _plain_rows(w.detach().t())
+    return Int8Weight(rows.codes.contiguous(), rows.scales.contiguous())
+
+
+def dequantize_weight(w: Int8Weight, dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """``[K, N]``, rounded to ``dtype``."""
+    return (w.codes.float() * w.scales[:, None]).to(dtype).t()
+
+
+def pair_features(rows: int, n: int) -> int:
+    """Features of a tile of 256 rows: 256, or 128 where those of 256 would leave most pairs of SMs without one."""
+    return 128 if -(-rows // 256) * -(-n // 256) <= 37 else 256
+
+
+def int8_linear(x: Union[Tensor, Int8Rows], w: Int8Weight, *, out: Optional[Tensor] = None, accumulate: bool = False,
+                dtype: Optional[torch.dtype] = None, resident: bool = False) -> Tensor:
+    """``x [..., K] @ w`` with exact integer sums of the codes, times the scales of row and column, rounded once to ``dtype`` (that
+    of ``x`` where it is a tensor, which is quantised by rows first; else bf16); into ``out [..., N]``, or with ``accumulate`` added to
+    it ahead of that rounding.  ``out`` may overlap ``x``.  ``resident``: as in ``cuda_ops.gemm``.  Serving only: there is no gradient."""
+    k, n = w.shape
+    held = isinstance(x, Int8Rows)
+    codes = x.codes if held else x
+    device = codes.device
+    if codes.shape[-1:] != (k,) or device != w.codes.device:
+        raise ValueError(f"x {tuple(codes.shape)} on {device} and a {w.shape} weight on {w.codes.device}")
+    shape = codes.shape[:-1] + (n,)
+    if held:
+        if codes.dtype != torch.int8 or x.scales.shape != codes.shape[:-1] or x.scales.dtype != torch.float32 or x.scales.device != device:
+            raise ValueError(f"rows in 8 bits are int8 codes and an fp32 scale for each: {codes.dtype}, {tuple(x.scales.shape)} "
+                             f"{x.scales.dtype}")
+        dtype = dtype or (torch.bfloat16 if out is None else out.dtype)
+    else:
+        dtype = dtype or x.dtype
+    _no_gradient("int8_linear", x.scales if held else x, w.scales, out)
+    given = out is not None
+    if not given:
+        if accumulate:
+            raise ValueError("accumulate needs out")
+        out = torch.empty(shape, dtype=dtype, device=device)
+    elif out.shape != shape or out.dtype != dtype or out.device != device or not out.is_contiguous():
+        raise ValueError(f"out {tuple(out.shape)} {out.dtype}: contiguous {tuple(shape)} {dtype} is wanted")
+    if not held:
+        x = quantize_rows(x)
+    if not _on_kernel(out):
+        # (Products of codes and their sums are whole numbers below 2^53.)
+        sums = (x.codes.double() @ w.codes.double().t()).float()
+        y = sums * x.scales[..., None] * w.scales
+        return out.copy_(out.float() + y if accumulate else y)
+    rows = out.numel() // n
+    if rows == 0:
+        return out
+    codes, scales, w_scales = x.codes, x.scales, w.scales
+    if held:
+        if not codes.is_contiguous() or codes.data_ptr() % 16 or (given and _overlap(codes, out)):
+            codes = codes.clone(memory_format=torch.contiguous_format)
+        if not scales.is_contiguous() or (given and _overlap(scales, out)):
+            scales = scales.clone(memory_format=torch.contiguous_format)
+    if w.codes.data_ptr() % 16 or w_scales.data_ptr() % 16:
+        w = Int8Weight(w.codes.clone(), w_scales.clone())
+        w_scales, resident = w.scales, False
+    word = cuda_ops.status_word(device).data_ptr()
+    if rows <= 128:
+        _call(device, "axb_gemm_skinny_int8", codes.data_ptr(), scales.data_ptr(), w.codes.data_ptr(), w_scales.data_ptr(),
+              out.data_ptr(), rows, n, k, k, k, n, 1 if accumulate else 0, 0, 1 if resident else 0, word)
+        return out
+    y = out
+    if out.data_ptr() % 16:  # a view into a larger buffer: tiles are stored as vectors
+        y = out.clone() if accumulate else torch.empty_like(out)
+    _call(device, "axb_int8_gemm", codes.data_ptr(), scales.data_ptr(), w.codes.data_ptr(), w_scales.data_ptr(), y.data_ptr(), rows,
+          n, k, k, k, n, 1 if accumulate else 0, pair_features(rows, n), word)
+    return out if y is out else out.copy_(y)
+
+
+# ------------------------------------------------------------------------------------------
+# Cache.
+# ------------------------------------------------------------------------------------------
+
+
+class Int8Pages(NamedTuple):
+    """A page pool of keys or values: ``codes [pages, Nkv, page_size, H]`` (int8) and ``tops [pages, Nkv]`` (bf16), the largest
+    magnitudes of their blocks (rounded to bf16, where the values are not): a code stands for ``code * top / 127``."""
+
+    codes: Tensor
+    tops: Tensor
+
+
+def int8_pages(num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, device=None) -> Int8Pages:
+    """A pool of zeros."""
+    if head_dim not in (64, 128):
+        raise ValueError(f"the 8-bit cache holds heads of 64 or 128, not {head_dim}")
+    if page_size < PAGE_UNIT or page_size % PAGE_UNIT:
+        raise ValueError(f"pages of the 8-bit cache hold a multiple of {PAGE_UNIT} tokens, not {page_size}")
+    return Int8Pages(torch.zeros((num_pages, num_kv_heads, page_size, head_dim), dtype=torch.int8, device=device),
+                     torch.zeros((num_pages, num_kv_heads), dtype=torch.bfloat16, device=device))
+
+
+def page_values(pages: Int8Pages, dtype: torch.dtype = torch.float32) -> Tensor:
+    """What a pool (or pages of it) stands for: ``[pages, Nkv, page_size, H]``."""
+    return (pages.codes.float() * pages.tops.float()[..., None, None] / 127.0).to(dtype)
+
+
+def _check_pages(k_pages: Int8Pages, v_pages: Int8Pages, page_table: Tensor, batch: int, heads: int, head_dim: int,
+                 device: torch.device) -> tuple:
+    """``(pages, Nkv, page size)`` of a cache that fits."""
+    (kc, kt), (vc, vt) = k_pages, v_pages
+    shape = kc.shape
+    num_pages, nkv, page_size, held = shape if len(shape) == 4 else (0, 0, 0, 0)
+    if (held != head_dim or head_dim not in (64, 128) or not nkv or heads % nkv or not num_pages or not page_size
+            or page_size % PAGE_UNIT or vc.shape != shape or kt.shape != (num_pages, nkv) or vt.shape != kt.shape):
+        raise ValueError(f"8-bit pages {tuple(shape)} with {tuple(kt.shape)}, {tuple(vc.shape)} with {tuple(vt.shape)} for {heads} "
+                         f"heads of {head_dim} (64 or 128; a multiple of {PAGE_UNIT} tokens a page)")
+    if num_pages * nkv * page_size >= 2 ** 31 - 1:
+        raise ValueError(f"8-bit pages {tuple(shape)} have 2^31 rows or more")
+    for codes, tops in (k_pages, v_pages):
+        if (codes.dtype is not torch.int8 or tops.dtype is not torch.bfloat16 or codes.device != device or tops.device != device
+                or not codes.is_contiguous() or not tops.is_contiguous() or codes.data_ptr() % 16):
+            raise ValueError(f"8-bit pages are contiguous, 16-byte aligned int8 and bf16 tensors on {device}")
+    if (page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch
+            or page_table.device != device or not page_table.is_contiguous()):
+        raise ValueError(f"a page table is a contiguous int32 matrix of {batch} rows on {device}: {tuple(page_table.shape)} "
+                         f"{page_table.dtype}")
+    return num_pages, nkv, page_size
+
+
+def _append_plain(k, v, k_pages, v_pages, page_table, start, live):
+    num_pages, nkv, page_size, _ = k_pages.codes.shape
+    b, t = k.shape[:2]
+    device = k.device
+    at = torch.arange(t, device=device)
+    keep = (at < live[:, None]) if live is not None else torch.ones((b, t), dtype=torch.bool, device=device)
+    begin = start.clamp(min=0).long()
+    row0 = begin % page_size
+    rel = row0[:, None] + at
+    block, row = rel // page_size, rel % page_size                    # of each token, counted from its sequence's first
+    many = (t + page_size - 2) // page_size + 1
+    col = begin[:, None] // page_size + torch.arange(many, device=device)
+    placed = (start >= 0)[:, None] & (col < page_table.shape[1])
+    page = torch.zeros_like(col)
+    if page_table.shape[1]:
+        page = page_table.long().gather(1, torch.where(placed, col, 0))
+    placed &= (page >= 0) & (page < num_pages)
+    touched = torch.zeros((b, many), dtype=torch.int32, device=device).scatter_add_(1, block, keep.int()) > 0
+    _report_places((touched & ~placed).any(), "a token's place is outside the page table, or its page outside the pool")
+    page = torch.where(placed, page, 0)
+    goes_on = touched[:, 0] & placed[:, 0] & (row0 > 0)               # with a block that has tokens
+    write = touched & placed
+    out = []
+    for x, pages in ((k, k_pages), (v, v_pages)):
+        size = torch.where(keep[..., None], x.abs().amax(-1).float(), 0.0)
+        size = torch.where(torch.isfinite(size), size, torch.inf)
+        old = torch.where(goes_on[:, None], pages.tops[page[:, 0]].float().abs(), 0.0)
+        top = torch.zeros((b, many, nkv), device=device)
+        top[:, 0] = torch.where(torch.isfinite(old), old, torch.inf)
+        top.scatter_reduce_(1, block[..., None].expand(b, t, nkv), size, "amax")
+        top = _tops(top.bfloat16().float())
+        turned = _codes(pages.codes[page[:, 0]].double() * old[..., None, None].double(), top[:, 0, :, None, None], 1)
+        turns = goes_on[:, None] & (top[:, 0] > 0)
+        turns = turns[..., None] & (torch.arange(page_size, device=device) < row0[:, None])[:, None]
+        for i in goes_on.nonzero()[:, 0].tolist():
+            pages.codes[page[i, 0]] = torch.where(turns[i][..., None], turned[i], pages.codes[page[i, 0]])
+        mine = top.gather(1, block[..., None].expand(b, t, nkv))[..., None]
+        codes = _codes(x, mine)
+        there = keep & write.gather(1, block)
+        pages.codes[page.gather(1, block)[there], :, row[there]] = codes[there]
+        pages.tops[page[write]] = top[write].bfloat16()
+        out.append(torch.where(keep[..., None, None], codes.float() * mine / 127.0, 0).to(x.dtype))
+    return out
+
+
+def append_int8(k: Tensor, v: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, page_table: Tensor, start: Tensor, *,
+                live: Optional[Tensor] = None, values: bool = False) -> Optional[tuple[Tensor, Tensor]]:
+    """Quantises ``k`` and ``v [B, T, Nkv, H]`` (strided views may be given) into the pages of positions ``start[b] ..`` of
+    ``page_table [B, max_pages]``; ``start [B]`` and ``live [B]`` (how many of the T tokens are there; None: all) are int32.
+    A page whose first token is among them starts anew; one that goes on keeps the tokens ahead of ``start``, under its new
+    largest magnitude.  What a page holds behind the new tokens has no meaning; other pages do not change.  ``values``: also
+    returns what the cache stands for at these tokens, ``(k, v)`` of the inputs' shape and type, zeros behind ``live``.  No two
+    columns of the page table may name the same page where it is written."""
+    b, t, nkv, h = k.shape
+    if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
+        raise ValueError(f"k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} differ")
+    device = k.device
+    num_pages, held, page_size = _check_pages(k_pages, v_pages, page_table, b, nkv, h, device)
+    if held != nkv:
+        raise ValueError(f"pages of {held} heads for {nkv}")
+    _check_counts(start, b, "start", device)
+    if live is not None:
+        _check_counts(live, b, "live", device)
+    _no_gradient("append_int8", k, v, k_pages.tops, v_pages.tops)
+    if not _on_kernel(k):
+        if not b or not t:
+            return (k.clone(), v.clone()) if values else None
+        out = _append_plain(k, v, k_pages, v_pages, page_table, start, live)
+        return tuple(out) if values else None
+    k, v = _aligned_rows(k), _aligned_rows(v)
+    out = (k.new_empty((b, t, nkv, h)), k.new_empty((b, t, nkv, h))) if values else None
+    _call(device, "axb_int8_append", k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3],
+          out[0].data_ptr() if values else None, out[1].data_ptr() if values else None, k_pages.codes.data_ptr(),
+          k_pages.tops.data_ptr(), v_pages.codes.data_ptr(), v_pages.tops.data_ptr(), page_table.data_ptr(), start.data_ptr(),
+          None if live is None else live.data_ptr(), b, t, nkv, h, page_size, page_table.shape[1], num_pages,
+          cuda_ops.status_word(device).data_ptr())
+    return out
+
+
+def attention_splits(batch: int, num_kv_heads: int, group: int, max_len: int, sms: int = 148) -> int:
+    """KV splits of attention over the 8-bit cache: one wave of CTAs (three fit an SM; one takes a split, a KV head and eight
+    query heads), 64 tokens or more for each.  Beyond 8, which meet in a cluster, the clusters' parts are merged by a second
+    launch: for long sequences, and as many as clusters of 8 fit the GPU."""
+    ctas = max(1, batch * num_kv_heads * ((group + 7) // 8))
+    splits = max(1, min(max_len // 64, 3 * sms // ctas))
+    if splits <= 8:
+        return splits
+    many = min((math.isqrt(max_len) // 4 + 4) // 8, 384 // ctas // 8) * 8
+    return many if many >= 24 else 8
+
+
+def _attention_plain(q, k_pages, v_pages, page_table, lengths, scale):
+    b, nq, h = q.shape
+    num_pages, _, page_size, _ = k_pages.codes.shape
+    pages, seen, bad = _read_places(page_table, lengths, page_size, num_pages)
+    _report_places(bad, "a length behind the page table, or a page outside the pool")
+    k, v = (page_values(Int8Pages(x.codes[pages], x.tops[pages])).transpose(1, 2).flatten(2, 3) for x in (k_pages, v_pages))
+    seen = seen[:, None, :, None]
+    k, v = torch.where(seen, k, 0), torch.where(seen, v, 0)
+    scores = q.float().unflatten(1, (k.shape[1], -1)) @ k.transpose(2, 3) * scale
+    p = torch.softmax(scores.masked_fill(~seen.transpose(2, 3), -torch.inf), -1)
+    out = torch.where(seen.any(2, keepdim=True), p @ v, 0)
+    return out.reshape(b, nq, h).to(q.dtype)
+
+
+def _check_scale(scale: float) -> None:
+    if not 0 < scale < 2 ** 20:
+        raise ValueError(f"softmax_scale {scale} is not in (0, 2^20)")
+
+
+def paged_decode_attention_int8(q: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, page_table: Tensor, lengths: Tensor, *,
+                                softmax_scale: Optional[float] = None, splits: Optional[int] = None,
+                                out: Optional[Tensor] = None, scratch: Optional[Tensor] = None) -> Tensor:
+    """q ``[B, Nq, H]``; page_table ``[B, max_pages]``, lengths ``[B]`` int32 (valid tokens per sequence; 0: zeros).  Query heads
+    are grouped by KV head.  ``out`` may be ``q``, or overlap it.  ``scratch``: ``attention_scratch_floats`` fp32 values, for
+    more than eight splits (made a multiple of eight); calls that overlap on the GPU need one each.  Queries from 2^-40 to 2^56 and
+    pages' tops from 2^-40 to 2^50 keep their digits; larger ones may overflow.  Returns ``[B, Nq, H]``."""
+    b, nq, h = q.shape
+    device = q.device
+    num_pages, nkv, page_size = _check_pages(k_pages, v_pages, page_table, b, nq, h, device)
+    _check_counts(lengths, b, "lengths", device)
+    scale = 1.0 / math.sqrt(h) if softmax_scale is None else softmax_scale
+    _check_scale(scale)
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != device or not out.is_contiguous()):
+        raise ValueError(f"out {tuple(out.shape)} {out.dtype}: contiguous {tuple(q.shape)} {q.dtype} is wanted")
+    _no_gradient("paged_decode_attention_int8", q, k_pages.tops, v_pages.tops, out)
+    if not _on_kernel(q):
+        y = _attention_plain(q, k_pages, v_pages, page_table, lengths, scale)
+        return y if out is None else out.copy_(y)
+    # (In place is fine: a CTA, and its cluster, has its heads' queries before it stores their output.)
+    if not q.is_contiguous() or q.data_ptr() % 16 or (out is not None and q.data_ptr() != out.data_ptr() and _overlap(q, out)):
+        q = q.clone(memory_format=torch.contiguous_format)
+    if out is None:
+        out = torch.empty_like(q)
+    _launch_attention(q, k_pages, v_pages, page_table, lengths, -1, out, scratch, b, nq, nkv, h, page_size, num_pages, splits, scale)
+    return out
+
+
+def _launch_attention(q, k_pages, v_pages, page_table, lengths, limit, out, scratch, b, nq, nkv, h, page_size, num_pages, splits, scale):
+    max_pages, device = page_table.shape[1], q.device
+    if splits is None:
+        splits = attention_splits(b, nkv, nq // nkv, max_pages * page_size)
+    if splits > 8:
+        splits = -(-splits // 8) * 8
+        floats = attention_scratch_floats(b, nq, h, splits)
+        if scratch is None:
+            scratch = torch.empty(floats, dtype=torch.float32, device=device)
+        elif (scratch.numel() < floats or scratch.dtype != torch.float32 or scratch.device != device
+              or not scratch.is_contiguous() or scratch.data_ptr() % 8):
+            raise ValueError(f"scratch is {floats} contiguous fp32 values on {device}, 8-byte aligned")
+    _call(device, "axb_int8_decode_attn", q.data_ptr(), k_pages.codes.data_ptr(), k_pages.tops.data_ptr(), v_pages.codes.data_ptr(),
+          v_pages.tops.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(),
+          None if scratch is None else scratch.data_ptr(), limit, b, nq, nkv, h, page_size, max_pages, num_pages, splits, scale,
+          cuda_ops.status_word(device).data_ptr())
+
+
+def attention_scratch_floats(batch: int, num_q_heads: int, head_dim: int, splits: int) -> int:
+    """fp32 values that the parts of more than eight splits take (a multiple of eight)."""
+    splits = -(-splits // 8) * 8 if splits > 8 else splits
+    return _lib().axb_int8_attn_scratch_floats(batch, num_q_heads, head_dim, splits)
+
+
+def _check_packed(qkv: Tensor, k_pages: Int8Pages, table: Tensor, nq: int) -> tuple[int, int]:
+    """``(Nkv, H)`` of a packed projection that fits the cache and the rotation table."""
+    nkv, h = k_pages.codes.shape[1], k_pages.codes.shape[3]
+    if qkv.shape[-1] != (nq + 2 * nkv) * h or not qkv.is_contiguous() or qkv.data_ptr() % 16:
+        raise ValueError(f"a packed projection of {nq} + 2 x {nkv} heads of {h} is contiguous and 16-byte aligned: {tuple(qkv.shape)}")
+    if (table.dtype != torch.float32 or table.shape[1:] != (h // 2, 2) or not len(table) or not table.is_contiguous()
+            or table.device != qkv.device or table.data_ptr() % 16):
+        raise ValueError(f"a rotation table is [positions, {h // 2}, 2] fp32 on {qkv.device}: {tuple(table.shape)} {table.dtype}")
+    return nkv, h
+
+
+def rope_decode_attention_int8(qkv: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, page_table: Tensor, lengths: Tensor,
+                               table: Tensor, *, num_q_heads: int, softmax_scale: float, splits: Optional[int] = None,
+                               scratch: Optional[Tensor] = None) -> Tensor:
+    """``qkv [B, (Nq + 2 Nkv) * H]`` of the token at position ``lengths - 1``: rotates its query and key by ``table [positions,
+    H / 2, 2]`` (``decode_ops.rope_table``), appends key and value to the cache and attends to it.  Rows of length 0, and those
+    behind the page table or the rotation table, append nothing and get zeros.  Returns ``[B, Nq, H]``."""
+    nkv, h = _check_packed(qkv, k_pages, table, num_q_heads)
+    if qkv.dim() != 2:
+        raise ValueError(f"a step takes one token a sequence, [B, width]: {tuple(qkv.shape)}")
+    b, device = qkv.shape[0], qkv.device
+    num_pages, _, page_size = _check_pages(k_pages, v_pages, page_table, b, num_q_heads, h, device)
+    _check_counts(lengths, b, "lengths", device)
+    _check_scale(softmax_scale)
+    _no_gradient("rope_decode_attention_int8", qkv, k_pages.tops, v_pages.tops, table)
+    limit = min(table.shape[0], page_table.shape[1] * page_size)
+    if not _on_kernel(qkv):
+        if not b:
+            return qkv.new_empty((0, num_q_heads, h))
+        q, k, v = (x[:, None] for x in _split_qkv(qkv, num_q_heads, nkv))
+        without = lengths > limit  # a place or a rotation
+        _report_places(without.any(), f"a position behind a rotation table of {table.shape[0]} or the page table")
+        lengths = torch.where(without, 0, lengths)
+        pos = lengths[:, None].long() - 1
+        q, k = _rotate(q, table, pos), _rotate(k, table, pos)
+        _append_plain(k, v, k_pages, v_pages, page_table, lengths - 1, (lengths > 0).to(torch.int32))
+        return paged_decode_attention_int8(q[:, 0], k_pages, v_pages, page_table, lengths, softmax_scale=softmax_scale)
+    out = torch.empty((b, num_q_heads, h), dtype=qkv.dtype, device=device)  # the rotated queries, then what they attend to
+    _call(device, "axb_int8_rope_append", qkv.data_ptr(), out.data_ptr(), k_pages.codes.data_ptr(), k_pages.tops.data_ptr(),
+          v_pages.codes.data_ptr(), v_pages.tops.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), None, table.data_ptr(),
+          table.shape[0], b, 1, num_q_heads, nkv, h, page_size, page_table.shape[1], num_pages,
+          cuda_ops.status_word(device).data_ptr())
+    _launch_attention(out, k_pages, v_pages, page_table, lengths, limit, out, scratch, b, num_q_heads, nkv, h, page_size, num_pages,
+                      splits, softmax_scale)
+    return out
+
+
+def prompt_attention_int8(qkv: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, page_table: Tensor, table: Tensor, *,
+                          num_q_heads: int, softmax_scale: float, live: Optional[Tensor] = None) -> Tensor:
+    """Whole prompts from position 0: ``qkv [B, T, (Nq + 2 Nkv) * H]`` of one projection, ``live [B]`` (int32; None: T) tokens of
+    each.  Rotates queries and keys by ``table``, appends keys and values to the cache and runs causal attention over what the
+    cache then stands for: in ``qkv`` queries are replaced by rotated ones, keys and values by the cache's, rounded to
+    ``qkv``'s type (zeros behind ``live``).  Returns ``[B, T, Nq * H]``."""
+    nkv, h = _check_packed(qkv, k_pages, table, num_q_heads)
+    b, t, width = qkv.shape
+    device = qkv.device
+    num_pages, _, page_size = _check_pages(k_pages, v_pages, page_table, b, num_q_heads, h, device)
+    if table.shape[0] < t or page_table.shape[1] * page_size < t:
+        raise ValueError(f"{b} x {t} tokens, a rotation table of {table.shape[0]} positions, a page table {tuple(page_table.shape)}")
+    if live is not None:
+        _check_counts(live, b, "live", device)
+    _no_gradient("prompt_attention_int8", qkv, k_pages.tops, v_pages.tops, table)
+    if not qkv.numel():
+        return qkv.new_empty((b, t, num_q_heads * h))
+    q, k, v = _split_qkv(qkv, num_q_heads, nkv)
+    if not _on_kernel(qkv):
+        pos = torch.arange(t, device=qkv.device).expand(b, t)
+        q.copy_(_rotate(q, table, pos))
+        start = torch.zeros(b, dtype=torch.int32, device=qkv.device)
+        for x, y in zip((k, v), _append_plain(_rotate(k, table, pos), v, k_pages, v_pages, page_table, start, live)):
+            x.copy_(y)
+        out = dispatch.reference.attention(q, k, v, causal=True, softmax_scale=softmax_scale)
+        return out.reshape(b, t, num_q_heads * h)
+    from axlearn_b200.ops import decode_ops
+
+    _call(device, "axb_int8_rope_append", qkv.data_ptr(), None, k_pages.codes.data_ptr(), k_pages.tops.data_ptr(),
+          v_pages.codes.data_ptr(), v_pages.tops.data_ptr(), page_table.data_ptr(), None, None if live is None else live.data_ptr(),
+          table.data_ptr(), table.shape[0], b, t, num_q_heads, nkv, h, page_size, page_table.shape[1], num_pages,
+          cuda_ops.status_word(device).data_ptr())
+    with _on(device):
+        return decode_ops.packed_prompt_attention(qkv, num_q_heads=num_q_heads, num_kv_heads=nkv, softmax_scale=softmax_scale)
