@@ -294,7 +294,7 @@ int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   if (lane == 0) {
     for (int i = 0; i < kI8AttnStages; ++i) mbar_init(&s_full[warp][i], 1);
     fence_barrier_init();
-    fence_proxy_async();
+    asm volatile("fence.proxy.async;" ::: "memory");  // the barriers, and the pools as the kernel before left them
   }
   __syncwarp();
 
@@ -713,11 +713,12 @@ extern "C" int axb_int8_rope_append(void* qkv, void* q_out, void* k_codes, void*
   using namespace axb;
   const bool step = lengths != nullptr;
   if (!int8_cache_fits(head_dim, page_size, num_kv_heads, num_pages, k_codes, v_codes) || num_q_heads < 1 || B < 0 || T < 0 ||
-      (step ? T != 1 || q_out == nullptr || angle_rows < 1 : angle_rows < T))
+      (step ? T != 1 || angle_rows < 1 : angle_rows < T))
     return -10;
+  if (B == 0 || T == 0) return 0;
+  if (step && q_out == nullptr) return -10;
   for (const void* x : {static_cast<const void*>(qkv), static_cast<const void*>(q_out), static_cast<const void*>(angle)})
     if (!aligned16(x)) return -10;
-  if (B == 0 || T == 0) return 0;
   Int8AppendParams p = {};
   __nv_bfloat16* q = static_cast<__nv_bfloat16*>(qkv);
   const int64_t t = static_cast<int64_t>(num_q_heads + 2 * num_kv_heads) * head_dim;
@@ -760,8 +761,8 @@ extern "C" int axb_int8_decode_attn(const void* q, const void* k_codes, const vo
       num_q_heads % num_kv_heads || splits < 1 || B < 0 || B > 65535 || !(softmax_scale > 0.f && softmax_scale < 1048576.f) ||
       !aligned16(q) || num_kv_heads * ((num_q_heads / num_kv_heads + kI8AttnRows - 1) / kI8AttnRows) > 65535)
     return -10;
-  if (splits > kI8AttnCluster && (scratch == nullptr || (reinterpret_cast<uintptr_t>(scratch) & 7) || splits % kI8AttnCluster)) return -10;
   if (B == 0) return 0;
+  if (splits > kI8AttnCluster && (scratch == nullptr || (reinterpret_cast<uintptr_t>(scratch) & 7) || splits % kI8AttnCluster)) return -10;
   Int8AttnParams p = {};
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.k_tops = static_cast<const __nv_bfloat16*>(k_tops), p.v_tops = static_cast<const __nv_bfloat16*>(v_tops);

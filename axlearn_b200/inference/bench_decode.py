@@ -65,8 +65,8 @@ def main():
     ap.add_argument("--prompt-len", type=int, default=2048)
     ap.add_argument("--new-tokens", type=int, default=256)
     ap.add_argument("--page-size", type=int, default=16)
-    ap.add_argument("--weight-bits", type=int, default=16, choices=(4, 16))
-    ap.add_argument("--cache-bits", type=int, default=16, choices=(4, 16))
+    ap.add_argument("--weight-bits", type=int, default=16, choices=(4, 8, 16))
+    ap.add_argument("--cache-bits", type=int, default=16, choices=(4, 8, 16))
     ap.add_argument("--no-graph", action="store_true")
     args = ap.parse_args()
 
@@ -81,8 +81,8 @@ def main():
         group = dist.group.WORLD
     dims = MODELS[args.model]
     weights = random_weights(dims, rank=rank, world=world, device=device)
-    if args.weight_bits == 4:
-        weights = quantize_weights(weights)
+    if args.weight_bits != 16:
+        weights = quantize_weights(weights, bits=args.weight_bits)
     engine = DecodeEngine(weights, dims, batch=args.batch, max_len=args.prompt_len + args.new_tokens + 16,
                           page_size=args.page_size, group=group, device=device, use_graph=not args.no_graph,
                           cache_bits=args.cache_bits)

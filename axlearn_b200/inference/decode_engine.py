@@ -21,8 +21,9 @@ persistent buffers, so the engine:
 * captures one decode step (all layers, head, greedy pick, length bump) in a CUDA graph and
   replays it per token.
 
-With ``cache_bits=4`` the pools hold keys and values in 4 bits, and weights may be in 4 bits too (``quantize_weights``):
-``ops/int4_ops.py``, on one GPU.
+With ``cache_bits`` of 4 or 8 the pools hold keys and values in as many, and weights may be in 4 or 8 bits too
+(``quantize_weights``): ``ops/int4_ops.py`` and ``ops/int8_ops.py``, on one GPU.  Products with 8-bit weights take their rows in 8
+bits, straight from the norms and the activation.
 
 Prefill runs the same weights over whole prompts with the flash-attention forward kernel and
 writes K/V into the pages.  Sequences own a contiguous run of pages (sequence ``b`` owns pages
@@ -42,10 +43,11 @@ from typing import Any, Optional, Union
 import torch
 
 from axlearn_b200.common.utils import flatten_items
-from axlearn_b200.ops import cuda_ops, decode_ops, int4_ops, packed_ops, step_ops
+from axlearn_b200.ops import cuda_ops, decode_ops, int4_ops, int8_ops, packed_ops, step_ops
 
 Tensor = torch.Tensor
-Matrix = Union[Tensor, int4_ops.Int4Weight]
+Matrix = Union[Tensor, int4_ops.Int4Weight, int8_ops.Int8Weight]
+Rows = Union[Tensor, int8_ops.Int8Rows]
 
 
 @dataclasses.dataclass
@@ -71,12 +73,17 @@ class LayerWeights:
     wdown: Matrix       # [F_l, D]
 
 
-def quantize_weights(weights: dict, *, group: int = 128) -> dict:
-    """The weights of an engine with the layers' matrices in 4 bits (``int4_ops.quantize_weight``); norms, embedding and
-    output head stay as they are."""
+def quantize_weights(weights: dict, *, group: int = 128, bits: int = 4) -> dict:
+    """The weights of an engine with the layers' matrices in 4 bits (``int4_ops.quantize_weight``, groups of ``group``) or in 8
+    (``int8_ops.quantize_weight``); norms, embedding and output head stay as they are."""
+    if bits not in (4, 8):
+        raise ValueError(f"weights of {bits} bits: 4 or 8 are there")
+
+    def matrix(w: Tensor) -> Matrix:
+        return int4_ops.quantize_weight(w, group=group) if bits == 4 else int8_ops.quantize_weight(w)
+
     def layer(lw: LayerWeights) -> LayerWeights:
-        return dataclasses.replace(lw, **{name: int4_ops.quantize_weight(getattr(lw, name), group=group)
-                                          for name in ("wqkv", "wo", "wgu", "wdown")})
+        return dataclasses.replace(lw, **{name: matrix(getattr(lw, name)) for name in ("wqkv", "wo", "wgu", "wdown")})
 
     return {**weights, "layers": [layer(lw) for lw in weights["layers"]]}
 
@@ -166,6 +173,9 @@ class BaseDecodeEngine:
         """Buffers a step changes and that a warm-up step must leave as they were."""
         return [self.lengths, self.tokens]
 
+    def _before_warm_up(self) -> None:
+        """Keeps a warm-up step from changing more than ``_mutable_buffers`` and places that the next step writes."""
+
     def _check_status(self) -> None:
         if self.device.type == "cuda":
             cuda_ops.check_status(self.device)
@@ -216,6 +226,7 @@ class BaseDecodeEngine:
             # epoch of a tensor-parallel all-reduce keeps counting: peers warm up the same number of steps.
             buffers = self._mutable_buffers()
             saved = [t.clone() for t in buffers]
+            self._before_warm_up()
             s = torch.cuda.Stream(device=self.device)
             s.wait_stream(torch.cuda.current_stream(self.device))
             with torch.cuda.stream(s):
@@ -262,8 +273,8 @@ class BaseDecodeEngine:
 
 class DecodeEngine(BaseDecodeEngine):
     """Greedy generation for ``batch`` sequences of up to ``max_len`` tokens on one GPU of a
-    tensor-parallel group (``group=None``: single GPU).  ``cache_bits``: 16 or 4, on one GPU also with the weights of
-    ``quantize_weights``."""
+    tensor-parallel group (``group=None``: single GPU).  ``cache_bits``: 16, or on one GPU 8 or 4, where also the weights of
+    ``quantize_weights`` run."""
 
     def __init__(self, weights: dict, dims: FujiDims, *, batch: int, max_len: int, page_size: int = 16,
                  group=None, device=None, use_graph: bool = True, prefill_chunk_tokens: int = 16384, cache_bits: int = 16):
@@ -282,18 +293,19 @@ class DecodeEngine(BaseDecodeEngine):
         self.nq_l, self.nkv_l = d.num_heads // self.world, d.num_kv_heads // self.world
         self.max_pages = (max_len + page_size - 1) // page_size
         self.max_len = self.max_pages * page_size
-        if cache_bits not in (4, 16):
-            raise ValueError(f"a cache of {cache_bits} bits: 4 or 16 are there")
+        if cache_bits not in (4, 8, 16):
+            raise ValueError(f"a cache of {cache_bits} bits: 4, 8 or 16 are there")
         self.cache_bits = cache_bits
-        if self.world > 1 and (cache_bits == 4 or any(
-                isinstance(w, int4_ops.Int4Weight) for lw in weights["layers"] for w in (lw.wqkv, lw.wo, lw.wgu, lw.wdown))):
-            raise NotImplementedError("4-bit weights and caches run on one GPU")
+        if self.world > 1 and (cache_bits != 16 or not all(
+                isinstance(w, Tensor) for lw in weights["layers"] for w in (lw.wqkv, lw.wo, lw.wgu, lw.wdown))):
+            raise NotImplementedError("4-bit and 8-bit weights and caches run on one GPU")
         self.k_pools, self.v_pools = ([self._pool(batch * self.max_pages) for _ in range(d.num_layers)] for _ in range(2))
         self.page_table = torch.arange(batch * self.max_pages, dtype=torch.int32, device=self.device).reshape(
             batch, self.max_pages)
-        if cache_bits == 4:
-            self.splits = int4_ops.attention_splits(batch, self.nkv_l, self.nq_l // self.nkv_l, self.max_len)
-            floats = int4_ops.attention_scratch_floats(batch, self.nq_l, d.head_dim, self.splits)
+        if cache_bits != 16:
+            ops = int4_ops if cache_bits == 4 else int8_ops
+            self.splits = ops.attention_splits(batch, self.nkv_l, self.nq_l // self.nkv_l, self.max_len)
+            floats = ops.attention_scratch_floats(batch, self.nq_l, d.head_dim, self.splits)
             self._rope_table = decode_ops.rope_table(self.max_len, d.head_dim, d.rope_theta, self.device)
         else:
             self.splits = decode_ops.tile_splits(batch, self.nkv_l, self.nq_l // self.nkv_l, self.max_len)
@@ -307,14 +319,20 @@ class DecodeEngine(BaseDecodeEngine):
         self._prefill_chunk_tokens = prefill_chunk_tokens
 
     # ------------------------------------------------------------------ shared pieces
-    def _pool(self, pages: int) -> Union[Tensor, int4_ops.Int4Pages]:
+    def _pool(self, pages: int) -> Union[Tensor, int4_ops.Int4Pages, int8_ops.Int8Pages]:
         if self.cache_bits == 4:
             return int4_ops.int4_pages(pages, self.page_size, self.nkv_l, self.dims.head_dim, device=self.device)
+        if self.cache_bits == 8:
+            return int8_ops.int8_pages(pages, self.page_size, self.nkv_l, self.dims.head_dim, device=self.device)
         return torch.zeros((pages, self.page_size, self.nkv_l, self.dims.head_dim), dtype=torch.bfloat16, device=self.device)
 
     def _id_range(self) -> Optional[tuple]:
         rows = self.w["emb"].shape[0]
         return -rows, rows  # negative ids count from the end
+
+    def _before_warm_up(self) -> None:
+        if self.cache_bits == 8:
+            self.lengths.fill_(-1)  # sequences of length 0 in the step: an append would turn the codes of the pages that it goes to
 
     def _gemm_reduce(self, a: Tensor, w: Tensor, residual: Tensor, site: int) -> Tensor:
         """``residual + sum over ranks of (a @ w)``; the finish kernel sums the peers' slots.
@@ -334,8 +352,12 @@ class DecodeEngine(BaseDecodeEngine):
         return self._allreduce.finish(site, residual=residual.reshape(-1)).reshape(residual.shape)
 
     # ------------------------------------------------------------------ prefill
-    def _add_norm(self, x: Tensor, branch: Optional[Tensor], scale: Tensor) -> tuple[Tensor, Tensor]:
-        """``x + branch`` (``x`` without a branch) and its norm, in one pass where the kernel takes the width."""
+    def _add_norm(self, x: Tensor, branch: Optional[Tensor], scale: Tensor, w: Matrix) -> tuple[Tensor, Rows]:
+        """``x + branch`` (``x`` without a branch) and its norm as the operand of products with ``w``, in one pass where the
+        kernel takes the width."""
+        if isinstance(w, int8_ops.Int8Weight):
+            rows, total = int8_ops.add_rms_norm_int8(x, branch, scale, self.dims.norm_eps)
+            return total, rows
         if branch is None:
             return x, cuda_ops.rms_norm(x, scale, self.dims.norm_eps)
         y, total, _ = cuda_ops._rmsnorm_forward(  # pylint: disable=protected-access
@@ -343,11 +365,18 @@ class DecodeEngine(BaseDecodeEngine):
         return total, y
 
     @staticmethod
-    def _product(x: Tensor, w: Matrix) -> Tensor:
+    def _product(x: Rows, w: Matrix) -> Tensor:
         """``x [rows, K] @ w``: the kernel without an autograd node around it where it takes the sizes."""
         if isinstance(w, int4_ops.Int4Weight):
             return int4_ops.int4_linear(x, w)
+        if isinstance(w, int8_ops.Int8Weight):
+            return int8_ops.int8_linear(x, w)
         return cuda_ops.linear(x, w) if x.shape[1] % 8 or w.shape[1] % 8 else cuda_ops.gemm(x, w)
+
+    @staticmethod
+    def _gated(gu: Tensor, w: Matrix) -> Rows:
+        """``silu(gate) * up`` of a (gate | up) product, as the operand of products with ``w``."""
+        return int8_ops.swiglu_int8(gu) if isinstance(w, int8_ops.Int8Weight) else decode_ops.swiglu_packed(gu)
 
     def _sum_ranks(self, x: Tensor) -> Tensor:
         if self.world > 1:
@@ -367,30 +396,37 @@ class DecodeEngine(BaseDecodeEngine):
         assert b == self.batch and t <= self.max_len
         h = d.head_dim
         per_chunk = max(1, self._prefill_chunk_tokens // t)
-        table = self._rope_table if self.cache_bits == 4 else decode_ops.rope_table(t, h, d.rope_theta, self.device)
+        table = self._rope_table if self.cache_bits != 16 else decode_ops.rope_table(t, h, d.rope_theta, self.device)
         last_hidden = torch.empty((b, d.hidden_dim), dtype=torch.bfloat16, device=self.device)
+        # (Padding would count among the largest magnitudes of the pages that it shares with a prompt.)
+        live = None if lengths is None or self.cache_bits != 8 else lengths.to(device=self.device, dtype=torch.int32)
         for b0 in range(0, b, per_chunk):
             b1 = min(b, b0 + per_chunk)
             rows = (b1 - b0) * t
             x = self.w["emb"][prompt_ids[b0:b1].reshape(rows)]                # [bs * T, D]
             branch = None  # what the last product adds to x: summed inside the next norm
             for li, lw in enumerate(self.w["layers"]):
-                x, hn = self._add_norm(x, branch, lw.attn_norm)
+                x, hn = self._add_norm(x, branch, lw.attn_norm, lw.wqkv)
                 qkv = self._product(hn, lw.wqkv).reshape(b1 - b0, t, -1)
                 if self.cache_bits == 4:
                     attn = int4_ops.prompt_attention_int4(
                         qkv, self.k_pools[li], self.v_pools[li], self.page_table[b0:b1], table, num_q_heads=self.nq_l,
                         softmax_scale=self._softmax_scale)
+                elif self.cache_bits == 8:
+                    attn = int8_ops.prompt_attention_int8(
+                        qkv, self.k_pools[li], self.v_pools[li], self.page_table[b0:b1], table, num_q_heads=self.nq_l,
+                        softmax_scale=self._softmax_scale, live=None if live is None else live[b0:b1])
                 else:
                     attn = decode_ops.prompt_attention(
                         qkv, self.k_pools[li].view(b, self.max_len, self.nkv_l, h)[b0:b1],
                         self.v_pools[li].view(b, self.max_len, self.nkv_l, h)[b0:b1], table, num_q_heads=self.nq_l,
                         softmax_scale=self._softmax_scale)
                 branch = self._sum_ranks(self._product(attn.reshape(rows, self.nq_l * h), lw.wo))
-                x, hn = self._add_norm(x, branch, lw.ffn_norm)
-                act = None if isinstance(lw.wgu, int4_ops.Int4Weight) else cuda_ops.gemm_swiglu(hn, lw.wgu)
+                x, hn = self._add_norm(x, branch, lw.ffn_norm, lw.wgu)
+                plain = isinstance(lw.wgu, Tensor) and isinstance(lw.wdown, Tensor)
+                act = cuda_ops.gemm_swiglu(hn, lw.wgu) if plain else None
                 if act is None:
-                    act = decode_ops.swiglu_packed(self._product(hn, lw.wgu))
+                    act = self._gated(self._product(hn, lw.wgu), lw.wdown)
                 branch = self._sum_ranks(self._product(act, lw.wdown))
             if lengths is None:
                 last = (slice(None), -1)
@@ -413,11 +449,18 @@ class DecodeEngine(BaseDecodeEngine):
         cuda_ops.gemm(hn, self.w["head"].t(), out=self.logits, resident=True)
 
     # ------------------------------------------------------------------ decode
+    def _step_norm(self, x: Tensor, scale: Tensor, w: Matrix) -> Rows:
+        if isinstance(w, int8_ops.Int8Weight):
+            return int8_ops.add_rms_norm_int8(x, None, scale, self.dims.norm_eps)[0]
+        return cuda_ops.rms_norm(x, scale, self.dims.norm_eps)
+
     @staticmethod
-    def _step_product(x: Tensor, w: Matrix, residual: Optional[Tensor] = None) -> Tensor:
+    def _step_product(x: Rows, w: Matrix, residual: Optional[Tensor] = None) -> Tensor:
         """``x @ w``, into ``residual`` where there is one."""
         if isinstance(w, int4_ops.Int4Weight):
             return int4_ops.int4_linear(x, w, out=residual, accumulate=residual is not None)
+        if isinstance(w, int8_ops.Int8Weight):
+            return int8_ops.int8_linear(x, w, out=residual, accumulate=residual is not None, resident=True)
         return cuda_ops.gemm(x, w, out=residual, accumulate=residual is not None, resident=True)
 
     def _attend(self, layer: int, qkv: Tensor) -> Tensor:
@@ -425,6 +468,10 @@ class DecodeEngine(BaseDecodeEngine):
         cache = (self.k_pools[layer], self.v_pools[layer], self.page_table, self.lengths)
         if self.cache_bits == 4:
             return int4_ops.rope_decode_attention_int4(
+                qkv, *cache, self._rope_table, num_q_heads=self.nq_l, softmax_scale=self._softmax_scale, splits=self.splits,
+                scratch=self._scratch)
+        if self.cache_bits == 8:
+            return int8_ops.rope_decode_attention_int8(
                 qkv, *cache, self._rope_table, num_q_heads=self.nq_l, softmax_scale=self._softmax_scale, splits=self.splits,
                 scratch=self._scratch)
         return decode_ops.rope_decode_attention(
@@ -445,15 +492,15 @@ class DecodeEngine(BaseDecodeEngine):
             self.lengths.add_(1).clamp_(max=self.max_len)
             x = self.w["emb"][self.tokens]                                    # [B, D]
         for li, lw in enumerate(self.w["layers"]):
-            hn = cuda_ops.rms_norm(x, lw.attn_norm, d.norm_eps)
+            hn = self._step_norm(x, lw.attn_norm, lw.wqkv)
             attn = self._attend(li, self._step_product(hn, lw.wqkv))
             attn2 = attn.reshape(self.batch, self.nq_l * d.head_dim)
             if self.world > 1:
                 x = self._gemm_reduce(attn2, lw.wo, x, 2 * li)
             else:
                 self._step_product(attn2, lw.wo, residual=x)
-            hn = cuda_ops.rms_norm(x, lw.ffn_norm, d.norm_eps)
-            act = decode_ops.swiglu_packed(self._step_product(hn, lw.wgu))
+            hn = self._step_norm(x, lw.ffn_norm, lw.wgu)
+            act = self._gated(self._step_product(hn, lw.wgu), lw.wdown)
             if self.world > 1:
                 x = self._gemm_reduce(act, lw.wdown, x, 2 * li + 1)
             else:
@@ -618,7 +665,14 @@ def _bits(name: str) -> int:
     value = os.environ.get("AXB200_DECODE_WEIGHT_BITS", "16") if name == "WEIGHT" else os.environ.get("AXB200_DECODE_CACHE_BITS", "16")
     if value not in ("4", "16"):
         raise ValueError(f"AXB200_DECODE_{name}_BITS is 4 or 16, not {value!r}")
-    return int(value)
+    eights = [part for part in os.environ.get("AXB200_DECODE_INT8", "").split(",") if part]
+    if any(part not in ("weights", "cache") for part in eights):
+        raise ValueError(f"AXB200_DECODE_INT8 lists weights and cache, not {eights}")
+    if {"WEIGHT": "weights", "CACHE": "cache"}[name] not in eights:
+        return int(value)
+    if value != "16":
+        raise ValueError(f"AXB200_DECODE_INT8 and AXB200_DECODE_{name}_BITS={value} name different formats")
+    return 8
 
 
 def engine_for_decoder(decoder, *, batch: int, max_len: int) -> Optional[BaseDecodeEngine]:
@@ -654,8 +708,8 @@ def engine_for_decoder(decoder, *, batch: int, max_len: int) -> Optional[BaseDec
     if engine is None:
         _ENGINES.clear()          # one resident engine: its caches and weight copies are large
         weights = weights_from_fuji_state({"decoder": state}, dims, device=emb.device)
-        if weight_bits == 4:
-            weights = quantize_weights(weights)
+        if weight_bits != 16:
+            weights = quantize_weights(weights, bits=weight_bits)
         engine = DecodeEngine(weights, dims, batch=batch, max_len=max_len, device=emb.device, cache_bits=cache_bits)
         _ENGINES[key] = engine
     return engine

@@ -326,3 +326,467 @@ def test_append_has_the_bits_of_the_plain_statement(b, t, kv, dim, page_size, pa
         if live is not None:
             live = (live - 1).clamp(min=0)
     int8_ops.append_int8(k, v, k_pages, v_pages, table, start, live=live)
+
+
+@pytest.mark.parametrize("nq,kv,dim,splits", [(4, 4, 128, 1), (8, 2, 64, 3), (20, 2, 128, 9), (32, 8, 128, None)])
+def test_a_step_is_rotation_append_and_attention(nq, kv, dim, splits):
+    lengths = torch.tensor([1, 16, 17, 200, 0, 63, 144], dtype=torch.int32, device="cuda")
+    b, gen = len(lengths), _gen(nq)
+    k_pages, v_pages, table = _cache(b, 13, 16, kv, dim, seed=nq)
+    rope = decode_ops.rope_table(208, dim, 1e4, torch.device("cuda"))
+    qkv = (2 * _normal(gen, b, (nq + 2 * kv) * dim)).bfloat16()
+    kept = qkv.clone()
+    pools = [int8_ops.Int8Pages(p.codes.clone(), p.tops.clone()) for p in (k_pages, v_pages)]
+    got = int8_ops.rope_decode_attention_int8(qkv, k_pages, v_pages, table, lengths, rope, num_q_heads=nq, softmax_scale=0.08,
+                                              splits=splits)
+    assert torch.equal(qkv, kept) and not got[4].any()
+    # The same as separate calls: a prompt's rotation of one token, append, attention.
+    turned = qkv.clone().view(b, 1, -1, dim)
+    angle = rope[(lengths.long() - 1).clamp(min=0)][:, None, None]
+    x = turned[..., :nq + kv, :].float().unflatten(-1, (-1, 2))
+    sn, cs = angle[..., 0], angle[..., 1]
+    both = torch.stack((x[..., 0].double() * cs - x[..., 1].double() * sn, x[..., 1].double() * cs + x[..., 0].double() * sn), -1).flatten(-2)
+    turned[..., :nq + kv, :] = both.bfloat16()
+    q, k, v = turned.split((nq, kv, kv), 2)
+    int8_ops.append_int8(k, v, *pools, table, lengths - 1, live=(lengths > 0).int())
+    # (A rotation in 32 bits may round the other way: by a step of bf16, or of codes.)
+    for p, o in zip((k_pages, v_pages), pools):
+        assert (p.tops.float() / o.tops.float() - 1).abs().max() <= 2.0 ** -7
+        assert (int8_ops.page_values(p) - int8_ops.page_values(o)).abs().max() <= 2.1 * o.tops.float().max() / 127
+    assert torch.equal(v_pages.codes, pools[1].codes)
+    out = int8_ops.paged_decode_attention_int8(got.clone(), k_pages, v_pages, table, lengths, softmax_scale=0.08, splits=splits)
+    assert out.shape == got.shape
+    want, bound = _attention64(q[:, 0], k_pages, v_pages, table, lengths, 0.08)
+    # Queries that round the other way move scores, by 2^-8 of a few of their products.
+    assert ((got.double() - want).abs() <= bound + 2.0 ** -6).all()
+
+
+def test_a_step_without_a_place_appends_nothing():
+    k_pages, v_pages, table = _cache(4, 2, 16, 2, 64)
+    rope = decode_ops.rope_table(24, 64, 1e4, torch.device("cuda"))
+    lengths = torch.tensor([25, 20, 33, 0], dtype=torch.int32, device="cuda")
+    table = table.clone()
+    before = [p.codes.clone() for p in (k_pages, v_pages)]
+    qkv = _normal(_gen(7), 4, 8 * 64).bfloat16()
+    got = int8_ops.rope_decode_attention_int8(qkv, k_pages, v_pages, table, lengths, rope, num_q_heads=4, softmax_scale=0.1)
+    with pytest.raises(RuntimeError, match="status 5"):
+        cuda_ops.check_status()
+    assert not got[[0, 2, 3]].any() and got[1].any()
+    for p, old in zip((k_pages, v_pages), before):
+        others = torch.ones(len(old), dtype=torch.bool, device="cuda")
+        others[table[1, 1].long()] = False
+        assert torch.equal(p.codes[others], old[others])
+
+
+def test_bad_places_are_reported_and_not_touched():
+    k_pages, v_pages, table = _cache(3, 3, 16, 2, 128)
+    table = table.clone()
+    q = _normal(_gen(8), 3, 4, 128).bfloat16()
+    lengths = torch.tensor([20, 48, 30], dtype=torch.int32, device="cuda")
+    want = int8_ops.paged_decode_attention_int8(q, k_pages, v_pages, table, lengths)
+    cuda_ops.check_status()
+    for bad in (-1, 12, 2 ** 31 - 1):
+        at = table.clone()
+        at[1, 1] = bad
+        for splits in (1, 4, 16):
+            got = int8_ops.paged_decode_attention_int8(q, k_pages, v_pages, at, lengths, splits=splits)
+            with pytest.raises(RuntimeError, match="status 5"):
+                cuda_ops.check_status()
+            assert got.isfinite().all() and (got[[0, 2]].float() - want[[0, 2]].float()).abs().max() < 0.05
+    got = int8_ops.paged_decode_attention_int8(q, k_pages, v_pages, table, lengths + 30)
+    with pytest.raises(RuntimeError, match="status 5"):
+        cuda_ops.check_status()
+    x = _normal(_gen(9), 3, 20, 2, 128).bfloat16()
+    at = table.clone()
+    at[2, 1] = 12
+    start = torch.tensor([-5, 40, 0], dtype=torch.int32, device="cuda")
+    live = torch.tensor([20, 20, 20], dtype=torch.int32, device="cuda")
+    other = [int8_ops.Int8Pages(p.codes.clone(), p.tops.clone()) for p in (k_pages, v_pages)]
+    got = int8_ops.append_int8(x, x, k_pages, v_pages, at, start, live=live, values=True)
+    with pytest.raises(RuntimeError, match="status 5"):
+        cuda_ops.check_status()
+    want = _plain(int8_ops.append_int8, x, x, *other, at, start, live=live, values=True)
+    with pytest.raises(RuntimeError, match="status 5"):
+        cuda_ops.check_status()
+    for a, o, p, y in zip(got, want, (k_pages, v_pages), other):
+        assert torch.equal(a, o) and torch.equal(p.codes, y.codes) and torch.equal(p.tops, y.tops)
+
+
+@pytest.mark.parametrize("b,t,nq,kv,dim", [(2, 300, 8, 2, 128), (1, 1, 4, 4, 64), (3, 130, 12, 4, 64), (3, 1300, 6, 2, 128)])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_prompts_attend_to_what_the_cache_stands_for(b, t, nq, kv, dim, ragged):
+    gen = _gen(t)
+    max_pages = -(-t // 16)
+    k_pages, v_pages, table = _cache(b, max_pages, 16, kv, dim, seed=t)
+    rope = decode_ops.rope_table(t, dim, 1e4, torch.device("cuda"))
+    qkv = _normal(gen, b, t, (nq + 2 * kv) * dim).bfloat16()
+    live = torch.randint(1, t + 1, (b,), generator=gen, device="cuda", dtype=torch.int32) if ragged else None
+    mine = qkv.clone()
+    got = int8_ops.prompt_attention_int8(mine, k_pages, v_pages, table, rope, num_q_heads=nq, softmax_scale=dim ** -0.5, live=live)
+    q, k, v = mine.view(b, t, -1, dim).split((nq, kv, kv), 2)
+    given = qkv.view(b, t, -1, dim)[:, :, nq:]
+    for i in range(b):
+        n = t if live is None else int(live[i])
+        pos = torch.arange(n, device="cuda")
+        for x, pages, raw in ((k, k_pages, None), (v, v_pages, given[:, :, kv:])):
+            held = int8_ops.page_values(pages, torch.bfloat16)[table[i, pos // 16].long(), :, pos % 16]
+            assert torch.equal(x[i, :n], held) and not x[i, n:].any()
+            if raw is not None:
+                tops = pages.tops[table[i, pos // 16].long()].float()[..., None]
+                assert ((held.float() - raw[i, :n].float()).abs() <= tops * (0.5 / 127 + 2.0 ** -8) + 1e-6).all()
+    want = dispatch.reference.attention(q.double(), k.double(), v.double(), causal=True, softmax_scale=dim ** -0.5).reshape(b, t, -1)
+    # Probabilities and the output rounded to bf16, of values of up to five.
+    assert (got.double() - want).abs().max() <= 2 * 2.0 ** -8 * 5
+
+
+def test_scratch_that_does_not_fit_is_refused():
+    k_pages, v_pages, table = _cache(1, 64, 16, 1, 128)
+    q, lengths = _normal(_gen(1), 1, 2, 128).bfloat16(), torch.tensor([1000], dtype=torch.int32, device="cuda")
+    floats = int8_ops.attention_scratch_floats(1, 2, 128, 16)
+    assert floats == 2 * 2 * 130 and int8_ops.attention_scratch_floats(1, 2, 128, 8) == 0
+    call = lambda scratch: int8_ops.paged_decode_attention_int8(q, k_pages, v_pages, table, lengths, splits=9, scratch=scratch)  # noqa: E731
+    for bad in (torch.empty(floats - 1, device="cuda"), torch.empty(floats, device="cuda").half(), torch.empty(floats),
+                torch.empty(2 * floats, device="cuda")[::2], torch.empty(floats + 1, device="cuda")[1:]):
+        with pytest.raises(ValueError):
+            call(bad)
+    assert torch.equal(call(torch.empty(floats, device="cuda")), call(None))
+
+
+@pytest.mark.parametrize("nq,kv,dim,splits", [(8, 2, 128, 1), (8, 8, 64, 8), (40, 2, 128, 3), (4, 1, 128, 16)])
+def test_attention_in_place(nq, kv, dim, splits):
+    k_pages, v_pages, table = _cache(3, 40, 16, kv, dim)
+    lengths = torch.tensor([600, 3, 0], dtype=torch.int32, device="cuda")
+    q = _normal(_gen(2), 3, nq, dim).bfloat16()
+    want = int8_ops.paged_decode_attention_int8(q, k_pages, v_pages, table, lengths, splits=splits)
+    room = torch.cat([torch.zeros(nq * dim, device="cuda").bfloat16(), q.flatten()])
+    moved = room[nq * dim:].view(3, nq, dim)
+    assert torch.equal(int8_ops.paged_decode_attention_int8(moved, k_pages, v_pages, table, lengths, splits=splits,
+                                                            out=room[:-nq * dim].view(3, nq, dim)), want)
+    assert torch.equal(int8_ops.paged_decode_attention_int8(q, k_pages, v_pages, table, lengths, splits=splits, out=q), want)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_scale,v_scale", [(2.0 ** 50, 2.0 ** 45), (2.0 ** -40, 2.0 ** -40), (1.0, 2.0 ** -40)])
+def test_attention_over_small_and_large_values(dim, q_scale, v_scale):
+    k_pages, v_pages, table = _cache(2, 20, 16, 2, dim)
+    k_pages = int8_ops.Int8Pages(k_pages.codes, (k_pages.tops.float() / max(q_scale, 1.0)).bfloat16())
+    v_pages = int8_ops.Int8Pages(v_pages.codes, (v_pages.tops.float() * v_scale).bfloat16())
+    lengths = torch.tensor([300, 45], dtype=torch.int32, device="cuda")
+    q = (_normal(_gen(3), 2, 4, dim) * q_scale).bfloat16()
+    got = int8_ops.paged_decode_attention_int8(q, k_pages, v_pages, table, lengths)
+    want, bound = _attention64(q, k_pages, v_pages, table, lengths, dim ** -0.5)
+    assert ((got.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("splits", [1, 8, 16])
+def test_scores_far_apart(splits):
+    """One key of a sequence takes all the weight, wherever it stands; the others' scores are hundreds below."""
+    k_pages, v_pages, table = _cache(1, 40, 16, 1, 128)
+    q = _normal(_gen(4), 1, 8, 128).bfloat16()
+    lengths = torch.tensor([640], dtype=torch.int32, device="cuda")
+    for at in (0, 17, 33, 639):
+        page, row = table[0, at // 16].long(), at % 16
+        kept = k_pages.codes[page, 0, row].clone()
+        k_pages.codes[page, 0, row] = (q[0, 0].float() * 127 / q[0, 0].abs().amax()).round().to(torch.int8)
+        got = int8_ops.paged_decode_attention_int8(q, k_pages, v_pages, table, lengths, splits=splits, softmax_scale=3.0)
+        want, bound = _attention64(q, k_pages, v_pages, table, lengths, 3.0)
+        # Scores of some 3000 in 32 bits: 2^-12 in the exponent, and as much again of weights of other heads' keys.
+        assert ((got.double() - want).abs() <= bound + 2.0 ** -9).all()
+        k_pages.codes[page, 0, row] = kept
+
+
+def test_values_that_are_not_numbers_stay_where_they_belong():
+    k_pages, v_pages, table = _cache(3, 4, 16, 2, 128)
+    lengths = torch.tensor([40, 33, 64], dtype=torch.int32, device="cuda")
+    q = _normal(_gen(5), 3, 8, 128).bfloat16()
+    want = int8_ops.paged_decode_attention_int8(q, k_pages, v_pages, table, lengths)
+    q = q.clone()
+    q[0, 1, 5] = float("nan")
+    k_pages.tops[table[1, 1].long(), 0] = float("nan")
+    v_pages.tops[table[2, 3].long(), 1] = float("nan")
+    got = int8_ops.paged_decode_attention_int8(q, k_pages, v_pages, table, lengths)
+    bad = got.isnan().any(-1)
+    expect = torch.zeros_like(bad)
+    expect[0, 1], expect[1, :4], expect[2, 4:] = True, True, True
+    assert torch.equal(bad, expect) and torch.equal(got[~expect], want[~expect])
+
+
+@pytest.mark.parametrize("dim,page_size", [(128, 64), (64, 128)])
+def test_pools_beyond_32_bits(dim, page_size):
+    """Pages whose bytes lie behind 2^32: appended to and attended to like any others."""
+    if torch.cuda.mem_get_info()[0] < 30e9:
+        pytest.skip("needs 15 GB")
+    kv, pages = 8, 2 ** 32 // (8 * page_size * dim) + 40
+    k_pages, v_pages = (int8_ops.int8_pages(pages, page_size, kv, dim, device="cuda") for _ in range(2))
+    table = torch.tensor([[pages - 1, pages - 3, pages - 20], [2, pages - 30, 5]], dtype=torch.int32, device="cuda")
+    x = _normal(_gen(6), 2, 2 * page_size + 9, 2 * kv, dim).bfloat16()
+    start = torch.zeros(2, dtype=torch.int32, device="cuda")
+    k, v = int8_ops.append_int8(x[:, :, :kv], x[:, :, kv:], k_pages, v_pages, table, start, values=True)
+    held = int8_ops.page_values(int8_ops.Int8Pages(k_pages.codes[table.long()].flatten(0, 1), k_pages.tops[table.long()].flatten(0, 1)),
+                                torch.bfloat16).view(2, 3, kv, page_size, dim).transpose(2, 3).flatten(1, 2)
+    assert torch.equal(held[:, :x.shape[1]], k)
+    q, lengths = _normal(_gen(7), 2, 16, dim).bfloat16(), torch.full((2,), x.shape[1], dtype=torch.int32, device="cuda")
+    got = int8_ops.paged_decode_attention_int8(q, k_pages, v_pages, table, lengths)
+    want, bound = _attention64(q, k_pages, v_pages, table, lengths, dim ** -0.5)
+    assert ((got.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+def test_linear_of_codes_beyond_32_bits(rows):
+    """A weight of 4.3 GB: its last columns."""
+    if torch.cuda.mem_get_info()[0] < 12e9:
+        pytest.skip("needs 6 GB")
+    k, n = 65536, 65536 + 512
+    gen = _gen(rows)
+    codes = torch.empty(n, k, dtype=torch.int8, device="cuda")
+    for lo in range(0, n, 4096):
+        codes[lo:lo + 4096] = torch.randint(-127, 128, (min(4096, n - lo), k), generator=gen, device="cuda", dtype=torch.int8)
+    w = int8_ops.Int8Weight(codes, torch.rand(n, generator=gen, device="cuda") * 2.0 ** -14)
+    held = int8_ops.quantize_rows(_normal(gen, rows, k).bfloat16())
+    got = int8_ops.int8_linear(held, w)
+    for at in (slice(0, 128), slice(n - 128, n)):
+        want = (held.codes.double() @ codes[at].double().t()) * (held.scales.double()[:, None] * w.scales[at].double())
+        _close(got[:, at], want)
+
+
+def test_calls_replay_in_a_graph_and_on_another_stream():
+    """Every entry point, captured together and replayed over other inputs, and again on a stream of its own."""
+    gen = _gen(10)
+    k_pages, v_pages, table = _cache(3, 20, 16, 2, 128)
+    lengths = torch.tensor([40, 1, 300], dtype=torch.int32, device="cuda")
+    rope = decode_ops.rope_table(320, 128, 1e4, torch.device("cuda"))
+    x, r, norm = _normal(gen, 3, 512).bfloat16(), _normal(gen, 3, 512).bfloat16(), torch.ones(512, device="cuda").bfloat16()
+    wide = _normal(gen, 200, 512).bfloat16()
+    wqkv, wgu, wdown = _weight(gen, 512, 8 * 128), _weight(gen, 512, 2048), _weight(gen, 1024, 512)
+
+    def chain(pools):
+        rows, total = int8_ops.add_rms_norm_int8(x, r, norm, 1e-5)
+        attn = int8_ops.rope_decode_attention_int8(int8_ops.int8_linear(rows, wqkv), *pools, table, lengths, rope, num_q_heads=4,
+                                                   softmax_scale=0.1, splits=16)
+        act = int8_ops.swiglu_int8(int8_ops.int8_linear(int8_ops.quantize_rows(attn.flatten(1)), wgu))
+        out = int8_ops.int8_linear(act, wdown, out=total, accumulate=True)
+        many = int8_ops.int8_linear(wide, wgu)
+        k = attn.view(3, 1, 4, 128)[:, :, :2]
+        int8_ops.append_int8(k, k, *pools, table, lengths, values=False)
+        return out, many, int8_ops.paged_decode_attention_int8(attn, *pools, table, lengths)
+
+    def copies():
+        return [int8_ops.Int8Pages(p.codes.clone(), p.tops.clone()) for p in (k_pages, v_pages)]
+
+    want = [t.clone() for t in chain(copies())]
+    pools, side = copies(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [t.clone() for t in chain(pools)]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    held = copies()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = chain(held)
+    for seed in (11, 12):
+        for p, o in zip(held, copies()):
+            p.codes.copy_(o.codes), p.tops.copy_(o.tops)
+        x.copy_(_normal(_gen(seed), 3, 512)), wide.copy_(_normal(_gen(seed), 200, 512))
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(out, chain(copies())))
+
+
+def test_products_of_all_kinds_replay_in_graphs_side_by_side():
+    gen = _gen(13)
+    cases = []
+    for rows, k, n in ((1, 2048, 2048), (16, 4096, 1024), (100, 1024, 4096), (300, 1024, 2048)):
+        held, w = int8_ops.quantize_rows(_normal(gen, rows, k).bfloat16()), _weight(gen, k, n)
+        cases.append((held, w, int8_ops.int8_linear(held, w).clone()))
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = [int8_ops.int8_linear(held, w) for held, w, _ in cases]
+        graphs.append((graph, out, torch.cuda.Stream()))
+    for _ in range(20):
+        for graph, _, stream in graphs:
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, out, _ in graphs:
+        assert all(torch.equal(y, want) for y, (_, _, want) in zip(out, cases))
+
+
+@pytest.mark.parametrize("splits", [None, 1, 8, 9, 16])
+def test_empty_calls(splits):
+    k_pages, v_pages, table = _cache(2, 2, 16, 2, 64)
+    none, rope = torch.zeros(0, dtype=torch.int32, device="cuda"), decode_ops.rope_table(32, 64, 1e4, torch.device("cuda"))
+    empty = torch.zeros(0, 4, 64, device="cuda").bfloat16()
+    assert int8_ops.paged_decode_attention_int8(empty, k_pages, v_pages, table[:0], none, splits=splits).shape == (0, 4, 64)
+    assert int8_ops.rope_decode_attention_int8(torch.zeros(0, 512, device="cuda").bfloat16(), k_pages, v_pages, table[:0], none, rope,
+                                               num_q_heads=4, softmax_scale=0.1, splits=splits).shape == (0, 4, 64)
+    zeros = torch.zeros(2, dtype=torch.int32, device="cuda")
+    got = int8_ops.paged_decode_attention_int8(torch.ones(2, 4, 64, device="cuda").bfloat16(), k_pages, v_pages, table, zeros, splits=splits)
+    assert not got.any()
+    no_pages = torch.zeros(2, 0, dtype=torch.int32, device="cuda")
+    assert not int8_ops.paged_decode_attention_int8(torch.ones(2, 4, 64, device="cuda").bfloat16(), k_pages, v_pages, no_pages, zeros,
+                                                    splits=splits).any()
+    for x in (torch.zeros(0, 3, 2, 64, device="cuda").bfloat16(), torch.zeros(2, 0, 2, 64, device="cuda").bfloat16()):
+        k, v = int8_ops.append_int8(x, x, k_pages, v_pages, table[:len(x)], zeros[:len(x)], values=True)
+        assert k.shape == v.shape == x.shape
+    w = _weight(_gen(1), 16, 8)
+    assert int8_ops.int8_linear(torch.zeros(0, 16, device="cuda").bfloat16(), w).shape == (0, 8)
+    rows, total = int8_ops.add_rms_norm_int8(torch.zeros(0, 16, device="cuda").bfloat16(), None, torch.ones(16, device="cuda"), 1e-5)
+    assert rows.codes.shape == (0, 16) and total.shape == (0, 16)
+
+
+def test_differentiated_operands_are_refused():
+    k_pages, v_pages, table = _cache(1, 2, 16, 1, 64)
+    w, one = _weight(_gen(1), 16, 8), torch.ones(1, dtype=torch.int32, device="cuda")
+    x, q, k = (torch.ones(*s, device="cuda").bfloat16().requires_grad_() for s in ((2, 16), (1, 1, 64), (1, 1, 1, 64)))
+    for call in (lambda: int8_ops.quantize_rows(x), lambda: int8_ops.swiglu_int8(x), lambda: int8_ops.int8_linear(x, w),
+                 lambda: int8_ops.add_rms_norm_int8(x, None, torch.ones(16, device="cuda"), 1e-5),
+                 lambda: int8_ops.append_int8(k, k, k_pages, v_pages, table, one),
+                 lambda: int8_ops.paged_decode_attention_int8(q, k_pages, v_pages, table, one)):
+        with pytest.raises(ValueError, match="no gradient"):
+            call()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_other_types_run_the_plain_statements_on_the_gpu(dtype):
+    gen = _gen(14)
+    x = _normal(gen, 5, 64).to(dtype)
+    w = int8_ops.quantize_weight(_normal(gen, 64, 24))
+    cpu = int8_ops.Int8Weight(w.codes.cpu(), w.scales.cpu())
+    got = int8_ops.int8_linear(x, w)
+    assert got.dtype == dtype and torch.equal(got.cpu(), int8_ops.int8_linear(x.cpu(), cpu))
+    k_pages, v_pages, table = _cache(2, 3, 16, 2, 64)
+    other = [int8_ops.Int8Pages(p.codes.cpu(), p.tops.cpu()) for p in (k_pages, v_pages)]
+    k, start = _normal(gen, 2, 20, 2, 64).to(dtype), torch.tensor([3, 16], dtype=torch.int32, device="cuda")
+    a = int8_ops.append_int8(k, k, k_pages, v_pages, table, start, values=True)
+    b = int8_ops.append_int8(k.cpu(), k.cpu(), *other, table.cpu(), start.cpu(), values=True)
+    assert all(torch.equal(p.codes.cpu(), o.codes) and torch.equal(p.tops.cpu(), o.tops) for p, o in zip((k_pages, v_pages), other))
+    assert all((y.cpu().double() - z.double()).abs().max() <= 2 * torch.finfo(dtype).eps * z.abs().max() for y, z in zip(a, b))
+
+
+# ------------------------------------------------------------------------------------------
+# The engine.
+# ------------------------------------------------------------------------------------------
+
+
+def _engine_weights(d, f, vocab, nq, nkv, layers, seed=0):
+    from axlearn_b200.inference.decode_engine import FujiDims, LayerWeights
+
+    g = _gen(seed)
+
+    def w(*shape):
+        return (_normal(g, *shape) * shape[0] ** -0.5).bfloat16()
+
+    weights = {"layers": [LayerWeights(attn_norm=1 + 0.1 * w(d), wqkv=w(d, (nq + 2 * nkv) * 128), wo=w(nq * 128, d),
+                                       ffn_norm=1 + 0.1 * w(d), wgu=w(d, 2 * f), wdown=w(f, d)) for _ in range(layers)],
+               "emb": w(vocab, d) * 16, "head": w(vocab, d), "final_norm": 1 + 0.1 * w(d)}
+    return weights, FujiDims(num_layers=layers, hidden_dim=d, num_heads=nq, num_kv_heads=nkv, head_dim=128, ffn_dim=f,
+                             vocab_size=vocab)
+
+
+@pytest.mark.parametrize("weight_bits,cache_bits", [(8, 8), (8, 16), (16, 8), (4, 8), (8, 4)])
+@pytest.mark.parametrize("b,nq,nkv", [(1, 4, 4), (5, 8, 2)])
+def test_engine_in_8_bits_matches_its_plain_statements(weight_bits, cache_bits, b, nq, nkv):
+    """Prompts and steps with the kernels against the same engine on the plain statements, the captured step against separate
+    launches."""
+    from axlearn_b200.inference import decode_engine
+
+    weights, dims = _engine_weights(256, 528, 1000, nq, nkv, 2, seed=b)
+    if weight_bits != 16:
+        weights = decode_engine.quantize_weights(weights, group=64, bits=weight_bits)
+        assert weight_bits == 4 or all(isinstance(lw.wgu, int8_ops.Int8Weight) for lw in weights["layers"])
+    ids = torch.randint(0, 1000, (b, 90), device="cuda", generator=_gen(1))
+    lengths = torch.randint(1, 71, (b,), device="cuda", generator=_gen(2))
+    lengths[0] = 70
+
+    def engine(use_graph):
+        return decode_engine.DecodeEngine(weights, dims, batch=b, max_len=96, use_graph=use_graph, cache_bits=cache_bits)
+
+    chained, separate, plain = engine(True), engine(False), engine(False)
+
+    def close():
+        # Two layers of some five operations, each of which may round its output the other way (2^-8 of it); norms and
+        # residuals pass that on with a gain of about one.  A value that does moves to the next code in 2^-8 |x| / s of the cases, by s:
+        # with |x| about 0.8 sigma and A about 3.5 sigma, s = 0.028 sigma, that is sqrt(2 * 2^-8 * 0.8 * 0.028) = 0.013 sigma (rms; both
+        # sides may move) of each of the four products' rows and of keys and values, in each layer.  In 4 bits 0.042 of those.
+        off = (separate.logits - plain.logits).norm() / plain.logits.norm()
+        limit = 10 * 2.0 ** -8 + (2 * 4 * 0.013 if weight_bits == 8 else 0)
+        assert off < limit + (2 * 2 * 0.013 if cache_bits == 8 else 2 * 0.042 if cache_bits == 4 else 0), off
+
+    firsts = [e.prefill(ids[:, :70], lengths=lengths) for e in (chained, separate)]
+    assert torch.equal(firsts[0], firsts[1])
+    _plain(plain.prefill, ids[:, :70], lengths=lengths)
+    close()
+    for i in range(70, 90):
+        x, y = chained.step_logits(ids[:, i]).clone(), separate.step_logits(ids[:, i])
+        assert torch.equal(x, y)
+        _plain(plain.step_logits, ids[:, i])
+        close()
+    tokens = chained.generate(ids[:, :33], 5)
+    assert tokens.shape == (b, 5) and torch.equal(tokens, separate.generate(ids[:, :33], 5))
+
+
+@pytest.mark.parametrize("batch", [1, 16])
+def test_engine_steps_in_8_bits_at_serving_widths(batch):
+    """Kernels that overlap for long: replays of the chained step against separate launches, bit for bit."""
+    from axlearn_b200.inference import decode_engine
+
+    weights, dims = _engine_weights(4096, 14336, 8192, 32, 8, 2, seed=3)
+    weights = decode_engine.quantize_weights(weights, bits=8)
+    engines = [decode_engine.DecodeEngine(weights, dims, batch=batch, max_len=2048, use_graph=use, cache_bits=8) for use in (True, False)]
+    ids = torch.randint(0, 8192, (batch, 1500), device="cuda", generator=_gen(4))
+    lengths = torch.randint(1, 1501, (batch,), device="cuda", generator=_gen(5))
+    for e in engines:
+        e.prefill(ids, lengths=lengths)
+    for i in range(12):
+        x, y = (e.step_logits(ids[:, i]).clone() for e in engines)
+        assert torch.equal(x, y), i
+
+
+def test_engine_in_8_bits_is_close_to_16_bits():
+    """What both formats lose on a small model: rows, weights and cache are each off by up to half of 1 / 127 of their largest value."""
+    from axlearn_b200.inference import decode_engine
+
+    weights, dims = _engine_weights(512, 1024, 1000, 8, 2, 2, seed=9)
+    ids = torch.randint(0, 1000, (3, 60), device="cuda", generator=_gen(1))
+    logits = []
+    for bits in (16, 8):
+        w = weights if bits == 16 else decode_engine.quantize_weights(weights, bits=8)
+        e = decode_engine.DecodeEngine(w, dims, batch=3, max_len=64, use_graph=False, cache_bits=bits)
+        e.prefill(ids[:, :59])
+        logits.append(e.step_logits(ids[:, 59]).clone())
+    # A uniform rounding of s = 0.03 sigma is 0.03 / sqrt(12) = 0.009 of a value (rms); two for each of four products, two for the
+    # cache, in two layers, all passed on with a gain of about one: sqrt(20) * 0.009 = 0.04, and twice that for its spread.
+    assert (logits[1] - logits[0]).norm() / logits[0].norm() < 0.08
+
+
+def test_sample_decode_takes_the_formats_of_the_environment(monkeypatch):
+    from axlearn_b200.common import decoding, logit_modifiers, prng
+    from axlearn_b200.common.module import functional
+    from axlearn_b200.common.utils import tree_map
+    from axlearn_b200.inference import decode_engine
+    from tests.test_gpu_decode import _tiny_model
+
+    model, params = _tiny_model(1)
+    params = tree_map(lambda t: t.cuda().bfloat16() if t.is_floating_point() else t.cuda(), params)
+    prefix = torch.randint(2, 512, (2, 24), device="cuda", generator=_gen(6))
+    prefix[1, 9:] = 0
+    kwargs = dict(input_batch={"prefix": prefix}, num_decodes=2, max_sequence_length=40, logits_modifier=logit_modifiers.top_k_logits(1),
+                  stop_decoding_condition=decoding.StopOnSubsequence([[511]]))
+    seen = []
+    real = decode_engine.DecodeEngine.step_logits
+    monkeypatch.setattr(decode_engine.DecodeEngine, "step_logits", lambda self, tokens: (seen.append(self), real(self, tokens))[1])
+    monkeypatch.setenv("AXB200_DECODE_INT8", "weights,cache")
+    out, _ = functional(model, prng.PRNGKey(5), params, kwargs, is_training=False, method="sample_decode")
+    assert out.sequences.shape == (2, 2, 39) and seen[-1].cache_bits == 8
+    assert isinstance(seen[-1].w["layers"][0].wo, int8_ops.Int8Weight)
+    monkeypatch.setenv("AXB200_DECODE_INT8", "cache")
+    functional(model, prng.PRNGKey(5), params, kwargs, is_training=False, method="sample_decode")
+    assert seen[-1].cache_bits == 8 and isinstance(seen[-1].w["layers"][0].wo, torch.Tensor)
+    for name, value in (("AXB200_DECODE_INT8", "caches"), ("AXB200_DECODE_CACHE_BITS", "4")):
+        monkeypatch.setenv("AXB200_DECODE_INT8", "cache")
+        monkeypatch.setenv(name, value)
+        with pytest.raises(ValueError, match="AXB200_DECODE_INT8"):
+            functional(model, prng.PRNGKey(5), params, kwargs, is_training=False, method="sample_decode")
