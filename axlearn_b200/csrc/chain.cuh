@@ -56,4 +56,17 @@ inline void launch_chained(void (*kernel)(Params...), dim3 grid, dim3 block, siz
   cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);  // errors: cudaGetLastError, as after <<< >>>
 }
 
+// A launch that follows another of the same call, chained whatever the setting: its kernel waits for that one, and by then for
+// everything ahead of it.
+class ChainedBehind {
+ public:
+  ChainedBehind() : before_(chain_launches) { chain_launches = true; }
+  ~ChainedBehind() { chain_launches = before_; }
+  ChainedBehind(const ChainedBehind&) = delete;
+  ChainedBehind& operator=(const ChainedBehind&) = delete;
+
+ private:
+  bool before_;
+};
+
 }  // namespace axb

@@ -35,6 +35,7 @@
 #include "chain.cuh"
 #include "cluster.cuh"
 #include "host_utils.cuh"
+#include "int8.cuh"
 #include "opt_in.cuh"
 #include "sm100.cuh"
 
@@ -139,6 +140,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   static_assert(!I::kWhole || (!X_MN && !W_MN), "8-bit operands are read along K");
   constexpr int kGroup = S::kGroup, kSkK = I::kK;
   extern __shared__ uint8_t smem_raw[];
+  __shared__ float x_scales[I::kWhole ? BN : 1];  // read by the epilogue while the products run
   uint8_t* smem =
       reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S::kRingBytes);
@@ -279,12 +281,17 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     }
   } else {
     chain_wait();  // ahead of the first read or write of C
+    if (I::kWhole) {
+      const int row = static_cast<int>(threadIdx.x) - 64;
+      if (row < BN && row < p.M) x_scales[row] = p.x_scales[row];
+    }
     if (kEarlyC > 1 && p.accumulate && n0 + feature < p.N) {
 #pragma unroll
       for (int i = 0; i < kEarlyC; ++i)
         if (rank + i * split < p.M) before[i] = skinny_read(out + static_cast<int64_t>(rank + i * split) * p.ldc);
     }
     ok = mbar_wait_warp(done_bar, 0, p.status, kStatusWaitTimeoutEpilogue);
+    if (I::kWhole) asm volatile("bar.sync 1, 128;" ::: "memory");  // of the epilogue's warps: the scales are there
   }
   __syncwarp();
   if (S::kPush && splits) cluster_wait();
@@ -323,7 +330,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             if (c + j >= p.M) break;
-            float v = I::value(__uint_as_float(r[j]), I::kWhole ? p.x_scales[c + j] : 0.f, w_scale);
+            float v = I::value(__uint_as_float(r[j]), I::kWhole ? x_scales[c + j] : 0.f, w_scale);
             if (p.accumulate) v += kEarlyC > 1 ? before[j] : skinny_read(dst + j * p.ldc);
             skinny_write(dst + j * p.ldc, v);
           }
@@ -346,7 +353,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
         float sum = v[0];
 #pragma unroll
         for (int s = 1; s < kSkMaxSplit; ++s) sum = I::add(sum, v[s]);
-        sum = I::value(sum, I::kWhole ? p.x_scales[row] : 0.f, w_scale);
+        sum = I::value(sum, I::kWhole ? x_scales[row] : 0.f, w_scale);
         skinny_write(out + static_cast<int64_t>(row) * p.ldc, p.accumulate ? sum + old : sum);
       };
       if constexpr (kEarlyC > 1) {
@@ -567,21 +574,22 @@ extern "C" int axb_gemm_skinny(const void* X, const void* W, void* C, int M, int
 #undef AXB_SKINNY_BN
 }
 
-// C[M, N] (bf16, row pitch ldc) = x_scales[m] w_scales[n] sum_k X[m, k] W[n, k] (+ C when accumulate) of 8-bit whole numbers, X
-// [M, K] and W [N, K] along K with pitches ldx and ldw that are multiples of 16, M <= 128.  `split`, `w_resident` as above.
-extern "C" int axb_gemm_skinny_int8(const void* X, const float* x_scales, const void* W, const float* w_scales, void* C, int M, int N,
-                                    int K, int64_t ldx, int64_t ldw, int64_t ldc, int accumulate, int split, int w_resident,
-                                    int* status, cudaStream_t stream) {
+// y[M, N] (bf16) = x_scales[m] w_scales[n] sum_k x[m, k] w[n, k] (+ y when accumulate) of 8-bit whole numbers, x [M, K] and w [N, K]
+// one row behind the other and 16-byte aligned, M <= 128, K a multiple of 16.  `plan`: slices of K; `resident`: as above.
+extern "C" int axb_gemm_skinny_int8(const axb::Int8LinearCall* call, cudaStream_t stream) {
   using namespace axb;
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
-  if (M > 128) return -20;
-  if ((ldx % 16) || (ldw % 16) || (reinterpret_cast<uintptr_t>(X) & 15) || (reinterpret_cast<uintptr_t>(W) & 15) ||
-      (reinterpret_cast<uintptr_t>(C) & 1))
+  const Int8LinearCall& a = *call;
+  if (a.M <= 0 || a.N <= 0 || a.K <= 0) return 0;
+  if (a.M > 128) return -20;
+  if (a.N > 0x40000000 || a.K > (1 << 17) || a.K % 16 || (reinterpret_cast<uintptr_t>(a.x) & 15) ||
+      (reinterpret_cast<uintptr_t>(a.w) & 15) || (reinterpret_cast<uintptr_t>(a.y) & 1))
     return -10;
-  if (split < 0 || split > kSkMaxSplit || split > (K + SkinnyIn<int8_t>::kK - 1) / SkinnyIn<int8_t>::kK) return -15;
-  const SkinnyGemmParams p{M, N, K, C, ldc, status, accumulate, split, w_resident && chain_launches ? 1 : 0, x_scales, w_scales};
-  if (M <= 16) return launch_skinny<16, false, false, __nv_bfloat16, int8_t>(X, W, ldx, ldw, p, stream);
-  if (M <= 32) return launch_skinny<32, false, false, __nv_bfloat16, int8_t>(X, W, ldx, ldw, p, stream);
-  if (M <= 64) return launch_skinny<64, false, false, __nv_bfloat16, int8_t>(X, W, ldx, ldw, p, stream);
-  return launch_skinny<128, false, false, __nv_bfloat16, int8_t>(X, W, ldx, ldw, p, stream);
+  if (a.plan < 0 || a.plan > kSkMaxSplit || a.plan > (a.K + SkinnyIn<int8_t>::kK - 1) / SkinnyIn<int8_t>::kK) return -15;
+  const int M = static_cast<int>(a.M);
+  const SkinnyGemmParams p{M, static_cast<int>(a.N), static_cast<int>(a.K), a.y, a.N, a.status, a.accumulate != 0,
+                           static_cast<int>(a.plan), a.resident && chain_launches ? 1 : 0, a.x_scales, a.w_scales};
+  if (M <= 16) return launch_skinny<16, false, false, __nv_bfloat16, int8_t>(a.x, a.w, a.K, a.K, p, stream);
+  if (M <= 32) return launch_skinny<32, false, false, __nv_bfloat16, int8_t>(a.x, a.w, a.K, a.K, p, stream);
+  if (M <= 64) return launch_skinny<64, false, false, __nv_bfloat16, int8_t>(a.x, a.w, a.K, a.K, p, stream);
+  return launch_skinny<128, false, false, __nv_bfloat16, int8_t>(a.x, a.w, a.K, a.K, p, stream);
 }

@@ -8,6 +8,8 @@
 #include <float.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 namespace axb {
 
 constexpr float kInt8Least = 0x1p-119f;
@@ -66,5 +68,80 @@ __device__ __forceinline__ uint2 int8_pack(const float (&level)[8]) {
 
 // A bad index that the device found: code 5 of the status word.
 __device__ __forceinline__ void int8_report(int* status) { *reinterpret_cast<volatile int*>(status) = 5; }
+
+// Arguments of the entry points travel as one block of 64-bit words (pointers, whole numbers, and doubles), in the order of their
+// structs: twenty of ctypes' conversions cost 3 us, packing them 1.
+struct Int8RowsCall {
+  const void* x;
+  void* codes;
+  float* scales;
+  int64_t rows, dim, ldx, gated;
+};
+struct Int8NormCall {
+  const void *x, *residual, *weight;
+  void *total, *codes;
+  float* scales;
+  void* values;
+  int64_t rows, dim;
+  double eps;
+};
+struct Int8LinearCall {
+  const void* x;
+  const float* x_scales;
+  const void* w;
+  const float* w_scales;
+  void* y;
+  int64_t M, N, K, accumulate, plan, resident;  // plan: slices of K (0: free) of up to 128 rows, features of a tile of more
+  int* status;
+};
+struct Int8DenseCall {
+  const void* x;  // [M, K] in bf16
+  int64_t ldx;
+  void* held;     // room for its codes [M, K] and, behind them, scales [M]
+  const void* w;
+  const float* w_scales;
+  void* y;
+  int64_t M, N, K, accumulate, features, resident;  // features: 0: up to 128 rows
+  int* status;
+};
+struct Int8AppendCall {
+  const void *k, *v;
+  int64_t k_b, k_t, k_h, v_b, v_t, v_h;
+  void *k_out, *v_out, *k_codes, *k_tops, *v_codes, *v_tops;
+  const int *page_table, *start, *live;
+  int64_t B, T, num_kv_heads, head_dim, page_size, max_pages, num_pages;
+  int* status;
+};
+struct Int8RopeAppendCall {
+  void *qkv, *q_out, *k_codes, *k_tops, *v_codes, *v_tops;
+  const int *page_table, *lengths, *live;
+  const float* angle;
+  int64_t angle_rows, B, T, num_q_heads, num_kv_heads, head_dim, page_size, max_pages, num_pages;
+  int* status;
+};
+struct Int8AttnCall {
+  const void *q, *k_codes, *k_tops, *v_codes, *v_tops;
+  const int *page_table, *lengths;
+  void* out;
+  float* scratch;
+  int64_t limit, B, num_q_heads, num_kv_heads, head_dim, page_size, max_pages, num_pages, splits;
+  double softmax_scale;
+  int* status;
+};
+
+}  // namespace axb
+
+extern "C" int axb_int8_rows(const axb::Int8RowsCall* call, cudaStream_t stream);
+extern "C" int axb_int8_gemm(const axb::Int8LinearCall* call, cudaStream_t stream);
+extern "C" int axb_gemm_skinny_int8(const axb::Int8LinearCall* call, cudaStream_t stream);
+
+namespace axb {
+
+// Whether whole numbers of a call are those of an `int`.
+inline bool int8_ints(std::initializer_list<int64_t> values) {
+  for (int64_t v : values)
+    if (v < -0x7fffffffll || v > 0x7fffffffll) return false;
+  return true;
+}
 
 }  // namespace axb

@@ -662,86 +662,88 @@ static int int8_attn(const void* k_codes, const void* v_codes, const Int8AttnPar
   const int rc = p.splits > 1 ? launch_int8_attn<H, true>(map[0], map[1], p, grid, stream)
                               : launch_int8_attn<H, false>(map[0], map[1], p, grid, stream);
   if (rc != 0) return rc;
-  if (p.splits > kI8AttnCluster)
+  if (p.splits > kI8AttnCluster) {
+    ChainedBehind chained;
     launch_chained(int8_combine_kernel<H>, B * p.num_q_heads, H, 0, stream, p.part_out, p.part_ml, p.out,
                    p.splits / kI8AttnCluster);
+  }
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
 // What the entry points below ask of a cache.
-static bool int8_cache_fits(int head_dim, int page_size, int num_kv_heads, int num_pages, const void* k_codes, const void* v_codes) {
+static bool int8_cache_fits(int64_t head_dim, int64_t page_size, int64_t num_kv_heads, int64_t num_pages, const void* k_codes,
+                            const void* v_codes) {
   return (head_dim == 64 || head_dim == 128) && page_size >= 16 && page_size % 16 == 0 && num_kv_heads >= 1 && num_pages >= 1 &&
-         static_cast<int64_t>(num_pages) * num_kv_heads * page_size < 0x7fffffffll && aligned16(k_codes) && aligned16(v_codes);
+         int8_ints({page_size, num_kv_heads, num_pages}) && num_pages * num_kv_heads < 0x7fffffffll / page_size &&
+         aligned16(k_codes) && aligned16(v_codes);
 }
 
 }  // namespace axb
 
 // k and v [B, T, Nkv, H] with element strides of (sequence, token, head); k_out and v_out (null: not wanted) are contiguous.
 // -10: not supported.
-extern "C" int axb_int8_append(const void* k, const void* v, int64_t k_b, int64_t k_t, int64_t k_h, int64_t v_b, int64_t v_t,
-                               int64_t v_h, void* k_out, void* v_out, void* k_codes, void* k_tops, void* v_codes, void* v_tops,
-                               const int* page_table, const int* start, const int* live, int B, int T, int num_kv_heads,
-                               int head_dim, int page_size, int max_pages, int num_pages, int* status, cudaStream_t stream) {
+extern "C" int axb_int8_append(const axb::Int8AppendCall* call, cudaStream_t stream) {
   using namespace axb;
-  if (!int8_cache_fits(head_dim, page_size, num_kv_heads, num_pages, k_codes, v_codes) || B < 0 || T < 0 ||
-      (k_b | k_t | k_h | v_b | v_t | v_h) % 8)
+  const Int8AppendCall& a = *call;
+  if (!int8_cache_fits(a.head_dim, a.page_size, a.num_kv_heads, a.num_pages, a.k_codes, a.v_codes) || a.B < 0 || a.T < 0 ||
+      !int8_ints({a.B, a.T, a.max_pages}) || (a.k_b | a.k_t | a.k_h | a.v_b | a.v_t | a.v_h) % 8)
     return -10;
-  for (const void* x : {k, v, static_cast<const void*>(k_out), static_cast<const void*>(v_out)})
+  if (a.B == 0 || a.T == 0) return 0;
+  for (const void* x : {a.k, a.v, static_cast<const void*>(a.k_out), static_cast<const void*>(a.v_out)})
     if (!aligned16(x)) return -10;
-  if (B == 0 || T == 0) return 0;
   Int8AppendParams p = {};
-  p.k = {static_cast<const __nv_bfloat16*>(k), k_b, k_t, k_h};
-  p.v = {static_cast<const __nv_bfloat16*>(v), v_b, v_t, v_h};
-  p.k_out = static_cast<__nv_bfloat16*>(k_out);
-  p.v_out = static_cast<__nv_bfloat16*>(v_out);
-  p.out_h = head_dim, p.out_t = static_cast<int64_t>(num_kv_heads) * head_dim, p.out_b = T * p.out_t;
-  p.k_pool = {static_cast<uint8_t*>(k_codes), static_cast<__nv_bfloat16*>(k_tops)};
-  p.v_pool = {static_cast<uint8_t*>(v_codes), static_cast<__nv_bfloat16*>(v_tops)};
-  p.page_table = page_table, p.start = start, p.live = live, p.status = status;
-  p.T = T, p.num_kv_heads = num_kv_heads, p.max_pages = max_pages, p.num_pages = num_pages;
-  return int8_append(p, B, page_size, head_dim, stream);
+  p.k = {static_cast<const __nv_bfloat16*>(a.k), a.k_b, a.k_t, a.k_h};
+  p.v = {static_cast<const __nv_bfloat16*>(a.v), a.v_b, a.v_t, a.v_h};
+  p.k_out = static_cast<__nv_bfloat16*>(a.k_out);
+  p.v_out = static_cast<__nv_bfloat16*>(a.v_out);
+  p.out_h = a.head_dim, p.out_t = a.num_kv_heads * a.head_dim, p.out_b = a.T * p.out_t;
+  p.k_pool = {static_cast<uint8_t*>(a.k_codes), static_cast<__nv_bfloat16*>(a.k_tops)};
+  p.v_pool = {static_cast<uint8_t*>(a.v_codes), static_cast<__nv_bfloat16*>(a.v_tops)};
+  p.page_table = a.page_table, p.start = a.start, p.live = a.live, p.status = a.status;
+  p.T = static_cast<int>(a.T), p.num_kv_heads = static_cast<int>(a.num_kv_heads);
+  p.max_pages = static_cast<int>(a.max_pages), p.num_pages = static_cast<int>(a.num_pages);
+  return int8_append(p, static_cast<int>(a.B), static_cast<int>(a.page_size), static_cast<int>(a.head_dim), stream);
 }
 
 // qkv [B, T, (Nq + 2 Nkv) * H] of one projection, queries and keys to be rotated by `angle` ([position][H / 2] of (sin, cos)).
 // Whole prompts (`lengths` null) start at position 0 and have `live` tokens (null: T): rotated queries and what the cache then
 // stands for replace queries, keys and values (zeros behind `live`).  A decoding step has T = 1 token at position lengths - 1;
 // its rotated queries go to q_out [B, Nq, H], and sequences of length 0 or behind the table or the rotations append nothing.
-extern "C" int axb_int8_rope_append(void* qkv, void* q_out, void* k_codes, void* k_tops, void* v_codes, void* v_tops,
-                                    const int* page_table, const int* lengths, const int* live, const float* angle, int angle_rows,
-                                    int B, int T, int num_q_heads, int num_kv_heads, int head_dim, int page_size, int max_pages,
-                                    int num_pages, int* status, cudaStream_t stream) {
+extern "C" int axb_int8_rope_append(const axb::Int8RopeAppendCall* call, cudaStream_t stream) {
   using namespace axb;
-  const bool step = lengths != nullptr;
-  if (!int8_cache_fits(head_dim, page_size, num_kv_heads, num_pages, k_codes, v_codes) || num_q_heads < 1 || B < 0 || T < 0 ||
-      (step ? T != 1 || angle_rows < 1 : angle_rows < T))
+  const Int8RopeAppendCall& a = *call;
+  const bool step = a.lengths != nullptr;
+  if (!int8_cache_fits(a.head_dim, a.page_size, a.num_kv_heads, a.num_pages, a.k_codes, a.v_codes) || a.num_q_heads < 1 || a.B < 0 ||
+      a.T < 0 || !int8_ints({a.B, a.T, a.max_pages, a.num_q_heads}) || (step ? a.T != 1 || a.angle_rows < 1 : a.angle_rows < a.T))
     return -10;
-  if (B == 0 || T == 0) return 0;
-  if (step && q_out == nullptr) return -10;
-  for (const void* x : {static_cast<const void*>(qkv), static_cast<const void*>(q_out), static_cast<const void*>(angle)})
+  if (a.B == 0 || a.T == 0) return 0;
+  if (step && a.q_out == nullptr) return -10;
+  for (const void* x : {static_cast<const void*>(a.qkv), static_cast<const void*>(a.q_out), static_cast<const void*>(a.angle)})
     if (!aligned16(x)) return -10;
   Int8AppendParams p = {};
-  __nv_bfloat16* q = static_cast<__nv_bfloat16*>(qkv);
-  const int64_t t = static_cast<int64_t>(num_q_heads + 2 * num_kv_heads) * head_dim;
-  p.q = {q, T * t, t, head_dim};
-  p.k = {q + num_q_heads * head_dim, T * t, t, head_dim};
-  p.v = {p.k.x + num_kv_heads * head_dim, T * t, t, head_dim};
+  __nv_bfloat16* q = static_cast<__nv_bfloat16*>(a.qkv);
+  const int64_t t = (a.num_q_heads + 2 * a.num_kv_heads) * a.head_dim, h = a.head_dim;
+  p.q = {q, a.T * t, t, h};
+  p.k = {q + a.num_q_heads * h, a.T * t, t, h};
+  p.v = {p.k.x + a.num_kv_heads * h, a.T * t, t, h};
   if (step) {
-    p.q_out = static_cast<__nv_bfloat16*>(q_out);
-    p.q_out_b = p.q_out_t = static_cast<int64_t>(num_q_heads) * head_dim;
-    const int64_t capacity = static_cast<int64_t>(max_pages) * page_size;
-    p.limit = static_cast<int>(capacity < angle_rows ? capacity : angle_rows);
+    p.q_out = static_cast<__nv_bfloat16*>(a.q_out);
+    p.q_out_b = p.q_out_t = a.num_q_heads * h;
+    const int64_t capacity = a.max_pages * a.page_size, most = capacity < a.angle_rows ? capacity : a.angle_rows;
+    p.limit = static_cast<int>(most < 0x7fffffff ? most : 0x7fffffff);
   } else {
-    p.q_out = q, p.q_out_b = T * t, p.q_out_t = t;
-    p.k_out = q + num_q_heads * head_dim;
-    p.v_out = p.k_out + num_kv_heads * head_dim;
-    p.out_b = T * t, p.out_t = t, p.out_h = head_dim;
+    p.q_out = q, p.q_out_b = a.T * t, p.q_out_t = t;
+    p.k_out = q + a.num_q_heads * h;
+    p.v_out = p.k_out + a.num_kv_heads * h;
+    p.out_b = a.T * t, p.out_t = t, p.out_h = h;
   }
-  p.k_pool = {static_cast<uint8_t*>(k_codes), static_cast<__nv_bfloat16*>(k_tops)};
-  p.v_pool = {static_cast<uint8_t*>(v_codes), static_cast<__nv_bfloat16*>(v_tops)};
-  p.page_table = page_table, p.lengths = lengths, p.live = live, p.status = status;
-  p.angle = reinterpret_cast<const float2*>(angle);
-  p.T = T, p.num_q_heads = num_q_heads, p.num_kv_heads = num_kv_heads, p.max_pages = max_pages, p.num_pages = num_pages;
-  return int8_append(p, B, page_size, head_dim, stream);
+  p.k_pool = {static_cast<uint8_t*>(a.k_codes), static_cast<__nv_bfloat16*>(a.k_tops)};
+  p.v_pool = {static_cast<uint8_t*>(a.v_codes), static_cast<__nv_bfloat16*>(a.v_tops)};
+  p.page_table = a.page_table, p.lengths = a.lengths, p.live = a.live, p.status = a.status;
+  p.angle = reinterpret_cast<const float2*>(a.angle);
+  p.T = static_cast<int>(a.T), p.num_q_heads = static_cast<int>(a.num_q_heads), p.num_kv_heads = static_cast<int>(a.num_kv_heads);
+  p.max_pages = static_cast<int>(a.max_pages), p.num_pages = static_cast<int>(a.num_pages);
+  return int8_append(p, static_cast<int>(a.B), static_cast<int>(a.page_size), static_cast<int>(a.head_dim), stream);
 }
 
 // Scratch of axb_int8_decode_attn in floats: up to a cluster's splits meet without any.  More are a multiple of a cluster's.
@@ -752,28 +754,32 @@ extern "C" int64_t axb_int8_attn_scratch_floats(int B, int num_q_heads, int head
 
 // One new token a sequence: q [B, Nq, H] over the cache, into out [B, Nq, H] (which may be q).  `limit` (-1: none): sequences
 // behind it get zeros.
-extern "C" int axb_int8_decode_attn(const void* q, const void* k_codes, const void* k_tops, const void* v_codes, const void* v_tops,
-                                    const int* page_table, const int* lengths, void* out, float* scratch, int limit, int B,
-                                    int num_q_heads, int num_kv_heads, int head_dim, int page_size, int max_pages, int num_pages,
-                                    int splits, float softmax_scale, int* status, cudaStream_t stream) {
+extern "C" int axb_int8_decode_attn(const axb::Int8AttnCall* call, cudaStream_t stream) {
   using namespace axb;
-  if (!int8_cache_fits(head_dim, page_size, num_kv_heads, num_pages, k_codes, v_codes) || num_q_heads < 1 ||
-      num_q_heads % num_kv_heads || splits < 1 || B < 0 || B > 65535 || !(softmax_scale > 0.f && softmax_scale < 1048576.f) ||
-      !aligned16(q) || num_kv_heads * ((num_q_heads / num_kv_heads + kI8AttnRows - 1) / kI8AttnRows) > 65535)
+  const Int8AttnCall& a = *call;
+  if (!int8_cache_fits(a.head_dim, a.page_size, a.num_kv_heads, a.num_pages, a.k_codes, a.v_codes) || a.num_q_heads < 1 ||
+      a.num_q_heads % a.num_kv_heads || a.splits < 1 || a.B < 0 || a.B > 65535 || !int8_ints({a.num_q_heads, a.max_pages, a.splits}) ||
+      !(a.softmax_scale > 0. && a.softmax_scale < 1048576.) || !aligned16(a.q) ||
+      a.num_kv_heads * ((a.num_q_heads / a.num_kv_heads + kI8AttnRows - 1) / kI8AttnRows) > 65535)
     return -10;
-  if (B == 0) return 0;
-  if (splits > kI8AttnCluster && (scratch == nullptr || (reinterpret_cast<uintptr_t>(scratch) & 7) || splits % kI8AttnCluster)) return -10;
+  if (a.B == 0) return 0;
+  if (a.splits > kI8AttnCluster &&
+      (a.scratch == nullptr || (reinterpret_cast<uintptr_t>(a.scratch) & 7) || a.splits % kI8AttnCluster))
+    return -10;
   Int8AttnParams p = {};
-  p.q = static_cast<const __nv_bfloat16*>(q);
-  p.k_tops = static_cast<const __nv_bfloat16*>(k_tops), p.v_tops = static_cast<const __nv_bfloat16*>(v_tops);
-  p.page_table = page_table, p.lengths = lengths;
-  p.part_out = scratch;
-  p.part_ml = scratch == nullptr ? nullptr : scratch + static_cast<int64_t>(B) * num_q_heads * (splits / kI8AttnCluster) * head_dim;
-  p.out = static_cast<__nv_bfloat16*>(out);
-  p.status = status;
-  p.page = FastDiv(page_size);
-  p.num_q_heads = num_q_heads, p.num_kv_heads = num_kv_heads, p.max_pages = max_pages, p.num_pages = num_pages;
-  p.splits = splits, p.limit = limit;
-  p.scale_log2 = softmax_scale * (1.4426950408889634f / 127.f * kInt8Back);
-  return head_dim == 128 ? int8_attn<128>(k_codes, v_codes, p, B, stream) : int8_attn<64>(k_codes, v_codes, p, B, stream);
+  p.q = static_cast<const __nv_bfloat16*>(a.q);
+  p.k_tops = static_cast<const __nv_bfloat16*>(a.k_tops), p.v_tops = static_cast<const __nv_bfloat16*>(a.v_tops);
+  p.page_table = a.page_table, p.lengths = a.lengths;
+  p.part_out = a.scratch;
+  p.part_ml = a.scratch == nullptr ? nullptr : a.scratch + a.B * a.num_q_heads * (a.splits / kI8AttnCluster) * a.head_dim;
+  p.out = static_cast<__nv_bfloat16*>(a.out);
+  p.status = a.status;
+  p.page = FastDiv(static_cast<int>(a.page_size));
+  p.num_q_heads = static_cast<int>(a.num_q_heads), p.num_kv_heads = static_cast<int>(a.num_kv_heads);
+  p.max_pages = static_cast<int>(a.max_pages), p.num_pages = static_cast<int>(a.num_pages);
+  p.splits = static_cast<int>(a.splits);
+  p.limit = static_cast<int>(a.limit < 0 ? -1 : a.limit < 0x7fffffff ? a.limit : 0x7fffffff);
+  p.scale_log2 = static_cast<float>(a.softmax_scale) * (1.4426950408889634f / 127.f * kInt8Back);
+  const int B = static_cast<int>(a.B);
+  return a.head_dim == 128 ? int8_attn<128>(a.k_codes, a.v_codes, p, B, stream) : int8_attn<64>(a.k_codes, a.v_codes, p, B, stream);
 }

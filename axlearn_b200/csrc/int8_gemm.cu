@@ -5,24 +5,28 @@
 // features, 128 values of K a stage; one thread of the first CTA issues `tcgen05.mma.cta_group::2.kind::i8`; both drain their
 // 128 rows: a thread owns a row of x, so its scale is one register, and the features' scales are loads that a warp shares.
 // The next tile runs into the other half of tensor memory meanwhile.
+#include "chain.cuh"
 #include "cta_pair.cuh"
 #include "host_utils.cuh"
+#include "int8.cuh"
 #include "opt_in.cuh"
 #include "sm100.cuh"
 
 namespace axb {
 
 constexpr int kI8Rows = 128, kI8K = 128;  // rows of x a CTA, values of K a stage
-constexpr int kI8Threads = 192;           // producer, issuer, four epilogue warps
+constexpr int kI8Epilogue = 8;            // warps: two for each quarter of the rows, one for either half of the features
+constexpr int kI8Threads = 32 * (2 + kI8Epilogue);  // + producer, issuer
 
 template <int TN>  // features of a tile
 struct Int8PairCfg {
   static constexpr int kHalf = TN / 2;
   static constexpr int kABytes = kI8Rows * kI8K, kBBytes = kHalf * kI8K, kStageBytes = kABytes + kBBytes;
   static constexpr int kStages = TN == 256 ? 6 : 8;
-  static constexpr int kStagingPerWarp = 2 * 4096;  // two tiles of 32 rows x 64 features
-  static constexpr int kRingBytes = kStages * kStageBytes, kStagingBytes = 4 * kStagingPerWarp;
-  static constexpr int kSmem = kRingBytes + kStagingBytes + 512 + 1024;  // barriers, alignment slack
+  static constexpr int kStagingPerWarp = 4096;  // 32 rows x 64 features
+  static constexpr int kRingBytes = kStages * kStageBytes, kStagingBytes = kI8Epilogue * kStagingPerWarp;
+  static constexpr int kScaleBytes = TN * 4;  // of the features
+  static constexpr int kSmem = kRingBytes + kStagingBytes + kScaleBytes + 512 + 1024;  // barriers, alignment slack
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
@@ -47,7 +51,8 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   uint8_t* staging = smem + S::kRingBytes;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(staging + S::kStagingBytes);
+  float* feature_scales = reinterpret_cast<float*>(staging + S::kStagingBytes);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(staging + S::kStagingBytes + S::kScaleBytes);
   uint64_t* empty_bar = full_bar + kStages;
   uint64_t* tmem_full = empty_bar + kStages;
   uint64_t* tmem_empty = tmem_full + 2;
@@ -71,7 +76,7 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tmem_full[a], 1);
-      mbar_init(&tmem_empty[a], 8);  // four epilogue warps in each CTA of the pair
+      mbar_init(&tmem_empty[a], 2 * kI8Epilogue);  // the epilogue warps of both CTAs
     }
     fence_barrier_init();
     fence_proxy_async();
@@ -164,39 +169,40 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
       }
     }
   } else {
-    const int quarter = warp & 3;  // tensor-memory lanes [32 * quarter, +32) belong to this warp
-    uint8_t* my_staging = staging + quarter * S::kStagingPerWarp;
+    const int quarter = warp & 3, side = (warp - 2) >> 2;  // tensor-memory lanes [32 * quarter, +32), either half of the columns
+    const int thread = threadIdx.x - 64;
+    uint8_t* tile = staging + (warp - 2) * S::kStagingPerWarp;
     const uint32_t empty_addr = map_to_cta(smem_u32(&tmem_empty[0]), 0);
     int acc = 0;
-    uint32_t acc_phase = 0, store_seq = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
     for (int t = pair; t < num_tiles; t += num_pairs) {
       int m_blk, n_blk;
       tile_at(t, m_blk, n_blk);
       const int row0 = m_blk * 2 * kI8Rows + static_cast<int>(rank) * kI8Rows + quarter * 32, n0 = n_blk * TN;
       const bool inside = row0 + lane < p.M;
       const float xs = inside ? p.x_scales[row0 + lane] : 0.f;
-      if (!mbar_wait_warp_relaxed(&tmem_full[acc], acc_phase, p.status, kStatusWaitTimeoutEpilogue)) break;
+      // (All epilogue warps pass these barriers for every tile, also behind a wait that gave up.)
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * kI8Epilogue) : "memory");  // the tile before has been multiplied by its scales
+      if (thread < TN && n0 + thread < p.N) feature_scales[thread] = p.w_scales[n0 + thread];
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * kI8Epilogue) : "memory");
+      if (ok) ok = mbar_wait_warp_relaxed(&tmem_full[acc], acc_phase, p.status, kStatusWaitTimeoutEpilogue);
+      if (!ok) continue;
       tc_fence_after_sync();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * TN;
 #pragma unroll 1
-      for (int ch = 0; ch < TN / 64; ++ch) {
+      for (int ch = side * (TN / 128); ch < (side + 1) * (TN / 128); ++ch) {
         const int n = n0 + ch * 64;
-        // The staging tile about to be written was read by the store issued two chunks ago.
-        if (lane == 0) tma_store_wait_read<1>();
+        // The staging tile was read by the store issued a chunk ago.
+        if (lane == 0) tma_store_wait_read<0>();
         __syncwarp();
-        uint8_t* tile = my_staging + (store_seq & 1) * 4096;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           uint32_t r[32];
           tmem_ld_32x32(taddr + ch * 64 + half * 32, r);
-          float4 ws[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int at = n + half * 32 + j * 4;
-            ws[j] = at < p.N ? *reinterpret_cast<const float4*>(p.w_scales + at) : make_float4(0.f, 0.f, 0.f, 0.f);
-          }
+          const float4* ws = reinterpret_cast<const float4*>(feature_scales + ch * 64 + half * 32);
           tmem_ld_wait();
-          if (ch == TN / 64 - 1 && half == 1) {
+          if (ch == (side + 1) * (TN / 128) - 1 && half == 1) {
             // All of this warp's reads of the accumulator are done: hand it back early.
             tc_fence_before_sync();
             __syncwarp();
@@ -207,7 +213,7 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
             float f[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              const float4& w4 = ws[2 * v + (i >> 2)];
+              const float4 w4 = ws[2 * v + (i >> 2)];
               const float w = (i & 3) == 0 ? w4.x : (i & 3) == 1 ? w4.y : (i & 3) == 2 ? w4.z : w4.w;
               f[i] = __int2float_rn(static_cast<int>(r[8 * v + i])) * xs * w;
             }
@@ -231,7 +237,6 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
           if (row0 < p.M && n < p.N) tma_store_2d(&map_y, tile, n, row0);
           tma_store_commit();
         }
-        ++store_seq;
       }
       if (++acc == 2) {
         acc = 0;
@@ -280,19 +285,42 @@ static int launch_int8_pair(const void* x, const void* w, int64_t ldx, int64_t l
 
 }  // namespace axb
 
-// x [M, K] and w [N, K] along K with pitches that are multiples of 16; y in bf16 with a pitch that is a multiple of 8; the scales
-// 16-byte aligned; N a multiple of 8, K at most 2^17.  `features`: of a tile, 256 or 128.  -10: not supported.
-extern "C" int axb_int8_gemm(const void* x, const float* x_scales, const void* w, const float* w_scales, void* y, int M, int N, int K,
-                             int64_t ldx, int64_t ldw, int64_t ldy, int accumulate, int features, int* status,
-                             cudaStream_t stream) {
+// y[M, N] of x [M, K] and w [N, K], all one row behind the other and 16-byte aligned; N a multiple of 8, K one of 16 and at most
+// 2^17.  `plan`: features of a tile, 256 or 128.  -10: not supported.
+extern "C" int axb_int8_gemm(const axb::Int8LinearCall* call, cudaStream_t stream) {
   using namespace axb;
-  if (M <= 0 || N <= 0) return 0;
-  if (K < 1 || K > (1 << 17) || N % 8 || ldx % 16 || ldw % 16 || ldy % 8 || (features != 256 && features != 128) || M > 0x40000000 ||
-      N > 0x40000000)
+  const Int8LinearCall& a = *call;
+  if (a.M <= 0 || a.N <= 0) return 0;
+  if (a.K < 16 || a.K > (1 << 17) || a.K % 16 || a.N % 8 || (a.plan != 256 && a.plan != 128) || a.M > 0x40000000 || a.N > 0x40000000)
     return -10;
-  for (const void* a : {x, w, static_cast<const void*>(y), static_cast<const void*>(w_scales)})
-    if (reinterpret_cast<uintptr_t>(a) & 15) return -10;
-  if (static_cast<int64_t>((M + 255) / 256) * ((N + features - 1) / features) > 0x7fffff00) return -10;
-  const Int8GemmParams p{M, N, K, accumulate, x_scales, w_scales, static_cast<__nv_bfloat16*>(y), ldy, status, 8};
-  return features == 256 ? launch_int8_pair<256>(x, w, ldx, ldw, p, stream) : launch_int8_pair<128>(x, w, ldx, ldw, p, stream);
+  for (const void* x : {a.x, a.w, static_cast<const void*>(a.y), static_cast<const void*>(a.w_scales)})
+    if (reinterpret_cast<uintptr_t>(x) & 15) return -10;
+  if ((a.M + 255) / 256 * ((a.N + a.plan - 1) / a.plan) > 0x7fffff00) return -10;
+  const Int8GemmParams p{static_cast<int>(a.M), static_cast<int>(a.N), static_cast<int>(a.K), a.accumulate != 0,
+                         a.x_scales, a.w_scales, static_cast<__nv_bfloat16*>(a.y), a.N, a.status, 8};
+  return a.plan == 256 ? launch_int8_pair<256>(a.x, a.w, a.K, a.K, p, stream) : launch_int8_pair<128>(a.x, a.w, a.K, a.K, p, stream);
+}
+
+// y of x [M, K] in bf16 (pitch ldx), whose rows are quantised first.  The product of few rows is put on the GPU behind that at once:
+// its stages fill with the weight, which was there before the rows' kernel started, while that still runs (16 x 14336 x 4096:
+// %FIG%).
+extern "C" int axb_int8_dense(const axb::Int8DenseCall* call, cudaStream_t stream) {
+  using namespace axb;
+  const Int8DenseCall& a = *call;
+  if (a.M <= 0 || a.N <= 0) return 0;
+  if (a.K < 16 || a.K % 16 || a.K > (1 << 17)) return -10;
+  int8_t* codes = static_cast<int8_t*>(a.held);
+  float* scales = reinterpret_cast<float*>(codes + a.M * a.K);
+  const Int8RowsCall rows{a.x, codes, scales, a.M, a.K, a.ldx, 0};
+  const int rc = axb_int8_rows(&rows, stream);
+  if (rc != 0) return rc;
+  const Int8LinearCall product{codes, scales, a.w, a.w_scales, a.y, a.M, a.N, a.K, a.accumulate, a.features, 1, a.status};
+  if (a.features != 0) return axb_int8_gemm(&product, stream);
+  if (chain_launches && !a.resident) {
+    Int8LinearCall plain = product;
+    plain.resident = 0;
+    return axb_gemm_skinny_int8(&plain, stream);
+  }
+  ChainedBehind chained;
+  return axb_gemm_skinny_int8(&product, stream);
 }

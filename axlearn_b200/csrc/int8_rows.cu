@@ -129,7 +129,7 @@ static int int8_rows(const Int8RowsParams& p, int64_t rows, cudaStream_t stream)
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
-static bool int8_rows_fit(int64_t rows, int dim, int64_t ldx) {
+static bool int8_rows_fit(int64_t rows, int64_t dim, int64_t ldx) {
   return rows >= 0 && rows <= 0x7fffffff && dim >= 8 && dim % 8 == 0 && dim <= kInt8RowsMost && ldx % 8 == 0;
 }
 
@@ -137,34 +137,34 @@ static bool int8_rows_fit(int64_t rows, int dim, int64_t ldx) {
 
 // codes [rows, dim], scales [rows] of x [rows, dim] with a pitch of ldx; `gated`: of silu(x[:, :dim]) * x[:, dim:].  All pointers
 // 16-byte aligned; -10: not supported.
-extern "C" int axb_int8_rows(const void* x, void* codes, float* scales, int64_t rows, int dim, int64_t ldx, int gated,
-                             cudaStream_t stream) {
+extern "C" int axb_int8_rows(const axb::Int8RowsCall* call, cudaStream_t stream) {
   using namespace axb;
-  if (!int8_rows_fit(rows, dim, ldx)) return -10;
-  for (const void* a : {x, static_cast<const void*>(codes)})
-    if (reinterpret_cast<uintptr_t>(a) & 15) return -10;
-  if (rows == 0) return 0;
+  const Int8RowsCall& a = *call;
+  if (!int8_rows_fit(a.rows, a.dim, a.ldx)) return -10;
+  for (const void* x : {a.x, static_cast<const void*>(a.codes)})
+    if (reinterpret_cast<uintptr_t>(x) & 15) return -10;
+  if (a.rows == 0) return 0;
   Int8RowsParams p = {};
-  p.x = static_cast<const __nv_bfloat16*>(x);
-  p.ldx = ldx, p.codes = static_cast<int8_t*>(codes), p.scales = scales, p.dim = dim;
-  return gated ? int8_rows<kRowsSwiglu>(p, rows, stream) : int8_rows<kRowsPlain>(p, rows, stream);
+  p.x = static_cast<const __nv_bfloat16*>(a.x);
+  p.ldx = a.ldx, p.codes = static_cast<int8_t*>(a.codes), p.scales = a.scales, p.dim = static_cast<int>(a.dim);
+  return a.gated ? int8_rows<kRowsSwiglu>(p, a.rows, stream) : int8_rows<kRowsPlain>(p, a.rows, stream);
 }
 
 // t = x + residual in bf16 (x without one), into `total`; codes and scales of t rsqrt(mean t^2 + eps) weight, and what they stand
 // for into `values` (null: not wanted).  Rows of `dim` values one behind the other, 16-byte aligned.
-extern "C" int axb_int8_add_rms_norm(const void* x, const void* residual, const void* weight, void* total, void* codes,
-                                     float* scales, void* values, int64_t rows, int dim, float eps, cudaStream_t stream) {
+extern "C" int axb_int8_add_rms_norm(const axb::Int8NormCall* call, cudaStream_t stream) {
   using namespace axb;
-  if (!int8_rows_fit(rows, dim, dim) || (residual != nullptr && total == nullptr)) return -10;
-  for (const void* a : {x, residual, weight, static_cast<const void*>(total), static_cast<const void*>(codes),
-                        static_cast<const void*>(values)})
-    if (reinterpret_cast<uintptr_t>(a) & 15) return -10;
-  if (rows == 0) return 0;
+  const Int8NormCall& a = *call;
+  if (!int8_rows_fit(a.rows, a.dim, a.dim) || (a.residual != nullptr && a.total == nullptr)) return -10;
+  for (const void* x : {a.x, a.residual, a.weight, static_cast<const void*>(a.total), static_cast<const void*>(a.codes),
+                        static_cast<const void*>(a.values)})
+    if (reinterpret_cast<uintptr_t>(x) & 15) return -10;
+  if (a.rows == 0) return 0;
   Int8RowsParams p = {};
-  p.x = static_cast<const __nv_bfloat16*>(x), p.other = static_cast<const __nv_bfloat16*>(residual);
-  p.weight = static_cast<const __nv_bfloat16*>(weight);
-  p.codes = static_cast<int8_t*>(codes), p.scales = scales;
-  p.total = static_cast<__nv_bfloat16*>(total), p.values = static_cast<__nv_bfloat16*>(values);
-  p.dim = dim, p.eps = eps;
-  return int8_rows<kRowsNorm>(p, rows, stream);
+  p.x = static_cast<const __nv_bfloat16*>(a.x), p.other = static_cast<const __nv_bfloat16*>(a.residual);
+  p.weight = static_cast<const __nv_bfloat16*>(a.weight);
+  p.codes = static_cast<int8_t*>(a.codes), p.scales = a.scales;
+  p.total = static_cast<__nv_bfloat16*>(a.total), p.values = static_cast<__nv_bfloat16*>(a.values);
+  p.dim = static_cast<int>(a.dim), p.eps = static_cast<float>(a.eps);
+  return int8_rows<kRowsNorm>(p, a.rows, stream);
 }

@@ -127,6 +127,11 @@ def _stream() -> int:
     return _raw_stream(_device_index())
 
 
+def current_device() -> int:
+    """Index of the current device, without the checks of its initialisation (operands on a GPU have made them)."""
+    return torch.cuda.current_device() if _device_index is None else _device_index()
+
+
 def _transformed() -> bool:
     """Whether forward-mode differentiation or a function transform is on, which know torch's operators but not a kernel
     behind their back; unknown counts as on."""

@@ -25,8 +25,8 @@ the pool does not have, a position behind a table) are not touched: on the GPU t
 from __future__ import annotations
 
 import ctypes
-import dataclasses
 import math
+import struct
 from typing import NamedTuple, Optional, Union
 
 import torch
@@ -34,7 +34,6 @@ import torch
 from axlearn_b200.ops import cuda_ops, dispatch
 from axlearn_b200.ops.int4_ops import (
     _aligned_rows,
-    _check_counts,
     _no_gradient,
     _on,
     _on_kernel,
@@ -45,43 +44,43 @@ from axlearn_b200.ops.int4_ops import (
     _split_qkv,
 )
 
-c_void_p, c_int, c_int64, c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
 Tensor = torch.Tensor
 
 LEAST = 2.0 ** -119
 MAX_ROW = 65536        # values of a row that the row kernels keep
 MAX_K = 1 << 17        # products of 127 x 127 whose sums fit 32 bits
 PAGE_UNIT = 16         # tokens of a page are a multiple of
-_configured = False
+# Entry points and the 64-bit words of their arguments (``csrc/int8.cuh``).
+_WORDS = {"axb_int8_rows": "7q", "axb_int8_add_rms_norm": "9qd", "axb_gemm_skinny_int8": "12q", "axb_int8_gemm": "12q",
+          "axb_int8_dense": "13q",
+          "axb_int8_append": "25q", "axb_int8_rope_append": "20q", "axb_int8_decode_attn": "18qdq"}
+_entries: dict = {}
 
 
-def _lib():
-    global _configured
+def _entry(name: str) -> tuple:
     h = cuda_ops.lib()
-    if not _configured:
-        h.axb_int8_rows.argtypes = [c_void_p] * 3 + [c_int64, c_int, c_int64, c_int, c_void_p]
-        h.axb_int8_add_rms_norm.argtypes = [c_void_p] * 7 + [c_int64, c_int, c_float, c_void_p]
-        h.axb_gemm_skinny_int8.argtypes = [c_void_p] * 5 + [c_int] * 3 + [c_int64] * 3 + [c_int] * 3 + [c_void_p] * 2
-        h.axb_int8_gemm.argtypes = [c_void_p] * 5 + [c_int] * 3 + [c_int64] * 3 + [c_int] * 2 + [c_void_p] * 2
-        h.axb_int8_append.argtypes = [c_void_p] * 2 + [c_int64] * 6 + [c_void_p] * 9 + [c_int] * 7 + [c_void_p] * 2
-        h.axb_int8_rope_append.argtypes = [c_void_p] * 10 + [c_int] * 9 + [c_void_p] * 2
-        h.axb_int8_decode_attn.argtypes = [c_void_p] * 9 + [c_int] * 9 + [c_float, c_void_p, c_void_p]
-        h.axb_int8_attn_scratch_floats.argtypes = [c_int] * 4
-        h.axb_int8_attn_scratch_floats.restype = c_int64
-        for f in (h.axb_int8_rows, h.axb_int8_add_rms_norm, h.axb_gemm_skinny_int8, h.axb_int8_gemm, h.axb_int8_append,
-                  h.axb_int8_rope_append, h.axb_int8_decode_attn):
-            f.restype = c_int
-        _configured = True
-    return h
+    if name == "axb_int8_attn_scratch_floats":
+        f, pack = h.axb_int8_attn_scratch_floats, None
+        f.argtypes, f.restype = [ctypes.c_int] * 4, ctypes.c_int64
+    else:
+        f, pack = getattr(h, name), struct.Struct(_WORDS[name]).pack
+        f.argtypes, f.restype = [ctypes.c_char_p, ctypes.c_void_p], ctypes.c_int
+    _entries[name] = f, pack
+    return f, pack
 
 
-def _call(device: torch.device, name: str, *args) -> None:
-    """Launches on the device of the operands, on its current stream."""
-    if device.index != torch.cuda.current_device():
+def _call(device: int, name: str, *words) -> None:
+    """Launches on the device of the operands (its index), on its current stream."""
+    if device != cuda_ops.current_device():
         with torch.cuda.device(device):
-            return _call(device, name, *args)
-    rc = getattr(_lib(), name)(*args, cuda_ops._stream())  # pylint: disable=protected-access
-    return cuda_ops._check(rc, name)  # pylint: disable=protected-access
+            return _call(device, name, *words)
+    f, pack = _entries.get(name) or _entry(name)
+    return cuda_ops._check(f(pack(*words), cuda_ops._stream()), name)  # pylint: disable=protected-access
+
+
+def _status(device: int) -> int:
+    word = cuda_ops._status.get(device)  # pylint: disable=protected-access
+    return (cuda_ops.status_word(torch.device("cuda", device)) if word is None else word).data_ptr()
 
 
 # ------------------------------------------------------------------------------------------
@@ -155,12 +154,12 @@ def swiglu_int8(gu: Tensor) -> Int8Rows:
 
 
 def _launch_rows(x: Tensor, dim: int, gated: bool) -> Int8Rows:
-    shape, device = x.shape[:-1], x.device
-    codes = torch.empty(shape + (dim,), dtype=torch.int8, device=device)
-    scales = torch.empty(shape, dtype=torch.float32, device=device)
+    shape = x.shape[:-1]
+    codes = torch.empty(shape + (dim,), dtype=torch.int8, device=x.device)
+    scales = torch.empty(shape, dtype=torch.float32, device=x.device)
     if codes.numel():
         x, rows, pitch = _row_operand(x, x.shape[-1])
-        _call(device, "axb_int8_rows", x.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, dim, pitch, 1 if gated else 0)
+        _call(x.get_device(), "axb_int8_rows", x.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, dim, pitch, gated)
     return Int8Rows(codes, scales)
 
 
@@ -175,7 +174,8 @@ def add_rms_norm_int8(x: Tensor, residual: Optional[Tensor], scale: Tensor, eps:
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
         raise ValueError(f"residual {tuple(residual.shape)} {residual.dtype} for x {tuple(x.shape)} {x.dtype}")
     _no_gradient("add_rms_norm_int8", x, residual, scale)
-    scale = scale.to(x.dtype)
+    if scale.dtype != x.dtype:
+        scale = scale.to(x.dtype)
     if not _on_kernel(x):
         total = x if residual is None else x + residual
         t = total.float()
@@ -183,26 +183,27 @@ def add_rms_norm_int8(x: Tensor, residual: Optional[Tensor], scale: Tensor, eps:
         top = _tops(y.abs().amax(-1, keepdim=True))
         rows = Int8Rows(_codes(y, top), (top / 127.0 * torch.rsqrt(t.square().mean(-1, keepdim=True) + eps))[..., 0])
         return (rows, total, row_values(rows, x.dtype)) if values else (rows, total)
-    device, shape = x.device, x.shape[:-1]
     x, n, pitch = _row_operand(x, d)
     if pitch != d:
         x = x.contiguous()
-    total = x
+    total, other = x, 0
     if residual is not None:
-        residual = residual.contiguous()
-        if residual.data_ptr() % 16:
-            residual = residual.clone()
-        total = torch.empty_like(x)
-    scale = scale.contiguous()
-    if scale.data_ptr() % 16:
-        scale = scale.clone()
-    rows = Int8Rows(torch.empty(x.shape, dtype=torch.int8, device=device), torch.empty(shape, dtype=torch.float32, device=device))
+        residual = _aligned(residual)
+        total, other = torch.empty_like(x), residual.data_ptr()
+    scale = _aligned(scale)
+    rows = Int8Rows(torch.empty_like(x, dtype=torch.int8), torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device))
     held = torch.empty_like(x) if values else None
     if n:
-        _call(device, "axb_int8_add_rms_norm", x.data_ptr(), None if residual is None else residual.data_ptr(), scale.data_ptr(),
-              None if residual is None else total.data_ptr(), rows.codes.data_ptr(), rows.scales.data_ptr(),
-              None if held is None else held.data_ptr(), n, d, eps)
+        _call(x.get_device(), "axb_int8_add_rms_norm", x.data_ptr(), other, scale.data_ptr(), total.data_ptr() if other else 0,
+              rows.codes.data_ptr(), rows.scales.data_ptr(), held.data_ptr() if values else 0, n, d, eps)
     return (rows, total, held) if values else (rows, total)
+
+
+def _aligned(x: Tensor) -> Tensor:
+    """``x`` as a contiguous tensor at a multiple of 16 bytes."""
+    if not x.is_contiguous() or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
 
 
 # ------------------------------------------------------------------------------------------
@@ -210,26 +211,21 @@ def add_rms_norm_int8(x: Tensor, residual: Optional[Tensor], scale: Tensor, eps:
 # ------------------------------------------------------------------------------------------
 
 
-@dataclasses.dataclass(frozen=True)
 class Int8Weight:
     """A matrix ``[K, N]`` in 8 bits: ``codes [N, K]`` (int8), a block for each of its columns, and ``scales [N]`` (fp32)."""
 
-    codes: Tensor
-    scales: Tensor
+    __slots__ = ("codes", "scales", "shape")
 
-    def __post_init__(self):
-        codes, scales = self.codes, self.scales
-        if (codes.dim() != 2 or codes.dtype != torch.int8 or scales.dtype != torch.float32 or scales.shape != codes.shape[:1]
-                or codes.device != scales.device or not codes.is_contiguous() or not scales.is_contiguous()):
-            raise ValueError(f"codes {tuple(codes.shape)} {codes.dtype} and scales {tuple(scales.shape)} {scales.dtype} are not "
-                             "those of an 8-bit weight: contiguous [N, K] int8 and [N] fp32")
-        n, k = codes.shape
+    def __init__(self, codes: Tensor, scales: Tensor):
+        shape = codes.shape
+        if (len(shape) != 2 or codes.dtype is not torch.int8 or scales.dtype is not torch.float32 or scales.shape != shape[:1]
+                or codes.get_device() != scales.get_device() or not codes.is_contiguous() or not scales.is_contiguous()):
+            raise ValueError(f"codes {tuple(shape)} {codes.dtype} and scales {tuple(scales.shape)} {scales.dtype} are not those of an "
+                             "8-bit weight: contiguous [N, K] int8 and [N] fp32")
+        n, k = shape
         if k < 16 or k % 16 or k > MAX_K or n < 8 or n % 8:
             raise ValueError(f"an 8-bit weight [{k}, {n}] has rows in sixteens up to {MAX_K} and columns in eights")
-
-    @property
-    def shape(self) -> tuple[int, int]:
-        return self.codes.shape[1], self.codes.shape[0]
+        self.codes, self.scales, self.shape = codes, scales, (k, n)
 
 
 def quantize_weight(w: Tensor) -> Int8Weight:
@@ -245,9 +241,20 @@ def dequantize_weight(w: Int8Weight, dtype: torch.dtype = torch.bfloat16) -> Ten
     return (w.codes.float() * w.scales[:, None]).to(dtype).t()
 
 
-def pair_features(rows: int, n: int) -> int:
-    """Features of a tile of 256 rows: 256, or 128 where those of 256 would leave most pairs of SMs without one."""
-    return 128 if -(-rows // 256) * -(-n // 256) <= 37 else 256
+def pair_features(rows: int, n: int, sms: int = 148) -> int:
+    """Features of a tile of 256 rows: 256, or 128 where that is fewer waves' time: a tile of 128 takes 0.62 of one of 256 (us
+    with 128 / 256, rows x K x N: 256 x 2048 x 8192 9.9 / 12.5, 300 x 4096 x 12288 23.4 / 25.8, 333 x 2048 x 8192 12.8 / 12.6, 1024
+    x 4096 x 4096 17.7 / 17.1, 8192 x 4096 x 4096 103 / 89)."""
+    blocks, pairs = -(-rows // 256), sms // 2
+    wide, narrow = -(-blocks * -(-n // 256) // pairs), -(-blocks * -(-n // 128) // pairs)
+    return 128 if 5 * narrow < 8 * wide else 256
+
+
+def few_rows(rows: int, k: int, n: int, sms: int = 148) -> bool:
+    """Whether a product streams the weight past all rows, in slices of K where columns are few: up to 128 rows, and up to 96 where K is
+    short and tiles of 256 rows by 128 columns are one wave (us so / in tiles: 96 x 4096 x 4096 11.9 / 11.6, 128 rows of it 13.5 /
+    11.6, 128 x 4096 x 12288 15.9 / 18.7, 128 x 14336 x 4096 19.7 / 24.6)."""
+    return rows <= 96 or (rows <= 128 and (k > 4096 or -(-n // 128) > sms // 2))
 
 
 def int8_linear(x: Union[Tensor, Int8Rows], w: Int8Weight, *, out: Optional[Tensor] = None, accumulate: bool = False,
@@ -257,13 +264,14 @@ def int8_linear(x: Union[Tensor, Int8Rows], w: Int8Weight, *, out: Optional[Tens
     it ahead of that rounding.  ``out`` may overlap ``x``.  ``resident``: as in ``cuda_ops.gemm``.  Serving only: there is no gradient."""
     k, n = w.shape
     held = isinstance(x, Int8Rows)
-    codes = x.codes if held else x
-    device = codes.device
-    if codes.shape[-1:] != (k,) or device != w.codes.device:
-        raise ValueError(f"x {tuple(codes.shape)} on {device} and a {w.shape} weight on {w.codes.device}")
-    shape = codes.shape[:-1] + (n,)
+    codes, w_codes = x.codes if held else x, w.codes
+    shape, device = codes.shape, codes.get_device()
+    if shape[-1:] != (k,) or device != w_codes.get_device():
+        raise ValueError(f"x {tuple(shape)} on {codes.device} and a {w.shape} weight on {w_codes.device}")
+    shape = shape[:-1] + (n,)
     if held:
-        if codes.dtype != torch.int8 or x.scales.shape != codes.shape[:-1] or x.scales.dtype != torch.float32 or x.scales.device != device:
+        if (codes.dtype is not torch.int8 or x.scales.shape != shape[:-1] or x.scales.dtype is not torch.float32
+                or x.scales.get_device() != device):
             raise ValueError(f"rows in 8 bits are int8 codes and an fp32 scale for each: {codes.dtype}, {tuple(x.scales.shape)} "
                              f"{x.scales.dtype}")
         dtype = dtype or (torch.bfloat16 if out is None else out.dtype)
@@ -274,38 +282,39 @@ def int8_linear(x: Union[Tensor, Int8Rows], w: Int8Weight, *, out: Optional[Tens
     if not given:
         if accumulate:
             raise ValueError("accumulate needs out")
-        out = torch.empty(shape, dtype=dtype, device=device)
-    elif out.shape != shape or out.dtype != dtype or out.device != device or not out.is_contiguous():
+        out = torch.empty(shape, dtype=dtype, device=codes.device)
+    elif out.shape != shape or out.dtype != dtype or out.get_device() != device or not out.is_contiguous():
         raise ValueError(f"out {tuple(out.shape)} {out.dtype}: contiguous {tuple(shape)} {dtype} is wanted")
-    if not held:
-        x = quantize_rows(x)
-    if not _on_kernel(out):
+    w_scales = w.scales
+    if not _on_kernel(out) or (not held and x.dtype is not torch.bfloat16):
+        codes, scales = x if held else quantize_rows(x)
         # (Products of codes and their sums are whole numbers below 2^53.)
-        sums = (x.codes.double() @ w.codes.double().t()).float()
-        y = sums * x.scales[..., None] * w.scales
+        sums = (codes.double() @ w_codes.double().t()).float()
+        y = sums * scales[..., None] * w_scales
         return out.copy_(out.float() + y if accumulate else y)
     rows = out.numel() // n
     if rows == 0:
         return out
-    codes, scales, w_scales = x.codes, x.scales, w.scales
+    if w_codes.data_ptr() % 16 or w_scales.data_ptr() % 16:
+        w_codes, w_scales, resident = w_codes.clone(), w_scales.clone(), False
+    few, y = few_rows(rows, k, n), out
+    if not few and out.data_ptr() % 16:  # a view into a larger buffer: tiles are stored as vectors
+        y = out.clone() if accumulate else torch.empty_like(out)
     if held:
-        if not codes.is_contiguous() or codes.data_ptr() % 16 or (given and _overlap(codes, out)):
+        codes, scales = x
+        if given and _overlap(codes, out):  # other columns' products still read x
             codes = codes.clone(memory_format=torch.contiguous_format)
         if not scales.is_contiguous() or (given and _overlap(scales, out)):
             scales = scales.clone(memory_format=torch.contiguous_format)
-    if w.codes.data_ptr() % 16 or w_scales.data_ptr() % 16:
-        w = Int8Weight(w.codes.clone(), w_scales.clone())
-        w_scales, resident = w.scales, False
-    word = cuda_ops.status_word(device).data_ptr()
-    if rows <= 128:
-        _call(device, "axb_gemm_skinny_int8", codes.data_ptr(), scales.data_ptr(), w.codes.data_ptr(), w_scales.data_ptr(),
-              out.data_ptr(), rows, n, k, k, k, n, 1 if accumulate else 0, 0, 1 if resident else 0, word)
-        return out
-    y = out
-    if out.data_ptr() % 16:  # a view into a larger buffer: tiles are stored as vectors
-        y = out.clone() if accumulate else torch.empty_like(out)
-    _call(device, "axb_int8_gemm", codes.data_ptr(), scales.data_ptr(), w.codes.data_ptr(), w_scales.data_ptr(), y.data_ptr(), rows,
-          n, k, k, k, n, 1 if accumulate else 0, pair_features(rows, n), word)
+        codes = _aligned(codes)
+        _call(device, "axb_gemm_skinny_int8" if few else "axb_int8_gemm", codes.data_ptr(), scales.data_ptr(), w_codes.data_ptr(),
+              w_scales.data_ptr(), y.data_ptr(), rows, n, k, accumulate, 0 if few else pair_features(rows, n), resident, _status(device))
+    else:
+        _check_row(k)
+        x, _, pitch = _row_operand(x, k)
+        room = torch.empty(rows * (k + 4), dtype=torch.uint8, device=x.device)  # codes, then scales
+        _call(device, "axb_int8_dense", x.data_ptr(), pitch, room.data_ptr(), w_codes.data_ptr(), w_scales.data_ptr(), y.data_ptr(), rows, n,
+              k, accumulate, 0 if few else pair_features(rows, n), resident, _status(device))
     return out if y is out else out.copy_(y)
 
 
@@ -338,26 +347,34 @@ def page_values(pages: Int8Pages, dtype: torch.dtype = torch.float32) -> Tensor:
 
 
 def _check_pages(k_pages: Int8Pages, v_pages: Int8Pages, page_table: Tensor, batch: int, heads: int, head_dim: int,
-                 device: torch.device) -> tuple:
-    """``(pages, Nkv, page size)`` of a cache that fits."""
+                 device: int) -> tuple:
+    """``(pages, Nkv, page size, columns of the table)`` of a cache that fits; ``device``: index of the operands' one."""
     (kc, kt), (vc, vt) = k_pages, v_pages
     shape = kc.shape
     num_pages, nkv, page_size, held = shape if len(shape) == 4 else (0, 0, 0, 0)
+    tops = (num_pages, nkv)
     if (held != head_dim or head_dim not in (64, 128) or not nkv or heads % nkv or not num_pages or not page_size
-            or page_size % PAGE_UNIT or vc.shape != shape or kt.shape != (num_pages, nkv) or vt.shape != kt.shape):
+            or page_size % PAGE_UNIT or vc.shape != shape or kt.shape != tops or vt.shape != tops):
         raise ValueError(f"8-bit pages {tuple(shape)} with {tuple(kt.shape)}, {tuple(vc.shape)} with {tuple(vt.shape)} for {heads} "
                          f"heads of {head_dim} (64 or 128; a multiple of {PAGE_UNIT} tokens a page)")
-    if num_pages * nkv * page_size >= 2 ** 31 - 1:
+    if num_pages * nkv * page_size >= 2 ** 31 - 1 - page_size:
         raise ValueError(f"8-bit pages {tuple(shape)} have 2^31 rows or more")
-    for codes, tops in (k_pages, v_pages):
-        if (codes.dtype is not torch.int8 or tops.dtype is not torch.bfloat16 or codes.device != device or tops.device != device
-                or not codes.is_contiguous() or not tops.is_contiguous() or codes.data_ptr() % 16):
-            raise ValueError(f"8-bit pages are contiguous, 16-byte aligned int8 and bf16 tensors on {device}")
-    if (page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch
-            or page_table.device != device or not page_table.is_contiguous()):
-        raise ValueError(f"a page table is a contiguous int32 matrix of {batch} rows on {device}: {tuple(page_table.shape)} "
+    if (kc.dtype is not torch.int8 or vc.dtype is not torch.int8 or kt.dtype is not torch.bfloat16 or vt.dtype is not torch.bfloat16
+            or not (kc.get_device() == vc.get_device() == kt.get_device() == vt.get_device() == device)
+            or not (kc.is_contiguous() and vc.is_contiguous() and kt.is_contiguous() and vt.is_contiguous())
+            or (kc.data_ptr() | vc.data_ptr()) % 16):
+        raise ValueError("8-bit pages are contiguous, 16-byte aligned int8 and bf16 tensors on the operands' device")
+    table = page_table.shape
+    if (page_table.dtype is not torch.int32 or len(table) != 2 or table[0] != batch or page_table.get_device() != device
+            or not page_table.is_contiguous()):
+        raise ValueError(f"a page table is a contiguous int32 matrix of {batch} rows on the operands' device: {tuple(table)} "
                          f"{page_table.dtype}")
-    return num_pages, nkv, page_size
+    return num_pages, nkv, page_size, table[1]
+
+
+def _check_counts(counts: Tensor, batch: int, name: str, device: int) -> None:
+    if counts.dtype is not torch.int32 or counts.shape != (batch,) or not counts.is_contiguous() or counts.get_device() != device:
+        raise ValueError(f"{name} is [{batch}] int32 on the operands' device: {tuple(counts.shape)} {counts.dtype}")
 
 
 def _append_plain(k, v, k_pages, v_pages, page_table, start, live):
@@ -416,8 +433,8 @@ def append_int8(k: Tensor, v: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, pa
     b, t, nkv, h = k.shape
     if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
         raise ValueError(f"k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} differ")
-    device = k.device
-    num_pages, held, page_size = _check_pages(k_pages, v_pages, page_table, b, nkv, h, device)
+    device = k.get_device()
+    num_pages, held, page_size, max_pages = _check_pages(k_pages, v_pages, page_table, b, nkv, h, device)
     if held != nkv:
         raise ValueError(f"pages of {held} heads for {nkv}")
     _check_counts(start, b, "start", device)
@@ -431,11 +448,10 @@ def append_int8(k: Tensor, v: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, pa
         return tuple(out) if values else None
     k, v = _aligned_rows(k), _aligned_rows(v)
     out = (k.new_empty((b, t, nkv, h)), k.new_empty((b, t, nkv, h))) if values else None
-    _call(device, "axb_int8_append", k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3],
-          out[0].data_ptr() if values else None, out[1].data_ptr() if values else None, k_pages.codes.data_ptr(),
-          k_pages.tops.data_ptr(), v_pages.codes.data_ptr(), v_pages.tops.data_ptr(), page_table.data_ptr(), start.data_ptr(),
-          None if live is None else live.data_ptr(), b, t, nkv, h, page_size, page_table.shape[1], num_pages,
-          cuda_ops.status_word(device).data_ptr())
+    _call(device, "axb_int8_append", k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], out[0].data_ptr() if values else 0,
+          out[1].data_ptr() if values else 0, k_pages.codes.data_ptr(), k_pages.tops.data_ptr(), v_pages.codes.data_ptr(),
+          v_pages.tops.data_ptr(), page_table.data_ptr(), start.data_ptr(), 0 if live is None else live.data_ptr(), b, t, nkv, h,
+          page_size, max_pages, num_pages, _status(device))
     return out
 
 
@@ -478,12 +494,12 @@ def paged_decode_attention_int8(q: Tensor, k_pages: Int8Pages, v_pages: Int8Page
     more than eight splits (made a multiple of eight); calls that overlap on the GPU need one each.  Queries from 2^-40 to 2^56 and
     pages' tops from 2^-40 to 2^50 keep their digits; larger ones may overflow.  Returns ``[B, Nq, H]``."""
     b, nq, h = q.shape
-    device = q.device
-    num_pages, nkv, page_size = _check_pages(k_pages, v_pages, page_table, b, nq, h, device)
+    device = q.get_device()
+    cache = _check_pages(k_pages, v_pages, page_table, b, nq, h, device)
     _check_counts(lengths, b, "lengths", device)
     scale = 1.0 / math.sqrt(h) if softmax_scale is None else softmax_scale
     _check_scale(scale)
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != device or not out.is_contiguous()):
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.get_device() != device or not out.is_contiguous()):
         raise ValueError(f"out {tuple(out.shape)} {out.dtype}: contiguous {tuple(q.shape)} {q.dtype} is wanted")
     _no_gradient("paged_decode_attention_int8", q, k_pages.tops, v_pages.tops, out)
     if not _on_kernel(q):
@@ -494,32 +510,33 @@ def paged_decode_attention_int8(q: Tensor, k_pages: Int8Pages, v_pages: Int8Page
         q = q.clone(memory_format=torch.contiguous_format)
     if out is None:
         out = torch.empty_like(q)
-    _launch_attention(q, k_pages, v_pages, page_table, lengths, -1, out, scratch, b, nq, nkv, h, page_size, num_pages, splits, scale)
+    _launch_attention(q, k_pages, v_pages, page_table, lengths, -1, out, scratch, b, nq, h, *cache, splits, scale, device)
     return out
 
 
-def _launch_attention(q, k_pages, v_pages, page_table, lengths, limit, out, scratch, b, nq, nkv, h, page_size, num_pages, splits, scale):
-    max_pages, device = page_table.shape[1], q.device
+def _launch_attention(q, k_pages, v_pages, page_table, lengths, limit, out, scratch, b, nq, h, num_pages, nkv, page_size, max_pages,
+                      splits, scale, device):
     if splits is None:
         splits = attention_splits(b, nkv, nq // nkv, max_pages * page_size)
     if splits > 8:
         splits = -(-splits // 8) * 8
         floats = attention_scratch_floats(b, nq, h, splits)
         if scratch is None:
-            scratch = torch.empty(floats, dtype=torch.float32, device=device)
-        elif (scratch.numel() < floats or scratch.dtype != torch.float32 or scratch.device != device
+            scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
+        elif (scratch.numel() < floats or scratch.dtype != torch.float32 or scratch.get_device() != device
               or not scratch.is_contiguous() or scratch.data_ptr() % 8):
-            raise ValueError(f"scratch is {floats} contiguous fp32 values on {device}, 8-byte aligned")
+            raise ValueError(f"scratch is {floats} contiguous fp32 values on {q.device}, 8-byte aligned")
     _call(device, "axb_int8_decode_attn", q.data_ptr(), k_pages.codes.data_ptr(), k_pages.tops.data_ptr(), v_pages.codes.data_ptr(),
           v_pages.tops.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(),
-          None if scratch is None else scratch.data_ptr(), limit, b, nq, nkv, h, page_size, max_pages, num_pages, splits, scale,
-          cuda_ops.status_word(device).data_ptr())
+          0 if scratch is None else scratch.data_ptr(), limit, b, nq, nkv, h, page_size, max_pages, num_pages, splits, scale,
+          _status(device))
 
 
 def attention_scratch_floats(batch: int, num_q_heads: int, head_dim: int, splits: int) -> int:
     """fp32 values that the parts of more than eight splits take (a multiple of eight)."""
     splits = -(-splits // 8) * 8 if splits > 8 else splits
-    return _lib().axb_int8_attn_scratch_floats(batch, num_q_heads, head_dim, splits)
+    f, _ = _entries.get("axb_int8_attn_scratch_floats") or _entry("axb_int8_attn_scratch_floats")
+    return f(batch, num_q_heads, head_dim, splits)
 
 
 def _check_packed(qkv: Tensor, k_pages: Int8Pages, table: Tensor, nq: int) -> tuple[int, int]:
@@ -542,12 +559,12 @@ def rope_decode_attention_int8(qkv: Tensor, k_pages: Int8Pages, v_pages: Int8Pag
     nkv, h = _check_packed(qkv, k_pages, table, num_q_heads)
     if qkv.dim() != 2:
         raise ValueError(f"a step takes one token a sequence, [B, width]: {tuple(qkv.shape)}")
-    b, device = qkv.shape[0], qkv.device
-    num_pages, _, page_size = _check_pages(k_pages, v_pages, page_table, b, num_q_heads, h, device)
+    b, device = qkv.shape[0], qkv.get_device()
+    num_pages, _, page_size, max_pages = cache = _check_pages(k_pages, v_pages, page_table, b, num_q_heads, h, device)
     _check_counts(lengths, b, "lengths", device)
     _check_scale(softmax_scale)
     _no_gradient("rope_decode_attention_int8", qkv, k_pages.tops, v_pages.tops, table)
-    limit = min(table.shape[0], page_table.shape[1] * page_size)
+    limit = min(table.shape[0], max_pages * page_size)
     if not _on_kernel(qkv):
         if not b:
             return qkv.new_empty((0, num_q_heads, h))
@@ -559,13 +576,12 @@ def rope_decode_attention_int8(qkv: Tensor, k_pages: Int8Pages, v_pages: Int8Pag
         q, k = _rotate(q, table, pos), _rotate(k, table, pos)
         _append_plain(k, v, k_pages, v_pages, page_table, lengths - 1, (lengths > 0).to(torch.int32))
         return paged_decode_attention_int8(q[:, 0], k_pages, v_pages, page_table, lengths, softmax_scale=softmax_scale)
-    out = torch.empty((b, num_q_heads, h), dtype=qkv.dtype, device=device)  # the rotated queries, then what they attend to
+    out = qkv.new_empty((b, num_q_heads, h))  # the rotated queries, then what they attend to
     _call(device, "axb_int8_rope_append", qkv.data_ptr(), out.data_ptr(), k_pages.codes.data_ptr(), k_pages.tops.data_ptr(),
-          v_pages.codes.data_ptr(), v_pages.tops.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), None, table.data_ptr(),
-          table.shape[0], b, 1, num_q_heads, nkv, h, page_size, page_table.shape[1], num_pages,
-          cuda_ops.status_word(device).data_ptr())
-    _launch_attention(out, k_pages, v_pages, page_table, lengths, limit, out, scratch, b, num_q_heads, nkv, h, page_size, num_pages,
-                      splits, softmax_scale)
+          v_pages.codes.data_ptr(), v_pages.tops.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), 0, table.data_ptr(),
+          table.shape[0], b, 1, num_q_heads, nkv, h, page_size, max_pages, num_pages, _status(device))
+    _launch_attention(out, k_pages, v_pages, page_table, lengths, limit, out, scratch, b, num_q_heads, h, *cache, splits, softmax_scale,
+                      device)
     return out
 
 
@@ -576,10 +592,10 @@ def prompt_attention_int8(qkv: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, p
     cache then stands for: in ``qkv`` queries are replaced by rotated ones, keys and values by the cache's, rounded to
     ``qkv``'s type (zeros behind ``live``).  Returns ``[B, T, Nq * H]``."""
     nkv, h = _check_packed(qkv, k_pages, table, num_q_heads)
-    b, t, width = qkv.shape
-    device = qkv.device
-    num_pages, _, page_size = _check_pages(k_pages, v_pages, page_table, b, num_q_heads, h, device)
-    if table.shape[0] < t or page_table.shape[1] * page_size < t:
+    b, t, _ = qkv.shape
+    device = qkv.get_device()
+    num_pages, _, page_size, max_pages = _check_pages(k_pages, v_pages, page_table, b, num_q_heads, h, device)
+    if table.shape[0] < t or max_pages * page_size < t:
         raise ValueError(f"{b} x {t} tokens, a rotation table of {table.shape[0]} positions, a page table {tuple(page_table.shape)}")
     if live is not None:
         _check_counts(live, b, "live", device)
@@ -597,9 +613,8 @@ def prompt_attention_int8(qkv: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, p
         return out.reshape(b, t, num_q_heads * h)
     from axlearn_b200.ops import decode_ops
 
-    _call(device, "axb_int8_rope_append", qkv.data_ptr(), None, k_pages.codes.data_ptr(), k_pages.tops.data_ptr(),
-          v_pages.codes.data_ptr(), v_pages.tops.data_ptr(), page_table.data_ptr(), None, None if live is None else live.data_ptr(),
-          table.data_ptr(), table.shape[0], b, t, num_q_heads, nkv, h, page_size, page_table.shape[1], num_pages,
-          cuda_ops.status_word(device).data_ptr())
-    with _on(device):
+    _call(device, "axb_int8_rope_append", qkv.data_ptr(), 0, k_pages.codes.data_ptr(), k_pages.tops.data_ptr(),
+          v_pages.codes.data_ptr(), v_pages.tops.data_ptr(), page_table.data_ptr(), 0, 0 if live is None else live.data_ptr(),
+          table.data_ptr(), table.shape[0], b, t, num_q_heads, nkv, h, page_size, max_pages, num_pages, _status(device))
+    with _on(qkv.device):
         return decode_ops.packed_prompt_attention(qkv, num_q_heads=num_q_heads, num_kv_heads=nkv, softmax_scale=softmax_scale)
