@@ -214,7 +214,7 @@ struct Int8AttnParams {
   FastDiv page;
   int num_q_heads, num_kv_heads, max_pages, num_pages, splits;
   int limit;               // a decoding step: longer sequences than this had no place or rotation and get zeros; else -1
-  float scale_log2;        // softmax scale * log2(e) / 127 * 2^kInt8Back, > 0
+  float scale_log2;        // softmax scale * log2(e) / 127, > 0
 };
 
 constexpr int kI8AttnThreads = 128, kI8AttnWarps = kI8AttnThreads / 32;
@@ -225,8 +225,8 @@ constexpr int kI8AttnStages = 2;
 constexpr int kI8AttnCluster = 8;
 constexpr float kI8Slack = 8.f;
 
-// Codes as operands: c + 128, a byte in the low half of a bf16 lane, is the number (c + 128) 2^-133 as it lies (a denormal, then
-// the first binade of the same spacing).  The other operand carries 2^64, so that products stay in fp32's range.
+// V's codes as operands: c + 128, a byte in the low half of a bf16 lane, is the number (c + 128) 2^-133 as it lies (a denormal,
+// then the first binade of the same spacing).  P carries 2^64, so that products stay in fp32's range.
 constexpr float kInt8Up = 0x1p64f, kInt8Back = 0x1p69f;
 
 __device__ __forceinline__ uint32_t int8_even(uint32_t x) { return (x & 0x00ff00ffu) ^ 0x00800080u; }
@@ -238,11 +238,37 @@ __device__ __forceinline__ uint32_t int8_turned_round(uint32_t x) {
   return y;
 }
 
+// d = a b + c in bf16.
+__device__ __forceinline__ void int8_mma_add(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+
+// Sums of products of codes and a digit of q, from kInt8Sums: whole numbers below 2^22 that are the last bits of a float.
+constexpr int kInt8Sums = 0x4b400000;  // 1.5 * 2^23
+template <bool kSigned>
+__device__ __forceinline__ void int8_mma_sum(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (kSigned)
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Two matrices of 16 keys x 16 dims, a row a lane (0 .. 15, 16 .. 31): lane (r, c) gets keys 4c .. 4c + 3 of dims r and r + 8 of each.
+__device__ __forceinline__ void int8_load_turned(uint32_t (&v)[4], uint32_t row) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(row));
+}
+
 template <int H>
 struct Int8Tile {
   static constexpr int kChunk = kI8Chunk * H, kBytes = 4 * kChunk;  // two chunks of K, two of V
+  static constexpr int kPart = H + 4;                               // floats of a head's part: no bank conflicts
   static constexpr int kSmem(int rows) {
-    const int merge = (kI8AttnWarps + 1) * rows * (H + 2) * 4, tiles = kI8AttnWarps * kI8AttnStages * kBytes;
+    const int merge = (kI8AttnWarps + 1) * rows * (kPart + 2) * 4, tiles = kI8AttnWarps * kI8AttnStages * kBytes;
     return (merge > tiles ? merge : tiles) + 1024;  // alignment slack
   }
   // 16-byte unit u of a chunk's row, as TMA swizzles it: eight lanes of both products hit all banks.
@@ -252,11 +278,12 @@ struct Int8Tile {
   }
 };
 
-// S^T = K Q^T: 16 keys are the rows of the m16n8k16 tile, the query heads its columns; a lane takes H / 4 neighbouring dims of a
-// key, so that a word of four codes is two operand registers.  O^T = V^T P^T: 16 dims are the rows, P is turned round by
-// `movmatrix`.  A chunk of 16 keys is of one page, so A / 127 of K multiplies its scores, and that of V its products in fp32;
-// codes enter as c + 128, and 128 times the sums of q and of P leave again.  P is rounded to bf16 once and normalised by the
-// sum of what it was rounded to.  The maximum that P is relative to moves only when a score passes it by kI8Slack.
+// S^T = K Q^T in integers: 16 keys are the rows of the m16n8k32 tile, the query heads its columns, K's codes operands as they lie.
+// A head's q is a whole number of 24 bits times a power of two, three digits of 8 bits, so that scores are exact to 2^-23 of its
+// largest value.  O^T = V^T P^T in bf16: 16 dims are the rows, `ldmatrix` turns V round and `movmatrix` P, and a word of four
+// codes becomes two operand registers.  A chunk of 16 keys is of one page, so A / 127 of K multiplies its scores, and that of V its
+// products in fp32; codes of V enter as c + 128, and 128 times the sums of P leave again.  P is rounded to bf16 once and normalised
+// by the sum of what it was rounded to.  The maximum that P is relative to moves only when a score passes it by kI8Slack.
 //
 // A tile is 32 keys, a warp's own from TMA to its sums: no barrier of the CTA before the end.  Tiles go round the warps of all
 // splits, splits of eight or less are a cluster whose parts meet in distributed shared memory, more are clusters whose parts a
@@ -266,7 +293,7 @@ __global__ void __launch_bounds__(kI8AttnThreads, 3)
 int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Int8AttnParams p) {
   chain_link();
   using Tile = Int8Tile<H>;
-  constexpr int kSteps = H / 16;  // MMAs of a chunk in either product
+  constexpr int kSteps = H / 16, kDigitSteps = H / 32;  // MMAs of a chunk in V's product, in K's for a digit
   extern __shared__ uint8_t s_raw[];
   __shared__ __align__(8) uint64_t s_full[kI8AttnWarps][kI8AttnStages];
   uint8_t* s_ring = s_raw + (((smem_u32(s_raw) + 1023u) & ~1023u) - smem_u32(s_raw));
@@ -329,61 +356,79 @@ int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   uint32_t page = page_of(0), page_next = page_of(1);
   Places now = places(0, page), next = places(1, page_next);
   page = page_of(2);
+  uint32_t none = __ballot_sync(0xffffffffu, now.row < 0);  // chunks of the batch without keys
   uint8_t* ring = s_ring + warp * kI8AttnStages * Tile::kBytes;
-  // Tile `n` of the warp, whose batch is `now` or the next one.
+  // Tile `n` of the warp, whose batch is `now` or the next one: lanes 0 and 1 fetch a chunk each.
   auto load_tile = [&](int n, int stage, bool ahead) {
-    const int at = ahead ? next.row : now.row;
-    const int row_a = __shfl_sync(0xffffffffu, at, (n & 15) * 2), row_b = __shfl_sync(0xffffffffu, at, (n & 15) * 2 + 1);
-    if (lane == 0) {
+    const int row = __shfl_sync(0xffffffffu, ahead ? next.row : now.row, (n & 15) * 2 + (lane & 1));
+    const uint32_t there = __ballot_sync(0xffffffffu, row >= 0) & 3;
+    if (lane < 2) {
       uint64_t* bar = &s_full[warp][stage];
-      uint8_t* dst = ring + stage * Tile::kBytes;
-      mbar_arrive_expect_tx(bar, ((row_a >= 0) + (row_b >= 0)) * 2 * Tile::kChunk);
-      if (row_a >= 0) tma_load_2d(dst, &map_k, bar, 0, row_a);
-      if (row_b >= 0) tma_load_2d(dst + Tile::kChunk, &map_k, bar, 0, row_b);
-      if (row_a >= 0) tma_load_2d(dst + 2 * Tile::kChunk, &map_v, bar, 0, row_a);
-      if (row_b >= 0) tma_load_2d(dst + 3 * Tile::kChunk, &map_v, bar, 0, row_b);
+      uint8_t* dst = ring + stage * Tile::kBytes + lane * Tile::kChunk;
+      if (lane == 0) mbar_arrive_expect_tx(bar, __popc(there) * 2 * Tile::kChunk);
+      if (row >= 0) {
+        tma_load_2d(dst, &map_k, bar, 0, row);
+        tma_load_2d(dst + 2 * Tile::kChunk, &map_v, bar, 0, row);
+      }
     }
   };
 #pragma unroll
   for (int i = 0; i < kI8AttnStages; ++i)
     if (tile0 + i * step < hi) load_tile(i, i, false);
 
-  // Q of head r: MMA j takes dims H / 4 * c + 4 j + (0, 2) and (1, 3).
-  uint32_t qb[kSteps][2];
-  float q_sum[2];
+  // 16-byte units of K's rows that a lane takes: of 128-byte rows two that leave those of the next lanes' rows other banks.
+  const int unit0 = H == 128 ? (c & 1) + ((c >> 1) << 2) : c;
+  // Q of head r in three digits, q = 2^(e - 22) (65536 q2 + 256 q1 + q0), e the exponent of its largest value; step j takes eight
+  // dims of a unit.
+  uint32_t qd[3][kDigitSteps][2];
+  float q_scale[2];
   {
-    float sum = 0.f;
-    const __nv_bfloat162 up = __float2bfloat162_rn(kInt8Up);
-    const __nv_bfloat16* q = p.q + (static_cast<int64_t>(b) * p.num_q_heads + qh0 + r) * H + c * (H / 4);
+    const __nv_bfloat16* q = p.q + (static_cast<int64_t>(b) * p.num_q_heads + qh0 + r) * H;
+    uint4 x[kDigitSteps];
+    uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < kSteps / 2; ++i) {
-      const uint4 x = r < rows ? *reinterpret_cast<const uint4*>(q + i * 8) : make_uint4(0, 0, 0, 0);
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    for (int j = 0; j < kDigitSteps; ++j) {
+      x[j] = r < rows ? *reinterpret_cast<const uint4*>(q + (unit0 + (j >> 1) * 2) * 16 + (j & 1) * 8) : make_uint4(0, 0, 0, 0);
+      top = __vmaxu2(top, __vmaxu2(x[j].x & 0x7fff7fffu, x[j].y & 0x7fff7fffu));
+      top = __vmaxu2(top, __vmaxu2(x[j].z & 0x7fff7fffu, x[j].w & 0x7fff7fffu));
+    }
+    top = max(top & 0xffffu, top >> 16);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // (Queries below 2^-64 are not told apart any further.)
+    const int e = max(static_cast<int>(top >> 7) - 127, -64);
+    const float up = __int_as_float((22 - e + 127) << 23);  // (of an infinity or NaN: what comes out is not used)
+    float back = top >= 0x7f80u ? __int_as_float(0x7fffffff) : __int_as_float((e - 22 + 127) << 23);
+    back *= p.scale_log2;
+    q_scale[0] = __shfl_sync(0xffffffffu, back, 8 * c);
+    q_scale[1] = __shfl_sync(0xffffffffu, back, 8 * c + 4);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = unpack2(w[j]);
-        sum += f.x + f.y;
-      }
+    for (int j = 0; j < kDigitSteps; ++j) {
+      const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t e = __byte_perm(w[2 * j], w[2 * j + 1], 0x5410), o = __byte_perm(w[2 * j], w[2 * j + 1], 0x7632);
-        const __nv_bfloat162 be = __hmul2(reinterpret_cast<const __nv_bfloat162&>(e), up);
-        const __nv_bfloat162 bo = __hmul2(reinterpret_cast<const __nv_bfloat162&>(o), up);
-        qb[2 * i + j][0] = reinterpret_cast<const uint32_t&>(be);
-        qb[2 * i + j][1] = reinterpret_cast<const uint32_t&>(bo);
+      for (int i = 0; i < 2; ++i) {
+        const float2 f0 = unpack2(w[2 * i]), f1 = unpack2(w[2 * i + 1]);
+        const int n0 = __float2int_rn(f0.x * up), n1 = __float2int_rn(f0.y * up), n2 = __float2int_rn(f1.x * up),
+                  n3 = __float2int_rn(f1.y * up);
+#pragma unroll
+        for (int digit = 0; digit < 3; ++digit) {
+          const uint32_t pick = digit | (digit + 4) << 4;
+          qd[digit][j][i] = __byte_perm(__byte_perm(n0, n1, pick), __byte_perm(n2, n3, pick), 0x5410);
+        }
       }
     }
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    sum *= -128.f / kInt8Back;
-    q_sum[0] = __shfl_sync(0xffffffffu, sum, 8 * c);
-    q_sum[1] = __shfl_sync(0xffffffffu, sum, 8 * c + 4);
   }
 
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, w_sum[2] = {0.f, 0.f};  // heads 2c, 2c + 1; l and w_sum of this lane's keys
-  float acc[kSteps][4];  // [i][dims H / 8 * r + 2 i, + 1][columns 2c, 2c + 1]
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, w_sum[2] = {0.f, 0.f};  // heads 2c, 2c + 1
+  float acc[kSteps][4];  // [i][dim 16 i + r: columns 2c, 2c + 1; dim 16 i + 8 + r]
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+  const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+  const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+  // Slots r and r + 8 of a chunk's rows are keys 2r and 2r + 1, so that after `movmatrix` lane c has P of the keys that `ldmatrix` gives
+  // it of V.
+  const uint8_t* k_at = ring + Tile::unit(2 * r, unit0);
+  const uint32_t v_at = smem_u32(ring) + 2 * Tile::kChunk;
 
   int stage = 0, n = 0;
   uint32_t phase = 0;
@@ -391,6 +436,7 @@ int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   for (int tile = tile0; tile < hi; tile += step, ++n) {
     if (n > 0 && (n & 15) == 0) {
       now = next;
+      none = __ballot_sync(0xffffffffu, now.row < 0);
       const int batch = n >> 4;
       next = places(batch + 1, page);
       page = page_of(batch + 2);
@@ -399,44 +445,50 @@ int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       ok = false;
       break;
     }
-    const uint8_t* st = ring + stage * Tile::kBytes;
-    const int lane_a = (n & 15) * 2;
+    const int at_stage = stage * Tile::kBytes, lane_a = (n & 15) * 2;
     const uint32_t tops = static_cast<uint32_t>(now.k_top) | static_cast<uint32_t>(now.v_top) << 16;
     float s[2][4], vt[2];
 #pragma unroll
     for (int ch = 0; ch < 2; ++ch) {
       const uint32_t pair = __shfl_sync(0xffffffffu, tops, lane_a + ch);
-      const float kt = __uint_as_float(pair << 16) * p.scale_log2;
+      const float kt = __uint_as_float(pair << 16);
       vt[ch] = __uint_as_float(pair & 0xffff0000u) * (1.f / 127.f);
-      uint32_t w[2][kSteps];
+      uint32_t w[2][2 * kDigitSteps];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
-        for (int u = 0; u < kSteps / 4; ++u)
-          *reinterpret_cast<uint4*>(&w[i][4 * u]) =
-              *reinterpret_cast<const uint4*>(st + ch * Tile::kChunk + Tile::unit(8 * i + r, kSteps / 4 * c + u));
+        for (int u = 0; u < kDigitSteps / 2; ++u) {
+          // (The next row, the second unit: bits of the swizzled place, and the row's own.)
+          const uint8_t* at = H == 128 ? ring + Tile::unit(2 * r + i, unit0 + 2 * u) : k_at + i * H;
+          *reinterpret_cast<uint4*>(&w[i][4 * u]) = *reinterpret_cast<const uint4*>(at + at_stage + ch * Tile::kChunk);
+        }
       }
-      float d[4] = {q_sum[0], q_sum[1], q_sum[0], q_sum[1]};
+      int d[3][4];
 #pragma unroll
-      for (int j = 0; j < kSteps; ++j) {
-        const uint32_t a[4] = {int8_even(w[0][j]), int8_even(w[1][j]), int8_odd(w[0][j]), int8_odd(w[1][j])};
-        mma(d, a, qb[j][0], qb[j][1]);
+      for (int digit = 0; digit < 3; ++digit) d[digit][0] = d[digit][1] = d[digit][2] = d[digit][3] = kInt8Sums;
+#pragma unroll
+      for (int j = 0; j < kDigitSteps; ++j) {
+        int8_mma_sum<false>(d[0], w[0][2 * j], w[1][2 * j], w[0][2 * j + 1], w[1][2 * j + 1], qd[0][j][0], qd[0][j][1]);
+        int8_mma_sum<false>(d[1], w[0][2 * j], w[1][2 * j], w[0][2 * j + 1], w[1][2 * j + 1], qd[1][j][0], qd[1][j][1]);
+        int8_mma_sum<true>(d[2], w[0][2 * j], w[1][2 * j], w[0][2 * j + 1], w[1][2 * j + 1], qd[2][j][0], qd[2][j][1]);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[ch][i] = d[i] * kt;
+      for (int i = 0; i < 4; ++i) {
+        float f[3];
+#pragma unroll
+        for (int digit = 0; digit < 3; ++digit) f[digit] = __int_as_float(d[digit][i]) - __int_as_float(kInt8Sums);
+        s[ch][i] = fmaf(f[2], 65536.f, fmaf(f[1], 256.f, f[0])) * (q_scale[i & 1] * kt);
+      }
     }
-    if ((tile + 1) * static_cast<int64_t>(kI8AttnKeys) > len) {
+    const uint32_t empty = none >> lane_a & 3;  // chunks behind the sequence, or of a page that is not in the pool
+    if (empty != 0 || (tile + 1) * static_cast<int64_t>(kI8AttnKeys) > len) {
 #pragma unroll
       for (int ch = 0; ch < 2; ++ch) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          if (tile * kI8AttnKeys + ch * kI8Chunk + i * 8 + r >= len) s[ch][2 * i] = s[ch][2 * i + 1] = -INFINITY;
+          if ((empty >> ch & 1) || tile * kI8AttnKeys + ch * kI8Chunk + 2 * r + i >= len) s[ch][2 * i] = s[ch][2 * i + 1] = -INFINITY;
       }
     }
-    // A page that is not in the pool has no keys.
-#pragma unroll
-    for (int ch = 0; ch < 2; ++ch)
-      if (__shfl_sync(0xffffffffu, now.row, lane_a + ch) < 0) s[ch][0] = s[ch][1] = s[ch][2] = s[ch][3] = -INFINITY;
     float top[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) top[h] = fmaxf(fmaxf(s[0][h], s[0][2 + h]), fmaxf(s[1][h], s[1][2 + h]));
@@ -454,46 +506,32 @@ int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         for (int i = 0; i < kSteps; ++i) acc[i][h] *= by, acc[i][2 + h] *= by;
       }
     }
+    const float base[2] = {m[0] == -INFINITY ? 0.f : 64.f - m[0], m[1] == -INFINITY ? 0.f : 64.f - m[1]};
 #pragma unroll
     for (int ch = 0; ch < 2; ++ch) {
       uint32_t pt[2];
-      float sums[2] = {0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float e[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) e[h] = ex2(s[ch][2 * i + h] + (m[h] == -INFINITY ? 0.f : 64.f - m[h]));  // (NaN stays)
-        const uint32_t two = pack2(e[0], e[1]);
-        sums[0] += __uint_as_float(two << 16);
-        sums[1] += __uint_as_float(two & 0xffff0000u);
-        pt[i] = int8_turned_round(two);
-      }
+      for (int i = 0; i < 2; ++i)  // (NaN stays)
+        pt[i] = int8_turned_round(pack2(ex2(s[ch][2 * i] + base[0]), ex2(s[ch][2 * i + 1] + base[1])));
+      float sums[4];  // of P, in every lane of a column
+      int8_mma_add(sums, ones, pt[0], pt[1], zero);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         l[h] += sums[h];
         w_sum[h] = fmaf(vt[ch], sums[h] * (1.f / kInt8Up), w_sum[h]);
       }
-      constexpr int kWords = kSteps / 2;  // of a key that a lane takes: dims H / 8 * r ..
-      uint32_t w[4][kWords];              // keys 2c, 2c + 1, 2c + 8, 2c + 9
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = 2 * c + (i & 1) + 8 * (i >> 1);
-        const uint8_t* at = st + (2 + ch) * Tile::kChunk;
-        if constexpr (H == 128) *reinterpret_cast<uint4*>(w[i]) = *reinterpret_cast<const uint4*>(at + Tile::unit(key, r));
-        else *reinterpret_cast<uint2*>(w[i]) = *reinterpret_cast<const uint2*>(at + Tile::unit(key, r >> 1) + (r & 1) * 8);
-      }
       const float back = vt[ch] * kInt8Back;
 #pragma unroll
-      for (int j = 0; j < kWords; ++j) {
+      for (int i = 0; i < kSteps; i += 2) {
+        uint32_t v[4];
+        int8_load_turned(v, v_at + at_stage + ch * Tile::kChunk + Tile::unit(lane & 15, i + (lane >> 4)));
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t x = __byte_perm(w[0][j], w[1][j], half ? 0x7632 : 0x5410);
-          const uint32_t y = __byte_perm(w[2][j], w[3][j], half ? 0x7632 : 0x5410);
-          const uint32_t a[4] = {int8_even(x), int8_odd(x), int8_even(y), int8_odd(y)};
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-          mma(d, a, pt[0], pt[1]);
+        for (int t = 0; t < 2; ++t) {
+          const uint32_t a[4] = {int8_even(v[2 * t]), int8_even(v[2 * t + 1]), int8_odd(v[2 * t]), int8_odd(v[2 * t + 1])};
+          float d[4];
+          int8_mma_add(d, a, pt[0], pt[1], zero);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[2 * j + half][i] = fmaf(back, d[i], acc[2 * j + half][i]);
+          for (int e = 0; e < 4; ++e) acc[i + t][e] = fmaf(back, d[e], acc[i + t][e]);
         }
       }
     }
@@ -508,23 +546,18 @@ int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   if (!ok)  // let copies that may still be in flight land
     for (int i = 0; i < 2000; ++i) __nanosleep(1000);
   __syncthreads();  // the merge buffers overlay the tiles
-  float* s_part = reinterpret_cast<float*>(s_ring);  // 4 warps and the CTA: [rows][H] sums, then maxima, then weights
-  const int per_warp = rows * H;
+  constexpr int kPart = Tile::kPart;
+  float* s_part = reinterpret_cast<float*>(s_ring);  // 4 warps and the CTA: [rows][kPart] sums, then maxima, then weights
+  const int per_warp = rows * kPart;
   float* s_m = s_part + (kI8AttnWarps + 1) * per_warp;
   float* s_l = s_m + (kI8AttnWarps + 1) * rows;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-#pragma unroll
-    for (int off = 4; off <= 16; off <<= 1) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], off);
-      w_sum[h] += __shfl_xor_sync(0xffffffffu, w_sum[h], off);
-    }
     if (2 * c + h >= rows) continue;
-    float* dst = s_part + warp * per_warp + (2 * c + h) * H + r * (H / 8);
+    float* dst = s_part + warp * per_warp + (2 * c + h) * kPart + r;
     const float low = -128.f * w_sum[h];
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i)
-      *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(acc[i][h] + low, acc[i][2 + h] + low);
+    for (int i = 0; i < kSteps; ++i) dst[16 * i] = acc[i][h] + low, dst[16 * i + 8] = acc[i][2 + h] + low;
     if (r == 0) {
       s_m[warp * rows + 2 * c + h] = m[h];
       s_l[warp * rows + 2 * c + h] = l[h] * (1.f / kInt8Up);
@@ -543,13 +576,13 @@ int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     for (int w = 0; w < kI8AttnWarps; ++w) {
       const float f = mm == -INFINITY ? 1.f : exp2f(s_m[w * rows + g] - mm);
       ll += s_l[w * rows + g] * f;
-      o += s_part[w * per_warp + g * H + d] * f;
+      o += s_part[w * per_warp + g * kPart + d] * f;
     }
     const int64_t row = static_cast<int64_t>(b) * p.num_q_heads + qh0 + g;
     if (p.splits == 1) {
       p.out[row * H + d] = __float2bfloat16(ll == 0.f ? 0.f : o / ll);
     } else {
-      s_part[kI8AttnWarps * per_warp + g * H + d] = o;
+      s_part[kI8AttnWarps * per_warp + g * kPart + d] = o;
       if (d == 0) {
         s_m[kI8AttnWarps * rows + g] = mm;
         s_l[kI8AttnWarps * rows + g] = ll;
@@ -566,7 +599,7 @@ int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         const bool have = s < cluster;
         mv[s] = have ? ld_cluster_f32(sptr(s_m + kI8AttnWarps * rows + g), s) : -INFINITY;
         lv[s] = have ? ld_cluster_f32(sptr(s_l + kI8AttnWarps * rows + g), s) : 0.f;
-        ov[s] = have ? ld_cluster_f32(sptr(s_part + kI8AttnWarps * per_warp + g * H + d), s) : 0.f;
+        ov[s] = have ? ld_cluster_f32(sptr(s_part + kI8AttnWarps * per_warp + g * kPart + d), s) : 0.f;
       }
       float mm = -INFINITY;
 #pragma unroll
@@ -779,7 +812,7 @@ extern "C" int axb_int8_decode_attn(const axb::Int8AttnCall* call, cudaStream_t 
   p.max_pages = static_cast<int>(a.max_pages), p.num_pages = static_cast<int>(a.num_pages);
   p.splits = static_cast<int>(a.splits);
   p.limit = static_cast<int>(a.limit < 0 ? -1 : a.limit < 0x7fffffff ? a.limit : 0x7fffffff);
-  p.scale_log2 = static_cast<float>(a.softmax_scale) * (1.4426950408889634f / 127.f * kInt8Back);
+  p.scale_log2 = static_cast<float>(a.softmax_scale) * (1.4426950408889634f / 127.f);
   const int B = static_cast<int>(a.B);
   return a.head_dim == 128 ? int8_attn<128>(a.k_codes, a.v_codes, p, B, stream) : int8_attn<64>(a.k_codes, a.v_codes, p, B, stream);
 }
