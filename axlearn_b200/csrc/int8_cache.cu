@@ -207,8 +207,8 @@ struct Int8AttnParams {
   const __nv_bfloat16 *k_tops, *v_tops;
   const int* page_table;
   const int* lengths;
-  float* part_out;         // [B, Nq, splits / 8, H]: of each cluster, where there are several
-  float* part_ml;          // [B, Nq, splits / 8, 2]
+  float* part_out;         // [B, Nq, splits, H]: more than a cluster's
+  float* part_ml;          // [B, Nq, splits, 2]
   __nv_bfloat16* out;
   int* status;
   FastDiv page;
@@ -217,13 +217,18 @@ struct Int8AttnParams {
   float scale_log2;        // softmax scale * log2(e) / 127, > 0
 };
 
-constexpr int kI8AttnThreads = 128, kI8AttnWarps = kI8AttnThreads / 32;
 constexpr int kI8AttnRows = 8;   // query heads of a CTA: the columns of both products
 constexpr int kI8Chunk = 16;     // keys of an MMA, of one page
 constexpr int kI8AttnKeys = 2 * kI8Chunk;
 constexpr int kI8AttnStages = 2;
 constexpr int kI8AttnCluster = 8;
 constexpr float kI8Slack = 8.f;
+
+// Warps of a CTA: four, three CTAs an SM, or, of more splits than a cluster has, twelve that have an SM to themselves: a third of the
+// parts (1 x 130001 tokens, 8 KV heads: 16 splits of twelve 49.5 us, 32 of four 51.6, 48 of four 53.8).
+constexpr int kI8FewWarps = 4, kI8ManyWarps = 12;
+// Where a CTA's sums go: out, the CTA of its cluster that finishes a head, or scratch for a second launch.
+enum Int8Merge { kMergeNone, kMergeCluster, kMergeScratch };
 
 // V's codes as operands: c + 128, a byte in the low half of a bf16 lane, is the number (c + 128) 2^-133 as it lies (a denormal,
 // then the first binade of the same spacing).  P carries 2^64, so that products stay in fp32's range.
@@ -263,12 +268,12 @@ __device__ __forceinline__ void int8_load_turned(uint32_t (&v)[4], uint32_t row)
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(row));
 }
 
-template <int H>
+template <int H, int kWarps>
 struct Int8Tile {
   static constexpr int kChunk = kI8Chunk * H, kBytes = 4 * kChunk;  // two chunks of K, two of V
   static constexpr int kPart = H + 4;                               // floats of a head's part: no bank conflicts
   static constexpr int kSmem(int rows) {
-    const int merge = (kI8AttnWarps + 1) * rows * (kPart + 2) * 4, tiles = kI8AttnWarps * kI8AttnStages * kBytes;
+    const int merge = (kWarps + 1) * rows * (kPart + 2) * 4, tiles = kWarps * kI8AttnStages * kBytes;
     return (merge > tiles ? merge : tiles) + 1024;  // alignment slack
   }
   // 16-byte unit u of a chunk's row, as TMA swizzles it: eight lanes of both products hit all banks.
@@ -286,16 +291,16 @@ struct Int8Tile {
 // by the sum of what it was rounded to.  The maximum that P is relative to moves only when a score passes it by kI8Slack.
 //
 // A tile is 32 keys, a warp's own from TMA to its sums: no barrier of the CTA before the end.  Tiles go round the warps of all
-// splits, splits of eight or less are a cluster whose parts meet in distributed shared memory, more are clusters whose parts a
-// second launch joins.
-template <int H, bool kCluster>
-__global__ void __launch_bounds__(kI8AttnThreads, 3)
+// splits; splits of eight or less are a cluster whose parts meet in distributed shared memory, those of more are joined by a second
+// launch.
+template <int H, int kWarps, Int8Merge kMerge>
+__global__ void __launch_bounds__(32 * kWarps, 12 / kWarps)
 int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Int8AttnParams p) {
   chain_link();
-  using Tile = Int8Tile<H>;
+  using Tile = Int8Tile<H, kWarps>;
   constexpr int kSteps = H / 16, kDigitSteps = H / 32;  // MMAs of a chunk in V's product, in K's for a digit
   extern __shared__ uint8_t s_raw[];
-  __shared__ __align__(8) uint64_t s_full[kI8AttnWarps][kI8AttnStages];
+  __shared__ __align__(8) uint64_t s_full[kWarps][kI8AttnStages];
   uint8_t* s_ring = s_raw + (((smem_u32(s_raw) + 1023u) & ~1023u) - smem_u32(s_raw));
   const int split = blockIdx.x;
   const int group = p.num_q_heads / p.num_kv_heads;
@@ -315,8 +320,8 @@ int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     len = p.limit >= 0 ? 0 : static_cast<int>(capacity);
   }
   len = max(len, 0);
-  const int hi = len / kI8AttnKeys + (len % kI8AttnKeys != 0), step = kI8AttnWarps * p.splits;
-  const int tile0 = split * kI8AttnWarps + warp;
+  const int hi = len / kI8AttnKeys + (len % kI8AttnKeys != 0), step = kWarps * p.splits;
+  const int tile0 = split * kWarps + warp;
   const int* table = p.page_table + static_cast<int64_t>(b) * p.max_pages;
   if (lane == 0) {
     for (int i = 0; i < kI8AttnStages; ++i) mbar_init(&s_full[warp][i], 1);
@@ -547,10 +552,10 @@ int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     for (int i = 0; i < 2000; ++i) __nanosleep(1000);
   __syncthreads();  // the merge buffers overlay the tiles
   constexpr int kPart = Tile::kPart;
-  float* s_part = reinterpret_cast<float*>(s_ring);  // 4 warps and the CTA: [rows][kPart] sums, then maxima, then weights
+  float* s_part = reinterpret_cast<float*>(s_ring);  // the warps and the CTA: [rows][kPart] sums, then maxima, then weights
   const int per_warp = rows * kPart;
-  float* s_m = s_part + (kI8AttnWarps + 1) * per_warp;
-  float* s_l = s_m + (kI8AttnWarps + 1) * rows;
+  float* s_m = s_part + (kWarps + 1) * per_warp;
+  float* s_l = s_m + (kWarps + 1) * rows;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     if (2 * c + h >= rows) continue;
@@ -565,41 +570,45 @@ int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   }
   __syncthreads();
   // Thread (g, d) of H threads a head owns output dim d.
-  constexpr int kSets = kI8AttnThreads / H;
+  constexpr int kSets = 32 * kWarps / H;
   const int d = threadIdx.x % H;
   for (int g = threadIdx.x / H; g < rows; g += kSets) {
     float mm = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kI8AttnWarps; ++w) mm = fmaxf(mm, s_m[w * rows + g]);
+    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w * rows + g]);
     float ll = 0.f, o = 0.f;
 #pragma unroll
-    for (int w = 0; w < kI8AttnWarps; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
       const float f = mm == -INFINITY ? 1.f : exp2f(s_m[w * rows + g] - mm);
       ll += s_l[w * rows + g] * f;
       o += s_part[w * per_warp + g * kPart + d] * f;
     }
     const int64_t row = static_cast<int64_t>(b) * p.num_q_heads + qh0 + g;
-    if (p.splits == 1) {
+    if constexpr (kMerge == kMergeNone) {
       p.out[row * H + d] = __float2bfloat16(ll == 0.f ? 0.f : o / ll);
+    } else if constexpr (kMerge == kMergeScratch) {
+      const int64_t part = row * p.splits + split;
+      p.part_out[part * H + d] = o;
+      if (d == 0) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(mm, ll);
     } else {
-      s_part[kI8AttnWarps * per_warp + g * kPart + d] = o;
+      s_part[kWarps * per_warp + g * kPart + d] = o;
       if (d == 0) {
-        s_m[kI8AttnWarps * rows + g] = mm;
-        s_l[kI8AttnWarps * rows + g] = ll;
+        s_m[kWarps * rows + g] = mm;
+        s_l[kWarps * rows + g] = ll;
       }
     }
   }
-  if constexpr (kCluster) {
-    const int cluster = min(p.splits, kI8AttnCluster), rank = split % cluster, cluster_parts = p.splits / cluster;
+  if constexpr (kMerge == kMergeCluster) {
+    const int cluster = p.splits, rank = split;
     cluster_sync_all();
     for (int g = rank * kSets + threadIdx.x / H; g < rows; g += cluster * kSets) {
       float mv[kI8AttnCluster], lv[kI8AttnCluster], ov[kI8AttnCluster];
 #pragma unroll
       for (int s = 0; s < kI8AttnCluster; ++s) {
         const bool have = s < cluster;
-        mv[s] = have ? ld_cluster_f32(sptr(s_m + kI8AttnWarps * rows + g), s) : -INFINITY;
-        lv[s] = have ? ld_cluster_f32(sptr(s_l + kI8AttnWarps * rows + g), s) : 0.f;
-        ov[s] = have ? ld_cluster_f32(sptr(s_part + kI8AttnWarps * per_warp + g * kPart + d), s) : 0.f;
+        mv[s] = have ? ld_cluster_f32(sptr(s_m + kWarps * rows + g), s) : -INFINITY;
+        lv[s] = have ? ld_cluster_f32(sptr(s_l + kWarps * rows + g), s) : 0.f;
+        ov[s] = have ? ld_cluster_f32(sptr(s_part + kWarps * per_warp + g * kPart + d), s) : 0.f;
       }
       float mm = -INFINITY;
 #pragma unroll
@@ -612,19 +621,13 @@ int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         o += ov[s] * f;
       }
       const int64_t row = static_cast<int64_t>(b) * p.num_q_heads + qh0 + g;
-      if (cluster_parts == 1) {
-        p.out[row * H + d] = __float2bfloat16(ll == 0.f ? 0.f : o / ll);
-      } else {
-        const int64_t part = row * cluster_parts + split / cluster;
-        p.part_out[part * H + d] = o;
-        if (d == 0) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(mm, ll);
-      }
+      p.out[row * H + d] = __float2bfloat16(ll == 0.f ? 0.f : o / ll);
     }
     cluster_sync_all();  // a CTA's shared memory outlives its readers
   }
 }
 
-// The clusters' parts of a row, eight at a time on their way.
+// The splits' parts of a row, eight at a time on their way.
 template <int H>
 __global__ void __launch_bounds__(H)
 int8_combine_kernel(const float* part_out, const float* part_ml, __nv_bfloat16* out, int parts) {
@@ -659,22 +662,24 @@ int8_combine_kernel(const float* part_out, const float* part_ml, __nv_bfloat16* 
   out[row * H + d] = __float2bfloat16(ll == 0.f ? 0.f : o / ll);
 }
 
-template <int H, bool kCluster>
+template <int H, int kWarps, Int8Merge kMerge>
 static int launch_int8_attn(const CUtensorMap& map_k, const CUtensorMap& map_v, const Int8AttnParams& p, dim3 grid,
                             cudaStream_t stream) {
-  constexpr auto kernel = int8_attn_kernel<H, kCluster>;
+  constexpr auto kernel = int8_attn_kernel<H, kWarps, kMerge>;
+  constexpr int kSmem = Int8Tile<H, kWarps>::kSmem(kI8AttnRows);
+  static_assert(12 / kWarps * (kSmem + 1024 + 512) <= 228 * 1024, "resident CTAs");
   static OptIn opt_in;
-  if (!opt_in.done(kernel, Int8Tile<H>::kSmem(kI8AttnRows))) return -3;
+  if (!opt_in.done(kernel, kSmem)) return -3;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {static_cast<unsigned>(p.splits < kI8AttnCluster ? p.splits : kI8AttnCluster), 1, 1};
+  attr[0].val.clusterDim = {static_cast<unsigned>(p.splits), 1, 1};
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(kI8AttnThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(Int8Tile<H>::kSmem(kI8AttnRows));
+  cfg.blockDim = dim3(32 * kWarps);
+  cfg.dynamicSmemBytes = static_cast<size_t>(kSmem);
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = static_cast<unsigned>(chain_attribute(attr, kCluster ? 1 : 0));
+  cfg.numAttrs = static_cast<unsigned>(chain_attribute(attr, kMerge == kMergeCluster ? 1 : 0));
   return cudaLaunchKernelEx(&cfg, kernel, map_k, map_v, p) == cudaSuccess ? 0 : -4;
 }
 
@@ -692,13 +697,13 @@ static int int8_attn(const void* k_codes, const void* v_codes, const Int8AttnPar
   }
   const int g = p.num_q_heads / p.num_kv_heads;
   const dim3 grid(p.splits, p.num_kv_heads * ((g + kI8AttnRows - 1) / kI8AttnRows), B);
-  const int rc = p.splits > 1 ? launch_int8_attn<H, true>(map[0], map[1], p, grid, stream)
-                              : launch_int8_attn<H, false>(map[0], map[1], p, grid, stream);
+  const int rc = p.splits == 1                ? launch_int8_attn<H, kI8FewWarps, kMergeNone>(map[0], map[1], p, grid, stream)
+                 : p.splits <= kI8AttnCluster ? launch_int8_attn<H, kI8FewWarps, kMergeCluster>(map[0], map[1], p, grid, stream)
+                                              : launch_int8_attn<H, kI8ManyWarps, kMergeScratch>(map[0], map[1], p, grid, stream);
   if (rc != 0) return rc;
   if (p.splits > kI8AttnCluster) {
     ChainedBehind chained;
-    launch_chained(int8_combine_kernel<H>, B * p.num_q_heads, H, 0, stream, p.part_out, p.part_ml, p.out,
-                   p.splits / kI8AttnCluster);
+    launch_chained(int8_combine_kernel<H>, B * p.num_q_heads, H, 0, stream, p.part_out, p.part_ml, p.out, p.splits);
   }
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
@@ -779,14 +784,14 @@ extern "C" int axb_int8_rope_append(const axb::Int8RopeAppendCall* call, cudaStr
   return int8_append(p, static_cast<int>(a.B), static_cast<int>(a.page_size), static_cast<int>(a.head_dim), stream);
 }
 
-// Scratch of axb_int8_decode_attn in floats: up to a cluster's splits meet without any.  More are a multiple of a cluster's.
+// Scratch of axb_int8_decode_attn in floats: up to a cluster's splits meet without any.
 extern "C" int64_t axb_int8_attn_scratch_floats(int B, int num_q_heads, int head_dim, int splits) {
   if (splits <= axb::kI8AttnCluster) return 0;
-  return static_cast<int64_t>(B) * num_q_heads * (splits / axb::kI8AttnCluster) * (head_dim + 2);
+  return static_cast<int64_t>(B) * num_q_heads * splits * (head_dim + 2);
 }
 
 // One new token a sequence: q [B, Nq, H] over the cache, into out [B, Nq, H] (which may be q).  `limit` (-1: none): sequences
-// behind it get zeros.
+// behind it get zeros. 
 extern "C" int axb_int8_decode_attn(const axb::Int8AttnCall* call, cudaStream_t stream) {
   using namespace axb;
   const Int8AttnCall& a = *call;
@@ -796,15 +801,13 @@ extern "C" int axb_int8_decode_attn(const axb::Int8AttnCall* call, cudaStream_t 
       a.num_kv_heads * ((a.num_q_heads / a.num_kv_heads + kI8AttnRows - 1) / kI8AttnRows) > 65535)
     return -10;
   if (a.B == 0) return 0;
-  if (a.splits > kI8AttnCluster &&
-      (a.scratch == nullptr || (reinterpret_cast<uintptr_t>(a.scratch) & 7) || a.splits % kI8AttnCluster))
-    return -10;
+  if (a.splits > kI8AttnCluster && (a.scratch == nullptr || (reinterpret_cast<uintptr_t>(a.scratch) & 7))) return -10;
   Int8AttnParams p = {};
   p.q = static_cast<const __nv_bfloat16*>(a.q);
   p.k_tops = static_cast<const __nv_bfloat16*>(a.k_tops), p.v_tops = static_cast<const __nv_bfloat16*>(a.v_tops);
   p.page_table = a.page_table, p.lengths = a.lengths;
   p.part_out = a.scratch;
-  p.part_ml = a.scratch == nullptr ? nullptr : a.scratch + a.B * a.num_q_heads * (a.splits / kI8AttnCluster) * a.head_dim;
+  p.part_ml = a.scratch == nullptr ? nullptr : a.scratch + a.B * a.num_q_heads * a.splits * a.head_dim;
   p.out = static_cast<__nv_bfloat16*>(a.out);
   p.status = a.status;
   p.page = FastDiv(static_cast<int>(a.page_size));

@@ -456,15 +456,17 @@ def append_int8(k: Tensor, v: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, pa
 
 
 def attention_splits(batch: int, num_kv_heads: int, group: int, max_len: int, sms: int = 148) -> int:
-    """KV splits of attention over the 8-bit cache: one wave of CTAs (three fit an SM; one takes a split, a KV head and eight
-    query heads), 64 tokens or more for each.  Beyond 8, which meet in a cluster, the clusters' parts are merged by a second
-    launch: for long sequences, and as many as clusters of 8 fit the GPU."""
+    """KV splits of attention over the 8-bit cache, a CTA for each split, KV head and eight query heads.  Up to eight are a cluster:
+    2, 4 or 8 of them, 64 tokens or more for each, as many as make up to 9 CTAs on 4 SMs (us with 1 / 2 / 4 / 8: 16 x 2048 tokens, 8
+    heads 20.4 18.3 24.1 29.2, 20 x 2048 25.2 22.6 26.6, 8 x 4000 of 64 dims 28.2 17.1 13.3 18.2, 8 x 2048, 32 heads 26.1 34.4).  Long
+    sequences of few heads take as many as fill most SMs with CTAs of three times the warps, and a second launch that joins them
+    (8 heads with 8 / 16 / 18 / 24: 16000 tokens 20.5 15.2 16.2 18.5, 130001 tokens 127 49.5 51.7 69, 4000 tokens 8.7 9.0; one head with
+    16 / 32 / 64 / 128: 60000 tokens 26.0 18.9 19.5 24.5)."""
     ctas = max(1, batch * num_kv_heads * ((group + 7) // 8))
-    splits = max(1, min(max_len // 64, 3 * sms // ctas))
-    if splits <= 8:
-        return splits
-    many = min((math.isqrt(max_len) // 4 + 4) // 8, 384 // ctas // 8) * 8
-    return many if many >= 24 else 8
+    if max_len > 8192 and ctas * 9 <= sms:
+        return min(48, max(9, 128 // ctas))
+    most = min(max_len // 64, 9 * sms // (4 * ctas))
+    return 8 if most >= 8 else 4 if most >= 4 else 2 if most >= 2 else 1
 
 
 def _attention_plain(q, k_pages, v_pages, page_table, lengths, scale):
@@ -491,7 +493,7 @@ def paged_decode_attention_int8(q: Tensor, k_pages: Int8Pages, v_pages: Int8Page
                                 out: Optional[Tensor] = None, scratch: Optional[Tensor] = None) -> Tensor:
     """q ``[B, Nq, H]``; page_table ``[B, max_pages]``, lengths ``[B]`` int32 (valid tokens per sequence; 0: zeros).  Query heads
     are grouped by KV head.  ``out`` may be ``q``, or overlap it.  ``scratch``: ``attention_scratch_floats`` fp32 values, for
-    more than eight splits (made a multiple of eight); calls that overlap on the GPU need one each.  Queries from 2^-40 to 2^56 and
+    more than eight splits; calls that overlap on the GPU need one each.  Queries from 2^-40 to 2^56 and
     pages' tops from 2^-40 to 2^50 keep their digits; larger ones may overflow.  Returns ``[B, Nq, H]``."""
     b, nq, h = q.shape
     device = q.get_device()
@@ -519,7 +521,6 @@ def _launch_attention(q, k_pages, v_pages, page_table, lengths, limit, out, scra
     if splits is None:
         splits = attention_splits(b, nkv, nq // nkv, max_pages * page_size)
     if splits > 8:
-        splits = -(-splits // 8) * 8
         floats = attention_scratch_floats(b, nq, h, splits)
         if scratch is None:
             scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
@@ -533,8 +534,7 @@ def _launch_attention(q, k_pages, v_pages, page_table, lengths, limit, out, scra
 
 
 def attention_scratch_floats(batch: int, num_q_heads: int, head_dim: int, splits: int) -> int:
-    """fp32 values that the parts of more than eight splits take (a multiple of eight)."""
-    splits = -(-splits // 8) * 8 if splits > 8 else splits
+    """fp32 values that the parts of more than eight splits take."""
     f, _ = _entries.get("axb_int8_attn_scratch_floats") or _entry("axb_int8_attn_scratch_floats")
     return f(batch, num_q_heads, head_dim, splits)
 

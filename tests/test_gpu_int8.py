@@ -443,8 +443,8 @@ def test_scratch_that_does_not_fit_is_refused():
     k_pages, v_pages, table = _cache(1, 64, 16, 1, 128)
     q, lengths = _normal(_gen(1), 1, 2, 128).bfloat16(), torch.tensor([1000], dtype=torch.int32, device="cuda")
     floats = int8_ops.attention_scratch_floats(1, 2, 128, 16)
-    assert floats == 2 * 2 * 130 and int8_ops.attention_scratch_floats(1, 2, 128, 8) == 0
-    call = lambda scratch: int8_ops.paged_decode_attention_int8(q, k_pages, v_pages, table, lengths, splits=9, scratch=scratch)  # noqa: E731
+    assert floats == 2 * 16 * 130 and int8_ops.attention_scratch_floats(1, 2, 128, 8) == 0
+    call = lambda scratch: int8_ops.paged_decode_attention_int8(q, k_pages, v_pages, table, lengths, splits=16, scratch=scratch)  # noqa: E731
     for bad in (torch.empty(floats - 1, device="cuda"), torch.empty(floats, device="cuda").half(), torch.empty(floats),
                 torch.empty(2 * floats, device="cuda")[::2], torch.empty(floats + 1, device="cuda")[1:]):
         with pytest.raises(ValueError):
