@@ -28,22 +28,24 @@ struct Int8Scale {
   __device__ __forceinline__ bool empty() const { return inverse == 0.f; }
 };
 
-// Codes of eight values.  A product with the rounded kFactor / A is within 2^-15 of kFactor x / A, so its rounding is right
-// unless it ends next to a half; there kFactor x - c A tells whether a neighbour is nearer.  With x and A of 8 bits (a cache) or
-// of 16 (products of two bf16 numbers) that difference is exact.
+// Codes of eight values as bytes, and as floats.  x times the rounded kFactor / A is within 2^-15 of kFactor x / A, so its
+// rounding is right unless it ends next to a half; there kFactor x - c A tells whether a neighbour is nearer.  With x and A of 8
+// bits (a cache) or of 16 (products of two bf16 numbers) that difference is exact.
 template <int kFactor>
-__device__ __forceinline__ void int8_levels(const float (&x)[8], const Int8Scale<kFactor>& s, float (&level)[8]) {
+__device__ __forceinline__ uint2 int8_codes(const float (&x)[8], const Int8Scale<kFactor>& s, float (&level)[8]) {
   if (s.empty()) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) level[i] = 0.f;
-    return;
+    return make_uint2(0, 0);
   }
   float off_by = 0.f;
+  uint32_t u[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float t = x[i] * s.inverse;
-    level[i] = (t + kInt8Whole) - kInt8Whole;
-    off_by = fmaxf(off_by, fabsf(t - level[i]));
+    const float whole = fmaf(x[i], s.inverse, kInt8Whole);
+    u[i] = __float_as_uint(whole);
+    level[i] = whole - kInt8Whole;
+    off_by = fmaxf(off_by, fabsf(fmaf(x[i], s.inverse, -level[i])));
   }
   if (off_by > 0.5f - 0x1p-14f) {
     const float half = 0.5f * s.top;
@@ -53,15 +55,9 @@ __device__ __forceinline__ void int8_levels(const float (&x)[8], const Int8Scale
       const bool odd = static_cast<int>(level[i]) & 1;
       if (rest > half || (rest == half && odd)) level[i] += 1.f;
       if (rest < -half || (rest == -half && odd)) level[i] -= 1.f;
+      u[i] = __float_as_uint(level[i] + kInt8Whole);
     }
   }
-}
-
-// Eight codes as bytes.
-__device__ __forceinline__ uint2 int8_pack(const float (&level)[8]) {
-  uint32_t u[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(level[i] + kInt8Whole);
   return make_uint2(__byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410),
                     __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410));
 }

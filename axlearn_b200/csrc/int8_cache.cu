@@ -41,18 +41,19 @@ struct Int8AppendParams {
 };
 
 constexpr int kInt8AppendThreads = 256;
-constexpr int kInt8Held = 8;  // rows that a thread keeps
+constexpr int kInt8Held = 8;  // 16-byte units of rows that a thread keeps in shared memory
 constexpr int kInt8QRows = 4;
 
 // A unit is what a call brings for one block: up to a page's tokens of the keys, or the values, of a KV head.  Its kWarps warps
 // hold them in registers while the largest magnitude is found (further rows are read again), and turn the codes that are
 // there already, if the magnitude has grown.  Units behind those rotate kInt8QRows times kRows query heads of a token.
 template <int H, int kWarps>
-__global__ void __launch_bounds__(kInt8AppendThreads)
+__global__ void __launch_bounds__(kInt8AppendThreads, 4)
 int8_append_kernel(Int8AppendParams p) {
   chain_link();
   constexpr int kLanes = H / 8, kThreads = 32 * kWarps, kRows = kThreads / kLanes, kUnits = kInt8AppendThreads / kThreads;
   __shared__ uint32_t s_top[kInt8AppendThreads / 32];
+  __shared__ uint4 s_held[kInt8Held][kInt8AppendThreads];  // (a thread's own: no bank conflicts, no barriers)
   const int in = threadIdx.x % kThreads, place = threadIdx.x / kThreads;
   const int l8 = in % kLanes, row_at = in / kLanes;
   uint32_t unit = blockIdx.x * kUnits + place;
@@ -104,17 +105,22 @@ int8_append_kernel(Int8AppendParams p) {
   const __nv_bfloat16* src = source.x + b * source.b + t0 * source.t + head * source.h + l8 * 8;
   const float2* angle = is_v || p.angle == nullptr
                             ? nullptr : p.angle + (static_cast<int64_t>(begin) + t0) * (H / 2) + l8 * 4;
-  auto load = [&](int r) {
-    const uint4 x = *reinterpret_cast<const uint4*>(src + r * source.t);
-    return angle == nullptr ? x : rotate8(x, angle + static_cast<int64_t>(r) * (H / 2));
+  src += row_at * source.t;
+  if (angle != nullptr) angle += static_cast<int64_t>(row_at) * (H / 2);
+  const int64_t src_step = kRows * source.t;
+  auto load = [&](int i) {  // row row_at + i kRows
+    const uint4 x = *reinterpret_cast<const uint4*>(src + i * src_step);
+    return angle == nullptr ? x : rotate8(x, angle + static_cast<int64_t>(i) * (kRows * H / 2));
   };
   auto largest = [](uint32_t m, const uint4& x) {  // of both halves; NaN is the largest of all
     m = __vmaxu2(m, __vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu));
     return __vmaxu2(m, __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
   };
-  uint4 x[kInt8Held];
+  const int mine = row_at < rows ? (rows - row_at + kRows - 1) / kRows : 0, held = min(mine, kInt8Held);  // rows of this thread
 #pragma unroll
-  for (int i = 0; i < kInt8Held; ++i) x[i] = row_at + i * kRows < rows ? load(row_at + i * kRows) : zeros;
+  for (int i = 0; i < kInt8Held; ++i)
+    if (i < mine) cp16(&s_held[i][threadIdx.x], src + i * src_step);
+  cp_commit();
   // The place: a sequence that starts ahead of its first position has none.
   const Int8Pool& pool = is_v ? p.v_pool : p.k_pool;
   const int64_t col = static_cast<int64_t>(col0) + j;
@@ -126,9 +132,14 @@ int8_append_kernel(Int8AppendParams p) {
   const uint32_t old = placed && row0 > 0
                            ? static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(pool.tops + block) & 0x7fff) << 16 : 0u;
   uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < kInt8Held; ++i) m = largest(m, x[i]);
-  for (int r = row_at + kInt8Held * kRows; r < rows; r += kRows) m = largest(m, load(r));
+  cp_wait_all();
+#pragma unroll 4
+  for (int i = 0; i < held; ++i) {
+    uint4& x = s_held[i][threadIdx.x];
+    if (angle != nullptr) x = rotate8(x, angle + i * (kRows * H / 2));
+    m = largest(m, x);
+  }
+  for (int i = kInt8Held; i < mine; ++i) m = largest(m, load(i));
   m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
   if constexpr (kWarps > 1) {
     if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = m;
@@ -151,31 +162,32 @@ int8_append_kernel(Int8AppendParams p) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           f[i] = by * static_cast<float>(static_cast<int8_t>((i < 4 ? was.x : was.y) >> (8 * (i & 3))));
-        int8_levels(f, turn, level);
-        *at = int8_pack(level);
+        *at = int8_codes(f, turn, level);
       }
     }
   }
   const float back = s.top * (1.f / 127.f);
-  auto hold = [&](int r, const uint4& v) {
+  codes += row_at * H;
+  if (out != nullptr) out += row_at * p.out_t;
+  const int64_t out_step = kRows * p.out_t;
+  auto hold = [&](int i, const uint4& v) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     float f[8], level[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 two = unpack2(w[i]);
-      f[2 * i] = two.x, f[2 * i + 1] = two.y;
+    for (int j = 0; j < 4; ++j) {
+      const float2 two = unpack2(w[j]);
+      f[2 * j] = two.x, f[2 * j + 1] = two.y;
     }
-    int8_levels(f, s, level);
-    if (placed) *reinterpret_cast<uint2*>(codes + static_cast<int64_t>(r) * H) = int8_pack(level);
+    const uint2 bytes = int8_codes(f, s, level);
+    if (placed) *reinterpret_cast<uint2*>(codes + i * (kRows * H)) = bytes;
     if (out != nullptr)
-      *reinterpret_cast<uint4*>(out + r * p.out_t) =
+      *reinterpret_cast<uint4*>(out + i * out_step) =
           make_uint4(pack2(level[0] * back, level[1] * back), pack2(level[2] * back, level[3] * back),
                      pack2(level[4] * back, level[5] * back), pack2(level[6] * back, level[7] * back));
   };
-#pragma unroll
-  for (int i = 0; i < kInt8Held; ++i)
-    if (row_at + i * kRows < rows) hold(row_at + i * kRows, x[i]);
-  for (int r = row_at + kInt8Held * kRows; r < rows; r += kRows) hold(r, load(r));
+#pragma unroll 1
+  for (int i = 0; i < held; ++i) hold(i, s_held[i][threadIdx.x]);
+  for (int i = kInt8Held; i < mine; ++i) hold(i, load(i));
 }
 
 template <int H, int kWarps>

@@ -104,8 +104,7 @@ int8_rows_kernel(Int8RowsParams p) {
     const int v = threadIdx.x + i * blockDim.x;
     if (v >= vectors) continue;
     float level[8];
-    int8_levels(f[i], s, level);
-    reinterpret_cast<uint2*>(p.codes + row * p.dim)[v] = int8_pack(level);
+    reinterpret_cast<uint2*>(p.codes + row * p.dim)[v] = int8_codes(f[i], s, level);
     if (p.values != nullptr)
       reinterpret_cast<uint4*>(p.values + row * p.dim)[v] =
           make_uint4(pack2(level[0] * scale, level[1] * scale), pack2(level[2] * scale, level[3] * scale),
