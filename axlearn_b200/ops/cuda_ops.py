@@ -132,6 +132,11 @@ def current_device() -> int:
     return torch.cuda.current_device() if _device_index is None else _device_index()
 
 
+def raw_stream(device: int) -> int:
+    """The current stream of the device with that index."""
+    return torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device)
+
+
 def _transformed() -> bool:
     """Whether forward-mode differentiation or a function transform is on, which know torch's operators but not a kernel
     behind their back; unknown counts as on."""

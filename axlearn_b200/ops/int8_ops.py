@@ -75,7 +75,7 @@ def _call(device: int, name: str, *words) -> None:
         with torch.cuda.device(device):
             return _call(device, name, *words)
     f, pack = _entries.get(name) or _entry(name)
-    return cuda_ops._check(f(pack(*words), cuda_ops._stream()), name)  # pylint: disable=protected-access
+    return cuda_ops._check(f(pack(*words), cuda_ops.raw_stream(device)), name)  # pylint: disable=protected-access
 
 
 def _status(device: int) -> int:
@@ -153,10 +153,18 @@ def swiglu_int8(gu: Tensor) -> Int8Rows:
     return _launch_rows(gu, gu.shape[-1] // 2, True)
 
 
+def _row_scales(x: Tensor) -> Tensor:
+    """Room for a scale of each row (from a whole number, which torch takes 0.8 us faster than a tuple)."""
+    shape = x.shape
+    if len(shape) == 2:
+        return torch.empty(shape[0], dtype=torch.float32, device=x.device)
+    return torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+
+
 def _launch_rows(x: Tensor, dim: int, gated: bool) -> Int8Rows:
     shape = x.shape[:-1]
     codes = torch.empty(shape + (dim,), dtype=torch.int8, device=x.device)
-    scales = torch.empty(shape, dtype=torch.float32, device=x.device)
+    scales = _row_scales(x)
     if codes.numel():
         x, rows, pitch = _row_operand(x, x.shape[-1])
         _call(x.get_device(), "axb_int8_rows", x.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, dim, pitch, gated)
@@ -191,7 +199,7 @@ def add_rms_norm_int8(x: Tensor, residual: Optional[Tensor], scale: Tensor, eps:
         residual = _aligned(residual)
         total, other = torch.empty_like(x), residual.data_ptr()
     scale = _aligned(scale)
-    rows = Int8Rows(torch.empty_like(x, dtype=torch.int8), torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device))
+    rows = Int8Rows(torch.empty_like(x, dtype=torch.int8), _row_scales(x))
     held = torch.empty_like(x) if values else None
     if n:
         _call(x.get_device(), "axb_int8_add_rms_norm", x.data_ptr(), other, scale.data_ptr(), total.data_ptr() if other else 0,
@@ -348,7 +356,8 @@ def page_values(pages: Int8Pages, dtype: torch.dtype = torch.float32) -> Tensor:
 
 def _check_pages(k_pages: Int8Pages, v_pages: Int8Pages, page_table: Tensor, batch: int, heads: int, head_dim: int,
                  device: int) -> tuple:
-    """``(pages, Nkv, page size, columns of the table)`` of a cache that fits; ``device``: index of the operands' one."""
+    """``(pages, Nkv, page size, columns of the table)`` and where codes and tops lie, of a cache that fits; ``device``: index of the
+    operands' one."""
     (kc, kt), (vc, vt) = k_pages, v_pages
     shape = kc.shape
     num_pages, nkv, page_size, held = shape if len(shape) == 4 else (0, 0, 0, 0)
@@ -359,17 +368,18 @@ def _check_pages(k_pages: Int8Pages, v_pages: Int8Pages, page_table: Tensor, bat
                          f"heads of {head_dim} (64 or 128; a multiple of {PAGE_UNIT} tokens a page)")
     if num_pages * nkv * page_size >= 2 ** 31 - 1 - page_size:
         raise ValueError(f"8-bit pages {tuple(shape)} have 2^31 rows or more")
+    at_k, at_v = kc.data_ptr(), vc.data_ptr()
     if (kc.dtype is not torch.int8 or vc.dtype is not torch.int8 or kt.dtype is not torch.bfloat16 or vt.dtype is not torch.bfloat16
             or not (kc.get_device() == vc.get_device() == kt.get_device() == vt.get_device() == device)
             or not (kc.is_contiguous() and vc.is_contiguous() and kt.is_contiguous() and vt.is_contiguous())
-            or (kc.data_ptr() | vc.data_ptr()) % 16):
+            or (at_k | at_v) % 16):
         raise ValueError("8-bit pages are contiguous, 16-byte aligned int8 and bf16 tensors on the operands' device")
     table = page_table.shape
     if (page_table.dtype is not torch.int32 or len(table) != 2 or table[0] != batch or page_table.get_device() != device
             or not page_table.is_contiguous()):
         raise ValueError(f"a page table is a contiguous int32 matrix of {batch} rows on the operands' device: {tuple(table)} "
                          f"{page_table.dtype}")
-    return num_pages, nkv, page_size, table[1]
+    return (num_pages, nkv, page_size, table[1]), (at_k, kt.data_ptr(), at_v, vt.data_ptr())
 
 
 def _check_counts(counts: Tensor, batch: int, name: str, device: int) -> None:
@@ -430,11 +440,11 @@ def append_int8(k: Tensor, v: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, pa
     largest magnitude.  What a page holds behind the new tokens has no meaning; other pages do not change.  ``values``: also
     returns what the cache stands for at these tokens, ``(k, v)`` of the inputs' shape and type, zeros behind ``live``.  No two
     columns of the page table may name the same page where it is written."""
-    b, t, nkv, h = k.shape
-    if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
-        raise ValueError(f"k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} differ")
-    device = k.get_device()
-    num_pages, held, page_size, max_pages = _check_pages(k_pages, v_pages, page_table, b, nkv, h, device)
+    shape, device = k.shape, k.get_device()
+    b, t, nkv, h = shape
+    if v.shape != shape or v.dtype is not k.dtype or v.get_device() != device:
+        raise ValueError(f"k {tuple(shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} differ")
+    (num_pages, held, page_size, max_pages), pools = _check_pages(k_pages, v_pages, page_table, b, nkv, h, device)
     if held != nkv:
         raise ValueError(f"pages of {held} heads for {nkv}")
     _check_counts(start, b, "start", device)
@@ -447,10 +457,10 @@ def append_int8(k: Tensor, v: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, pa
         out = _append_plain(k, v, k_pages, v_pages, page_table, start, live)
         return tuple(out) if values else None
     k, v = _aligned_rows(k), _aligned_rows(v)
-    out = (k.new_empty((b, t, nkv, h)), k.new_empty((b, t, nkv, h))) if values else None
-    _call(device, "axb_int8_append", k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], out[0].data_ptr() if values else 0,
-          out[1].data_ptr() if values else 0, k_pages.codes.data_ptr(), k_pages.tops.data_ptr(), v_pages.codes.data_ptr(),
-          v_pages.tops.data_ptr(), page_table.data_ptr(), start.data_ptr(), 0 if live is None else live.data_ptr(), b, t, nkv, h,
+    k_strides, v_strides = k.stride(), v.stride()
+    out = (k.new_empty(shape), k.new_empty(shape)) if values else None
+    _call(device, "axb_int8_append", k.data_ptr(), v.data_ptr(), *k_strides[:3], *v_strides[:3], out[0].data_ptr() if values else 0,
+          out[1].data_ptr() if values else 0, *pools, page_table.data_ptr(), start.data_ptr(), 0 if live is None else live.data_ptr(), b, t, nkv, h,
           page_size, max_pages, num_pages, _status(device))
     return out
 
@@ -497,7 +507,7 @@ def paged_decode_attention_int8(q: Tensor, k_pages: Int8Pages, v_pages: Int8Page
     pages' tops from 2^-40 to 2^50 keep their digits; larger ones may overflow.  Returns ``[B, Nq, H]``."""
     b, nq, h = q.shape
     device = q.get_device()
-    cache = _check_pages(k_pages, v_pages, page_table, b, nq, h, device)
+    cache, pools = _check_pages(k_pages, v_pages, page_table, b, nq, h, device)
     _check_counts(lengths, b, "lengths", device)
     scale = 1.0 / math.sqrt(h) if softmax_scale is None else softmax_scale
     _check_scale(scale)
@@ -512,12 +522,12 @@ def paged_decode_attention_int8(q: Tensor, k_pages: Int8Pages, v_pages: Int8Page
         q = q.clone(memory_format=torch.contiguous_format)
     if out is None:
         out = torch.empty_like(q)
-    _launch_attention(q, k_pages, v_pages, page_table, lengths, -1, out, scratch, b, nq, h, *cache, splits, scale, device)
+    _launch_attention(q, pools, page_table, lengths, -1, out, scratch, b, nq, h, cache, splits, scale, device)
     return out
 
 
-def _launch_attention(q, k_pages, v_pages, page_table, lengths, limit, out, scratch, b, nq, h, num_pages, nkv, page_size, max_pages,
-                      splits, scale, device):
+def _launch_attention(q, pools, page_table, lengths, limit, out, scratch, b, nq, h, cache, splits, scale, device):
+    num_pages, nkv, page_size, max_pages = cache
     if splits is None:
         splits = attention_splits(b, nkv, nq // nkv, max_pages * page_size)
     if splits > 8:
@@ -527,8 +537,7 @@ def _launch_attention(q, k_pages, v_pages, page_table, lengths, limit, out, scra
         elif (scratch.numel() < floats or scratch.dtype != torch.float32 or scratch.get_device() != device
               or not scratch.is_contiguous() or scratch.data_ptr() % 8):
             raise ValueError(f"scratch is {floats} contiguous fp32 values on {q.device}, 8-byte aligned")
-    _call(device, "axb_int8_decode_attn", q.data_ptr(), k_pages.codes.data_ptr(), k_pages.tops.data_ptr(), v_pages.codes.data_ptr(),
-          v_pages.tops.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(),
+    _call(device, "axb_int8_decode_attn", q.data_ptr(), *pools, page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(),
           0 if scratch is None else scratch.data_ptr(), limit, b, nq, nkv, h, page_size, max_pages, num_pages, splits, scale,
           _status(device))
 
@@ -560,7 +569,8 @@ def rope_decode_attention_int8(qkv: Tensor, k_pages: Int8Pages, v_pages: Int8Pag
     if qkv.dim() != 2:
         raise ValueError(f"a step takes one token a sequence, [B, width]: {tuple(qkv.shape)}")
     b, device = qkv.shape[0], qkv.get_device()
-    num_pages, _, page_size, max_pages = cache = _check_pages(k_pages, v_pages, page_table, b, num_q_heads, h, device)
+    cache, pools = _check_pages(k_pages, v_pages, page_table, b, num_q_heads, h, device)
+    num_pages, _, page_size, max_pages = cache
     _check_counts(lengths, b, "lengths", device)
     _check_scale(softmax_scale)
     _no_gradient("rope_decode_attention_int8", qkv, k_pages.tops, v_pages.tops, table)
@@ -577,11 +587,9 @@ def rope_decode_attention_int8(qkv: Tensor, k_pages: Int8Pages, v_pages: Int8Pag
         _append_plain(k, v, k_pages, v_pages, page_table, lengths - 1, (lengths > 0).to(torch.int32))
         return paged_decode_attention_int8(q[:, 0], k_pages, v_pages, page_table, lengths, softmax_scale=softmax_scale)
     out = qkv.new_empty((b, num_q_heads, h))  # the rotated queries, then what they attend to
-    _call(device, "axb_int8_rope_append", qkv.data_ptr(), out.data_ptr(), k_pages.codes.data_ptr(), k_pages.tops.data_ptr(),
-          v_pages.codes.data_ptr(), v_pages.tops.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), 0, table.data_ptr(),
+    _call(device, "axb_int8_rope_append", qkv.data_ptr(), out.data_ptr(), *pools, page_table.data_ptr(), lengths.data_ptr(), 0, table.data_ptr(),
           table.shape[0], b, 1, num_q_heads, nkv, h, page_size, max_pages, num_pages, _status(device))
-    _launch_attention(out, k_pages, v_pages, page_table, lengths, limit, out, scratch, b, num_q_heads, h, *cache, splits, softmax_scale,
-                      device)
+    _launch_attention(out, pools, page_table, lengths, limit, out, scratch, b, num_q_heads, h, cache, splits, softmax_scale, device)
     return out
 
 
@@ -594,7 +602,7 @@ def prompt_attention_int8(qkv: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, p
     nkv, h = _check_packed(qkv, k_pages, table, num_q_heads)
     b, t, _ = qkv.shape
     device = qkv.get_device()
-    num_pages, _, page_size, max_pages = _check_pages(k_pages, v_pages, page_table, b, num_q_heads, h, device)
+    (num_pages, _, page_size, max_pages), pools = _check_pages(k_pages, v_pages, page_table, b, num_q_heads, h, device)
     if table.shape[0] < t or max_pages * page_size < t:
         raise ValueError(f"{b} x {t} tokens, a rotation table of {table.shape[0]} positions, a page table {tuple(page_table.shape)}")
     if live is not None:
@@ -613,8 +621,7 @@ def prompt_attention_int8(qkv: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, p
         return out.reshape(b, t, num_q_heads * h)
     from axlearn_b200.ops import decode_ops
 
-    _call(device, "axb_int8_rope_append", qkv.data_ptr(), 0, k_pages.codes.data_ptr(), k_pages.tops.data_ptr(),
-          v_pages.codes.data_ptr(), v_pages.tops.data_ptr(), page_table.data_ptr(), 0, 0 if live is None else live.data_ptr(),
+    _call(device, "axb_int8_rope_append", qkv.data_ptr(), 0, *pools, page_table.data_ptr(), 0, 0 if live is None else live.data_ptr(),
           table.data_ptr(), table.shape[0], b, t, num_q_heads, nkv, h, page_size, max_pages, num_pages, _status(device))
     with _on(qkv.device):
         return decode_ops.packed_prompt_attention(qkv, num_q_heads=num_q_heads, num_kv_heads=nkv, softmax_scale=softmax_scale)
