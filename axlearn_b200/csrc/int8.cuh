@@ -15,51 +15,56 @@ namespace axb {
 constexpr float kInt8Least = 0x1p-119f;
 constexpr float kInt8Whole = 12582912.f;  // 1.5 * 2^23: whole numbers are the last bits
 
-// What turns values into codes: A, and kFactor / A (0 in blocks of zeros and of NaN).  kFactor is 127, or 1 where values are
-// codes times another block's A.
+// What turns values into codes.  kFactor is 127, or 1 where values are codes times another block's A.
 template <int kFactor = 127>
 struct Int8Scale {
-  float top, inverse;
-  __device__ __forceinline__ explicit Int8Scale(float a) : top(a), inverse(0.f) {
+  float top;                          // A, as the block has it: NaN, or 0 of a block of zeros
+  float factor, divisor, reciprocal;  // kFactor and A, both 2^-8 of it where kFactor x could leave fp32
+  __device__ __forceinline__ explicit Int8Scale(float a) : top(a) {
     if (!(a <= FLT_MAX)) top = __int_as_float(0x7fffffff);
     else if (a < kInt8Least) top = 0.f;
-    else inverse = kFactor / a;
+    const float down = a > 0x1p100f ? 0x1p-8f : 1.f;
+    factor = kFactor * down, divisor = a * down;
+    reciprocal = top > 0.f ? __frcp_rn(divisor) : 0.f;
   }
-  __device__ __forceinline__ bool empty() const { return inverse == 0.f; }
+  __device__ __forceinline__ bool empty() const { return reciprocal == 0.f; }
 };
 
-// Codes of eight values as bytes, and as floats.  x times the rounded kFactor / A is within 2^-15 of kFactor x / A, so its
-// rounding is right unless it ends next to a half; there kFactor x - c A tells whether a neighbour is nearer.  With x and A of 8
-// bits (a cache) or of 16 (products of two bf16 numbers) that difference is exact.
+// Codes of eight values as bytes.  The quotient is a product with the reciprocal and one correction by the exact remainder, which
+// rounds it correctly in 32 bits; with x and A of 8 bits (a cache) or of 16 (products of two bf16 numbers) a quotient that is not
+// k + 1/2 is off it by more than half a unit, so adding 1.5 2^23 rounds as in exact arithmetic.  Ties are no rare case to be left
+// to a branch: x = A / 2 is 63.5 (every second vector of 256 values has one; 16384 x 4096 rows 49.1 us with such a branch).
 template <int kFactor>
-__device__ __forceinline__ uint2 int8_codes(const float (&x)[8], const Int8Scale<kFactor>& s, float (&level)[8]) {
-  if (s.empty()) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) level[i] = 0.f;
-    return make_uint2(0, 0);
-  }
-  float off_by = 0.f;
+__device__ __forceinline__ uint2 int8_codes(const float (&x)[8], const Int8Scale<kFactor>& s) {
+  if (s.empty()) return make_uint2(0, 0);
   uint32_t u[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float whole = fmaf(x[i], s.inverse, kInt8Whole);
-    u[i] = __float_as_uint(whole);
-    level[i] = whole - kInt8Whole;
-    off_by = fmaxf(off_by, fabsf(fmaf(x[i], s.inverse, -level[i])));
-  }
-  if (off_by > 0.5f - 0x1p-14f) {
-    const float half = 0.5f * s.top;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float rest = fmaf(static_cast<float>(kFactor), x[i], -level[i] * s.top);
-      const bool odd = static_cast<int>(level[i]) & 1;
-      if (rest > half || (rest == half && odd)) level[i] += 1.f;
-      if (rest < -half || (rest == -half && odd)) level[i] -= 1.f;
-      u[i] = __float_as_uint(level[i] + kInt8Whole);
-    }
+    const float y = x[i] * s.factor, q = y * s.reciprocal;
+    u[i] = __float_as_uint(fmaf(fmaf(-q, s.divisor, y), s.reciprocal, q) + kInt8Whole);
   }
   return make_uint2(__byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410),
                     __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410));
+}
+
+// What codes stand for, rounded to bf16: times A / 127.
+__device__ __forceinline__ uint4 int8_values(uint2 codes, float scale) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t two = (i & 2 ? codes.y : codes.x) >> (16 * (i & 1));
+    const __nv_bfloat162 v = __floats2bfloat162_rn(static_cast<float>(static_cast<int8_t>(two)) * scale,
+                                                   static_cast<float>(static_cast<int8_t>(two >> 8)) * scale);
+    w[i] = reinterpret_cast<const uint32_t&>(v);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The larger magnitude; NaN is the largest of all.
+__device__ __forceinline__ float int8_larger(float top, float x) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(top), "f"(fabsf(x)));
+  return y;
 }
 
 // A bad index that the device found: code 5 of the status word.

@@ -158,11 +158,11 @@ int8_append_kernel(Int8AppendParams p) {
       for (int r = row_at; r < row0; r += kRows) {
         uint2* at = reinterpret_cast<uint2*>(codes + static_cast<int64_t>(r - row0) * H);
         const uint2 was = *at;
-        float f[8], level[8];
+        float f[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           f[i] = by * static_cast<float>(static_cast<int8_t>((i < 4 ? was.x : was.y) >> (8 * (i & 3))));
-        *at = int8_codes(f, turn, level);
+        *at = int8_codes(f, turn);
       }
     }
   }
@@ -172,18 +172,15 @@ int8_append_kernel(Int8AppendParams p) {
   const int64_t out_step = kRows * p.out_t;
   auto hold = [&](int i, const uint4& v) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    float f[8], level[8];
+    float f[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 two = unpack2(w[j]);
       f[2 * j] = two.x, f[2 * j + 1] = two.y;
     }
-    const uint2 bytes = int8_codes(f, s, level);
+    const uint2 bytes = int8_codes(f, s);
     if (placed) *reinterpret_cast<uint2*>(codes + i * (kRows * H)) = bytes;
-    if (out != nullptr)
-      *reinterpret_cast<uint4*>(out + i * out_step) =
-          make_uint4(pack2(level[0] * back, level[1] * back), pack2(level[2] * back, level[3] * back),
-                     pack2(level[4] * back, level[5] * back), pack2(level[6] * back, level[7] * back));
+    if (out != nullptr) *reinterpret_cast<uint4*>(out + i * out_step) = int8_values(bytes, back);
   };
 #pragma unroll 1
   for (int i = 0; i < held; ++i) hold(i, s_held[i][threadIdx.x]);

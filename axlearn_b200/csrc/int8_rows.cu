@@ -22,7 +22,7 @@ struct Int8RowsParams {
   float* scales;
   __nv_bfloat16 *total, *values;   // null: not wanted
   int dim;
-  float eps;
+  float inverse_dim, eps;
 };
 
 template <int KIND, int VPT>
@@ -35,8 +35,7 @@ int8_rows_kernel(Int8RowsParams p) {
   const int vectors = p.dim >> 3, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const uint4* x = reinterpret_cast<const uint4*>(p.x + (KIND == kRowsNorm ? row * p.dim : row * p.ldx));
   float f[VPT][8];
-  uint32_t top = 0;  // bits of the largest magnitude: NaN is the largest of all
-  float sum = 0.f;
+  float most[4] = {}, sum = 0.f;
   {
     uint4 a[VPT], b[VPT], w[VPT];
 #pragma unroll
@@ -72,14 +71,17 @@ int8_rows_kernel(Int8RowsParams p) {
           t.x *= by.x, t.y *= by.y;
         } else if (KIND == kRowsSwiglu) {
           const float2 up = unpack2(o[j]);
-          t.x = t.x / (1.f + expf(-t.x)) * up.x;
-          t.y = t.y / (1.f + expf(-t.y)) * up.y;
+          // (Two units of the quotient and |t| 2^-24 of the exponential: nothing beside half a code.)
+          t.x = __fdividef(t.x, 1.f + __expf(-t.x)) * up.x;
+          t.y = __fdividef(t.y, 1.f + __expf(-t.y)) * up.y;
         }
         f[i][2 * j] = t.x, f[i][2 * j + 1] = t.y;
-        top = max(top, max(__float_as_uint(t.x) & 0x7fffffffu, __float_as_uint(t.y) & 0x7fffffffu));
+        most[j] = int8_larger(int8_larger(most[j], t.x), t.y);
       }
     }
   }
+  // (Bits are in the same order, NaN at the end.)
+  uint32_t top = __float_as_uint(int8_larger(int8_larger(most[0], most[1]), int8_larger(most[2], most[3])));
   top = __reduce_max_sync(0xffffffffu, top);
   if (KIND == kRowsNorm) {
 #pragma unroll
@@ -96,19 +98,17 @@ int8_rows_kernel(Int8RowsParams p) {
     }
   }
   const Int8Scale<> s(__uint_as_float(top));
-  float scale = s.top / 127.f;
-  if (KIND == kRowsNorm) scale *= 1.f / sqrtf(sum / p.dim + p.eps);
+  float scale = 0.f;  // (one thread's, unless all need it)
+  if (threadIdx.x == 0 || p.values != nullptr) scale = s.top / 127.f;
+  if (KIND == kRowsNorm) scale *= rsqrtf(fmaf(sum, p.inverse_dim, p.eps));
   if (threadIdx.x == 0) p.scales[row] = scale;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
     if (v >= vectors) continue;
-    float level[8];
-    reinterpret_cast<uint2*>(p.codes + row * p.dim)[v] = int8_codes(f[i], s, level);
-    if (p.values != nullptr)
-      reinterpret_cast<uint4*>(p.values + row * p.dim)[v] =
-          make_uint4(pack2(level[0] * scale, level[1] * scale), pack2(level[2] * scale, level[3] * scale),
-                     pack2(level[4] * scale, level[5] * scale), pack2(level[6] * scale, level[7] * scale));
+    const uint2 codes = int8_codes(f[i], s);
+    reinterpret_cast<uint2*>(p.codes + row * p.dim)[v] = codes;
+    if (p.values != nullptr) reinterpret_cast<uint4*>(p.values + row * p.dim)[v] = int8_values(codes, scale);
   }
 }
 
@@ -116,7 +116,7 @@ constexpr int kInt8RowsMost = 1024 * 8 * 8;  // values of a row
 
 template <int KIND>
 static int int8_rows(const Int8RowsParams& p, int64_t rows, cudaStream_t stream) {
-  const int vectors = p.dim / 8, most = rows >= 296 ? 128 : 512;
+  const int vectors = p.dim / 8, most = rows >= 296 ? 128 : 1024;
   int vpt = 1;
   while (vpt < 8 && (vectors + vpt - 1) / vpt > (vpt < 4 ? most : 1024)) vpt *= 2;
   const int threads = ((vectors + vpt - 1) / vpt + 31) / 32 * 32;
@@ -164,6 +164,6 @@ extern "C" int axb_int8_add_rms_norm(const axb::Int8NormCall* call, cudaStream_t
   p.weight = static_cast<const __nv_bfloat16*>(a.weight);
   p.codes = static_cast<int8_t*>(a.codes), p.scales = a.scales;
   p.total = static_cast<__nv_bfloat16*>(a.total), p.values = static_cast<__nv_bfloat16*>(a.values);
-  p.dim = static_cast<int>(a.dim), p.eps = static_cast<float>(a.eps);
+  p.dim = static_cast<int>(a.dim), p.inverse_dim = 1.f / p.dim, p.eps = static_cast<float>(a.eps);
   return int8_rows<kRowsNorm>(p, a.rows, stream);
 }
