@@ -4,18 +4,15 @@
 // KV head are a block, and one run of memory; page table [B, max_pages], H 64 or 128, page_size a multiple of 16.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
-#include <float.h>
 #include <math.h>
 #include <stdint.h>
 
 #include "cache_rows.cuh"
 #include "chain.cuh"
 #include "cluster.cuh"
-#include "host_utils.cuh"
 #include "int8.cuh"
 #include "mma_sync.cuh"
 #include "opt_in.cuh"
-#include "sm100.cuh"
 
 namespace axb {
 
@@ -213,6 +210,7 @@ static int int8_append(Int8AppendParams& p, int B, int page_size, int head_dim, 
 
 struct Int8AttnParams {
   const __nv_bfloat16* q;  // [B, Nq, H]
+  const uint8_t *k_codes, *v_codes;
   const __nv_bfloat16 *k_tops, *v_tops;
   const int* page_table;
   const int* lengths;
@@ -262,13 +260,19 @@ __device__ __forceinline__ void int8_mma_add(float (&d)[4], const uint32_t (&a)[
 // Sums of products of codes and a digit of q, from kInt8Sums: whole numbers below 2^22 that are the last bits of a float.
 constexpr int kInt8Sums = 0x4b400000;  // 1.5 * 2^23
 template <bool kSigned>
-__device__ __forceinline__ void int8_mma_sum(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void int8_mma_sum(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const int* c) {
   if constexpr (kSigned)
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
   else
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
+}
+
+__device__ __forceinline__ void int8_copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
 // Two matrices of 16 keys x 16 dims, a row a lane (0 .. 15, 16 .. 31): lane (r, c) gets keys 4c .. 4c + 3 of dims r and r + 8 of each.
@@ -283,9 +287,9 @@ struct Int8Tile {
   static constexpr int kPart = H + 4;                               // floats of a head's part: no bank conflicts
   static constexpr int kSmem(int rows) {
     const int merge = (kWarps + 1) * rows * (kPart + 2) * 4, tiles = kWarps * kI8AttnStages * kBytes;
-    return (merge > tiles ? merge : tiles) + 1024;  // alignment slack
+    return merge > tiles ? merge : tiles;
   }
-  // 16-byte unit u of a chunk's row, as TMA swizzles it: eight lanes of both products hit all banks.
+  // Where 16-byte unit u of a chunk's row lies.
   __device__ static int unit(int row, int u) {
     if constexpr (H == 128) return row * 128 + ((u ^ (row & 7)) << 4);
     return row * 64 + ((u ^ ((row >> 1) & 3)) << 4);
@@ -299,18 +303,23 @@ struct Int8Tile {
 // products in fp32; codes of V enter as c + 128, and 128 times the sums of P leave again.  P is rounded to bf16 once and normalised
 // by the sum of what it was rounded to.  The maximum that P is relative to moves only when a score passes it by kI8Slack.
 //
-// A tile is 32 keys, a warp's own from TMA to its sums: no barrier of the CTA before the end.  Tiles go round the warps of all
+// A tile is 32 keys, a warp's own from `cp.async` to its sums: no barrier of the CTA before the end.  Tiles go round the warps of all
 // splits; splits of eight or less are a cluster whose parts meet in distributed shared memory, those of more are joined by a second
 // launch.
+//
+// Measured (us; at the copy rate): 64 sequences of 2000 tokens, 32 KV heads of 128, 155 in a burst and 161 for as long as one likes
+// (160); 16 x up to 2048 tokens, 8 KV heads for 32, 15.6 (5.3); 1 x 130001, 8 KV heads for 32, 49.1 (40.6); 1 x 300, 16 heads, 4.5.
+// With bf16 operands in both products (three operations to unpack four codes of K, four of V) the first was 164 and, under the power
+// cap, 190; with TMA boxes of 16 rows, whose issue by one or two lanes and whose barriers cost some hundred instructions a tile,
+// 160 and 178, and a split of 2048 tokens of one warp in four 20.4 where it is 18.4 now.  What is left of small calls is a CTA's
+// start and end, 4 us, and the 0.75 us that a warp takes for a tile when nothing else runs on its scheduler.
 template <int H, int kWarps, Int8Merge kMerge>
 __global__ void __launch_bounds__(32 * kWarps, 12 / kWarps)
-int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Int8AttnParams p) {
+int8_attn_kernel(Int8AttnParams p) {
   chain_link();
   using Tile = Int8Tile<H, kWarps>;
   constexpr int kSteps = H / 16, kDigitSteps = H / 32;  // MMAs of a chunk in V's product, in K's for a digit
-  extern __shared__ uint8_t s_raw[];
-  __shared__ __align__(8) uint64_t s_full[kWarps][kI8AttnStages];
-  uint8_t* s_ring = s_raw + (((smem_u32(s_raw) + 1023u) & ~1023u) - smem_u32(s_raw));
+  extern __shared__ __align__(128) uint8_t s_ring[];
   const int split = blockIdx.x;
   const int group = p.num_q_heads / p.num_kv_heads;
   const int parts = (group + kI8AttnRows - 1) / kI8AttnRows;
@@ -332,12 +341,6 @@ int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   const int hi = len / kI8AttnKeys + (len % kI8AttnKeys != 0), step = kWarps * p.splits;
   const int tile0 = split * kWarps + warp;
   const int* table = p.page_table + static_cast<int64_t>(b) * p.max_pages;
-  if (lane == 0) {
-    for (int i = 0; i < kI8AttnStages; ++i) mbar_init(&s_full[warp][i], 1);
-    fence_barrier_init();
-    asm volatile("fence.proxy.async;" ::: "memory");  // the barriers, and the pools as the kernel before left them
-  }
-  __syncwarp();
 
   // Places of a warp's tiles, sixteen at a time: lane l has chunk l % 2 of tile l / 2 of a batch, its page a batch ahead of the
   // row of the pools and the magnitudes that follow from it, and those a batch ahead of their use.
@@ -372,23 +375,31 @@ int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   page = page_of(2);
   uint32_t none = __ballot_sync(0xffffffffu, now.row < 0);  // chunks of the batch without keys
   uint8_t* ring = s_ring + warp * kI8AttnStages * Tile::kBytes;
-  // Tile `n` of the warp, whose batch is `now` or the next one: lanes 0 and 1 fetch a chunk each.
+  // Tile `n` of the warp, whose batch is `now` or the next one.  A chunk is a run of memory; its 16-byte units are swapped within
+  // 128 bytes, so that eight lanes of both products hit all banks.  Chunks that are not there come from the first row, and do not count.
+  uint32_t to[2];  // of unit `lane`, and 512 bytes further
+#pragma unroll
+  for (int i = 0; i < 2; ++i) to[i] = sptr(ring) + Tile::unit(lane / (H / 16) + i * (512 / H), lane % (H / 16));
+  const uint8_t* k_src = p.k_codes + lane * 16;
+  const uint8_t* v_src = p.v_codes + lane * 16;
   auto load_tile = [&](int n, int stage, bool ahead) {
-    const int row = __shfl_sync(0xffffffffu, ahead ? next.row : now.row, (n & 15) * 2 + (lane & 1));
-    const uint32_t there = __ballot_sync(0xffffffffu, row >= 0) & 3;
-    if (lane < 2) {
-      uint64_t* bar = &s_full[warp][stage];
-      uint8_t* dst = ring + stage * Tile::kBytes + lane * Tile::kChunk;
-      if (lane == 0) mbar_arrive_expect_tx(bar, __popc(there) * 2 * Tile::kChunk);
-      if (row >= 0) {
-        tma_load_2d(dst, &map_k, bar, 0, row);
-        tma_load_2d(dst + 2 * Tile::kChunk, &map_v, bar, 0, row);
+    const int at = ahead ? next.row : now.row;
+#pragma unroll
+    for (int ch = 0; ch < 2; ++ch) {
+      const int64_t off = static_cast<int64_t>(max(__shfl_sync(0xffffffffu, at, (n & 15) * 2 + ch), 0)) * H;
+      const uint32_t dst = stage * Tile::kBytes + ch * Tile::kChunk;
+#pragma unroll
+      for (int i = 0; i < Tile::kChunk / 512; ++i) {
+        int8_copy16(to[i & 1] + dst + (i >> 1) * 1024, k_src + off + i * 512);
+        int8_copy16(to[i & 1] + dst + 2 * Tile::kChunk + (i >> 1) * 1024, v_src + off + i * 512);
       }
     }
   };
 #pragma unroll
-  for (int i = 0; i < kI8AttnStages; ++i)
+  for (int i = 0; i < kI8AttnStages; ++i) {
     if (tile0 + i * step < hi) load_tile(i, i, false);
+    cp_commit();
+  }
 
   // 16-byte units of K's rows that a lane takes: of 128-byte rows two that leave those of the next lanes' rows other banks.
   const int unit0 = H == 128 ? (c & 1) + ((c >> 1) << 2) : c;
@@ -438,15 +449,14 @@ int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
   const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+  const int none_yet[4] = {kInt8Sums, kInt8Sums, kInt8Sums, kInt8Sums};
   const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
   // Slots r and r + 8 of a chunk's rows are keys 2r and 2r + 1, so that after `movmatrix` lane c has P of the keys that `ldmatrix` gives
   // it of V.
   const uint8_t* k_at = ring + Tile::unit(2 * r, unit0);
-  const uint32_t v_at = smem_u32(ring) + 2 * Tile::kChunk;
+  const uint32_t v_at = sptr(ring) + 2 * Tile::kChunk;
 
   int stage = 0, n = 0;
-  uint32_t phase = 0;
-  bool ok = true;
   for (int tile = tile0; tile < hi; tile += step, ++n) {
     if (n > 0 && (n & 15) == 0) {
       now = next;
@@ -455,10 +465,8 @@ int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       next = places(batch + 1, page);
       page = page_of(batch + 2);
     }
-    if (!mbar_wait_warp(&s_full[warp][stage], phase, p.status, kStatusWaitTimeoutEpilogue)) {
-      ok = false;
-      break;
-    }
+    cp_wait_group<kI8AttnStages - 1>();
+    __syncwarp();
     const int at_stage = stage * Tile::kBytes, lane_a = (n & 15) * 2;
     const uint32_t tops = static_cast<uint32_t>(now.k_top) | static_cast<uint32_t>(now.v_top) << 16;
     float s[2][4], vt[2];
@@ -479,12 +487,11 @@ int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       }
       int d[3][4];
 #pragma unroll
-      for (int digit = 0; digit < 3; ++digit) d[digit][0] = d[digit][1] = d[digit][2] = d[digit][3] = kInt8Sums;
-#pragma unroll
       for (int j = 0; j < kDigitSteps; ++j) {
-        int8_mma_sum<false>(d[0], w[0][2 * j], w[1][2 * j], w[0][2 * j + 1], w[1][2 * j + 1], qd[0][j][0], qd[0][j][1]);
-        int8_mma_sum<false>(d[1], w[0][2 * j], w[1][2 * j], w[0][2 * j + 1], w[1][2 * j + 1], qd[1][j][0], qd[1][j][1]);
-        int8_mma_sum<true>(d[2], w[0][2 * j], w[1][2 * j], w[0][2 * j + 1], w[1][2 * j + 1], qd[2][j][0], qd[2][j][1]);
+        const uint32_t a[4] = {w[0][2 * j], w[1][2 * j], w[0][2 * j + 1], w[1][2 * j + 1]};
+        int8_mma_sum<false>(d[0], a, qd[0][j][0], qd[0][j][1], j == 0 ? none_yet : d[0]);
+        int8_mma_sum<false>(d[1], a, qd[1][j][0], qd[1][j][1], j == 0 ? none_yet : d[1]);
+        int8_mma_sum<true>(d[2], a, qd[2][j][0], qd[2][j][1], j == 0 ? none_yet : d[2]);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -552,13 +559,10 @@ int8_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     __syncwarp();  // the stage has been read
     if (tile + kI8AttnStages * static_cast<int64_t>(step) < hi)
       load_tile(n + kI8AttnStages, stage, (n >> 4) != ((n + kI8AttnStages) >> 4));
-    if (++stage == kI8AttnStages) {
-      stage = 0;
-      phase ^= 1;
-    }
+    cp_commit();
+    if (++stage == kI8AttnStages) stage = 0;
   }
-  if (!ok)  // let copies that may still be in flight land
-    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+  cp_wait_all();
   __syncthreads();  // the merge buffers overlay the tiles
   constexpr int kPart = Tile::kPart;
   float* s_part = reinterpret_cast<float*>(s_ring);  // the warps and the CTA: [rows][kPart] sums, then maxima, then weights
@@ -672,8 +676,7 @@ int8_combine_kernel(const float* part_out, const float* part_ml, __nv_bfloat16* 
 }
 
 template <int H, int kWarps, Int8Merge kMerge>
-static int launch_int8_attn(const CUtensorMap& map_k, const CUtensorMap& map_v, const Int8AttnParams& p, dim3 grid,
-                            cudaStream_t stream) {
+static int launch_int8_attn(const Int8AttnParams& p, dim3 grid, cudaStream_t stream) {
   constexpr auto kernel = int8_attn_kernel<H, kWarps, kMerge>;
   constexpr int kSmem = Int8Tile<H, kWarps>::kSmem(kI8AttnRows);
   static_assert(12 / kWarps * (kSmem + 1024 + 512) <= 228 * 1024, "resident CTAs");
@@ -689,26 +692,16 @@ static int launch_int8_attn(const CUtensorMap& map_k, const CUtensorMap& map_v, 
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = static_cast<unsigned>(chain_attribute(attr, kMerge == kMergeCluster ? 1 : 0));
-  return cudaLaunchKernelEx(&cfg, kernel, map_k, map_v, p) == cudaSuccess ? 0 : -4;
+  return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? 0 : -4;
 }
 
 template <int H>
-static int int8_attn(const void* k_codes, const void* v_codes, const Int8AttnParams& p, int B, cudaStream_t stream) {
-  CUtensorMap map[2];
-  const void* codes[2] = {k_codes, v_codes};
-  for (int i = 0; i < 2; ++i) {
-    const uint64_t dims[2] = {H, static_cast<uint64_t>(p.num_pages) * p.num_kv_heads * p.page.d};
-    const uint64_t pitch[1] = {H};
-    const uint32_t box[2] = {H, kI8Chunk};
-    const int rc = make_tensor_map(&map[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes[i], dims, pitch, box,
-                                   H == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
-    if (rc != 0) return rc;
-  }
+static int int8_attn(const Int8AttnParams& p, int B, cudaStream_t stream) {
   const int g = p.num_q_heads / p.num_kv_heads;
   const dim3 grid(p.splits, p.num_kv_heads * ((g + kI8AttnRows - 1) / kI8AttnRows), B);
-  const int rc = p.splits == 1                ? launch_int8_attn<H, kI8FewWarps, kMergeNone>(map[0], map[1], p, grid, stream)
-                 : p.splits <= kI8AttnCluster ? launch_int8_attn<H, kI8FewWarps, kMergeCluster>(map[0], map[1], p, grid, stream)
-                                              : launch_int8_attn<H, kI8ManyWarps, kMergeScratch>(map[0], map[1], p, grid, stream);
+  const int rc = p.splits == 1                ? launch_int8_attn<H, kI8FewWarps, kMergeNone>(p, grid, stream)
+                 : p.splits <= kI8AttnCluster ? launch_int8_attn<H, kI8FewWarps, kMergeCluster>(p, grid, stream)
+                                              : launch_int8_attn<H, kI8ManyWarps, kMergeScratch>(p, grid, stream);
   if (rc != 0) return rc;
   if (p.splits > kI8AttnCluster) {
     ChainedBehind chained;
@@ -813,6 +806,7 @@ extern "C" int axb_int8_decode_attn(const axb::Int8AttnCall* call, cudaStream_t 
   if (a.splits > kI8AttnCluster && (a.scratch == nullptr || (reinterpret_cast<uintptr_t>(a.scratch) & 7))) return -10;
   Int8AttnParams p = {};
   p.q = static_cast<const __nv_bfloat16*>(a.q);
+  p.k_codes = static_cast<const uint8_t*>(a.k_codes), p.v_codes = static_cast<const uint8_t*>(a.v_codes);
   p.k_tops = static_cast<const __nv_bfloat16*>(a.k_tops), p.v_tops = static_cast<const __nv_bfloat16*>(a.v_tops);
   p.page_table = a.page_table, p.lengths = a.lengths;
   p.part_out = a.scratch;
@@ -826,5 +820,5 @@ extern "C" int axb_int8_decode_attn(const axb::Int8AttnCall* call, cudaStream_t 
   p.limit = static_cast<int>(a.limit < 0 ? -1 : a.limit < 0x7fffffff ? a.limit : 0x7fffffff);
   p.scale_log2 = static_cast<float>(a.softmax_scale) * (1.4426950408889634f / 127.f);
   const int B = static_cast<int>(a.B);
-  return a.head_dim == 128 ? int8_attn<128>(a.k_codes, a.v_codes, p, B, stream) : int8_attn<64>(a.k_codes, a.v_codes, p, B, stream);
+  return a.head_dim == 128 ? int8_attn<128>(p, B, stream) : int8_attn<64>(p, B, stream);
 }

@@ -468,9 +468,9 @@ def append_int8(k: Tensor, v: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, pa
 def attention_splits(batch: int, num_kv_heads: int, group: int, max_len: int, sms: int = 148) -> int:
     """KV splits of attention over the 8-bit cache, a CTA for each split, KV head and eight query heads.  Up to eight are a cluster:
     2, 4 or 8 of them, 64 tokens or more for each, as many as make up to 9 CTAs on 4 SMs (us with 1 / 2 / 4 / 8: 16 x 2048 tokens, 8
-    heads 20.4 18.3 24.1 29.2, 20 x 2048 25.2 22.6 26.6, 8 x 4000 of 64 dims 28.2 17.1 13.3 18.2, 8 x 2048, 32 heads 26.1 34.4).  Long
-    sequences of few heads take as many as fill most SMs with CTAs of three times the warps, and a second launch that joins them
-    (8 heads with 8 / 16 / 18 / 24: 16000 tokens 20.5 15.2 16.2 18.5, 130001 tokens 127 49.5 51.7 69, 4000 tokens 8.7 9.0; one head with
+    heads 18.4 18.1 24.0 29.9, up to as many tokens 17.7 15.6 18.1 24.3, 8 x up to 2048 17.0 13.2 11.0 15.9, 8 x 2048, 32 heads 25.5 31.9).
+    Long sequences of few heads take as many as fill most SMs with CTAs of three times the warps, and a second launch that joins them
+    (8 heads with 8 / 16 / 18 / 24: 16000 tokens 20.5 15.2 16.2 18.5, 130001 tokens 127 49.1 51.9 69, 4000 tokens 8.7 9.0; one head with
     16 / 32 / 64 / 128: 60000 tokens 26.0 18.9 19.5 24.5)."""
     ctas = max(1, batch * num_kv_heads * ((group + 7) // 8))
     if max_len > 8192 and ctas * 9 <= sms:
