@@ -308,7 +308,7 @@ struct Int8Tile {
 // launch.
 //
 // Measured (us; at the copy rate): 64 sequences of 2000 tokens, 32 KV heads of 128, 155 in a burst and 161 for as long as one likes
-// (160); 16 x up to 2048 tokens, 8 KV heads for 32, 15.6 (5.3); 1 x 130001, 8 KV heads for 32, 49.1 (40.6); 1 x 300, 16 heads, 4.5.
+// (160); 16 x up to 2048 tokens, 8 KV heads for 32, 14.9 (5.3); 1 x 130001, 8 KV heads for 32, 47.6 (40.6); 1 x 300, 16 heads, 4.5.
 // With bf16 operands in both products (three operations to unpack four codes of K, four of V) the first was 164 and, under the power
 // cap, 190; with TMA boxes of 16 rows, whose issue by one or two lanes and whose barriers cost some hundred instructions a tile,
 // 160 and 178, and a split of 2048 tokens of one warp in four 20.4 where it is 18.4 now.  What is left of small calls is a CTA's
@@ -331,26 +331,36 @@ int8_attn_kernel(Int8AttnParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, c = lane & 3;
   const int page_size = static_cast<int>(p.page.d);
-  int len = p.lengths[b];
   const int64_t capacity = p.max_pages * static_cast<int64_t>(page_size);
-  if (len > capacity || (p.limit >= 0 && len > p.limit)) {
-    if (threadIdx.x == 0) int8_report(p.status);
-    len = p.limit >= 0 ? 0 : static_cast<int>(capacity);
-  }
-  len = max(len, 0);
-  const int hi = len / kI8AttnKeys + (len % kI8AttnKeys != 0), step = kWarps * p.splits;
-  const int tile0 = split * kWarps + warp;
+  const int step = kWarps * p.splits, tile0 = split * kWarps + warp;
   const int* table = p.page_table + static_cast<int64_t>(b) * p.max_pages;
+  // 16-byte units of K's rows that a lane takes: of 128-byte rows two that leave those of the next lanes' rows other banks.
+  const int unit0 = H == 128 ? (c & 1) + ((c >> 1) << 2) : c;
+  const __nv_bfloat16* q_at = p.q + (static_cast<int64_t>(b) * p.num_q_heads + qh0 + r) * H + unit0 * 16;
+  const uint4 zeros = make_uint4(0, 0, 0, 0);
 
   // Places of a warp's tiles, sixteen at a time: lane l has chunk l % 2 of tile l / 2 of a batch, its page a batch ahead of the
   // row of the pools and the magnitudes that follow from it, and those a batch ahead of their use.
   auto position = [&](int batch) -> int64_t {
     return (static_cast<int64_t>(tile0) + (static_cast<int64_t>(batch) * 16 + (lane >> 1)) * step) * kI8AttnKeys + (lane & 1) * kI8Chunk;
   };
-  auto page_of = [&](int batch) -> uint32_t {
+  auto page_of = [&](int batch, int64_t end) -> uint32_t {
     const int64_t pos = position(batch);
-    return pos < len ? static_cast<uint32_t>(table[p.page.div(static_cast<uint32_t>(pos))]) : 0u;
+    return pos < end ? static_cast<uint32_t>(table[p.page.div(static_cast<uint32_t>(pos))]) : 0u;
   };
+  // (The table's first entries and the queries do not wait for the length: 4.48 us where it was 4.70 at 1 x 300 tokens, 14.85 for 15.8
+  // at 16 x up to 2048.)
+  int len = p.lengths[b];
+  uint32_t page = page_of(0, min(capacity, int64_t{0x7fffffff})), page_next = page_of(1, min(capacity, int64_t{0x7fffffff}));
+  uint4 q_raw[kDigitSteps];
+#pragma unroll
+  for (int j = 0; j < kDigitSteps; ++j) q_raw[j] = r < rows ? *reinterpret_cast<const uint4*>(q_at + (j >> 1) * 32 + (j & 1) * 8) : zeros;
+  if (len > capacity || (p.limit >= 0 && len > p.limit)) {
+    if (threadIdx.x == 0) int8_report(p.status);
+    len = p.limit >= 0 ? 0 : static_cast<int>(capacity);
+  }
+  len = max(len, 0);
+  const int hi = len / kI8AttnKeys + (len % kI8AttnKeys != 0);
   struct Places {
     int row;  // of the pools; -1: no keys
     uint16_t k_top, v_top;
@@ -370,9 +380,8 @@ int8_attn_kernel(Int8AttnParams p) {
     at.v_top = *reinterpret_cast<const uint16_t*>(p.v_tops + block);
     return at;
   };
-  uint32_t page = page_of(0), page_next = page_of(1);
   Places now = places(0, page), next = places(1, page_next);
-  page = page_of(2);
+  page = page_of(2, len);
   uint32_t none = __ballot_sync(0xffffffffu, now.row < 0);  // chunks of the batch without keys
   uint8_t* ring = s_ring + warp * kI8AttnStages * Tile::kBytes;
   // Tile `n` of the warp, whose batch is `now` or the next one.  A chunk is a run of memory; its 16-byte units are swapped within
@@ -401,21 +410,16 @@ int8_attn_kernel(Int8AttnParams p) {
     cp_commit();
   }
 
-  // 16-byte units of K's rows that a lane takes: of 128-byte rows two that leave those of the next lanes' rows other banks.
-  const int unit0 = H == 128 ? (c & 1) + ((c >> 1) << 2) : c;
   // Q of head r in three digits, q = 2^(e - 22) (65536 q2 + 256 q1 + q0), e the exponent of its largest value; step j takes eight
   // dims of a unit.
   uint32_t qd[3][kDigitSteps][2];
   float q_scale[2];
   {
-    const __nv_bfloat16* q = p.q + (static_cast<int64_t>(b) * p.num_q_heads + qh0 + r) * H;
-    uint4 x[kDigitSteps];
     uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < kDigitSteps; ++j) {
-      x[j] = r < rows ? *reinterpret_cast<const uint4*>(q + (unit0 + (j >> 1) * 2) * 16 + (j & 1) * 8) : make_uint4(0, 0, 0, 0);
-      top = __vmaxu2(top, __vmaxu2(x[j].x & 0x7fff7fffu, x[j].y & 0x7fff7fffu));
-      top = __vmaxu2(top, __vmaxu2(x[j].z & 0x7fff7fffu, x[j].w & 0x7fff7fffu));
+      top = __vmaxu2(top, __vmaxu2(q_raw[j].x & 0x7fff7fffu, q_raw[j].y & 0x7fff7fffu));
+      top = __vmaxu2(top, __vmaxu2(q_raw[j].z & 0x7fff7fffu, q_raw[j].w & 0x7fff7fffu));
     }
     top = max(top & 0xffffu, top >> 16);
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -429,7 +433,7 @@ int8_attn_kernel(Int8AttnParams p) {
     q_scale[1] = __shfl_sync(0xffffffffu, back, 8 * c + 4);
 #pragma unroll
     for (int j = 0; j < kDigitSteps; ++j) {
-      const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+      const uint32_t w[4] = {q_raw[j].x, q_raw[j].y, q_raw[j].z, q_raw[j].w};
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float2 f0 = unpack2(w[2 * i]), f1 = unpack2(w[2 * i + 1]);
@@ -463,7 +467,7 @@ int8_attn_kernel(Int8AttnParams p) {
       none = __ballot_sync(0xffffffffu, now.row < 0);
       const int batch = n >> 4;
       next = places(batch + 1, page);
-      page = page_of(batch + 2);
+      page = page_of(batch + 2, len);
     }
     cp_wait_group<kI8AttnStages - 1>();
     __syncwarp();
@@ -793,7 +797,7 @@ extern "C" int64_t axb_int8_attn_scratch_floats(int B, int num_q_heads, int head
 }
 
 // One new token a sequence: q [B, Nq, H] over the cache, into out [B, Nq, H] (which may be q).  `limit` (-1: none): sequences
-// behind it get zeros. 
+// behind it get zeros.
 extern "C" int axb_int8_decode_attn(const axb::Int8AttnCall* call, cudaStream_t stream) {
   using namespace axb;
   const Int8AttnCall& a = *call;

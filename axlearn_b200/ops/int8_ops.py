@@ -25,6 +25,7 @@ the pool does not have, a position behind a table) are not touched: on the GPU t
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import struct
 from typing import NamedTuple, Optional, Union
@@ -157,13 +158,13 @@ def _row_scales(x: Tensor) -> Tensor:
     """Room for a scale of each row (from a whole number, which torch takes 0.8 us faster than a tuple)."""
     shape = x.shape
     if len(shape) == 2:
-        return torch.empty(shape[0], dtype=torch.float32, device=x.device)
-    return torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+        return x.new_empty(shape[0], dtype=torch.float32)
+    return x.new_empty(shape[:-1], dtype=torch.float32)
 
 
 def _launch_rows(x: Tensor, dim: int, gated: bool) -> Int8Rows:
     shape = x.shape[:-1]
-    codes = torch.empty(shape + (dim,), dtype=torch.int8, device=x.device)
+    codes = x.new_empty(shape + (dim,), dtype=torch.int8)
     scales = _row_scales(x)
     if codes.numel():
         x, rows, pitch = _row_operand(x, x.shape[-1])
@@ -290,7 +291,7 @@ def int8_linear(x: Union[Tensor, Int8Rows], w: Int8Weight, *, out: Optional[Tens
     if not given:
         if accumulate:
             raise ValueError("accumulate needs out")
-        out = torch.empty(shape, dtype=dtype, device=codes.device)
+        out = codes.new_empty(shape, dtype=dtype)
     elif out.shape != shape or out.dtype != dtype or out.get_device() != device or not out.is_contiguous():
         raise ValueError(f"out {tuple(out.shape)} {out.dtype}: contiguous {tuple(shape)} {dtype} is wanted")
     w_scales = w.scales
@@ -320,7 +321,7 @@ def int8_linear(x: Union[Tensor, Int8Rows], w: Int8Weight, *, out: Optional[Tens
     else:
         _check_row(k)
         x, _, pitch = _row_operand(x, k)
-        room = torch.empty(rows * (k + 4), dtype=torch.uint8, device=x.device)  # codes, then scales
+        room = x.new_empty(rows * (k + 4), dtype=torch.uint8)  # codes, then scales
         _call(device, "axb_int8_dense", x.data_ptr(), pitch, room.data_ptr(), w_codes.data_ptr(), w_scales.data_ptr(), y.data_ptr(), rows, n,
               k, accumulate, 0 if few else pair_features(rows, n), resident, _status(device))
     return out if y is out else out.copy_(y)
@@ -458,25 +459,37 @@ def append_int8(k: Tensor, v: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, pa
         return tuple(out) if values else None
     k, v = _aligned_rows(k), _aligned_rows(v)
     k_strides, v_strides = k.stride(), v.stride()
-    out = (k.new_empty(shape), k.new_empty(shape)) if values else None
+    out = None
+    if values:
+        out = (torch.empty_like(k, memory_format=torch.contiguous_format), torch.empty_like(v, memory_format=torch.contiguous_format))
     _call(device, "axb_int8_append", k.data_ptr(), v.data_ptr(), *k_strides[:3], *v_strides[:3], out[0].data_ptr() if values else 0,
           out[1].data_ptr() if values else 0, *pools, page_table.data_ptr(), start.data_ptr(), 0 if live is None else live.data_ptr(), b, t, nkv, h,
           page_size, max_pages, num_pages, _status(device))
     return out
 
 
+@functools.lru_cache(maxsize=1024)
 def attention_splits(batch: int, num_kv_heads: int, group: int, max_len: int, sms: int = 148) -> int:
     """KV splits of attention over the 8-bit cache, a CTA for each split, KV head and eight query heads.  Up to eight are a cluster:
-    2, 4 or 8 of them, 64 tokens or more for each, as many as make up to 9 CTAs on 4 SMs (us with 1 / 2 / 4 / 8: 16 x 2048 tokens, 8
-    heads 18.4 18.1 24.0 29.9, up to as many tokens 17.7 15.6 18.1 24.3, 8 x up to 2048 17.0 13.2 11.0 15.9, 8 x 2048, 32 heads 25.5 31.9).
-    Long sequences of few heads take as many as fill most SMs with CTAs of three times the warps, and a second launch that joins them
-    (8 heads with 8 / 16 / 18 / 24: 16000 tokens 20.5 15.2 16.2 18.5, 130001 tokens 127 49.1 51.9 69, 4000 tokens 8.7 9.0; one head with
-    16 / 32 / 64 / 128: 60000 tokens 26.0 18.9 19.5 24.5)."""
+    the number of 1, 2, 4 and 8 that costs least, at 0.75 us for 128 tokens of a CTA, 1.6 us for each CTA that an SM starts and 0.7 us for
+    the meeting, 64 tokens or more for each, as long as all CTAs run at once, three an SM (us with 1 / 2 / 4 / 8, sequences of up to so
+    many tokens, 8 KV heads: 16 x 2048 17.4 14.7 17.0 23.1, 8 x 2048 16.7 12.6 10.3 15.0, 6 x 2048 16.1 12.1 9.4 9.6, 27 x 512
+    9.4 10.6 17.2, 12 x 512 7.1 7.9 7.2 13.4; 32 x 2048, all as long, 25.8 36.9).  Tables of more than 8192 tokens, where lengths differ by more, may take
+    twice that (42 x 9600 108 85, all as long 141 146; 30 x 9600 85 69 and 98 124).  Long sequences of few heads take as many as fill
+    most SMs with CTAs of three times the warps, and a second launch that joins them (8 heads with 8 / 16 / 18 / 24: 16000 tokens 18.7 14.0
+    15.7, 130001 tokens 127 47.6 51.9 69; one head with 16 / 32 / 64 / 128: 60000 tokens 26.0 18.9 19.5 24.5)."""
     ctas = max(1, batch * num_kv_heads * ((group + 7) // 8))
-    if max_len > 8192 and ctas * 9 <= sms:
+    long = max_len > 8192
+    if long and ctas * 9 <= sms:
         return min(48, max(9, 128 // ctas))
-    most = min(max_len // 64, 9 * sms // (4 * ctas))
-    return 8 if most >= 8 else 4 if most >= 4 else 2 if most >= 2 else 1
+    best, least = 1, math.inf
+    for splits in (1, 2, 4, 8):
+        if splits > 1 and (splits * 64 > max_len or splits * ctas > (6 if long else 3) * sms):
+            break
+        cost = 0.75 / 128 * max_len / splits + 1.6 * -(-splits * ctas // sms) + (0.7 if splits > 1 else 0.0)
+        if cost < least:
+            best, least = splits, cost
+    return best
 
 
 def _attention_plain(q, k_pages, v_pages, page_table, lengths, scale):
