@@ -42,8 +42,12 @@ constexpr int kInt8Held = 8;  // 16-byte units of rows that a thread keeps in sh
 constexpr int kInt8QRows = 4;
 
 // A unit is what a call brings for one block: up to a page's tokens of the keys, or the values, of a KV head.  Its kWarps warps
-// hold them in registers while the largest magnitude is found (further rows are read again), and turn the codes that are
+// hold them in shared memory while the largest magnitude is found (further rows are read again), and turn the codes that are
 // there already, if the magnitude has grown.  Units behind those rotate kInt8QRows times kRows query heads of a token.
+//
+// Measured: 8 x 2048 tokens of 8 heads of 128 with the cache's values, 24 us (18.5 at the copy rate); with rows in registers and a branch
+// for ties 26.3.  One token for each of 64 sequences 4.5, where that was 5.8: a launch, and behind it four loads that each wait
+// for the one before, of the position, its page, the page's largest magnitude and, where that grows, its codes.
 template <int H, int kWarps>
 __global__ void __launch_bounds__(kInt8AppendThreads, 4)
 int8_append_kernel(Int8AppendParams p) {

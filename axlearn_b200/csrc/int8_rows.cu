@@ -4,6 +4,9 @@
 // A CTA takes a row and keeps it in registers, so that memory is read once: the largest magnitude and, for the norm, the sum of
 // squares meet in one barrier, since a norm's codes do not depend on its 1 / rms, which only the scale carries: with t the
 // summed row and w the norm's weights, round(127 t w / max |t w|).  t w has 16 bits, so codes are those of exact arithmetic.
+//
+// Measured: the norm of 8192 x 4096 with residual, sum and values 46.3 us (46.1 at the copy rate); rows of 16384 x 4096 39 (30.7), where
+// ties of the quotient decide (a branch for them 49).  One row of 2048 takes 1.9, an empty launch's time.
 #include <math.h>
 
 #include "chain.cuh"
