@@ -584,7 +584,8 @@ extern "C" int axb_gemm_skinny(const void* X, const void* W, void* C, int M, int
 
 // y[M, N] (bf16) = x_scales[m] w_scales[n] sum_k x[m, k] w[n, k] (+ y when accumulate) of 8-bit whole numbers, x [M, K] and w [N, K]
 // one row behind the other and 16-byte aligned, M <= 128, K a multiple of 16.  The weight's bytes bound it: 1 x 4096 x 28672 23 us
-// with the rows' own kernel (18.0 at the copy rate), 16 x 14336 x 4096 15.0 (9.1), 2 of each a launch and its first loads.  `plan`: slices of K; `resident`: as above.
+// with the rows' own kernel (18.0 at the copy rate), 16 x 14336 x 4096 15.0 (9.1), 2 of each a launch and its first loads.
+// `plan`: slices of K; `resident`: as above.
 extern "C" int axb_gemm_skinny_int8(const axb::Int8LinearCall* call, cudaStream_t stream) {
   using namespace axb;
   const Int8LinearCall& a = *call;
