@@ -49,31 +49,41 @@ constexpr int kSkMaxSplit = 8;  // portable cluster size
 // BN rows of X; `LAYOUT`: how a CTA fills its SM.
 //   kPair  one 128-feature tile, half an SM's shared memory: two CTAs per SM;
 //   kDeep  one tile, the whole SM: twice the stages in flight, for grids of at most one CTA per SM;
-//   kWide  two tiles side by side, the whole SM: 512 contiguous bytes per K row of an N-major W where one tile has 256.
-enum SkinnyLayout { kPair, kDeep, kWide };
+//   kWide  two tiles side by side, the whole SM: 512 contiguous bytes per K row of an N-major W where one tile has 256;
+//   kEven  8-bit operands in place of kWide: two tiles of which the second has as few features as spread N evenly over the SMs (us
+//          kPair / kWide / kEven: 1 x 4096 x 19200 21.0 19.1 16.3, x 22016 21.8 20.2 18.7, x 28672 24.1 23.0 22.4; 64 rows of these
+//          25.5 20.5 19.6, 26.5 22.3 21.4, 28.8 25.7 25.8).
+enum SkinnyLayout { kPair, kDeep, kWide, kEven };
 
 template <int BN, SkinnyLayout LAYOUT>
 struct SkinnyCfg {
-  static constexpr int kTiles = LAYOUT == kWide ? 2 : 1;
-  static constexpr int kFeatures = kTiles * kSkTile;
+  static constexpr int kTiles = LAYOUT == kWide || LAYOUT == kEven ? 2 : 1;
+  static constexpr int kFeatures = kTiles * kSkTile;  // (kEven: at most)
   static constexpr int kWBytes = kFeatures * kSkRow;
   static constexpr int kXBytes = BN * kSkRow;
   static constexpr int kBlockBytes = kWBytes + kXBytes;
   static constexpr int kBlocks = (LAYOUT == kPair ? 110 * 1024 : 200 * 1024) / kBlockBytes;
   // A stage, the unit of waits and commits, is one or two k-blocks.
-  static constexpr int kGroup = BN <= 16 ? 2 : 1;
-  static constexpr int kStages = kBlocks / kGroup;
+  static constexpr int kGroup = BN <= 16 && LAYOUT != kEven ? 2 : 1;
+  // Stages of kEven: MMAs read the second tile's 128 rows whole, also in the last stage, and what lies behind its features makes
+  // sums that nobody reads.
+  static constexpr int kEvenRing = 200 * 1024, kEvenLeast = kSkTile + 8;
+  __host__ __device__ static constexpr int even_stages(int features) {
+    const int block = features * kSkRow + kXBytes;
+    return (kEvenRing - (block > kWBytes ? block : kWBytes)) / block + 1;
+  }
+  static constexpr int kStages = LAYOUT == kEven ? even_stages(kEvenLeast) : kBlocks / kGroup;
   // A split tile of few rows receives the other slices' partial sums behind the stages: [slice][own row][feature].
-  static constexpr bool kPush = LAYOUT != kWide && BN <= 32;
+  static constexpr bool kPush = kTiles == 1 && BN <= 32;
   static constexpr int kInboxBytes = kPush ? (BN + kSkMaxSplit - 1) * kSkTile * 4 : 0;
   static constexpr int kSplitStages = kPush ? (kBlocks * kBlockBytes - kInboxBytes) / (kGroup * kBlockBytes) : kStages;
-  static constexpr int kRingBytes = kBlocks * kBlockBytes;
+  static constexpr int kRingBytes = LAYOUT == kEven ? kEvenRing : kBlocks * kBlockBytes;
   static constexpr int kSmem = kRingBytes + 512 + 1024;  // barriers, alignment slack
   static constexpr int kResident = LAYOUT == kPair ? 2 : 1;
   static constexpr int kTmemCols = kTiles * BN < 32 ? 32 : kTiles * BN;
   static_assert(kResident * (kSmem + 1024) <= 228 * 1024 && kSmem <= 227 * 1024, "resident CTAs per SM");
   static_assert(kSplitStages >= 2, "a ring");
-  static_assert(LAYOUT == kWide || kPush || BN * kSkTile * 4 <= kRingBytes, "partial sums reuse the stages");
+  static_assert(kTiles > 1 || kPush || BN * kSkTile * 4 <= kRingBytes, "partial sums reuse the stages");
 };
 
 struct SkinnyGemmParams {
@@ -85,6 +95,7 @@ struct SkinnyGemmParams {
   int split;
   int w_resident;  // in a chained launch: nothing that runs just before this kernel writes W
   const float *x_scales, *w_scales;  // 8-bit operands: of the rows of X and of the features
+  int features;                      // kEven: of a CTA, a multiple of 8
 };
 
 // Operands in 8 bits (`int8_t`) are products of whole numbers in 32-bit integers, exact in any order; a sum counts times the
@@ -138,6 +149,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   using S = SkinnyCfg<BN, LAYOUT>;
   using I = SkinnyIn<In>;
   static_assert(!I::kWhole || (!X_MN && !W_MN), "8-bit operands are read along K");
+  static_assert(I::kWhole ? LAYOUT != kWide : LAYOUT != kEven, "two tiles");
   constexpr int kGroup = S::kGroup, kSkK = I::kK;
   extern __shared__ uint8_t smem_raw[];
   __shared__ float x_scales[I::kWhole ? BN : 1];  // read by the epilogue while the products run
@@ -150,10 +162,12 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = p.split;
-  const bool splits = LAYOUT != kWide && split > 1;
-  const int stages = splits ? S::kSplitStages : S::kStages;
+  const bool splits = S::kTiles == 1 && split > 1;
+  const int features = LAYOUT == kEven ? p.features : S::kFeatures;
+  const int w_bytes = LAYOUT == kEven ? features * kSkRow : S::kWBytes, block_bytes = w_bytes + S::kXBytes;
+  const int stages = LAYOUT == kEven ? S::even_stages(features) : splits ? S::kSplitStages : S::kStages;
   const int rank = splits ? static_cast<int>(cluster_rank()) : 0;
-  const int n0 = static_cast<int>(blockIdx.x) / split * S::kFeatures;
+  const int n0 = static_cast<int>(blockIdx.x) / split * features;
   const int num_kb = (p.K + kSkK - 1) / kSkK;
   const int kb_lo = rank * num_kb / split, kb_hi = (rank + 1) * num_kb / split;
 
@@ -183,22 +197,24 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
   const int feature = (warp & 3) * 32 + lane;
   OutT* out = static_cast<OutT*>(p.C) + n0 + feature;
   // C of up to 16 rows is read while the products run: rows rank, rank + split, ...
-  constexpr int kEarlyC = BN <= 16 && LAYOUT != kWide ? 16 : 1;
+  constexpr int kEarlyC = BN <= 16 && S::kTiles == 1 ? 16 : 1;
   float before[kEarlyC];
 
   bool ok = true;
   if (warp == 0) {
     if (elect_one()) {
-      auto block_at = [&](int stage, int j) { return smem + (stage * kGroup + j) * S::kBlockBytes; };
+      auto block_at = [&](int stage, int j) { return smem + (stage * kGroup + j) * block_bytes; };
       auto load_w = [&](int stage, int kb) {
         const int blocks = kb_hi - kb < kGroup ? kb_hi - kb : kGroup;
-        mbar_arrive_expect_tx(&full_bar[stage], blocks * S::kBlockBytes);
+        mbar_arrive_expect_tx(&full_bar[stage], blocks * block_bytes);
 #pragma unroll
         for (int j = 0; j < kGroup; ++j) {
           if (j >= blocks) break;
           uint8_t* sw = block_at(stage, j);
           const int k0 = (kb + j) * kSkK;
-          if constexpr (!W_MN) {
+          if constexpr (LAYOUT == kEven) {
+            tma_load_2d(sw, &tmap_w, &full_bar[stage], k0, n0);  // all features
+          } else if constexpr (!W_MN) {
 #pragma unroll
             for (int t = 0; t < S::kTiles; ++t)
               tma_load_2d(sw + t * (kSkTile * kSkRow), &tmap_w, &full_bar[stage], k0, n0 + t * kSkTile);
@@ -225,7 +241,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
 #pragma unroll
         for (int j = 0; j < kGroup; ++j) {
           if (kb + j >= kb_hi) break;
-          uint8_t* sx = block_at(stage, j) + S::kWBytes;
+          uint8_t* sx = block_at(stage, j) + w_bytes;
           const int k0 = (kb + j) * kSkK;
           if constexpr (!X_MN) {
             tma_load_2d(sx, &tmap_x, &full_bar[stage], k0, 0);
@@ -256,8 +272,8 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
 #pragma unroll
         for (int j = 0; j < kGroup; ++j) {
           if (kb + j >= kb_hi) break;
-          const uint32_t sw = smem_u32(smem + (stage * kGroup + j) * S::kBlockBytes);
-          const uint32_t sx = sw + S::kWBytes;
+          const uint32_t sw = smem_u32(smem + (stage * kGroup + j) * block_bytes);
+          const uint32_t sx = sw + w_bytes;
 #pragma unroll
           for (int k = 0; k < kSkRow / 32; ++k) {
             const uint64_t dx =
@@ -306,7 +322,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
 #pragma unroll
     for (int t = 0; t < S::kTiles; ++t) {
       const uint32_t taddr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + t * BN;
-      const bool stores = n0 + t * kSkTile + feature < p.N;
+      const bool stores = n0 + t * kSkTile + feature < p.N && (LAYOUT != kEven || t * kSkTile + feature < features);
       const float w_scale = I::kWhole && stores ? p.w_scales[n0 + t * kSkTile + feature] : 0.f;
 #pragma unroll 1
       for (int c = 0; c < BN; c += 16) {
@@ -421,16 +437,16 @@ struct SkinnyKernel {
   // little more.  Fitted to chained launches of every split and layout over N of 640 to 32768, K of 1024 to 14336 and 1
   // to 100 rows: the choice is 2 % behind the fastest on average (6 % with the constants of the kernel before this
   // one).
-  static float cost(int N, int num_kb, int split) {
+  static float cost(int N, int num_kb, int split, int features = S::kFeatures) {
     static std::atomic<int> cache[kSkMaxSplit + 1];
-    const int ctas = (N + S::kFeatures - 1) / S::kFeatures * split;
+    const int ctas = (N + features - 1) / features * split;
     const int resident = resident_ctas(kernel, S::kSmem, split, cache);
     const float sms = static_cast<float>(resident_ctas(kernel, S::kSmem, 1, cache)) / S::kResident;
     const int waves = (ctas + resident - 1) / resident;
     const int stages = ((num_kb + split - 1) / split + S::kGroup - 1) / S::kGroup;
     const float at_once = static_cast<float>(ctas < resident ? ctas : resident);
-    const float port = S::kBlockBytes * fmaxf(1.f, at_once / sms) / 1.1e5f;
-    const float memory = at_once * S::kWBytes / 7.1e6f;
+    const float port = (features * kSkRow + S::kXBytes) * fmaxf(1.f, at_once / sms) / 1.1e5f;
+    const float memory = at_once * (features * kSkRow) / 7.1e6f;
     const float issue = (BN > 16 ? 0.23f : 0.21f) * S::kTiles;
     const float work = static_cast<float>(stages * S::kGroup) * fmaxf(fmaxf(port, memory), issue);
     const float rows = S::kPush ? 0.01f * BN : 0.13f * BN / split;
@@ -438,9 +454,18 @@ struct SkinnyKernel {
     return static_cast<float>(waves) * (work + 1.25f) + (split > 1 ? meet : 0.f);
   }
 
+  // Of a CTA, for as many waves as kFeatures would take.
+  static int even_features(int N) {
+    static std::atomic<int> cache[2];
+    const int sms = resident_ctas(kernel, S::kSmem, 1, cache), most = sms * S::kFeatures;
+    const int ctas = (N + most - 1) / most * sms;
+    return ((N + ctas - 1) / ctas + 7) / 8 * 8;
+  }
+
   static int launch(const CUtensorMap& tw, const CUtensorMap& tx, const SkinnyGemmParams& p, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>((p.N + S::kFeatures - 1) / S::kFeatures * p.split));
+    const int features = LAYOUT == kEven ? p.features : S::kFeatures;
+    cfg.gridDim = dim3(static_cast<unsigned>((p.N + features - 1) / features * p.split));
     cfg.blockDim = dim3(kSkThreads);
     cfg.dynamicSmemBytes = S::kSmem;
     cfg.stream = stream;
@@ -458,18 +483,15 @@ struct SkinnyKernel {
   }
 };
 
-// The cheapest layout and split; `forced` split (0 = free).
+// The cheapest layout and split, and kEven's features; `forced` split (0 = free).
 template <int BN, bool X_MN, bool W_MN, typename OutT, typename In = __nv_bfloat16>
-static bool skinny_plan(int N, int K, int forced, int* split, SkinnyLayout* layout) {
+static bool skinny_plan(int N, int K, int forced, int* split, SkinnyLayout* layout, int* features) {
+  constexpr SkinnyLayout kBoth = SkinnyIn<In>::kWhole ? kEven : kWide;
   using Pair = SkinnyKernel<BN, kPair, X_MN, W_MN, OutT, In>;
   using Deep = SkinnyKernel<BN, kDeep, X_MN, W_MN, OutT, In>;
-  using Wide = SkinnyKernel<BN, kWide, X_MN, W_MN, OutT, In>;
-  // Rows of 8-bit weights lie along K: two tiles side by side are no longer runs of memory (1 x 4096 x 22016 20.0 us, 17.5 of pairs).
-  constexpr bool kWideToo = !SkinnyIn<In>::kWhole;
-  if (!Deep::configure() || !Pair::configure()) return false;
-  if constexpr (kWideToo) {
-    if (!Wide::configure()) return false;
-  }
+  using Both = SkinnyKernel<BN, kBoth, X_MN, W_MN, OutT, In>;
+  if (!Deep::configure() || !Pair::configure() || !Both::configure()) return false;
+  *features = kBoth == kEven ? Both::even_features(N) : 2 * kSkTile;
   constexpr int kSkK = SkinnyIn<In>::kK;
   const int num_kb = (K + kSkK - 1) / kSkK;
   float best = 0.f;
@@ -484,9 +506,7 @@ static bool skinny_plan(int N, int K, int forced, int* split, SkinnyLayout* layo
     if (forced > 0 ? s != forced : (s > 1 && num_kb / s < 2)) continue;
     consider(Deep::cost(N, num_kb, s), s, kDeep);
     consider(Pair::cost(N, num_kb, s), s, kPair);
-    if constexpr (kWideToo) {
-      if (s == 1) consider(Wide::cost(N, num_kb, 1), 1, kWide);
-    }
+    if (s == 1 && *features > kSkTile) consider(Both::cost(N, num_kb, 1, *features), 1, kBoth);
   }
   return *split > 0;
 }
@@ -495,13 +515,13 @@ template <int BN, bool X_MN, bool W_MN, typename OutT, typename In = __nv_bfloat
 static int launch_skinny(const void* X, const void* W, int64_t ldx, int64_t ldw, SkinnyGemmParams p,
                          cudaStream_t stream) {
   SkinnyLayout layout = kPair;
-  if (!skinny_plan<BN, X_MN, W_MN, OutT, In>(p.N, p.K, p.split, &p.split, &layout)) return -15;
+  if (!skinny_plan<BN, X_MN, W_MN, OutT, In>(p.N, p.K, p.split, &p.split, &layout, &p.features)) return -15;
   CUtensorMap tw, tx;
   constexpr int kSkK = SkinnyIn<In>::kK;
   const uint64_t k = static_cast<uint64_t>(p.K), n = static_cast<uint64_t>(p.N), m = static_cast<uint64_t>(p.M);
   const uint64_t wdims[2] = {W_MN ? n : k, W_MN ? k : n};
   const uint64_t wstride[1] = {static_cast<uint64_t>(ldw) * sizeof(In)};
-  const uint32_t wbox[2] = {W_MN ? 64 : kSkK, static_cast<uint32_t>(W_MN ? kSkK : kSkTile)};
+  const uint32_t wbox[2] = {W_MN ? 64 : kSkK, static_cast<uint32_t>(W_MN ? kSkK : layout == kEven ? p.features : kSkTile)};
   int rc = make_tensor_map(&tw, SkinnyIn<In>::kType, 2, W, wdims, wstride, wbox,
                            CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc != 0) return rc;
@@ -514,7 +534,7 @@ static int launch_skinny(const void* X, const void* W, int64_t ldx, int64_t ldw,
   switch (layout) {
     case kDeep: return SkinnyKernel<BN, kDeep, X_MN, W_MN, OutT, In>::launch(tw, tx, p, stream);
     case kWide:
-      if constexpr (!SkinnyIn<In>::kWhole) return SkinnyKernel<BN, kWide, X_MN, W_MN, OutT, In>::launch(tw, tx, p, stream);
+    case kEven: return SkinnyKernel<BN, SkinnyIn<In>::kWhole ? kEven : kWide, X_MN, W_MN, OutT, In>::launch(tw, tx, p, stream);
     default: return SkinnyKernel<BN, kPair, X_MN, W_MN, OutT, In>::launch(tw, tx, p, stream);
   }
 }
@@ -531,13 +551,13 @@ extern "C" int axb_chain_launches(int on) {
 // K slices that the kernel would choose for a problem with K-major X and N-major W (1 = no split).
 extern "C" int axb_gemm_splitk_plan(int M, int N, int K) {
   using namespace axb;
-  int split = 1;
+  int split = 1, features = 0;
   SkinnyLayout layout;
   bool ok;
-  if (M <= 16) ok = skinny_plan<16, false, true, __nv_bfloat16>(N, K, 0, &split, &layout);
-  else if (M <= 32) ok = skinny_plan<32, false, true, __nv_bfloat16>(N, K, 0, &split, &layout);
-  else if (M <= 64) ok = skinny_plan<64, false, true, __nv_bfloat16>(N, K, 0, &split, &layout);
-  else if (M <= 128) ok = skinny_plan<128, false, true, __nv_bfloat16>(N, K, 0, &split, &layout);
+  if (M <= 16) ok = skinny_plan<16, false, true, __nv_bfloat16>(N, K, 0, &split, &layout, &features);
+  else if (M <= 32) ok = skinny_plan<32, false, true, __nv_bfloat16>(N, K, 0, &split, &layout, &features);
+  else if (M <= 64) ok = skinny_plan<64, false, true, __nv_bfloat16>(N, K, 0, &split, &layout, &features);
+  else if (M <= 128) ok = skinny_plan<128, false, true, __nv_bfloat16>(N, K, 0, &split, &layout, &features);
   else ok = false;
   return ok ? split : 1;
 }
@@ -561,7 +581,7 @@ extern "C" int axb_gemm_skinny(const void* X, const void* W, void* C, int M, int
       (reinterpret_cast<uintptr_t>(C) & 15) || (ldc % (out_fp32 ? 4 : 8)))
     return -10;
   if (split < 0 || split > kSkMaxSplit || split > (K + SkinnyIn<__nv_bfloat16>::kK - 1) / SkinnyIn<__nv_bfloat16>::kK) return -15;
-  const SkinnyGemmParams p{M, N, K, C, ldc, status, accumulate, split, w_resident && chain_launches ? 1 : 0, nullptr, nullptr};
+  const SkinnyGemmParams p{M, N, K, C, ldc, status, accumulate, split, w_resident && chain_launches ? 1 : 0, nullptr, nullptr, 0};
 #define AXB_SKINNY_BN(BN, XM, WM, T) return launch_skinny<BN, XM, WM, T>(X, W, ldx, ldw, p, stream)
 #define AXB_SKINNY(WM, T)                                  \
   do {                                                     \
@@ -583,8 +603,8 @@ extern "C" int axb_gemm_skinny(const void* X, const void* W, void* C, int M, int
 }
 
 // y[M, N] (bf16) = x_scales[m] w_scales[n] sum_k x[m, k] w[n, k] (+ y when accumulate) of 8-bit whole numbers, x [M, K] and w [N, K]
-// one row behind the other and 16-byte aligned, M <= 128, K a multiple of 16.  The weight's bytes bound it: 1 x 4096 x 28672 23 us
-// with the rows' own kernel (18.0 at the copy rate), 16 x 14336 x 4096 15.0 (9.1), 2 of each a launch and its first loads.
+// one row behind the other and 16-byte aligned, M <= 128, K a multiple of 16.  The weight's bytes bound it: 1 x 4096 x 28672 22.4 us
+// (18.0 at the copy rate), 16 x 14336 x 4096 with the rows' own kernel 15.0 (9.1), 2 of each a launch and its first loads.
 // `plan`: slices of K; `resident`: as above.
 extern "C" int axb_gemm_skinny_int8(const axb::Int8LinearCall* call, cudaStream_t stream) {
   using namespace axb;
@@ -597,7 +617,7 @@ extern "C" int axb_gemm_skinny_int8(const axb::Int8LinearCall* call, cudaStream_
   if (a.plan < 0 || a.plan > kSkMaxSplit || a.plan > (a.K + SkinnyIn<int8_t>::kK - 1) / SkinnyIn<int8_t>::kK) return -15;
   const int M = static_cast<int>(a.M);
   const SkinnyGemmParams p{M, static_cast<int>(a.N), static_cast<int>(a.K), a.y, a.N, a.status, a.accumulate != 0,
-                           static_cast<int>(a.plan), a.resident && chain_launches ? 1 : 0, a.x_scales, a.w_scales};
+                           static_cast<int>(a.plan), a.resident && chain_launches ? 1 : 0, a.x_scales, a.w_scales, 0};
   if (M <= 16) return launch_skinny<16, false, false, __nv_bfloat16, int8_t>(a.x, a.w, a.K, a.K, p, stream);
   if (M <= 32) return launch_skinny<32, false, false, __nv_bfloat16, int8_t>(a.x, a.w, a.K, a.K, p, stream);
   if (M <= 64) return launch_skinny<64, false, false, __nv_bfloat16, int8_t>(a.x, a.w, a.K, a.K, p, stream);

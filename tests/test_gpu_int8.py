@@ -141,6 +141,20 @@ def test_linear_of_few_rows(rows, k, n):
     _close(out, want, old)
 
 
+@pytest.mark.parametrize("rows", [1, 16, 31, 50, 96])
+@pytest.mark.parametrize("k,n", [(16, 18952), (1104, 19208), (400, 25000), (2064, 37888), (144, 37896), (272, 56840)])
+def test_linear_of_few_rows_and_more_features_than_a_tile_an_sm(rows, k, n):
+    gen = _gen(rows + n)
+    w, held = _weight(gen, k, n), int8_ops.quantize_rows(_normal(gen, rows, k).bfloat16())
+    want = _linear64(held, w)
+    _close(int8_ops.int8_linear(held, w), want)
+    room = _normal(gen, rows + 1, n).bfloat16()  # (its last row has to stay)
+    old = room.clone()
+    int8_ops.int8_linear(held, w, out=room[:rows], accumulate=True)
+    _close(room[:rows], want, old[:rows])
+    assert torch.equal(room[rows], old[rows])
+
+
 @pytest.mark.parametrize("rows", [129, 255, 256, 257, 513, 1500])
 @pytest.mark.parametrize("k,n", [(16, 8), (208, 136), (1104, 392), (4096, 1032), (272, 9480)])
 def test_linear_of_many_rows(rows, k, n):
