@@ -232,7 +232,7 @@ constexpr int kI8AttnRows = 8;   // query heads of a CTA: the columns of both pr
 constexpr int kI8Chunk = 16;     // keys of an MMA, of one page
 constexpr int kI8AttnKeys = 2 * kI8Chunk;
 constexpr int kI8AttnStages = 2;
-constexpr int kI8AttnCluster = 8;
+constexpr int kI8AttnCluster = 8, kI8MostSplits = 1024;
 constexpr float kI8Slack = 8.f;
 
 // Warps of a CTA: four, three CTAs an SM, or, of more splits than a cluster has, twelve that have an SM to themselves: a third of the
@@ -806,7 +806,7 @@ extern "C" int axb_int8_decode_attn(const axb::Int8AttnCall* call, cudaStream_t 
   using namespace axb;
   const Int8AttnCall& a = *call;
   if (!int8_cache_fits(a.head_dim, a.page_size, a.num_kv_heads, a.num_pages, a.k_codes, a.v_codes) || a.num_q_heads < 1 ||
-      a.num_q_heads % a.num_kv_heads || a.splits < 1 || a.B < 0 || a.B > 65535 || !int8_ints({a.num_q_heads, a.max_pages, a.splits}) ||
+      a.num_q_heads % a.num_kv_heads || a.splits < 1 || a.splits > kI8MostSplits || a.B < 0 || a.B > 65535 || !int8_ints({a.num_q_heads, a.max_pages}) ||
       !(a.softmax_scale > 0. && a.softmax_scale < 1048576.) || !aligned16(a.q) ||
       a.num_kv_heads * ((a.num_q_heads / a.num_kv_heads + kI8AttnRows - 1) / kI8AttnRows) > 65535)
     return -10;

@@ -50,6 +50,7 @@ Tensor = torch.Tensor
 LEAST = 2.0 ** -119
 MAX_ROW = 65536        # values of a row that the row kernels keep
 MAX_K = 1 << 17        # products of 127 x 127 whose sums fit 32 bits
+MAX_SPLITS = 1024      # of a sequence's keys
 PAGE_UNIT = 16         # tokens of a page are a multiple of
 # Entry points and the 64-bit words of their arguments (``csrc/int8.cuh``).
 _WORDS = {"axb_int8_rows": "7q", "axb_int8_add_rms_norm": "9qd", "axb_gemm_skinny_int8": "12q", "axb_int8_gemm": "12q",
@@ -383,6 +384,11 @@ def _check_pages(k_pages: Int8Pages, v_pages: Int8Pages, page_table: Tensor, bat
     return (num_pages, nkv, page_size, table[1]), (at_k, kt.data_ptr(), at_v, vt.data_ptr())
 
 
+def _check_apart(pools: tuple) -> None:
+    if pools[0] == pools[2] or pools[1] == pools[3]:
+        raise ValueError("keys and values are appended to pools of their own")
+
+
 def _check_counts(counts: Tensor, batch: int, name: str, device: int) -> None:
     if counts.dtype is not torch.int32 or counts.shape != (batch,) or not counts.is_contiguous() or counts.get_device() != device:
         raise ValueError(f"{name} is [{batch}] int32 on the operands' device: {tuple(counts.shape)} {counts.dtype}")
@@ -448,6 +454,7 @@ def append_int8(k: Tensor, v: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, pa
     (num_pages, held, page_size, max_pages), pools = _check_pages(k_pages, v_pages, page_table, b, nkv, h, device)
     if held != nkv:
         raise ValueError(f"pages of {held} heads for {nkv}")
+    _check_apart(pools)
     _check_counts(start, b, "start", device)
     if live is not None:
         _check_counts(live, b, "live", device)
@@ -506,9 +513,11 @@ def _attention_plain(q, k_pages, v_pages, page_table, lengths, scale):
     return out.reshape(b, nq, h).to(q.dtype)
 
 
-def _check_scale(scale: float) -> None:
+def _check_attention(scale: float, splits: Optional[int]) -> None:
     if not 0 < scale < 2 ** 20:
         raise ValueError(f"softmax_scale {scale} is not in (0, 2^20)")
+    if splits is not None and not 1 <= splits <= MAX_SPLITS:
+        raise ValueError(f"{splits} splits: 1 to {MAX_SPLITS}")
 
 
 def paged_decode_attention_int8(q: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, page_table: Tensor, lengths: Tensor, *,
@@ -523,7 +532,7 @@ def paged_decode_attention_int8(q: Tensor, k_pages: Int8Pages, v_pages: Int8Page
     cache, pools = _check_pages(k_pages, v_pages, page_table, b, nq, h, device)
     _check_counts(lengths, b, "lengths", device)
     scale = 1.0 / math.sqrt(h) if softmax_scale is None else softmax_scale
-    _check_scale(scale)
+    _check_attention(scale, splits)
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.get_device() != device or not out.is_contiguous()):
         raise ValueError(f"out {tuple(out.shape)} {out.dtype}: contiguous {tuple(q.shape)} {q.dtype} is wanted")
     _no_gradient("paged_decode_attention_int8", q, k_pages.tops, v_pages.tops, out)
@@ -584,8 +593,9 @@ def rope_decode_attention_int8(qkv: Tensor, k_pages: Int8Pages, v_pages: Int8Pag
     b, device = qkv.shape[0], qkv.get_device()
     cache, pools = _check_pages(k_pages, v_pages, page_table, b, num_q_heads, h, device)
     num_pages, _, page_size, max_pages = cache
+    _check_apart(pools)
     _check_counts(lengths, b, "lengths", device)
-    _check_scale(softmax_scale)
+    _check_attention(softmax_scale, splits)
     _no_gradient("rope_decode_attention_int8", qkv, k_pages.tops, v_pages.tops, table)
     limit = min(table.shape[0], max_pages * page_size)
     if not _on_kernel(qkv):
@@ -616,6 +626,7 @@ def prompt_attention_int8(qkv: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, p
     b, t, _ = qkv.shape
     device = qkv.get_device()
     (num_pages, _, page_size, max_pages), pools = _check_pages(k_pages, v_pages, page_table, b, num_q_heads, h, device)
+    _check_apart(pools)
     if table.shape[0] < t or max_pages * page_size < t:
         raise ValueError(f"{b} x {t} tokens, a rotation table of {table.shape[0]} positions, a page table {tuple(page_table.shape)}")
     if live is not None:

@@ -281,6 +281,17 @@ def test_attention_at_tile_split_and_page_edges(nq, kv, dim, page_size, splits):
     assert ((got.double() - want).abs() <= bound).all(), ((got.double() - want).abs() / bound.clamp(min=1e-30)).max()
 
 
+@pytest.mark.parametrize("nq,kv,dim,page_size", [(4, 2, 128, 16), (9, 1, 64, 48)])
+@pytest.mark.parametrize("splits", [1, 2, 5, 11])
+def test_attention_over_many_tiles_a_warp(nq, kv, dim, page_size, splits):
+    lengths = torch.tensor([2048, 2049, 9001, 4097 * splits, 3, 6144], dtype=torch.int32, device="cuda")
+    k_pages, v_pages, table = _cache(len(lengths), -(-int(lengths.max()) // page_size), page_size, kv, dim, seed=splits)
+    q = _normal(_gen(splits), len(lengths), nq, dim).bfloat16()
+    got = int8_ops.paged_decode_attention_int8(q, k_pages, v_pages, table, lengths, splits=splits)
+    want, bound = _attention64(q, k_pages, v_pages, table, lengths, dim ** -0.5)
+    assert ((got.double() - want).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("b,nq,kv,dim,tokens,page_size", [(1, 16, 16, 128, 300, 16), (1, 8, 2, 128, 40000, 64), (33, 32, 8, 64, 700, 16),
                                                           (7, 32, 8, 128, 1, 16), (1, 1, 1, 64, 30000, 16)])
 def test_attention_with_splits_of_its_own(b, nq, kv, dim, tokens, page_size):
@@ -626,6 +637,26 @@ def test_products_of_all_kinds_replay_in_graphs_side_by_side():
     torch.cuda.synchronize()
     for _, out, _ in graphs:
         assert all(torch.equal(y, want) for y, (_, _, want) in zip(out, cases))
+
+
+def test_attention_of_many_splits_replays_in_graphs_side_by_side():
+    lengths = torch.tensor([700, 3000], dtype=torch.int32, device="cuda")
+    k_pages, v_pages, table = _cache(2, 3000 // 16 + 1, 16, 2, 128)
+    queries = [_normal(_gen(i), 2, 8, 128).bfloat16() for i in range(2)]
+    want = [int8_ops.paged_decode_attention_int8(q, k_pages, v_pages, table, lengths, splits=16).clone() for q in queries]
+    graphs = []
+    for q in queries:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = int8_ops.paged_decode_attention_int8(q, k_pages, v_pages, table, lengths, splits=16)
+        graphs.append((graph, out, torch.cuda.Stream()))
+    for _ in range(20):
+        for graph, _, stream in graphs:
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, y) for (_, out, _), y in zip(graphs, want))
 
 
 @pytest.mark.parametrize("splits", [None, 1, 8, 9, 16])

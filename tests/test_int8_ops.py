@@ -294,6 +294,7 @@ def _attend_args(**change):
     dict(v_pages=lambda a: int8_ops.Int8Pages(a["v_pages"].codes[1:], a["v_pages"].tops[1:])),
     dict(v_pages=lambda a: int8_ops.Int8Pages(a["v_pages"].codes[:, :, ::2], a["v_pages"].tops)),
     dict(softmax_scale=lambda a: 0.0), dict(softmax_scale=lambda a: float("nan")), dict(softmax_scale=lambda a: 2.0 ** 20),
+    dict(splits=lambda a: 0), dict(splits=lambda a: 1025),
     dict(out=lambda a: torch.zeros(2, 4, 32)), dict(out=lambda a: torch.zeros(2, 4, 64, dtype=torch.bfloat16)),
 ])
 def test_attention_refuses(change):
@@ -304,7 +305,8 @@ def test_attention_refuses(change):
 @pytest.mark.parametrize("change", [
     dict(v=lambda a: a["v"][:, :2]), dict(k=lambda a: a["k"][:, :, :1], v=lambda a: a["v"][:, :, :1]),
     dict(start=lambda a: a["start"].long()), dict(live=lambda a: torch.zeros(3, dtype=torch.int32)),
-    dict(k=lambda a: a["k"][..., :32], v=lambda a: a["v"][..., :32]),
+    dict(k=lambda a: a["k"][..., :32], v=lambda a: a["v"][..., :32]), dict(v_pages=lambda a: a["k_pages"]),
+    dict(v_pages=lambda a: int8_ops.Int8Pages(a["v_pages"].codes, a["k_pages"].tops)),
 ])
 def test_append_refuses(change):
     k_pages, v_pages, table = _cache(2, 2, 16, 2, 64)
