@@ -1,5 +1,6 @@
 """8-bit rows, weights and cache on the GPU, against 64 bits or the plain statements."""
 
+import gc
 import math
 
 import pytest
@@ -21,6 +22,14 @@ def _normal(gen, *shape):
 def _plain(fn, *args, **kwargs):
     with dispatch.use_reference_ops():
         return fn(*args, **kwargs)
+
+
+@pytest.fixture(autouse=True, scope="module")
+def _memory():
+    """Gives memory back: other tests count the segments that the allocator makes."""
+    yield
+    gc.collect()
+    torch.cuda.empty_cache()
 
 
 @pytest.fixture(autouse=True)
