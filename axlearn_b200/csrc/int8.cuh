@@ -34,27 +34,35 @@ struct Int8Scale {
 // rounds it correctly in 32 bits; with x and A of 8 bits (a cache) or of 16 (products of two bf16 numbers) a quotient that is not
 // k + 1/2 is off it by more than half a unit, so adding 1.5 2^23 rounds as in exact arithmetic.  Ties are no rare case to be left
 // to a branch: x = A / 2 is 63.5 (every second vector of 256 values has one; 16384 x 4096 rows 49.1 us with such a branch).
+// A level is a float with its code in the last bits.
 template <int kFactor>
-__device__ __forceinline__ uint2 int8_codes(const float (&x)[8], const Int8Scale<kFactor>& s) {
-  if (s.empty()) return make_uint2(0, 0);
-  uint32_t u[8];
+__device__ __forceinline__ void int8_levels(uint32_t (&u)[8], const float (&x)[8], const Int8Scale<kFactor>& s) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float y = x[i] * s.factor, q = y * s.reciprocal;
-    u[i] = __float_as_uint(fmaf(fmaf(-q, s.divisor, y), s.reciprocal, q) + kInt8Whole);
+    u[i] = s.empty() ? __float_as_uint(kInt8Whole) : __float_as_uint(fmaf(fmaf(-q, s.divisor, y), s.reciprocal, q) + kInt8Whole);
   }
+}
+
+__device__ __forceinline__ uint2 int8_bytes(const uint32_t (&u)[8]) {
   return make_uint2(__byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410),
                     __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410));
 }
 
-// What codes stand for, rounded to bf16: times A / 127.
-__device__ __forceinline__ uint4 int8_values(uint2 codes, float scale) {
+template <int kFactor>
+__device__ __forceinline__ uint2 int8_codes(const float (&x)[8], const Int8Scale<kFactor>& s) {
+  uint32_t u[8];
+  int8_levels(u, x, s);
+  return int8_bytes(u);
+}
+
+// What levels stand for, rounded to bf16: their codes times A / 127.
+__device__ __forceinline__ uint4 int8_values(const uint32_t (&u)[8], float scale) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t two = (i & 2 ? codes.y : codes.x) >> (16 * (i & 1));
-    const __nv_bfloat162 v = __floats2bfloat162_rn(static_cast<float>(static_cast<int8_t>(two)) * scale,
-                                                   static_cast<float>(static_cast<int8_t>(two >> 8)) * scale);
+    const __nv_bfloat162 v = __floats2bfloat162_rn((__uint_as_float(u[2 * i]) - kInt8Whole) * scale,
+                                                   (__uint_as_float(u[2 * i + 1]) - kInt8Whole) * scale);
     w[i] = reinterpret_cast<const uint32_t&>(v);
   }
   return make_uint4(w[0], w[1], w[2], w[3]);

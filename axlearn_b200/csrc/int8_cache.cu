@@ -179,9 +179,10 @@ int8_append_kernel(Int8AppendParams p) {
       const float2 two = unpack2(w[j]);
       f[2 * j] = two.x, f[2 * j + 1] = two.y;
     }
-    const uint2 bytes = int8_codes(f, s);
-    if (placed) *reinterpret_cast<uint2*>(codes + i * (kRows * H)) = bytes;
-    if (out != nullptr) *reinterpret_cast<uint4*>(out + i * out_step) = int8_values(bytes, back);
+    uint32_t u[8];
+    int8_levels(u, f, s);
+    if (placed) *reinterpret_cast<uint2*>(codes + i * (kRows * H)) = int8_bytes(u);
+    if (out != nullptr) *reinterpret_cast<uint4*>(out + i * out_step) = int8_values(u, back);
   };
 #pragma unroll 1
   for (int i = 0; i < held; ++i) hold(i, s_held[i][threadIdx.x]);

@@ -109,9 +109,10 @@ int8_rows_kernel(Int8RowsParams p) {
   for (int i = 0; i < VPT; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
     if (v >= vectors) continue;
-    const uint2 codes = int8_codes(f[i], s);
-    reinterpret_cast<uint2*>(p.codes + row * p.dim)[v] = codes;
-    if (p.values != nullptr) reinterpret_cast<uint4*>(p.values + row * p.dim)[v] = int8_values(codes, scale);
+    uint32_t u[8];
+    int8_levels(u, f[i], s);
+    reinterpret_cast<uint2*>(p.codes + row * p.dim)[v] = int8_bytes(u);
+    if (p.values != nullptr) reinterpret_cast<uint4*>(p.values + row * p.dim)[v] = int8_values(u, scale);
   }
 }
 
