@@ -25,6 +25,7 @@
 // (segment ids :179-205, block skipping by mask_fn) and the cuDNN call at :792-926.
 #include <stdlib.h>
 
+#include "f32x2.cuh"
 #include "host_utils.cuh"
 #include "sm100.cuh"
 
@@ -87,26 +88,6 @@ __device__ __forceinline__ float tanh_approx(float x) {
   float y;
   asm("tanh.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-
-// Two-wide fp32 arithmetic (one issue slot for two lanes of work on the FMA pipe).
-__device__ __forceinline__ uint64_t f32x2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void f32x2_split(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {

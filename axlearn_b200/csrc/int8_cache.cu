@@ -45,8 +45,8 @@ constexpr int kInt8QRows = 4;
 // hold them in shared memory while the largest magnitude is found (further rows are read again), and turn the codes that are
 // there already, if the magnitude has grown.  Units behind those rotate kInt8QRows times kRows query heads of a token.
 //
-// Measured: 8 x 2048 tokens of 8 heads of 128 with the cache's values, 24 us (18.5 at the copy rate); with rows in registers and a branch
-// for ties 26.3.  One token for each of 64 sequences 4.5, where that was 5.8: a launch, and behind it four loads that each wait
+// Measured: 8 x 2048 tokens of 8 heads of 128 with the cache's values, 23.4 us (18.5 at the copy rate); with rows in registers and a branch
+// for ties 26.3.  One token for each of 64 sequences 4.2, where that was 5.8: a launch, and behind it four loads that each wait
 // for the one before, of the position, its page, the page's largest magnitude and, where that grows, its codes.
 template <int H, int kWarps>
 __global__ void __launch_bounds__(kInt8AppendThreads, 4)
@@ -180,7 +180,7 @@ int8_append_kernel(Int8AppendParams p) {
       f[2 * j] = two.x, f[2 * j + 1] = two.y;
     }
     uint32_t u[8];
-    int8_levels(u, f, s);
+    int8_levels<false>(u, f, s);
     if (placed) *reinterpret_cast<uint2*>(codes + i * (kRows * H)) = int8_bytes(u);
     if (out != nullptr) *reinterpret_cast<uint4*>(out + i * out_step) = int8_values(u, back);
   };

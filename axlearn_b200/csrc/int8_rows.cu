@@ -5,8 +5,9 @@
 // squares meet in one barrier, since a norm's codes do not depend on its 1 / rms, which only the scale carries: with t the
 // summed row and w the norm's weights, round(127 t w / max |t w|).  t w has 16 bits, so codes are those of exact arithmetic.
 //
-// Measured: the norm of 8192 x 4096 with residual, sum and values 46.3 us (46.1 at the copy rate); rows of 16384 x 4096 39 (30.7), where
-// ties of the quotient decide (a branch for them 49).  One row of 2048 takes 1.9, an empty launch's time.
+// Measured: the norm of 8192 x 4096 with residual, sum and values 46.3 us (46.1 at the copy rate); rows of 16384 x 4096 33.5 (30.7), of
+// 16384 x 11008 97 (83), silu(gate) * up of it 183 (138), which its exponentials and quotients bound.  One row of 2048 takes 1.6 to 1.9,
+// an empty launch's time.
 #include <math.h>
 
 #include "chain.cuh"
@@ -28,8 +29,8 @@ struct Int8RowsParams {
   float inverse_dim, eps;
 };
 
-template <int KIND, int VPT>
-__global__ void __launch_bounds__(1024)
+template <int KIND, int VPT, int kThreads>
+__global__ void __launch_bounds__(kThreads)
 int8_rows_kernel(Int8RowsParams p) {
   chain_link();
   __shared__ float s_sum[32];
@@ -110,7 +111,7 @@ int8_rows_kernel(Int8RowsParams p) {
     const int v = threadIdx.x + i * blockDim.x;
     if (v >= vectors) continue;
     uint32_t u[8];
-    int8_levels(u, f[i], s);
+    int8_levels<KIND == kRowsPlain>(u, f[i], s);
     reinterpret_cast<uint2*>(p.codes + row * p.dim)[v] = int8_bytes(u);
     if (p.values != nullptr) reinterpret_cast<uint4*>(p.values + row * p.dim)[v] = int8_values(u, scale);
   }
@@ -120,15 +121,18 @@ constexpr int kInt8RowsMost = 1024 * 8 * 8;  // values of a row
 
 template <int KIND>
 static int int8_rows(const Int8RowsParams& p, int64_t rows, cudaStream_t stream) {
+  // Many rows: vectors of a thread so that CTAs are small; few: so that a row is spread wide.  Four vectors and more need the registers
+  // that 512 threads leave (rows of 16384 x 11008 97 us, 103 with 1024 threads' registers).
   const int vectors = p.dim / 8, most = rows >= 296 ? 128 : 1024;
   int vpt = 1;
-  while (vpt < 8 && (vectors + vpt - 1) / vpt > (vpt < 4 ? most : 1024)) vpt *= 2;
+  while (vpt < 8 && (vectors + vpt - 1) / vpt > (vpt < 4 ? most : 512)) vpt *= 2;
   const int threads = ((vectors + vpt - 1) / vpt + 31) / 32 * 32;
   const dim3 grid(static_cast<unsigned>(rows));
-  if (vpt == 1) launch_chained(int8_rows_kernel<KIND, 1>, grid, threads, 0, stream, p);
-  else if (vpt == 2) launch_chained(int8_rows_kernel<KIND, 2>, grid, threads, 0, stream, p);
-  else if (vpt == 4) launch_chained(int8_rows_kernel<KIND, 4>, grid, threads, 0, stream, p);
-  else launch_chained(int8_rows_kernel<KIND, 8>, grid, threads, 0, stream, p);
+  if (vpt == 1) launch_chained(int8_rows_kernel<KIND, 1, 1024>, grid, threads, 0, stream, p);
+  else if (vpt == 2) launch_chained(int8_rows_kernel<KIND, 2, 1024>, grid, threads, 0, stream, p);
+  else if (vpt == 4) launch_chained(int8_rows_kernel<KIND, 4, 512>, grid, threads, 0, stream, p);
+  else if (threads <= 512) launch_chained(int8_rows_kernel<KIND, 8, 512>, grid, threads, 0, stream, p);
+  else launch_chained(int8_rows_kernel<KIND, 8, 1024>, grid, threads, 0, stream, p);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
