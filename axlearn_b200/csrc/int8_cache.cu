@@ -312,11 +312,12 @@ struct Int8Tile {
 // splits; splits of eight or less are a cluster whose parts meet in distributed shared memory, those of more are joined by a second
 // launch.
 //
-// Measured (us; at the copy rate): 64 sequences of 2000 tokens, 32 KV heads of 128, 155 in a burst and 161 for as long as one likes
-// (160); 16 x up to 2048 tokens, 8 KV heads for 32, 14.9 (5.3); 1 x 130001, 8 KV heads for 32, 47.6 (40.6); 1 x 300, 16 heads, 4.5.
+// Measured (us; at the copy rate): 64 sequences of 2000 tokens, 32 KV heads of 128, 154 in a burst and 161 for as long as one likes
+// (160); 16 x up to 2048 tokens, 8 KV heads for 32, 14.3 (5.3); 1 x 130001, 8 KV heads for 32, 46.7 (40.6); 1 x 300, 16 heads, 4.2.
 // With bf16 operands in both products (three operations to unpack four codes of K, four of V) the first was 164 and, under the power
 // cap, 190; with TMA boxes of 16 rows, whose issue by one or two lanes and whose barriers cost some hundred instructions a tile,
-// 160 and 178, and a split of 2048 tokens of one warp in four 20.4 where it is 18.4 now.  What is left of small calls is a CTA's
+// 160 and 178, and a split of 2048 tokens of one warp in four 20.4 where it is 18 now; without two
+// numbers an instruction for scores and sums 4.5, 14.9, 155 and 47.8.  What is left of small calls is a CTA's
 // start and end, 4 us, and the 0.75 us that a warp takes for a tile when nothing else runs on its scheduler.
 template <int H, int kWarps, Int8Merge kMerge>
 __global__ void __launch_bounds__(32 * kWarps, 12 / kWarps)
@@ -353,7 +354,7 @@ int8_attn_kernel(Int8AttnParams p) {
     const int64_t pos = position(batch);
     return pos < end ? static_cast<uint32_t>(table[p.page.div(static_cast<uint32_t>(pos))]) : 0u;
   };
-  // (The table's first entries and the queries do not wait for the length: 4.48 us where it was 4.70 at 1 x 300 tokens, 14.85 for 15.8
+  // (The table's first entries and the queries do not wait for the length: 4.5 us where it was 4.7 at 1 x 300 tokens, 14.9 for 15.8
   // at 16 x up to 2048.)
   int len = p.lengths[b];
   uint32_t page = page_of(0, min(capacity, int64_t{0x7fffffff})), page_next = page_of(1, min(capacity, int64_t{0x7fffffff}));
@@ -453,10 +454,12 @@ int8_attn_kernel(Int8AttnParams p) {
     }
   }
 
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, w_sum[2] = {0.f, 0.f};  // heads 2c, 2c + 1
-  float acc[kSteps][4];  // [i][dim 16 i + r: columns 2c, 2c + 1; dim 16 i + 8 + r]
+  float m[2] = {-INFINITY, -INFINITY};  // heads 2c, 2c + 1
+  uint64_t l = 0, w_sum = 0;            // pairs of them
+  uint64_t acc[kSteps][2];  // pairs of heads 2c, 2c + 1 for dims 16 i + r and 16 i + 8 + r
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+  for (int i = 0; i < kSteps; ++i) acc[i][0] = acc[i][1] = 0;
+  const uint64_t q_scales = f32x2(q_scale[0], q_scale[1]);
   const float zero[4] = {0.f, 0.f, 0.f, 0.f};
   const int none_yet[4] = {kInt8Sums, kInt8Sums, kInt8Sums, kInt8Sums};
   const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
@@ -478,7 +481,8 @@ int8_attn_kernel(Int8AttnParams p) {
     __syncwarp();
     const int at_stage = stage * Tile::kBytes, lane_a = (n & 15) * 2;
     const uint32_t tops = static_cast<uint32_t>(now.k_top) | static_cast<uint32_t>(now.v_top) << 16;
-    float s[2][4], vt[2];
+    uint64_t s[2][2];  // keys 2r and 2r + 1 of a chunk, pairs of heads
+    float vt[2];
 #pragma unroll
     for (int ch = 0; ch < 2; ++ch) {
       const uint32_t pair = __shfl_sync(0xffffffffu, tops, lane_a + ch);
@@ -502,12 +506,15 @@ int8_attn_kernel(Int8AttnParams p) {
         int8_mma_sum<false>(d[1], a, qd[1][j][0], qd[1][j][1], j == 0 ? none_yet : d[1]);
         int8_mma_sum<true>(d[2], a, qd[2][j][0], qd[2][j][1], j == 0 ? none_yet : d[2]);
       }
+      const float start = -__int_as_float(kInt8Sums);
+      const uint64_t by = mul2(q_scales, f32x2(kt, kt));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float f[3];
+      for (int i = 0; i < 2; ++i) {
+        uint64_t f[3];
 #pragma unroll
-        for (int digit = 0; digit < 3; ++digit) f[digit] = __int_as_float(d[digit][i]) - __int_as_float(kInt8Sums);
-        s[ch][i] = fmaf(f[2], 65536.f, fmaf(f[1], 256.f, f[0])) * (q_scale[i & 1] * kt);
+        for (int digit = 0; digit < 3; ++digit)
+          f[digit] = add2(f32x2(__int_as_float(d[digit][2 * i]), __int_as_float(d[digit][2 * i + 1])), f32x2(start, start));
+        s[ch][i] = mul2(fma2(f[2], f32x2(65536.f, 65536.f), fma2(f[1], f32x2(256.f, 256.f), f[0])), by);
       }
     }
     const uint32_t empty = none >> lane_a & 3;  // chunks behind the sequence, or of a page that is not in the pool
@@ -516,41 +523,48 @@ int8_attn_kernel(Int8AttnParams p) {
       for (int ch = 0; ch < 2; ++ch) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          if ((empty >> ch & 1) || tile * kI8AttnKeys + ch * kI8Chunk + 2 * r + i >= len) s[ch][2 * i] = s[ch][2 * i + 1] = -INFINITY;
+          if ((empty >> ch & 1) || tile * kI8AttnKeys + ch * kI8Chunk + 2 * r + i >= len) s[ch][i] = f32x2(-INFINITY, -INFINITY);
       }
     }
     float top[2];
+    {
+      float x[4][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) top[h] = fmaxf(fmaxf(s[0][h], s[0][2 + h]), fmaxf(s[1][h], s[1][2 + h]));
+      for (int i = 0; i < 4; ++i) f32x2_split(s[i >> 1][i & 1], x[i][0], x[i][1]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) top[h] = fmaxf(fmaxf(x[0][h], x[1][h]), fmaxf(x[2][h], x[3][h]));
+    }
     if (__any_sync(0xffffffffu, top[0] > m[0] + kI8Slack || top[1] > m[1] + kI8Slack)) {
+      float by[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
         for (int off = 4; off <= 16; off <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], off));
         const float m_new = fmaxf(m[h], top[h]);
-        const float by = m[h] == -INFINITY ? 0.f : ex2(m[h] - m_new);  // (nothing is there yet)
+        by[h] = m[h] == -INFINITY ? 0.f : ex2(m[h] - m_new);  // (nothing is there yet)
         m[h] = m_new;
-        l[h] *= by;
-        w_sum[h] *= by;
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) acc[i][h] *= by, acc[i][2 + h] *= by;
       }
+      const uint64_t both = f32x2(by[0], by[1]);
+      l = mul2(l, both), w_sum = mul2(w_sum, both);
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) acc[i][0] = mul2(acc[i][0], both), acc[i][1] = mul2(acc[i][1], both);
     }
-    const float base[2] = {m[0] == -INFINITY ? 0.f : 64.f - m[0], m[1] == -INFINITY ? 0.f : 64.f - m[1]};
+    const uint64_t base = f32x2(m[0] == -INFINITY ? 0.f : 64.f - m[0], m[1] == -INFINITY ? 0.f : 64.f - m[1]);
 #pragma unroll
     for (int ch = 0; ch < 2; ++ch) {
       uint32_t pt[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)  // (NaN stays)
-        pt[i] = int8_turned_round(pack2(ex2(s[ch][2 * i] + base[0]), ex2(s[ch][2 * i + 1] + base[1])));
+      for (int i = 0; i < 2; ++i) {  // (NaN stays)
+        float x, y;
+        f32x2_split(add2(s[ch][i], base), x, y);
+        pt[i] = int8_turned_round(pack2(ex2(x), ex2(y)));
+      }
       float sums[4];  // of P, in every lane of a column
       int8_mma_add(sums, ones, pt[0], pt[1], zero);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        l[h] += sums[h];
-        w_sum[h] = fmaf(vt[ch], sums[h] * (1.f / kInt8Up), w_sum[h]);
-      }
-      const float back = vt[ch] * kInt8Back;
+      const uint64_t both = f32x2(sums[0], sums[1]);
+      l = add2(l, both);
+      w_sum = fma2(f32x2(vt[ch], vt[ch]), mul2(both, f32x2(1.f / kInt8Up, 1.f / kInt8Up)), w_sum);
+      const uint64_t back = f32x2(vt[ch] * kInt8Back, vt[ch] * kInt8Back);
 #pragma unroll
       for (int i = 0; i < kSteps; i += 2) {
         uint32_t v[4];
@@ -561,7 +575,7 @@ int8_attn_kernel(Int8AttnParams p) {
           float d[4];
           int8_mma_add(d, a, pt[0], pt[1], zero);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i + t][e] = fmaf(back, d[e], acc[i + t][e]);
+          for (int e = 0; e < 2; ++e) acc[i + t][e] = fma2(back, f32x2(d[2 * e], d[2 * e + 1]), acc[i + t][e]);
         }
       }
     }
@@ -578,16 +592,26 @@ int8_attn_kernel(Int8AttnParams p) {
   const int per_warp = rows * kPart;
   float* s_m = s_part + (kWarps + 1) * per_warp;
   float* s_l = s_m + (kWarps + 1) * rows;
+  float l_of[2], w_of[2];
+  f32x2_split(l, l_of[0], l_of[1]);
+  f32x2_split(w_sum, w_of[0], w_of[1]);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     if (2 * c + h >= rows) continue;
     float* dst = s_part + warp * per_warp + (2 * c + h) * kPart + r;
-    const float low = -128.f * w_sum[h];
+    const float low = -128.f * w_of[h];
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) dst[16 * i] = acc[i][h] + low, dst[16 * i + 8] = acc[i][2 + h] + low;
+    for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x[2];
+        f32x2_split(acc[i][e], x[0], x[1]);
+        dst[16 * i + 8 * e] = x[h] + low;
+      }
+    }
     if (r == 0) {
       s_m[warp * rows + 2 * c + h] = m[h];
-      s_l[warp * rows + 2 * c + h] = l[h] * (1.f / kInt8Up);
+      s_l[warp * rows + 2 * c + h] = l_of[h] * (1.f / kInt8Up);
     }
   }
   __syncthreads();
@@ -807,8 +831,8 @@ extern "C" int axb_int8_decode_attn(const axb::Int8AttnCall* call, cudaStream_t 
   using namespace axb;
   const Int8AttnCall& a = *call;
   if (!int8_cache_fits(a.head_dim, a.page_size, a.num_kv_heads, a.num_pages, a.k_codes, a.v_codes) || a.num_q_heads < 1 ||
-      a.num_q_heads % a.num_kv_heads || a.splits < 1 || a.splits > kI8MostSplits || a.B < 0 || a.B > 65535 || !int8_ints({a.num_q_heads, a.max_pages}) ||
-      !(a.softmax_scale > 0. && a.softmax_scale < 1048576.) || !aligned16(a.q) ||
+      a.num_q_heads % a.num_kv_heads || a.splits < 1 || a.splits > kI8MostSplits || a.B < 0 || a.B > 65535 ||
+      !int8_ints({a.num_q_heads, a.max_pages}) || !(a.softmax_scale > 0. && a.softmax_scale < 1048576.) || !aligned16(a.q) ||
       a.num_kv_heads * ((a.num_q_heads / a.num_kv_heads + kI8AttnRows - 1) / kI8AttnRows) > 65535)
     return -10;
   if (a.B == 0) return 0;

@@ -481,17 +481,19 @@ def attention_splits(batch: int, num_kv_heads: int, group: int, max_len: int, sm
     the number of 1, 2, 4 and 8 that costs least, at 0.75 us for 128 tokens of a CTA, 1.6 us for each CTA that an SM starts and 0.7 us for
     the meeting, 64 tokens or more for each, as long as all CTAs run at once, three an SM (us with 1 / 2 / 4 / 8, sequences of up to so
     many tokens, 8 KV heads: 16 x 2048 17.4 14.7 17.0 23.1, 8 x 2048 16.7 12.6 10.3 15.0, 6 x 2048 16.1 12.1 9.4 9.6, 27 x 512
-    9.4 10.6 17.2, 12 x 512 7.1 7.9 7.2 13.4; 32 x 2048, all as long, 25.8 36.9).  Tables of more than 8192 tokens, where lengths differ by more, may take
-    twice that (42 x 9600 108 85, all as long 141 146; 30 x 9600 85 69 and 98 124).  Long sequences of few heads take as many as fill
-    most SMs with CTAs of three times the warps, and a second launch that joins them (8 heads with 8 / 16 / 18 / 24: 16000 tokens 18.7 14.0
-    15.7, 130001 tokens 127 47.6 51.9 69; one head with 16 / 32 / 64 / 128: 60000 tokens 26.0 18.9 19.5 24.5)."""
+    9.4 10.6 17.2, 12 x 512 7.1 7.9 7.2 13.4; 32 x 2048, all as long, 25.8 36.9).  Tables of 4096 tokens and more, where lengths differ
+    by more, may take two also where that is four CTAs an SM or more (40 x 4096 49 40, 64 x 4096 61 58, all as long 59 67 and 112 97; not 32
+    x 4096 41 35, 46 59), and those of more than 8192 twice as many CTAs (42 x 9600 108 85, 30 x 9600 85 69, all as long 141 146 and 98 124).
+    Long sequences of few heads take as many as fill most SMs with CTAs of three times the warps, and a second launch that joins them
+    (8 heads with 8 / 16 / 18 / 24: 16000 tokens 18.7 14.0 15.7, 130001 tokens 127 47.6 51.9 69; one head with 16 / 32 / 64 / 128: 60000
+    tokens 26.0 18.9 19.5 24.5)."""
     ctas = max(1, batch * num_kv_heads * ((group + 7) // 8))
-    long = max_len > 8192
-    if long and ctas * 9 <= sms:
+    if max_len > 8192 and ctas * 9 <= sms:
         return min(48, max(9, 128 // ctas))
+    at_once = (6 if max_len > 8192 else 3) * sms
     best, least = 1, math.inf
     for splits in (1, 2, 4, 8):
-        if splits > 1 and (splits * 64 > max_len or splits * ctas > (6 if long else 3) * sms):
+        if splits > 1 and (splits * 64 > max_len or (splits * ctas > at_once and (splits > 2 or max_len < 4096 or splits * ctas < 4 * sms))):
             break
         cost = 0.75 / 128 * max_len / splits + 1.6 * -(-splits * ctas // sms) + (0.7 if splits > 1 else 0.0)
         if cost < least:
