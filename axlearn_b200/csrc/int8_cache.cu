@@ -154,8 +154,10 @@ int8_append_kernel(Int8AppendParams p) {
   if (placed) {
     if (in == 0) pool.tops[block] = __float2bfloat16(s.top);
     if (row0 > 0 && __float_as_uint(s.top) != old && !s.empty()) {
-      const Int8Scale<1> turn(top);
-      const float by = __uint_as_float(old);
+      // (Codes times an A that has been scaled down with the new one, as A above 2^121 times 127 is infinite.)
+      Int8Scale<1> turn(top);
+      const float by = __uint_as_float(old) * turn.factor;
+      turn.factor = 1.f;
       for (int r = row_at; r < row0; r += kRows) {
         uint2* at = reinterpret_cast<uint2*>(codes + static_cast<int64_t>(r - row0) * H);
         const uint2 was = *at;

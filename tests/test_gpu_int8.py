@@ -362,6 +362,31 @@ def test_append_has_the_bits_of_the_plain_statement(b, t, kv, dim, page_size, pa
     int8_ops.append_int8(k, v, k_pages, v_pages, table, start, live=live)
 
 
+@pytest.mark.parametrize("old,new", [(2.0 ** 121, 1.5 * 2.0 ** 121), (1.5 * 2.0 ** 121, 2.0 ** 122), (2.0 ** 122, 2.0 ** 124),
+                                     (2.0 ** 126, 1.9921875 * 2.0 ** 127), (2.0 ** -119, 2.0 ** 127), (2.0 ** 100, 1.5 * 2.0 ** 100),
+                                     (2.0 ** -119, 1.0078125 * 2.0 ** -119), (2.0 ** -119, 2.0 ** -118), (2.0 ** -118, 1.5 * 2.0 ** -117)])
+@pytest.mark.parametrize("dim,page_size,t", [(128, 16, 1), (64, 128, 20)])
+def test_codes_of_pages_that_grow_at_the_ends_of_the_range(old, new, dim, page_size, t):
+    """Every code under every pair of magnitudes, in 64 bits."""
+    k_pages, v_pages, table = _cache(2, 2, page_size, 2, dim)
+    row = torch.arange(128, device="cuda")[-dim:].to(torch.int8)
+    for p in (k_pages, v_pages):
+        p.codes[:, :, 0], p.codes[:, :, 1], p.codes[:, :, 2] = row, -row, row - 64
+        p.tops.fill_(old)
+    x = _normal(_gen(1), 2, t, 2, dim)
+    x = (x / x.abs().amax(-1, keepdim=True) * new).bfloat16()
+    start = torch.tensor([5, 3], dtype=torch.int32, device="cuda")
+    want = [torch.round(p.codes.double() * (old / new)) for p in (k_pages, v_pages)]
+    int8_ops.append_int8(x, -x, k_pages, v_pages, table, start)
+    for sign, p, turned in zip((1, -1), (k_pages, v_pages), want):
+        for i, first in enumerate(start.tolist()):
+            page = table[i, 0].long()
+            assert (p.tops[page].double() == new).all() and torch.equal(p.codes[page, :, :first].double(), turned[page, :, :first])
+            count = min(t, page_size - first)
+            codes = torch.round(127 * (sign * x[i, :count].double().transpose(0, 1)) / new)
+            assert torch.equal(p.codes[page, :, first:first + count].double(), codes)
+
+
 @pytest.mark.parametrize("nq,kv,dim,splits", [(4, 4, 128, 1), (8, 2, 64, 3), (20, 2, 128, 9), (32, 8, 128, None)])
 def test_a_step_is_rotation_append_and_attention(nq, kv, dim, splits):
     lengths = torch.tensor([1, 16, 17, 200, 0, 63, 144], dtype=torch.int32, device="cuda")
