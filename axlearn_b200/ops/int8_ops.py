@@ -351,9 +351,14 @@ def int8_pages(num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
                      torch.zeros((num_pages, num_kv_heads), dtype=torch.bfloat16, device=device))
 
 
+def _stand_for(codes: Tensor, top: Tensor) -> Tensor:
+    """``codes * top / 127`` in 32 bits, both factors of 2^-7 so that the product stays in range."""
+    return codes.float() * (top * 2.0 ** -7) / (127 * 2.0 ** -7)
+
+
 def page_values(pages: Int8Pages, dtype: torch.dtype = torch.float32) -> Tensor:
     """What a pool (or pages of it) stands for: ``[pages, Nkv, page_size, H]``."""
-    return (pages.codes.float() * pages.tops.float()[..., None, None] / 127.0).to(dtype)
+    return _stand_for(pages.codes, pages.tops.float()[..., None, None]).to(dtype)
 
 
 def _check_pages(k_pages: Int8Pages, v_pages: Int8Pages, page_table: Tensor, batch: int, heads: int, head_dim: int,
@@ -435,7 +440,7 @@ def _append_plain(k, v, k_pages, v_pages, page_table, start, live):
         there = keep & write.gather(1, block)
         pages.codes[page.gather(1, block)[there], :, row[there]] = codes[there]
         pages.tops[page[write]] = top[write].bfloat16()
-        out.append(torch.where(keep[..., None, None], codes.float() * mine / 127.0, 0).to(x.dtype))
+        out.append(torch.where(keep[..., None, None], _stand_for(codes, mine), 0).to(x.dtype))
     return out
 
 

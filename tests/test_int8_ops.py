@@ -157,6 +157,26 @@ def test_a_page_that_grows_keeps_its_tokens_within_its_roundings():
         assert (held[t] - tokens[t].float()).abs().max() <= sum(0.5 * a / 127 for a in grown) * (1 + 2.0 ** -20)
 
 
+@pytest.mark.parametrize("old,new", [(2.0 ** 121, 1.5 * 2.0 ** 121), (2.0 ** 122, 2.0 ** 124), (2.0 ** 126, 1.9921875 * 2.0 ** 127),
+                                     (2.0 ** -119, 2.0 ** 127), (2.0 ** -119, 1.0078125 * 2.0 ** -119), (2.0 ** -119, 2.0 ** -118)])
+def test_pages_at_the_ends_of_the_range(old, new):
+    """Codes, magnitudes and what they stand for, of a page that goes on and of a new one."""
+    k_pages, v_pages, table = _cache(1, 2, 16, 1, 128)
+    for pages in (k_pages, v_pages):
+        pages.codes[:, :, :5] = torch.randint(-127, 128, (1, 1, 5, 128), generator=torch.Generator().manual_seed(3), dtype=torch.int8)
+        pages.tops.fill_(old)
+    x = _values(1, 20, 1, 128, seed=13)
+    x = (x / x.abs().amax(-1, keepdim=True) * new).bfloat16()
+    want = [(p.codes.clone(), p.tops.clone()) for p in (k_pages, v_pages)]
+    values = [_append_loop(y, *held, table, [5], [20]) for y, held in zip((x, -x), want)]
+    got = int8_ops.append_int8(x, -x, k_pages, v_pages, table, torch.tensor([5], dtype=torch.int32), values=True)
+    for pages, (codes, tops), y, z in zip((k_pages, v_pages), want, got, values):
+        assert torch.equal(pages.codes, codes) and torch.equal(pages.tops, tops) and torch.equal(y, z) and y.isfinite().all()
+        exact = codes.double() * tops.double()[..., None, None] / 127
+        # A product of 15 bits, which is exact, and a quotient in 32.
+        assert ((int8_ops.page_values(pages).double() - exact).abs() <= 2.0 ** -24 * exact.abs()).all()
+
+
 def test_blocks_that_are_not_finite_and_blocks_of_zeros():
     k_pages, v_pages, table = _cache(1, 2, 16, 2, 64)
     page = int(table[0, 0])
