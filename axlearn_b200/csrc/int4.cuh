@@ -31,7 +31,4 @@ __device__ __forceinline__ uint32_t int4_high(uint32_t x) { return x & 0x00f000f
 __device__ __forceinline__ float pair_s(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float pair_m(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
 
-// A bad index that the device found: code 5 of the status word.
-__device__ __forceinline__ void int4_report(int* status) { *reinterpret_cast<volatile int*>(status) = 5; }
-
 }  // namespace axb

@@ -13,6 +13,7 @@
 #include "cluster.cuh"
 #include "int4.cuh"
 #include "mma_sync.cuh"
+#include "status.cuh"
 
 namespace axb {
 
@@ -185,7 +186,7 @@ int4_append_kernel(Int4AppendParams p) {
       if (page < static_cast<uint32_t>(p.num_pages))
         slot = (static_cast<int64_t>(page) * p.num_kv_heads + head) * page_size + (pos - col * page_size);
       else
-        int4_report(p.status);
+        report_bad_argument(p.status);
     }
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
@@ -347,7 +348,7 @@ int4_attn_kernel(Int4AttnParams p) {
   const int step = kAttnWarps * p.splits;
   int tile = split * kAttnWarps + warp;
   if (len > p.max_pages * static_cast<int64_t>(p.page_size) || (kAppend && len > p.angle_rows)) {
-    if (threadIdx.x == 0) int4_report(p.status);
+    if (threadIdx.x == 0) report_bad_argument(p.status);
     len = kAppend ? 0 : p.max_pages * p.page_size;  // a new token without a place or a rotation: nothing is appended
   }
   const int hi = (max(len, 0) + kAttnKeys - 1) / kAttnKeys;
@@ -366,7 +367,7 @@ int4_attn_kernel(Int4AttnParams p) {
     const int t = tile * kAttnKeys + lane;
     if (tile >= hi || t >= cached) return kNone;
     if (page >= static_cast<uint32_t>(p.num_pages)) {
-      int4_report(p.status);
+      report_bad_argument(p.status);
       return kNone;
     }
     return (page * p.num_kv_heads + kvh) * p.page_size + (t - col_of(t) * p.page_size);
@@ -427,7 +428,7 @@ int4_attn_kernel(Int4AttnParams p) {
       new_word = row_word<H>(quantize8(x, new_pair, level), l8, new_byte);
       const uint32_t to = static_cast<uint32_t>(table[col_of(pos)]);
       if (to >= static_cast<uint32_t>(p.num_pages)) {
-        int4_report(p.status);
+        report_bad_argument(p.status);
       } else if (first == 0 && lane < 2 * kRowLanes) {  // (the other parts of a large group have the same)
         const int64_t slot =
             (static_cast<int64_t>(to) * p.num_kv_heads + kvh) * p.page_size + (pos - col_of(pos) * p.page_size);

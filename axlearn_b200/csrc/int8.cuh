@@ -89,9 +89,6 @@ __device__ __forceinline__ float int8_larger(float top, float x) {
   return y;
 }
 
-// A bad index that the device found: code 5 of the status word.
-__device__ __forceinline__ void int8_report(int* status) { *reinterpret_cast<volatile int*>(status) = 5; }
-
 // Arguments of the entry points travel as one block of 64-bit words (pointers, whole numbers, and doubles), in the order of their
 // structs: twenty of ctypes' conversions cost 3 us, packing them 1.
 struct Int8RowsCall {

@@ -13,6 +13,7 @@
 #include "int8.cuh"
 #include "mma_sync.cuh"
 #include "opt_in.cuh"
+#include "status.cuh"
 
 namespace axb {
 
@@ -128,7 +129,7 @@ int8_append_kernel(Int8AppendParams p) {
   uint32_t page = 0xffffffffu;
   if (begin >= 0 && col < p.max_pages) page = static_cast<uint32_t>(p.page_table[static_cast<int64_t>(b) * p.max_pages + col]);
   const bool placed = page < static_cast<uint32_t>(p.num_pages);
-  if (!placed) int8_report(p.status);
+  if (!placed) report_bad_argument(p.status);
   const int64_t block = placed ? static_cast<int64_t>(page) * p.num_kv_heads + head : 0;
   const uint32_t old = placed && row0 > 0
                            ? static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(pool.tops + block) & 0x7fff) << 16 : 0u;
@@ -364,7 +365,7 @@ int8_attn_kernel(Int8AttnParams p) {
 #pragma unroll
   for (int j = 0; j < kDigitSteps; ++j) q_raw[j] = r < rows ? *reinterpret_cast<const uint4*>(q_at + (j >> 1) * 32 + (j & 1) * 8) : zeros;
   if (len > capacity || (p.limit >= 0 && len > p.limit)) {
-    if (threadIdx.x == 0) int8_report(p.status);
+    if (threadIdx.x == 0) report_bad_argument(p.status);
     len = p.limit >= 0 ? 0 : static_cast<int>(capacity);
   }
   len = max(len, 0);
@@ -378,7 +379,7 @@ int8_attn_kernel(Int8AttnParams p) {
     Places at{-1, 0, 0};
     if (pos >= len) return at;
     if (page >= static_cast<uint32_t>(p.num_pages)) {
-      int8_report(p.status);
+      report_bad_argument(p.status);
       return at;
     }
     const uint32_t col = p.page.div(static_cast<uint32_t>(pos));

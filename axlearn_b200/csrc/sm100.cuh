@@ -14,17 +14,9 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-namespace axb {
+#include "status.cuh"
 
-// Status codes written to the global status word (0 = ok).
-enum : int {
-  kStatusOk = 0,
-  kStatusWaitTimeoutProducer = 1,
-  kStatusWaitTimeoutMma = 2,
-  kStatusWaitTimeoutEpilogue = 3,
-  kStatusWaitTimeoutPeer = 4,
-  kStatusBadArgument = 5,
-};
+namespace axb {
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));

@@ -111,7 +111,7 @@ embed_rows_kernel(const uint4* __restrict__ table, const int64_t* ids, uint4* ou
     out[b * vecs + i] = ok ? __ldg(table + id * table_ld + i)
                            : make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
   if (threadIdx.x == 0) {
-    if (!ok && status != nullptr) atomicCAS(status, 0, kStatusBadArgument);
+    if (!ok && status != nullptr) report_bad_argument(status);
     if (lengths != nullptr) lengths[b] = min(lengths[b] + 1, max_len);
   }
 }

@@ -174,16 +174,18 @@ _STATUS_TEXT = {
 
 
 def status_word(device: Optional[torch.device] = None) -> torch.Tensor:
+    """What kernels report (``csrc/status.cuh``): a wait that gave up, and a bad argument."""
     idx = torch.cuda.current_device() if device is None or device.index is None else device.index
     if idx not in _status:
-        _status[idx] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+        _status[idx] = torch.zeros(2, dtype=torch.int32, device=torch.device("cuda", idx))
     return _status[idx]
 
 
 def check_status(device: Optional[torch.device] = None, *, clear: bool = True) -> None:
-    """Raises if any kernel on ``device`` reported a bounded-wait timeout (synchronises)."""
+    """Raises if any kernel on ``device`` reported a bounded-wait timeout, or else a bad argument (synchronises)."""
     w = status_word(device)
-    code = int(w.item())
+    waits, arguments = w.tolist()
+    code = waits or arguments
     if code != 0:
         if clear:
             w.zero_()

@@ -355,7 +355,7 @@ def _check_counts(counts: Tensor, batch: int, name: str, device) -> Tensor:
 def _report_places(bad: Tensor, what: str) -> None:
     """``bad`` (a truth value): an error on the host, the status word on the GPU."""
     if bad.is_cuda:
-        word = cuda_ops.status_word(bad.device)
+        word = cuda_ops.status_word(bad.device)[1]
         word.copy_(torch.where(bad, 5, word))
     elif bool(bad):
         raise IndexError(what)

@@ -471,6 +471,51 @@ def test_bad_places_are_reported_and_not_touched():
         assert torch.equal(a, o) and torch.equal(p.codes, y.codes) and torch.equal(p.tops, y.tops)
 
 
+def _report_a_bad_place(plain):
+    k_pages, v_pages, table = _cache(1, 1, 16, 1, 64)
+    x = _normal(_gen(1), 1, 1, 1, 64).bfloat16()
+    args = (x, x, k_pages, v_pages, torch.full_like(table, 99), torch.zeros(1, dtype=torch.int32, device="cuda"))
+    _plain(int8_ops.append_int8, *args) if plain else int8_ops.append_int8(*args)
+
+
+@pytest.mark.parametrize("plain", [False, True])
+def test_a_bad_place_does_not_hide_a_wait_that_gave_up(plain):
+    word = cuda_ops.status_word()
+    word[0] = 2  # as a kernel whose wait gave up leaves it
+    try:
+        _report_a_bad_place(plain)
+        with pytest.raises(RuntimeError, match="status 2"):
+            cuda_ops.check_status()
+        cuda_ops.check_status()
+        _report_a_bad_place(plain)
+        with pytest.raises(RuntimeError, match="status 5"):
+            cuda_ops.check_status()
+    finally:
+        word.zero_()
+
+
+@pytest.mark.parametrize("product", ["int8", "bf16"])
+def test_products_behind_a_bad_place_take_no_longer(product):
+    """A kernel waits 2 ms on its way out where a wait gave up, not where an index was bad."""
+    gen = _gen(2)
+    w, x = _weight(gen, 256, 256), _normal(gen, 300, 256).bfloat16()
+    held, plain = int8_ops.quantize_rows(x), _normal(gen, 256, 256).bfloat16()
+    call = (lambda: int8_ops.int8_linear(held, w)) if product == "int8" else (lambda: cuda_ops.gemm(x, plain))
+    want = call()
+    _report_a_bad_place(False)
+    times = []
+    for _ in range(5):
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        start.record()
+        got = call()
+        end.record()
+        end.synchronize()
+        times.append(start.elapsed_time(end))
+    with pytest.raises(RuntimeError, match="status 5"):
+        cuda_ops.check_status()
+    assert torch.equal(got, want) and min(times) < 1
+
+
 @pytest.mark.parametrize("b,t,nq,kv,dim", [(2, 300, 8, 2, 128), (1, 1, 4, 4, 64), (3, 130, 12, 4, 64), (3, 1300, 6, 2, 128)])
 @pytest.mark.parametrize("ragged", [False, True])
 def test_prompts_attend_to_what_the_cache_stands_for(b, t, nq, kv, dim, ragged):
