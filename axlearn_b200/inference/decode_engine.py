@@ -423,8 +423,8 @@ class DecodeEngine(BaseDecodeEngine):
                         softmax_scale=self._softmax_scale)
                 branch = self._sum_ranks(self._product(attn.reshape(rows, self.nq_l * h), lw.wo))
                 x, hn = self._add_norm(x, branch, lw.ffn_norm, lw.wgu)
-                plain = isinstance(lw.wgu, Tensor) and isinstance(lw.wdown, Tensor)
-                act = cuda_ops.gemm_swiglu(hn, lw.wgu) if plain else None
+                fused = isinstance(lw.wgu, Tensor) and not isinstance(lw.wdown, int8_ops.Int8Weight)
+                act = cuda_ops.gemm_swiglu(hn, lw.wgu) if fused else None
                 if act is None:
                     act = self._gated(self._product(hn, lw.wgu), lw.wdown)
                 branch = self._sum_ranks(self._product(act, lw.wdown))

@@ -869,6 +869,23 @@ def test_engine_steps_in_8_bits_at_serving_widths(batch):
         assert torch.equal(x, y), i
 
 
+@pytest.mark.parametrize("down,fused", [(16, True), (4, True), (8, False)])
+def test_prompts_fuse_gate_and_up_wherever_the_down_projection_takes_16_bits(down, fused, monkeypatch):
+    import dataclasses
+
+    from axlearn_b200.inference import decode_engine
+    from axlearn_b200.ops import int4_ops
+
+    weights, dims = _engine_weights(256, 512, 1000, 4, 4, 2)
+    hold = {16: lambda w: w, 8: int8_ops.quantize_weight, 4: int4_ops.quantize_weight}[down]
+    weights["layers"] = [dataclasses.replace(lw, wdown=hold(lw.wdown)) for lw in weights["layers"]]
+    calls, real = [], cuda_ops.gemm_swiglu
+    monkeypatch.setattr(cuda_ops, "gemm_swiglu", lambda *args: (calls.append(args), real(*args))[1])
+    engine = decode_engine.DecodeEngine(weights, dims, batch=2, max_len=96, use_graph=False)
+    engine.prefill(torch.randint(0, 1000, (2, 64), device="cuda", generator=_gen(1)))
+    assert len(calls) == (2 if fused else 0) and engine.logits.isfinite().all()
+
+
 def test_engine_in_8_bits_is_close_to_16_bits():
     """What both formats lose on a small model: rows, weights and cache are each off by up to half of 1 / 127 of their largest value."""
     from axlearn_b200.inference import decode_engine
