@@ -151,7 +151,8 @@ def swiglu_int8(gu: Tensor) -> Int8Rows:
     _no_gradient("swiglu_int8", gu)
     if not _on_kernel(gu):
         gate, up = gu.float().chunk(2, -1)
-        return _plain_rows(torch.nn.functional.silu(gate) * up)
+        far = gate < -80  # 1 + exp(gate) is 1, and 1 + exp(-gate) about to be infinite
+        return _plain_rows(torch.where(far, gate * torch.exp(gate), torch.nn.functional.silu(gate)) * up)
     return _launch_rows(gu, gu.shape[-1] // 2, True)
 
 

@@ -114,6 +114,23 @@ def test_swiglu_is_its_formula(rows, dim):
     assert ((int8_ops.row_values(got).double() - y).abs() <= (0.5 + 127 * 2.0 ** -20) * top / 127).all()
 
 
+def test_swiglu_of_gates_far_below_zero():
+    """Rows whose largest product is one of a gate beyond -87.3 = log 2^-126."""
+    gate = torch.linspace(-90, -86, 4 * 64, device="cuda").bfloat16().view(4, 64)
+    up = torch.full((4, 64), 2.0 ** 20, device="cuda").bfloat16()
+    up[1], up[2, 1::2] = 2.0 ** 100, -1
+    gu = torch.cat([gate, up], 1)
+    got = int8_ops.swiglu_int8(gu)
+    gate, up = gu.double().chunk(2, -1)
+    y = gate * torch.sigmoid(gate) * up
+    top = y.abs().amax(-1, keepdim=True)
+    # Half a level; |t| 2^-24 and two units of the exponential, whose denormal values (from 2^-131 = exp(-90.8) on) have 19 bits.
+    assert got.codes.any(1).all() and ((int8_ops.row_values(got).double() - y).abs() <= (0.5 + 127 * 2.0 ** -16) * top / 127).all()
+    gu = torch.tensor([[-float("inf"), 1.0] * 8, [float("inf"), 1.0] * 8, [-200.0] * 16, [0.0, -0.0] * 8], device="cuda").bfloat16()
+    rows = int8_ops.swiglu_int8(torch.cat([gu, torch.ones_like(gu)], 1))
+    assert rows.scales[:2].isnan().all() and not rows.codes.any() and not rows.scales[2:].any()
+
+
 # ------------------------------------------------------------------------------------------
 # Products.
 # ------------------------------------------------------------------------------------------

@@ -71,6 +71,20 @@ def test_swiglu_is_its_formula():
     assert ((int8_ops.row_values(rows).double() - y).abs() <= (0.5 + 127 * 2.0 ** -20) * top / 127).all()
 
 
+def test_swiglu_of_gates_far_below_zero():
+    gate = torch.linspace(-90, -79, 64).view(4, 16)
+    up = torch.full((4, 16), 2.0 ** 20)
+    up[1], up[2, 1::2] = 2.0 ** 100, -1
+    rows = int8_ops.swiglu_int8(torch.cat([gate, up], 1))
+    y = gate.double() * torch.sigmoid(gate.double()) * up.double()
+    top = y.abs().amax(-1, keepdim=True)
+    # Half a level; three products in 32 bits, and exponentials of a unit that are denormal from 2^-130 on (20 bits).
+    assert rows.codes.any(1).all() and ((int8_ops.row_values(rows).double() - y).abs() <= (0.5 + 127 * 2.0 ** -18) * top / 127).all()
+    gu = torch.tensor([[-float("inf"), 1.0] * 8, [float("inf"), 1.0] * 8, [-200.0] * 16, [0.0, -0.0] * 8])
+    rows = int8_ops.swiglu_int8(torch.cat([gu, torch.ones_like(gu)], 1))
+    assert rows.scales[:2].isnan().all() and not rows.codes.any() and not rows.scales[2:].any()
+
+
 @pytest.mark.parametrize("k,n", [(16, 8), (48, 24), (272, 40)])
 def test_linear_is_the_product_of_what_both_stand_for(k, n):
     w = int8_ops.quantize_weight(_values(k, n, seed=5) * 0.1)
