@@ -651,6 +651,7 @@ def prompt_attention_int8(qkv: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, p
             x.copy_(y)
         out = dispatch.reference.attention(q, k, v, causal=True, softmax_scale=softmax_scale)
         return out.reshape(b, t, num_q_heads * h)
+    _check_attention(softmax_scale, None)
     from axlearn_b200.ops import decode_ops
 
     _call(device, "axb_int8_rope_append", qkv.data_ptr(), 0, *pools, page_table.data_ptr(), 0, 0 if live is None else live.data_ptr(),

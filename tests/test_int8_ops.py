@@ -393,6 +393,21 @@ def test_sizes_and_types_that_are_refused():
                                        live=torch.ones(2))
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.1, math.nan, math.inf, 2.0 ** 20])
+def test_scales_that_are_refused_leave_the_cache_as_it_was(scale):
+    k_pages, v_pages, table = _cache(2, 2, 16, 2, 64)
+    _fill(k_pages, 1), _fill(v_pages, 2)
+    kept = [x.clone() for x in (*k_pages, *v_pages)]
+    rope, qkv = torch.zeros(32, 32, 2), _values(2, 3, 384)
+    given = qkv.clone()
+    with pytest.raises(ValueError, match="softmax_scale"):
+        int8_ops.prompt_attention_int8(qkv, k_pages, v_pages, table, rope, num_q_heads=2, softmax_scale=scale)
+    with pytest.raises(ValueError, match="softmax_scale"):
+        int8_ops.rope_decode_attention_int8(qkv[:, 0].contiguous(), k_pages, v_pages, table, torch.ones(2, dtype=torch.int32), rope,
+                                            num_q_heads=2, softmax_scale=scale)
+    assert torch.equal(qkv, given) and all(torch.equal(x, y) for x, y in zip((*k_pages, *v_pages), kept))
+
+
 def _calls_with_operands():
     k_pages, v_pages, table = _cache(1, 2, 16, 1, 64)
     weight = int8_ops.quantize_weight(_values(16, 8))
