@@ -51,6 +51,7 @@ LEAST = 2.0 ** -119
 MAX_ROW = 65536        # values of a row that the row kernels keep
 MAX_K = 1 << 17        # products of 127 x 127 whose sums fit 32 bits
 MAX_SPLITS = 1024      # of a sequence's keys
+MAX_GRID = 65535       # sequences of an attention launch, and groups of eight query heads of one KV head
 PAGE_UNIT = 16         # tokens of a page are a multiple of
 # Entry points and the 64-bit words of their arguments (``csrc/int8.cuh``).
 _WORDS = {"axb_int8_rows": "7q", "axb_int8_add_rms_norm": "9qd", "axb_gemm_skinny_int8": "12q", "axb_int8_gemm": "12q",
@@ -550,23 +551,33 @@ def paged_decode_attention_int8(q: Tensor, k_pages: Int8Pages, v_pages: Int8Page
     # (In place is fine: a CTA, and its cluster, has its heads' queries before it stores their output.)
     if not q.is_contiguous() or q.data_ptr() % 16 or (out is not None and q.data_ptr() != out.data_ptr() and _overlap(q, out)):
         q = q.clone(memory_format=torch.contiguous_format)
+    splits, scratch = _plan_attention(q, scratch, b, nq, h, cache, splits, device)
     if out is None:
         out = torch.empty_like(q)
     _launch_attention(q, pools, page_table, lengths, -1, out, scratch, b, nq, h, cache, splits, scale, device)
     return out
 
 
-def _launch_attention(q, pools, page_table, lengths, limit, out, scratch, b, nq, h, cache, splits, scale, device):
-    num_pages, nkv, page_size, max_pages = cache
+def _plan_attention(like: Tensor, scratch: Optional[Tensor], b: int, nq: int, h: int, cache: tuple, splits: Optional[int],
+                    device: int) -> tuple:
+    """``(splits, scratch)`` of a launch; what it refuses is refused ahead of an append."""
+    _, nkv, page_size, max_pages = cache
+    if not nq or max(b, nkv * -(-nq // (8 * nkv))) > MAX_GRID:
+        raise ValueError(f"{b} sequences, {nq} query heads for {nkv}: 1 to {MAX_GRID} groups of eight heads, up to {MAX_GRID} sequences")
     if splits is None:
         splits = attention_splits(b, nkv, nq // nkv, max_pages * page_size)
     if splits > 8:
         floats = attention_scratch_floats(b, nq, h, splits)
         if scratch is None:
-            scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
+            scratch = torch.empty(floats, dtype=torch.float32, device=like.device)
         elif (scratch.numel() < floats or scratch.dtype != torch.float32 or scratch.get_device() != device
               or not scratch.is_contiguous() or scratch.data_ptr() % 8):
-            raise ValueError(f"scratch is {floats} contiguous fp32 values on {q.device}, 8-byte aligned")
+            raise ValueError(f"scratch is {floats} contiguous fp32 values on {like.device}, 8-byte aligned")
+    return splits, scratch
+
+
+def _launch_attention(q, pools, page_table, lengths, limit, out, scratch, b, nq, h, cache, splits, scale, device):
+    num_pages, nkv, page_size, max_pages = cache
     _call(device, "axb_int8_decode_attn", q.data_ptr(), *pools, page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(),
           0 if scratch is None else scratch.data_ptr(), limit, b, nq, nkv, h, page_size, max_pages, num_pages, splits, scale,
           _status(device))
@@ -617,6 +628,7 @@ def rope_decode_attention_int8(qkv: Tensor, k_pages: Int8Pages, v_pages: Int8Pag
         q, k = _rotate(q, table, pos), _rotate(k, table, pos)
         _append_plain(k, v, k_pages, v_pages, page_table, lengths - 1, (lengths > 0).to(torch.int32))
         return paged_decode_attention_int8(q[:, 0], k_pages, v_pages, page_table, lengths, softmax_scale=softmax_scale)
+    splits, scratch = _plan_attention(qkv, scratch, b, num_q_heads, h, cache, splits, device)
     out = qkv.new_empty((b, num_q_heads, h))  # the rotated queries, then what they attend to
     _call(device, "axb_int8_rope_append", qkv.data_ptr(), out.data_ptr(), *pools, page_table.data_ptr(), lengths.data_ptr(), 0, table.data_ptr(),
           table.shape[0], b, 1, num_q_heads, nkv, h, page_size, max_pages, num_pages, _status(device))
@@ -639,6 +651,7 @@ def prompt_attention_int8(qkv: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, p
         raise ValueError(f"{b} x {t} tokens, a rotation table of {table.shape[0]} positions, a page table {tuple(page_table.shape)}")
     if live is not None:
         _check_counts(live, b, "live", device)
+    _check_attention(softmax_scale, None)
     _no_gradient("prompt_attention_int8", qkv, k_pages.tops, v_pages.tops, table)
     if not qkv.numel():
         return qkv.new_empty((b, t, num_q_heads * h))
@@ -651,9 +664,10 @@ def prompt_attention_int8(qkv: Tensor, k_pages: Int8Pages, v_pages: Int8Pages, p
             x.copy_(y)
         out = dispatch.reference.attention(q, k, v, causal=True, softmax_scale=softmax_scale)
         return out.reshape(b, t, num_q_heads * h)
-    _check_attention(softmax_scale, None)
     from axlearn_b200.ops import decode_ops
 
+    if max(b, num_q_heads) > MAX_GRID:
+        raise ValueError(f"{b} prompts, {num_q_heads} query heads: up to {MAX_GRID} of each")
     _call(device, "axb_int8_rope_append", qkv.data_ptr(), 0, *pools, page_table.data_ptr(), 0, 0 if live is None else live.data_ptr(),
           table.data_ptr(), table.shape[0], b, t, num_q_heads, nkv, h, page_size, max_pages, num_pages, _status(device))
     with _on(qkv.device):

@@ -573,6 +573,27 @@ def test_scratch_that_does_not_fit_is_refused():
     assert torch.equal(call(torch.empty(floats, device="cuda")), call(None))
 
 
+def test_a_step_that_is_refused_appends_nothing():
+    k_pages, v_pages, table = _cache(1, 64, 16, 1, 64)
+    rope = decode_ops.rope_table(1024, 64, 1e4, torch.device("cuda"))
+    kept = [x.clone() for x in (*k_pages, *v_pages)]
+    many = int8_ops.MAX_GRID + 1
+    lengths = torch.zeros(many, dtype=torch.int32, device="cuda")
+    lengths[0] = 1000
+    qkv = _normal(_gen(1), many, 3 * 64).bfloat16()
+    for b, scratch in ((1, torch.empty(8, device="cuda")), (many, None)):
+        with pytest.raises(ValueError):
+            int8_ops.rope_decode_attention_int8(qkv[:b], k_pages, v_pages, table.expand(b, -1).contiguous(), lengths[:b], rope,
+                                                num_q_heads=1, softmax_scale=0.1, splits=16, scratch=scratch)
+    given = qkv.clone()
+    with pytest.raises(ValueError):
+        int8_ops.prompt_attention_int8(qkv[:, None], k_pages, v_pages, table.expand(many, -1).contiguous(), rope, num_q_heads=1,
+                                       softmax_scale=0.1, live=torch.zeros_like(lengths))
+    with pytest.raises(ValueError):
+        int8_ops.paged_decode_attention_int8(qkv.view(many, 3, 64)[:, :1], k_pages, v_pages, table.expand(many, -1).contiguous(), lengths)
+    assert torch.equal(qkv, given) and all(torch.equal(x, y) for x, y in zip((*k_pages, *v_pages), kept))
+
+
 @pytest.mark.parametrize("nq,kv,dim,splits", [(8, 2, 128, 1), (8, 8, 64, 8), (40, 2, 128, 3), (4, 1, 128, 16)])
 def test_attention_in_place(nq, kv, dim, splits):
     k_pages, v_pages, table = _cache(3, 40, 16, kv, dim)
