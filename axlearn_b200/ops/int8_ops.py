@@ -493,10 +493,13 @@ def attention_splits(batch: int, num_kv_heads: int, group: int, max_len: int, sm
     x 4096 41 35, 46 59), and those of more than 8192 twice as many CTAs (42 x 9600 108 85, 30 x 9600 85 69, all as long 141 146 and 98 124).
     Long sequences of few heads take as many as fill most SMs with CTAs of three times the warps, and a second launch that joins them
     (8 heads with 8 / 16 / 18 / 24: 16000 tokens 18.7 14.0 15.7, 130001 tokens 127 47.6 51.9 69; one head with 16 / 32 / 64 / 128: 60000
-    tokens 26.0 18.9 19.5 24.5)."""
+    tokens 26.0 18.9 19.5 24.5), but no more than leave each warp a tile of 32 keys (so / 48: one head 8208 tokens 8.5 10.4, 12000 8.9
+    10.4, two heads 9.2 11.3, 9.9 11.4), and 48, which short sequences in a wide table pay for, up to 2^18 tokens (one head with 48 / 96:
+    131072 tokens 21.5 20.8, 262144 32.0 26.8, a million 92 60, but 8208 10.4 14.5).  What the rule costs elsewhere: 300 tokens of 8 heads
+    in a table of 16384 8.5 where one split takes 5.7; nothing at 130001 tokens of 32 heads (8 splits: 160, at the copy rate 163)."""
     ctas = max(1, batch * num_kv_heads * ((group + 7) // 8))
     if max_len > 8192 and ctas * 9 <= sms:
-        return min(48, max(9, 128 // ctas))
+        return max(9, min(128 // ctas, 48 if max_len < 2 ** 18 else 96, -(-max_len // (12 * 32))))
     at_once = (6 if max_len > 8192 else 3) * sms
     best, least = 1, math.inf
     for splits in (1, 2, 4, 8):

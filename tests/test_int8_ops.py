@@ -458,6 +458,20 @@ def test_empty_calls():
         assert got.shape == shape[:2] + (128,)
 
 
+def test_splits_have_keys_and_fit():
+    for ctas in (1, 2, 3, 5, 8, 14, 16, 17, 40, 148, 600):
+        for tokens in (1, 63, 64, 127, 128, 500, 4095, 4096, 8192, 8193, 8208, 12000, 16384, 60000, 2 ** 18 - 1, 2 ** 18, 10 ** 6):
+            splits = int8_ops.attention_splits(1, ctas, 1, tokens)
+            assert 1 <= splits <= int8_ops.MAX_SPLITS
+            if splits <= 8:  # a cluster
+                assert splits in (1, 2, 4, 8) and (splits == 1 or splits * 64 <= tokens)
+                assert splits <= 2 or splits * ctas <= (6 if tokens > 8192 else 3) * 148
+            else:            # twelve warps a split, a tile of 32 keys for each; a CTA an SM
+                assert tokens > 8192 and (splits - 1) * 12 * 32 < tokens and splits * ctas <= 148
+    assert [int8_ops.attention_splits(1, 1, 1, tokens) for tokens in (8192, 8208, 16384, 60000, 10 ** 6)] == [8, 22, 43, 48, 96]
+    assert [int8_ops.attention_splits(1, 8, 4, tokens) for tokens in (300, 16384, 130048)] == [4, 16, 16]
+
+
 @pytest.mark.parametrize("batch,kv,group,tokens", [(1, 16, 1, 300), (16, 8, 4, 2048), (64, 32, 1, 2000), (1, 8, 4, 130048), (0, 8, 1, 64),
                                                    (1, 1, 1, 1), (1, 1, 40, 10 ** 6)])
 def test_splits_of_attention(batch, kv, group, tokens):
