@@ -437,6 +437,26 @@ def test_a_step_is_rotation_append_and_attention(nq, kv, dim, splits):
     assert ((got.double() - want).abs() <= bound + 2.0 ** -6).all()
 
 
+@pytest.mark.parametrize("nq,kv,dim,splits", [(4, 4, 128, 1), (8, 2, 64, 3), (20, 2, 128, 9), (32, 8, 128, None)])
+def test_a_step_attends_to_the_cache_that_it_leaves(nq, kv, dim, splits):
+    """Bit for bit: its rotated queries are those of the same token as the last one of a prompt."""
+    b, t, gen = 3, 77, _gen(nq + dim)
+    rope = decode_ops.rope_table(96, dim, 1e4, torch.device("cuda"))
+    qkv = _normal(gen, b, t, (nq + 2 * kv) * dim).bfloat16()
+    lengths = torch.tensor([77, 1, 33], dtype=torch.int32, device="cuda")
+    k_pages, v_pages, table = _cache(b, 6, 16, kv, dim, seed=nq)
+    whole = qkv.clone()
+    int8_ops.prompt_attention_int8(whole, k_pages, v_pages, table, rope, num_q_heads=nq, softmax_scale=0.08)
+    int8_ops.prompt_attention_int8(qkv.clone(), k_pages, v_pages, table, rope, num_q_heads=nq, softmax_scale=0.08, live=lengths - 1)
+    at = torch.arange(b, device="cuda")
+    got = int8_ops.rope_decode_attention_int8(qkv[at, lengths.long() - 1], k_pages, v_pages, table, lengths, rope, num_q_heads=nq,
+                                              softmax_scale=0.08, splits=splits)
+    q = whole[at, lengths.long() - 1, :nq * dim].view(b, nq, dim)
+    assert torch.equal(got, int8_ops.paged_decode_attention_int8(q, k_pages, v_pages, table, lengths, softmax_scale=0.08, splits=splits))
+    want, bound = _attention64(q, k_pages, v_pages, table, lengths, 0.08)
+    assert ((got.double() - want).abs() <= bound).all()
+
+
 def test_a_step_without_a_place_appends_nothing():
     k_pages, v_pages, table = _cache(4, 2, 16, 2, 64)
     rope = decode_ops.rope_table(24, 64, 1e4, torch.device("cuda"))

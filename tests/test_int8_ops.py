@@ -472,6 +472,24 @@ def test_splits_have_keys_and_fit():
     assert [int8_ops.attention_splits(1, 8, 4, tokens) for tokens in (300, 16384, 130048)] == [4, 16, 16]
 
 
+@pytest.mark.parametrize("rows,k,n,few", [(96, 4096, 4096, True), (97, 4096, 4096, False), (128, 4096, 4096, False), (128, 4112, 4096, True),
+                                          (129, 4112, 4096, False), (128, 4096, 74 * 128, False), (128, 4096, 74 * 128 + 8, True),
+                                          (1, 16, 8, True), (129, 131072, 40000, False)])
+def test_products_that_stream_the_weight(rows, k, n, few):
+    """96 rows, and 128 where K is above 4096 or tiles of 128 columns are more than the 74 pairs of SMs."""
+    assert int8_ops.few_rows(rows, k, n) is few
+
+
+@pytest.mark.parametrize("rows,n,features", [
+    (256, 74 * 128, 128), (256, 74 * 128 + 8, 256),      # one wave of narrow tiles, or two (1.24 of a wide one's time)
+    (512, 37 * 128, 128), (512, 37 * 128 + 8, 256),
+    (256, 74 * 256, 256), (256, 74 * 256 + 8, 128),      # two narrow waves for one wide one; three for two
+    (333, 8192, 256), (8192, 22016, 256), (129, 8, 128),
+])
+def test_features_of_a_tile(rows, n, features):
+    assert int8_ops.pair_features(rows, n) == features
+
+
 @pytest.mark.parametrize("batch,kv,group,tokens", [(1, 16, 1, 300), (16, 8, 4, 2048), (64, 32, 1, 2000), (1, 8, 4, 130048), (0, 8, 1, 64),
                                                    (1, 1, 1, 1), (1, 1, 40, 10 ** 6)])
 def test_splits_of_attention(batch, kv, group, tokens):
