@@ -664,8 +664,8 @@ def dims_from_decoder(decoder) -> Optional[FujiDims]:
 def _bits(name: str) -> int:
     value = os.environ.get("AXB200_DECODE_WEIGHT_BITS", "16") if name == "WEIGHT" else os.environ.get("AXB200_DECODE_CACHE_BITS", "16")
     if value not in ("4", "16"):
-        raise ValueError(f"AXB200_DECODE_{name}_BITS is 4 or 16, not {value!r}")
-    eights = [part for part in os.environ.get("AXB200_DECODE_INT8", "").split(",") if part]
+        raise ValueError(f"AXB200_DECODE_{name}_BITS is 4 or 16, not {value!r}; AXB200_DECODE_INT8 names what is held in 8 bits")
+    eights = [part.strip() for part in os.environ.get("AXB200_DECODE_INT8", "").split(",") if part.strip()]
     if any(part not in ("weights", "cache") for part in eights):
         raise ValueError(f"AXB200_DECODE_INT8 lists weights and cache, not {eights}")
     if {"WEIGHT": "weights", "CACHE": "cache"}[name] not in eights:

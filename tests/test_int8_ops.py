@@ -408,6 +408,25 @@ def test_scales_that_are_refused_leave_the_cache_as_it_was(scale):
     assert torch.equal(qkv, given) and all(torch.equal(x, y) for x, y in zip((*k_pages, *v_pages), kept))
 
 
+def test_formats_of_the_environment(monkeypatch):
+    from axlearn_b200.inference import decode_engine
+
+    bits = decode_engine._bits  # pylint: disable=protected-access
+    assert (bits("WEIGHT"), bits("CACHE")) == (16, 16)
+    for value, want in (("weights", (8, 16)), ("cache", (16, 8)), ("weights,cache", (8, 8)), (" cache, weights ", (8, 8)), ("", (16, 16))):
+        monkeypatch.setenv("AXB200_DECODE_INT8", value)
+        assert (bits("WEIGHT"), bits("CACHE")) == want
+    monkeypatch.setenv("AXB200_DECODE_CACHE_BITS", "8")
+    with pytest.raises(ValueError, match="4 or 16.*AXB200_DECODE_INT8"):
+        bits("CACHE")
+    for value in ("4", "16"):
+        monkeypatch.setenv("AXB200_DECODE_CACHE_BITS", value)
+        assert bits("CACHE") == int(value)
+    monkeypatch.setenv("AXB200_DECODE_INT8", "caches")
+    with pytest.raises(ValueError, match="AXB200_DECODE_INT8"):
+        bits("CACHE")
+
+
 def _calls_with_operands():
     k_pages, v_pages, table = _cache(1, 2, 16, 1, 64)
     weight = int8_ops.quantize_weight(_values(16, 8))
