@@ -12,7 +12,9 @@
 // Only tables of parameters that a step does not write may be `const __restrict__`.
 //
 // Launches are chained only while the calling thread captures a decoding step (`axb_chain_launches`): there, what may
-// be read ahead of the wait is known.  Kernels that stream much memory in one wave or with many small CTAs (expert
+// be read ahead of the wait is known.  The exception is a call of two launches whose second follows the first in any
+// setting (`ChainedBehind`): the first is launched in the ordinary way, so what is read ahead of the second's wait -- weights
+// -- was complete before the first started.  Kernels that stream much memory in one wave or with many small CTAs (expert
 // products, state-space and latent decoding) keep ordinary launches: started early, their CTAs go to the SMs that
 // happen to have room, and the uneven spread costs more than the launch (32 experts at batch 16: 59 -> 92 us, state-space
 // decoding 21.5 -> 25).

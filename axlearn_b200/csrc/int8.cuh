@@ -32,8 +32,8 @@ struct Int8Scale {
   __device__ __forceinline__ bool empty() const { return reciprocal == 0.f; }
 };
 
-// Codes of eight values as bytes.  The quotient is a product with the reciprocal and one correction by the exact remainder, which
-// rounds it correctly in 32 bits; with x and A of 8 bits (a cache) or of 16 (products of two bf16 numbers) a quotient that is not
+// Codes of eight values as bytes.  The quotient is a product with the reciprocal and one correction by the exact remainder of a fused
+// product (Markstein, IBM J. Res. Dev. 34, 1990), which rounds it correctly in 32 bits; with x and A of 8 bits (a cache) or of 16 (products of two bf16 numbers) a quotient that is not
 // k + 1/2 is off it by more than half a unit, so adding 1.5 2^23 rounds as in exact arithmetic.  Ties are no rare case to be left
 // to a branch: x = A / 2 is 63.5 (every second vector of 256 values has one; 16384 x 4096 rows 49.1 us with such a branch, 39.6 without).
 // A level is a float with its code in the last bits.  `kPairs`: two values an instruction, where it pays (us without / with them: rows of

@@ -240,7 +240,8 @@ constexpr int kI8AttnCluster = 8, kI8MostSplits = 1024;
 constexpr float kI8Slack = 8.f;
 
 // Warps of a CTA: four, three CTAs an SM, or, of more splits than a cluster has, twelve that have an SM to themselves: a third of the
-// parts (1 x 130001 tokens, 8 KV heads: 16 splits of twelve 49.5 us, 32 of four 51.6, 48 of four 53.8).
+// parts (1 x 130001 tokens, 8 KV heads, before scores and sums were two numbers an instruction: 16 splits of twelve 49.5 us, 32 of
+// four 51.6, 48 of four 53.8; 46.7 now).
 constexpr int kI8FewWarps = 4, kI8ManyWarps = 12;
 // Where a CTA's sums go: out, the CTA of its cluster that finishes a head, or scratch for a second launch.
 enum Int8Merge { kMergeNone, kMergeCluster, kMergeScratch };

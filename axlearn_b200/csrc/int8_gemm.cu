@@ -1,14 +1,16 @@
 // y[M, N] = x_scales[m] w_scales[n] sum_k x[m, k] w[n, k] (+ y) of 8-bit whole numbers on CTA pairs (`gemm_2cta.cu` is the same
-// division of work for bf16): sums are 32-bit integers in tensor memory, exact for K up to 2^17, and are rounded once, to y.
+// division of work for bf16): sums are 32-bit integers in tensor memory, exact for K up to 2^17.  A sum above 2^24 is rounded on its
+// way to fp32, as are its products with the two scales; behind that comes the rounding to y.
 //
 // Two CTAs on neighbouring SMs share a tile of 256 rows.  Each stages its own 128 rows of x and its own half of the tile's
 // features, 128 values of K a stage; one thread of the first CTA issues `tcgen05.mma.cta_group::2.kind::i8`; both drain their
 // 128 rows: a thread owns a row of x, so its scale is one register, and the features' scales are loads that a warp shares.
 // The next tile runs into the other half of tensor memory meanwhile.
 //
-// Measured with the rows' own kernel: 8192 x 4096 x 22016 441 to 465 us on a cool GPU (444 at twice the measured rate of bf16) and
-// 520 for as long as one likes, under the power cap; 333 x 2048 x 8192 12.5 us (3.5): two launches, a wave of 64 tiles of 256 x 256 for
-// 74 pairs, of whose 512 rows 333 are there.
+// Measured: 8192 x 4096 x 22016 441 to 465 us on a cool GPU (444 at twice the measured rate of bf16) and 520 for as long as one likes,
+// under the power cap; 333 x 2048 x 8192 12.2 us (3.5): one wave of 64 tiles of 256 x 256 for 74 pairs, of whose 512 rows 333 are
+// there.  In a row of calls 333 x K x 8192 takes 7.6 us at K = 128 and 2.5 for each 1024 of K (13.3 at 2048): what lies beside the MMAs is
+// the launch, the pair's barriers and tensor memory, the first loads, and the drain of a tile, 128 features a warp.
 #include "chain.cuh"
 #include "cta_pair.cuh"
 #include "host_utils.cuh"

@@ -6,7 +6,7 @@
 // summed row and w the norm's weights, round(127 t w / max |t w|).  t w has 16 bits, so codes are those of exact arithmetic.
 //
 // Measured: the norm of 8192 x 4096 with residual, sum and values 46.3 us (46.1 at the copy rate); rows of 16384 x 4096 33.5 (30.7), of
-// 16384 x 11008 97 (83), silu(gate) * up of it 183 (138), which its exponentials and quotients bound.  One row of 2048 takes 1.6 to 1.9,
+// 16384 x 11008 97 (83), silu(gate) * up of it 185 (138), which its exponentials and quotients bound.  One row of 2048 takes 1.6 to 1.9,
 // an empty launch's time.
 #include <math.h>
 

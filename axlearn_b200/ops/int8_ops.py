@@ -271,9 +271,11 @@ def few_rows(rows: int, k: int, n: int, sms: int = 148) -> bool:
 
 def int8_linear(x: Union[Tensor, Int8Rows], w: Int8Weight, *, out: Optional[Tensor] = None, accumulate: bool = False,
                 dtype: Optional[torch.dtype] = None, resident: bool = False) -> Tensor:
-    """``x [..., K] @ w`` with exact integer sums of the codes, times the scales of row and column, rounded once to ``dtype`` (that
-    of ``x`` where it is a tensor, which is quantised by rows first; else bf16); into ``out [..., N]``, or with ``accumulate`` added to
-    it ahead of that rounding.  ``out`` may overlap ``x``.  ``resident``: as in ``cuda_ops.gemm``.  Serving only: there is no gradient."""
+    """``x [..., K] @ w`` with exact integer sums of the codes, times the scales of row and column in 32 bits, rounded to ``dtype``
+    (that of ``x`` where it is a tensor, which is quantised by rows first; else bf16); into ``out [..., N]``, or with ``accumulate``
+    added to it ahead of that rounding.  ``out`` may overlap ``x``.  ``resident``: as in ``cuda_ops.gemm``.  The kernels' output is bf16:
+    for a tensor or ``dtype`` of another type the plain statement runs, on the GPU as well, which is torch's product of 64-bit copies of
+    rows and weight (eight times the weight's memory, and slower by orders).  Serving only: there is no gradient."""
     k, n = w.shape
     held = isinstance(x, Int8Rows)
     codes, w_codes = x.codes if held else x, w.codes
